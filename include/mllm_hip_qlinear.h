@@ -610,6 +610,48 @@ int mllm_hip_matmul_set_tile(int side);
 int mllm_hip_matmul_set_split(int side);
 int mllm_hip_matmul_split_side(int64_t batch, int64_t M, int64_t N, int64_t K, int transpose_a, int transpose_b);
 
+/* ---------------------------------------------------------------------------------------------------------
+ * Between a decoder layer's projections: norms and rotation of the query and key heads, a paged cache of keys and values,
+ * attention over it; and the token that follows from the logits.
+ *
+ * The cache: keys and values in bf16, pages of page_size slots, slot s of page p of head h at element
+ * p * page_stride + s * slot_stride + h * head_stride (the same for k and v; strides multiples of 8, pointers 16-byte aligned), head_dim
+ * elements in a row.  Offsets are 64-bit; pages * page_size < 2^31.
+ * ------------------------------------------------------------------------------------------------------- */
+typedef struct mllm_hip_kv_cache {
+  void* k;
+  void* v;
+  int64_t page_stride, slot_stride, head_stride; /* in elements */
+  int64_t pages;
+  int64_t page_size; /* any number of slots from 1 on */
+  int heads, head_dim;
+} mllm_hip_kv_cache;
+/* `heads` heads of every token: token t, head h at element t * x_token_stride + h * x_head_stride of x, the results in y likewise.  Rows
+ * and pointers 16-byte aligned.  y may be x with the same strides.  weight: fp32 [head_dim] of the RMSNorm, NULL: no norm. */
+typedef struct mllm_hip_rope_part {
+  const void* x;
+  void* y;
+  const float* weight;
+  int64_t x_token_stride, x_head_stride, y_token_stride, y_head_stride; /* in elements */
+  int heads;
+} mllm_hip_rope_part;
+
+/* Up to four tensors of heads (queries and keys) in one launch: y = rotate(norm(x)), norm as mllm_hip_rmsnorm over the head, then
+ * pairs (a, b) of the first rot_dim elements turned by positions[t] * inv_freq[j]: a cos - b sin, b cos + a sin.  Pair j is elements
+ * j and j + rot_dim / 2, or (interleaved) 2 j and 2 j + 1.  dtype of x and y: F32 or BF16, rounded once; the angles are fp64 up to the
+ * fraction of a turn.  positions int32 [T] (any value), inv_freq fp64 [rot_dim / 2]; rot_dim 0: no rotation, neither is read.
+ * head_dim % 8 == 0, <= 512; rot_dim % 16 == 0, <= head_dim.  T = 0 does nothing. */
+int mllm_hip_qk_norm_rope(int nparts, const mllm_hip_rope_part* parts, int dtype, int64_t T, int head_dim, float epsilon,
+                          int add_unit_offset, const int32_t* positions, const double* inv_freq, int rot_dim, int interleaved,
+                          void* stream);
+/* The keys of T tokens, normed and rotated as above, and their values, rounded to bf16, into the cache: token t at slot
+ * slots[t] % page_size of page slots[t] / page_size.  A slot below 0 or behind the cache stores nothing (padded tokens); two tokens
+ * with one slot leave either's elements there.  k->y and v's y and weight are not looked at.  q (may be NULL): the queries in the
+ * same launch, rotate(norm(q)) into q->y as above. */
+int mllm_hip_kv_append(const mllm_hip_rope_part* q, const mllm_hip_rope_part* k, const mllm_hip_rope_part* v, int dtype, int64_t T,
+                       const mllm_hip_kv_cache* cache, const int64_t* slots, float epsilon, int add_unit_offset,
+                       const int32_t* positions, const double* inv_freq, int rot_dim, int interleaved, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

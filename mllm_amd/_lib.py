@@ -22,6 +22,18 @@ class GemvFusion(C.Structure):
     _fields_ = [("residual", C.POINTER(C.c_void_p)), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
+class RopePart(C.Structure):
+    """mllm_hip_rope_part"""
+    _fields_ = [("x", C.c_void_p), ("y", C.c_void_p), ("weight", C.c_void_p), ("x_token_stride", C.c_int64), ("x_head_stride", C.c_int64),
+                ("y_token_stride", C.c_int64), ("y_head_stride", C.c_int64), ("heads", C.c_int)]
+
+
+class KVCache(C.Structure):
+    """mllm_hip_kv_cache"""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("page_stride", C.c_int64), ("slot_stride", C.c_int64), ("head_stride", C.c_int64),
+                ("pages", C.c_int64), ("page_size", C.c_int64), ("heads", C.c_int), ("head_dim", C.c_int)]
+
+
 class HipQLinearError(RuntimeError):
     pass
 
@@ -182,6 +194,9 @@ def lib():
         L.mllm_hip_matmul_split_side.argtypes = [i64, i64, i64, i64, ci, ci]
         L.mllm_hip_matmul_f32.argtypes = [vp, vp, vp, i64, i64, i64, ci, ci, vp]
         L.mllm_hip_matmul_batched.argtypes = [vp, vp, vp, ci, i64, i64, i64, i64, i64, i64, i64, ci, ci, vp]
+        cf, rp, kv = C.c_float, C.POINTER(RopePart), C.POINTER(KVCache)
+        L.mllm_hip_qk_norm_rope.argtypes = [ci, rp, ci, i64, ci, cf, ci, vp, vp, ci, ci, vp]
+        L.mllm_hip_kv_append.argtypes = [rp, rp, rp, ci, i64, kv, vp, cf, ci, vp, vp, ci, ci, vp]
         _lib = L
     return _lib
 

@@ -291,6 +291,125 @@ PyObject* linear_kq_gemm(Args a) {
                      shorter ? mllm_hip_linear_kq_gemm_short : mllm_hip_linear_kq_gemm);
 }
 
+// ---- heads of tokens, the paged cache, attention over it, sampling
+double real(PyObject* o) {
+  const double v = PyFloat_AsDouble(o);
+  if (v == -1.0 && PyErr_Occurred()) throw Raised();
+  return v;
+}
+int64_t current_device() { return integer(Owned(PyObject_CallNoArgs(g_device)).o); }
+// a tensor of this type on the current device (whose stream the call goes to)
+const at::Tensor& local(PyObject* o, int64_t device, at::ScalarType type) {
+  const at::Tensor& t = tensor(o);
+  require(t.is_cuda() && t.get_device() == device && t.scalar_type() == type);
+  return t;
+}
+// a contiguous vector of n elements, or null where none is given
+template <typename T>
+const T* vector_of(PyObject* o, int64_t device, at::ScalarType type, int64_t n) {
+  if (o == Py_None) return nullptr;
+  const at::Tensor& t = local(o, device, type);
+  require(t.dim() == 1 && t.size(0) == n && t.is_contiguous());
+  return static_cast<const T*>(t.data_ptr());
+}
+int64_t stride_of(const at::Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }  // (of a single row any number may stand there)
+// [T, heads, D] with rows in one piece
+mllm_hip_rope_part heads_of(const at::Tensor& x, int64_t T, int64_t D, at::ScalarType type, int64_t device) {
+  require(x.is_cuda() && x.get_device() == device && x.scalar_type() == type && x.dim() == 3 && x.size(0) == T && x.size(2) == D && (D == 1 || x.stride(2) == 1));
+  require(x.size(1) >= 1 && x.size(1) <= 65536);
+  return mllm_hip_rope_part{x.data_ptr(), nullptr, nullptr, stride_of(x, 0), stride_of(x, 1), 0, 0, (int)x.size(1)};
+}
+// where a part's results go: the given tensor or a new one
+void results_to(mllm_hip_rope_part& p, const at::Tensor& x, PyObject* out, at::Tensor& made, int64_t device) {
+  if (out == Py_None) made = at::empty(x.sizes(), x.options());
+  else made = tensor(out);
+  const mllm_hip_rope_part y = heads_of(made, x.size(0), x.size(2), x.scalar_type(), device);
+  require(y.heads == p.heads);
+  p.y = made.data_ptr();
+  p.y_token_stride = y.x_token_stride;
+  p.y_head_stride = y.x_head_stride;
+}
+struct Rotation {
+  const int32_t* positions;
+  const double* inv_freq;
+  int rot_dim;
+};
+Rotation rotation_of(PyObject* positions, PyObject* inv_freq, int64_t T, int64_t device) {
+  require((positions == Py_None) == (inv_freq == Py_None));
+  if (positions == Py_None) return Rotation{nullptr, nullptr, 0};
+  const at::Tensor& f = local(inv_freq, device, at::kDouble);
+  require(f.dim() == 1 && f.is_contiguous() && f.size(0) <= 65536);
+  return Rotation{vector_of<int32_t>(positions, device, at::kInt, T), static_cast<const double*>(f.data_ptr()), 2 * (int)f.size(0)};
+}
+// keys and values [pages, page_size, heads, D] of one layout
+mllm_hip_kv_cache cache_of(PyObject* ko, PyObject* vo, int64_t device) {
+  const at::Tensor &k = local(ko, device, at::kBFloat16), &v = local(vo, device, at::kBFloat16);
+  require(k.dim() == 4 && v.dim() == 4 && k.sizes() == v.sizes() && k.size(0) >= 1 && k.size(1) >= 1 && k.size(2) >= 1 && k.size(2) <= 65536 && k.size(3) >= 1 &&
+          k.size(3) <= 65536);
+  for (int d = 0; d < 3; d++) require(stride_of(k, d) == stride_of(v, d));
+  require(k.size(3) == 1 || (k.stride(3) == 1 && v.stride(3) == 1));
+  return mllm_hip_kv_cache{k.data_ptr(), v.data_ptr(), stride_of(k, 0), stride_of(k, 1), stride_of(k, 2), k.size(0), k.size(1), (int)k.size(2), (int)k.size(3)};
+}
+
+// (q, k, positions, inv_freq, q_weight, k_weight, eps, add_unit_offset, interleaved, out)
+PyObject* qk_norm_rope(Args a) {
+  const int64_t device = current_device();
+  const at::Tensor &q = tensor(a[0]), &k = tensor(a[1]);
+  const int dtype = xdtype(q);
+  require(q.dim() == 3);
+  const int64_t T = q.size(0), D = q.size(2);
+  mllm_hip_rope_part parts[2] = {heads_of(q, T, D, q.scalar_type(), device), heads_of(k, T, D, q.scalar_type(), device)};
+  PyObject *oq = Py_None, *ok = Py_None;
+  if (a[9] != Py_None) {
+    require(PyTuple_Check(a[9]) && PyTuple_GET_SIZE(a[9]) == 2);
+    oq = PyTuple_GET_ITEM(a[9], 0), ok = PyTuple_GET_ITEM(a[9], 1);
+  }
+  at::Tensor yq, yk;
+  results_to(parts[0], q, oq, yq, device);
+  results_to(parts[1], k, ok, yk, device);
+  parts[0].weight = vector_of<float>(a[4], device, at::kFloat, D);
+  parts[1].weight = vector_of<float>(a[5], device, at::kFloat, D);
+  const Rotation r = rotation_of(a[2], a[3], T, device);
+  const float eps = (float)real(a[6]);
+  const int unit = truth(a[7]), next = truth(a[8]);
+  require(D <= 65536);
+  void* st = stream();
+  run("mllm_hip_qk_norm_rope", [&] { return mllm_hip_qk_norm_rope(2, parts, dtype, T, (int)D, eps, unit, r.positions, r.inv_freq, r.rot_dim, next, st); });
+  Owned qo(THPVariable_Wrap(yq)), ko(THPVariable_Wrap(yk));
+  return PyTuple_Pack(2, qo.o, ko.o);
+}
+
+// (k, v, k_cache, v_cache, slots, positions, inv_freq, k_weight, q, q_weight, eps, add_unit_offset, interleaved, out)
+PyObject* kv_append(Args a) {
+  const int64_t device = current_device();
+  const at::Tensor &k = tensor(a[0]), &v = tensor(a[1]);
+  const int dtype = xdtype(k);
+  require(k.dim() == 3);
+  const mllm_hip_kv_cache cache = cache_of(a[2], a[3], device);
+  const int64_t T = k.size(0), D = cache.head_dim;
+  mllm_hip_rope_part kp = heads_of(k, T, D, k.scalar_type(), device), vp = heads_of(v, T, D, k.scalar_type(), device), qp = {};
+  require(kp.heads == cache.heads && vp.heads == cache.heads);
+  kp.weight = vector_of<float>(a[7], device, at::kFloat, D);
+  at::Tensor y;
+  if (a[8] != Py_None) {
+    const at::Tensor& q = tensor(a[8]);
+    qp = heads_of(q, T, D, k.scalar_type(), device);
+    results_to(qp, q, a[13], y, device);
+    qp.weight = vector_of<float>(a[9], device, at::kFloat, D);
+  }
+  require(a[4] != Py_None);
+  const int64_t* slots = vector_of<int64_t>(a[4], device, at::kLong, T);
+  const Rotation r = rotation_of(a[5], a[6], T, device);
+  const float eps = (float)real(a[10]);
+  const int unit = truth(a[11]), next = truth(a[12]);
+  void* st = stream();
+  run("mllm_hip_kv_append", [&] {
+    return mllm_hip_kv_append(a[8] != Py_None ? &qp : nullptr, &kp, &vp, dtype, T, &cache, slots, eps, unit, r.positions, r.inv_freq, r.rot_dim, next, st);
+  });
+  if (a[8] == Py_None) Py_RETURN_NONE;
+  return THPVariable_Wrap(y);
+}
+
 template <PyObject* (*F)(Args), int N>
 PyObject* entry(PyObject*, Args args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -307,7 +426,8 @@ PyObject* entry(PyObject*, Args args, Py_ssize_t n) {
 }
 #define CALL(name, n) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(entry<name, n>)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {CALL(linear_q_gemv, 8), CALL(linear_q_gemv_multi, 6), CALL(softmax, 1), CALL(topk, 4), CALL(matmul, 5),
-                           CALL(w8a8_linear_packed, 7), CALL(w4a16_gemm_packed, 6), CALL(linear_q_gemm, 7), CALL(linear_kq_gemm, 6), {nullptr, nullptr, 0, nullptr}};
+                           CALL(w8a8_linear_packed, 7), CALL(w4a16_gemm_packed, 6), CALL(linear_q_gemm, 7), CALL(linear_kq_gemm, 6),
+                           CALL(qk_norm_rope, 10), CALL(kv_append, 14), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "mllm_calls", nullptr, -1, g_methods};
 
 }  // namespace

@@ -663,3 +663,19 @@ def matmul(a, b, transpose_a=False, transpose_b=False, out=None):
     single matrix shared by every batch entry.  Last bits of fp32 results depend on the call's sizes (which instructions it
     takes), never on other rows or columns.  mllm/backends/cpu/ops/MatMulOp.cpp:19-90."""
     return _calls().matmul(a, b, transpose_a, transpose_b, out)
+
+
+# ----------------------------------------------------------------------------- between a layer's projections: heads, the paged cache
+def qk_norm_rope(q, k, positions=None, inv_freq=None, q_weight=None, k_weight=None, eps=1e-6, add_unit_offset=False, interleaved=False, out=None):
+    """RMSNorm of every head (q_weight / k_weight fp32 [D], None: no norm) and rotation by positions int32 [T] times inv_freq fp64
+    [rot_dim / 2] (None: no rotation) of q [T, Hq, D] and k [T, Hkv, D], fp32 or bf16, any strides of whole 16 bytes with heads in one piece.
+    Pairs: elements j and j + rot_dim / 2, interleaved: 2j and 2j + 1.  Returns (q, k) anew, or in out=(q, k), which may be the inputs."""
+    return _calls().qk_norm_rope(q, k, positions, inv_freq, q_weight, k_weight, eps, add_unit_offset, interleaved, out)
+
+
+def kv_append(k, v, k_cache, v_cache, slots, positions=None, inv_freq=None, k_weight=None, q=None, q_weight=None, eps=1e-6, add_unit_offset=False,
+              interleaved=False, out=None):
+    """k [T, Hkv, D], normed and rotated as by qk_norm_rope, and v into a paged cache: k_cache, v_cache bf16 [pages, page_size, Hkv, D] of
+    one layout (any strides of whole 16 bytes); token t goes to slots[t] (int64: page * page_size + place in the page; outside the cache:
+    stored nowhere; two tokens with one slot leave either's elements).  q [T, Hq, D]: the queries in the same launch, returned anew or in `out`."""
+    return _calls().kv_append(k, v, k_cache, v_cache, slots, positions, inv_freq, k_weight, q, q_weight, eps, add_unit_offset, interleaved, out)

@@ -1,0 +1,54 @@
+"""Refusals of the operators between a layer's projections at the C ABI, without a GPU: made-up addresses that a refused call never reads."""
+import ctypes as C
+
+import pytest
+
+from mllm_amd import _lib
+
+P = 0x7F0000100000
+ODD = P + 2
+BADARG, SHAPE, ALIGN = -1, -2, -3
+F32, BF16 = 0, 1
+
+
+def _part(**changed):
+    p = dict(x=P, y=P, weight=P, x_token_stride=512, x_head_stride=128, y_token_stride=512, y_head_stride=128, heads=4)
+    p.update(changed)
+    return _lib.RopePart(**p)
+
+
+def _cache(**changed):
+    c = dict(k=P, v=P, page_stride=16 * 512, slot_stride=512, head_stride=128, pages=8, page_size=16, heads=4, head_dim=128)
+    c.update(changed)
+    return _lib.KVCache(**c)
+
+
+def _rope(part=None, nparts=1, dtype=F32, T=1, D=128, pos=P, freq=P, rot=128):
+    return _lib.lib().mllm_hip_qk_norm_rope(nparts, C.byref(part if part is not None else _part()), dtype, T, D, 1e-6, 0, pos, freq, rot, 0, None)
+
+
+@pytest.mark.parametrize("args,want", [
+    (dict(nparts=0), BADARG), (dict(nparts=5), BADARG), (dict(dtype=2), BADARG), (dict(T=-1), BADARG), (dict(T=1 << 31), SHAPE), (dict(D=0), BADARG), (dict(D=12), SHAPE),
+    (dict(D=520), SHAPE), (dict(rot=-16), BADARG), (dict(rot=8), SHAPE), (dict(rot=144), SHAPE), (dict(pos=None), BADARG), (dict(freq=None), BADARG), (dict(freq=P + 4), ALIGN),
+    (dict(pos=P + 1), ALIGN), (dict(part=_part(x=None)), BADARG), (dict(part=_part(y=None)), BADARG), (dict(part=_part(heads=0)), BADARG), (dict(part=_part(heads=65537)), SHAPE),
+    (dict(part=_part(x=ODD)), ALIGN), (dict(part=_part(y=ODD)), ALIGN), (dict(part=_part(weight=ODD)), ALIGN), (dict(part=_part(x_token_stride=130)), ALIGN),
+    (dict(part=_part(y_head_stride=2)), ALIGN), (dict(part=_part(x_head_stride=132), dtype=BF16), ALIGN), (dict(T=0), 0), (dict(T=0, pos=None, freq=None, rot=0), 0)])
+def test_qk_norm_rope(args, want):
+    assert _rope(**args) == want
+
+
+def _append(k=None, v=None, q=None, cache=None, slots=P, T=1, dtype=BF16, rot=128, no_cache=False):
+    ref = lambda s: C.byref(s) if s is not None else None  # noqa: E731
+    k = _part() if k is None else k
+    v = _part() if v is None else v
+    return _lib.lib().mllm_hip_kv_append(ref(q), ref(k), ref(v), dtype, T, None if no_cache else ref(cache or _cache()), slots, 1e-6, 0, P, P, rot, 0, None)
+
+
+@pytest.mark.parametrize("args,want", [
+    (dict(no_cache=True), BADARG), (dict(slots=None), BADARG), (dict(slots=P + 4), ALIGN), (dict(cache=_cache(k=None)), BADARG), (dict(cache=_cache(v=None)), BADARG),
+    (dict(cache=_cache(k=ODD)), ALIGN), (dict(cache=_cache(page_stride=100)), ALIGN), (dict(cache=_cache(slot_stride=4)), ALIGN), (dict(cache=_cache(head_stride=132)), ALIGN),
+    (dict(cache=_cache(pages=0)), BADARG), (dict(cache=_cache(page_size=0)), BADARG), (dict(cache=_cache(pages=1 << 27, page_size=16)), SHAPE), (dict(cache=_cache(heads=2)), SHAPE),
+    (dict(cache=_cache(head_dim=100)), SHAPE), (dict(k=_part(heads=2)), SHAPE), (dict(v=_part(heads=5)), SHAPE), (dict(k=_part(x=None)), BADARG), (dict(v=_part(x=ODD)), ALIGN),
+    (dict(q=_part(y=None)), BADARG), (dict(q=_part(y=ODD)), ALIGN), (dict(k=_part(y=None), v=_part(y=None, weight=None), T=0), 0), (dict(rot=24), SHAPE), (dict(dtype=5), BADARG)])
+def test_kv_append(args, want):
+    assert _append(**args) == want
