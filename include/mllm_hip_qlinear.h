@@ -628,29 +628,49 @@ typedef struct mllm_hip_kv_cache {
 } mllm_hip_kv_cache;
 /* `heads` heads of every token: token t, head h at element t * x_token_stride + h * x_head_stride of x, the results in y likewise.  Rows
  * and pointers 16-byte aligned.  y may be x with the same strides.  weight: fp32 [head_dim] of the RMSNorm, NULL: no norm. */
-typedef struct mllm_hip_rope_part {
+typedef struct mllm_hip_heads {
   const void* x;
   void* y;
   const float* weight;
   int64_t x_token_stride, x_head_stride, y_token_stride, y_head_stride; /* in elements */
   int heads;
-} mllm_hip_rope_part;
+} mllm_hip_heads;
 
 /* Up to four tensors of heads (queries and keys) in one launch: y = rotate(norm(x)), norm as mllm_hip_rmsnorm over the head, then
  * pairs (a, b) of the first rot_dim elements turned by positions[t] * inv_freq[j]: a cos - b sin, b cos + a sin.  Pair j is elements
  * j and j + rot_dim / 2, or (interleaved) 2 j and 2 j + 1.  dtype of x and y: F32 or BF16, rounded once; the angles are fp64 up to the
  * fraction of a turn.  positions int32 [T] (any value), inv_freq fp64 [rot_dim / 2]; rot_dim 0: no rotation, neither is read.
  * head_dim % 8 == 0, <= 512; rot_dim % 16 == 0, <= head_dim.  T = 0 does nothing. */
-int mllm_hip_qk_norm_rope(int nparts, const mllm_hip_rope_part* parts, int dtype, int64_t T, int head_dim, float epsilon,
+int mllm_hip_qk_norm_rope(int nparts, const mllm_hip_heads* parts, int dtype, int64_t T, int head_dim, float epsilon,
                           int add_unit_offset, const int32_t* positions, const double* inv_freq, int rot_dim, int interleaved,
                           void* stream);
 /* The keys of T tokens, normed and rotated as above, and their values, rounded to bf16, into the cache: token t at slot
  * slots[t] % page_size of page slots[t] / page_size.  A slot below 0 or behind the cache stores nothing (padded tokens); two tokens
  * with one slot leave either's elements there.  k->y and v's y and weight are not looked at.  q (may be NULL): the queries in the
  * same launch, rotate(norm(q)) into q->y as above. */
-int mllm_hip_kv_append(const mllm_hip_rope_part* q, const mllm_hip_rope_part* k, const mllm_hip_rope_part* v, int dtype, int64_t T,
+int mllm_hip_kv_append(const mllm_hip_heads* q, const mllm_hip_heads* k, const mllm_hip_heads* v, int dtype, int64_t T,
                        const mllm_hip_kv_cache* cache, const int64_t* slots, float epsilon, int add_unit_offset,
                        const int32_t* positions, const double* inv_freq, int rot_dim, int interleaved, void* stream);
+
+/* Attention of new tokens over a paged cache that holds them already: token t of sequence b (rows cu_tokens[b] + t of q, cu_tokens
+ * int32 [B + 1]) sees the first prefix[b] positions of its sequence and, of the sequence's new tokens (positions prefix[b] + j), the ones
+ * whose bit is set in its row of the tree: bit j % 64 of word j / 64, tree_words words a row, rows of q tree_stride words apart;
+ * bits that are not there count as 0.  tree NULL: j <= t.  One token a sequence is a decode step, a tree the verification
+ * of drafted tokens, many tokens without a tree a (chunk of a) prompt.
+ *   o[t][h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * (q . k_j) - max), of key head h / (heads / kv heads); a token that sees
+ *   nothing: zeros.  What a token does not see has no effect on it, NaN included.
+ * Position i of sequence b is slot i % page_size of page block_table[b * table_stride + i / page_size] (int32); positions from table_len *
+ * page_size on are not there, pages outside the cache read as zeros.  q->x, q->y: F32 or BF16, 16-byte aligned rows (weight is not
+ * looked at); rows of q in no sequence stay as they are in y.  y may not be x.  head_dim 64, 128 or 256, heads a multiple of the cache's, scale > 0.
+ * max_tokens and max_keys: the host's bounds of a sequence's new tokens (more are left out) and positions (any; it decides into how many
+ * ranges keys are cut).  fp32 results are within fp32 sums of the formula, bf16 ones take the weights p in bf16.
+ * workspace: ..._workspace_bytes (0: none), 16-byte aligned; less is MLLM_HIP_E_BADARG.  One launch, two where keys are cut. */
+size_t mllm_hip_attention_paged_workspace_bytes(int dtype, int64_t T, int64_t B, int heads, int kv_heads, int head_dim, int64_t max_tokens,
+                                                int64_t max_keys);
+int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_t T, const mllm_hip_kv_cache* cache, const int32_t* block_table,
+                             int64_t table_stride, int64_t table_len, const int32_t* cu_tokens, const int32_t* prefix, int64_t B,
+                             int64_t max_tokens, int64_t max_keys, const uint64_t* tree, int64_t tree_stride, int64_t tree_words, float scale,
+                             void* workspace, size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -22,8 +22,8 @@ class GemvFusion(C.Structure):
     _fields_ = [("residual", C.POINTER(C.c_void_p)), ("workspace", C.c_void_p), ("workspace_bytes", C.c_size_t)]
 
 
-class RopePart(C.Structure):
-    """mllm_hip_rope_part"""
+class Heads(C.Structure):
+    """mllm_hip_heads"""
     _fields_ = [("x", C.c_void_p), ("y", C.c_void_p), ("weight", C.c_void_p), ("x_token_stride", C.c_int64), ("x_head_stride", C.c_int64),
                 ("y_token_stride", C.c_int64), ("y_head_stride", C.c_int64), ("heads", C.c_int)]
 
@@ -194,9 +194,12 @@ def lib():
         L.mllm_hip_matmul_split_side.argtypes = [i64, i64, i64, i64, ci, ci]
         L.mllm_hip_matmul_f32.argtypes = [vp, vp, vp, i64, i64, i64, ci, ci, vp]
         L.mllm_hip_matmul_batched.argtypes = [vp, vp, vp, ci, i64, i64, i64, i64, i64, i64, i64, ci, ci, vp]
-        cf, rp, kv = C.c_float, C.POINTER(RopePart), C.POINTER(KVCache)
+        cf, rp, kv = C.c_float, C.POINTER(Heads), C.POINTER(KVCache)
         L.mllm_hip_qk_norm_rope.argtypes = [ci, rp, ci, i64, ci, cf, ci, vp, vp, ci, ci, vp]
         L.mllm_hip_kv_append.argtypes = [rp, rp, rp, ci, i64, kv, vp, cf, ci, vp, vp, ci, ci, vp]
+        L.mllm_hip_attention_paged_workspace_bytes.restype = C.c_size_t
+        L.mllm_hip_attention_paged_workspace_bytes.argtypes = [ci, i64, i64, ci, ci, ci, i64, i64]
+        L.mllm_hip_attention_paged.argtypes = [rp, ci, i64, kv, vp, i64, i64, vp, vp, i64, i64, i64, vp, i64, i64, cf, vp, C.c_size_t, vp]
         _lib = L
     return _lib
 

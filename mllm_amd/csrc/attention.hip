@@ -1,0 +1,587 @@
+// Attention of one token, a tree of drafted tokens or a chunk of a prompt over a paged cache, for gfx950.
+//
+//   o[t][h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale * (q[t][h] . k_j) - m),  m = max_j,  over the keys j that token t sees:
+//   the prefix of its sequence and those of the sequence's new tokens whose bit is set in its row of the tree (without a tree: itself
+//   and the ones before it).
+//
+// The rows of one matrix product are (token, query head of the group) pairs that share a key head: with one token and four query heads a
+// key head, four rows.  Everything is turned so that nothing of P leaves its lane:
+//   S^T = K Q^T   v_mfma_f32_16x16x32_bf16, first operand 16 keys (a lane: 8 consecutive elements of one key), second 16 rows of Q.  Result: a
+//                 lane has one row of Q (lane % 16) and four keys.  Two such products, first operand rows r = keys 8 (r / 4) + r % 4 and the same + 4,
+//                 leave a lane with the eight consecutive keys 8 (lane / 16) .. + 7 of its row,
+//   O^T = V^T P^T which is what the second operand of the product over 32 keys takes.  V^T comes from LDS through the transposing reads.
+// A row's maximum, sum and the correction of O when the maximum grows are therefore numbers of a lane; sums over keys cross lanes twice per 32 keys
+// (the maximum) and once at the end (the sum).  Scores, maxima, sums and O are fp32.
+//
+// Roundings: bf16 queries as they are; P to bf16 for the product with V (off by 2^-9 of each weight, whose signs average; the sum takes P as it
+// was).  fp32 queries enter as three bf16 parts that add up to them (8 bits each, three products), P as two (2^-17 of each weight).
+//
+// A workgroup has four waves, WR along rows times 4 / WR along keys, and goes through a range of keys in tiles: 16-byte loads into registers while
+// the tile before them is worked on, from there into LDS.  Rows of a tile lie there with their 16-byte pieces exclusive-ored by bits of the
+// key's number, so that the 16 lanes of an operand read different banks.  Where rows and heads leave CUs idle the keys are cut into ranges
+// (splits), whose O, maximum and sum meet in the workspace; a second launch joins them.
+#include "item8.h"
+
+namespace mllmhip {
+
+typedef short at_s16x4 __attribute__((ext_vector_type(4)));
+typedef short at_s16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 at_bf16x8 __attribute__((ext_vector_type(8)));
+typedef float at_f32x4 __attribute__((ext_vector_type(4)));
+
+struct AttnArgs {
+  const void* q;
+  void* o;
+  int64_t q_token, q_head, o_token, o_head;
+  const uint16_t *k, *v;
+  int64_t page_stride, slot_stride, head_stride;
+  uint32_t pages, page, page_mul;  // key / page = (key * page_mul) >> page_shift for key < 2^31
+  int page_shift;
+  const int32_t* table;
+  int64_t table_stride;
+  int table_len;
+  const int32_t *cu, *prefix;
+  const uint64_t* tree;
+  int64_t tree_stride;
+  int words;
+  int T, B, kv, group, max_rows, row_tiles, splits, chunk;
+  float c;  // scale * log2 e
+  float *part_o, *part_ml;  // [split][token][query head][head_dim], [split][token][query head][2]
+};
+__device__ const u32x4 g_zero_row[1] = {};  // what a page outside the cache reads as
+
+// sequence b: its first row of q, its number of new tokens, of prefix keys and of keys
+struct Seq {
+  int first, n, prefix, keys;
+};
+__device__ __forceinline__ Seq sequence(const AttnArgs& a, int b) {
+  Seq s;
+  const int lo = a.cu[b], hi = min(a.cu[b + 1], a.T);
+  s.first = max(lo, 0);
+  s.n = max(hi - s.first, 0);
+  s.prefix = max(a.prefix[b], 0);
+  s.keys = (int)min((int64_t)s.prefix + s.n, (int64_t)a.table_len * a.page);
+  return s;
+}
+
+// 8 bf16 of a register quad as an operand
+__device__ __forceinline__ at_bf16x8 frag(u32x4 v) { return __builtin_bit_cast(at_bf16x8, v); }
+__device__ __forceinline__ at_f32x4 mma(at_bf16x8 x, at_bf16x8 y, at_f32x4 acc) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, acc, 0, 0, 0); }
+
+template <int D, int NQ, int WR, bool F32>
+struct Attn {
+  static constexpr int WK = 4 / WR;                      // waves along keys
+  static constexpr int KT = WK * 32 < 64 ? 64 : WK * 32;  // keys of a tile
+  static constexpr int SUB = KT / (WK * 32);             // 32-key steps of a wave per tile
+  static constexpr int C = D / 8;                        // 16-byte pieces of a row
+  static constexpr int RPI = 64 / C;                     // rows a wave loads per instruction
+  static constexpr int NLOAD = KT / 4 / RPI;             // loads of keys (and of values) of a lane per tile
+  static constexpr int PARTS = F32 ? 3 : 1, PPARTS = F32 ? 2 : 1;
+  static constexpr int ROWS = NQ * 16;                   // rows of a wave
+  static __device__ __forceinline__ int swz(int row) { return (C == 8) ? (row & 3) | ((row >> 3) & 1) << 2 : (row & 3) | ((row >> 3) & 3) << 2; }
+};
+
+// which of the keys k0 .. k0 + 7 token `token` of the sequence sees
+__device__ __forceinline__ uint32_t seen_keys(const AttnArgs& a, const Seq& s, int k0, int token) {
+  uint32_t see = 0;
+  const int j0 = k0 - s.prefix;  // the new token that key k0 is
+  if (j0 <= -8) {
+    see = 0xff;
+  } else if (a.tree) {  // eight bits of the token's row from bit j0 on, ones in front of bit 0
+    const int lo = max(j0, 0), w = lo >> 6, in = lo & 63;
+    const uint64_t* row = a.tree + (int64_t)(s.first + token) * a.tree_stride;
+    uint64_t bits = w < a.words ? row[w] >> in : 0;
+    if (in > 56 && w + 1 < a.words) bits |= row[w + 1] << (64 - in);
+    see = (uint32_t)bits << (lo - j0) | ((1u << (lo - j0)) - 1);
+  } else {
+    see = (2u << min(max(token - j0, 0), 7)) - 1;  // bits 0 .. token - j0
+    if (token < j0) see = 0;
+  }
+  const int left = s.keys - k0;
+  return left >= 8 ? see & 0xff : left <= 0 ? 0 : see & ((1u << left) - 1);
+}
+// whether one of two bf16 is infinite or no number
+__device__ __forceinline__ bool odd_pair(uint32_t v) { return (v & 0x7f80u) == 0x7f80u || (v & 0x7f800000u) == 0x7f800000u; }
+__device__ __forceinline__ uint32_t finite_pair(uint32_t v) {
+  return ((v & 0x7f80u) == 0x7f80u ? 0u : v & 0xffffu) | ((v & 0x7f800000u) == 0x7f800000u ? 0u : v & 0xffff0000u);
+}
+
+// The infinities and NaNs of a step's values, key by key, into the rows that see them (rare)
+template <int D, int NQ>
+__device__ __forceinline__ void odd_values(const uint16_t* s_v, int base, const uint32_t (&see)[NQ], const at_bf16x8 (&fp)[NQ], at_f32x4 (&acc)[NQ][D / 16]) {
+  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
+  constexpr int C = D / 8;
+#pragma unroll 1
+  for (int key = 0; key < 32; key++) {
+    const int row = base + key, x = (C == 8) ? (row & 3) | ((row >> 3) & 1) << 2 : (row & 3) | ((row >> 3) & 3) << 2;
+#pragma unroll
+    for (int i = 0; i < NQ; i++) {
+      const u32x4 mine = __builtin_bit_cast(u32x4, fp[i]);
+      const uint32_t pair = key % 8 / 2 == 0 ? mine.x : key % 8 / 2 == 1 ? mine.y : key % 8 / 2 == 2 ? mine.z : mine.w;
+      const float weight = __uint_as_float(key & 1 ? pair & 0xffff0000u : pair << 16);
+      const float p = __shfl(weight, key / 8 * 16 + col);
+      const bool seen = __shfl((int)see[i], key / 8 * 16 + col) >> (key % 8) & 1;
+#pragma unroll
+      for (int d = 0; d < D / 16; d++) {
+        const u32x2 v = *reinterpret_cast<const u32x2*>(s_v + row * D + ((2 * d + (g >> 1)) ^ x) * 8 + (g & 1) * 4);
+        const uint32_t w[4] = {v.x << 16, v.x & 0xffff0000u, v.y << 16, v.y & 0xffff0000u};
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (seen && (w[e] & 0x7f800000u) == 0x7f800000u) acc[i][d][e] += p * __uint_as_float(w[e]);
+      }
+    }
+  }
+}
+
+template <int D, int NQ, int WR, bool F32>
+__global__ __launch_bounds__(256) void attention_kernel(AttnArgs a) {
+  typedef Attn<D, NQ, WR, F32> P;
+  constexpr int KT = P::KT, C = P::C, WK = P::WK, NLOAD = P::NLOAD, KS = D / 32, DT = D / 16;
+  __shared__ __align__(16) uint16_t s_k[KT * D];
+  __shared__ __align__(16) uint16_t s_v[KT * D];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wr = wave % WR, wk = wave / WR;
+  const int col = lane & 15, g = lane >> 4;
+
+  // workgroup b runs on XCD b % 8: the row tiles of a range of keys follow one another on one XCD, whose L2 they share
+  const int idx = blockIdx.x >> 3, rt = idx % a.row_tiles, place = (idx / a.row_tiles) * 8 + (blockIdx.x & 7);
+  const int h = place % a.kv, split = place / a.kv % a.splits, b = place / a.kv / a.splits;
+  if (b >= a.B) return;
+  // A lane's pieces of a tile: piece lane % C, as it lies in LDS, of rows load_row(i)
+  const int piece = lane % C;
+  auto load_row = [&](int i) { return wave * (KT / 4) + i * P::RPI + lane / C; };
+  const int64_t head_at = h * a.head_stride;
+  int ids[NLOAD];
+  auto ask_pages = [&](int k0) {  // the pages of a tile's keys (the last page of the table for what lies behind it: never used)
+#pragma unroll
+    for (int i = 0; i < NLOAD; i++) {
+      const uint32_t key = (uint32_t)(k0 + load_row(i));
+      const uint32_t at = (uint32_t)(((uint64_t)key * a.page_mul) >> a.page_shift);
+      ids[i] = a.table[b * a.table_stride + min((int)at, a.table_len - 1)];
+    }
+  };
+  const int k_begin = split * a.chunk;
+  ask_pages(k_begin);  // (in front of the loads that say how many keys there are)
+  const Seq s = sequence(a, b);
+  const int rows = s.n * a.group, row0 = rt * P::ROWS * WR;
+  const int k_end = split + 1 == a.splits ? s.keys : min(k_begin + a.chunk, s.keys);
+  if (row0 >= rows || (split > 0 && k_begin >= k_end)) return;
+
+  // Q: second operand, row `col` of every 16, elements 32 s + 8 g .. + 7
+  at_bf16x8 fq[P::PARTS][NQ][KS];
+  int token[NQ];
+  int64_t o_at[NQ];
+#pragma unroll
+  for (int i = 0; i < NQ; i++) {
+    const int r = row0 + wr * P::ROWS + i * 16 + col;
+    const bool live = r < rows;
+    token[i] = live ? r / a.group : 0;
+    const int head = h * a.group + (live ? r - token[i] * a.group : 0);
+    o_at[i] = live ? (int64_t)(s.first + token[i]) * (a.kv * a.group) + head : -1;
+    const int64_t at = (s.first + token[i]) * a.q_token + head * a.q_head + 8 * g;
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) {
+      Item8<F32 ? MLLM_HIP_F32 : MLLM_HIP_BF16> it;
+      item_load<F32 ? MLLM_HIP_F32 : MLLM_HIP_BF16>(a.q, at + 32 * ks, it);
+      if (!F32) {
+        fq[0][i][ks] = frag(it.r[0]);
+      } else {  // x = hi + mid + lo, each cut off after 8 bits; what is no number or infinite is all in hi
+        float v[8];
+        item_to_f32<F32 ? MLLM_HIP_F32 : MLLM_HIP_BF16>(it, v);
+        uint32_t part[3][4];
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          uint32_t bits[3][2];
+#pragma unroll
+          for (int e = 0; e < 2; e++) {
+            const float x = v[2 * j + e];
+            const uint32_t hi = __float_as_uint(x) & 0xffff0000u;
+            const bool finite = (hi & 0x7f800000u) != 0x7f800000u;
+            const float r1 = finite ? x - __uint_as_float(hi) : 0.f;
+            const uint32_t mid = __float_as_uint(r1) & 0xffff0000u;
+            const float r2 = r1 - __uint_as_float(mid);
+            bits[0][e] = !finite && x != x ? 0x7fc00000u : hi;
+            bits[1][e] = mid;
+            bits[2][e] = __float_as_uint(r2) & 0xffff0000u;
+          }
+#pragma unroll
+          for (int p = 0; p < 3; p++) part[p][j] = bits[p][0] >> 16 | bits[p][1];
+        }
+#pragma unroll
+        for (int p = 0; p < P::PARTS; p++) fq[p][i][ks] = frag(u32x4{part[p][0], part[p][1], part[p][2], part[p][3]});
+      }
+    }
+  }
+
+  u32x4 rk[NLOAD], rv[NLOAD];
+  auto ask_tile = [&](int k0) {
+#pragma unroll
+    for (int i = 0; i < NLOAD; i++) {
+      const int row = load_row(i);
+      const uint32_t key = (uint32_t)(k0 + row);
+      const uint32_t in = key - (uint32_t)(((uint64_t)key * a.page_mul) >> a.page_shift) * a.page;
+      const bool good = (int)key < k_end && (uint32_t)ids[i] < a.pages;
+      const int64_t at = (int64_t)ids[i] * a.page_stride + in * a.slot_stride + head_at + (piece ^ P::swz(row)) * 8;
+      rk[i] = *(good ? reinterpret_cast<const u32x4*>(a.k + at) : g_zero_row);
+      rv[i] = *(good ? reinterpret_cast<const u32x4*>(a.v + at) : g_zero_row);
+    }
+  };
+
+  at_f32x4 acc[NQ][DT];
+  float m[NQ], l[NQ];  // the maximum so far times c; the sum of this lane's keys
+#pragma unroll
+  for (int i = 0; i < NQ; i++) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; d++) acc[i][d] = at_f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+
+  if (k_begin < k_end) {
+    ask_tile(k_begin);
+    ask_pages(k_begin + KT);
+  }
+  for (int k0 = k_begin; k0 < k_end; k0 += KT) {
+    __syncthreads();  // the tile before this one has been read
+#pragma unroll
+    for (int i = 0; i < NLOAD; i++) {
+      const int at = load_row(i) * D + piece * 8;
+      *reinterpret_cast<u32x4*>(s_k + at) = rk[i];
+      *reinterpret_cast<u32x4*>(s_v + at) = rv[i];
+    }
+    __syncthreads();
+    if (k0 + KT < k_end) {
+      ask_tile(k0 + KT);
+      ask_pages(k0 + 2 * KT);
+    }
+#pragma unroll
+    for (int u = 0; u < P::SUB; u++) {
+      const int base = (u * WK + wk) * 32;  // the step's first row in the tile
+      const int key0 = k0 + base;
+      if (key0 >= k_end) break;
+      at_f32x4 sa[NQ], sb[NQ];
+#pragma unroll
+      for (int i = 0; i < NQ; i++) sa[i] = sb[i] = at_f32x4{0.f, 0.f, 0.f, 0.f};
+      const int ra = base + 8 * (col >> 2) + (col & 3), x = P::swz(ra);
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) {
+        const int at = ra * D + ((4 * ks + g) ^ x) * 8;
+        const at_bf16x8 ka = frag(*reinterpret_cast<const u32x4*>(s_k + at)), kb = frag(*reinterpret_cast<const u32x4*>(s_k + at + 4 * D));
+#pragma unroll
+        for (int i = 0; i < NQ; i++) {
+#pragma unroll
+          for (int p = P::PARTS - 1; p >= 0; p--) {  // the smallest part first
+            sa[i] = mma(ka, fq[p][i][ks], sa[i]);
+            sb[i] = mma(kb, fq[p][i][ks], sb[i]);
+          }
+        }
+      }
+      const bool border = key0 + 32 > s.prefix;  // new tokens, or keys behind the last
+      at_bf16x8 fp[P::PPARTS][NQ];
+      uint32_t see[NQ];
+#pragma unroll
+      for (int i = 0; i < NQ; i++) {
+        float y[8] = {sa[i][0], sa[i][1], sa[i][2], sa[i][3], sb[i][0], sb[i][1], sb[i][2], sb[i][3]};
+        if (border) {
+          see[i] = seen_keys(a, s, key0 + 8 * g, token[i]);
+#pragma unroll
+          for (int j = 0; j < 8; j++) y[j] = see[i] >> j & 1 ? y[j] : -INFINITY;
+        }
+        float top = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
+        top = max32(max16(top)) * a.c;
+        if (__ballot(top > m[i])) {
+          const float next = fmaxf(m[i], top), fix = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - next);
+          m[i] = next;
+          l[i] *= fix;
+#pragma unroll
+          for (int d = 0; d < DT; d++) acc[i][d] *= fix;
+        }
+        const float ref = m[i] == -INFINITY ? 0.f : m[i];  // (nothing seen yet: every p is exp2(-inf))
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+          y[j] = __builtin_amdgcn_exp2f(fmaf(y[j], a.c, -ref));
+          l[i] += y[j];
+        }
+        if (!F32) {
+          fp[0][i] = frag(u32x4{pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7])});
+        } else {
+          float lo[8];
+          uint32_t hi[4];
+#pragma unroll
+          for (int j = 0; j < 8; j++) lo[j] = y[j] - __uint_as_float(__float_as_uint(y[j]) & 0xffff0000u);
+#pragma unroll
+          for (int j = 0; j < 4; j++) hi[j] = __float_as_uint(y[2 * j]) >> 16 | (__float_as_uint(y[2 * j + 1]) & 0xffff0000u);
+          fp[0][i] = frag(u32x4{hi[0], hi[1], hi[2], hi[3]});
+          fp[P::PPARTS - 1][i] = frag(u32x4{pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]), pack_bf16(lo[4], lo[5]), pack_bf16(lo[6], lo[7])});
+        }
+      }
+      // V^T: lane i of 16 asks for elements 4 (i % 4) .. + 3 of key 8 g + i / 4 and gets element i of keys 8 g .. + 3
+      const int rv0 = base + 8 * g + (col >> 2), xv = P::swz(rv0);
+      bool odd = false;
+#pragma unroll
+      for (int d = 0; d < DT; d++) {
+        const int at = rv0 * D + ((2 * d + ((col & 3) >> 1)) ^ xv) * 8 + (col & 1) * 4;
+        typedef __attribute__((address_space(3))) at_s16x4* lds_ptr;
+        const at_s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(s_v + at));
+        const at_s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(s_v + at + 4 * D));
+        u32x4 vt = __builtin_bit_cast(u32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
+        if (border) {  // a value that a row does not see must not reach it, and 0 * NaN would: such values are taken out here
+          odd |= odd_pair(vt.x) || odd_pair(vt.y) || odd_pair(vt.z) || odd_pair(vt.w);
+          vt = u32x4{finite_pair(vt.x), finite_pair(vt.y), finite_pair(vt.z), finite_pair(vt.w)};
+        }
+        const at_bf16x8 fv = frag(vt);
+#pragma unroll
+        for (int i = 0; i < NQ; i++) {
+#pragma unroll
+          for (int p = P::PPARTS - 1; p >= 0; p--) acc[i][d] = mma(fv, fp[p][i], acc[i][d]);
+        }
+      }
+      if (border && __ballot(odd)) odd_values<D, NQ>(s_v, base, see, fp[0], acc);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < NQ; i++) l[i] = sum32(sum16(l[i]));
+
+  // The waves along keys meet in LDS, 16 rows at a time: O of a row at [row][D + 4], its maximum and sum behind.
+  auto put = [&](int64_t at, int d, at_f32x4 x, float mm, float ll) {
+    if (a.splits > 1) {
+      const int64_t base = ((int64_t)split * a.T * (a.kv * a.group) + at);
+      *reinterpret_cast<at_f32x4*>(a.part_o + base * D + d) = x;
+      if (d == 0) {
+        a.part_ml[2 * base] = mm;
+        a.part_ml[2 * base + 1] = ll;
+      }
+    } else {
+      const float inv = ll > 0.f ? 1.0f / ll : (ll == 0.f ? 0.f : ll);  // (no key seen: zeros; a NaN stays)
+      x *= inv;
+      const int64_t token_ = at / (a.kv * a.group), head = at - token_ * (a.kv * a.group);
+      const int64_t to = token_ * a.o_token + head * a.o_head + d;
+      if (F32) *reinterpret_cast<at_f32x4*>(reinterpret_cast<float*>(a.o) + to) = x;
+      else *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(a.o) + to) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+    }
+  };
+  if constexpr (WK == 1) {
+#pragma unroll
+    for (int i = 0; i < NQ; i++) {
+      if (o_at[i] < 0) continue;
+#pragma unroll
+      for (int d = 0; d < DT; d++) put(o_at[i], 16 * d + 4 * g, acc[i][d], m[i], l[i]);
+    }
+  } else {
+    constexpr int HALF = D / 2;  // (half of O at a time: four waves' rows of 256 elements would not fit)
+    float* so = reinterpret_cast<float*>(s_k);   // [wave][16][HALF]
+    float* sm = reinterpret_cast<float*>(s_v);   // [wave][16][2]
+    static_assert(4 * 16 * HALF * 4 <= KT * D * 2 && 4 * 16 * 2 * 4 <= KT * D * 2, "");
+#pragma unroll
+    for (int i = 0; i < NQ; i++) {
+#pragma unroll
+      for (int part = 0; part < 2; part++) {
+        __syncthreads();
+#pragma unroll
+        for (int d = 0; d < DT / 2; d++) *reinterpret_cast<at_f32x4*>(so + (wave * 16 + col) * HALF + ((4 * d + g) ^ (col & 7)) * 4) = acc[i][part * (DT / 2) + d];
+        if (g == 0) {
+          sm[(wave * 16 + col) * 2] = m[i];
+          sm[(wave * 16 + col) * 2 + 1] = l[i];
+        }
+        __syncthreads();
+        // the WK waves of row block w: every one of them joins a share of its 16 rows
+        for (int e = wk * 64 + lane; e < 16 * (HALF / 4); e += WK * 64) {
+          const int r = e / (HALF / 4), p = e % (HALF / 4);
+          const int row = row0 + wr * P::ROWS + i * 16 + r;
+          if (row >= rows) continue;
+          float top = -INFINITY;
+#pragma unroll
+          for (int w = 0; w < WK; w++) top = fmaxf(top, sm[((w * WR + wr) * 16 + r) * 2]);
+          const float ref = top == -INFINITY ? 0.f : top;
+          at_f32x4 x = {0.f, 0.f, 0.f, 0.f};
+          float sum = 0.f;
+#pragma unroll
+          for (int w = 0; w < WK; w++) {
+            const int at = (w * WR + wr) * 16 + r;
+            const float f = __builtin_amdgcn_exp2f(sm[at * 2] - ref);
+            sum += sm[at * 2 + 1] * f;
+            x += *reinterpret_cast<const at_f32x4*>(so + at * HALF + (p ^ (r & 7)) * 4) * f;
+          }
+          const int t = row / a.group;
+          put((int64_t)(s.first + t) * (a.kv * a.group) + h * a.group + (row - t * a.group), part * HALF + p * 4, x, top, sum);
+        }
+      }
+    }
+  }
+}
+
+// Joins the splits of a row: one lane per four elements
+template <int D, bool F32>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a) {
+  constexpr int L = D / 4, PER = 256 / L;
+  const int heads = a.kv * a.group;
+  const int b = blockIdx.y;
+  const Seq s = sequence(a, b);
+  const int64_t i = (int64_t)blockIdx.x * PER + threadIdx.x / L;
+  if (i >= (int64_t)s.n * heads || i >= (int64_t)a.max_rows * a.kv) return;
+  const int d = threadIdx.x % L * 4;
+  const int64_t row = (int64_t)s.first * heads + i, step = (int64_t)a.T * heads;
+  const int used = max(1, min(a.splits, (s.keys + a.chunk - 1) / a.chunk));
+  float top = -INFINITY;
+  for (int k = 0; k < used; k++) top = fmaxf(top, a.part_ml[2 * (k * step + row)]);
+  const float ref = top == -INFINITY ? 0.f : top;
+  at_f32x4 x = {0.f, 0.f, 0.f, 0.f};
+  float sum = 0.f;
+  for (int k = 0; k < used; k++) {
+    const int64_t at = k * step + row;
+    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - ref);
+    sum += a.part_ml[2 * at + 1] * f;
+    x += *reinterpret_cast<const at_f32x4*>(a.part_o + at * D + d) * f;
+  }
+  x *= sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
+  const int64_t token = row / heads, to = token * a.o_token + (row - token * heads) * a.o_head + d;
+  if (F32) *reinterpret_cast<at_f32x4*>(reinterpret_cast<float*>(a.o) + to) = x;
+  else *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(a.o) + to) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------------
+struct AttnPlan {
+  int nq, wr, row_tiles, splits, chunk;
+};
+// Rows of a workgroup by the rows there are (tokens times query heads of a key head), then as many ranges of keys as give every CU two workgroups, of at
+// least two tiles each.
+static AttnPlan attention_plan(bool f32, int64_t B, int heads, int kv, int64_t max_tokens, int64_t max_keys, int D) {
+  AttnPlan p;
+  const int64_t rows = max_tokens * (heads / kv);
+  p.wr = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+  p.nq = rows <= 16 ? 1 : rows <= 128 || f32 ? 2 : 4;
+  if (D == 256 && p.nq > 2) p.nq = 2;
+  if (D == 256 && f32) p.nq = 1;
+  const int64_t per = (int64_t)p.nq * 16 * p.wr;
+  const int64_t tiles = (rows + per - 1) / per;
+  p.row_tiles = (int)(tiles < 0x7fffffff ? tiles : 0x7fffffff);
+  const int kt = p.wr == 1 ? 128 : 64;
+  const int64_t units = B * kv * tiles, most = (max_keys + 2 * kt - 1) / (2 * kt);
+  int64_t splits = units >= 512 ? 1 : 512 / units;
+  if (splits > most) splits = most < 1 ? 1 : most;
+  const int64_t chunk = (max_keys + splits - 1) / splits;
+  p.chunk = (int)((chunk + kt - 1) / kt * kt);
+  if (p.chunk < kt) p.chunk = kt;
+  p.splits = (int)((max_keys + p.chunk - 1) / p.chunk);
+  if (p.splits < 1) p.splits = 1;
+  return p;
+}
+static bool attention_sizes(int dtype, int64_t T, int64_t B, int heads, int kv, int head_dim, int64_t max_tokens, int64_t max_keys) {
+  return (dtype == MLLM_HIP_F32 || dtype == MLLM_HIP_BF16) && T >= 0 && B >= 0 && heads >= 1 && kv >= 1 && max_tokens >= 0 && max_keys >= 0;
+}
+static bool attention_shape(int64_t T, int64_t B, int heads, int kv, int head_dim, int64_t max_tokens, int64_t max_keys) {
+  return (head_dim == 64 || head_dim == 128 || head_dim == 256) && heads % kv == 0 && heads <= 65536 && T <= 0x7fffffff / heads && B <= 0x7fffffff / heads &&
+         max_tokens <= 0x7fffffff / heads && max_keys <= 0x7fff0000;
+}
+
+}  // namespace mllmhip
+
+using namespace mllmhip;
+
+MLLM_API size_t mllm_hip_attention_paged_workspace_bytes(int dtype, int64_t T, int64_t B, int heads, int kv_heads, int head_dim, int64_t max_tokens,
+                                                         int64_t max_keys) {
+  if (!attention_sizes(dtype, T, B, heads, kv_heads, head_dim, max_tokens, max_keys) || !attention_shape(T, B, heads, kv_heads, head_dim, max_tokens, max_keys)) return 0;
+  if (T == 0 || B == 0 || max_tokens == 0) return 0;
+  const AttnPlan p = attention_plan(dtype == MLLM_HIP_F32, B, heads, kv_heads, max_tokens, max_keys, head_dim);
+  return p.splits > 1 ? (size_t)p.splits * T * heads * (head_dim + 4) * sizeof(float) : 0;
+}
+
+MLLM_API int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_t T, const mllm_hip_kv_cache* cache, const int32_t* block_table,
+                                      int64_t table_stride, int64_t table_len, const int32_t* cu_tokens, const int32_t* prefix, int64_t B,
+                                      int64_t max_tokens, int64_t max_keys, const uint64_t* tree, int64_t tree_stride, int64_t tree_words, float scale,
+                                      void* workspace, size_t workspace_bytes, void* stream) {
+  if (!q || !cache || table_len < 0 || tree_words < 0 || !(scale > 0.f) || scale > 3e38f || cache->pages < 1 || cache->page_size < 1) return MLLM_HIP_E_BADARG;
+  if (!attention_sizes(dtype, T, B, q->heads, cache->heads, cache->head_dim, max_tokens, max_keys)) return MLLM_HIP_E_BADARG;
+  if (!attention_shape(T, B, q->heads, cache->heads, cache->head_dim, max_tokens, max_keys) || cache->pages > 0x7fffffff / cache->page_size ||
+      table_len > 0x7fff0000 / cache->page_size || tree_words > 0x1ffffff)
+    return MLLM_HIP_E_SHAPE;
+  if (T == 0 || B == 0 || max_tokens == 0) return 0;
+  if (!q->x || !q->y || !cache->k || !cache->v || !block_table || !cu_tokens || !prefix || table_len < 1) return MLLM_HIP_E_BADARG;
+  const int wide = dtype == MLLM_HIP_F32 ? 4 : 2;
+  auto al = [](const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
+  auto whole = [&](int64_t stride) { return stride * wide % 16 == 0; };
+  if (!al(q->x, 16) || !al(q->y, 16) || !al(cache->k, 16) || !al(cache->v, 16) || !whole(q->x_token_stride) || !whole(q->x_head_stride) || !whole(q->y_token_stride) ||
+      !whole(q->y_head_stride) || cache->page_stride % 8 || cache->slot_stride % 8 || cache->head_stride % 8 || !al(block_table, 4) || !al(cu_tokens, 4) || !al(prefix, 4) ||
+      !al(tree, 8) || !al(workspace, 16))
+    return MLLM_HIP_E_ALIGN;
+  const bool f32 = dtype == MLLM_HIP_F32;
+  const int heads = q->heads, D = cache->head_dim;
+  const AttnPlan p = attention_plan(f32, B, heads, cache->heads, max_tokens, max_keys, D);
+  const size_t need = p.splits > 1 ? (size_t)p.splits * T * heads * (D + 4) * sizeof(float) : 0;
+  if (need && (!workspace || workspace_bytes < need)) return MLLM_HIP_E_BADARG;
+  const int64_t groups = (B * cache->heads * p.splits + 7) / 8 * 8;
+  if (groups > 0x7fffffff / p.row_tiles) return MLLM_HIP_E_SHAPE;
+  AttnArgs a = {};
+  a.q = q->x;
+  a.o = q->y;
+  a.q_token = q->x_token_stride;
+  a.q_head = q->x_head_stride;
+  a.o_token = q->y_token_stride;
+  a.o_head = q->y_head_stride;
+  a.k = reinterpret_cast<const uint16_t*>(cache->k);
+  a.v = reinterpret_cast<const uint16_t*>(cache->v);
+  a.page_stride = cache->page_stride;
+  a.slot_stride = cache->slot_stride;
+  a.head_stride = cache->head_stride;
+  a.pages = (uint32_t)cache->pages;
+  a.page = (uint32_t)cache->page_size;
+  // key / page for key < 2^31: with 2^s >= page the multiplier ceil(2^(31 + s) / page) is off by less than 2^s / 2^31 of a key
+  int s = 0;
+  while ((1ll << s) < cache->page_size) s++;
+  a.page_mul = (uint32_t)(((1ull << (31 + s)) + cache->page_size - 1) / cache->page_size);
+  a.page_shift = 31 + s;
+  a.table = block_table;
+  a.table_stride = table_stride;
+  a.table_len = (int)table_len;
+  a.cu = cu_tokens;
+  a.prefix = prefix;
+  a.tree = tree;
+  a.tree_stride = tree_stride;
+  a.words = (int)tree_words;
+  a.T = (int)T;
+  a.B = (int)B;
+  a.kv = cache->heads;
+  a.group = heads / cache->heads;
+  a.max_rows = (int)(max_tokens * a.group);
+  a.row_tiles = p.row_tiles;
+  a.splits = p.splits;
+  a.chunk = p.chunk;
+  a.c = scale * 1.44269504088896341f;
+  a.part_o = reinterpret_cast<float*>(workspace);
+  a.part_ml = a.part_o ? a.part_o + (size_t)p.splits * T * heads * D : nullptr;
+  hipStream_t st = (hipStream_t)stream;
+  const dim3 grid((unsigned)(groups * p.row_tiles));
+  const int form = p.nq * 10 + p.wr;
+  auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a); };
+#define ATTN(D_, F_)                                                                   \
+  switch (form) {                                                                      \
+    case 11: go(attention_kernel<D_, 1, 1, F_>); break;                                \
+    case 12: go(attention_kernel<D_, 1, 2, F_>); break;                                \
+    case 14: go(attention_kernel<D_, 1, 4, F_>); break;                                \
+    case 21: go(attention_kernel<D_, 2, 1, F_>); break;                                \
+    case 22: go(attention_kernel<D_, 2, 2, F_>); break;                                \
+    case 24: go(attention_kernel<D_, 2, 4, F_>); break;                                \
+    default: go(attention_kernel<D_, F_ || D_ == 256 ? 2 : 4, 4, F_>); break;          \
+  }
+  if (D == 64) {
+    if (f32) { ATTN(64, true) } else { ATTN(64, false) }
+  } else if (D == 128) {
+    if (f32) { ATTN(128, true) } else { ATTN(128, false) }
+  } else {
+    if (f32) { ATTN(256, true) } else { ATTN(256, false) }
+  }
+#undef ATTN
+  RC_RET((int)hipGetLastError());
+  if (p.splits > 1) {
+    const int per = 256 / (D / 4);
+    const dim3 jgrid((unsigned)((max_tokens * heads + per - 1) / per), (unsigned)B);
+    auto join = [&](auto kern) { hipLaunchKernelGGL(kern, jgrid, dim3(256), 0, st, a); };
+    if (D == 64) {
+      if (f32) join(attention_join_kernel<64, true>); else join(attention_join_kernel<64, false>);
+    } else if (D == 128) {
+      if (f32) join(attention_join_kernel<128, true>); else join(attention_join_kernel<128, false>);
+    } else {
+      if (f32) join(attention_join_kernel<256, true>); else join(attention_join_kernel<256, false>);
+    }
+  }
+  return (int)hipGetLastError();
+}

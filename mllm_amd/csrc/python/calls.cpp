@@ -6,6 +6,8 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <cmath>
+
 #include <ATen/ATen.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/python_variable.h>
@@ -314,16 +316,16 @@ const T* vector_of(PyObject* o, int64_t device, at::ScalarType type, int64_t n) 
 }
 int64_t stride_of(const at::Tensor& t, int64_t dim) { return t.size(dim) > 1 ? t.stride(dim) : 0; }  // (of a single row any number may stand there)
 // [T, heads, D] with rows in one piece
-mllm_hip_rope_part heads_of(const at::Tensor& x, int64_t T, int64_t D, at::ScalarType type, int64_t device) {
+mllm_hip_heads heads_of(const at::Tensor& x, int64_t T, int64_t D, at::ScalarType type, int64_t device) {
   require(x.is_cuda() && x.get_device() == device && x.scalar_type() == type && x.dim() == 3 && x.size(0) == T && x.size(2) == D && (D == 1 || x.stride(2) == 1));
   require(x.size(1) >= 1 && x.size(1) <= 65536);
-  return mllm_hip_rope_part{x.data_ptr(), nullptr, nullptr, stride_of(x, 0), stride_of(x, 1), 0, 0, (int)x.size(1)};
+  return mllm_hip_heads{x.data_ptr(), nullptr, nullptr, stride_of(x, 0), stride_of(x, 1), 0, 0, (int)x.size(1)};
 }
 // where a part's results go: the given tensor or a new one
-void results_to(mllm_hip_rope_part& p, const at::Tensor& x, PyObject* out, at::Tensor& made, int64_t device) {
+void results_to(mllm_hip_heads& p, const at::Tensor& x, PyObject* out, at::Tensor& made, int64_t device) {
   if (out == Py_None) made = at::empty(x.sizes(), x.options());
   else made = tensor(out);
-  const mllm_hip_rope_part y = heads_of(made, x.size(0), x.size(2), x.scalar_type(), device);
+  const mllm_hip_heads y = heads_of(made, x.size(0), x.size(2), x.scalar_type(), device);
   require(y.heads == p.heads);
   p.y = made.data_ptr();
   p.y_token_stride = y.x_token_stride;
@@ -358,7 +360,7 @@ PyObject* qk_norm_rope(Args a) {
   const int dtype = xdtype(q);
   require(q.dim() == 3);
   const int64_t T = q.size(0), D = q.size(2);
-  mllm_hip_rope_part parts[2] = {heads_of(q, T, D, q.scalar_type(), device), heads_of(k, T, D, q.scalar_type(), device)};
+  mllm_hip_heads parts[2] = {heads_of(q, T, D, q.scalar_type(), device), heads_of(k, T, D, q.scalar_type(), device)};
   PyObject *oq = Py_None, *ok = Py_None;
   if (a[9] != Py_None) {
     require(PyTuple_Check(a[9]) && PyTuple_GET_SIZE(a[9]) == 2);
@@ -387,7 +389,7 @@ PyObject* kv_append(Args a) {
   require(k.dim() == 3);
   const mllm_hip_kv_cache cache = cache_of(a[2], a[3], device);
   const int64_t T = k.size(0), D = cache.head_dim;
-  mllm_hip_rope_part kp = heads_of(k, T, D, k.scalar_type(), device), vp = heads_of(v, T, D, k.scalar_type(), device), qp = {};
+  mllm_hip_heads kp = heads_of(k, T, D, k.scalar_type(), device), vp = heads_of(v, T, D, k.scalar_type(), device), qp = {};
   require(kp.heads == cache.heads && vp.heads == cache.heads);
   kp.weight = vector_of<float>(a[7], device, at::kFloat, D);
   at::Tensor y;
@@ -410,6 +412,44 @@ PyObject* kv_append(Args a) {
   return THPVariable_Wrap(y);
 }
 
+// (q, k_cache, v_cache, block_table, cu_tokens, prefix, max_tokens, max_keys, tree, scale, out, workspace)
+PyObject* attention_paged(Args a) {
+  const int64_t device = current_device();
+  const at::Tensor& q = tensor(a[0]);
+  const int dtype = xdtype(q);
+  require(q.dim() == 3);
+  const mllm_hip_kv_cache cache = cache_of(a[1], a[2], device);
+  const int64_t T = q.size(0);
+  mllm_hip_heads qp = heads_of(q, T, cache.head_dim, q.scalar_type(), device);
+  const at::Tensor& table = local(a[3], device, at::kInt);
+  require(table.dim() == 2 && (table.size(1) <= 1 || table.stride(1) == 1));
+  const int64_t B = table.size(0), tokens = integer(a[6]), keys = integer(a[7]);
+  require(a[4] != Py_None && a[5] != Py_None);
+  const int32_t *cu = vector_of<int32_t>(a[4], device, at::kInt, B + 1), *prefix = vector_of<int32_t>(a[5], device, at::kInt, B);
+  const uint64_t* tree = nullptr;
+  int64_t tree_stride = 0, words = 0;
+  if (a[8] != Py_None) {
+    const at::Tensor& t = local(a[8], device, at::kLong);
+    require(t.dim() == 2 && t.size(0) == T && (t.size(1) <= 1 || t.stride(1) == 1));
+    require(t.size(1) >= 1 || T == 0);
+    tree = reinterpret_cast<const uint64_t*>(t.data_ptr());
+    tree_stride = stride_of(t, 0), words = t.size(1);
+  }
+  const float scale = a[9] == Py_None ? 1.0f / std::sqrt((float)cache.head_dim) : (float)real(a[9]);
+  at::Tensor y, work;
+  results_to(qp, q, a[10], y, device);
+  require(T == 0 || qp.y != qp.x);
+  const size_t need = mllm_hip_attention_paged_workspace_bytes(dtype, T, B, qp.heads, cache.heads, cache.head_dim, tokens, keys);
+  void* wp = need || a[11] != Py_None ? workspace(a[11], need, work) : nullptr;
+  void* st = stream();
+  const int64_t table_stride = stride_of(table, 0), table_len = table.size(1);
+  const int32_t* tp = static_cast<const int32_t*>(table.data_ptr());
+  run("mllm_hip_attention_paged", [&] {
+    return mllm_hip_attention_paged(&qp, dtype, T, &cache, tp, table_stride, table_len, cu, prefix, B, tokens, keys, tree, tree_stride, words, scale, wp, need, st);
+  });
+  return THPVariable_Wrap(y);
+}
+
 template <PyObject* (*F)(Args), int N>
 PyObject* entry(PyObject*, Args args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -427,7 +467,7 @@ PyObject* entry(PyObject*, Args args, Py_ssize_t n) {
 #define CALL(name, n) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(entry<name, n>)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {CALL(linear_q_gemv, 8), CALL(linear_q_gemv_multi, 6), CALL(softmax, 1), CALL(topk, 4), CALL(matmul, 5),
                            CALL(w8a8_linear_packed, 7), CALL(w4a16_gemm_packed, 6), CALL(linear_q_gemm, 7), CALL(linear_kq_gemm, 6),
-                           CALL(qk_norm_rope, 10), CALL(kv_append, 14), {nullptr, nullptr, 0, nullptr}};
+                           CALL(qk_norm_rope, 10), CALL(kv_append, 14), CALL(attention_paged, 12), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "mllm_calls", nullptr, -1, g_methods};
 
 }  // namespace

@@ -130,7 +130,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
 static bool al16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // a part as the kernel takes it: checks of the strides that 16-byte loads and stores need
-static int rope_group(const mllm_hip_rope_part& p, int dtype, int head_dim, bool stored, RopeGroup& g) {
+static int rope_group(const mllm_hip_heads& p, int dtype, int head_dim, bool stored, RopeGroup& g) {
   const int wide = dtype == MLLM_HIP_F32 ? 4 : 2;
   if (!p.x || (stored && !p.y) || p.heads < 1) return MLLM_HIP_E_BADARG;
   if (p.heads > 65536) return MLLM_HIP_E_SHAPE;
@@ -183,7 +183,7 @@ static int rope_checks(int dtype, int64_t T, int head_dim, const int32_t* positi
 
 using namespace mllmhip;
 
-MLLM_API int mllm_hip_qk_norm_rope(int nparts, const mllm_hip_rope_part* parts, int dtype, int64_t T, int head_dim, float epsilon,
+MLLM_API int mllm_hip_qk_norm_rope(int nparts, const mllm_hip_heads* parts, int dtype, int64_t T, int head_dim, float epsilon,
                                    int add_unit_offset, const int32_t* positions, const double* inv_freq, int rot_dim,
                                    int interleaved, void* stream) {
   if (nparts < 1 || nparts > 4 || !parts) return MLLM_HIP_E_BADARG;
@@ -204,7 +204,7 @@ MLLM_API int mllm_hip_qk_norm_rope(int nparts, const mllm_hip_rope_part* parts, 
   return rope_launch(a, dtype, T, head_dim, rot_dim, interleaved, heads, (hipStream_t)stream);
 }
 
-MLLM_API int mllm_hip_kv_append(const mllm_hip_rope_part* q, const mllm_hip_rope_part* k, const mllm_hip_rope_part* v, int dtype, int64_t T,
+MLLM_API int mllm_hip_kv_append(const mllm_hip_heads* q, const mllm_hip_heads* k, const mllm_hip_heads* v, int dtype, int64_t T,
                                 const mllm_hip_kv_cache* cache, const int64_t* slots, float epsilon, int add_unit_offset,
                                 const int32_t* positions, const double* inv_freq, int rot_dim, int interleaved, void* stream) {
   if (!k || !v || !cache || !cache->k || !cache->v || (T && !slots) || cache->heads < 1 || cache->pages < 1 || cache->page_size < 1) return MLLM_HIP_E_BADARG;

@@ -679,3 +679,31 @@ def kv_append(k, v, k_cache, v_cache, slots, positions=None, inv_freq=None, k_we
     one layout (any strides of whole 16 bytes); token t goes to slots[t] (int64: page * page_size + place in the page; outside the cache:
     stored nowhere; two tokens with one slot leave either's elements).  q [T, Hq, D]: the queries in the same launch, returned anew or in `out`."""
     return _calls().kv_append(k, v, k_cache, v_cache, slots, positions, inv_freq, k_weight, q, q_weight, eps, add_unit_offset, interleaved, out)
+
+
+def attention_paged(q, k_cache, v_cache, block_table, cu_tokens, prefix, max_tokens, max_keys, tree=None, scale=None, out=None, workspace=None):
+    """softmax(scale * q k^T) v of new tokens, which the cache holds already, over their sequences: q [T, Hq, D] fp32 or bf16 (D 64, 128 or 256), rows
+    cu_tokens[b] .. cu_tokens[b + 1] - 1 (int32 [B + 1]) of sequence b behind the prefix[b] (int32 [B]) positions it had; position i is place
+    i % page_size of page block_table[b, i // page_size] (int32 [B, n]) of k_cache / v_cache as in kv_append.  A token sees the prefix and, of its
+    sequence's new tokens, the ones of its row of `tree` (int64 [T, words] of 64 bits, as tree_mask makes them; None: itself and
+    those before it).  max_tokens, max_keys: bounds of a sequence's new tokens and of its positions with them.  scale: 1 / sqrt(D).  A token that sees nothing
+    gets zeros; rows in no sequence are left as they are in `out` (a new tensor has any numbers there)."""
+    return _calls().attention_paged(q, k_cache, v_cache, block_table, cu_tokens, prefix, max_tokens, max_keys, tree, scale, out, workspace)
+
+
+def tree_mask(parents, words=None):
+    """Rows of bits for attention_paged, on the host: `parents` says for every token of a tree which token before it it continues (below 0: the
+    prefix); a token sees itself and its ancestors.  Returns int64 [n, words] (words: at least ceil(n / 64), the default)."""
+    n = len(parents)
+    need = -(-n // 64)
+    words = need if words is None else words
+    if words < need:
+        raise ValueError("%d words for %d tokens" % (words, n))
+    rows, full = [], (1 << 64) - 1
+    for i, p in enumerate(parents):
+        p = int(p)
+        if p >= i:
+            raise ValueError("token %d continues token %d, which does not come before it" % (i, p))
+        rows.append((rows[p] if p >= 0 else 0) | 1 << i)
+    signed = lambda w: w - (1 << 64) if w >> 63 else w  # noqa: E731
+    return torch.tensor([[signed(r >> (64 * w) & full) for w in range(words)] for r in rows], dtype=torch.int64).view(n, words)

@@ -25,11 +25,12 @@ def norm_rope(x, weight, eps, positions, inv_freq, interleaved, unit=False):
 
 def attention(q, k_cache, v_cache, table, cu, prefix, seen, scale):
     """q [T, Hq, D]; seen: one [n, n] truth array per sequence (which new tokens a new token sees).  Positions of pages outside the cache count
-    as zeros, positions behind the block table do not exist.  Returns float64 [T, Hq, D]; rows behind the last sequence are NaN."""
-    q, kc, vc = q.detach().cpu().double(), k_cache.detach().cpu().double(), v_cache.detach().cpu().double()
-    pages, page, kv, D = kc.shape
+    as zeros, positions behind the block table do not exist.  Returns float64 [T, Hq, D] (rows in no sequence NaN) and, for error bounds, the same
+    with |v| for v and the largest sum of a score's absolute terms [T, Hq, 1]."""
+    q = q.detach().cpu().double()
+    pages, page, kv, D = k_cache.shape
     group = q.shape[1] // kv
-    out = torch.full(q.shape, float("nan"), dtype=torch.float64)
+    out, size, terms = torch.full(q.shape, float("nan"), dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape[:2] + (1,), dtype=torch.float64)
     for b in range(len(cu) - 1):
         lo, n = int(cu[b]), int(cu[b + 1] - cu[b])
         length = min(int(prefix[b]) + n, table.shape[1] * page)
@@ -41,8 +42,9 @@ def attention(q, k_cache, v_cache, table, cu, prefix, seen, scale):
         see[:, int(prefix[b]):] = torch.as_tensor(seen[b])
         see = see[:, :length]
         for h in range(q.shape[1]):
-            k = torch.where(good[:, None], kc[ids, at % page, h // group], 0.0)
-            v = torch.where(good[:, None], vc[ids, at % page, h // group], 0.0)
+            if h % group == 0:
+                k, v = [c[ids.to(c.device), (at % page).to(c.device), h // group].cpu().double() for c in (k_cache, v_cache)]
+                k, v = [torch.where(good[:, None], c, 0.0) for c in (k, v)]
             for t in range(n):
                 m = see[t]
                 if not m.any():
@@ -50,8 +52,11 @@ def attention(q, k_cache, v_cache, table, cu, prefix, seen, scale):
                     continue
                 s = (k[m] @ q[lo + t, h]) * scale
                 p = (s - s.max()).exp()
-                out[lo + t, h] = (p / p.sum()) @ v[m]
-    return out
+                p = p / p.sum()
+                out[lo + t, h] = p @ v[m]
+                size[lo + t, h] = p @ v[m].abs()
+                terms[lo + t, h] = (k[m].abs() @ q[lo + t, h].abs()).max() * scale
+    return out, size, terms
 
 
 def ancestors(parents):

@@ -14,7 +14,7 @@ F32, BF16 = 0, 1
 def _part(**changed):
     p = dict(x=P, y=P, weight=P, x_token_stride=512, x_head_stride=128, y_token_stride=512, y_head_stride=128, heads=4)
     p.update(changed)
-    return _lib.RopePart(**p)
+    return _lib.Heads(**p)
 
 
 def _cache(**changed):
@@ -52,3 +52,43 @@ def _append(k=None, v=None, q=None, cache=None, slots=P, T=1, dtype=BF16, rot=12
     (dict(q=_part(y=None)), BADARG), (dict(q=_part(y=ODD)), ALIGN), (dict(k=_part(y=None), v=_part(y=None, weight=None), T=0), 0), (dict(rot=24), SHAPE), (dict(dtype=5), BADARG)])
 def test_kv_append(args, want):
     assert _append(**args) == want
+
+
+def _attend(q=None, cache=None, dtype=BF16, T=2, table=P, table_len=4, cu=P, prefix=P, B=1, tokens=2, keys=40, tree=None, words=0, scale=0.1, work=P, size=1 << 30, no_q=False):
+    q, cache = q if q is not None else _part(heads=8), cache if cache is not None else _cache()
+    return _lib.lib().mllm_hip_attention_paged(None if no_q else C.byref(q), dtype, T, C.byref(cache), table, 4, table_len, cu, prefix, B, tokens, keys, tree, words, words, scale, work, size, None)
+
+
+@pytest.mark.parametrize("args,want", [
+    (dict(no_q=True), BADARG), (dict(dtype=2), BADARG), (dict(T=-1), BADARG), (dict(B=-1), BADARG), (dict(tokens=-1), BADARG), (dict(keys=-1), BADARG), (dict(table=None), BADARG),
+    (dict(cu=None), BADARG), (dict(prefix=None), BADARG), (dict(table_len=0), BADARG), (dict(table_len=-1), BADARG), (dict(words=-1), BADARG), (dict(scale=0.0), BADARG),
+    (dict(scale=-0.1), BADARG), (dict(scale=float("nan")), BADARG), (dict(scale=float("inf")), BADARG), (dict(q=_part(heads=8, x=None)), BADARG), (dict(q=_part(heads=8, y=None)), BADARG),
+    (dict(q=_part(heads=0)), BADARG), (dict(q=_part(heads=6)), SHAPE), (dict(cache=_cache(head_dim=96)), SHAPE), (dict(cache=_cache(head_dim=32)), SHAPE),
+    (dict(cache=_cache(heads=0)), BADARG), (dict(cache=_cache(pages=1 << 27)), SHAPE), (dict(table_len=1 << 27), SHAPE), (dict(T=1 << 29), SHAPE), (dict(B=1 << 29), SHAPE),
+    (dict(tokens=1 << 29), SHAPE), (dict(keys=(1 << 31) - 1), SHAPE), (dict(words=1 << 26), SHAPE), (dict(q=_part(heads=8, x=ODD)), ALIGN), (dict(q=_part(heads=8, y=ODD)), ALIGN),
+    (dict(q=_part(heads=8, x_token_stride=516)), ALIGN), (dict(q=_part(heads=8, y_head_stride=68)), ALIGN), (dict(cache=_cache(slot_stride=4)), ALIGN), (dict(cache=_cache(v=ODD)), ALIGN),
+    (dict(table=ODD), ALIGN), (dict(cu=ODD), ALIGN), (dict(prefix=ODD), ALIGN), (dict(tree=P + 4, words=1), ALIGN), (dict(work=P + 8), ALIGN),
+    (dict(keys=4000, work=None), BADARG), (dict(keys=4000, size=1000), BADARG), (dict(T=0), 0), (dict(B=0), 0), (dict(tokens=0), 0)])
+def test_attention_paged(args, want):
+    assert _attend(**args) == want
+
+
+def test_attention_workspace():
+    size = _lib.lib().mllm_hip_attention_paged_workspace_bytes
+    assert size(BF16, 1, 1, 32, 8, 128, 1, 100) == 0  # one range of keys
+    a, b = size(BF16, 1, 1, 32, 8, 128, 1, 5000), size(F32, 1, 1, 32, 8, 128, 1, 5000)
+    assert a > 0 and a % (32 * (128 + 4) * 4) == 0 and a == b
+    assert size(BF16, 2048, 64, 32, 8, 128, 32, 5000) == 0  # rows enough for every CU
+    assert size(2, 1, 1, 32, 8, 128, 1, 5000) == 0 and size(BF16, 1, 1, 30, 8, 128, 1, 5000) == 0 and size(BF16, 0, 1, 32, 8, 128, 1, 5000) == 0
+
+
+def test_tree_mask():
+    from mllm_amd import qlinear as ql
+    assert ql.tree_mask([-1, 0, 0, 1]).tolist() == [[1], [3], [5], [11]]
+    chain = ql.tree_mask(list(range(-1, 129)))
+    assert chain.shape == (130, 3) and chain[63, 0] == -1 and chain[64].tolist() == [-1, 1, 0] and chain[129].tolist() == [-1, -1, 3]
+    assert ql.tree_mask([], 2).shape == (0, 2) and ql.tree_mask([-5], 2).tolist() == [[1, 0]]
+    with pytest.raises(ValueError):
+        ql.tree_mask([0])
+    with pytest.raises(ValueError):
+        ql.tree_mask(list(range(-1, 64)), 1)
