@@ -20,6 +20,8 @@
 // the tile before them is worked on, from there into LDS.  Rows of a tile lie there with their 16-byte pieces exclusive-ored by bits of the
 // key's number, so that the 16 lanes of an operand read different banks.  Where rows and heads leave CUs idle the keys are cut into ranges
 // (splits), whose O, maximum and sum meet in the workspace; a second launch joins them.
+#include <type_traits>
+
 #include "item8.h"
 
 namespace mllmhip {
@@ -34,8 +36,9 @@ struct AttnArgs {
   void* o;
   int64_t q_token, q_head, o_token, o_head;
   const uint16_t *k, *v;
-  int64_t page_stride, slot_stride, head_stride;
-  uint32_t pages, page, page_mul;  // key / page = (key * page_mul) >> page_shift for key < 2^31
+  int64_t head_stride;
+  uint32_t page_bytes, slot_bytes;
+  uint32_t pages, page, page_mul;  // key / page = (2 key * page_mul) >> 32 >> page_shift for key < 2^31
   int page_shift;
   const int32_t* table;
   int64_t table_stride;
@@ -48,7 +51,7 @@ struct AttnArgs {
   float c;  // scale * log2 e
   float *part_o, *part_ml;  // [split][token][query head][head_dim], [split][token][query head][2]
 };
-__device__ const u32x4 g_zero_row[1] = {};  // what a page outside the cache reads as
+__device__ u32x4 g_zero_row[1];  // what a page outside the cache reads as (never written)
 
 // sequence b: its first row of q, its number of new tokens, of prefix keys and of keys
 struct Seq {
@@ -78,6 +81,7 @@ struct Attn {
   static constexpr int NLOAD = KT / 4 / RPI;             // loads of keys (and of values) of a lane per tile
   static constexpr int PARTS = F32 ? 3 : 1, PPARTS = F32 ? 2 : 1;
   static constexpr int ROWS = NQ * 16;                   // rows of a wave
+  static constexpr int WAVES = D * NQ <= (F32 ? 128 : 256) ? 2 : 1;  // per SIMD: 256 registers each, or all 512 for one
   static __device__ __forceinline__ int swz(int row) { return (C == 8) ? (row & 3) | ((row >> 3) & 1) << 2 : (row & 3) | ((row >> 3) & 3) << 2; }
 };
 
@@ -101,40 +105,13 @@ __device__ __forceinline__ uint32_t seen_keys(const AttnArgs& a, const Seq& s, i
   return left >= 8 ? see & 0xff : left <= 0 ? 0 : see & ((1u << left) - 1);
 }
 // whether one of two bf16 is infinite or no number
-__device__ __forceinline__ bool odd_pair(uint32_t v) { return (v & 0x7f80u) == 0x7f80u || (v & 0x7f800000u) == 0x7f800000u; }
+__device__ __forceinline__ bool odd_pair(uint32_t v) { return ((v & 0x7f80u) == 0x7f80u) | ((v & 0x7f800000u) == 0x7f800000u); }
 __device__ __forceinline__ uint32_t finite_pair(uint32_t v) {
   return ((v & 0x7f80u) == 0x7f80u ? 0u : v & 0xffffu) | ((v & 0x7f800000u) == 0x7f800000u ? 0u : v & 0xffff0000u);
 }
 
-// The infinities and NaNs of a step's values, key by key, into the rows that see them (rare)
-template <int D, int NQ>
-__device__ __forceinline__ void odd_values(const uint16_t* s_v, int base, const uint32_t (&see)[NQ], const at_bf16x8 (&fp)[NQ], at_f32x4 (&acc)[NQ][D / 16]) {
-  const int lane = threadIdx.x & 63, col = lane & 15, g = lane >> 4;
-  constexpr int C = D / 8;
-#pragma unroll 1
-  for (int key = 0; key < 32; key++) {
-    const int row = base + key, x = (C == 8) ? (row & 3) | ((row >> 3) & 1) << 2 : (row & 3) | ((row >> 3) & 3) << 2;
-#pragma unroll
-    for (int i = 0; i < NQ; i++) {
-      const u32x4 mine = __builtin_bit_cast(u32x4, fp[i]);
-      const uint32_t pair = key % 8 / 2 == 0 ? mine.x : key % 8 / 2 == 1 ? mine.y : key % 8 / 2 == 2 ? mine.z : mine.w;
-      const float weight = __uint_as_float(key & 1 ? pair & 0xffff0000u : pair << 16);
-      const float p = __shfl(weight, key / 8 * 16 + col);
-      const bool seen = __shfl((int)see[i], key / 8 * 16 + col) >> (key % 8) & 1;
-#pragma unroll
-      for (int d = 0; d < D / 16; d++) {
-        const u32x2 v = *reinterpret_cast<const u32x2*>(s_v + row * D + ((2 * d + (g >> 1)) ^ x) * 8 + (g & 1) * 4);
-        const uint32_t w[4] = {v.x << 16, v.x & 0xffff0000u, v.y << 16, v.y & 0xffff0000u};
-#pragma unroll
-        for (int e = 0; e < 4; e++)
-          if (seen && (w[e] & 0x7f800000u) == 0x7f800000u) acc[i][d][e] += p * __uint_as_float(w[e]);
-      }
-    }
-  }
-}
-
 template <int D, int NQ, int WR, bool F32>
-__global__ __launch_bounds__(256) void attention_kernel(AttnArgs a) {
+__global__ __launch_bounds__(256, (Attn<D, NQ, WR, F32>::WAVES)) void attention_kernel(AttnArgs a) {
   typedef Attn<D, NQ, WR, F32> P;
   constexpr int KT = P::KT, C = P::C, WK = P::WK, NLOAD = P::NLOAD, KS = D / 32, DT = D / 16;
   __shared__ __align__(16) uint16_t s_k[KT * D];
@@ -149,14 +126,14 @@ __global__ __launch_bounds__(256) void attention_kernel(AttnArgs a) {
   // A lane's pieces of a tile: piece lane % C, as it lies in LDS, of rows load_row(i)
   const int piece = lane % C;
   auto load_row = [&](int i) { return wave * (KT / 4) + i * P::RPI + lane / C; };
-  const int64_t head_at = h * a.head_stride;
+  const int32_t* table = a.table + b * a.table_stride;
+  auto page_of = [&](uint32_t key) { return __umulhi(2 * key, a.page_mul) >> a.page_shift; };
   int ids[NLOAD];
   auto ask_pages = [&](int k0) {  // the pages of a tile's keys (the last page of the table for what lies behind it: never used)
 #pragma unroll
     for (int i = 0; i < NLOAD; i++) {
       const uint32_t key = (uint32_t)(k0 + load_row(i));
-      const uint32_t at = (uint32_t)(((uint64_t)key * a.page_mul) >> a.page_shift);
-      ids[i] = a.table[b * a.table_stride + min((int)at, a.table_len - 1)];
+      ids[i] = table[min((int)page_of(key), a.table_len - 1)];
     }
   };
   const int k_begin = split * a.chunk;
@@ -213,16 +190,18 @@ __global__ __launch_bounds__(256) void attention_kernel(AttnArgs a) {
   }
 
   u32x4 rk[NLOAD], rv[NLOAD];
+  typedef const __attribute__((address_space(1))) u32x4* global_row;  // (a select between generic pointers would be flat loads)
+  const uint64_t zero = (uint64_t)(uintptr_t)g_zero_row, k_at = (uint64_t)(uintptr_t)(a.k + h * a.head_stride), v_less_k = (uint64_t)(uintptr_t)a.v - (uint64_t)(uintptr_t)a.k;
   auto ask_tile = [&](int k0) {
 #pragma unroll
     for (int i = 0; i < NLOAD; i++) {
       const int row = load_row(i);
       const uint32_t key = (uint32_t)(k0 + row);
-      const uint32_t in = key - (uint32_t)(((uint64_t)key * a.page_mul) >> a.page_shift) * a.page;
+      const uint32_t in = key - page_of(key) * a.page;
       const bool good = (int)key < k_end && (uint32_t)ids[i] < a.pages;
-      const int64_t at = (int64_t)ids[i] * a.page_stride + in * a.slot_stride + head_at + (piece ^ P::swz(row)) * 8;
-      rk[i] = *(good ? reinterpret_cast<const u32x4*>(a.k + at) : g_zero_row);
-      rv[i] = *(good ? reinterpret_cast<const u32x4*>(a.v + at) : g_zero_row);
+      const uint64_t at = (uint64_t)(uint32_t)ids[i] * a.page_bytes + ((uint64_t)in * a.slot_bytes + (k_at + (piece ^ P::swz(row)) * 16));
+      rk[i] = *reinterpret_cast<global_row>(good ? at : zero);
+      rv[i] = *reinterpret_cast<global_row>(good ? at + v_less_k : zero);
     }
   };
 
@@ -240,24 +219,15 @@ __global__ __launch_bounds__(256) void attention_kernel(AttnArgs a) {
     ask_tile(k_begin);
     ask_pages(k_begin + KT);
   }
-  for (int k0 = k_begin; k0 < k_end; k0 += KT) {
-    __syncthreads();  // the tile before this one has been read
-#pragma unroll
-    for (int i = 0; i < NLOAD; i++) {
-      const int at = load_row(i) * D + piece * 8;
-      *reinterpret_cast<u32x4*>(s_k + at) = rk[i];
-      *reinterpret_cast<u32x4*>(s_v + at) = rv[i];
-    }
-    __syncthreads();
-    if (k0 + KT < k_end) {
-      ask_tile(k0 + KT);
-      ask_pages(k0 + 2 * KT);
-    }
-#pragma unroll
+  bool odd = false;  // infinities or NaNs among the values of this wave's new tokens
+  // the products of a tile; `border`: new tokens, or keys behind the last
+  auto work = [&](int k0, auto border_) {
+    constexpr bool border = decltype(border_)::value;
+#pragma unroll 1
     for (int u = 0; u < P::SUB; u++) {
       const int base = (u * WK + wk) * 32;  // the step's first row in the tile
       const int key0 = k0 + base;
-      if (key0 >= k_end) break;
+      if (border && key0 >= k_end) break;
       at_f32x4 sa[NQ], sb[NQ];
 #pragma unroll
       for (int i = 0; i < NQ; i++) sa[i] = sb[i] = at_f32x4{0.f, 0.f, 0.f, 0.f};
@@ -275,16 +245,14 @@ __global__ __launch_bounds__(256) void attention_kernel(AttnArgs a) {
           }
         }
       }
-      const bool border = key0 + 32 > s.prefix;  // new tokens, or keys behind the last
       at_bf16x8 fp[P::PPARTS][NQ];
-      uint32_t see[NQ];
 #pragma unroll
       for (int i = 0; i < NQ; i++) {
         float y[8] = {sa[i][0], sa[i][1], sa[i][2], sa[i][3], sb[i][0], sb[i][1], sb[i][2], sb[i][3]};
         if (border) {
-          see[i] = seen_keys(a, s, key0 + 8 * g, token[i]);
+          const uint32_t see = seen_keys(a, s, key0 + 8 * g, token[i]);
 #pragma unroll
-          for (int j = 0; j < 8; j++) y[j] = see[i] >> j & 1 ? y[j] : -INFINITY;
+          for (int j = 0; j < 8; j++) y[j] = see >> j & 1 ? y[j] : -INFINITY;
         }
         float top = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
         top = max32(max16(top)) * a.c;
@@ -316,7 +284,6 @@ __global__ __launch_bounds__(256) void attention_kernel(AttnArgs a) {
       }
       // V^T: lane i of 16 asks for elements 4 (i % 4) .. + 3 of key 8 g + i / 4 and gets element i of keys 8 g .. + 3
       const int rv0 = base + 8 * g + (col >> 2), xv = P::swz(rv0);
-      bool odd = false;
 #pragma unroll
       for (int d = 0; d < DT; d++) {
         const int at = rv0 * D + ((2 * d + ((col & 3) >> 1)) ^ xv) * 8 + (col & 1) * 4;
@@ -324,9 +291,11 @@ __global__ __launch_bounds__(256) void attention_kernel(AttnArgs a) {
         const at_s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(s_v + at));
         const at_s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(s_v + at + 4 * D));
         u32x4 vt = __builtin_bit_cast(u32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-        if (border) {  // a value that a row does not see must not reach it, and 0 * NaN would: such values are taken out here
-          odd |= odd_pair(vt.x) || odd_pair(vt.y) || odd_pair(vt.z) || odd_pair(vt.w);
-          vt = u32x4{finite_pair(vt.x), finite_pair(vt.y), finite_pair(vt.z), finite_pair(vt.w)};
+        if (border) {  // a value that a row does not see must not reach it, and 0 * NaN would: such values are taken out here and added below
+          if (__ballot(odd_pair(vt.x) || odd_pair(vt.y) || odd_pair(vt.z) || odd_pair(vt.w))) {
+            vt = u32x4{finite_pair(vt.x), finite_pair(vt.y), finite_pair(vt.z), finite_pair(vt.w)};
+            odd = true;
+          }
         }
         const at_bf16x8 fv = frag(vt);
 #pragma unroll
@@ -335,7 +304,47 @@ __global__ __launch_bounds__(256) void attention_kernel(AttnArgs a) {
           for (int p = P::PPARTS - 1; p >= 0; p--) acc[i][d] = mma(fv, fp[p][i], acc[i][d]);
         }
       }
-      if (border && __ballot(odd)) odd_values<D, NQ>(s_v, base, see, fp[0], acc);
+    }
+  };
+  // tiles from k0 on: of prefix keys alone, then (a loop of its own: its masks would take registers from the other) the rest
+  int k0 = k_begin;
+  auto tiles = [&](int end, auto border_) {
+   for (; k0 < end; k0 += KT) {
+    __syncthreads();  // the tile before this one has been read
+#pragma unroll
+    for (int i = 0; i < NLOAD; i++) {
+      const int at = load_row(i) * D + piece * 8;
+      *reinterpret_cast<u32x4*>(s_k + at) = rk[i];
+      *reinterpret_cast<u32x4*>(s_v + at) = rv[i];
+    }
+    __syncthreads();
+    if (k0 + KT < k_end) {
+      ask_tile(k0 + KT);
+      ask_pages(k0 + 2 * KT);
+    }
+    work(k0, border_);
+   }
+  };
+  tiles(min(s.prefix, k_end) - KT + 1, std::false_type());
+  tiles(k_end, std::true_type());
+  if (odd) {  // they reach the rows that see them whatever the weight (of 0 or more): no product is needed
+#pragma unroll 1
+    for (int key = max(s.prefix, k_begin); key < k_end; key++) {
+      const uint32_t page = page_of((uint32_t)key);
+      const uint32_t id = (uint32_t)table[min((int)page, a.table_len - 1)];
+      if ((key - k_begin) / 32 % WK != wk || id >= a.pages) continue;
+      const uint64_t at = (uint64_t)id * a.page_bytes + ((uint64_t)((uint32_t)key - page * a.page) * a.slot_bytes + (k_at + v_less_k + g * 8));
+#pragma unroll
+      for (int i = 0; i < NQ; i++) {
+        const bool seen = seen_keys(a, s, key, token[i]) & 1;
+#pragma unroll
+        for (int d = 0; d < DT; d++) {
+          const u32x2 v = *reinterpret_cast<const __attribute__((address_space(1))) u32x2*>(at + 32 * d);
+          const uint32_t w[4] = {v.x << 16, v.x & 0xffff0000u, v.y << 16, v.y & 0xffff0000u};
+#pragma unroll
+          for (int e = 0; e < 4; e++) acc[i][d][e] += seen && (w[e] & 0x7f800000u) == 0x7f800000u ? __uint_as_float(w[e]) : 0.f;
+        }
+      }
     }
   }
 #pragma unroll
@@ -492,7 +501,8 @@ MLLM_API int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_
   if (!q || !cache || table_len < 0 || tree_words < 0 || !(scale > 0.f) || scale > 3e38f || cache->pages < 1 || cache->page_size < 1) return MLLM_HIP_E_BADARG;
   if (!attention_sizes(dtype, T, B, q->heads, cache->heads, cache->head_dim, max_tokens, max_keys)) return MLLM_HIP_E_BADARG;
   if (!attention_shape(T, B, q->heads, cache->heads, cache->head_dim, max_tokens, max_keys) || cache->pages > 0x7fffffff / cache->page_size ||
-      table_len > 0x7fff0000 / cache->page_size || tree_words > 0x1ffffff)
+      table_len > 0x7fff0000 / cache->page_size || tree_words > 0x1ffffff || cache->page_stride < 0 || cache->slot_stride < 0 || cache->page_stride > 0x7fffffff ||
+      cache->slot_stride > 0x7fffffff)
     return MLLM_HIP_E_SHAPE;
   if (T == 0 || B == 0 || max_tokens == 0) return 0;
   if (!q->x || !q->y || !cache->k || !cache->v || !block_table || !cu_tokens || !prefix || table_len < 1) return MLLM_HIP_E_BADARG;
@@ -519,8 +529,8 @@ MLLM_API int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_
   a.o_head = q->y_head_stride;
   a.k = reinterpret_cast<const uint16_t*>(cache->k);
   a.v = reinterpret_cast<const uint16_t*>(cache->v);
-  a.page_stride = cache->page_stride;
-  a.slot_stride = cache->slot_stride;
+  a.page_bytes = (uint32_t)(cache->page_stride * 2);
+  a.slot_bytes = (uint32_t)(cache->slot_stride * 2);
   a.head_stride = cache->head_stride;
   a.pages = (uint32_t)cache->pages;
   a.page = (uint32_t)cache->page_size;
@@ -528,7 +538,7 @@ MLLM_API int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_
   int s = 0;
   while ((1ll << s) < cache->page_size) s++;
   a.page_mul = (uint32_t)(((1ull << (31 + s)) + cache->page_size - 1) / cache->page_size);
-  a.page_shift = 31 + s;
+  a.page_shift = s;
   a.table = block_table;
   a.table_stride = table_stride;
   a.table_len = (int)table_len;
