@@ -18,8 +18,8 @@
 //
 // A workgroup has four waves, WR along rows times 4 / WR along keys, and goes through a range of keys in tiles: 16-byte loads into registers while
 // the tile before them is worked on, from there into LDS.  Rows of a tile lie there with their 16-byte pieces exclusive-ored by bits of the
-// key's number, so that the 16 lanes of an operand read different banks.  Where rows and heads leave CUs idle the keys are cut into ranges
-// (splits), whose O, maximum and sum meet in the workspace; a second launch joins them.
+// key's number, so that the 16 lanes of an operand read different banks.  Where rows and heads leave CUs idle the keys are cut into ranges,
+// whose O, maximum and sum meet in the workspace; a second launch joins them.
 #include <type_traits>
 
 #include "item8.h"
@@ -47,9 +47,11 @@ struct AttnArgs {
   const uint64_t* tree;
   int64_t tree_stride;
   int words;
-  int T, B, kv, group, max_rows, row_tiles, splits, chunk;
+  int T, B, kv, group, max_tokens, row_tiles;
+  int ranges, min_tiles;  // ranges that all keys are cut into (0: a sequence is never cut), tiles of a range at least
   float c;  // scale * log2 e
-  float *part_o, *part_ml;  // [split][token][query head][head_dim], [split][token][query head][2]
+  float *part_o, *part_ml;  // of a sequence that is cut, [piece][its token][query head][head_dim] and [2]
+  int* info;                // [B][2]: first piece and number of pieces of a sequence
 };
 __device__ u32x4 g_zero_row[1];  // what a page outside the cache reads as (never written)
 
@@ -65,6 +67,55 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& a, int b) {
   s.prefix = max(a.prefix[b], 0);
   s.keys = (int)min((int64_t)s.prefix + s.n, (int64_t)a.table_len * a.page);
   return s;
+}
+
+// Where the keys are cut.  The tiles of all sequences, one sequence behind the other, are cut into ranges of equal length, one per workgroup (for
+// every key head and tile of rows), so that workgroups have as much to do whatever the sequences' lengths are.  A range can end one sequence
+// and begin another: its part of sequence b is piece range + b.  Every wave works out where its range begins, a sequence per lane.
+struct Place {
+  Seq s;
+  int b, start, per, total;  // its number, its first tile, the tiles of a range and of all sequences
+};
+template <int KT>
+__device__ __forceinline__ int tiles_of(const Seq& s) { return s.n > 0 ? (s.keys + KT - 1) / KT : 0; }
+template <int KT>
+__device__ __forceinline__ Place find_place(const AttnArgs& a, int range) {
+  Place p = {{0, 0, 0, 0}, 0, 0, 0, 0};
+  if (a.B == 1) {
+    p.s = sequence(a, 0);
+    p.total = tiles_of<KT>(p.s);
+    p.per = max(a.min_tiles, (p.total + a.ranges - 1) / a.ranges);
+    return p;
+  }
+  const int lane = threadIdx.x & 63;
+  Seq mine = sequence(a, min(lane, a.B - 1));
+  int total = lane < a.B ? tiles_of<KT>(mine) : 0;
+  for (int b = lane + 64; b < a.B; b += 64) total += tiles_of<KT>(sequence(a, b));
+#pragma unroll
+  for (int d = 32; d; d >>= 1) total += __shfl_xor(total, d);
+  p.total = __builtin_amdgcn_readfirstlane(total);
+  p.per = max(a.min_tiles, (p.total + a.ranges - 1) / a.ranges);
+  for (int b0 = 0; b0 < a.B; b0 += 64) {
+    if (b0) mine = sequence(a, min(b0 + lane, a.B - 1));
+    const int tiles = b0 + lane < a.B ? tiles_of<KT>(mine) : 0;
+    int up = tiles;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) {
+      const int o = __shfl_up(up, d);
+      up += lane >= d ? o : 0;
+    }
+    const uint64_t found = __ballot(p.start + up > range * p.per);
+    if (found) {
+      const int at = __builtin_ctzll(found);
+      p.b = b0 + at;
+      p.s = Seq{__builtin_amdgcn_readlane(mine.first, at), __builtin_amdgcn_readlane(mine.n, at), __builtin_amdgcn_readlane(mine.prefix, at),
+                __builtin_amdgcn_readlane(mine.keys, at)};
+      p.start += __builtin_amdgcn_readlane(up - tiles, at);
+      return p;
+    }
+    p.start += __builtin_amdgcn_readlane(up, 63);
+  }
+  return p;
 }
 
 // 8 bf16 of a register quad as an operand
@@ -110,19 +161,17 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t v) {
   return ((v & 0x7f80u) == 0x7f80u ? 0u : v & 0xffffu) | ((v & 0x7f800000u) == 0x7f800000u ? 0u : v & 0xffff0000u);
 }
 
+// The part of sequence b with keys k_begin .. k_end - 1, for key head h and row tile rt; `range` and `count` say where partial results go
 template <int D, int NQ, int WR, bool F32>
-__global__ __launch_bounds__(256, (Attn<D, NQ, WR, F32>::WAVES)) void attention_kernel(AttnArgs a) {
+__device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s, int b, int h, int rt, int k_begin, int k_end, int range, int count) {
   typedef Attn<D, NQ, WR, F32> P;
   constexpr int KT = P::KT, C = P::C, WK = P::WK, NLOAD = P::NLOAD, KS = D / 32, DT = D / 16;
   __shared__ __align__(16) uint16_t s_k[KT * D];
   __shared__ __align__(16) uint16_t s_v[KT * D];
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wr = wave % WR, wk = wave / WR;
   const int col = lane & 15, g = lane >> 4;
-
-  // workgroup b runs on XCD b % 8: the row tiles of a range of keys follow one another on one XCD, whose L2 they share
-  const int idx = blockIdx.x >> 3, rt = idx % a.row_tiles, place = (idx / a.row_tiles) * 8 + (blockIdx.x & 7);
-  const int h = place % a.kv, split = place / a.kv % a.splits, b = place / a.kv / a.splits;
-  if (b >= a.B) return;
+  const int rows = s.n * a.group, row0 = rt * P::ROWS * WR;
+  if (row0 >= rows) return;
   // A lane's pieces of a tile: piece lane % C, as it lies in LDS, of rows load_row(i)
   const int piece = lane % C;
   auto load_row = [&](int i) { return wave * (KT / 4) + i * P::RPI + lane / C; };
@@ -136,13 +185,7 @@ __global__ __launch_bounds__(256, (Attn<D, NQ, WR, F32>::WAVES)) void attention_
       ids[i] = table[min((int)page_of(key), a.table_len - 1)];
     }
   };
-  const int k_begin = split * a.chunk;
-  ask_pages(k_begin);  // (in front of the loads that say how many keys there are)
-  const Seq s = sequence(a, b);
-  const int rows = s.n * a.group, row0 = rt * P::ROWS * WR;
-  const int k_end = split + 1 == a.splits ? s.keys : min(k_begin + a.chunk, s.keys);
-  if (row0 >= rows || (split > 0 && k_begin >= k_end)) return;
-
+  ask_pages(k_begin);
   // Q: second operand, row `col` of every 16, elements 32 s + 8 g .. + 7
   at_bf16x8 fq[P::PARTS][NQ][KS];
   int token[NQ];
@@ -352,8 +395,10 @@ __global__ __launch_bounds__(256, (Attn<D, NQ, WR, F32>::WAVES)) void attention_
 
   // The waves along keys meet in LDS, 16 rows at a time: O of a row at [row][D + 4], its maximum and sum behind.
   auto put = [&](int64_t at, int d, at_f32x4 x, float mm, float ll) {
-    if (a.splits > 1) {
-      const int64_t base = ((int64_t)split * a.T * (a.kv * a.group) + at);
+    const int heads = a.kv * a.group;
+    if (count > 1) {
+      const int64_t in = at - (int64_t)s.first * heads, all = (int64_t)a.max_tokens * heads, base = (range + b) * all + in;
+      if (in >= all) return;  // (a token beyond the host's bound)
       *reinterpret_cast<at_f32x4*>(a.part_o + base * D + d) = x;
       if (d == 0) {
         a.part_ml[2 * base] = mm;
@@ -362,7 +407,7 @@ __global__ __launch_bounds__(256, (Attn<D, NQ, WR, F32>::WAVES)) void attention_
     } else {
       const float inv = ll > 0.f ? 1.0f / ll : (ll == 0.f ? 0.f : ll);  // (no key seen: zeros; a NaN stays)
       x *= inv;
-      const int64_t token_ = at / (a.kv * a.group), head = at - token_ * (a.kv * a.group);
+      const int64_t token_ = at / heads, head = at - token_ * heads;
       const int64_t to = token_ * a.o_token + head * a.o_head + d;
       if (F32) *reinterpret_cast<at_f32x4*>(reinterpret_cast<float*>(a.o) + to) = x;
       else *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(a.o) + to) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
@@ -418,61 +463,132 @@ __global__ __launch_bounds__(256, (Attn<D, NQ, WR, F32>::WAVES)) void attention_
   }
 }
 
-// Joins the splits of a row: one lane per four elements
-template <int D, bool F32>
-__global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a) {
-  constexpr int L = D / 4, PER = 256 / L;
-  const int heads = a.kv * a.group;
-  const int b = blockIdx.y;
-  const Seq s = sequence(a, b);
-  const int64_t i = (int64_t)blockIdx.x * PER + threadIdx.x / L;
-  if (i >= (int64_t)s.n * heads || i >= (int64_t)a.max_rows * a.kv) return;
-  const int d = threadIdx.x % L * 4;
-  const int64_t row = (int64_t)s.first * heads + i, step = (int64_t)a.T * heads;
-  const int used = max(1, min(a.splits, (s.keys + a.chunk - 1) / a.chunk));
-  float top = -INFINITY;
-  for (int k = 0; k < used; k++) top = fmaxf(top, a.part_ml[2 * (k * step + row)]);
-  const float ref = top == -INFINITY ? 0.f : top;
-  at_f32x4 x = {0.f, 0.f, 0.f, 0.f};
-  float sum = 0.f;
-  for (int k = 0; k < used; k++) {
-    const int64_t at = k * step + row;
-    const float f = __builtin_amdgcn_exp2f(a.part_ml[2 * at] - ref);
-    sum += a.part_ml[2 * at + 1] * f;
-    x += *reinterpret_cast<const at_f32x4*>(a.part_o + at * D + d) * f;
+template <int D, int NQ, int WR, bool F32>
+__global__ __launch_bounds__(256, (Attn<D, NQ, WR, F32>::WAVES)) void attention_kernel(AttnArgs a) {
+  constexpr int KT = Attn<D, NQ, WR, F32>::KT;
+  // workgroup i runs on XCD i % 8: the row tiles of a range of keys follow one another on one XCD, whose L2 they share
+  const int idx = blockIdx.x >> 3, rt = idx % a.row_tiles, place = (idx / a.row_tiles) * 8 + (blockIdx.x & 7);
+  const int h = place % a.kv, range = place / a.kv;
+  if (!a.ranges) {
+    if (range >= a.B) return;
+    const Seq s = sequence(a, range);
+    attention_piece<D, NQ, WR, F32>(a, s, range, h, rt, 0, s.keys, 0, 1);
+    return;
   }
+  Place p = find_place<KT>(a, range);
+  const int end = min((range + 1) * p.per, p.total);
+  for (int tile = range * p.per; tile < end;) {
+    const int tiles = tiles_of<KT>(p.s), stop = min(end, p.start + tiles);
+    const int first = p.start / p.per, count = (p.start + tiles - 1) / p.per - first + 1;
+    if (h == 0 && rt == 0 && tile == p.start && threadIdx.x < 2) a.info[2 * p.b + threadIdx.x] = threadIdx.x ? count : first + p.b;
+    attention_piece<D, NQ, WR, F32>(a, p.s, p.b, h, rt, (tile - p.start) * KT, min((stop - p.start) * KT, p.s.keys), range, count);
+    p.start += tiles;
+    tile = stop;
+    if (tile < end) {  // (there is a sequence with that tile)
+      do p.s = sequence(a, ++p.b);
+      while (tiles_of<KT>(p.s) == 0);
+    }
+  }
+}
+
+// Joins the pieces of a row: 16 bytes of it per lane, G groups of lanes along the pieces
+template <int D, bool F32, int G>
+__global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a) {
+  constexpr int L = D / 4, PER = 256 / L / G;
+  static_assert(PER >= 1, "");
+  __shared__ at_f32x4 s_x[G > 1 ? 256 : 1];
+  __shared__ float s_ml[G > 1 ? 256 / L * 2 : 1];
+  const int heads = a.kv * a.group, b = blockIdx.y, tid = threadIdx.x;
+  const int first = a.info[2 * b], count = a.info[2 * b + 1];
+  const Seq s = sequence(a, b);
+  if (s.n == 0 || count < 2) return;
+  const int i = blockIdx.x * PER + tid / L % PER, group = tid / L / PER;
+  const int64_t all = (int64_t)a.max_tokens * heads;
+  const bool live = i < min((int64_t)s.n * heads, all);
+  const int d = tid % L * 4;
+  float m = -INFINITY, sum = 0.f;
+  at_f32x4 x = {0.f, 0.f, 0.f, 0.f};
+  if (live) {
+    const float* ml = a.part_ml + 2 * (first * all + i);
+    const float* o = a.part_o + (first * all + i) * D + d;
+    constexpr int U = G > 1 ? 8 : 4;  // loads in flight
+    for (int k = group; k < count; k += U * G) {
+      float mk[U], lk[U];
+      at_f32x4 xk[U];
+#pragma unroll
+      for (int j = 0; j < U; j++) {
+        const int64_t at = (int64_t)min(k + j * G, count - 1) * all;
+        mk[j] = ml[2 * at];
+        lk[j] = ml[2 * at + 1];
+        xk[j] = *reinterpret_cast<const at_f32x4*>(o + at * D);
+      }
+#pragma unroll
+      for (int j = 0; j < U; j++) {
+        if (k + j * G >= count) break;
+        const float next = fmaxf(m, mk[j]), ref = next == -INFINITY ? 0.f : next;
+        const float f = __builtin_amdgcn_exp2f(m - ref), fk = __builtin_amdgcn_exp2f(mk[j] - ref);
+        x = x * f + xk[j] * fk;
+        sum = sum * f + lk[j] * fk;
+        m = next;
+      }
+    }
+  }
+  if constexpr (G > 1) {
+    s_x[tid] = x;
+    if (d == 0) {
+      s_ml[tid / L * 2] = m;
+      s_ml[tid / L * 2 + 1] = sum;
+    }
+    __syncthreads();
+    if (group) return;
+    const int row = tid / L;
+    float top = -INFINITY;
+    for (int k = 0; k < G; k++) top = fmaxf(top, s_ml[(k * PER + row) * 2]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    x = at_f32x4{0.f, 0.f, 0.f, 0.f};
+    sum = 0.f;
+    for (int k = 0; k < G; k++) {
+      const float f = __builtin_amdgcn_exp2f(s_ml[(k * PER + row) * 2] - ref);
+      x += s_x[tid + k * PER * L] * f;
+      sum += s_ml[(k * PER + row) * 2 + 1] * f;
+    }
+  }
+  if (!live) return;
   x *= sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
-  const int64_t token = row / heads, to = token * a.o_token + (row - token * heads) * a.o_head + d;
+  const int64_t token = i / heads, to = (s.first + token) * a.o_token + (i - token * heads) * a.o_head + d;
   if (F32) *reinterpret_cast<at_f32x4*>(reinterpret_cast<float*>(a.o) + to) = x;
   else *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(a.o) + to) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------
 struct AttnPlan {
-  int nq, wr, row_tiles, splits, chunk;
+  int nq, wr, row_tiles, ranges, min_tiles;
 };
-// Rows of a workgroup by the rows there are (tokens times query heads of a key head), then as many ranges of keys as give every CU two workgroups, of at
-// least two tiles each.
+// Rows of a workgroup by the rows there are (tokens times query heads of a key head).  Keys are cut while the workgroups without that are under 1024, into
+// ranges that give every CU two workgroups, of eight times as many keys as rows at least: what a range hands over is rows, what it reads keys.
 static AttnPlan attention_plan(bool f32, int64_t B, int heads, int kv, int64_t max_tokens, int64_t max_keys, int D) {
   AttnPlan p;
   const int64_t rows = max_tokens * (heads / kv);
-  p.wr = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
-  p.nq = rows <= 16 ? 1 : rows <= 128 || f32 ? 2 : 4;
-  if (D == 256 && p.nq > 2) p.nq = 2;
-  if (D == 256 && f32) p.nq = 1;
+  if (D == 256) {
+    p.wr = rows <= (f32 ? 32 : 64) ? 2 : 4;
+    p.nq = f32 || rows <= 32 ? 1 : 2;
+  } else {
+    p.wr = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
+    p.nq = rows <= 16 ? 1 : rows <= 128 || f32 ? 2 : 4;
+  }
   const int64_t per = (int64_t)p.nq * 16 * p.wr;
-  const int64_t tiles = (rows + per - 1) / per;
-  p.row_tiles = (int)(tiles < 0x7fffffff ? tiles : 0x7fffffff);
+  const int64_t row_tiles = (rows + per - 1) / per;
+  p.row_tiles = (int)row_tiles;
   const int kt = p.wr == 1 ? 128 : 64;
-  const int64_t units = B * kv * tiles, most = (max_keys + 2 * kt - 1) / (2 * kt);
-  int64_t splits = units >= 512 ? 1 : 512 / units;
-  if (splits > most) splits = most < 1 ? 1 : most;
-  const int64_t chunk = (max_keys + splits - 1) / splits;
-  p.chunk = (int)((chunk + kt - 1) / kt * kt);
-  if (p.chunk < kt) p.chunk = kt;
-  p.splits = (int)((max_keys + p.chunk - 1) / p.chunk);
-  if (p.splits < 1) p.splits = 1;
+  p.min_tiles = (int)((8 * (rows < per ? rows : per) + kt - 1) / kt);
+  const int64_t most = B * ((max_keys + p.min_tiles * kt - 1) / (p.min_tiles * kt)), wanted = (512 + kv * row_tiles - 1) / (kv * row_tiles);
+  p.ranges = B * kv * row_tiles >= 1024 || max_keys <= (int64_t)p.min_tiles * kt ? 0 : (int)(wanted < most ? wanted : most);
+  if (p.ranges <= 1 && B == 1) p.ranges = 0;
   return p;
+}
+// partial results of every piece, and of every sequence where its pieces are
+static size_t attention_room(const AttnPlan& p, int64_t B, int heads, int64_t max_tokens, int D) {
+  return p.ranges ? ((size_t)(p.ranges + B) * max_tokens * heads * (D + 2) + 2 * B) * sizeof(float) : 0;
 }
 static bool attention_sizes(int dtype, int64_t T, int64_t B, int heads, int kv, int head_dim, int64_t max_tokens, int64_t max_keys) {
   return (dtype == MLLM_HIP_F32 || dtype == MLLM_HIP_BF16) && T >= 0 && B >= 0 && heads >= 1 && kv >= 1 && max_tokens >= 0 && max_keys >= 0;
@@ -491,7 +607,7 @@ MLLM_API size_t mllm_hip_attention_paged_workspace_bytes(int dtype, int64_t T, i
   if (!attention_sizes(dtype, T, B, heads, kv_heads, head_dim, max_tokens, max_keys) || !attention_shape(T, B, heads, kv_heads, head_dim, max_tokens, max_keys)) return 0;
   if (T == 0 || B == 0 || max_tokens == 0) return 0;
   const AttnPlan p = attention_plan(dtype == MLLM_HIP_F32, B, heads, kv_heads, max_tokens, max_keys, head_dim);
-  return p.splits > 1 ? (size_t)p.splits * T * heads * (head_dim + 4) * sizeof(float) : 0;
+  return attention_room(p, B, heads, max_tokens, head_dim);
 }
 
 MLLM_API int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_t T, const mllm_hip_kv_cache* cache, const int32_t* block_table,
@@ -515,10 +631,11 @@ MLLM_API int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_
     return MLLM_HIP_E_ALIGN;
   const bool f32 = dtype == MLLM_HIP_F32;
   const int heads = q->heads, D = cache->head_dim;
-  const AttnPlan p = attention_plan(f32, B, heads, cache->heads, max_tokens, max_keys, D);
-  const size_t need = p.splits > 1 ? (size_t)p.splits * T * heads * (D + 4) * sizeof(float) : 0;
+  AttnPlan p = attention_plan(f32, B, heads, cache->heads, max_tokens, max_keys, D);
+  if (B * (table_len * cache->page_size / 64 + 1) > 0x1fffffff) p.ranges = 0;  // (tiles are counted in 32 bits)
+  const size_t need = attention_room(p, B, heads, max_tokens, D);
   if (need && (!workspace || workspace_bytes < need)) return MLLM_HIP_E_BADARG;
-  const int64_t groups = (B * cache->heads * p.splits + 7) / 8 * 8;
+  const int64_t pieces = p.ranges + B, groups = ((p.ranges ? p.ranges : B) * cache->heads + 7) / 8 * 8;
   if (groups > 0x7fffffff / p.row_tiles) return MLLM_HIP_E_SHAPE;
   AttnArgs a = {};
   a.q = q->x;
@@ -551,47 +668,54 @@ MLLM_API int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_
   a.B = (int)B;
   a.kv = cache->heads;
   a.group = heads / cache->heads;
-  a.max_rows = (int)(max_tokens * a.group);
+  a.max_tokens = (int)max_tokens;
   a.row_tiles = p.row_tiles;
-  a.splits = p.splits;
-  a.chunk = p.chunk;
+  a.ranges = p.ranges;
+  a.min_tiles = p.min_tiles;
   a.c = scale * 1.44269504088896341f;
   a.part_o = reinterpret_cast<float*>(workspace);
-  a.part_ml = a.part_o ? a.part_o + (size_t)p.splits * T * heads * D : nullptr;
+  if (p.ranges) {
+    a.part_ml = a.part_o + (size_t)pieces * max_tokens * heads * D;
+    a.info = reinterpret_cast<int*>(a.part_ml + (size_t)pieces * max_tokens * heads * 2);
+  }
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid((unsigned)(groups * p.row_tiles));
   const int form = p.nq * 10 + p.wr;
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a); };
-#define ATTN(D_, F_)                                                                   \
-  switch (form) {                                                                      \
-    case 11: go(attention_kernel<D_, 1, 1, F_>); break;                                \
-    case 12: go(attention_kernel<D_, 1, 2, F_>); break;                                \
-    case 14: go(attention_kernel<D_, 1, 4, F_>); break;                                \
-    case 21: go(attention_kernel<D_, 2, 1, F_>); break;                                \
-    case 22: go(attention_kernel<D_, 2, 2, F_>); break;                                \
-    case 24: go(attention_kernel<D_, 2, 4, F_>); break;                                \
-    default: go(attention_kernel<D_, F_ || D_ == 256 ? 2 : 4, 4, F_>); break;          \
-  }
+#define ATTN(D_, NQ_, WR_, F_) \
+  case NQ_ * 10 + WR_: go(attention_kernel<D_, NQ_, WR_, F_>); break;
+#define ATTN_D(D_)                                                                             \
+  if (f32) switch (form) { ATTN(D_, 1, 1, true) ATTN(D_, 2, 1, true) ATTN(D_, 2, 2, true) ATTN(D_, 2, 4, true) }  \
+  else switch (form) { ATTN(D_, 1, 1, false) ATTN(D_, 2, 1, false) ATTN(D_, 2, 2, false) ATTN(D_, 2, 4, false) ATTN(D_, 4, 4, false) }
   if (D == 64) {
-    if (f32) { ATTN(64, true) } else { ATTN(64, false) }
+    ATTN_D(64)
   } else if (D == 128) {
-    if (f32) { ATTN(128, true) } else { ATTN(128, false) }
+    ATTN_D(128)
+  } else if (f32) {
+    switch (form) { ATTN(256, 1, 2, true) ATTN(256, 1, 4, true) }
   } else {
-    if (f32) { ATTN(256, true) } else { ATTN(256, false) }
+    switch (form) { ATTN(256, 1, 2, false) ATTN(256, 2, 2, false) ATTN(256, 2, 4, false) }
   }
+#undef ATTN_D
 #undef ATTN
   RC_RET((int)hipGetLastError());
-  if (p.splits > 1) {
-    const int per = 256 / (D / 4);
+  if (p.ranges) {
+    // lanes along the ranges where a sequence has many of them: one row of 17 ranges by lanes that take them in turn was 11 us of dependent loads
+    const bool many = p.ranges >= 8 * B;
+    const int per = many ? 1 : 256 / (D / 4);
     const dim3 jgrid((unsigned)((max_tokens * heads + per - 1) / per), (unsigned)B);
     auto join = [&](auto kern) { hipLaunchKernelGGL(kern, jgrid, dim3(256), 0, st, a); };
+#define JOIN(D_, F_)                                               \
+  if (many) join(attention_join_kernel<D_, F_, 1024 / D_>);        \
+  else join(attention_join_kernel<D_, F_, 1>)
     if (D == 64) {
-      if (f32) join(attention_join_kernel<64, true>); else join(attention_join_kernel<64, false>);
+      if (f32) { JOIN(64, true); } else { JOIN(64, false); }
     } else if (D == 128) {
-      if (f32) join(attention_join_kernel<128, true>); else join(attention_join_kernel<128, false>);
+      if (f32) { JOIN(128, true); } else { JOIN(128, false); }
     } else {
-      if (f32) join(attention_join_kernel<256, true>); else join(attention_join_kernel<256, false>);
+      if (f32) { JOIN(256, true); } else { JOIN(256, false); }
     }
+#undef JOIN
   }
   return (int)hipGetLastError();
 }
