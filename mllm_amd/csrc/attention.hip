@@ -299,7 +299,7 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
         }
         float top = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
         top = max32(max16(top)) * a.c;
-        if (__ballot(top > m[i])) {
+        if (__ballot(top > m[i] + 8.f)) {  // (weights of up to 2^8 do as well: most steps leave O alone)
           const float next = fmaxf(m[i], top), fix = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - next);
           m[i] = next;
           l[i] *= fix;
@@ -565,7 +565,7 @@ struct AttnPlan {
   int nq, wr, row_tiles, ranges, min_tiles;
 };
 // Rows of a workgroup by the rows there are (tokens times query heads of a key head).  Keys are cut while the workgroups without that are under 1024, into
-// ranges that give every CU two workgroups, of eight times as many keys as rows at least: what a range hands over is rows, what it reads keys.
+// ranges that give every CU two workgroups, of twice as many keys as rows at least: what a range hands over is rows, what it reads keys.
 static AttnPlan attention_plan(bool f32, int64_t B, int heads, int kv, int64_t max_tokens, int64_t max_keys, int D) {
   AttnPlan p;
   const int64_t rows = max_tokens * (heads / kv);
@@ -574,13 +574,13 @@ static AttnPlan attention_plan(bool f32, int64_t B, int heads, int kv, int64_t m
     p.nq = f32 || rows <= 32 ? 1 : 2;
   } else {
     p.wr = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
-    p.nq = rows <= 16 ? 1 : rows <= 128 || f32 ? 2 : 4;
+    p.nq = rows <= 16 ? 1 : 2;
   }
   const int64_t per = (int64_t)p.nq * 16 * p.wr;
   const int64_t row_tiles = (rows + per - 1) / per;
   p.row_tiles = (int)row_tiles;
   const int kt = p.wr == 1 ? 128 : 64;
-  p.min_tiles = (int)((8 * (rows < per ? rows : per) + kt - 1) / kt);
+  p.min_tiles = (int)((2 * (rows < per ? rows : per) + kt - 1) / kt);
   const int64_t most = B * ((max_keys + p.min_tiles * kt - 1) / (p.min_tiles * kt)), wanted = (512 + kv * row_tiles - 1) / (kv * row_tiles);
   p.ranges = B * kv * row_tiles >= 1024 || max_keys <= (int64_t)p.min_tiles * kt ? 0 : (int)(wanted < most ? wanted : most);
   if (p.ranges <= 1 && B == 1) p.ranges = 0;
@@ -686,7 +686,7 @@ MLLM_API int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_
   case NQ_ * 10 + WR_: go(attention_kernel<D_, NQ_, WR_, F_>); break;
 #define ATTN_D(D_)                                                                             \
   if (f32) switch (form) { ATTN(D_, 1, 1, true) ATTN(D_, 2, 1, true) ATTN(D_, 2, 2, true) ATTN(D_, 2, 4, true) }  \
-  else switch (form) { ATTN(D_, 1, 1, false) ATTN(D_, 2, 1, false) ATTN(D_, 2, 2, false) ATTN(D_, 2, 4, false) ATTN(D_, 4, 4, false) }
+  else switch (form) { ATTN(D_, 1, 1, false) ATTN(D_, 2, 1, false) ATTN(D_, 2, 2, false) ATTN(D_, 2, 4, false) }
   if (D == 64) {
     ATTN_D(64)
   } else if (D == 128) {
