@@ -616,7 +616,8 @@ int mllm_hip_matmul_split_side(int64_t batch, int64_t M, int64_t N, int64_t K, i
  *
  * The cache: keys and values in bf16, pages of page_size slots, slot s of page p of head h at element
  * p * page_stride + s * slot_stride + h * head_stride (the same for k and v; strides multiples of 8, pointers 16-byte aligned), head_dim
- * elements in a row.  Offsets are 64-bit; pages * page_size < 2^31; strides of pages and slots from 0 to 2^31 - 1.
+ * elements in a row.  Offsets are 64-bit; pages * page_size < 2^31; 0 <= page_stride < 2^31, 0 < slot_stride (of more than one slot),
+ * page_size * slot_stride < 2^30.
  * ------------------------------------------------------------------------------------------------------- */
 typedef struct mllm_hip_kv_cache {
   void* k;

@@ -37,8 +37,9 @@ struct AttnArgs {
   int64_t q_token, q_head, o_token, o_head;
   const uint16_t *k, *v;
   int64_t head_stride;
-  uint32_t page_bytes, slot_bytes;
-  uint32_t pages, page, page_mul;  // key / page = (2 key * page_mul) >> 32 >> page_shift for key < 2^31
+  uint32_t page_bytes, slot_bytes, page_end;  // page_end: bytes of a page's slots
+  uint32_t step_pages, step_bytes;            // a tile's keys in whole pages and the bytes of the slots over
+  uint32_t pages, page, page_mul;             // key / page = (2 key * page_mul) >> 32 >> page_shift for key < 2^31
   int page_shift;
   const int32_t* table;
   int64_t table_stride;
@@ -53,7 +54,7 @@ struct AttnArgs {
   float *part_o, *part_ml;  // of a sequence that is cut, [piece][its token][query head][head_dim] and [2]
   int* info;                // [B][2]: first piece and number of pieces of a sequence
 };
-__device__ u32x4 g_zero_row[1];  // what a page outside the cache reads as (never written)
+__device__ u32x4 g_zero_row[32];  // what a page outside the cache reads as (never written)
 
 // sequence b: its first row of q, its number of new tokens, of prefix keys and of keys
 struct Seq {
@@ -118,6 +119,12 @@ __device__ __forceinline__ Place find_place(const AttnArgs& a, int range) {
   return p;
 }
 
+__device__ __forceinline__ float larger(float x, float y) { return __builtin_elementwise_maximum(x, y); }
+template <int N>  // the larger of a lane's and that of the lane N away
+__device__ __forceinline__ float across(float v) {
+  const u32x2 r = N == 16 ? lanes16(__float_as_uint(v)) : lanes32(__float_as_uint(v));
+  return larger(__uint_as_float(r.x), __uint_as_float(r.y));
+}
 // 8 bf16 of a register quad as an operand
 __device__ __forceinline__ at_bf16x8 frag(u32x4 v) { return __builtin_bit_cast(at_bf16x8, v); }
 __device__ __forceinline__ at_f32x4 mma(at_bf16x8 x, at_bf16x8 y, at_f32x4 acc) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, acc, 0, 0, 0); }
@@ -128,11 +135,10 @@ struct Attn {
   static constexpr int KT = WK * 32 < 64 ? 64 : WK * 32;  // keys of a tile
   static constexpr int SUB = KT / (WK * 32);             // 32-key steps of a wave per tile
   static constexpr int C = D / 8;                        // 16-byte pieces of a row
-  static constexpr int RPI = 64 / C;                     // rows a wave loads per instruction
-  static constexpr int NLOAD = KT / 4 / RPI;             // loads of keys (and of values) of a lane per tile
+  static constexpr int NLOAD = KT / 4 / 8;               // rows of a tile that a lane loads from
   static constexpr int PARTS = F32 ? 3 : 1, PPARTS = F32 ? 2 : 1;
   static constexpr int ROWS = NQ * 16;                   // rows of a wave
-  static constexpr int WAVES = D * NQ <= (F32 ? 128 : 256) ? 2 : 1;  // per SIMD: 256 registers each, or all 512 for one
+  static constexpr int WAVES = D == 256 ? 1 : 2;         // per SIMD: all 512 registers for one, or 256 each
   static __device__ __forceinline__ int swz(int row) { return (C == 8) ? (row & 3) | ((row >> 3) & 1) << 2 : (row & 3) | ((row >> 3) & 3) << 2; }
 };
 
@@ -172,31 +178,39 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
   const int col = lane & 15, g = lane >> 4;
   const int rows = s.n * a.group, row0 = rt * P::ROWS * WR;
   if (row0 >= rows) return;
-  // A lane's pieces of a tile: piece lane % C, as it lies in LDS, of rows load_row(i)
-  const int piece = lane % C;
-  auto load_row = [&](int i) { return wave * (KT / 4) + i * P::RPI + lane / C; };
+  // A lane loads 16-byte pieces p, p + 8, .. (p = lane % 8) of row lane / 8 of every eight rows.  Where a row's key is in the cache goes on from tile to
+  // tile without a division: `page` numbers into the table, `in` bytes into the page.
   const int32_t* table = a.table + b * a.table_stride;
-  auto page_of = [&](uint32_t key) { return __umulhi(2 * key, a.page_mul) >> a.page_shift; };
+  uint32_t page[NLOAD], in[NLOAD];
   int ids[NLOAD];
-  auto ask_pages = [&](int k0) {  // the pages of a tile's keys (the last page of the table for what lies behind it: never used)
+  auto load_row = [&](int i) { return wave * (KT / 4) + i * 8 + lane / 8; };
+#pragma unroll
+  for (int i = 0; i < NLOAD; i++) {
+    const uint32_t key = (uint32_t)(k_begin + load_row(i));
+    page[i] = __umulhi(2 * key, a.page_mul) >> a.page_shift;
+    in[i] = (key - page[i] * a.page) * a.slot_bytes;
+    ids[i] = table[min((int)page[i], a.table_len - 1)];
+  }
+  auto next_pages = [&]() {
 #pragma unroll
     for (int i = 0; i < NLOAD; i++) {
-      const uint32_t key = (uint32_t)(k0 + load_row(i));
-      ids[i] = table[min((int)page_of(key), a.table_len - 1)];
+      in[i] += a.step_bytes;
+      page[i] += a.step_pages;
+      const bool over = in[i] >= a.page_end;
+      in[i] -= over ? a.page_end : 0;
+      page[i] += over;
+      ids[i] = table[min((int)page[i], a.table_len - 1)];  // (behind the table: any page, never used)
     }
   };
-  ask_pages(k_begin);
   // Q: second operand, row `col` of every 16, elements 32 s + 8 g .. + 7
   at_bf16x8 fq[P::PARTS][NQ][KS];
   int token[NQ];
-  int64_t o_at[NQ];
 #pragma unroll
   for (int i = 0; i < NQ; i++) {
     const int r = row0 + wr * P::ROWS + i * 16 + col;
     const bool live = r < rows;
     token[i] = live ? r / a.group : 0;
     const int head = h * a.group + (live ? r - token[i] * a.group : 0);
-    o_at[i] = live ? (int64_t)(s.first + token[i]) * (a.kv * a.group) + head : -1;
     const int64_t at = (s.first + token[i]) * a.q_token + head * a.q_head + 8 * g;
 #pragma unroll
     for (int ks = 0; ks < KS; ks++) {
@@ -232,20 +246,23 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
     }
   }
 
-  u32x4 rk[NLOAD], rv[NLOAD];
+  u32x4 rk[NLOAD][C / 8], rv[NLOAD][C / 8];
   typedef const __attribute__((address_space(1))) u32x4* global_row;  // (a select between generic pointers would be flat loads)
-  const uint64_t zero = (uint64_t)(uintptr_t)g_zero_row, k_at = (uint64_t)(uintptr_t)(a.k + h * a.head_stride), v_less_k = (uint64_t)(uintptr_t)a.v - (uint64_t)(uintptr_t)a.k;
+  const uint64_t zero = (uint64_t)(uintptr_t)g_zero_row, k_at = (uint64_t)(uintptr_t)(a.k + h * a.head_stride) + lane % 8 * 16,
+                 v_less_k = (uint64_t)(uintptr_t)a.v - (uint64_t)(uintptr_t)a.k;
   auto ask_tile = [&](int k0) {
 #pragma unroll
     for (int i = 0; i < NLOAD; i++) {
-      const int row = load_row(i);
-      const uint32_t key = (uint32_t)(k0 + row);
-      const uint32_t in = key - page_of(key) * a.page;
-      const bool good = (int)key < k_end && (uint32_t)ids[i] < a.pages;
-      const uint64_t at = (uint64_t)(uint32_t)ids[i] * a.page_bytes + ((uint64_t)in * a.slot_bytes + (k_at + (piece ^ P::swz(row)) * 16));
-      rk[i] = *reinterpret_cast<global_row>(good ? at : zero);
-      rv[i] = *reinterpret_cast<global_row>(good ? at + v_less_k : zero);
+      const bool good = k0 + load_row(i) < k_end && (uint32_t)ids[i] < a.pages;
+      const uint64_t at = (uint64_t)(uint32_t)ids[i] * a.page_bytes + (k_at + in[i]);
+      const global_row kp = reinterpret_cast<global_row>(good ? at : zero), vp = reinterpret_cast<global_row>(good ? at + v_less_k : zero);
+#pragma unroll
+      for (int j = 0; j < C / 8; j++) {
+        rk[i][j] = kp[8 * j];
+        rv[i][j] = vp[8 * j];
+      }
     }
+    next_pages();
   };
 
   at_f32x4 acc[NQ][DT];
@@ -260,7 +277,6 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
 
   if (k_begin < k_end) {
     ask_tile(k_begin);
-    ask_pages(k_begin + KT);
   }
   bool odd = false;  // infinities or NaNs among the values of this wave's new tokens
   // the products of a tile; `border`: new tokens, or keys behind the last
@@ -297,8 +313,10 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
 #pragma unroll
           for (int j = 0; j < 8; j++) y[j] = see >> j & 1 ? y[j] : -INFINITY;
         }
-        float top = fmaxf(fmaxf(fmaxf(y[0], y[1]), fmaxf(y[2], y[3])), fmaxf(fmaxf(y[4], y[5]), fmaxf(y[6], y[7])));
-        top = max32(max16(top)) * a.c;
+        // (maximum, which hands a NaN on, is one instruction for three; fmaxf quiets each of its operands first)
+        float top = larger(larger(larger(y[0], y[1]), larger(y[2], y[3])), larger(larger(y[4], y[5]), larger(y[6], y[7])));
+        top = across<16>(top);
+        top = across<32>(top) * a.c;
         if (__ballot(top > m[i] + 8.f)) {  // (weights of up to 2^8 do as well: most steps leave O alone)
           const float next = fmaxf(m[i], top), fix = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - next);
           m[i] = next;
@@ -356,14 +374,17 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
     __syncthreads();  // the tile before this one has been read
 #pragma unroll
     for (int i = 0; i < NLOAD; i++) {
-      const int at = load_row(i) * D + piece * 8;
-      *reinterpret_cast<u32x4*>(s_k + at) = rk[i];
-      *reinterpret_cast<u32x4*>(s_v + at) = rv[i];
+      const int row = load_row(i);
+#pragma unroll
+      for (int j = 0; j < C / 8; j++) {
+        const int at = row * D + ((lane % 8 + 8 * j) ^ P::swz(row)) * 8;
+        *reinterpret_cast<u32x4*>(s_k + at) = rk[i][j];
+        *reinterpret_cast<u32x4*>(s_v + at) = rv[i][j];
+      }
     }
     __syncthreads();
     if (k0 + KT < k_end) {
       ask_tile(k0 + KT);
-      ask_pages(k0 + 2 * KT);
     }
     work(k0, border_);
    }
@@ -373,10 +394,10 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
   if (odd) {  // they reach the rows that see them whatever the weight (of 0 or more): no product is needed
 #pragma unroll 1
     for (int key = max(s.prefix, k_begin); key < k_end; key++) {
-      const uint32_t page = page_of((uint32_t)key);
-      const uint32_t id = (uint32_t)table[min((int)page, a.table_len - 1)];
+      const uint32_t at_page = __umulhi(2 * (uint32_t)key, a.page_mul) >> a.page_shift;
+      const uint32_t id = (uint32_t)table[min((int)at_page, a.table_len - 1)];
       if ((key - k_begin) / 32 % WK != wk || id >= a.pages) continue;
-      const uint64_t at = (uint64_t)id * a.page_bytes + ((uint64_t)((uint32_t)key - page * a.page) * a.slot_bytes + (k_at + v_less_k + g * 8));
+      const uint64_t at = (uint64_t)id * a.page_bytes + (((uint32_t)key - at_page * a.page) * a.slot_bytes + (uint64_t)(uintptr_t)(a.v + h * a.head_stride) + g * 8);
 #pragma unroll
       for (int i = 0; i < NQ; i++) {
         const bool seen = seen_keys(a, s, key, token[i]) & 1;
@@ -393,32 +414,42 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
 #pragma unroll
   for (int i = 0; i < NQ; i++) l[i] = sum32(sum16(l[i]));
 
-  // The waves along keys meet in LDS, 16 rows at a time: O of a row at [row][D + 4], its maximum and sum behind.
-  auto put = [&](int64_t at, int d, at_f32x4 x, float mm, float ll) {
-    const int heads = a.kv * a.group;
-    if (count > 1) {
-      const int64_t in = at - (int64_t)s.first * heads, all = (int64_t)a.max_tokens * heads, base = (range + b) * all + in;
-      if (in >= all) return;  // (a token beyond the host's bound)
-      *reinterpret_cast<at_f32x4*>(a.part_o + base * D + d) = x;
+  // Where a row's results go: 32-bit sizes of a row, 64-bit offsets worked out once per row.
+  const int heads = a.kv * a.group;
+  struct To {
+    void* o;
+    float* ml;
+    bool part;
+  };
+  auto where = [&](int row) {  // of 0 .. rows - 1; o null: a token beyond the host's bound
+    const int t = row / a.group, head = h * a.group + row - t * a.group;
+    if (count == 1) return To{reinterpret_cast<char*>(a.o) + ((s.first + t) * a.o_token + head * a.o_head) * (F32 ? 4 : 2), nullptr, false};
+    const int64_t at = ((int64_t)(range + b) * a.max_tokens + t) * heads + head;
+    return To{t < a.max_tokens ? a.part_o + at * D : nullptr, a.part_ml + 2 * at, true};
+  };
+  auto put = [&](const To& to, int d, at_f32x4 x, float mm, float ll) {
+    if (to.part) {
+      if (!to.o) return;
+      *reinterpret_cast<at_f32x4*>(reinterpret_cast<float*>(to.o) + d) = x;
       if (d == 0) {
-        a.part_ml[2 * base] = mm;
-        a.part_ml[2 * base + 1] = ll;
+        to.ml[0] = mm;
+        to.ml[1] = ll;
       }
     } else {
-      const float inv = ll > 0.f ? 1.0f / ll : (ll == 0.f ? 0.f : ll);  // (no key seen: zeros; a NaN stays)
-      x *= inv;
-      const int64_t token_ = at / heads, head = at - token_ * heads;
-      const int64_t to = token_ * a.o_token + head * a.o_head + d;
-      if (F32) *reinterpret_cast<at_f32x4*>(reinterpret_cast<float*>(a.o) + to) = x;
-      else *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(a.o) + to) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+      x *= ll > 0.f ? 1.0f / ll : (ll == 0.f ? 0.f : ll);  // (no key seen: zeros; a NaN stays)
+      if (F32) *reinterpret_cast<at_f32x4*>(reinterpret_cast<float*>(to.o) + d) = x;
+      else *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(to.o) + d) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
     }
   };
+  // The waves along keys meet in LDS, 16 rows at a time: O of a row at [row][HALF], its maximum and sum apart.
   if constexpr (WK == 1) {
 #pragma unroll
     for (int i = 0; i < NQ; i++) {
-      if (o_at[i] < 0) continue;
+      const int row = row0 + wr * P::ROWS + i * 16 + col;
+      if (row >= rows) continue;
+      const To to = where(row);
 #pragma unroll
-      for (int d = 0; d < DT; d++) put(o_at[i], 16 * d + 4 * g, acc[i][d], m[i], l[i]);
+      for (int d = 0; d < DT; d++) put(to, 16 * d + 4 * g, acc[i][d], m[i], l[i]);
     }
   } else {
     constexpr int HALF = D / 2;  // (half of O at a time: four waves' rows of 256 elements would not fit)
@@ -455,8 +486,7 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
             sum += sm[at * 2 + 1] * f;
             x += *reinterpret_cast<const at_f32x4*>(so + at * HALF + (p ^ (r & 7)) * 4) * f;
           }
-          const int t = row / a.group;
-          put((int64_t)(s.first + t) * (a.kv * a.group) + h * a.group + (row - t * a.group), part * HALF + p * 4, x, top, sum);
+          put(where(row), part * HALF + p * 4, x, top, sum);
         }
       }
     }
@@ -469,18 +499,25 @@ __global__ __launch_bounds__(256, (Attn<D, NQ, WR, F32>::WAVES)) void attention_
   // workgroup i runs on XCD i % 8: the row tiles of a range of keys follow one another on one XCD, whose L2 they share
   const int idx = blockIdx.x >> 3, rt = idx % a.row_tiles, place = (idx / a.row_tiles) * 8 + (blockIdx.x & 7);
   const int h = place % a.kv, range = place / a.kv;
-  if (!a.ranges) {
+  Place p = {{0, 0, 0, 0}, range, 0, 0, 0};
+  int tile = 0, end;
+  if (a.ranges) {
+    p = find_place<KT>(a, range);
+    tile = range * p.per;
+    end = min(tile + p.per, p.total);
+  } else {  // a sequence is a range
     if (range >= a.B) return;
-    const Seq s = sequence(a, range);
-    attention_piece<D, NQ, WR, F32>(a, s, range, h, rt, 0, s.keys, 0, 1);
-    return;
+    p.s = sequence(a, range);
+    end = p.total = tiles_of<KT>(p.s);
   }
-  Place p = find_place<KT>(a, range);
-  const int end = min((range + 1) * p.per, p.total);
-  for (int tile = range * p.per; tile < end;) {
+  while (tile < end) {
     const int tiles = tiles_of<KT>(p.s), stop = min(end, p.start + tiles);
-    const int first = p.start / p.per, count = (p.start + tiles - 1) / p.per - first + 1;
-    if (h == 0 && rt == 0 && tile == p.start && threadIdx.x < 2) a.info[2 * p.b + threadIdx.x] = threadIdx.x ? count : first + p.b;
+    int count = 1;
+    if (a.ranges) {
+      const int first = p.start / p.per;
+      count = (p.start + tiles - 1) / p.per - first + 1;
+      if (h == 0 && rt == 0 && tile == p.start && threadIdx.x < 2) a.info[2 * p.b + threadIdx.x] = threadIdx.x ? count : first + p.b;
+    }
     attention_piece<D, NQ, WR, F32>(a, p.s, p.b, h, rt, (tile - p.start) * KT, min((stop - p.start) * KT, p.s.keys), range, count);
     p.start += tiles;
     tile = stop;
@@ -569,13 +606,8 @@ struct AttnPlan {
 static AttnPlan attention_plan(bool f32, int64_t B, int heads, int kv, int64_t max_tokens, int64_t max_keys, int D) {
   AttnPlan p;
   const int64_t rows = max_tokens * (heads / kv);
-  if (D == 256) {
-    p.wr = rows <= (f32 ? 32 : 64) ? 2 : 4;
-    p.nq = f32 || rows <= 32 ? 1 : 2;
-  } else {
-    p.wr = rows <= 32 ? 1 : rows <= 64 ? 2 : 4;
-    p.nq = rows <= 16 ? 1 : 2;
-  }
+  p.nq = rows <= 32 || f32 || D == 256 ? 1 : 2;
+  p.wr = rows <= 16 && D < 256 ? 1 : rows <= 32 || (rows <= 64 && p.nq == 2) ? 2 : 4;
   const int64_t per = (int64_t)p.nq * 16 * p.wr;
   const int64_t row_tiles = (rows + per - 1) / per;
   p.row_tiles = (int)row_tiles;
@@ -618,7 +650,8 @@ MLLM_API int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_
   if (!attention_sizes(dtype, T, B, q->heads, cache->heads, cache->head_dim, max_tokens, max_keys)) return MLLM_HIP_E_BADARG;
   if (!attention_shape(T, B, q->heads, cache->heads, cache->head_dim, max_tokens, max_keys) || cache->pages > 0x7fffffff / cache->page_size ||
       table_len > 0x7fff0000 / cache->page_size || tree_words > 0x1ffffff || cache->page_stride < 0 || cache->slot_stride < 0 || cache->page_stride > 0x7fffffff ||
-      cache->slot_stride > 0x7fffffff)
+      cache->slot_stride > 0x3fffffff / cache->page_size ||
+      (cache->slot_stride == 0 && cache->page_size > 1))
     return MLLM_HIP_E_SHAPE;
   if (T == 0 || B == 0 || max_tokens == 0) return 0;
   if (!q->x || !q->y || !cache->k || !cache->v || !block_table || !cu_tokens || !prefix || table_len < 1) return MLLM_HIP_E_BADARG;
@@ -648,6 +681,10 @@ MLLM_API int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_
   a.v = reinterpret_cast<const uint16_t*>(cache->v);
   a.page_bytes = (uint32_t)(cache->page_stride * 2);
   a.slot_bytes = (uint32_t)(cache->slot_stride * 2);
+  a.page_end = cache->page_size == 1 ? 1 : (uint32_t)(cache->page_size * cache->slot_stride * 2);  // (a page of one slot: `in` stays 0)
+  const int kt = p.wr == 1 ? 128 : 64;
+  a.step_pages = (uint32_t)(kt / cache->page_size);
+  a.step_bytes = (uint32_t)(kt % cache->page_size * cache->slot_stride * 2);
   a.head_stride = cache->head_stride;
   a.pages = (uint32_t)cache->pages;
   a.page = (uint32_t)cache->page_size;
@@ -684,9 +721,9 @@ MLLM_API int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a); };
 #define ATTN(D_, NQ_, WR_, F_) \
   case NQ_ * 10 + WR_: go(attention_kernel<D_, NQ_, WR_, F_>); break;
-#define ATTN_D(D_)                                                                             \
-  if (f32) switch (form) { ATTN(D_, 1, 1, true) ATTN(D_, 2, 1, true) ATTN(D_, 2, 2, true) ATTN(D_, 2, 4, true) }  \
-  else switch (form) { ATTN(D_, 1, 1, false) ATTN(D_, 2, 1, false) ATTN(D_, 2, 2, false) ATTN(D_, 2, 4, false) }
+#define ATTN_D(D_)                                                                                        \
+  if (f32) switch (form) { ATTN(D_, 1, 1, true) ATTN(D_, 1, 2, true) ATTN(D_, 1, 4, true) }                \
+  else switch (form) { ATTN(D_, 1, 1, false) ATTN(D_, 1, 2, false) ATTN(D_, 2, 2, false) ATTN(D_, 2, 4, false) }
   if (D == 64) {
     ATTN_D(64)
   } else if (D == 128) {
@@ -694,7 +731,7 @@ MLLM_API int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_
   } else if (f32) {
     switch (form) { ATTN(256, 1, 2, true) ATTN(256, 1, 4, true) }
   } else {
-    switch (form) { ATTN(256, 1, 2, false) ATTN(256, 2, 2, false) ATTN(256, 2, 4, false) }
+    switch (form) { ATTN(256, 1, 2, false) ATTN(256, 1, 4, false) }
   }
 #undef ATTN_D
 #undef ATTN

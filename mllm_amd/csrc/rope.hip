@@ -210,7 +210,8 @@ MLLM_API int mllm_hip_kv_append(const mllm_hip_heads* q, const mllm_hip_heads* k
   if (!k || !v || !cache || !cache->k || !cache->v || (T && !slots) || cache->heads < 1 || cache->pages < 1 || cache->page_size < 1) return MLLM_HIP_E_BADARG;
   RC_RET(rope_checks(dtype, T, cache->head_dim, positions, inv_freq, rot_dim));
   if (k->heads != cache->heads || v->heads != cache->heads || cache->pages > 0x7fffffff / cache->page_size || cache->page_stride < 0 ||
-      cache->slot_stride < 0 || cache->page_stride > 0x7fffffff || cache->slot_stride > 0x7fffffff)
+      cache->slot_stride < 0 || cache->page_stride > 0x7fffffff || cache->slot_stride > 0x3fffffff / cache->page_size ||
+      (cache->slot_stride == 0 && cache->page_size > 1))
     return MLLM_HIP_E_SHAPE;
   if (!al16(cache->k) || !al16(cache->v) || cache->page_stride % 8 || cache->slot_stride % 8 || cache->head_stride % 8 ||
       reinterpret_cast<uintptr_t>(slots) % 8)
