@@ -673,6 +673,18 @@ int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_t T, cons
                              int64_t max_tokens, int64_t max_keys, const uint64_t* tree, int64_t tree_stride, int64_t tree_words, float scale,
                              void* workspace, size_t workspace_bytes, void* stream);
 
+/* A token from every row of logits [rows][vocab] (F32 or BF16, rows row_stride elements apart) and a uniform number u[row] in [0, 1):
+ *   w_i = exp((x_i - max) / temperature), 0 below 2^-52; in descending order (equal logits: lowest index first) the first top_k are kept (0 or
+ *   less: all), of these the shortest beginning whose mass is top_p of theirs or more (at least one; 1 or more: all), of these the ones with
+ *   w_i >= min_p (1 at most).  The token is the first kept one, in the order of the index, at which the running sum exceeds u times the sum of what is kept.
+ * temperature of 0 or less: the largest logit's lowest index.  A NaN counts as -inf; infinite maxima share the weight; a row without a logit
+ * above -inf gives -1.  Settings are fp32 / int32 [rows] each; NULL: 1, 0, 1, 0.  Sums in fp64, the same result on every call.
+ * vocab <= 2^24, rows <= 65535.  workspace: ..._workspace_bytes, 16-byte aligned; less is MLLM_HIP_E_BADARG.  Up to four launches. */
+size_t mllm_hip_sample_workspace_bytes(int64_t rows, int64_t vocab);
+int mllm_hip_sample(const void* logits, int dtype, int64_t row_stride, int64_t rows, int64_t vocab, const float* u, const float* temperature,
+                    const int32_t* top_k, const float* top_p, const float* min_p, int32_t* tokens, void* workspace, size_t workspace_bytes,
+                    void* stream);
+
 #ifdef __cplusplus
 }
 #endif

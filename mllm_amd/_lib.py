@@ -200,6 +200,9 @@ def lib():
         L.mllm_hip_attention_paged_workspace_bytes.restype = C.c_size_t
         L.mllm_hip_attention_paged_workspace_bytes.argtypes = [ci, i64, i64, ci, ci, ci, i64, i64]
         L.mllm_hip_attention_paged.argtypes = [rp, ci, i64, kv, vp, i64, i64, vp, vp, i64, i64, i64, vp, i64, i64, cf, vp, C.c_size_t, vp]
+        L.mllm_hip_sample_workspace_bytes.restype = C.c_size_t
+        L.mllm_hip_sample_workspace_bytes.argtypes = [i64, i64]
+        L.mllm_hip_sample.argtypes = [vp, ci, i64, i64, i64, vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp]
         _lib = L
     return _lib
 

@@ -450,6 +450,27 @@ PyObject* attention_paged(Args a) {
   return THPVariable_Wrap(y);
 }
 
+// (logits, u, temperature, top_k, top_p, min_p, out, workspace)
+PyObject* sample(Args a) {
+  const int64_t device = current_device();
+  const at::Tensor& x = tensor(a[0]);
+  const int dtype = xdtype(x);
+  require(x.is_cuda() && x.get_device() == device && x.dim() == 2 && x.size(1) >= 1 && (x.size(1) == 1 || x.stride(1) == 1));
+  const int64_t rows = x.size(0), vocab = x.size(1), stride = stride_of(x, 0);
+  require(a[1] != Py_None);
+  const float *u = vector_of<float>(a[1], device, at::kFloat, rows), *t = vector_of<float>(a[2], device, at::kFloat, rows),
+              *p = vector_of<float>(a[4], device, at::kFloat, rows), *min_p = vector_of<float>(a[5], device, at::kFloat, rows);
+  const int32_t* k = vector_of<int32_t>(a[3], device, at::kInt, rows);
+  at::Tensor made, work;
+  if (a[6] == Py_None) made = empty({rows}, at::kInt);
+  int32_t* tokens = a[6] == Py_None ? static_cast<int32_t*>(made.data_ptr()) : const_cast<int32_t*>(vector_of<int32_t>(a[6], device, at::kInt, rows));
+  const size_t need = mllm_hip_sample_workspace_bytes(rows, vocab);
+  void* wp = need || a[7] != Py_None ? workspace(a[7], need, work) : nullptr;
+  void *xp = x.data_ptr(), *st = stream();
+  run("mllm_hip_sample", [&] { return mllm_hip_sample(xp, dtype, stride, rows, vocab, u, t, k, p, min_p, tokens, wp, need, st); });
+  return a[6] == Py_None ? THPVariable_Wrap(made) : given(a[6]);
+}
+
 template <PyObject* (*F)(Args), int N>
 PyObject* entry(PyObject*, Args args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -467,7 +488,7 @@ PyObject* entry(PyObject*, Args args, Py_ssize_t n) {
 #define CALL(name, n) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(entry<name, n>)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {CALL(linear_q_gemv, 8), CALL(linear_q_gemv_multi, 6), CALL(softmax, 1), CALL(topk, 4), CALL(matmul, 5),
                            CALL(w8a8_linear_packed, 7), CALL(w4a16_gemm_packed, 6), CALL(linear_q_gemm, 7), CALL(linear_kq_gemm, 6),
-                           CALL(qk_norm_rope, 10), CALL(kv_append, 14), CALL(attention_paged, 12), {nullptr, nullptr, 0, nullptr}};
+                           CALL(qk_norm_rope, 10), CALL(kv_append, 14), CALL(attention_paged, 12), CALL(sample, 8), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "mllm_calls", nullptr, -1, g_methods};
 
 }  // namespace

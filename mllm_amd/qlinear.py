@@ -707,3 +707,12 @@ def tree_mask(parents, words=None):
         rows.append((rows[p] if p >= 0 else 0) | 1 << i)
     signed = lambda w: w - (1 << 64) if w >> 63 else w  # noqa: E731
     return torch.tensor([[signed(r >> (64 * w) & full) for w in range(words)] for r in rows], dtype=torch.int64).view(n, words)
+
+
+# ----------------------------------------------------------------------------- the token that follows
+def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out=None, workspace=None):
+    """A token int32 [rows] from every row of logits [rows, vocab] (fp32 or bf16) and uniform numbers u fp32 [rows]: weights exp((x - max) /
+    temperature); the top_k largest (0: all), of these the shortest beginning with top_p of their mass (1: all), of these the ones of min_p of the
+    largest weight or more; the first kept one in the order of the index at which the running sum exceeds u of all.  Settings: fp32
+    (top_k int32) [rows], None: 1, 0, 1, 0.  temperature 0: the largest logit.  Equal logits: lowest index first.  The same inputs give the same token."""
+    return _calls().sample(logits, u, temperature, top_k, top_p, min_p, out, workspace)

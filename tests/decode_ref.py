@@ -88,9 +88,7 @@ def sample(logits, u, temperature, top_k, top_p, min_p):
     if p < 1:
         before = np.concatenate([[0.0], np.cumsum(w[order])])
         w[order[max(1, int(np.searchsorted(before, p * before[-1], "left"))):]] = 0
-    keep = w >= float(np.float32(min_p))
-    keep[order[0]] = True
-    w[~keep] = 0
+    w[w < min(float(np.float32(min_p)), 1.0)] = 0
     up_to = np.cumsum(w)
     i = int(np.searchsorted(up_to, float(np.float32(u)) * up_to[-1], "right"))
     return min(i, int(np.nonzero(w)[0][-1]))

@@ -92,3 +92,22 @@ def test_tree_mask():
         ql.tree_mask([0])
     with pytest.raises(ValueError):
         ql.tree_mask(list(range(-1, 64)), 1)
+
+
+def _sample(x=P, dtype=F32, stride=1000, rows=2, vocab=1000, u=P, t=None, k=None, p=None, m=None, out=P, work=P, size=1 << 30):
+    return _lib.lib().mllm_hip_sample(x, dtype, stride, rows, vocab, u, t, k, p, m, out, work, size, None)
+
+
+@pytest.mark.parametrize("args,want", [
+    (dict(x=None), BADARG), (dict(u=None), BADARG), (dict(out=None), BADARG), (dict(work=None), BADARG), (dict(dtype=2), BADARG), (dict(rows=-1), BADARG), (dict(vocab=0), BADARG),
+    (dict(stride=-1), BADARG), (dict(vocab=(1 << 24) + 1), SHAPE), (dict(rows=65536), SHAPE), (dict(x=ODD), ALIGN), (dict(x=P + 1, dtype=BF16), ALIGN), (dict(u=ODD), ALIGN),
+    (dict(t=ODD), ALIGN), (dict(k=ODD), ALIGN), (dict(p=ODD), ALIGN), (dict(m=ODD), ALIGN), (dict(out=ODD), ALIGN), (dict(work=P + 8), ALIGN), (dict(size=1000), BADARG),
+    (dict(rows=0, x=None, u=None, out=None, work=None), 0)])
+def test_sample(args, want):
+    assert _sample(**args) == want
+
+
+def test_sample_workspace():
+    size = _lib.lib().mllm_hip_sample_workspace_bytes
+    assert size(0, 100) == 0 and size(4, 0) == 0 and size(1, 1 << 25) == 0
+    assert size(8, 151936) >= 8 * 151936 * 4 and size(8, 151936) % 16 == 0
