@@ -17,7 +17,7 @@
 
 namespace mllmhip {
 
-enum { SMP_STEPS = 512, SMP_WG = 512, SMP_BINS = 2048, SMP_LAST = 1024 };
+enum { SMP_STEPS = 512, SMP_WG = 512, SMP_BINS = 2048, SMP_LAST = 1024, SMP_RANKED = 512, SMP_PIECES = 16 };
 
 struct SampleRow {  // what launch 3 finds out about a row
   int lo, hi;       // the border's steps; lo = SMP_STEPS: everything is kept
@@ -129,13 +129,24 @@ __device__ __forceinline__ void share(int vecs, int pieces, int p, int waves, in
 // A row's weights: its maximum, what divides its logits, and the steps
 struct SampleScale {
   float top, step;
-  double inv_t, t;
+  double c;       // 64 / (t ln 2)
   bool infinite;  // the maximum is: its equals weigh 1, the rest nothing
   float min_w;
+  const double* table;  // 2^(j / 64), j = 0 .. 63
+  // exp((v - top) / t) = 2^(n / 64) e^(r ln 2 / 64) with n + r = (v - top) c, |r| <= 1/2: the table, a power of two and five terms of the series (the
+  // sixth is under 2^-54).  Off by 2^-52 and what rounding (v - top) c leaves of up to 36, 2^-47; the library's exp of a quotient took three times as long.
   __device__ __forceinline__ double weight(float v) const {
     if (infinite) return v == INFINITY ? 1.0 : 0.0;
-    const double w = exp(((double)v - (double)top) / t);
-    return w < 0x1p-52 ? 0.0 : w;
+    const double y = ((double)v - (double)top) * c;
+    if (!(y > -3328.0)) return 0.0;  // 52 * 64: below 2^-52
+    const double n = rint(y), r = (y - n) * 0.010830424696249145;
+    const int i = (int)n;
+    double e = fma(r, 1.0 / 120.0, 1.0 / 24.0);
+    e = fma(r, e, 1.0 / 6.0);
+    e = fma(r, e, 0.5);
+    e = fma(r, e, 1.0);
+    e = fma(r, e, 1.0);
+    return __builtin_ldexp(e * table[i & 63], i >> 6);
   }
   // the step of a logit; SMP_STEPS: its weight is below 2^-52
   __device__ __forceinline__ int step_of(float v) const {
@@ -145,8 +156,11 @@ struct SampleScale {
   }
   __device__ __forceinline__ bool heavy(double w) const { return w > 0.0 && w >= (double)min_w; }
 };
-__device__ __forceinline__ SampleScale scale_of(const SampleArgs& a, int row) {
+// (the caller waits for the other waves before it takes a weight)
+__device__ __forceinline__ SampleScale scale_of(const SampleArgs& a, int row, double* table) {
   SampleScale s;
+  if (threadIdx.x < 64) table[threadIdx.x] = exp2((double)threadIdx.x / 64.0);
+  s.table = table;
   float top = -INFINITY, low = INFINITY;
   for (int i = threadIdx.x & 63; i < a.pieces; i += 64) {
     top = fmaxf(top, a.ends[2 * (row * a.pieces + i)]);
@@ -159,13 +173,28 @@ __device__ __forceinline__ SampleScale scale_of(const SampleArgs& a, int row) {
   }
   const float t = a.t ? a.t[row] : 1.0f;
   s.top = top;
-  s.t = t;
+  s.c = 92.332482616893656877 / (double)t;
   s.infinite = top == INFINITY;
   s.min_w = a.min_p ? fminf(a.min_p[row], 1.0f) : 0.0f;
   // 52 ln 2 = 36.04 times t below the maximum weights end; a little more than the range, so that the last of it is in the last step
   const float range = fminf(top - low, 36.05f * t) * 1.00001f;
   s.step = range > 1e-30f ? (float)SMP_STEPS / range : 0.f;
   return s;
+}
+// What cuts a row.  few: so small a k that all it keeps is listed and ranked, and no step's mass is needed
+struct SampleCut {
+  int k;
+  float p;
+  bool by_count, by_mass, few;
+};
+__device__ __forceinline__ SampleCut cut_of(const SampleArgs& a, int row) {
+  SampleCut c;
+  c.k = a.k ? a.k[row] : 0;
+  c.p = a.p ? a.p[row] : 1.0f;
+  c.by_count = c.k > 0 && c.k < a.V;
+  c.by_mass = c.p < 1.0f;
+  c.few = c.by_count && c.k <= SMP_RANKED / 2;
+  return c;
 }
 __device__ __forceinline__ bool greedy(const SampleArgs& a, int row) { return a.t && !(a.t[row] > 0.f); }
 
@@ -217,10 +246,12 @@ __global__ __launch_bounds__(SMP_WG) void sample_steps_kernel(SampleArgs a) {
   __shared__ unsigned long long s_mass[SMP_STEPS];
   const int piece = blockIdx.x, row = blockIdx.y;
   if (greedy(a, row)) return;
-  const bool by_count = a.k && a.k[row] > 0 && a.k[row] < a.V, by_mass = a.p && a.p[row] < 1.0f;
-  if (!by_count && !by_mass) return;  // nothing is cut off
-  const SampleScale s = scale_of(a, row);
+  __shared__ double s_table[64];
+  const SampleCut cut = cut_of(a, row);
+  if (!cut.by_count && !cut.by_mass) return;  // nothing is cut off
+  const SampleScale s = scale_of(a, row, s_table);
   if (s.top == -INFINITY) return;
+  const bool by_mass = cut.by_mass && !cut.few;
   for (int i = threadIdx.x; i < SMP_STEPS; i += SMP_WG) s_count[i] = 0, s_mass[i] = 0;
   __syncthreads();
   const SampleSpan<XT> span(a, row);
@@ -274,21 +305,35 @@ __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
   __shared__ double s_sum[SMP_WG / 64];
   const int piece = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (greedy(a, row)) return;
-  const SampleScale s = scale_of(a, row);
+  __shared__ double s_table[64];
+  const SampleCut cut = cut_of(a, row);
+  const int k = cut.k;
+  const float p = cut.p;
+  const bool by_count = cut.by_count, by_mass = cut.by_mass && !cut.few;
+  // (all pieces' steps are on their way at once: one after the other they were 14 us)
+  uint32_t counts_of[SMP_PIECES];
+  unsigned long long mass_of[SMP_PIECES];
+  if (by_count || by_mass) {
+    const int64_t at = (int64_t)row * a.pieces * SMP_STEPS + tid;
+#pragma unroll
+    for (int i = 0; i < SMP_PIECES; i++) {
+      const int64_t from = at + (int64_t)min(i, a.pieces - 1) * SMP_STEPS;
+      counts_of[i] = a.count[from];
+      mass_of[i] = by_mass ? a.mass[from] : 0;
+    }
+  }
+  const SampleScale s = scale_of(a, row, s_table);
   if (s.top == -INFINITY) return;
-  const int k = a.k ? a.k[row] : 0;
-  const float p = a.p ? a.p[row] : 1.0f;
-  const bool by_count = k > 0 && k < a.V, by_mass = p < 1.0f;
   SampleRow r = {SMP_STEPS, SMP_STEPS, 0, 0, 0, 0, 0, 0};
   uint32_t mine = 0;  // elements of step tid in the pieces in front of this one
   if (by_count || by_mass) {
     unsigned long long count = 0, mass = 0;
-    const int64_t at = (int64_t)row * a.pieces * SMP_STEPS + tid;
-    for (int i = 0; i < a.pieces; i++) {
-      const uint32_t c = a.count[at + (int64_t)i * SMP_STEPS];
-      if (i < piece) mine += c;
-      count += c;
-      mass += a.mass[at + (int64_t)i * SMP_STEPS];
+#pragma unroll
+    for (int i = 0; i < SMP_PIECES; i++) {
+      if (i >= a.pieces) break;
+      if (i < piece) mine += counts_of[i];
+      count += counts_of[i];
+      mass += mass_of[i];
     }
     const unsigned long long counts = running<unsigned long long, SMP_WG>(count, s_wave), masses = running<unsigned long long, SMP_WG>(mass, s_wave);
     s_count[tid] = (uint32_t)counts;
@@ -301,7 +346,10 @@ __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
     r.cut = s_first[0] < SMP_STEPS;
     r.hi = s_first[0];
     r.mass = s_mass[SMP_STEPS - 1];
-    if (by_mass) {  // with a cut by count the mass of what it keeps is only known to be that in front of step hi or more
+    if (cut.few) {
+      r.lo = 0;
+      r.hi = min(r.hi, SMP_STEPS - 1);
+    } else if (by_mass) {  // with a cut by count the mass of what it keeps is only known to be that in front of step hi or more
       const double target = (double)p * (double)(r.cut ? up_to(r.hi, true) : r.mass);
       if ((double)masses >= target && (tid == 0 || (double)(masses - mass) < target)) atomicMin(&s_first[1], tid);
       __syncthreads();
@@ -320,7 +368,7 @@ __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
     __syncthreads();
     mine = tid >= r.lo && tid <= r.hi ? mine : 0;
   }
-  // where this piece's part of the list begins
+  // where this piece's part of the list begins (and the weights' table is there)
   running<unsigned long long, SMP_WG>(mine, s_wave);
   uint32_t from = 0;
   for (int w = 0; w < SMP_WG / 64; w++) from += (uint32_t)s_wave[w];
@@ -418,7 +466,8 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
     if (lane == 0) a.token[row] = top == -INFINITY ? -1 : at;
     return;
   }
-  const SampleScale s = scale_of(a, row);
+  __shared__ double s_table[64];
+  const SampleScale s = scale_of(a, row, s_table);
   if (s.top == -INFINITY) {
     if (tid == 0) a.token[row] = -1;
     return;
@@ -426,7 +475,9 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
   const SampleRow r = a.row[row];
   const SampleSpan<XT> span(a, row);
   const uint32_t* list = a.list + (int64_t)row * a.V;
-  const float p = a.p ? a.p[row] : 1.0f;
+  const SampleCut cut = cut_of(a, row);
+  const float p = cut.p;
+  __syncthreads();
 
   // The border among the listed elements: the `want`-th of them (mass < 0), or the first at which their mass and base reach `target`.  Every
   // round counts the elements of a range of keys in 2048 bins from above and goes on with one bin.
@@ -489,21 +540,69 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
       }
     }
   };
-  SampleBorder edge = {0, 0xffffffffu, 0};
-  if (r.lo < SMP_STEPS) {
+  uint32_t edge_key = 0;  // what is above it is kept, and what equals it up to index `last`
+  int last = 0x7fffffff;
+  if (r.lo < SMP_STEPS && r.listed <= SMP_RANKED) {
+    // Few: everyone's rank and the mass in front of it, by comparing all with all; lanes of an element share the others.
+    __shared__ unsigned long long s_of[SMP_RANKED];
+    __shared__ uint32_t s_element[SMP_RANKED];
+    int size = 16;
+    while (size < (int)r.listed) size <<= 1;
+    const int share_ = SMP_LAST / size, e = tid / share_, part = tid % share_;  // 2 .. 64 lanes
+    if (tid < SMP_RANKED) {
+      const float v = tid < (int)r.listed ? span.at((int)list[tid]) : -INFINITY;
+      s_element[tid] = key_of(v);
+      s_of[tid] = tid < (int)r.listed ? units(v) : 0;
+    }
+    if (tid < 2) s_key[tid] = 0;
+    if (tid < 3) s_bin[tid] = 0;
+    __syncthreads();
+    const uint32_t key = s_element[e];
+    const unsigned long long own = s_of[e];
+    uint32_t rank = 0;
+    unsigned long long before = 0;
+    for (int i = part; i < (int)r.listed; i += share_) {
+      const uint32_t o = s_element[i];
+      const bool front = o > key || (o == key && i < e);
+      rank += front;
+      before += front ? s_of[i] : 0;
+    }
+    for (int d = 1; d < share_; d <<= 1) {
+      rank += __shfl_xor(rank, d);
+      before += __shfl_xor(before, d);
+    }
+    rank += r.above;
+    before += r.mass_above;
+    const bool here = e < (int)r.listed && part == 0;
+    if (here && (r.cut ? rank == (uint32_t)cut.k - 1 : rank == r.above + r.listed - 1)) {  // the last that the count leaves: its number, the mass up to it
+      s_key[0] = e;
+      s_bin[0] = before + own;
+    }
+    __syncthreads();
+    const double target = (double)p * (double)(r.cut || cut.few ? s_bin[0] : r.mass);
+    if (cut.by_mass && here && (!r.cut || rank < (uint32_t)cut.k) && (double)before < target && (double)(before + own) >= target) {  // at most one
+      s_key[0] = e;
+      s_bin[1] = 1;
+    }
+    // (a mass of nothing or less is reached in front of the first, which is kept all the same)
+    if (cut.by_mass && here && rank == 0 && !(target > 0.0)) s_key[0] = e;
+    __syncthreads();
+    edge_key = s_element[s_key[0]];
+    last = (int)list[s_key[0]];
+  } else if (r.lo < SMP_STEPS) {
+    SampleBorder edge = {0, 0xffffffffu, 0};
     unsigned long long mass = r.mass;
     if (r.cut) {
       edge = border(false, (unsigned long long)a.k[row] - r.above, 0.0, r.mass_above);
       mass = edge.mass;
     }
-    if (p < 1.0f) {
+    if (cut.by_mass) {
       const SampleBorder e = border(true, 0, (double)p * (double)mass, r.mass_above);
       if (!r.cut || e.key > edge.key || (e.key == edge.key && e.equals < edge.equals)) edge = e;
     }
-  }
-  // the index of the last equal that is kept (the list is in the order of the index)
-  int last = 0x7fffffff;
-  if (r.lo < SMP_STEPS && edge.equals != 0xffffffffu) {
+    edge_key = edge.key;
+    // the index of the last equal that is kept (the list is in the order of the index)
+    if (edge.equals != 0xffffffffu) {
     __syncthreads();
     if (tid == 0) s_at = 0x7fffffff;
     const uint32_t per = (r.listed + SMP_LAST - 1) / SMP_LAST, i0 = min(r.listed, tid * per), i1 = min(r.listed, i0 + per);
@@ -517,13 +616,14 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
     }
     __syncthreads();
     last = s_at;
+    }
   }
   auto kept = [&](int i, float v) {  // the weight of a kept element, 0 of another
     const int step = s.step_of(v);
     if (step >= SMP_STEPS || step > r.hi) return 0.0;
     if (step >= r.lo) {
       const uint32_t key = key_of(v);
-      if (key < edge.key || (key == edge.key && i > last)) return 0.0;
+      if (key < edge_key || (key == edge_key && i > last)) return 0.0;
     }
     const double w = s.weight(v);
     return s.heavy(w) ? w : 0.0;
@@ -619,11 +719,11 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------------
-// Pieces of a row: enough workgroups for the chip, of 4096 logits at least, and 16 at most (launch 3 adds up the steps of all pieces in every one)
+// Pieces of a row: enough workgroups for the chip, of 4096 logits at least, and SMP_PIECES at most (launch 3 adds up the steps of all pieces in every one)
 static int sample_pieces(int64_t rows, int64_t V) {
   const int64_t most = (V + 4095) / 4096, want = (1024 + rows - 1) / rows;
   const int64_t n = want < most ? want : most;
-  return (int)(n > 16 ? 16 : n);
+  return (int)(n > SMP_PIECES ? SMP_PIECES : n);
 }
 static size_t sample_room(int64_t rows, int64_t V, int pieces) {
   const size_t rp = (size_t)rows * pieces;
