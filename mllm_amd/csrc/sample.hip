@@ -17,7 +17,8 @@
 
 namespace mllmhip {
 
-enum { SMP_STEPS = 512, SMP_WG = 512, SMP_BINS = 2048, SMP_LAST = 1024, SMP_RANKED = 512, SMP_PIECES = 16 };
+enum { SMP_STEPS = 512, SMP_WG = 512, SMP_BIN_BITS = 9, SMP_BINS = 1 << SMP_BIN_BITS, SMP_LAST = 1024, SMP_RANKED = 128, SMP_FEW = 256, SMP_HELD = 2048,
+       SMP_PIECES = 16, SMP_HOLD = 5 };
 
 struct SampleRow {  // what launch 3 finds out about a row
   int lo, hi;       // the border's steps; lo = SMP_STEPS: everything is kept
@@ -40,16 +41,12 @@ struct SampleArgs {
   int* top;         // [rows][pieces]: index of the maximum
   uint32_t* count;  // [rows][pieces][SMP_STEPS]
   uint64_t* mass;   // the same
-  double* sum;      // [rows][pieces]
-  uint32_t* from;   // [rows][pieces]: where the piece's elements begin in the list
+  double* sum;      // [rows][pieces][waves]
+  uint32_t* from;   // the same: where a wave's elements begin in the list
   uint32_t* list;   // [rows][V]
   SampleRow* row;
 };
 
-template <int XT>
-struct SampleVec {
-  static constexpr int N = XT == MLLM_HIP_F32 ? 4 : 8;  // logits of 16 bytes
-};
 // a logit as the operator takes it: no number counts as -inf, -0 as 0
 __device__ __forceinline__ float logit(float v) { return v != v ? -INFINITY : v + 0.0f; }
 __device__ __forceinline__ uint32_t key_of(float v) {  // larger logits, larger keys
@@ -58,81 +55,128 @@ __device__ __forceinline__ uint32_t key_of(float v) {  // larger logits, larger 
 }
 __device__ __forceinline__ float of_key(uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
-// A row as 16-byte vectors: `head` elements in front of the first aligned one, `vecs` vectors, the rest behind.
+// A row as 16-byte vectors of N logits: vector 0 ends where the first aligned one begins (it may be empty), the last one is what is left.
+// Elements of a vector that the row does not have count as -inf.
 template <int XT>
 struct SampleSpan {
-  static constexpr int N = SampleVec<XT>::N;
+  static constexpr int N = XT == MLLM_HIP_F32 ? 4 : 8;
   const char* x;
-  int V, head, vecs;
+  int V, lead, vecs;  // lead: elements that vector 0 lacks in front
   __device__ __forceinline__ SampleSpan(const SampleArgs& a, int row) {
     constexpr int wide = 16 / N;
     x = reinterpret_cast<const char*>(a.x) + row * a.stride * wide;
     V = a.V;
-    head = min(V, (int)((16 - (reinterpret_cast<uintptr_t>(x) & 15)) & 15) / wide);
-    vecs = (V - head) / N;
+    lead = (int)(reinterpret_cast<uintptr_t>(x) & 15) / wide;
+    vecs = (lead + V + N - 1) / N;
   }
   __device__ __forceinline__ float at(int i) const {
     return logit(XT == MLLM_HIP_F32 ? reinterpret_cast<const float*>(x)[i] : bf16_to_f32(reinterpret_cast<const uint16_t*>(x)[i]));
   }
-  // Calls f(i, v, n) in the order of the index for vectors v0 .. v1 - 1 by a wave, with the elements in front of the first and behind the last vector of
-  // the row: a lane's n elements v[0 .. n - 1] are i .. i + n - 1 (lanes in ascending order; every lane comes along, with n = 0 if it has none)
-  template <typename F>
-  __device__ __forceinline__ void walk(int v0, int v1, F&& f) const {
-    const int lane = threadIdx.x & 63;
-    float v[N];
-    if (v0 == 0 && head) {
-      v[0] = lane < head ? at(lane) : 0.f;
-      f(lane, v, lane < head ? 1 : 0);
+  __device__ __forceinline__ int first_of(int vec) const { return vec * N - lead; }
+  __device__ __forceinline__ bool whole(int vec) const { return first_of(vec) >= 0 && first_of(vec) + N <= V; }
+  __device__ __forceinline__ u32x4 load(int vec) const { return *reinterpret_cast<const u32x4*>(x + (int64_t)first_of(vec) * (16 / N)); }
+  __device__ __forceinline__ u32x4 part(int vec) const {  // element by element
+    const int i = first_of(vec);
+    uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+    for (int e = 0; e < N; e++) {
+      const bool in = i + e >= 0 && i + e < V;
+      if (XT == MLLM_HIP_F32) w[e % 4] = in ? reinterpret_cast<const uint32_t*>(x)[i + e] : 0xff800000u;
+      else w[e / 2 % 4] |= (uint32_t)(in ? reinterpret_cast<const uint16_t*>(x)[i + e] : 0xff80u) << (e % 2 * 16);
     }
-    constexpr int U = 4;  // vectors in flight
-    for (int b = v0; b < v1; b += 64 * U) {
-      u32x4 r[U];
+    return u32x4{w[0], w[1], w[2], w[3]};
+  }
+  static __device__ __forceinline__ void logits(const u32x4& r, float (&v)[N]) {
+    const uint32_t w[4] = {r.x, r.y, r.z, r.w};
 #pragma unroll
-      for (int j = 0; j < U; j++) {
-        const int at_ = min(b + j * 64 + lane, v1 - 1);
-        r[j] = *reinterpret_cast<const u32x4*>(x + (int64_t)head * (16 / N) + (int64_t)at_ * 16);
+    for (int e = 0; e < 4; e++) {
+      if (XT == MLLM_HIP_F32) {
+        v[e] = logit(__uint_as_float(w[e]));
+      } else {
+        v[2 * e % N] = logit(__uint_as_float(w[e] << 16));
+        v[(2 * e + 1) % N] = logit(__uint_as_float(w[e] & 0xffff0000u));
       }
-#pragma unroll
-      for (int j = 0; j < U; j++) {
-        if (b + j * 64 >= v1) break;
-        const int at_ = b + j * 64 + lane;
-        const uint32_t w[4] = {r[j].x, r[j].y, r[j].z, r[j].w};
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          if (XT == MLLM_HIP_F32) {
-            v[e] = logit(__uint_as_float(w[e]));
-          } else {
-            v[2 * e % N] = logit(__uint_as_float(w[e] << 16));
-            v[(2 * e + 1) % N] = logit(__uint_as_float(w[e] & 0xffff0000u));
-          }
-        }
-        f(head + at_ * N, v, at_ < v1 ? N : 0);
-      }
-    }
-    const int tail = head + vecs * N;
-    if (v1 == vecs && tail < V) {
-      v[0] = tail + lane < V ? at(tail + lane) : 0.f;
-      f(tail + lane, v, tail + lane < V ? 1 : 0);
     }
   }
 };
-// vectors of wave `wave` of `waves` in piece p
-__device__ __forceinline__ void share(int vecs, int pieces, int p, int waves, int wave, int& v0, int& v1) {
-  const int per = (vecs + pieces - 1) / pieces, a = min(vecs, p * per), b = min(vecs, a + per), each = (b - a + waves - 1) / waves;
-  v0 = min(b, a + wave * each);
-  v1 = min(b, v0 + each);
-  // who has the row's first or last vector also has what is in front of or behind it; a row without vectors belongs to the first wave
-  if (vecs == 0) v0 = 0, v1 = p == 0 && wave == 0 ? 0 : -1;
-  else if (v0 == v1) v0 = v1 = -1;
-}
+// A wave's vectors of a row, in the order of the index.  They go through LDS (H vectors a lane at a time, on their way all at once), so that the loop over
+// them is short: code is fetched anew by every launch, and unrolled over registers these kernels ran for as long as that took.
+template <int XT, int H>
+struct SampleWalk {
+  typedef SampleSpan<XT> Span;
+  static constexpr int N = Span::N;
+  const Span& span;
+  u32x4* lds;  // [H][64] of this wave
+  int v0, v1, held;
+  __device__ __forceinline__ SampleWalk(const Span& span_, u32x4* lds_, int pieces, int p, int waves, int wave) : span(span_), lds(lds_ + wave * H * 64), held(-1) {
+    const int per = (span.vecs + pieces - 1) / pieces, a = min(span.vecs, p * per), b = min(span.vecs, a + per), each = (b - a + waves - 1) / waves;
+    v0 = min(b, a + wave * each);
+    v1 = min(b, v0 + each);
+  }
+  __device__ __forceinline__ void hold(int from) {
+    if (held == from) return;
+    held = from;
+    const int lane = threadIdx.x & 63;
+    u32x4 r[H];
+#pragma unroll
+    for (int j = 0; j < H; j++) {
+      const int vec = min(from + j * 64 + lane, v1 - 1);
+      r[j] = span.whole(vec) ? span.load(vec) : u32x4{0, 0, 0, 0};
+    }
+#pragma unroll
+    for (int j = 0; j < H; j++) lds[j * 64 + lane] = r[j];
+#pragma unroll 1
+    for (int end = 0; end < 2; end++) {  // the row's first and last vector
+      const int vec = end ? span.vecs - 1 : 0;
+      if (vec >= from && vec < min(v1, from + H * 64) && !span.whole(vec) && (vec - from) % 64 == lane) lds[vec - from] = span.part(vec);
+    }
+  }
+  // f(i, v): a lane's elements i .. i + N - 1; every lane comes along, with -inf where it has none
+  template <typename F>
+  __device__ __forceinline__ void operator()(F&& f) {
+    const int lane = threadIdx.x & 63;
+    for (int b = v0; b < v1; b += H * 64) {
+      hold(b);
+#pragma unroll 1
+      for (int at = b + lane, j = 0; j < H && b + j * 64 < v1; j++, at += 64) {
+        float v[N];
+        Span::logits(lds[j * 64 + lane], v);
+        if (at >= v1) {
+#pragma unroll
+          for (int e = 0; e < N; e++) v[e] = -INFINITY;
+        }
+        f(span.first_of(at), v);
+      }
+    }
+  }
+};
 
+// 2^(j / 64), rounded to nearest
+__device__ const double g_pow64[64] = {
+    0x1.0000000000000p+0, 0x1.02c9a3e778061p+0, 0x1.059b0d3158574p+0, 0x1.0874518759bc8p+0,
+    0x1.0b5586cf9890fp+0, 0x1.0e3ec32d3d1a2p+0, 0x1.11301d0125b51p+0, 0x1.1429aaea92de0p+0,
+    0x1.172b83c7d517bp+0, 0x1.1a35beb6fcb75p+0, 0x1.1d4873168b9aap+0, 0x1.2063b88628cd6p+0,
+    0x1.2387a6e756238p+0, 0x1.26b4565e27cddp+0, 0x1.29e9df51fdee1p+0, 0x1.2d285a6e4030bp+0,
+    0x1.306fe0a31b715p+0, 0x1.33c08b26416ffp+0, 0x1.371a7373aa9cbp+0, 0x1.3a7db34e59ff7p+0,
+    0x1.3dea64c123422p+0, 0x1.4160a21f72e2ap+0, 0x1.44e086061892dp+0, 0x1.486a2b5c13cd0p+0,
+    0x1.4bfdad5362a27p+0, 0x1.4f9b2769d2ca7p+0, 0x1.5342b569d4f82p+0, 0x1.56f4736b527dap+0,
+    0x1.5ab07dd485429p+0, 0x1.5e76f15ad2148p+0, 0x1.6247eb03a5585p+0, 0x1.6623882552225p+0,
+    0x1.6a09e667f3bcdp+0, 0x1.6dfb23c651a2fp+0, 0x1.71f75e8ec5f74p+0, 0x1.75feb564267c9p+0,
+    0x1.7a11473eb0187p+0, 0x1.7e2f336cf4e62p+0, 0x1.82589994cce13p+0, 0x1.868d99b4492edp+0,
+    0x1.8ace5422aa0dbp+0, 0x1.8f1ae99157736p+0, 0x1.93737b0cdc5e5p+0, 0x1.97d829fde4e50p+0,
+    0x1.9c49182a3f090p+0, 0x1.a0c667b5de565p+0, 0x1.a5503b23e255dp+0, 0x1.a9e6b5579fdbfp+0,
+    0x1.ae89f995ad3adp+0, 0x1.b33a2b84f15fbp+0, 0x1.b7f76f2fb5e47p+0, 0x1.bcc1e904bc1d2p+0,
+    0x1.c199bdd85529cp+0, 0x1.c67f12e57d14bp+0, 0x1.cb720dcef9069p+0, 0x1.d072d4a07897cp+0,
+    0x1.d5818dcfba487p+0, 0x1.da9e603db3285p+0, 0x1.dfc97337b9b5fp+0, 0x1.e502ee78b3ff6p+0,
+    0x1.ea4afa2a490dap+0, 0x1.efa1bee615a27p+0, 0x1.f50765b6e4540p+0, 0x1.fa7c1819e90d8p+0};
+typedef __attribute__((address_space(3))) double* lds_double;
 // A row's weights: its maximum, what divides its logits, and the steps
 struct SampleScale {
   float top, step;
   double c;       // 64 / (t ln 2)
   bool infinite;  // the maximum is: its equals weigh 1, the rest nothing
   float min_w;
-  const double* table;  // 2^(j / 64), j = 0 .. 63
+  lds_double table;  // 2^(j / 64), j = 0 .. 63
   // exp((v - top) / t) = 2^(n / 64) e^(r ln 2 / 64) with n + r = (v - top) c, |r| <= 1/2: the table, a power of two and five terms of the series (the
   // sixth is under 2^-54).  Off by 2^-52 and what rounding (v - top) c leaves of up to 36, 2^-47; the library's exp of a quotient took three times as long.
   __device__ __forceinline__ double weight(float v) const {
@@ -154,12 +198,16 @@ struct SampleScale {
     const float q = (top - v) * step;
     return q < (float)SMP_STEPS ? (int)q : SMP_STEPS;
   }
+  // a weight in whole units, 2^51 to the weight of 1 at most: added to 2^52 they are the low bits of the sum
+  __device__ __forceinline__ unsigned long long units(float v, double unit) const {
+    return (unsigned long long)__double_as_longlong(fma(weight(v), unit, 0x1p52)) & 0xfffffffffffffull;
+  }
   __device__ __forceinline__ bool heavy(double w) const { return w > 0.0 && w >= (double)min_w; }
 };
 // (the caller waits for the other waves before it takes a weight)
-__device__ __forceinline__ SampleScale scale_of(const SampleArgs& a, int row, double* table) {
+__device__ __forceinline__ SampleScale scale_of(const SampleArgs& a, int row, lds_double table) {
   SampleScale s;
-  if (threadIdx.x < 64) table[threadIdx.x] = exp2((double)threadIdx.x / 64.0);
+  if (threadIdx.x < 64) table[threadIdx.x] = g_pow64[threadIdx.x];
   s.table = table;
   float top = -INFINITY, low = INFINITY;
   for (int i = threadIdx.x & 63; i < a.pieces; i += 64) {
@@ -193,7 +241,7 @@ __device__ __forceinline__ SampleCut cut_of(const SampleArgs& a, int row) {
   c.p = a.p ? a.p[row] : 1.0f;
   c.by_count = c.k > 0 && c.k < a.V;
   c.by_mass = c.p < 1.0f;
-  c.few = c.by_count && c.k <= SMP_RANKED / 2;
+  c.few = c.by_count && c.k <= SMP_FEW;
   return c;
 }
 __device__ __forceinline__ bool greedy(const SampleArgs& a, int row) { return a.t && !(a.t[row] > 0.f); }
@@ -201,23 +249,21 @@ __device__ __forceinline__ bool greedy(const SampleArgs& a, int row) { return a.
 // ---- 1: ends of every piece -------------------------------------------------------------------------------------------------
 template <int XT>
 __global__ __launch_bounds__(SMP_WG) void sample_ends_kernel(SampleArgs a) {
+  __shared__ __align__(16) u32x4 s_x[SMP_WG * SMP_HOLD];
   __shared__ float s_top[SMP_WG / 64], s_low[SMP_WG / 64];
   __shared__ int s_at[SMP_WG / 64];
   const int piece = blockIdx.x, row = blockIdx.y, lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
   const SampleSpan<XT> span(a, row);
-  int v0, v1;
-  share(span.vecs, a.pieces, piece, SMP_WG / 64, wave, v0, v1);
+  SampleWalk<XT, SMP_HOLD> walk(span, s_x, a.pieces, piece, SMP_WG / 64, wave);
   float top = -INFINITY, low = INFINITY;
   int at = 0x7fffffff;
-  if (v1 >= 0)
-    span.walk(v0, v1, [&](int i, const float (&v)[SampleSpan<XT>::N], int n) {
+  walk([&](int i, const float (&v)[SampleSpan<XT>::N]) {
 #pragma unroll
-      for (int e = 0; e < SampleSpan<XT>::N; e++) {
-        if (e >= n) break;
-        if (v[e] > top) top = v[e], at = i + e;
-        if (v[e] > -INFINITY) low = fminf(low, v[e]);
-      }
-    });
+    for (int e = 0; e < SampleSpan<XT>::N; e++) {
+      if (v[e] > top) top = v[e], at = i + e;
+      low = fminf(low, v[e] > -INFINITY ? v[e] : INFINITY);
+    }
+  });
 #pragma unroll
   for (int d = 32; d; d >>= 1) {
     const float o = __shfl_xor(top, d);
@@ -228,6 +274,7 @@ __global__ __launch_bounds__(SMP_WG) void sample_ends_kernel(SampleArgs a) {
   if (lane == 0) s_top[wave] = top, s_low[wave] = low, s_at[wave] = at;
   __syncthreads();
   if (threadIdx.x == 0) {
+#pragma unroll 1
     for (int w = 1; w < SMP_WG / 64; w++) {
       if (s_top[w] > top) top = s_top[w], at = s_at[w];  // (waves are in the order of the index)
       low = fminf(low, s_low[w]);
@@ -242,6 +289,7 @@ __global__ __launch_bounds__(SMP_WG) void sample_ends_kernel(SampleArgs a) {
 // ---- 2: counts and masses of the steps --------------------------------------------------------------------------------------
 template <int XT>
 __global__ __launch_bounds__(SMP_WG) void sample_steps_kernel(SampleArgs a) {
+  __shared__ __align__(16) u32x4 s_x[SMP_WG * SMP_HOLD];
   __shared__ uint32_t s_count[SMP_STEPS];
   __shared__ unsigned long long s_mass[SMP_STEPS];
   const int piece = blockIdx.x, row = blockIdx.y;
@@ -249,25 +297,24 @@ __global__ __launch_bounds__(SMP_WG) void sample_steps_kernel(SampleArgs a) {
   __shared__ double s_table[64];
   const SampleCut cut = cut_of(a, row);
   if (!cut.by_count && !cut.by_mass) return;  // nothing is cut off
-  const SampleScale s = scale_of(a, row, s_table);
+  const SampleSpan<XT> span(a, row);
+  SampleWalk<XT, SMP_HOLD> walk(span, s_x, a.pieces, piece, SMP_WG / 64, threadIdx.x >> 6);
+  if (walk.v0 < walk.v1) walk.hold(walk.v0);  // asked for before the row's maximum
+  const SampleScale s = scale_of(a, row, (lds_double)s_table);
   if (s.top == -INFINITY) return;
   const bool by_mass = cut.by_mass && !cut.few;
   for (int i = threadIdx.x; i < SMP_STEPS; i += SMP_WG) s_count[i] = 0, s_mass[i] = 0;
   __syncthreads();
-  const SampleSpan<XT> span(a, row);
-  int v0, v1;
-  share(span.vecs, a.pieces, piece, SMP_WG / 64, threadIdx.x >> 6, v0, v1);
-  if (v1 >= 0)
-    span.walk(v0, v1, [&](int, const float (&v)[SampleSpan<XT>::N], int n) {
+  walk([&](int, const float (&v)[SampleSpan<XT>::N]) {
 #pragma unroll
-      for (int e = 0; e < SampleSpan<XT>::N; e++) {
-        const int step = e < n ? s.step_of(v[e]) : SMP_STEPS;
-        if (step < SMP_STEPS) {
-          atomicAdd(&s_count[step], 1u);
-          if (by_mass) atomicAdd(&s_mass[step], (unsigned long long)(s.weight(v[e]) * a.unit + 0.5));
-        }
+    for (int e = 0; e < SampleSpan<XT>::N; e++) {
+      const int step = s.step_of(v[e]);
+      if (step < SMP_STEPS) {
+        atomicAdd(&s_count[step], 1u);
+        if (by_mass) atomicAdd(&s_mass[step], s.units(v[e], a.unit));
       }
-    });
+    }
+  });
   __syncthreads();
   const int64_t to = ((int64_t)row * a.pieces + piece) * SMP_STEPS;
   for (int i = threadIdx.x; i < SMP_STEPS; i += SMP_WG) {
@@ -297,12 +344,13 @@ __device__ __forceinline__ T running(T v, T* s_wave) {
 template <int XT>
 __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
   static_assert(SMP_WG == SMP_STEPS, "a thread per step");
+  __shared__ __align__(16) u32x4 s_x[SMP_WG * SMP_HOLD];
   __shared__ unsigned long long s_wave[SMP_WG / 64];
   __shared__ unsigned long long s_mass[SMP_STEPS];
   __shared__ uint32_t s_count[SMP_STEPS];
   __shared__ int s_first[2];
   __shared__ uint32_t s_list[SMP_WG / 64];
-  __shared__ double s_sum[SMP_WG / 64];
+  __shared__ float s_dense[SMP_WG * 2];
   const int piece = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   if (greedy(a, row)) return;
   __shared__ double s_table[64];
@@ -310,6 +358,10 @@ __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
   const int k = cut.k;
   const float p = cut.p;
   const bool by_count = cut.by_count, by_mass = cut.by_mass && !cut.few;
+  const SampleSpan<XT> span(a, row);
+  constexpr int N = SampleSpan<XT>::N;
+  SampleWalk<XT, SMP_HOLD> walk(span, s_x, a.pieces, piece, SMP_WG / 64, wave);
+  if (walk.v0 < walk.v1) walk.hold(walk.v0);
   // (all pieces' steps are on their way at once: one after the other they were 14 us)
   uint32_t counts_of[SMP_PIECES];
   unsigned long long mass_of[SMP_PIECES];
@@ -322,7 +374,7 @@ __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
       mass_of[i] = by_mass ? a.mass[from] : 0;
     }
   }
-  const SampleScale s = scale_of(a, row, s_table);
+  const SampleScale s = scale_of(a, row, (lds_double)s_table);
   if (s.top == -INFINITY) return;
   SampleRow r = {SMP_STEPS, SMP_STEPS, 0, 0, 0, 0, 0, 0};
   uint32_t mine = 0;  // elements of step tid in the pieces in front of this one
@@ -373,48 +425,57 @@ __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
   uint32_t from = 0;
   for (int w = 0; w < SMP_WG / 64; w++) from += (uint32_t)s_wave[w];
 
-  const SampleSpan<XT> span(a, row);
-  constexpr int N = SampleSpan<XT>::N;
-  int v0, v1;
-  share(span.vecs, a.pieces, piece, SMP_WG / 64, wave, v0, v1);
+  // Where few elements are in front of the border a weight of each lane would be one of them at a time: they are collected, 64 and more, first.
+  float* dense = s_dense + wave * 128;
   double sum = 0.0;
   uint32_t listed = 0;
-  if (v1 >= 0)
-    span.walk(v0, v1, [&](int, const float (&v)[N], int n) {
+  int waiting = 0;
+  auto add = [&](int n) {
+    const double w = s.weight(dense[lane]);
+    sum += lane < n && s.heavy(w) ? w : 0.0;
+  };
+  walk([&](int, const float (&v)[N]) {
 #pragma unroll
-      for (int e = 0; e < N; e++) {
-        const int step = e < n ? s.step_of(v[e]) : SMP_STEPS;
-        if (step < r.lo) {
-          const double w = s.weight(v[e]);
-          sum += s.heavy(w) ? w : 0.0;
-        } else if (step <= r.hi && step < SMP_STEPS) {
-          listed++;
+    for (int e = 0; e < N; e++) {
+      const int step = s.step_of(v[e]);
+      const bool in = step < r.lo && step < SMP_STEPS;
+      listed += !in && step <= r.hi && step < SMP_STEPS;
+      const uint64_t who = __ballot(in);
+      if (who) {
+        if (in) dense[waiting + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = v[e];
+        waiting += __popcll(who);
+        if (waiting >= 64) {
+          add(64);
+          waiting -= 64;
+          const float rest = dense[64 + lane];
+          dense[lane] = rest;
         }
       }
-    });
+    }
+  });
+  add(waiting);
 #pragma unroll
   for (int d = 32; d; d >>= 1) {
     sum += __shfl_xor(sum, d);
     listed += __shfl_xor(listed, d);
   }
-  if (lane == 0) s_sum[wave] = sum, s_list[wave] = listed;
+  if (lane == 0) s_list[wave] = listed;
   __syncthreads();
-  if (tid == 0) {
-    double all = 0.0;
-    for (int w = 0; w < SMP_WG / 64; w++) all += s_sum[w];
-    a.sum[row * a.pieces + piece] = all;
-    a.from[row * a.pieces + piece] = from;
-    if (piece == 0) a.row[row] = r;
+  for (int w = 0; w < wave; w++) from += s_list[w];
+  if (lane == 0) {
+    const int to = (row * a.pieces + piece) * (SMP_WG / 64) + wave;
+    a.sum[to] = sum;
+    a.from[to] = from;
   }
+  if (tid == 0 && piece == 0) a.row[row] = r;
   if (listed == 0) return;
   uint32_t to = from;
-  for (int w = 0; w < wave; w++) to += s_list[w];
   uint32_t* list = a.list + (int64_t)row * a.V;
-  span.walk(v0, v1, [&](int i, const float (&v)[N], int n) {
+  walk([&](int i, const float (&v)[N]) {
     uint32_t in = 0;
 #pragma unroll
     for (int e = 0; e < N; e++) {
-      const int step = e < n ? s.step_of(v[e]) : SMP_STEPS;
+      const int step = s.step_of(v[e]);
       in |= (uint32_t)(step >= r.lo && step <= r.hi && step < SMP_STEPS) << e;
     }
     if (!__ballot(in != 0)) return;
@@ -435,7 +496,8 @@ __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
 
 // ---- 4: the border, the piece, the token --------------------------------------------------------------------------------------
 struct SampleBorder {
-  uint32_t key, equals;  // what is above `key` is kept, and the first `equals` of what has it
+  uint32_t key;  // what is above is kept, and what equals it up to index `last`
+  int last;
   unsigned long long mass;  // of all that
 };
 template <int XT>
@@ -445,7 +507,14 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
   __shared__ unsigned long long s_mass[SMP_BINS];
   __shared__ unsigned long long s_wave[W];
   __shared__ double s_sum[W];
-  __shared__ uint32_t s_key[2];
+  __shared__ __align__(16) u32x4 s_x[SMP_LAST * 3];
+  __shared__ uint32_t s_element[SMP_HELD], s_index[SMP_HELD];  // the list: keys, indexes and masses
+  __shared__ unsigned long long s_of[SMP_HELD];
+  struct __align__(16) Ranked {
+    unsigned long long order, mass;  // the key, then the place in the list (the earlier the larger)
+  };
+  __shared__ Ranked s_rank[SMP_RANKED];
+  __shared__ uint32_t s_ends[2];
   __shared__ int s_at;
   __shared__ unsigned long long s_bin[3];
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -467,7 +536,7 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
     return;
   }
   __shared__ double s_table[64];
-  const SampleScale s = scale_of(a, row, s_table);
+  const SampleScale s = scale_of(a, row, (lds_double)s_table);
   if (s.top == -INFINITY) {
     if (tid == 0) a.token[row] = -1;
     return;
@@ -479,144 +548,177 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
   const float p = cut.p;
   __syncthreads();
 
-  // The border among the listed elements: the `want`-th of them (mass < 0), or the first at which their mass and base reach `target`.  Every
-  // round counts the elements of a range of keys in 2048 bins from above and goes on with one bin.
-  auto units = [&](float v) { return (unsigned long long)(s.weight(v) * a.unit + 0.5); };
-  auto border = [&](bool by_mass, unsigned long long want, double target, unsigned long long base) {
-    __syncthreads();
-    if (tid == 0) s_key[0] = 0xffffffffu, s_key[1] = 0;
-    __syncthreads();
-    uint32_t low = 0xffffffffu, high = 0;
+  // The border among the listed elements: the `want`-th of them, or the first at which their mass and base reach `target`.  While more than SMP_RANKED are
+  // left, every round counts a range of keys in SMP_BINS bins from above and goes on with one of them; the rest are ranked against one another.
+  auto units = [&](float v) { return s.units(v, a.unit); };
+  const bool kept_in_lds = r.listed <= SMP_HELD;
+  if (r.lo < SMP_STEPS && kept_in_lds) {
     for (uint32_t i = tid; i < r.listed; i += SMP_LAST) {
-      const uint32_t key = key_of(span.at((int)list[i]));
-      low = min(low, key), high = max(high, key);
+      const uint32_t index = list[i];
+      const float v = span.at((int)index);
+      s_index[i] = index;
+      s_element[i] = key_of(v);
+      s_of[i] = units(v);
     }
-    atomicMin(&s_key[0], low);
-    atomicMax(&s_key[1], high);
-    __syncthreads();
-    low = s_key[0], high = s_key[1];
+  }
+  auto element = [&](uint32_t i) { return kept_in_lds ? s_element[i] : key_of(span.at((int)list[i])); };
+  auto mass_of = [&](uint32_t i, uint32_t key) { return kept_in_lds ? s_of[i] : units(of_key(key)); };
+  auto index_of = [&](uint32_t i) {
+    if (!kept_in_lds) return (int)list[i];
+    int index = (int)s_index[i];
+    asm volatile("" : "+v"(index));  // (merged with the other load it would be one from a generic address)
+    return index;
+  };
+  auto border = [&](bool by_mass, unsigned long long want, double target, unsigned long long base) __attribute__((always_inline)) {
+    uint32_t low = 0, high = 0xffffffffu, in = r.listed;
     unsigned long long counted = 0, mass = base;
+    bool narrowed = false;
     for (;;) {
+      if (in <= SMP_RANKED) {
+        // ranks and masses in front, by comparing all with all; lanes of an element share the others
+        __syncthreads();
+        if (tid == 0) s_at = 0;
+        __syncthreads();
+        for (uint32_t i = tid; i < r.listed; i += SMP_LAST) {
+          const uint32_t key = element(i);
+          if (key < low || key > high) continue;
+          s_rank[atomicAdd(&s_at, 1)] = Ranked{(unsigned long long)key << 32 | (0xffffffffu - i), mass_of(i, key)};
+        }
+        if (tid < 2) s_bin[tid] = ~0ull;
+        __syncthreads();
+        const int n = (int)in;
+        int size = 16;
+        while (size < n) size <<= 1;
+        const int share_ = SMP_LAST / size, e = tid / share_;  // 2 .. 64 lanes
+        const bool live = e < n;
+        const Ranked own = s_rank[live ? e : 0];
+        uint32_t rank = 0;
+        unsigned long long before = 0;
+#pragma unroll 4
+        for (int i = tid % share_; i < n; i += share_) {
+          const Ranked o = s_rank[i];
+          const bool front = o.order > own.order;
+          rank += front;
+          before += front ? o.mass : 0;
+        }
+        for (int d = 1; d < share_; d <<= 1) {
+          rank += __shfl_xor(rank, d);
+          before += __shfl_xor(before, d);
+        }
+        before += mass;
+        if (live && tid % share_ == 0) {
+          // (a mass of nothing or less is reached in front of the first, which is kept all the same)
+          const bool it = by_mass ? (double)(before + own.mass) >= target && ((double)before < target || (rank == 0 && counted == 0)) : counted + rank + 1 == want;
+          if (it || rank + 1 == in) {
+            atomicMin(&s_bin[0], (unsigned long long)(it ? 0 : 1) << 32 | (0xffffffffu - (uint32_t)own.order));  // the last where rounding to units leaves it short of the target
+            if (it) s_bin[1] = before + own.mass;
+          }
+        }
+        __syncthreads();
+        const uint32_t i = (uint32_t)s_bin[0];
+        return SampleBorder{element(i), index_of(i), s_bin[1]};
+      }
+      if (!narrowed) {  // the ends of the keys
+        narrowed = true;
+        __syncthreads();
+        if (tid == 0) s_ends[0] = 0xffffffffu, s_ends[1] = 0;
+        __syncthreads();
+        uint32_t least = 0xffffffffu, most = 0;
+        for (uint32_t i = tid; i < r.listed; i += SMP_LAST) {
+          const uint32_t key = element(i);
+          least = min(least, key), most = max(most, key);
+        }
+#pragma unroll 1
+        for (int d = 32; d; d >>= 1) least = min(least, (uint32_t)__shfl_xor((int)least, d)), most = max(most, (uint32_t)__shfl_xor((int)most, d));
+        if (lane == 0) {
+          atomicMin(&s_ends[0], least);
+          atomicMax(&s_ends[1], most);
+        }
+        __syncthreads();
+        low = s_ends[0], high = s_ends[1];
+      }
       const uint32_t width = high - low;
-      const int bits = width ? 32 - __clz(width) : 0, shift = max(0, bits - 11);
+      const int bits = width ? 32 - __clz(width) : 0, shift = max(0, bits - SMP_BIN_BITS);
       __syncthreads();
       for (int i = tid; i < SMP_BINS; i += SMP_LAST) s_count[i] = 0, s_mass[i] = 0;
       if (tid == 0) s_at = SMP_BINS;
       __syncthreads();
       for (uint32_t i = tid; i < r.listed; i += SMP_LAST) {
-        const float v = span.at((int)list[i]);
-        const uint32_t key = key_of(v);
+        const uint32_t key = element(i);
         if (key < low || key > high) continue;
         const uint32_t bin = (high - key) >> shift;
         atomicAdd(&s_count[bin], 1u);
-        atomicAdd(&s_mass[bin], units(v));
+        atomicAdd(&s_mass[bin], mass_of(i, key));
       }
       __syncthreads();
-      const unsigned long long c0 = s_count[2 * tid], c1 = s_count[2 * tid + 1], m0 = s_mass[2 * tid], m1 = s_mass[2 * tid + 1];
-      const unsigned long long c = running<unsigned long long, SMP_LAST>(c0 + c1, s_wave) - c0 - c1 + counted, m = running<unsigned long long, SMP_LAST>(m0 + m1, s_wave) - m0 - m1 + mass;
-      const bool first = by_mass ? c0 && (double)(m + m0) >= target : c + c0 >= want, second = by_mass ? c1 && (double)(m + m0 + m1) >= target : c + c0 + c1 >= want;
-      if (first || second) atomicMin(&s_at, first ? 2 * tid : 2 * tid + 1);
-      __syncthreads();
-      const bool found = s_at < SMP_BINS;
-      if (!found && tid == 0) {  // (the mass falls short by what rounding to units took: everything)
-        s_bin[0] = counted, s_bin[1] = mass;
+      if (wave == 0) {  // a lane's bins, the lanes' sums, the lane that crosses, its bin
+        constexpr int PER = SMP_BINS / 64;
+        unsigned long long c = 0, m = 0;
+#pragma unroll 1
+        for (int j = 0; j < PER; j++) c += s_count[lane * PER + j], m += s_mass[lane * PER + j];
+        const unsigned long long own_c = c, own_m = m;
+#pragma unroll 1
+        for (int d = 1; d < 64; d <<= 1) {
+          const unsigned long long oc = __shfl_up(c, d), om = __shfl_up(m, d);
+          if (lane >= d) c += oc, m += om;
+        }
+        c += counted, m += mass;
+        const uint64_t over = __ballot(by_mass ? own_c && (double)m >= target : c >= want);
+        if (over && lane == __builtin_ctzll(over)) {
+          c -= own_c, m -= own_m;
+#pragma unroll 1
+          for (int j = lane * PER; j < (lane + 1) * PER; j++) {
+            const unsigned long long bc = s_count[j], bm = s_mass[j];
+            if (by_mass ? bc && (double)(m + bm) >= target : c + bc >= want) {
+              s_at = j;
+              s_bin[0] = c, s_bin[1] = m, s_bin[2] = bc;
+              break;
+            }
+            c += bc, m += bm;
+          }
+        }
       }
-      if (found && s_at >> 1 == tid) {
-        s_bin[0] = s_at & 1 ? c + c0 : c;
-        s_bin[1] = s_at & 1 ? m + m0 : m;
-        s_bin[2] = s_at & 1 ? c1 : c0;
-      }
       __syncthreads();
-      if (!found) return SampleBorder{low, 0xffffffffu, ~0ull};
+      const int found = s_at;
+      if (found == SMP_BINS) return SampleBorder{low, 0x7fffffff, ~0ull};  // (the mass falls short by what rounding to units took: everything)
       counted = s_bin[0], mass = s_bin[1];
-      const uint32_t in = (uint32_t)s_bin[2];
-      high -= (uint32_t)s_at << shift;
+      in = (uint32_t)s_bin[2];
+      high -= (uint32_t)found << shift;
       low = max(low, high - min(high, (1u << shift) - 1));
-      if (shift == 0) {
+      if (shift == 0 && in > SMP_RANKED) {  // very many equal logits: the first so many of them, found by their number in the list, which is in the order of the index
         const unsigned long long w = units(of_key(high));
         const double over = w ? ceil((target - (double)mass) / (double)w) : (double)in;
-        const uint32_t equals = by_mass ? (uint32_t)fmin(fmax(over, 1.0), (double)in) : (uint32_t)min((unsigned long long)in, want - counted);
-        return SampleBorder{high, equals, mass + w * equals};
+        const unsigned long long equals = by_mass ? (unsigned long long)fmin(fmax(over, 1.0), (double)in) : want - counted;
+        __syncthreads();
+        const uint32_t per = (r.listed + SMP_LAST - 1) / SMP_LAST, i0 = min(r.listed, tid * per), i1 = min(r.listed, i0 + per);
+        unsigned long long have = 0;
+        for (uint32_t i = i0; i < i1; i++) have += element(i) == high;
+        const unsigned long long up = running<unsigned long long, SMP_LAST>(have, s_wave);
+        if (up >= equals && up - have < equals) {
+          unsigned long long n = up - have;
+          for (uint32_t i = i0; i < i1; i++)
+            if (element(i) == high && ++n == equals) s_at = index_of(i);
+        }
+        __syncthreads();
+        return SampleBorder{high, s_at, mass + w * equals};
       }
     }
   };
   uint32_t edge_key = 0;  // what is above it is kept, and what equals it up to index `last`
   int last = 0x7fffffff;
-  if (r.lo < SMP_STEPS && r.listed <= SMP_RANKED) {
-    // Few: everyone's rank and the mass in front of it, by comparing all with all; lanes of an element share the others.
-    __shared__ unsigned long long s_of[SMP_RANKED];
-    __shared__ uint32_t s_element[SMP_RANKED];
-    int size = 16;
-    while (size < (int)r.listed) size <<= 1;
-    const int share_ = SMP_LAST / size, e = tid / share_, part = tid % share_;  // 2 .. 64 lanes
-    if (tid < SMP_RANKED) {
-      const float v = tid < (int)r.listed ? span.at((int)list[tid]) : -INFINITY;
-      s_element[tid] = key_of(v);
-      s_of[tid] = tid < (int)r.listed ? units(v) : 0;
-    }
-    if (tid < 2) s_key[tid] = 0;
-    if (tid < 3) s_bin[tid] = 0;
-    __syncthreads();
-    const uint32_t key = s_element[e];
-    const unsigned long long own = s_of[e];
-    uint32_t rank = 0;
-    unsigned long long before = 0;
-    for (int i = part; i < (int)r.listed; i += share_) {
-      const uint32_t o = s_element[i];
-      const bool front = o > key || (o == key && i < e);
-      rank += front;
-      before += front ? s_of[i] : 0;
-    }
-    for (int d = 1; d < share_; d <<= 1) {
-      rank += __shfl_xor(rank, d);
-      before += __shfl_xor(before, d);
-    }
-    rank += r.above;
-    before += r.mass_above;
-    const bool here = e < (int)r.listed && part == 0;
-    if (here && (r.cut ? rank == (uint32_t)cut.k - 1 : rank == r.above + r.listed - 1)) {  // the last that the count leaves: its number, the mass up to it
-      s_key[0] = e;
-      s_bin[0] = before + own;
-    }
-    __syncthreads();
-    const double target = (double)p * (double)(r.cut || cut.few ? s_bin[0] : r.mass);
-    if (cut.by_mass && here && (!r.cut || rank < (uint32_t)cut.k) && (double)before < target && (double)(before + own) >= target) {  // at most one
-      s_key[0] = e;
-      s_bin[1] = 1;
-    }
-    // (a mass of nothing or less is reached in front of the first, which is kept all the same)
-    if (cut.by_mass && here && rank == 0 && !(target > 0.0)) s_key[0] = e;
-    __syncthreads();
-    edge_key = s_element[s_key[0]];
-    last = (int)list[s_key[0]];
-  } else if (r.lo < SMP_STEPS) {
-    SampleBorder edge = {0, 0xffffffffu, 0};
+  if (r.lo < SMP_STEPS) {
+    // by count first, which says what the mass is that top-p takes its part of; without a k that cuts: all, and its mass is known
     unsigned long long mass = r.mass;
-    if (r.cut) {
-      edge = border(false, (unsigned long long)a.k[row] - r.above, 0.0, r.mass_above);
-      mass = edge.mass;
-    }
-    if (cut.by_mass) {
-      const SampleBorder e = border(true, 0, (double)p * (double)mass, r.mass_above);
-      if (!r.cut || e.key > edge.key || (e.key == edge.key && e.equals < edge.equals)) edge = e;
+    SampleBorder edge = {0, 0x7fffffff, 0};
+#pragma unroll 1
+    for (int by_mass = r.cut || cut.few ? 0 : 1; by_mass <= (cut.by_mass ? 1 : 0); by_mass++) {
+      const unsigned long long want = r.cut ? (unsigned long long)cut.k - r.above : r.listed;  // (few and not cut: fewer than k have a weight, and all are listed)
+      const SampleBorder e = border(by_mass, want, (double)p * (double)mass, r.mass_above);
+      if (e.key > edge.key || (e.key == edge.key && e.last < edge.last)) edge = e;
+      mass = e.mass;
     }
     edge_key = edge.key;
-    // the index of the last equal that is kept (the list is in the order of the index)
-    if (edge.equals != 0xffffffffu) {
-    __syncthreads();
-    if (tid == 0) s_at = 0x7fffffff;
-    const uint32_t per = (r.listed + SMP_LAST - 1) / SMP_LAST, i0 = min(r.listed, tid * per), i1 = min(r.listed, i0 + per);
-    unsigned long long have = 0;
-    for (uint32_t i = i0; i < i1; i++) have += key_of(span.at((int)list[i])) == edge.key;
-    const unsigned long long up = running<unsigned long long, SMP_LAST>(have, s_wave);
-    if (up >= edge.equals && up - have < edge.equals) {
-      unsigned long long n = up - have;
-      for (uint32_t i = i0; i < i1; i++)
-        if (key_of(span.at((int)list[i])) == edge.key && ++n == edge.equals) s_at = (int)list[i];
-    }
-    __syncthreads();
-    last = s_at;
-    }
+    last = edge.last;
   }
   auto kept = [&](int i, float v) {  // the weight of a kept element, 0 of another
     const int step = s.step_of(v);
@@ -628,66 +730,100 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
     const double w = s.weight(v);
     return s.heavy(w) ? w : 0.0;
   };
-  // sums of the pieces, and the one in which the running sum passes u of all
-  double target = 0.0, before = 0.0;
-  int piece = -1;
-  {
-    __shared__ double s_piece[64];
-    for (int i = wave; i < a.pieces; i += W) {
-      const uint32_t i0 = a.from[row * a.pieces + i], i1 = i + 1 < a.pieces ? a.from[row * a.pieces + i + 1] : r.listed;
-      double sum = 0.0;
-      if (r.lo < SMP_STEPS)
-        for (uint32_t j = i0 + lane; j < i1; j += 64) sum += kept((int)list[j], span.at((int)list[j]));
-#pragma unroll
-      for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-      if (lane == 0) s_piece[i] = sum + a.sum[row * a.pieces + i];
+  if (r.lo == 0 && r.listed <= SMP_LAST) {  // all that is kept is in the list: an element per thread
+    const double w = tid < (int)r.listed ? kept((int)s_index[tid], of_key(s_element[tid])) : 0.0;
+    const double up = running<double, SMP_LAST>(w, s_sum);
+    if (tid == 0) s_at = 0x7fffffff, s_ends[0] = 0;
+    double total = 0.0;
+    for (int i = 0; i < W; i++) total += s_sum[i];
+    __syncthreads();
+    if (w > 0.0) {
+      atomicMax(&s_ends[0], (uint32_t)tid);
+      if (up > (double)a.u[row] * total) atomicMin(&s_at, tid);
     }
     __syncthreads();
-    double total = 0.0, run = 0.0;
-    for (int i = 0; i < a.pieces; i++) total += s_piece[i];
-    target = (double)a.u[row] * total;
-    for (int i = 0; i < a.pieces; i++) {
-      const double next = run + s_piece[i];
-      if (s_piece[i] > 0.0 && (piece < 0 || !(before + s_piece[piece] > target))) piece = i, before = run;
-      run = next;
-    }
+    if (tid == 0) a.token[row] = (int)s_index[s_at < SMP_LAST ? s_at : s_ends[0]];
+    return;
   }
-  if (piece < 0) {
+  // sums of the parts that launch 3 had a wave for, and the part in which the running sum passes u of all
+  constexpr int WAVES = SMP_WG / 64;
+  __shared__ double s_part[SMP_PIECES * WAVES];
+  __shared__ double s_start[2];
+  const int parts = a.pieces * WAVES;
+  for (int i = wave; i < parts; i += W) {
+    const int at = row * parts + i;
+    const uint32_t i0 = a.from[at], i1 = i + 1 < parts ? a.from[at + 1] : r.listed;
+    double sum = 0.0;
+    if (r.lo < SMP_STEPS)
+      for (uint32_t j = i0 + lane; j < i1; j += 64) sum += kept(index_of(j), of_key(element(j)));
+    if (i1 - i0 > 1) {
+#pragma unroll 1
+      for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+    }
+    if (lane == 0) s_part[i] = sum + a.sum[at];
+  }
+  __syncthreads();
+  // lane by lane two parts each: the first lane, then its part, whose end is beyond the target; the last of all with anything where rounding says none
+  auto pick = [&](const double* part, int n, double target, double start) __attribute__((always_inline)) {
+    const double x0 = 2 * lane < n ? part[2 * lane] : 0.0, x1 = 2 * lane + 1 < n ? part[2 * lane + 1] : 0.0;
+    double up = x0 + x1;
+#pragma unroll 1
+    for (int d = 1; d < 64; d <<= 1) {
+      const double o = __shfl_up(up, d);
+      if (lane >= d) up += o;
+    }
+    if (target < 0.0) target = -target * __shfl(up, 63);  // (a part of all: below)
+    const double front = start + up - x0 - x1;
+    const bool first = x0 > 0.0 && front + x0 > target, second = x1 > 0.0 && start + up > target;
+    const uint64_t over = __ballot(first || second), any = __ballot(x0 > 0.0 || x1 > 0.0);
+    if (!any) return -1;
+    const int who = over ? __builtin_ctzll(over) : 63 - __clzll(any);
+    const bool one = over ? !first : x1 > 0.0;
+    if (lane == who) s_start[0] = one ? front + x0 : front, s_start[1] = target;
+    return 2 * who + (int)__shfl((int)one, who);
+  };
+  const double u = fmax((double)a.u[row], 1e-300);  // (0 asks for the first part with anything, as any number this small does)
+  if (wave == 0) {
+    const int at = pick(s_part, parts, -u, 0.0);
+    if (lane == 0) s_at = at;
+  }
+  __syncthreads();
+  const int part = s_at;
+  if (part < 0) {
     if (tid == 0) a.token[row] = -1;
     return;
   }
-  // the same among the piece's waves, then among the elements of one
-  int v0, v1;
-  share(span.vecs, a.pieces, piece, W, wave, v0, v1);
+  const double before = s_start[0], target = s_start[1];
+  // the same among the runs of the part that this kernel's waves have, then among the elements of one
+  SampleWalk<XT, 3> walk(span, s_x, a.pieces, part / WAVES, WAVES, part % WAVES);
+  {
+    const int each = (walk.v1 - walk.v0 + W * 64 - 1) / (W * 64) * 64, end = walk.v1;
+    walk.lds = s_x + wave * 3 * 64;
+    walk.v0 = min(end, walk.v0 + wave * each);
+    walk.v1 = min(end, walk.v0 + each);
+  }
   double sum = 0.0;
-  if (v1 >= 0)
-    span.walk(v0, v1, [&](int i, const float (&v)[N], int n) {
+  walk([&](int i, const float (&v)[N]) {
 #pragma unroll
-      for (int e = 0; e < N; e++)
-        if (e < n) sum += kept(i + e, v[e]);
-    });
+    for (int e = 0; e < N; e++) sum += kept(i + e, v[e]);
+  });
 #pragma unroll
   for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
   if (lane == 0) s_sum[wave] = sum;
   __syncthreads();
-  int chosen = -1;
-  double run = before, start = before;
-  for (int w = 0; w < W; w++) {
-    const double next = run + s_sum[w];
-    if (s_sum[w] > 0.0 && (chosen < 0 || !(start + s_sum[chosen] > target))) chosen = w, start = run;
-    run = next;
-  }
+  const int chosen = pick(s_sum, W, target, before);  // (every wave: it writes the same)
   if (chosen < 0 && tid == 0) a.token[row] = -1;
   if (wave != chosen) return;
+  const double start = s_start[0];
   int token = -1, at_last = -1;
   double passed = start;
-  span.walk(v0, v1, [&](int i, const float (&v)[N], int n) {
+  walk([&](int i, const float (&v)[N]) {
     if (token >= 0) return;
     double w[N], mine = 0.0;
     int heaviest = -1;
 #pragma unroll
     for (int e = 0; e < N; e++) {
-      w[e] = e < n ? kept(i + e, v[e]) : 0.0;
+      w[e] = kept(i + e, v[e]);
       mine += w[e];
       if (w[e] > 0.0) heaviest = i + e;
     }
@@ -727,7 +863,7 @@ static int sample_pieces(int64_t rows, int64_t V) {
 }
 static size_t sample_room(int64_t rows, int64_t V, int pieces) {
   const size_t rp = (size_t)rows * pieces;
-  return align_up(rp * (SMP_STEPS * 12 + 8 + 4 + 8 + 4) + (size_t)rows * sizeof(SampleRow), 16) + (size_t)rows * V * 4;
+  return align_up(rp * (SMP_STEPS * 12 + 12 + 12 * (SMP_WG / 64)) + (size_t)rows * sizeof(SampleRow), 16) + (size_t)rows * V * 4;
 }
 
 }  // namespace mllmhip
@@ -765,12 +901,12 @@ MLLM_API int mllm_hip_sample(const void* logits, int dtype, int64_t row_stride, 
   a.token = tokens;
   int bits = 0;
   while ((1ll << bits) < vocab) bits++;
-  a.unit = (double)(1ull << (62 - bits));
+  a.unit = (double)(1ull << (62 - bits < 51 ? 62 - bits : 51));
   const size_t rp = (size_t)rows * pieces;
   char* w = reinterpret_cast<char*>(workspace);
   a.mass = reinterpret_cast<uint64_t*>(w);
   a.sum = reinterpret_cast<double*>(w + rp * SMP_STEPS * 8);
-  a.row = reinterpret_cast<SampleRow*>(a.sum + rp);
+  a.row = reinterpret_cast<SampleRow*>(a.sum + rp * (SMP_WG / 64));
   a.count = reinterpret_cast<uint32_t*>(a.row + rows);
   a.ends = reinterpret_cast<float*>(a.count + rp * SMP_STEPS);
   a.top = reinterpret_cast<int*>(a.ends + 2 * rp);
