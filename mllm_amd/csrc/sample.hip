@@ -204,28 +204,39 @@ struct SampleScale {
   }
   __device__ __forceinline__ bool heavy(double w) const { return w > 0.0 && w >= (double)min_w; }
 };
+// What every launch reads of a row first, all of it asked for at once: settings, and a piece's ends per lane
+struct SampleIn {
+  float t, p, min_p, top, low;
+  int k;
+  __device__ __forceinline__ SampleIn(const SampleArgs& a, int row) {
+    const int lane = threadIdx.x & (SMP_PIECES - 1);  // every SMP_PIECES lanes have all pieces
+    const f32x2 ends = reinterpret_cast<const f32x2*>(a.ends)[row * a.pieces + min(lane, a.pieces - 1)];
+    t = a.t ? a.t[row] : 1.0f;
+    k = a.k ? a.k[row] : 0;
+    p = a.p ? a.p[row] : 1.0f;
+    min_p = a.min_p ? fminf(a.min_p[row], 1.0f) : 0.0f;
+    top = ends.x;
+    low = ends.y;
+  }
+  __device__ __forceinline__ bool greedy() const { return !(t > 0.f); }
+};
 // (the caller waits for the other waves before it takes a weight)
-__device__ __forceinline__ SampleScale scale_of(const SampleArgs& a, int row, lds_double table) {
+__device__ __forceinline__ SampleScale scale_of(const SampleIn& in, lds_double table) {
   SampleScale s;
   if (threadIdx.x < 64) table[threadIdx.x] = g_pow64[threadIdx.x];
   s.table = table;
-  float top = -INFINITY, low = INFINITY;
-  for (int i = threadIdx.x & 63; i < a.pieces; i += 64) {
-    top = fmaxf(top, a.ends[2 * (row * a.pieces + i)]);
-    low = fminf(low, a.ends[2 * (row * a.pieces + i) + 1]);
-  }
+  float top = in.top, low = in.low;
 #pragma unroll
-  for (int d = 32; d; d >>= 1) {
+  for (int d = SMP_PIECES / 2; d; d >>= 1) {
     top = fmaxf(top, __shfl_xor(top, d));
     low = fminf(low, __shfl_xor(low, d));
   }
-  const float t = a.t ? a.t[row] : 1.0f;
   s.top = top;
-  s.c = 92.332482616893656877 / (double)t;
+  s.c = 92.332482616893656877 / (double)in.t;
   s.infinite = top == INFINITY;
-  s.min_w = a.min_p ? fminf(a.min_p[row], 1.0f) : 0.0f;
+  s.min_w = in.min_p;
   // 52 ln 2 = 36.04 times t below the maximum weights end; a little more than the range, so that the last of it is in the last step
-  const float range = fminf(top - low, 36.05f * t) * 1.00001f;
+  const float range = fminf(top - low, 36.05f * in.t) * 1.00001f;
   s.step = range > 1e-30f ? (float)SMP_STEPS / range : 0.f;
   return s;
 }
@@ -234,17 +245,14 @@ struct SampleCut {
   int k;
   float p;
   bool by_count, by_mass, few;
+  __device__ __forceinline__ SampleCut(const SampleArgs& a, const SampleIn& in) {
+    k = in.k;
+    p = in.p;
+    by_count = k > 0 && k < a.V;
+    by_mass = p < 1.0f;
+    few = by_count && k <= SMP_FEW;
+  }
 };
-__device__ __forceinline__ SampleCut cut_of(const SampleArgs& a, int row) {
-  SampleCut c;
-  c.k = a.k ? a.k[row] : 0;
-  c.p = a.p ? a.p[row] : 1.0f;
-  c.by_count = c.k > 0 && c.k < a.V;
-  c.by_mass = c.p < 1.0f;
-  c.few = c.by_count && c.k <= SMP_FEW;
-  return c;
-}
-__device__ __forceinline__ bool greedy(const SampleArgs& a, int row) { return a.t && !(a.t[row] > 0.f); }
 
 // ---- 1: ends of every piece -------------------------------------------------------------------------------------------------
 template <int XT>
@@ -293,14 +301,14 @@ __global__ __launch_bounds__(SMP_WG) void sample_steps_kernel(SampleArgs a) {
   __shared__ uint32_t s_count[SMP_STEPS];
   __shared__ unsigned long long s_mass[SMP_STEPS];
   const int piece = blockIdx.x, row = blockIdx.y;
-  if (greedy(a, row)) return;
   __shared__ double s_table[64];
-  const SampleCut cut = cut_of(a, row);
-  if (!cut.by_count && !cut.by_mass) return;  // nothing is cut off
   const SampleSpan<XT> span(a, row);
   SampleWalk<XT, SMP_HOLD> walk(span, s_x, a.pieces, piece, SMP_WG / 64, threadIdx.x >> 6);
-  if (walk.v0 < walk.v1) walk.hold(walk.v0);  // asked for before the row's maximum
-  const SampleScale s = scale_of(a, row, (lds_double)s_table);
+  const SampleIn in(a, row);
+  const SampleCut cut(a, in);
+  if (walk.v0 < walk.v1) walk.hold(walk.v0);
+  if (in.greedy() || (!cut.by_count && !cut.by_mass)) return;  // nothing is cut off
+  const SampleScale s = scale_of(in, (lds_double)s_table);
   if (s.top == -INFINITY) return;
   const bool by_mass = cut.by_mass && !cut.few;
   for (int i = threadIdx.x; i < SMP_STEPS; i += SMP_WG) s_count[i] = 0, s_mass[i] = 0;
@@ -352,16 +360,15 @@ __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
   __shared__ uint32_t s_list[SMP_WG / 64];
   __shared__ float s_dense[SMP_WG * 2];
   const int piece = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if (greedy(a, row)) return;
   __shared__ double s_table[64];
-  const SampleCut cut = cut_of(a, row);
-  const int k = cut.k;
-  const float p = cut.p;
-  const bool by_count = cut.by_count, by_mass = cut.by_mass && !cut.few;
   const SampleSpan<XT> span(a, row);
   constexpr int N = SampleSpan<XT>::N;
   SampleWalk<XT, SMP_HOLD> walk(span, s_x, a.pieces, piece, SMP_WG / 64, wave);
-  if (walk.v0 < walk.v1) walk.hold(walk.v0);
+  const SampleIn given(a, row);
+  const SampleCut cut(a, given);
+  const int k = cut.k;
+  const float p = cut.p;
+  const bool by_count = cut.by_count, by_mass = cut.by_mass && !cut.few;
   // (all pieces' steps are on their way at once: one after the other they were 14 us)
   uint32_t counts_of[SMP_PIECES];
   unsigned long long mass_of[SMP_PIECES];
@@ -374,7 +381,9 @@ __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
       mass_of[i] = by_mass ? a.mass[from] : 0;
     }
   }
-  const SampleScale s = scale_of(a, row, (lds_double)s_table);
+  if (walk.v0 < walk.v1) walk.hold(walk.v0);
+  if (given.greedy()) return;
+  const SampleScale s = scale_of(given, (lds_double)s_table);
   if (s.top == -INFINITY) return;
   SampleRow r = {SMP_STEPS, SMP_STEPS, 0, 0, 0, 0, 0, 0};
   uint32_t mine = 0;  // elements of step tid in the pieces in front of this one
@@ -518,7 +527,10 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
   __shared__ int s_at;
   __shared__ unsigned long long s_bin[3];
   const int row = blockIdx.x, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  if (greedy(a, row)) {
+  const SampleIn in(a, row);
+  const SampleRow r = a.row[row];  // (launch 3 writes none for a row it has nothing to do for)
+  const float u_of = a.u[row];
+  if (in.greedy()) {
     if (wave) return;
     float top = -INFINITY;
     int at = 0x7fffffff;
@@ -536,15 +548,14 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
     return;
   }
   __shared__ double s_table[64];
-  const SampleScale s = scale_of(a, row, (lds_double)s_table);
+  const SampleScale s = scale_of(in, (lds_double)s_table);
   if (s.top == -INFINITY) {
     if (tid == 0) a.token[row] = -1;
     return;
   }
-  const SampleRow r = a.row[row];
   const SampleSpan<XT> span(a, row);
   const uint32_t* list = a.list + (int64_t)row * a.V;
-  const SampleCut cut = cut_of(a, row);
+  const SampleCut cut(a, in);
   const float p = cut.p;
   __syncthreads();
 
@@ -570,11 +581,11 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
     return index;
   };
   auto border = [&](bool by_mass, unsigned long long want, double target, unsigned long long base) __attribute__((always_inline)) {
-    uint32_t low = 0, high = 0xffffffffu, in = r.listed;
+    uint32_t low = 0, high = 0xffffffffu, left = r.listed;
     unsigned long long counted = 0, mass = base;
     bool narrowed = false;
     for (;;) {
-      if (in <= SMP_RANKED) {
+      if (left <= SMP_RANKED) {
         // ranks and masses in front, by comparing all with all; lanes of an element share the others
         __syncthreads();
         if (tid == 0) s_at = 0;
@@ -586,7 +597,7 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
         }
         if (tid < 2) s_bin[tid] = ~0ull;
         __syncthreads();
-        const int n = (int)in;
+        const int n = (int)left;
         int size = 16;
         while (size < n) size <<= 1;
         const int share_ = SMP_LAST / size, e = tid / share_;  // 2 .. 64 lanes
@@ -609,7 +620,7 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
         if (live && tid % share_ == 0) {
           // (a mass of nothing or less is reached in front of the first, which is kept all the same)
           const bool it = by_mass ? (double)(before + own.mass) >= target && ((double)before < target || (rank == 0 && counted == 0)) : counted + rank + 1 == want;
-          if (it || rank + 1 == in) {
+          if (it || rank + 1 == left) {
             atomicMin(&s_bin[0], (unsigned long long)(it ? 0 : 1) << 32 | (0xffffffffu - (uint32_t)own.order));  // the last where rounding to units leaves it short of the target
             if (it) s_bin[1] = before + own.mass;
           }
@@ -682,13 +693,13 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
       const int found = s_at;
       if (found == SMP_BINS) return SampleBorder{low, 0x7fffffff, ~0ull};  // (the mass falls short by what rounding to units took: everything)
       counted = s_bin[0], mass = s_bin[1];
-      in = (uint32_t)s_bin[2];
+      left = (uint32_t)s_bin[2];
       high -= (uint32_t)found << shift;
       low = max(low, high - min(high, (1u << shift) - 1));
-      if (shift == 0 && in > SMP_RANKED) {  // very many equal logits: the first so many of them, found by their number in the list, which is in the order of the index
+      if (shift == 0 && left > SMP_RANKED) {  // very many equal logits: the first so many of them, found by their number in the list, which is in the order of the index
         const unsigned long long w = units(of_key(high));
-        const double over = w ? ceil((target - (double)mass) / (double)w) : (double)in;
-        const unsigned long long equals = by_mass ? (unsigned long long)fmin(fmax(over, 1.0), (double)in) : want - counted;
+        const double over = w ? ceil((target - (double)mass) / (double)w) : (double)left;
+        const unsigned long long equals = by_mass ? (unsigned long long)fmin(fmax(over, 1.0), (double)left) : want - counted;
         __syncthreads();
         const uint32_t per = (r.listed + SMP_LAST - 1) / SMP_LAST, i0 = min(r.listed, tid * per), i1 = min(r.listed, i0 + per);
         unsigned long long have = 0;
@@ -739,7 +750,7 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
     __syncthreads();
     if (w > 0.0) {
       atomicMax(&s_ends[0], (uint32_t)tid);
-      if (up > (double)a.u[row] * total) atomicMin(&s_at, tid);
+      if (up > (double)u_of * total) atomicMin(&s_at, tid);
     }
     __syncthreads();
     if (tid == 0) a.token[row] = (int)s_index[s_at < SMP_LAST ? s_at : s_ends[0]];
@@ -782,7 +793,7 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
     if (lane == who) s_start[0] = one ? front + x0 : front, s_start[1] = target;
     return 2 * who + (int)__shfl((int)one, who);
   };
-  const double u = fmax((double)a.u[row], 1e-300);  // (0 asks for the first part with anything, as any number this small does)
+  const double u = fmax((double)u_of, 1e-300);  // (0 asks for the first part with anything, as any number this small does)
   if (wave == 0) {
     const int at = pick(s_part, parts, -u, 0.0);
     if (lane == 0) s_at = at;
