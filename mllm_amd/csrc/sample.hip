@@ -348,6 +348,23 @@ __device__ __forceinline__ T running(T v, T* s_wave) {
   return v;
 }
 
+// inclusive sums of counts and masses over the workgroup, thread by thread
+template <int WG>
+__device__ __forceinline__ void running2(uint32_t& c, unsigned long long& m, uint32_t* s_c, unsigned long long* s_m) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+  for (int d = 1; d < 64; d <<= 1) {
+    const uint32_t oc = __shfl_up(c, d);
+    const unsigned long long om = __shfl_up(m, d);
+    if (lane >= d) c += oc, m += om;
+  }
+  if (lane == 63) s_c[wave] = c, s_m[wave] = m;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < WG / 64; w++)
+    if (w < wave) c += s_c[w], m += s_m[w];
+}
+
 // ---- 3: the border's steps, sums in front of them, a list of what is in them ---------------------------------------------------
 template <int XT>
 __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
@@ -388,7 +405,8 @@ __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
   SampleRow r = {SMP_STEPS, SMP_STEPS, 0, 0, 0, 0, 0, 0};
   uint32_t mine = 0;  // elements of step tid in the pieces in front of this one
   if (by_count || by_mass) {
-    unsigned long long count = 0, mass = 0;
+    uint32_t count = 0;
+    unsigned long long mass = 0;
 #pragma unroll
     for (int i = 0; i < SMP_PIECES; i++) {
       if (i >= a.pieces) break;
@@ -396,13 +414,15 @@ __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
       count += counts_of[i];
       mass += mass_of[i];
     }
-    const unsigned long long counts = running<unsigned long long, SMP_WG>(count, s_wave), masses = running<unsigned long long, SMP_WG>(mass, s_wave);
-    s_count[tid] = (uint32_t)counts;
+    uint32_t counts = count;
+    unsigned long long masses = mass;
+    running2<SMP_WG>(counts, masses, s_list, s_wave);
+    s_count[tid] = counts;
     s_mass[tid] = masses;
     if (tid < 2) s_first[tid] = SMP_STEPS;
     __syncthreads();
     auto up_to = [&](int step, bool m) -> unsigned long long { return step <= 0 ? 0 : m ? s_mass[step - 1] : s_count[step - 1]; };  // in front of a step
-    if (by_count && counts >= (unsigned long long)k && counts - count < (unsigned long long)k) s_first[0] = tid;
+    if (by_count && counts >= (uint32_t)k && counts - count < (uint32_t)k) s_first[0] = tid;
     __syncthreads();
     r.cut = s_first[0] < SMP_STEPS;
     r.hi = s_first[0];
@@ -430,9 +450,15 @@ __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
     mine = tid >= r.lo && tid <= r.hi ? mine : 0;
   }
   // where this piece's part of the list begins (and the weights' table is there)
-  running<unsigned long long, SMP_WG>(mine, s_wave);
+#pragma unroll
+  for (int d = 32; d; d >>= 1) mine += __shfl_xor(mine, d);
+  __syncthreads();
+  if (lane == 0) s_list[wave] = mine;
+  __syncthreads();
   uint32_t from = 0;
-  for (int w = 0; w < SMP_WG / 64; w++) from += (uint32_t)s_wave[w];
+#pragma unroll
+  for (int w = 0; w < SMP_WG / 64; w++) from += s_list[w];
+  __syncthreads();
 
   // Where few elements are in front of the border a weight of each lane would be one of them at a time: they are collected, 64 and more, first.
   float* dense = s_dense + wave * 128;
@@ -530,6 +556,10 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
   const SampleIn in(a, row);
   const SampleRow r = a.row[row];  // (launch 3 writes none for a row it has nothing to do for)
   const float u_of = a.u[row];
+  constexpr int WAVES = SMP_WG / 64;  // of launch 3
+  const int part_of = row * a.pieces * WAVES + min(tid, a.pieces * WAVES - 1);
+  const double own_sum = a.sum[part_of];
+  const uint32_t own_from = a.from[part_of];
   if (in.greedy()) {
     if (wave) return;
     float top = -INFINITY;
@@ -757,21 +787,33 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
     return;
   }
   // sums of the parts that launch 3 had a wave for, and the part in which the running sum passes u of all
-  constexpr int WAVES = SMP_WG / 64;
   __shared__ double s_part[SMP_PIECES * WAVES];
+  __shared__ uint32_t s_from[SMP_PIECES * WAVES + 1];
   __shared__ double s_start[2];
   const int parts = a.pieces * WAVES;
-  for (int i = wave; i < parts; i += W) {
-    const int at = row * parts + i;
-    const uint32_t i0 = a.from[at], i1 = i + 1 < parts ? a.from[at + 1] : r.listed;
-    double sum = 0.0;
-    if (r.lo < SMP_STEPS)
-      for (uint32_t j = i0 + lane; j < i1; j += 64) sum += kept(index_of(j), of_key(element(j)));
-    if (i1 - i0 > 1) {
+  if (r.lo == SMP_STEPS) {
+    if (tid < parts) s_part[tid] = own_sum;
+  } else if (kept_in_lds) {  // every listed weight by a thread of its own, then every part by one
+    for (uint32_t i = tid; i < r.listed; i += SMP_LAST) s_of[i] = (unsigned long long)__double_as_longlong(kept((int)s_index[i], of_key(s_element[i])));
+    if (tid < parts) s_from[tid] = own_from;
+    if (tid == 0) s_from[parts] = r.listed;
+    __syncthreads();
+    if (tid < parts) {
+      double sum = own_sum;
+      for (uint32_t i = s_from[tid], end = s_from[tid + 1]; i < end; i++) sum += __longlong_as_double((long long)s_of[i]);
+      s_part[tid] = sum;
+    }
+  } else {
+    if (tid < parts) s_from[tid] = own_from, s_part[tid] = own_sum;
+    if (tid == 0) s_from[parts] = r.listed;
+    __syncthreads();
+    for (int i = wave; i < parts; i += W) {
+      double sum = 0.0;
+      for (uint32_t j = s_from[i] + lane; j < s_from[i + 1]; j += 64) sum += kept(index_of(j), of_key(element(j)));
 #pragma unroll 1
       for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+      if (lane == 0) s_part[i] += sum;
     }
-    if (lane == 0) s_part[i] = sum + a.sum[at];
   }
   __syncthreads();
   // lane by lane two parts each: the first lane, then its part, whose end is beyond the target; the last of all with anything where rounding says none
