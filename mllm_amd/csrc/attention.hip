@@ -13,8 +13,8 @@
 // A row's maximum, sum and the correction of O when the maximum grows are therefore numbers of a lane; sums over keys cross lanes twice per 32 keys
 // (the maximum) and once at the end (the sum).  Scores, maxima, sums and O are fp32.
 //
-// Roundings: bf16 queries as they are; P to bf16 for the product with V (off by 2^-9 of each weight, whose signs average; the sum takes P as it
-// was).  fp32 queries enter as three bf16 parts that add up to them (8 bits each, three products), P as two (2^-17 of each weight).
+// Roundings: bf16 queries as they are; P to bf16 for the product with V (off by 2^-8 of each weight at most, of either sign; the sum takes P as it
+// was).  fp32 queries and P enter as three bf16 parts each that add up to them (8 bits each, three products); products with fewer were off by 5e-6.
 //
 // A workgroup has four waves, WR along rows times 4 / WR along keys, and goes through a range of keys in tiles: 16-byte loads into registers while
 // the tile before them is worked on, from there into LDS.  Rows of a tile lie there with their 16-byte pieces exclusive-ored by bits of the
@@ -136,12 +136,23 @@ struct Attn {
   static constexpr int SUB = KT / (WK * 32);             // 32-key steps of a wave per tile
   static constexpr int C = D / 8;                        // 16-byte pieces of a row
   static constexpr int NLOAD = KT / 4 / 8;               // rows of a tile that a lane loads from
-  static constexpr int PARTS = F32 ? 3 : 1, PPARTS = F32 ? 2 : 1;
+  static constexpr int PARTS = F32 ? 3 : 1, PPARTS = F32 ? 3 : 1;
   static constexpr int ROWS = NQ * 16;                   // rows of a wave
   static constexpr int WAVES = D == 256 ? 1 : 2;         // per SIMD: all 512 registers for one, or 256 each
   static __device__ __forceinline__ int swz(int row) { return (C == 8) ? (row & 3) | ((row >> 3) & 1) << 2 : (row & 3) | ((row >> 3) & 3) << 2; }
 };
 
+// Two numbers as three bf16 each, cut off after 8 bits of what is left: together they are the numbers.
+__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
+  const uint32_t xh = __float_as_uint(x), yh = __float_as_uint(y);
+  const float x1 = x - __uint_as_float(xh & 0xffff0000u), y1 = y - __uint_as_float(yh & 0xffff0000u);
+  const uint32_t xm = __float_as_uint(x1), ym = __float_as_uint(y1);
+  const float x2 = x1 - __uint_as_float(xm & 0xffff0000u), y2 = y1 - __uint_as_float(ym & 0xffff0000u);
+  hi = __builtin_amdgcn_perm(yh, xh, 0x07060302u);  // the high halves of both
+  mid = __builtin_amdgcn_perm(ym, xm, 0x07060302u);
+  lo = __builtin_amdgcn_perm(__float_as_uint(y2), __float_as_uint(x2), 0x07060302u);
+}
+__device__ __forceinline__ float finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u ? 0.f : x; }
 // which of the keys k0 .. k0 + 7 token `token` of the sequence sees
 __device__ __forceinline__ uint32_t seen_keys(const AttnArgs& a, const Seq& s, int k0, int token) {
   uint32_t see = 0;
@@ -174,7 +185,7 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
   constexpr int KT = P::KT, C = P::C, WK = P::WK, NLOAD = P::NLOAD, KS = D / 32, DT = D / 16;
   __shared__ __align__(16) uint16_t s_k[KT * D];
   __shared__ __align__(16) uint16_t s_v[KT * D];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, wr = wave % WR, wk = wave / WR;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave % WR, wk = wave / WR;
   const int col = lane & 15, g = lane >> 4;
   const int rows = s.n * a.group, row0 = rt * P::ROWS * WR;
   if (row0 >= rows) return;
@@ -218,27 +229,15 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
       item_load<F32 ? MLLM_HIP_F32 : MLLM_HIP_BF16>(a.q, at + 32 * ks, it);
       if (!F32) {
         fq[0][i][ks] = frag(it.r[0]);
-      } else {  // x = hi + mid + lo, each cut off after 8 bits; what is no number or infinite is all in hi
+      } else {
         float v[8];
         item_to_f32<F32 ? MLLM_HIP_F32 : MLLM_HIP_BF16>(it, v);
         uint32_t part[3][4];
 #pragma unroll
         for (int j = 0; j < 4; j++) {
-          uint32_t bits[3][2];
-#pragma unroll
-          for (int e = 0; e < 2; e++) {
-            const float x = v[2 * j + e];
-            const uint32_t hi = __float_as_uint(x) & 0xffff0000u;
-            const bool finite = (hi & 0x7f800000u) != 0x7f800000u;
-            const float r1 = finite ? x - __uint_as_float(hi) : 0.f;
-            const uint32_t mid = __float_as_uint(r1) & 0xffff0000u;
-            const float r2 = r1 - __uint_as_float(mid);
-            bits[0][e] = !finite && x != x ? 0x7fc00000u : hi;
-            bits[1][e] = mid;
-            bits[2][e] = __float_as_uint(r2) & 0xffff0000u;
-          }
-#pragma unroll
-          for (int p = 0; p < 3; p++) part[p][j] = bits[p][0] >> 16 | bits[p][1];
+          split2(finite(v[2 * j]), finite(v[2 * j + 1]), part[0][j], part[1][j], part[2][j]);
+          // (what is no number or infinite: all in the first part)
+          part[0][j] = (finite(v[2 * j]) == v[2 * j] ? part[0][j] & 0xffffu : f32_to_bf16(v[2 * j])) | (finite(v[2 * j + 1]) == v[2 * j + 1] ? part[0][j] & 0xffff0000u : (uint32_t)f32_to_bf16(v[2 * j + 1]) << 16);
         }
 #pragma unroll
         for (int p = 0; p < P::PARTS; p++) fq[p][i][ks] = frag(u32x4{part[p][0], part[p][1], part[p][2], part[p][3]});
@@ -275,9 +274,14 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
     for (int d = 0; d < DT; d++) acc[i][d] = at_f32x4{0.f, 0.f, 0.f, 0.f};
   }
 
-  if (k_begin < k_end) {
-    ask_tile(k_begin);
-  }
+  if (k_begin < k_end) ask_tile(k_begin);
+  // Q is here from now on: a wait for it in the loops would be one for the loads of the next tile, which come behind it
+#pragma unroll
+  for (int p = 0; p < P::PARTS; p++)
+#pragma unroll
+    for (int i = 0; i < NQ; i++)
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) asm volatile("" : "+v"(fq[p][i][ks]));
   bool odd = false;  // infinities or NaNs among the values of this wave's new tokens
   // the products of a tile; `border`: new tokens, or keys behind the last
   auto work = [&](int k0, auto border_) {
@@ -326,21 +330,16 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
         }
         const float ref = m[i] == -INFINITY ? 0.f : m[i];  // (nothing seen yet: every p is exp2(-inf))
 #pragma unroll
-        for (int j = 0; j < 8; j++) {
-          y[j] = __builtin_amdgcn_exp2f(fmaf(y[j], a.c, -ref));
-          l[i] += y[j];
-        }
+        for (int j = 0; j < 8; j++) y[j] = __builtin_amdgcn_exp2f(fmaf(y[j], a.c, -ref));
+        l[i] += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
         if (!F32) {
           fp[0][i] = frag(u32x4{pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7])});
         } else {
-          float lo[8];
-          uint32_t hi[4];
+          uint32_t part[3][4];
 #pragma unroll
-          for (int j = 0; j < 8; j++) lo[j] = y[j] - __uint_as_float(__float_as_uint(y[j]) & 0xffff0000u);
+          for (int j = 0; j < 4; j++) split2(y[2 * j], y[2 * j + 1], part[0][j], part[1][j], part[2][j]);
 #pragma unroll
-          for (int j = 0; j < 4; j++) hi[j] = __float_as_uint(y[2 * j]) >> 16 | (__float_as_uint(y[2 * j + 1]) & 0xffff0000u);
-          fp[0][i] = frag(u32x4{hi[0], hi[1], hi[2], hi[3]});
-          fp[P::PPARTS - 1][i] = frag(u32x4{pack_bf16(lo[0], lo[1]), pack_bf16(lo[2], lo[3]), pack_bf16(lo[4], lo[5]), pack_bf16(lo[6], lo[7])});
+          for (int p = 0; p < P::PPARTS; p++) fp[p][i] = frag(u32x4{part[p][0], part[p][1], part[p][2], part[p][3]});
         }
       }
       // V^T: lane i of 16 asks for elements 4 (i % 4) .. + 3 of key 8 g + i / 4 and gets element i of keys 8 g .. + 3
