@@ -134,6 +134,7 @@ struct Attn {
   static constexpr int WK = 4 / WR;                      // waves along keys
   static constexpr int KT = WK * 32 < 64 ? 64 : WK * 32;  // keys of a tile
   static constexpr int SUB = KT / (WK * 32);             // 32-key steps of a wave per tile
+  static constexpr bool TWO = KT == 64;                  // two tiles in LDS, one barrier each (tiles of 128 keys leave no room for that and a second workgroup)
   static constexpr int C = D / 8;                        // 16-byte pieces of a row
   static constexpr int NLOAD = KT / 4 / 8;               // rows of a tile that a lane loads from
   static constexpr int PARTS = F32 ? 3 : 1, PPARTS = F32 ? 3 : 1;
@@ -183,8 +184,8 @@ template <int D, int NQ, int WR, bool F32>
 __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s, int b, int h, int rt, int k_begin, int k_end, int range, int count) {
   typedef Attn<D, NQ, WR, F32> P;
   constexpr int KT = P::KT, C = P::C, WK = P::WK, NLOAD = P::NLOAD, KS = D / 32, DT = D / 16;
-  __shared__ __align__(16) uint16_t s_k[KT * D];
-  __shared__ __align__(16) uint16_t s_v[KT * D];
+  __shared__ __align__(16) uint16_t s_k[(P::TWO ? 2 : 1) * KT * D];
+  __shared__ __align__(16) uint16_t s_v[(P::TWO ? 2 : 1) * KT * D];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave % WR, wk = wave / WR;
   const int col = lane & 15, g = lane >> 4;
   const int rows = s.n * a.group, row0 = rt * P::ROWS * WR;
@@ -283,10 +284,11 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
 #pragma unroll
       for (int ks = 0; ks < KS; ks++) asm volatile("" : "+v"(fq[p][i][ks]));
   bool odd = false;  // infinities or NaNs among the values of this wave's new tokens
-  // the products of a tile; `border`: new tokens, or keys behind the last
-  auto work = [&](int k0, auto border_) {
+  // the products of a tile, which is in that half of LDS; `border`: new tokens, or keys behind the last
+  const bool busy = row0 + wr * P::ROWS < rows;  // (a wave without rows loads with the others and leaves its SIMD to them)
+  auto work = [&](int k0, auto border_, auto half) {
     constexpr bool border = decltype(border_)::value;
-#pragma unroll 1
+#pragma unroll
     for (int u = 0; u < P::SUB; u++) {
       const int base = (u * WK + wk) * 32;  // the step's first row in the tile
       const int key0 = k0 + base;
@@ -294,7 +296,7 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
       at_f32x4 sa[NQ], sb[NQ];
 #pragma unroll
       for (int i = 0; i < NQ; i++) sa[i] = sb[i] = at_f32x4{0.f, 0.f, 0.f, 0.f};
-      const int ra = base + 8 * (col >> 2) + (col & 3), x = P::swz(ra);
+      const int ra = half * KT + base + 8 * (col >> 2) + (col & 3), x = P::swz(ra);
 #pragma unroll
       for (int ks = 0; ks < KS; ks++) {
         const int at = ra * D + ((4 * ks + g) ^ x) * 8;
@@ -343,7 +345,7 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
         }
       }
       // V^T: lane i of 16 asks for elements 4 (i % 4) .. + 3 of key 8 g + i / 4 and gets element i of keys 8 g .. + 3
-      const int rv0 = base + 8 * g + (col >> 2), xv = P::swz(rv0);
+      const int rv0 = half * KT + base + 8 * g + (col >> 2), xv = P::swz(rv0);
 #pragma unroll
       for (int d = 0; d < DT; d++) {
         const int at = rv0 * D + ((2 * d + ((col & 3) >> 1)) ^ xv) * 8 + (col & 1) * 4;
@@ -366,30 +368,61 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
       }
     }
   };
-  // tiles from k0 on: of prefix keys alone, then (a loop of its own: its masks would take registers from the other) the rest
-  int k0 = k_begin;
-  auto tiles = [&](int end, auto border_) {
-   for (; k0 < end; k0 += KT) {
-    __syncthreads();  // the tile before this one has been read
+  auto put_tile = [&](auto half) {
 #pragma unroll
     for (int i = 0; i < NLOAD; i++) {
       const int row = load_row(i);
 #pragma unroll
       for (int j = 0; j < C / 8; j++) {
-        const int at = row * D + ((lane % 8 + 8 * j) ^ P::swz(row)) * 8;
+        const int at = half * (KT * D) + row * D + ((lane % 8 + 8 * j) ^ P::swz(row)) * 8;
         *reinterpret_cast<u32x4*>(s_k + at) = rk[i][j];
         *reinterpret_cast<u32x4*>(s_v + at) = rv[i][j];
       }
     }
-    __syncthreads();
-    if (k0 + KT < k_end) {
-      ask_tile(k0 + KT);
-    }
-    work(k0, border_);
-   }
   };
-  tiles(min(s.prefix, k_end) - KT + 1, std::false_type());
-  tiles(k_end, std::true_type());
+  typedef std::integral_constant<int, 0> Lower;
+  typedef std::integral_constant<int, P::TWO ? 1 : 0> Upper;
+  int k0 = k_begin;  // the tile that is worked on
+  if constexpr (P::TWO) {
+    if (k_begin < k_end) {
+      __syncthreads();  // what this workgroup had in LDS before has been read
+      put_tile(Lower());
+      if (k_begin + KT < k_end) ask_tile(k_begin + KT);
+      __syncthreads();
+    }
+    auto turn = [&](auto border_, auto half, auto other) {
+      if (busy) work(k0, border_, half);
+      k0 += KT;
+      if (k0 < k_end) {  // into the other half of LDS: everyone is past the tile that was there
+        put_tile(other);
+        if (k0 + KT < k_end) ask_tile(k0 + KT);
+        __syncthreads();
+      }
+    };
+    // Tiles of prefix keys alone, in turns whose halves of LDS are constants; then (a loop of its own: its masks would take registers from the other) the rest.
+    const int plain = min(s.prefix, k_end) - KT;  // the last tile that may begin there
+    int half = 0;
+    while (k0 <= plain) {
+      turn(std::false_type(), Lower(), Upper());
+      half = 1;
+      if (k0 > plain) break;
+      turn(std::false_type(), Upper(), Lower());
+      half = 0;
+    }
+    for (; k0 < k_end; half ^= 1) turn(std::true_type(), half, half ^ 1);
+  } else {
+    auto turn = [&](auto border_) {
+      __syncthreads();  // the tile before this one has been read
+      put_tile(Lower());
+      __syncthreads();
+      if (k0 + KT < k_end) ask_tile(k0 + KT);
+      work(k0, border_, Lower());
+      k0 += KT;
+    };
+    const int plain = min(s.prefix, k_end) - KT;
+    while (k0 <= plain) turn(std::false_type());
+    while (k0 < k_end) turn(std::true_type());
+  }
   if (odd) {  // they reach the rows that see them whatever the weight (of 0 or more): no product is needed
 #pragma unroll 1
     for (int key = max(s.prefix, k_begin); key < k_end; key++) {
