@@ -132,9 +132,8 @@ __device__ __forceinline__ at_f32x4 mma(at_bf16x8 x, at_bf16x8 y, at_f32x4 acc) 
 template <int D, int NQ, int WR, bool F32>
 struct Attn {
   static constexpr int WK = 4 / WR;                      // waves along keys
-  static constexpr int KT = WK * 32 < 64 ? 64 : WK * 32;  // keys of a tile
+  static constexpr int KT = 64;                          // keys of a tile
   static constexpr int SUB = KT / (WK * 32);             // 32-key steps of a wave per tile
-  static constexpr bool TWO = KT == 64;                  // two tiles in LDS, one barrier each (tiles of 128 keys leave no room for that and a second workgroup)
   static constexpr int C = D / 8;                        // 16-byte pieces of a row
   static constexpr int NLOAD = KT / 4 / 8;               // rows of a tile that a lane loads from
   static constexpr int PARTS = F32 ? 3 : 1, PPARTS = F32 ? 3 : 1;
@@ -184,8 +183,8 @@ template <int D, int NQ, int WR, bool F32>
 __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s, int b, int h, int rt, int k_begin, int k_end, int range, int count) {
   typedef Attn<D, NQ, WR, F32> P;
   constexpr int KT = P::KT, C = P::C, WK = P::WK, NLOAD = P::NLOAD, KS = D / 32, DT = D / 16;
-  __shared__ __align__(16) uint16_t s_k[(P::TWO ? 2 : 1) * KT * D];
-  __shared__ __align__(16) uint16_t s_v[(P::TWO ? 2 : 1) * KT * D];
+  __shared__ __align__(16) uint16_t s_k[2 * KT * D];
+  __shared__ __align__(16) uint16_t s_v[2 * KT * D];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave % WR, wk = wave / WR;
   const int col = lane & 15, g = lane >> 4;
   const int rows = s.n * a.group, row0 = rt * P::ROWS * WR;
@@ -381,47 +380,36 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
     }
   };
   typedef std::integral_constant<int, 0> Lower;
-  typedef std::integral_constant<int, P::TWO ? 1 : 0> Upper;
+  typedef std::integral_constant<int, 1> Upper;
   int k0 = k_begin;  // the tile that is worked on
-  if constexpr (P::TWO) {
-    if (k_begin < k_end) {
-      __syncthreads();  // what this workgroup had in LDS before has been read
-      put_tile(Lower());
-      if (k_begin + KT < k_end) ask_tile(k_begin + KT);
-      __syncthreads();
-    }
-    auto turn = [&](auto border_, auto half, auto other) {
-      if (busy) work(k0, border_, half);
-      k0 += KT;
-      if (k0 < k_end) {  // into the other half of LDS: everyone is past the tile that was there
-        put_tile(other);
-        if (k0 + KT < k_end) ask_tile(k0 + KT);
-        __syncthreads();
-      }
-    };
-    // Tiles of prefix keys alone, in turns whose halves of LDS are constants; then (a loop of its own: its masks would take registers from the other) the rest.
-    const int plain = min(s.prefix, k_end) - KT;  // the last tile that may begin there
-    int half = 0;
-    while (k0 <= plain) {
-      turn(std::false_type(), Lower(), Upper());
-      half = 1;
-      if (k0 > plain) break;
-      turn(std::false_type(), Upper(), Lower());
-      half = 0;
-    }
-    for (; k0 < k_end; half ^= 1) turn(std::true_type(), half, half ^ 1);
-  } else {
-    auto turn = [&](auto border_) {
-      __syncthreads();  // the tile before this one has been read
-      put_tile(Lower());
-      __syncthreads();
+  if (k_begin < k_end) {
+    __syncthreads();  // what this workgroup had in LDS before has been read
+    put_tile(Lower());
+    if (k_begin + KT < k_end) ask_tile(k_begin + KT);
+    __syncthreads();
+  }
+  auto turn = [&](auto border_, auto half, auto other) {
+    if (busy) work(k0, border_, half);
+    k0 += KT;
+    if (k0 < k_end) {  // into the other half of LDS: everyone is past the tile that was there
+      put_tile(other);
       if (k0 + KT < k_end) ask_tile(k0 + KT);
-      work(k0, border_, Lower());
-      k0 += KT;
-    };
-    const int plain = min(s.prefix, k_end) - KT;
-    while (k0 <= plain) turn(std::false_type());
-    while (k0 < k_end) turn(std::true_type());
+      __syncthreads();
+    }
+  };
+  // Tiles of prefix keys alone, in turns whose halves of LDS are constants; then (a loop of its own: its masks would take registers from the other) the rest.
+  const int plain = min(s.prefix, k_end) - KT;  // the last tile that may begin there
+  int half = 0;
+  while (k0 <= plain) {
+    turn(std::false_type(), Lower(), Upper());
+    half = 1;
+    if (k0 > plain) break;
+    turn(std::false_type(), Upper(), Lower());
+    half = 0;
+  }
+  while (k0 < k_end) {
+    turn(std::true_type(), half, half ^ 1);
+    half ^= 1;
   }
   if (odd) {  // they reach the rows that see them whatever the weight (of 0 or more): no product is needed
 #pragma unroll 1
@@ -633,20 +621,23 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a) {
 struct AttnPlan {
   int nq, wr, row_tiles, ranges, min_tiles;
 };
-// Rows of a workgroup by the rows there are (tokens times query heads of a key head).  Keys are cut while the workgroups without that are under 1024, into
-// ranges that give every CU two workgroups, of twice as many keys as rows at least: what a range hands over is rows, what it reads keys.
+// Rows of a workgroup by the rows there are (tokens times query heads of a key head): 32 rows a wave (16 with fp32 queries, whose parts, and with heads of 256,
+// whose O takes the registers), waves along rows before waves along keys.  Keys are cut while there are under 1024 workgroups without that and more than
+// four tiles of keys, into ranges that give every CU two workgroups, of twice as many keys as rows at least: what a range hands over is rows, what it
+// reads keys.  One token of 32 heads, uncut / cut, us: 128 keys 7.8 / 10.1, 256 9.4 / 10.5, 320 10.4 / 11.1, 500 13.2 / 10.4, 768 16.8 / 10.5.
+// The second launch, which joins the ranges, is what cutting costs (4 of them).
 static AttnPlan attention_plan(bool f32, int64_t B, int heads, int kv, int64_t max_tokens, int64_t max_keys, int D) {
   AttnPlan p;
   const int64_t rows = max_tokens * (heads / kv);
   p.nq = rows <= 32 || f32 || D == 256 ? 1 : 2;
-  p.wr = rows <= 16 && D < 256 ? 1 : rows <= 32 || (rows <= 64 && p.nq == 2) ? 2 : 4;
+  p.wr = rows <= 32 || (rows <= 64 && p.nq == 2) ? 2 : 4;
   const int64_t per = (int64_t)p.nq * 16 * p.wr;
   const int64_t row_tiles = (rows + per - 1) / per;
   p.row_tiles = (int)row_tiles;
-  const int kt = p.wr == 1 ? 128 : 64;
+  const int kt = 64;
   p.min_tiles = (int)((2 * (rows < per ? rows : per) + kt - 1) / kt);
   const int64_t most = B * ((max_keys + p.min_tiles * kt - 1) / (p.min_tiles * kt)), wanted = (512 + kv * row_tiles - 1) / (kv * row_tiles);
-  p.ranges = B * kv * row_tiles >= 1024 || max_keys <= (int64_t)p.min_tiles * kt ? 0 : (int)(wanted < most ? wanted : most);
+  p.ranges = B * kv * row_tiles >= 1024 || max_keys <= 4 * kt ? 0 : (int)(wanted < most ? wanted : most);
   if (p.ranges <= 1 && B == 1) p.ranges = 0;
   return p;
 }
@@ -714,7 +705,7 @@ MLLM_API int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_
   a.page_bytes = (uint32_t)(cache->page_stride * 2);
   a.slot_bytes = (uint32_t)(cache->slot_stride * 2);
   a.page_end = cache->page_size == 1 ? 1 : (uint32_t)(cache->page_size * cache->slot_stride * 2);  // (a page of one slot: `in` stays 0)
-  const int kt = p.wr == 1 ? 128 : 64;
+  const int kt = 64;
   a.step_pages = (uint32_t)(kt / cache->page_size);
   a.step_bytes = (uint32_t)(kt % cache->page_size * cache->slot_stride * 2);
   a.head_stride = cache->head_stride;
@@ -753,9 +744,9 @@ MLLM_API int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a); };
 #define ATTN(D_, NQ_, WR_, F_) \
   case NQ_ * 10 + WR_: go(attention_kernel<D_, NQ_, WR_, F_>); break;
-#define ATTN_D(D_)                                                                                        \
-  if (f32) switch (form) { ATTN(D_, 1, 1, true) ATTN(D_, 1, 2, true) ATTN(D_, 1, 4, true) }                \
-  else switch (form) { ATTN(D_, 1, 1, false) ATTN(D_, 1, 2, false) ATTN(D_, 2, 2, false) ATTN(D_, 2, 4, false) }
+#define ATTN_D(D_)                                                                            \
+  if (f32) switch (form) { ATTN(D_, 1, 2, true) ATTN(D_, 1, 4, true) }                        \
+  else switch (form) { ATTN(D_, 1, 2, false) ATTN(D_, 2, 2, false) ATTN(D_, 2, 4, false) }
   if (D == 64) {
     ATTN_D(64)
   } else if (D == 128) {
