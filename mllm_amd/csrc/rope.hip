@@ -18,12 +18,12 @@ struct RopeGroup {
   void* y;
   const float* w;
   int64_t x_token, x_head, y_token, y_head;
-  int head0, kind;
+  int heads, unit0, kind;  // unit0: the part's first unit of as many heads as a wave has at a time
 };
 struct RopeArgs {
   RopeGroup part[4];
-  int nparts, heads, D, rot, passes, add_unit_offset;
-  float eps;
+  int nparts, units, D, rot, passes, add_unit_offset;
+  float eps, inv_d;
   const int32_t* positions;
   const double* inv_freq;
   // the cache's addressing
@@ -32,97 +32,130 @@ struct RopeArgs {
   uint32_t page;
 };
 
-// G lanes per head of up to 8 * G elements, 256 / G heads of a token at a time
+// The value of the lane L away on the other side of a group of 2 L (L a power of two): lane ^ L
+template <int L>
+__device__ __forceinline__ float across(float v) {
+  if (L == 1) return dpp_f<0xB1>(v);                 // quad_perm [1,0,3,2]
+  if (L == 2) return dpp_f<0x4E>(v);                 // quad_perm [2,3,0,1]
+  if (L == 4) return dpp_f<0x1B>(dpp_f<0x141>(v));   // mirrored in eight, then in four
+  if (L == 8) return dpp_f<0x128>(v);                // turned by eight of sixteen
+  const u32x2 r = L == 16 ? lanes16(__float_as_uint(v)) : lanes32(__float_as_uint(v));
+  const int lane = threadIdx.x & 63;
+  return __uint_as_float(lane & L ? r.x : r.y);
+}
+
+// G lanes per head of up to 8 * G elements.  A wave has 64 / G heads of one part at a time -- addresses are numbers of the scalar unit -- and goes through
+// `passes` of them, up to ROPE_AHEAD on their way from memory at once.
+enum { ROPE_AHEAD = 3 };
 template <int XT, int G, bool NEXT>
 __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
-  __shared__ float s_cos[256], s_sin[256];
-  const int tid = threadIdx.x, lane = tid & 63, lg = tid % G, e = lg * 8;
+  __shared__ __align__(16) float s_cos[256];
+  __shared__ __align__(16) float s_sin[256];
+  constexpr int H = 64 / G;
+  const int tid = threadIdx.x, lane = tid & 63, lg = lane % G, e = lg * 8;
   const int64_t t = blockIdx.x;
   const int half = a.rot / 2;
-  int head = blockIdx.y * a.passes * (256 / G) + tid / G;
-  // (selects between scalar registers: a part looked up by a lane's index would be loads in front of the first load)
-  auto part_of = [&](int h) {
-    RopeGroup g = a.part[0];
+  const int unit0 = (blockIdx.y * a.passes) * 4 + __builtin_amdgcn_readfirstlane(tid >> 6);  // of H heads
+  struct Part {
+    RopeGroup g;
+    int head;  // this lane's, of the part
+    bool live;
+  };
+  auto part_of = [&](int unit) {
+    Part p;
+    p.g = a.part[0];
 #pragma unroll
     for (int j = 1; j < 4; j++)
-      if (j < a.nparts && h >= a.part[j].head0) g = a.part[j];
-    return g;
+      if (j < a.nparts && unit >= a.part[j].unit0) p.g = a.part[j];
+    p.head = (unit - p.g.unit0) * H + lane / G;
+    p.live = unit < a.units && p.head < p.g.heads && e < a.D;
+    return p;
   };
-  auto load = [&](int h, Item8<XT>& it) {
-    const RopeGroup g = part_of(h);
-    if (h < a.heads && e < a.D) item_load<XT>(g.x, t * g.x_token + (h - g.head0) * g.x_head + e, it);
-  };
-  Item8<XT> it = {};
-  load(head, it);
-  const int64_t slot = a.slots ? a.slots[t] : -1;
-  if (half > 0) {
-    if (tid < half) {
-      // turns in fp64: p * f is off by 2^-53 of itself, which at 2^20 radians is 1e-10
-      double turn = (double)a.positions[t] * a.inv_freq[tid] * 0.15915494309189533577;
-      turn -= rint(turn);
-      float sn, cs;
-      sincospif(2.0f * (float)turn, &sn, &cs);
-      s_cos[tid] = cs;
-      s_sin[tid] = sn;
+  int64_t stored = -1;  // where the token's slot is in the cache
+  if (a.slots) {
+    const int64_t slot = a.slots[t];
+    if (slot >= 0 && slot < a.slot_count) {
+      const uint32_t page = (uint32_t)slot / a.page;
+      stored = page * a.page_stride + ((uint32_t)slot - page * a.page) * a.slot_stride;
     }
-    __syncthreads();
   }
-  for (int p = 0; p < a.passes; p++, head += 256 / G) {
-    const int h = head;
-    float v[8];
-    item_to_f32<XT>(it, v);
-    if (p + 1 < a.passes) load(h + 256 / G, it);
-    if (h - tid / G >= a.heads) return;  // (no head of this workgroup is left)
-    const bool live = h < a.heads && e < a.D;
-    const RopeGroup g = part_of(h);
-    if (!live) {
+  for (int p0 = 0; p0 < a.passes; p0 += ROPE_AHEAD) {
+    Item8<XT> it[ROPE_AHEAD] = {};
 #pragma unroll
-      for (int j = 0; j < 8; j++) v[j] = 0.f;
+    for (int p = 0; p < ROPE_AHEAD; p++) {
+      if (p0 + p >= a.passes) break;
+      const Part q = part_of(unit0 + (p0 + p) * 4);
+      if (q.live) item_load<XT>(q.g.x, t * q.g.x_token + q.head * q.g.x_head + e, it[p]);
     }
-    float ss = 0.f;
-#pragma unroll
-    for (int j = 0; j < 8; j++) ss = fmaf(v[j], v[j], ss);
-    ss = group_sum<G>(ss);
-    if (live && g.w) {
-      const float rms = 1.0f / sqrtf(ss / (float)a.D + a.eps);
-      const float4 w0 = *reinterpret_cast<const float4*>(g.w + e), w1 = *reinterpret_cast<const float4*>(g.w + e + 4);
-      const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
-#pragma unroll
-      for (int j = 0; j < 8; j++) v[j] = v[j] * ((a.add_unit_offset ? w[j] + 1.0f : w[j]) * rms);
+    if (p0 == 0 && half > 0) {
+      if (tid < half) {
+        // turns in fp64: p * f is off by 2^-53 of itself, which at 2^20 radians is 1e-10
+        double turn = (double)a.positions[t] * a.inv_freq[tid] * 0.15915494309189533577;
+        turn -= rint(turn);
+        float sn, cs;
+        sincospif(2.0f * (float)turn, &sn, &cs);
+        s_cos[tid] = cs;
+        s_sin[tid] = sn;
+      }
+      __syncthreads();
     }
-    if (half > 0) {
-      const bool turns = live && g.kind != ROPE_VALUES && e < a.rot;
-      if (NEXT) {
-        if (turns) {
 #pragma unroll
-          for (int j = 0; j < 4; j++) {
-            const float cs = s_cos[e / 2 + j], sn = s_sin[e / 2 + j], x = v[2 * j], y = v[2 * j + 1];
-            v[2 * j] = x * cs - y * sn;
-            v[2 * j + 1] = y * cs + x * sn;
-          }
+    for (int p = 0; p < ROPE_AHEAD; p++) {
+      if (p0 + p >= a.passes) return;
+      const Part q = part_of(unit0 + (p0 + p) * 4);
+      float v[8];
+      item_to_f32<XT>(it[p], v);
+      if (q.g.w) {
+        float ss = 0.f;
+#pragma unroll
+        for (int j = 0; j < 8; j++) ss = fmaf(v[j], v[j], ss);
+        ss = group_sum<G>(ss);
+        // 1 / sqrt by the hardware's (off by an ulp) and a step of Newton's: within an ulp, in a fifth of the instructions of a division and a root
+        const float m = fmaf(ss, a.inv_d, a.eps);
+        float rms = __builtin_amdgcn_rsqf(m);
+        rms = m > 0.f && m < INFINITY ? fmaf(rms * 0.5f, fmaf(-m * rms, rms, 1.0f), rms) : rms;
+        if (q.live) {
+          const float4 w0 = *reinterpret_cast<const float4*>(q.g.w + e), w1 = *reinterpret_cast<const float4*>(q.g.w + e + 4);
+          const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
+#pragma unroll
+          for (int j = 0; j < 8; j++) v[j] = v[j] * ((a.add_unit_offset ? w[j] + 1.0f : w[j]) * rms);
         }
-      } else {  // the other half of the pairs is half / 8 lanes away
-        const bool first = e < half;
-        const int from = first ? lane + half / 8 : lane - half / 8, j0 = first ? e : e - half;
-        float o[8];
+      }
+      if (half > 0 && q.g.kind != ROPE_VALUES) {
+        const bool turns = q.live && e < a.rot;
+        if (NEXT) {
+          if (turns) {
 #pragma unroll
-        for (int j = 0; j < 8; j++) o[j] = __shfl(v[j], from);
-        if (turns) {
+            for (int j = 0; j < 4; j++) {
+              const float cs = s_cos[e / 2 + j], sn = s_sin[e / 2 + j], x = v[2 * j], y = v[2 * j + 1];
+              v[2 * j] = x * cs - y * sn;
+              v[2 * j + 1] = y * cs + x * sn;
+            }
+          }
+        } else {  // the other element of every pair is half / 8 lanes away
+          const bool first = e < half;
+          const int j0 = first ? e : e - half;
+          float o[8];
+          if (half == 8 * (G / 2)) {  // (the whole of a head of 8 G elements: the usual one)
 #pragma unroll
-          for (int j = 0; j < 8; j++) {
-            const float cs = s_cos[j0 + j], sn = s_sin[j0 + j];
-            v[j] = first ? v[j] * cs - o[j] * sn : v[j] * cs + o[j] * sn;
+            for (int j = 0; j < 8; j++) o[j] = across<G / 2>(v[j]);
+          } else {
+            const int from = first ? lane + half / 8 : lane - half / 8;
+#pragma unroll
+            for (int j = 0; j < 8; j++) o[j] = __shfl(v[j], from);
+          }
+          if (turns) {
+            const float4 c0 = *reinterpret_cast<const float4*>(s_cos + j0), c1 = *reinterpret_cast<const float4*>(s_cos + j0 + 4);
+            const float4 n0 = *reinterpret_cast<const float4*>(s_sin + j0), n1 = *reinterpret_cast<const float4*>(s_sin + j0 + 4);
+            const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w}, sn[8] = {n0.x, n0.y, n0.z, n0.w, n1.x, n1.y, n1.z, n1.w};
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = first ? v[j] * cs[j] - o[j] * sn[j] : v[j] * cs[j] + o[j] * sn[j];
           }
         }
       }
-    }
-    if (!live) continue;
-    const int hh = h - g.head0;
-    if (g.kind == ROPE_OUT) {
-      item_store<XT>(g.y, t * g.y_token + hh * g.y_head + e, v);
-    } else if (slot >= 0 && slot < a.slot_count) {
-      const uint32_t page = (uint32_t)slot / a.page, at = (uint32_t)slot - page * a.page;
-      item_store<MLLM_HIP_BF16>(g.y, page * a.page_stride + at * a.slot_stride + hh * a.head_stride + e, v);
+      if (!q.live) continue;
+      if (q.g.kind == ROPE_OUT) item_store<XT>(q.g.y, t * q.g.y_token + q.head * q.g.y_head + e, v);
+      else if (stored >= 0) item_store<MLLM_HIP_BF16>(q.g.y, stored + q.head * a.head_stride + e, v);
     }
   }
 }
@@ -137,21 +170,26 @@ static int rope_group(const mllm_hip_heads& p, int dtype, int head_dim, bool sto
   auto whole = [&](int64_t stride) { return stride * wide % 16 == 0; };
   if (!al16(p.x) || !whole(p.x_token_stride) || !whole(p.x_head_stride) || (p.weight && !al16(p.weight))) return MLLM_HIP_E_ALIGN;
   if (stored && (!al16(p.y) || !whole(p.y_token_stride) || !whole(p.y_head_stride))) return MLLM_HIP_E_ALIGN;
-  g = RopeGroup{p.x, p.y, p.weight, p.x_token_stride, p.x_head_stride, p.y_token_stride, p.y_head_stride, 0, ROPE_OUT};
+  g = RopeGroup{p.x, p.y, p.weight, p.x_token_stride, p.x_head_stride, p.y_token_stride, p.y_head_stride, p.heads, 0, ROPE_OUT};
   return 0;
 }
 
-// Workgroups of a token: one for all of its heads while there are tokens to fill the chip, else one per 256 / G heads.
+// Workgroups of a token: one for all of its heads while there are tokens to fill the chip, else one per four units.
 static const int64_t ROPE_FULL = 2048;
 
-static int rope_launch(RopeArgs& a, int dtype, int64_t T, int head_dim, int rot_dim, int interleaved, int heads, hipStream_t st) {
-  const int lanes = head_dim <= 64 ? 8 : head_dim <= 128 ? 16 : head_dim <= 256 ? 32 : 64;
-  const int all = (heads + 256 / lanes - 1) / (256 / lanes);
-  a.heads = heads;
+static int rope_launch(RopeArgs& a, int dtype, int64_t T, int head_dim, int rot_dim, int interleaved, hipStream_t st) {
+  const int lanes = head_dim <= 64 ? 8 : head_dim <= 128 ? 16 : head_dim <= 256 ? 32 : 64, per = 64 / lanes;
+  a.units = 0;
+  for (int i = 0; i < a.nparts; i++) {
+    a.part[i].unit0 = a.units;
+    a.units += (a.part[i].heads + per - 1) / per;
+  }
+  const int all = (a.units + 3) / 4;
   a.D = head_dim;
+  a.inv_d = 1.0f / (float)head_dim;
   a.rot = rot_dim;
   a.passes = T * all <= ROPE_FULL ? 1 : all;
-  const dim3 grid((unsigned)T, (unsigned)(all / a.passes));
+  const dim3 grid((unsigned)T, (unsigned)((all + a.passes - 1) / a.passes));
 #define ROPE(XT_, G_)                                                                                    \
   if (interleaved) hipLaunchKernelGGL((rope_kernel<XT_, G_, true>), grid, dim3(256), 0, st, a);          \
   else hipLaunchKernelGGL((rope_kernel<XT_, G_, false>), grid, dim3(256), 0, st, a)
@@ -190,18 +228,13 @@ MLLM_API int mllm_hip_qk_norm_rope(int nparts, const mllm_hip_heads* parts, int 
   RC_RET(rope_checks(dtype, T, head_dim, positions, inv_freq, rot_dim));
   if (T == 0) return 0;  // (tensors without elements have no addresses)
   RopeArgs a = {};
-  int heads = 0;
-  for (int i = 0; i < nparts; i++) {
-    RC_RET(rope_group(parts[i], dtype, head_dim, true, a.part[i]));
-    a.part[i].head0 = heads;
-    heads += parts[i].heads;
-  }
+  for (int i = 0; i < nparts; i++) RC_RET(rope_group(parts[i], dtype, head_dim, true, a.part[i]));
   a.nparts = nparts;
   a.eps = epsilon;
   a.add_unit_offset = add_unit_offset;
   a.positions = positions;
   a.inv_freq = inv_freq;
-  return rope_launch(a, dtype, T, head_dim, rot_dim, interleaved, heads, (hipStream_t)stream);
+  return rope_launch(a, dtype, T, head_dim, rot_dim, interleaved, (hipStream_t)stream);
 }
 
 MLLM_API int mllm_hip_kv_append(const mllm_hip_heads* q, const mllm_hip_heads* k, const mllm_hip_heads* v, int dtype, int64_t T,
@@ -225,13 +258,9 @@ MLLM_API int mllm_hip_kv_append(const mllm_hip_heads* q, const mllm_hip_heads* k
   a.part[1].y = cache->v;
   a.part[1].kind = ROPE_VALUES;
   a.part[1].w = nullptr;
-  a.part[1].head0 = k->heads;
-  int heads = k->heads + v->heads;
   a.nparts = 2;
   if (q) {
     RC_RET(rope_group(*q, dtype, cache->head_dim, true, a.part[2]));
-    a.part[2].head0 = heads;
-    heads += q->heads;
     a.nparts = 3;
   }
   a.eps = epsilon;
@@ -244,5 +273,5 @@ MLLM_API int mllm_hip_kv_append(const mllm_hip_heads* q, const mllm_hip_heads* k
   a.head_stride = cache->head_stride;
   a.slot_count = cache->pages * cache->page_size;
   a.page = (uint32_t)cache->page_size;
-  return rope_launch(a, dtype, T, cache->head_dim, rot_dim, interleaved, heads, (hipStream_t)stream);
+  return rope_launch(a, dtype, T, cache->head_dim, rot_dim, interleaved, (hipStream_t)stream);
 }
