@@ -21,12 +21,13 @@ enum { SMP_STEPS = 512, SMP_WG = 512, SMP_BIN_BITS = 9, SMP_BINS = 1 << SMP_BIN_
        SMP_PIECES = 16, SMP_HOLD = 5 };
 
 struct SampleRow {  // what launch 3 finds out about a row
-  int lo, hi;       // the border's steps; lo = SMP_STEPS: everything is kept
+  int lo, mid, hi;  // the steps that may hold the border by mass are lo .. mid, the one by count is in is hi; lo = SMP_STEPS: everything is kept
   int cut;          // 1: the k-th is within the row's weights
-  uint32_t above;   // elements in front of step lo
-  uint64_t mass_above, mass;  // of the elements in front of step lo, of all (both in units)
-  uint32_t listed;
-  int pad;
+  uint32_t listed;  // elements of steps lo .. mid and hi
+  uint32_t want;    // which of the listed, in descending order, is the k-th
+  uint64_t front;   // mass in front of step lo (in units)
+  uint64_t front_k; // that and what lies between mid and hi: with the listed ones in front of the k-th, all that is in front of it
+  uint64_t mass;    // of the row
 };
 struct SampleArgs {
   const void* x;
@@ -365,6 +366,8 @@ __device__ __forceinline__ void running2(uint32_t& c, unsigned long long& m, uin
     if (w < wave) c += s_c[w], m += s_m[w];
 }
 
+__device__ __forceinline__ bool in_list(const SampleRow& r, int step) { return (step >= r.lo && step <= r.mid) || (r.lo < SMP_STEPS && step == r.hi); }
+
 // ---- 3: the border's steps, sums in front of them, a list of what is in them ---------------------------------------------------
 template <int XT>
 __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
@@ -373,7 +376,7 @@ __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
   __shared__ unsigned long long s_wave[SMP_WG / 64];
   __shared__ unsigned long long s_mass[SMP_STEPS];
   __shared__ uint32_t s_count[SMP_STEPS];
-  __shared__ int s_first[2];
+  __shared__ int s_first[2], s_last;
   __shared__ uint32_t s_list[SMP_WG / 64];
   __shared__ float s_dense[SMP_WG * 2];
   const int piece = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -402,7 +405,7 @@ __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
   if (given.greedy()) return;
   const SampleScale s = scale_of(given, (lds_double)s_table);
   if (s.top == -INFINITY) return;
-  SampleRow r = {SMP_STEPS, SMP_STEPS, 0, 0, 0, 0, 0, 0};
+  SampleRow r = {SMP_STEPS, SMP_STEPS - 1, SMP_STEPS - 1, 0, 0, 0, 0, 0, 0};
   uint32_t mine = 0;  // elements of step tid in the pieces in front of this one
   if (by_count || by_mass) {
     uint32_t count = 0;
@@ -420,34 +423,42 @@ __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
     s_count[tid] = counts;
     s_mass[tid] = masses;
     if (tid < 2) s_first[tid] = SMP_STEPS;
+    if (tid == 2) s_last = SMP_STEPS - 1;
     __syncthreads();
     auto up_to = [&](int step, bool m) -> unsigned long long { return step <= 0 ? 0 : m ? s_mass[step - 1] : s_count[step - 1]; };  // in front of a step
     if (by_count && counts >= (uint32_t)k && counts - count < (uint32_t)k) s_first[0] = tid;
     __syncthreads();
     r.cut = s_first[0] < SMP_STEPS;
-    r.hi = s_first[0];
     r.mass = s_mass[SMP_STEPS - 1];
+    if (r.cut) r.hi = r.mid = s_first[0];
     if (cut.few) {
       r.lo = 0;
-      r.hi = min(r.hi, SMP_STEPS - 1);
-    } else if (by_mass) {  // with a cut by count the mass of what it keeps is only known to be that in front of step hi or more
-      const double target = (double)p * (double)(r.cut ? up_to(r.hi, true) : r.mass);
-      if ((double)masses >= target && (tid == 0 || (double)(masses - mass) < target)) atomicMin(&s_first[1], tid);
+    } else if (by_mass) {  // with a cut by count the mass of what it keeps is only known to be between that in front of step hi and with it
+      const double least = (double)p * (double)(r.cut ? up_to(r.hi, true) : r.mass), most = (double)p * (double)(r.cut ? up_to(r.hi + 1, true) : r.mass);
+      if ((double)masses >= least && (tid == 0 || (double)(masses - mass) < least)) atomicMin(&s_first[1], tid);
+      if ((double)masses >= most && (tid == 0 || (double)(masses - mass) < most)) atomicMin(&s_last, tid);
       __syncthreads();
-      r.lo = min(s_first[1], r.cut ? r.hi : SMP_STEPS - 1);
-      if (!r.cut) r.hi = r.lo;
-    } else {
+      r.mid = min(s_last, r.hi);
+      r.lo = min(s_first[1], r.mid);
+      if (!r.cut) r.hi = r.mid;
+    } else if (r.cut) {
       r.lo = r.hi;
     }
     if (r.lo < SMP_STEPS) {
-      r.above = (uint32_t)up_to(r.lo, false);
-      r.mass_above = up_to(r.lo, true);
-      r.listed = (uint32_t)(up_to(r.hi + 1, false) - r.above);
-    } else {
-      r.hi = SMP_STEPS - 1;
+      const int before = min(r.mid + 1, r.hi);  // the listed steps in front of hi are lo .. before - 1
+      const uint32_t front_listed = (uint32_t)(up_to(before, false) - up_to(r.lo, false));
+      r.front = up_to(r.lo, true);
+      r.listed = front_listed + (uint32_t)(up_to(r.hi + 1, false) - up_to(r.hi, false));
+      if (r.cut) {
+        r.want = (uint32_t)k - (uint32_t)up_to(r.hi, false) + front_listed;
+        r.front_k = up_to(r.hi, true) - (up_to(before, true) - r.front);
+      } else {
+        r.want = r.listed;  // (a small k that does not cut: fewer than k have a weight, and all of them are listed)
+        r.front_k = r.front;
+      }
     }
     __syncthreads();
-    mine = tid >= r.lo && tid <= r.hi ? mine : 0;
+    mine = in_list(r, tid) ? mine : 0;
   }
   // where this piece's part of the list begins (and the weights' table is there)
 #pragma unroll
@@ -474,7 +485,7 @@ __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
     for (int e = 0; e < N; e++) {
       const int step = s.step_of(v[e]);
       const bool in = step < r.lo && step < SMP_STEPS;
-      listed += !in && step <= r.hi && step < SMP_STEPS;
+      listed += in_list(r, step);
       const uint64_t who = __ballot(in);
       if (who) {
         if (in) dense[waiting + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = v[e];
@@ -511,7 +522,7 @@ __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
 #pragma unroll
     for (int e = 0; e < N; e++) {
       const int step = s.step_of(v[e]);
-      in |= (uint32_t)(step >= r.lo && step <= r.hi && step < SMP_STEPS) << e;
+      in |= (uint32_t)in_list(r, step) << e;
     }
     if (!__ballot(in != 0)) return;
     const uint32_t have = __popc(in);
@@ -753,8 +764,7 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
     SampleBorder edge = {0, 0x7fffffff, 0};
 #pragma unroll 1
     for (int by_mass = r.cut || cut.few ? 0 : 1; by_mass <= (cut.by_mass ? 1 : 0); by_mass++) {
-      const unsigned long long want = r.cut ? (unsigned long long)cut.k - r.above : r.listed;  // (few and not cut: fewer than k have a weight, and all are listed)
-      const SampleBorder e = border(by_mass, want, (double)p * (double)mass, r.mass_above);
+      const SampleBorder e = border(by_mass, r.want, (double)p * (double)mass, by_mass ? r.front : r.front_k);
       if (e.key > edge.key || (e.key == edge.key && e.last < edge.last)) edge = e;
       mass = e.mass;
     }
