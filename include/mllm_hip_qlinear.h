@@ -628,7 +628,8 @@ typedef struct mllm_hip_kv_cache {
   int heads, head_dim;
 } mllm_hip_kv_cache;
 /* `heads` heads of every token: token t, head h at element t * x_token_stride + h * x_head_stride of x, the results in y likewise.  Rows
- * and pointers 16-byte aligned.  y may be x with the same strides.  weight: fp32 [head_dim] of the RMSNorm, NULL: no norm. */
+ * and pointers 16-byte aligned.  y is x with the same strides or shares no element with any input, and no stride of y is 0 (of more
+ * than one token or head).  weight: fp32 [head_dim] of the RMSNorm, NULL: no norm. */
 typedef struct mllm_hip_heads {
   const void* x;
   void* y;
@@ -641,7 +642,7 @@ typedef struct mllm_hip_heads {
  * pairs (a, b) of the first rot_dim elements turned by positions[t] * inv_freq[j]: a cos - b sin, b cos + a sin.  Pair j is elements
  * j and j + rot_dim / 2, or (interleaved) 2 j and 2 j + 1.  dtype of x and y: F32 or BF16, rounded once; the angles are fp64 up to the
  * fraction of a turn.  positions int32 [T] (any value), inv_freq fp64 [rot_dim / 2]; rot_dim 0: no rotation, neither is read.
- * head_dim % 8 == 0, <= 512; rot_dim % 16 == 0, <= head_dim.  T = 0 does nothing. */
+ * head_dim % 8 == 0, <= 512; rot_dim % 16 == 0, <= head_dim; T < 2^24.  T = 0 does nothing. */
 int mllm_hip_qk_norm_rope(int nparts, const mllm_hip_heads* parts, int dtype, int64_t T, int head_dim, float epsilon,
                           int add_unit_offset, const int32_t* positions, const double* inv_freq, int rot_dim, int interleaved,
                           void* stream);
@@ -659,7 +660,7 @@ int mllm_hip_kv_append(const mllm_hip_heads* q, const mllm_hip_heads* k, const m
  * bits that are not there count as 0.  tree NULL: j <= t.  One token a sequence is a decode step, a tree the verification
  * of drafted tokens, many tokens without a tree a (chunk of a) prompt.
  *   o[t][h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * (q . k_j) - max), of key head h / (heads / kv heads); a token that sees
- *   nothing: zeros.  What a token does not see has no effect on it, NaN included.
+ *   nothing, or scores of -inf alone: zeros.  What a token does not see has no effect on it, NaN included.
  * Position i of sequence b is slot i % page_size of page block_table[b * table_stride + i / page_size] (int32); positions from table_len *
  * page_size on are not there, pages outside the cache read as zeros.  q->x, q->y: F32 or BF16, 16-byte aligned rows (weight is not
  * looked at); rows of q in no sequence stay as they are in y.  y may not be x.  head_dim 64, 128 or 256, heads a multiple of the cache's, scale > 0.

@@ -685,6 +685,7 @@ MLLM_API int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_
       !whole(q->y_head_stride) || cache->page_stride % 8 || cache->slot_stride % 8 || cache->head_stride % 8 || !al(block_table, 4) || !al(cu_tokens, 4) || !al(prefix, 4) ||
       !al(tree, 8) || !al(workspace, 16))
     return MLLM_HIP_E_ALIGN;
+  if (q->x == q->y || !own_places(*q, T)) return MLLM_HIP_E_BADARG;
   const bool f32 = dtype == MLLM_HIP_F32;
   const int heads = q->heads, D = cache->head_dim;
   AttnPlan p = attention_plan(f32, B, heads, cache->heads, max_tokens, max_keys, D);
@@ -692,7 +693,7 @@ MLLM_API int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_
   const size_t need = attention_room(p, B, heads, max_tokens, D);
   if (need && (!workspace || workspace_bytes < need)) return MLLM_HIP_E_BADARG;
   const int64_t pieces = p.ranges + B, groups = ((p.ranges ? p.ranges : B) * cache->heads + 7) / 8 * 8;
-  if (groups > 0x7fffffff / p.row_tiles) return MLLM_HIP_E_SHAPE;
+  if (groups > 0xffffff / p.row_tiles) return MLLM_HIP_E_SHAPE;
   AttnArgs a = {};
   a.q = q->x;
   a.o = q->y;

@@ -53,4 +53,11 @@ __device__ __forceinline__ void item_store(void* p, int64_t elem, float (&v)[8])
   }
 }
 
+// Every head of the results has a place of its own, and where that is the place of x, it is that of the same head
+inline bool own_places(const mllm_hip_heads& p, int64_t T) {
+  const bool tokens = T > 1, heads = p.heads > 1;
+  if ((tokens && !p.y_token_stride) || (heads && !p.y_head_stride)) return false;
+  return p.x != p.y || !((tokens && p.x_token_stride != p.y_token_stride) || (heads && p.x_head_stride != p.y_head_stride));
+}
+
 }  // namespace mllmhip

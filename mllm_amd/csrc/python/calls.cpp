@@ -326,7 +326,7 @@ void results_to(mllm_hip_heads& p, const at::Tensor& x, PyObject* out, at::Tenso
   if (out == Py_None) made = at::empty(x.sizes(), x.options());
   else made = tensor(out);
   const mllm_hip_heads y = heads_of(made, x.size(0), x.size(2), x.scalar_type(), device);
-  require(y.heads == p.heads);
+  require(y.heads == p.heads && (y.x_token_stride || x.size(0) <= 1) && (y.x_head_stride || x.size(1) <= 1));  // (a place for every head)
   p.y = made.data_ptr();
   p.y_token_stride = y.x_token_stride;
   p.y_head_stride = y.x_head_stride;
@@ -353,6 +353,14 @@ mllm_hip_kv_cache cache_of(PyObject* ko, PyObject* vo, int64_t device) {
   return mllm_hip_kv_cache{k.data_ptr(), v.data_ptr(), stride_of(k, 0), stride_of(k, 1), stride_of(k, 2), k.size(0), k.size(1), (int)k.size(2), (int)k.size(3)};
 }
 
+// a given workspace on the current device in one piece, or a new one
+void* workspace_on(int64_t device, PyObject* o, size_t bytes, at::Tensor& made) {
+  if (o == Py_None) return bytes ? workspace(o, bytes, made) : nullptr;
+  const at::Tensor& t = tensor(o);
+  require(t.is_cuda() && t.get_device() == device && t.is_contiguous());
+  return workspace(o, bytes, made);
+}
+
 // (q, k, positions, inv_freq, q_weight, k_weight, eps, add_unit_offset, interleaved, out)
 PyObject* qk_norm_rope(Args a) {
   const int64_t device = current_device();
@@ -369,6 +377,7 @@ PyObject* qk_norm_rope(Args a) {
   at::Tensor yq, yk;
   results_to(parts[0], q, oq, yq, device);
   results_to(parts[1], k, ok, yk, device);
+  require(T == 0 || parts[0].y != parts[1].y);
   parts[0].weight = vector_of<float>(a[4], device, at::kFloat, D);
   parts[1].weight = vector_of<float>(a[5], device, at::kFloat, D);
   const Rotation r = rotation_of(a[2], a[3], T, device);
@@ -391,6 +400,7 @@ PyObject* kv_append(Args a) {
   const int64_t T = k.size(0), D = cache.head_dim;
   mllm_hip_heads kp = heads_of(k, T, D, k.scalar_type(), device), vp = heads_of(v, T, D, k.scalar_type(), device), qp = {};
   require(kp.heads == cache.heads && vp.heads == cache.heads);
+  require((cache.page_stride || cache.pages == 1) && (cache.head_stride || cache.heads == 1));  // (what is stored has a place of its own)
   kp.weight = vector_of<float>(a[7], device, at::kFloat, D);
   at::Tensor y;
   if (a[8] != Py_None) {
@@ -440,7 +450,7 @@ PyObject* attention_paged(Args a) {
   results_to(qp, q, a[10], y, device);
   require(T == 0 || qp.y != qp.x);
   const size_t need = mllm_hip_attention_paged_workspace_bytes(dtype, T, B, qp.heads, cache.heads, cache.head_dim, tokens, keys);
-  void* wp = need || a[11] != Py_None ? workspace(a[11], need, work) : nullptr;
+  void* wp = workspace_on(device, a[11], need, work);
   void* st = stream();
   const int64_t table_stride = stride_of(table, 0), table_len = table.size(1);
   const int32_t* tp = static_cast<const int32_t*>(table.data_ptr());
@@ -465,7 +475,7 @@ PyObject* sample(Args a) {
   if (a[6] == Py_None) made = empty({rows}, at::kInt);
   int32_t* tokens = a[6] == Py_None ? static_cast<int32_t*>(made.data_ptr()) : const_cast<int32_t*>(vector_of<int32_t>(a[6], device, at::kInt, rows));
   const size_t need = mllm_hip_sample_workspace_bytes(rows, vocab);
-  void* wp = need || a[7] != Py_None ? workspace(a[7], need, work) : nullptr;
+  void* wp = workspace_on(device, a[7], need, work);
   void *xp = x.data_ptr(), *st = stream();
   run("mllm_hip_sample", [&] { return mllm_hip_sample(xp, dtype, stride, rows, vocab, u, t, k, p, min_p, tokens, wp, need, st); });
   return a[6] == Py_None ? THPVariable_Wrap(made) : given(a[6]);

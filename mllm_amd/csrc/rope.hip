@@ -163,13 +163,14 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
 static bool al16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
 // a part as the kernel takes it: checks of the strides that 16-byte loads and stores need
-static int rope_group(const mllm_hip_heads& p, int dtype, int head_dim, bool stored, RopeGroup& g) {
+static int rope_group(const mllm_hip_heads& p, int dtype, int64_t T, bool stored, RopeGroup& g) {
   const int wide = dtype == MLLM_HIP_F32 ? 4 : 2;
   if (!p.x || (stored && !p.y) || p.heads < 1) return MLLM_HIP_E_BADARG;
   if (p.heads > 65536) return MLLM_HIP_E_SHAPE;
   auto whole = [&](int64_t stride) { return stride * wide % 16 == 0; };
   if (!al16(p.x) || !whole(p.x_token_stride) || !whole(p.x_head_stride) || (p.weight && !al16(p.weight))) return MLLM_HIP_E_ALIGN;
   if (stored && (!al16(p.y) || !whole(p.y_token_stride) || !whole(p.y_head_stride))) return MLLM_HIP_E_ALIGN;
+  if (stored && !own_places(p, T)) return MLLM_HIP_E_BADARG;
   g = RopeGroup{p.x, p.y, p.weight, p.x_token_stride, p.x_head_stride, p.y_token_stride, p.y_head_stride, p.heads, 0, ROPE_OUT};
   return 0;
 }
@@ -212,7 +213,7 @@ static int rope_launch(RopeArgs& a, int dtype, int64_t T, int head_dim, int rot_
 static int rope_checks(int dtype, int64_t T, int head_dim, const int32_t* positions, const double* inv_freq, int rot_dim) {
   if ((dtype != MLLM_HIP_F32 && dtype != MLLM_HIP_BF16) || T < 0 || head_dim < 1 || rot_dim < 0) return MLLM_HIP_E_BADARG;
   if (T && rot_dim && (!positions || !inv_freq)) return MLLM_HIP_E_BADARG;
-  if (head_dim % 8 || head_dim > 512 || rot_dim > head_dim || rot_dim % 16 || T > 0x7fffffff) return MLLM_HIP_E_SHAPE;
+  if (head_dim % 8 || head_dim > 512 || rot_dim > head_dim || rot_dim % 16 || T > 0xffffff) return MLLM_HIP_E_SHAPE;
   if (reinterpret_cast<uintptr_t>(positions) % 4 || reinterpret_cast<uintptr_t>(inv_freq) % 8) return MLLM_HIP_E_ALIGN;
   return 0;
 }
@@ -228,7 +229,7 @@ MLLM_API int mllm_hip_qk_norm_rope(int nparts, const mllm_hip_heads* parts, int 
   RC_RET(rope_checks(dtype, T, head_dim, positions, inv_freq, rot_dim));
   if (T == 0) return 0;  // (tensors without elements have no addresses)
   RopeArgs a = {};
-  for (int i = 0; i < nparts; i++) RC_RET(rope_group(parts[i], dtype, head_dim, true, a.part[i]));
+  for (int i = 0; i < nparts; i++) RC_RET(rope_group(parts[i], dtype, T, true, a.part[i]));
   a.nparts = nparts;
   a.eps = epsilon;
   a.add_unit_offset = add_unit_offset;
@@ -251,8 +252,8 @@ MLLM_API int mllm_hip_kv_append(const mllm_hip_heads* q, const mllm_hip_heads* k
     return MLLM_HIP_E_ALIGN;
   if (T == 0) return 0;
   RopeArgs a = {};
-  RC_RET(rope_group(*k, dtype, cache->head_dim, false, a.part[0]));
-  RC_RET(rope_group(*v, dtype, cache->head_dim, false, a.part[1]));
+  RC_RET(rope_group(*k, dtype, T, false, a.part[0]));
+  RC_RET(rope_group(*v, dtype, T, false, a.part[1]));
   a.part[0].y = cache->k;
   a.part[0].kind = ROPE_KEYS;
   a.part[1].y = cache->v;
@@ -260,7 +261,7 @@ MLLM_API int mllm_hip_kv_append(const mllm_hip_heads* q, const mllm_hip_heads* k
   a.part[1].w = nullptr;
   a.nparts = 2;
   if (q) {
-    RC_RET(rope_group(*q, dtype, cache->head_dim, true, a.part[2]));
+    RC_RET(rope_group(*q, dtype, T, true, a.part[2]));
     a.nparts = 3;
   }
   a.eps = epsilon;

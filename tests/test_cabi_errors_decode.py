@@ -111,3 +111,18 @@ def test_sample_workspace():
     size = _lib.lib().mllm_hip_sample_workspace_bytes
     assert size(0, 100) == 0 and size(4, 0) == 0 and size(1, 1 << 25) == 0
     assert size(8, 151936) >= 8 * 151936 * 4 and size(8, 151936) % 16 == 0
+
+
+@pytest.mark.parametrize("part,T,want", [
+    (dict(y_token_stride=0), 2, BADARG), (dict(y_head_stride=0), 1, BADARG), (dict(x_token_stride=1024), 2, BADARG), (dict(x_head_stride=256), 1, BADARG),
+    (dict(x_token_stride=0), 2, BADARG), (dict(), 1 << 24, SHAPE)])
+def test_results_without_places_of_their_own_and_very_many_tokens(part, T, want):
+    """Two heads of the results in one place, a result where another head's input is, more tokens than a launch has workgroups."""
+    assert _rope(part=_part(**part), T=T) == want
+
+
+def test_attention_over_its_queries_and_of_very_many_tokens():
+    ask = lambda T=1, B=1, tokens=1, **q: _lib.lib().mllm_hip_attention_paged(  # noqa: E731
+        C.byref(_part(**dict(dict(y=P + (1 << 30)), **q))), F32, T, C.byref(_cache()), P, 8, 8, P, P, B, tokens, 0, None, 0, 0, 0.1, None, 0, None)
+    assert ask(y=P) == BADARG and ask(T=2, tokens=2, y_token_stride=0) == BADARG and ask(y_head_stride=0) == BADARG
+    assert ask(T=1 << 22, B=1 << 22) == SHAPE

@@ -307,3 +307,12 @@ def test_refusals():
     wrong = Case([1], [30], 4, 2, 96, 16, torch.float32)
     with pytest.raises(_lib.HipQLinearError):
         wrong.run()
+
+
+def test_workspaces_and_results_that_cannot_be_used():
+    announce("refusals of workspaces and results")
+    c = Case([2], [3000], 4, 2, 128, 16, torch.float32)
+    wide = torch.empty((1 << 22, 2), dtype=torch.uint8, device="cuda")
+    for bad in (dict(workspace=torch.empty(1 << 22, dtype=torch.uint8)), dict(workspace=wide[:, 0]), dict(out=torch.empty((1, 4, 128), device="cuda").expand(2, 4, 128))):
+        with pytest.raises(AssertionError):
+            c.run(**bad)

@@ -188,3 +188,20 @@ def test_refusals():
         args.update(bad)
         with pytest.raises((AssertionError, TypeError)):
             ql.kv_append(**args)
+
+
+def test_results_without_places_of_their_own_are_refused():
+    announce("refusals of results in one place")
+    x, f = torch.zeros((2, 4, 64), device="cuda"), _freq(64)
+    pos, slots = torch.zeros(2, dtype=torch.int32, device="cuda"), torch.zeros(2, dtype=torch.int64, device="cuda")
+    one = torch.zeros((1, 4, 64), device="cuda").expand(2, 4, 64)
+    y = torch.empty_like(x)
+    for out in ((one, y), (y, one), (torch.zeros((2, 1, 64), device="cuda").expand(2, 4, 64), y), (y, y)):
+        with pytest.raises(AssertionError):
+            ql.qk_norm_rope(x, x, pos, f, out=out)
+    kc, vc = (torch.zeros((1, 8, 4, 64), dtype=torch.bfloat16, device="cuda").expand(2, 8, 4, 64) for _ in range(2))
+    with pytest.raises(AssertionError):
+        ql.kv_append(x, x, kc, vc, slots)
+    square = torch.zeros((4, 4, 64), device="cuda")  # heads and tokens in the other order, over the input itself
+    with pytest.raises(_lib.HipQLinearError):
+        ql.qk_norm_rope(square, torch.zeros((4, 4, 64), device="cuda"), torch.zeros(4, dtype=torch.int32, device="cuda"), f, out=(square.transpose(0, 1), torch.empty_like(square)))

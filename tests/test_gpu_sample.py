@@ -179,3 +179,24 @@ def test_no_rows_and_refusals():
             ql.sample(**args)
     with pytest.raises(_lib.HipQLinearError):
         ql.sample(x, u, workspace=torch.empty(64, dtype=torch.uint8, device="cuda"))
+
+
+def test_workspaces_that_cannot_be_used():
+    announce("refusals of workspaces")
+    x, u = torch.zeros((3, 100), device="cuda"), torch.zeros(3, device="cuda")
+    for room in (torch.empty(1 << 22, dtype=torch.uint8), torch.empty((1 << 22, 2), dtype=torch.uint8, device="cuda")[:, 0]):
+        with pytest.raises(AssertionError):
+            ql.sample(x, u, workspace=room)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("k", [257, 5000])
+@pytest.mark.parametrize("spread", [3.0, 0.2])
+def test_many_kept_of_which_a_share(dtype, k, spread):
+    """The border by mass far in front of the one by count, in its step, and behind it (more kept than there are)."""
+    announce("sample many kept of which a share", dtype, k, spread)
+    rng = np.random.default_rng(k)
+    x = (rng.standard_normal((24, 7058)) * spread).astype(np.float32)
+    p = np.tile(np.array([1e-6, 0.05, 0.3, 0.6, 0.9, 0.999, 0.999999, 1.0], np.float32), 3)
+    t = np.repeat(np.array([0.5, 1.0, 1.7], np.float32), 8)
+    _check(x, rng.random(24).astype(np.float32), t, np.full(24, k, np.int32), p, np.zeros(24, np.float32), dtype)
