@@ -298,14 +298,14 @@ __global__ __launch_bounds__(SMP_WG) void sample_ends_kernel(SampleArgs a) {
 
 // ---- 2: counts and masses of the steps --------------------------------------------------------------------------------------
 template <int XT>
-__global__ __launch_bounds__(SMP_WG) void sample_steps_kernel(SampleArgs a) {
-  __shared__ __align__(16) u32x4 s_x[SMP_WG * SMP_HOLD];
+__global__ __launch_bounds__(SMP_LAST) void sample_steps_kernel(SampleArgs a) {
+  __shared__ __align__(16) u32x4 s_x[SMP_LAST * 3];
   __shared__ uint32_t s_count[SMP_STEPS];
   __shared__ unsigned long long s_mass[SMP_STEPS];
   const int piece = blockIdx.x, row = blockIdx.y;
   __shared__ double s_table[64];
   const SampleSpan<XT> span(a, row);
-  SampleWalk<XT, SMP_HOLD> walk(span, s_x, a.pieces, piece, SMP_WG / 64, threadIdx.x >> 6);
+  SampleWalk<XT, 3> walk(span, s_x, a.pieces, piece, SMP_LAST / 64, threadIdx.x >> 6);
   const SampleIn in(a, row);
   const SampleCut cut(a, in);
   if (walk.v0 < walk.v1) walk.hold(walk.v0);
@@ -313,7 +313,7 @@ __global__ __launch_bounds__(SMP_WG) void sample_steps_kernel(SampleArgs a) {
   const SampleScale s = scale_of(in, (lds_double)s_table);
   if (s.top == -INFINITY) return;
   const bool by_mass = cut.by_mass && !cut.few;
-  for (int i = threadIdx.x; i < SMP_STEPS; i += SMP_WG) s_count[i] = 0, s_mass[i] = 0;
+  for (int i = threadIdx.x; i < SMP_STEPS; i += SMP_LAST) s_count[i] = 0, s_mass[i] = 0;
   __syncthreads();
   walk([&](int, const float (&v)[SampleSpan<XT>::N]) {
 #pragma unroll
@@ -327,7 +327,7 @@ __global__ __launch_bounds__(SMP_WG) void sample_steps_kernel(SampleArgs a) {
   });
   __syncthreads();
   const int64_t to = ((int64_t)row * a.pieces + piece) * SMP_STEPS;
-  for (int i = threadIdx.x; i < SMP_STEPS; i += SMP_WG) {
+  for (int i = threadIdx.x; i < SMP_STEPS; i += SMP_LAST) {
     a.count[to + i] = s_count[i];
     a.mass[to + i] = s_mass[i];
   }
@@ -391,27 +391,25 @@ struct SampleBounds {
     auto of = [&](int l) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(least), l)); };
     front = of(0), mid = of(16), before = of(32), last = of(48);
   }
-  __device__ __forceinline__ uint64_t listed(float v, uint64_t in_front) const {
-    const uint64_t some = __ballot(v >= last) & ~in_front;
-    return some ? some & ~(__ballot(v >= before) & ~__ballot(v >= mid)) : 0;
-  }
+  // of the elements from hi's on that are not in front, the listed ones
+  __device__ __forceinline__ uint64_t listed(float v, uint64_t some) const { return some & ~(__ballot(v >= before) & ~__ballot(v >= mid)); }
 };
 
 // ---- 3: the border's steps, sums in front of them, a list of what is in them ---------------------------------------------------
 template <int XT>
 __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
   static_assert(SMP_WG == SMP_STEPS, "a thread per step");
+  constexpr int N = SampleSpan<XT>::N;
   __shared__ __align__(16) u32x4 s_x[SMP_WG * SMP_HOLD];
   __shared__ unsigned long long s_wave[SMP_WG / 64];
   __shared__ unsigned long long s_mass[SMP_STEPS];
   __shared__ uint32_t s_count[SMP_STEPS];
   __shared__ int s_first[2], s_last;
   __shared__ uint32_t s_list[SMP_WG / 64];
-  __shared__ float s_dense[SMP_WG * 2];
+  __shared__ float s_dense[SMP_WG * (1 + N)];
   const int piece = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   __shared__ double s_table[64];
   const SampleSpan<XT> span(a, row);
-  constexpr int N = SampleSpan<XT>::N;
   SampleWalk<XT, SMP_HOLD> walk(span, s_x, a.pieces, piece, SMP_WG / 64, wave);
   const SampleIn given(a, row);
   const SampleCut cut(a, given);
@@ -501,45 +499,48 @@ __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
   __syncthreads();
 
   // Where few elements are in front of the border a weight of each lane would be one of them at a time: they are collected, 64 and more, first.
-  float* dense = s_dense + wave * 128;
+  float* dense = s_dense + wave * (64 + 64 * N);
   double sum = 0.0;
   uint32_t listed = 0;
   int waiting = 0;
   auto add = [&](int n) {
-    const double w = s.weight(dense[lane]);
+    const double w = s.weight(dense[waiting + lane]);
     sum += lane < n && s.heavy(w) ? w : 0.0;
   };
   const SampleBounds bound(s, r);
   walk([&](int, const float (&v)[N]) {
-    uint64_t any = 0, all = ~0ull;
+    uint64_t front[N], some[N], any = 0, all = ~0ull, list = 0;
 #pragma unroll
-    for (int e = 0; e < N; e++) any |= __ballot(v[e] >= bound.last), all &= __ballot(v[e] >= bound.front);
-    if (!any) return;
+    for (int e = 0; e < N; e++) {
+      front[e] = __ballot(v[e] >= bound.front);
+      some[e] = __ballot(v[e] >= bound.last) & ~front[e];
+      any |= front[e], all &= front[e], list |= some[e];
+    }
+    if (list) {
+#pragma unroll
+      for (int e = 0; e < N; e++) listed += (uint32_t)__popcll(bound.listed(v[e], some[e]));
+    }
     if (!~all) {
 #pragma unroll
       for (int e = 0; e < N; e++) {
         const double w = s.weight(v[e]);
         sum += s.heavy(w) ? w : 0.0;
       }
-      return;
-    }
+    } else if (any) {
 #pragma unroll
-    for (int e = 0; e < N; e++) {
-      const uint64_t who = __ballot(v[e] >= bound.front);
-      listed += (uint32_t)__popcll(bound.listed(v[e], who));
-      if (who) {
-        if (v[e] >= bound.front) dense[waiting + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0))] = v[e];
-        waiting += __popcll(who);
-        if (waiting >= 64) {
-          add(64);
-          waiting -= 64;
-          const float rest = dense[64 + lane];
-          dense[lane] = rest;
-        }
+      for (int e = 0; e < N; e++) {
+        if (v[e] >= bound.front) dense[__builtin_amdgcn_mbcnt_hi((uint32_t)(front[e] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)front[e], waiting))] = v[e];
+        waiting += __popcll(front[e]);
+      }
+      while (waiting >= 64) {
+        waiting -= 64;
+        add(64);
       }
     }
   });
-  add(waiting);
+  const int rest = waiting;
+  waiting = 0;
+  add(rest);
 #pragma unroll
   for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
   if (lane == 0) s_list[wave] = listed;
@@ -557,8 +558,10 @@ __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
   walk([&](int i, const float (&v)[N]) {
     uint64_t in[N], any = 0;
 #pragma unroll
-    for (int e = 0; e < N; e++) any |= in[e] = bound.listed(v[e], __ballot(v[e] >= bound.front));
+    for (int e = 0; e < N; e++) any |= in[e] = __ballot(v[e] >= bound.last) & ~__ballot(v[e] >= bound.front);
     if (!any) return;
+#pragma unroll
+    for (int e = 0; e < N; e++) in[e] = bound.listed(v[e], in[e]);
     uint32_t put = to;  // (a lane's elements follow one another)
 #pragma unroll
     for (int e = 0; e < N; e++) {
@@ -1011,7 +1014,7 @@ MLLM_API int mllm_hip_sample(const void* logits, int dtype, int64_t row_stride, 
   hipStream_t st = (hipStream_t)stream;
   auto go = [&](auto ends, auto steps, auto border, auto token) {
     hipLaunchKernelGGL(ends, grid, dim3(SMP_WG), 0, st, a);
-    if (top_k || top_p) hipLaunchKernelGGL(steps, grid, dim3(SMP_WG), 0, st, a);
+    if (top_k || top_p) hipLaunchKernelGGL(steps, grid, dim3(SMP_LAST), 0, st, a);
     hipLaunchKernelGGL(border, grid, dim3(SMP_WG), 0, st, a);
     hipLaunchKernelGGL(token, dim3((unsigned)rows), dim3(SMP_LAST), 0, st, a);
   };
