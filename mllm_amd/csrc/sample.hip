@@ -18,7 +18,7 @@
 namespace mllmhip {
 
 enum { SMP_STEPS = 512, SMP_WG = 512, SMP_BIN_BITS = 9, SMP_BINS = 1 << SMP_BIN_BITS, SMP_LAST = 1024, SMP_RANKED = 128, SMP_FEW = 256, SMP_HELD = 2048,
-       SMP_PIECES = 16, SMP_HOLD = 5 };
+       SMP_PIECES = 16, SMP_HOLD = 5, SMP_FOUND = 128 };
 
 struct SampleRow {  // what launch 3 finds out about a row
   int lo, mid, hi;  // the steps that may hold the border by mass are lo .. mid, the one by count is in is hi; lo = SMP_STEPS: everything is kept
@@ -109,22 +109,27 @@ struct SampleWalk {
   static constexpr int N = Span::N;
   const Span& span;
   u32x4* lds;  // [H][64] of this wave
-  int v0, v1, held;
-  __device__ __forceinline__ SampleWalk(const Span& span_, u32x4* lds_, int pieces, int p, int waves, int wave) : span(span_), lds(lds_ + wave * H * 64), held(-1) {
+  int v0, v1, held, asked;
+  u32x4 r[H];  // on their way
+  __device__ __forceinline__ SampleWalk(const Span& span_, u32x4* lds_, int pieces, int p, int waves, int wave) : span(span_), lds(lds_ + wave * H * 64), held(-1), asked(-1) {
     const int per = (span.vecs + pieces - 1) / pieces, a = min(span.vecs, p * per), b = min(span.vecs, a + per), each = (b - a + waves - 1) / waves;
     v0 = min(b, a + wave * each);
     v1 = min(b, v0 + each);
   }
-  __device__ __forceinline__ void hold(int from) {
-    if (held == from) return;
-    held = from;
+  __device__ __forceinline__ void ask(int from) {
+    asked = from;
     const int lane = threadIdx.x & 63;
-    u32x4 r[H];
 #pragma unroll
     for (int j = 0; j < H; j++) {
       const int vec = min(from + j * 64 + lane, v1 - 1);
       r[j] = span.whole(vec) ? span.load(vec) : u32x4{0, 0, 0, 0};
     }
+  }
+  __device__ __forceinline__ void hold(int from) {
+    if (held == from) return;
+    if (asked != from) ask(from);
+    held = from;
+    const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int j = 0; j < H; j++) lds[j * 64 + lane] = r[j];
 #pragma unroll 1
@@ -139,6 +144,7 @@ struct SampleWalk {
     const int lane = threadIdx.x & 63;
     for (int b = v0; b < v1; b += H * 64) {
       hold(b);
+      if (b + H * 64 < v1) ask(b + H * 64);
 #pragma unroll 1
       for (int at = b + lane, j = 0; j < H && b + j * 64 < v1; j++, at += 64) {
         float v[N];
@@ -406,6 +412,7 @@ __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
   __shared__ uint32_t s_count[SMP_STEPS];
   __shared__ int s_first[2], s_last;
   __shared__ uint32_t s_list[SMP_WG / 64];
+  __shared__ uint32_t s_found[SMP_WG / 64][SMP_FOUND];  // the first of a wave's listed elements: mostly all
   __shared__ float s_dense[SMP_WG * (1 + N)];
   const int piece = blockIdx.x, row = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   __shared__ double s_table[64];
@@ -501,14 +508,14 @@ __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
   // Where few elements are in front of the border a weight of each lane would be one of them at a time: they are collected, 64 and more, first.
   float* dense = s_dense + wave * (64 + 64 * N);
   double sum = 0.0;
-  uint32_t listed = 0;
+  uint32_t listed = 0, *found = s_found[wave];
   int waiting = 0;
   auto add = [&](int n) {
     const double w = s.weight(dense[waiting + lane]);
     sum += lane < n && s.heavy(w) ? w : 0.0;
   };
   const SampleBounds bound(s, r);
-  walk([&](int, const float (&v)[N]) {
+  walk([&](int i, const float (&v)[N]) {
     uint64_t front[N], some[N], any = 0, all = ~0ull, list = 0;
 #pragma unroll
     for (int e = 0; e < N; e++) {
@@ -517,8 +524,19 @@ __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
       any |= front[e], all &= front[e], list |= some[e];
     }
     if (list) {
+      uint32_t put = listed;  // (a lane's elements follow one another)
 #pragma unroll
-      for (int e = 0; e < N; e++) listed += (uint32_t)__popcll(bound.listed(v[e], some[e]));
+      for (int e = 0; e < N; e++) {
+        some[e] = bound.listed(v[e], some[e]);
+        put = __builtin_amdgcn_mbcnt_hi((uint32_t)(some[e] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)some[e], put));
+        listed += (uint32_t)__popcll(some[e]);
+      }
+#pragma unroll
+      for (int e = 0; e < N; e++) {
+        const bool in = some[e] >> lane & 1;
+        if (in && put < SMP_FOUND) found[put] = (uint32_t)(i + e);
+        put += in;
+      }
     }
     if (!~all) {
 #pragma unroll
@@ -555,6 +573,10 @@ __global__ __launch_bounds__(SMP_WG) void sample_border_kernel(SampleArgs a) {
   if (listed == 0) return;
   uint32_t to = from;
   uint32_t* list = a.list + (int64_t)row * a.V;
+  if (listed <= SMP_FOUND) {
+    for (uint32_t j = lane; j < listed; j += 64) list[to + j] = found[j];
+    return;
+  }
   walk([&](int i, const float (&v)[N]) {
     uint64_t in[N], any = 0;
 #pragma unroll
