@@ -182,15 +182,14 @@ typedef __attribute__((address_space(3))) double* lds_double;
 struct SampleScale {
   float top, step;
   double c;       // 64 / (t ln 2)
-  bool infinite;  // the maximum is: its equals weigh 1, the rest nothing
+  double at;      // the maximum; 2^1000 where it is infinite, and infinite logits count as that: its equals weigh 1, the rest nothing
   float min_w;
   lds_double table;  // 2^(j / 64), j = 0 .. 63
   // exp((v - top) / t) = 2^(n / 64) e^(r ln 2 / 64) with n + r = (v - top) c, |r| <= 1/2: the table, a power of two and five terms of the series (the
   // sixth is under 2^-54).  Off by 2^-52 and what rounding (v - top) c leaves of up to 36, 2^-47; the library's exp of a quotient took three times as long.
+  // No branches: eight of them are worked on at a time.
   __device__ __forceinline__ double weight(float v) const {
-    if (infinite) return v == INFINITY ? 1.0 : 0.0;
-    const double y = ((double)v - (double)top) * c;
-    if (!(y > -3328.0)) return 0.0;  // 52 * 64: below 2^-52
+    const double y = fmax((fmin((double)v, 0x1p1000) - at) * c, -3400.0);
     const double n = rint(y), r = (y - n) * 0.010830424696249145;
     const int i = (int)n;
     double e = fma(r, 1.0 / 120.0, 1.0 / 24.0);
@@ -198,14 +197,11 @@ struct SampleScale {
     e = fma(r, e, 0.5);
     e = fma(r, e, 1.0);
     e = fma(r, e, 1.0);
-    return __builtin_ldexp(e * table[i & 63], i >> 6);
+    e = __builtin_ldexp(e * table[i & 63], i >> 6);
+    return y > -3328.0 ? e : 0.0;  // 52 * 64: below 2^-52
   }
-  // the step of a logit; SMP_STEPS: its weight is below 2^-52
-  __device__ __forceinline__ int step_of(float v) const {
-    if (infinite) return v == INFINITY ? 0 : SMP_STEPS;
-    const float q = (top - v) * step;
-    return q < (float)SMP_STEPS ? (int)q : SMP_STEPS;
-  }
+  // the step of a logit; SMP_STEPS: its weight is below 2^-52 (inf - inf is step 0)
+  __device__ __forceinline__ int step_of(float v) const { return (int)fminf(fmaxf((top - v) * step, 0.0f), (float)SMP_STEPS); }
   // a weight in whole units, 2^51 to the weight of 1 at most: added to 2^52 they are the low bits of the sum
   __device__ __forceinline__ unsigned long long units(float v, double unit) const {
     return (unsigned long long)__double_as_longlong(fma(weight(v), unit, 0x1p52)) & 0xfffffffffffffull;
@@ -241,11 +237,11 @@ __device__ __forceinline__ SampleScale scale_of(const SampleIn& in, lds_double t
   }
   s.top = top + 0.0f;
   s.c = 92.332482616893656877 / (double)in.t;
-  s.infinite = top == INFINITY;
+  s.at = top == INFINITY ? 0x1p1000 : (double)top;
   s.min_w = in.min_p;
   // 52 ln 2 = 36.04 times t below the maximum weights end; a little more than the range, so that the last of it is in the last step
-  const float range = fminf(top - low, 36.05f * in.t) * 1.00001f;
-  s.step = range > 1e-30f ? (float)SMP_STEPS / range : 0.f;
+  const float range = fminf(fminf(top - low, 36.05f * in.t) * 1.00001f, 3e38f);
+  s.step = range > 1e-30f && top < INFINITY ? (float)SMP_STEPS / range : 1.0f;
   return s;
 }
 // What cuts a row.  few: so small a k that all it keeps is listed and ranked, and no step's mass is needed
@@ -324,7 +320,7 @@ __global__ __launch_bounds__(SMP_LAST) void sample_steps_kernel(SampleArgs a) {
   walk([&](int, const float (&v)[SampleSpan<XT>::N]) {
 #pragma unroll
     for (int e = 0; e < SampleSpan<XT>::N; e++) {
-      const int step = s.step_of(v[e]);
+      const int step = s.step_of(fmaxf(v[e], -INFINITY));  // (no number: -inf)
       if (step < SMP_STEPS) {
         atomicAdd(&s_count[step], 1u);
         if (by_mass) atomicAdd(&s_mass[step], s.units(v[e], a.unit));
