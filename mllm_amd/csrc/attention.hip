@@ -189,6 +189,34 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
   const int col = lane & 15, g = lane >> 4;
   const int rows = s.n * a.group, row0 = rt * P::ROWS * WR;
   if (row0 >= rows) return;
+  // Without a tree the tile's last token sees the most keys, and what its first one sees all of them see: keys behind the one are left out, tiles in front
+  // of the other need no masks.
+  int all = min(s.prefix, k_end);
+  if (!a.tree) {
+    const int64_t first = row0 / a.group, last = (min(rows, row0 + P::ROWS * WR) - 1) / a.group;
+    all = (int)min(s.prefix + first + 1, (int64_t)k_end);
+    k_end = (int)min(s.prefix + last + 1, (int64_t)k_end);
+  }
+  // Where a row's results go: 32-bit sizes of a row, 64-bit offsets worked out once per row.
+  const int heads = a.kv * a.group;
+  struct To {
+    void* o;
+    float* ml;
+    bool part;
+  };
+  auto where = [&](int row) {  // of 0 .. rows - 1; o null: a token beyond the host's bound
+    const int t = row / a.group, head = h * a.group + row - t * a.group;
+    if (count == 1) return To{reinterpret_cast<char*>(a.o) + ((s.first + t) * a.o_token + head * a.o_head) * (F32 ? 4 : 2), nullptr, false};
+    const int64_t at = ((int64_t)(range + b) * a.max_tokens + t) * heads + head;
+    return To{t < a.max_tokens ? a.part_o + at * D : nullptr, a.part_ml + 2 * at, true};
+  };
+  if (k_begin >= k_end && count > 1) {  // no row sees any: the join does not look at their O
+    for (int row = row0 + tid; row < min(rows, row0 + P::ROWS * WR); row += 256) {
+      const To to = where(row);
+      if (to.o) to.ml[0] = -INFINITY, to.ml[1] = 0.f;
+    }
+    return;
+  }
   // A lane loads 16-byte pieces p, p + 8, .. (p = lane % 8) of row lane / 8 of every eight rows.  Where a row's key is in the cache goes on from tile to
   // tile without a division: `page` numbers into the table, `in` bytes into the page.
   const int32_t* table = a.table + b * a.table_stride;
@@ -283,7 +311,7 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
 #pragma unroll
       for (int ks = 0; ks < KS; ks++) asm volatile("" : "+v"(fq[p][i][ks]));
   bool odd = false;  // infinities or NaNs among the values of this wave's new tokens
-  // the products of a tile, which is in that half of LDS; `border`: new tokens, or keys behind the last
+  // the products of a tile, which is in that half of LDS; `border`: keys that some rows do not see, or behind the last
   const bool busy = row0 + wr * P::ROWS < rows;  // (a wave without rows loads with the others and leaves its SIMD to them)
   auto work = [&](int k0, auto border_, auto half) {
     constexpr bool border = decltype(border_)::value;
@@ -397,8 +425,8 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
       __syncthreads();
     }
   };
-  // Tiles of prefix keys alone, in turns whose halves of LDS are constants; then (a loop of its own: its masks would take registers from the other) the rest.
-  const int plain = min(s.prefix, k_end) - KT;  // the last tile that may begin there
+  // Tiles of keys that every row sees, in turns whose halves of LDS are constants; then (a loop of its own: its masks would take registers from the other) the rest.
+  const int plain = all - KT;  // the last tile that may begin there
   int half = 0;
   while (k0 <= plain) {
     turn(std::false_type(), Lower(), Upper());
@@ -407,13 +435,14 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
     turn(std::false_type(), Upper(), Lower());
     half = 0;
   }
+  const int masked = k0;
   while (k0 < k_end) {
     turn(std::true_type(), half, half ^ 1);
     half ^= 1;
   }
   if (odd) {  // they reach the rows that see them whatever the weight (of 0 or more): no product is needed
 #pragma unroll 1
-    for (int key = max(s.prefix, k_begin); key < k_end; key++) {
+    for (int key = max(s.prefix, masked); key < k_end; key++) {
       const uint32_t at_page = __umulhi(2 * (uint32_t)key, a.page_mul) >> a.page_shift;
       const uint32_t id = (uint32_t)table[min((int)at_page, a.table_len - 1)];
       if ((key - k_begin) / 32 % WK != wk || id >= a.pages) continue;
@@ -434,19 +463,6 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
 #pragma unroll
   for (int i = 0; i < NQ; i++) l[i] = sum32(sum16(l[i]));
 
-  // Where a row's results go: 32-bit sizes of a row, 64-bit offsets worked out once per row.
-  const int heads = a.kv * a.group;
-  struct To {
-    void* o;
-    float* ml;
-    bool part;
-  };
-  auto where = [&](int row) {  // of 0 .. rows - 1; o null: a token beyond the host's bound
-    const int t = row / a.group, head = h * a.group + row - t * a.group;
-    if (count == 1) return To{reinterpret_cast<char*>(a.o) + ((s.first + t) * a.o_token + head * a.o_head) * (F32 ? 4 : 2), nullptr, false};
-    const int64_t at = ((int64_t)(range + b) * a.max_tokens + t) * heads + head;
-    return To{t < a.max_tokens ? a.part_o + at * D : nullptr, a.part_ml + 2 * at, true};
-  };
   auto put = [&](const To& to, int d, at_f32x4 x, float mm, float ll) {
     if (to.part) {
       if (!to.o) return;
@@ -517,7 +533,7 @@ template <int D, int NQ, int WR, bool F32>
 __global__ __launch_bounds__(256, (Attn<D, NQ, WR, F32>::WAVES)) void attention_kernel(AttnArgs a) {
   constexpr int KT = Attn<D, NQ, WR, F32>::KT;
   // workgroup i runs on XCD i % 8: the row tiles of a range of keys follow one another on one XCD, whose L2 they share
-  const int idx = blockIdx.x >> 3, rt = idx % a.row_tiles, place = (idx / a.row_tiles) * 8 + (blockIdx.x & 7);
+  const int idx = blockIdx.x >> 3, rt = a.row_tiles - 1 - idx % a.row_tiles, place = (idx / a.row_tiles) * 8 + (blockIdx.x & 7);
   const int h = place % a.kv, range = place / a.kv;
   Place p = {{0, 0, 0, 0}, range, 0, 0, 0};
   int tile = 0, end;
@@ -584,7 +600,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a) {
         if (k + j * G >= count) break;
         const float next = fmaxf(m, mk[j]), ref = next == -INFINITY ? 0.f : next;
         const float f = __builtin_amdgcn_exp2f(m - ref), fk = __builtin_amdgcn_exp2f(mk[j] - ref);
-        x = x * f + xk[j] * fk;
+        x = x * f + (mk[j] == -INFINITY ? at_f32x4{0.f, 0.f, 0.f, 0.f} : xk[j] * fk);
         sum = sum * f + lk[j] * fk;
         m = next;
       }

@@ -316,3 +316,30 @@ def test_workspaces_and_results_that_cannot_be_used():
     for bad in (dict(workspace=torch.empty(1 << 22, dtype=torch.uint8)), dict(workspace=wide[:, 0]), dict(out=torch.empty((1, 4, 128), device="cuda").expand(2, 4, 128))):
         with pytest.raises(AssertionError):
             c.run(**bad)
+
+
+@pytest.mark.parametrize("counts,prefixes,Hq,Hkv,D,page", [
+    ([700, 1, 333], [0, 900, 129], 4, 1, 128, 16), ([1300], [70], 2, 1, 64, 24), ([513], [0], 8, 8, 128, 64), ([400, 0, 260], [5, 9, 0], 6, 2, 256, 16), ([257], [1025], 3, 1, 64, 1)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("max_keys", [None, 1, 40000])
+def test_long_prompts(counts, prefixes, Hq, Hkv, D, page, dtype, max_keys):
+    """Tiles of tokens that see all, some or none of a range of keys; partial results in a workspace that held NaNs."""
+    announce("attention long prompts", counts, prefixes, Hq, Hkv, D, page, dtype, max_keys)
+    c = Case(counts, prefixes, Hq, Hkv, D, page, dtype, seed=sum(counts))
+    room = torch.full((1 << 28,), 0xFF, dtype=torch.uint8, device="cuda")
+    c.check(c.run(workspace=room, **({} if max_keys is None else dict(max_keys=max_keys))))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("key", [0, 63, 150, 299, 639])
+def test_later_tokens_of_a_prompt_have_no_effect(dtype, key):
+    announce("attention later tokens", dtype, key)
+    c = Case([640], [100], 4, 1, 128, 16, dtype, seed=key)
+    clean = c.want()
+    at = (int(c.table[0, (100 + key) // 16]), (100 + key) % 16)
+    c.k[at], c.v[at] = float("nan"), float("inf")
+    for max_keys in (740, 1):
+        got = c.run(max_keys=max_keys).cpu().double()
+        bound = _bound(*clean, dtype, 128, 740)
+        assert ((got[:key] - clean[0][:key]).abs() <= bound[:key]).all()
+        assert not torch.isfinite(got[key:]).any()
