@@ -638,10 +638,11 @@ struct AttnPlan {
   int nq, wr, row_tiles, ranges, min_tiles;
 };
 // Rows of a workgroup by the rows there are (tokens times query heads of a key head): 32 rows a wave (16 with fp32 queries, whose parts, and with heads of 256,
-// whose O takes the registers), waves along rows before waves along keys.  Keys are cut while there are under 1024 workgroups without that and more than
-// four tiles of keys, into ranges that give every CU two workgroups, of twice as many keys as rows at least: what a range hands over is rows, what it
-// reads keys.  One token of 32 heads, uncut / cut, us: 128 keys 7.8 / 10.1, 256 9.4 / 10.5, 320 10.4 / 11.1, 500 13.2 / 10.4, 768 16.8 / 10.5.
-// The second launch, which joins the ranges, is what cutting costs (4 of them).
+// whose O takes the registers), waves along rows before waves along keys.  Keys are cut while there are under 1024 workgroups without that and more keys
+// than four tiles and than two ranges have, into ranges that give every CU two workgroups, of twice as many keys as rows at least: what a range hands over
+// is rows, what it reads keys.  One token of 32 heads, uncut / cut, us: 128 keys 7.8 / 10.1, 256 9.4 / 10.5, 320 10.4 / 11.1, 500 13.2 / 10.4, 768 16.8 / 10.5:
+// the second launch, which joins the ranges, is what cutting costs (4 of them).  Prompts with no more keys than two ranges: four of 300 tokens 21.5 / 38,
+// eight chunks of 30 over 500 keys 24.8 / 30.0, one of 128 over 500 24.7 / 22.4; up to four ranges: one of 128 over 1000 39 / 25.
 static AttnPlan attention_plan(bool f32, int64_t B, int heads, int kv, int64_t max_tokens, int64_t max_keys, int D) {
   AttnPlan p;
   const int64_t rows = max_tokens * (heads / kv);
@@ -653,7 +654,7 @@ static AttnPlan attention_plan(bool f32, int64_t B, int heads, int kv, int64_t m
   const int kt = 64;
   p.min_tiles = (int)((2 * (rows < per ? rows : per) + kt - 1) / kt);
   const int64_t most = B * ((max_keys + p.min_tiles * kt - 1) / (p.min_tiles * kt)), wanted = (512 + kv * row_tiles - 1) / (kv * row_tiles);
-  p.ranges = B * kv * row_tiles >= 1024 || max_keys <= 4 * kt ? 0 : (int)(wanted < most ? wanted : most);
+  p.ranges = B * kv * row_tiles >= 1024 || max_keys <= (p.min_tiles > 2 ? 2 * p.min_tiles : 4) * kt ? 0 : (int)(wanted < most ? wanted : most);
   if (p.ranges <= 1 && B == 1) p.ranges = 0;
   return p;
 }
