@@ -20,6 +20,12 @@
 // the tile before them is worked on, from there into LDS.  Rows of a tile lie there with their 16-byte pieces exclusive-ored by bits of the
 // key's number, so that the 16 lanes of an operand read different banks.  Where rows and heads leave CUs idle the keys are cut into ranges,
 // whose O, maximum and sum meet in the workspace; a second launch joins them.
+//
+// What bounds it, 32 query and 8 key heads of 128: with few rows the reading of keys and values (16 fp32 tokens over up to 8000 keys each 75 us, 341 MB: 4.5
+// TB/s; a copy of 2 GB has 4.96), one token over 4097 keys (12.8 us, 16.8 MB) two launches and the loads that wait for one another in each: lengths, table, keys,
+// partial results.  32 trees of 64 tokens over up to 8192 keys (253 us, 137 GFLOP, 711 MB) the matrix and the vector pipe in turns, 30 and 40 % of the
+// time busy: registers leave two waves a SIMD, and LDS is busy 30 %.  Eight trees of 29 over up to 5000 (50 us) keys and values at 4 TB/s and, half
+// of the time, partial results (34 MB written and read) and starts.  A prompt of 8192 bf16 tokens 690 us, 800 TFLOP/s of what it has to compute.
 #include <type_traits>
 
 #include "item8.h"
@@ -193,29 +199,13 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
   // of the other need no masks.
   int all = min(s.prefix, k_end);
   if (!a.tree) {
-    const int64_t first = row0 / a.group, last = (min(rows, row0 + P::ROWS * WR) - 1) / a.group;
-    all = (int)min(s.prefix + first + 1, (int64_t)k_end);
-    k_end = (int)min(s.prefix + last + 1, (int64_t)k_end);
-  }
-  // Where a row's results go: 32-bit sizes of a row, 64-bit offsets worked out once per row.
-  const int heads = a.kv * a.group;
-  struct To {
-    void* o;
-    float* ml;
-    bool part;
-  };
-  auto where = [&](int row) {  // of 0 .. rows - 1; o null: a token beyond the host's bound
-    const int t = row / a.group, head = h * a.group + row - t * a.group;
-    if (count == 1) return To{reinterpret_cast<char*>(a.o) + ((s.first + t) * a.o_token + head * a.o_head) * (F32 ? 4 : 2), nullptr, false};
-    const int64_t at = ((int64_t)(range + b) * a.max_tokens + t) * heads + head;
-    return To{t < a.max_tokens ? a.part_o + at * D : nullptr, a.part_ml + 2 * at, true};
-  };
-  if (k_begin >= k_end && count > 1) {  // no row sees any: the join does not look at their O
-    for (int row = row0 + tid; row < min(rows, row0 + P::ROWS * WR); row += 256) {
-      const To to = where(row);
-      if (to.o) to.ml[0] = -INFINITY, to.ml[1] = 0.f;
+    int first = 0, last = s.n - 1;
+    if (rows > P::ROWS * WR) {  // (a single token has no time for divisions)
+      first = row0 / a.group;
+      last = (min(rows, row0 + P::ROWS * WR) - 1) / a.group;
     }
-    return;
+    all = min(k_end - 1 - first, s.prefix) + first + 1;  // prefix + first + 1, k_end at most
+    k_end = min(k_end - 1 - last, s.prefix) + last + 1;
   }
   // A lane loads 16-byte pieces p, p + 8, .. (p = lane % 8) of row lane / 8 of every eight rows.  Where a row's key is in the cache goes on from tile to
   // tile without a division: `page` numbers into the table, `in` bytes into the page.
@@ -463,6 +453,19 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
 #pragma unroll
   for (int i = 0; i < NQ; i++) l[i] = sum32(sum16(l[i]));
 
+  // Where a row's results go: 32-bit sizes of a row, 64-bit offsets worked out once per row.
+  const int heads = a.kv * a.group;
+  struct To {
+    void* o;
+    float* ml;
+    bool part;
+  };
+  auto where = [&](int row) {  // of 0 .. rows - 1; o null: a token beyond the host's bound
+    const int t = row / a.group, head = h * a.group + row - t * a.group;
+    if (count == 1) return To{reinterpret_cast<char*>(a.o) + ((s.first + t) * a.o_token + head * a.o_head) * (F32 ? 4 : 2), nullptr, false};
+    const int64_t at = ((int64_t)(range + b) * a.max_tokens + t) * heads + head;
+    return To{t < a.max_tokens ? a.part_o + at * D : nullptr, a.part_ml + 2 * at, true};
+  };
   auto put = [&](const To& to, int d, at_f32x4 x, float mm, float ll) {
     if (to.part) {
       if (!to.o) return;
@@ -533,7 +536,7 @@ template <int D, int NQ, int WR, bool F32>
 __global__ __launch_bounds__(256, (Attn<D, NQ, WR, F32>::WAVES)) void attention_kernel(AttnArgs a) {
   constexpr int KT = Attn<D, NQ, WR, F32>::KT;
   // workgroup i runs on XCD i % 8: the row tiles of a range of keys follow one another on one XCD, whose L2 they share
-  const int idx = blockIdx.x >> 3, rt = a.row_tiles - 1 - idx % a.row_tiles, place = (idx / a.row_tiles) * 8 + (blockIdx.x & 7);
+  const int idx = blockIdx.x >> 3, rt = idx % a.row_tiles, place = (idx / a.row_tiles) * 8 + (blockIdx.x & 7);
   const int h = place % a.kv, range = place / a.kv;
   Place p = {{0, 0, 0, 0}, range, 0, 0, 0};
   int tile = 0, end;
@@ -600,7 +603,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a) {
         if (k + j * G >= count) break;
         const float next = fmaxf(m, mk[j]), ref = next == -INFINITY ? 0.f : next;
         const float f = __builtin_amdgcn_exp2f(m - ref), fk = __builtin_amdgcn_exp2f(mk[j] - ref);
-        x = x * f + (mk[j] == -INFINITY ? at_f32x4{0.f, 0.f, 0.f, 0.f} : xk[j] * fk);
+        x = x * f + xk[j] * fk;
         sum = sum * f + lk[j] * fk;
         m = next;
       }
