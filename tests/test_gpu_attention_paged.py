@@ -2,8 +2,8 @@
 
 Bounds, relative to size = sum_j p_j |v_j| of an element.  Scores: products of bf16 parts are exact, their fp32 sums of 3 D (fp32 queries) or D terms wander by
 8 sqrt(terms) 2^-24 of the sum of the absolute terms at most (eight deviations); an error d of the scores moves the weights by 2 d.  The
-exponents' single rounding and its function: 2^-19 for arguments up to 32.  Sums over keys: 8 sqrt(keys) 2^-24.  The weights go into the product with V as two bf16
-parts with fp32 queries (2^-17 at most) and as one with bf16 queries (2^-8, half a step), whose results are rounded once more (2^-8)."""
+exponents' single rounding and its function: 2^-19 for arguments up to 32.  Sums over keys: 8 sqrt(keys) 2^-24.  The weights go into the product with V as three bf16
+parts with fp32 queries (which add up to them; 2^-17, two parts' share, is allowed) and as one with bf16 queries (2^-8, half a step), whose results are rounded once more (2^-8)."""
 import numpy as np
 import pytest
 import torch
