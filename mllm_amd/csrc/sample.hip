@@ -105,8 +105,9 @@ struct SampleSpan {
     }
   }
 };
-// A wave's vectors of a row, in the order of the index.  They go through LDS (H vectors a lane at a time, on their way all at once), so that the loop over
-// them is short: code is fetched anew by every launch, and unrolled over registers these kernels ran for as long as that took.
+// A wave's vectors of a row, in the order of the index.  They go through LDS (H vectors a lane at a time, on their way all at once while those before
+// them are worked on), so that the loop over them is short: code is fetched anew by every launch, and unrolled over registers these kernels ran for as long
+// as that took.
 template <int XT, int H>
 struct SampleWalk {
   typedef SampleSpan<XT> Span;

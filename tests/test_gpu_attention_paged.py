@@ -343,3 +343,18 @@ def test_later_tokens_of_a_prompt_have_no_effect(dtype, key):
         bound = _bound(*clean, dtype, 128, 740)
         assert ((got[:key] - clean[0][:key]).abs() <= bound[:key]).all()
         assert not torch.isfinite(got[key:]).any()
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(2, 1, 64), (4, 4, 128)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tree", [None, _random_tree])
+def test_many_ragged_sequences(Hq, Hkv, D, dtype, tree):
+    """More sequences than a wave has lanes, some of them empty, whose tiles are cut into ranges that begin and end anywhere."""
+    announce("attention many sequences", Hq, Hkv, D, dtype, tree is not None)
+    rng = np.random.default_rng(Hq)
+    counts = rng.choice([0, 1, 1, 2, 5], 190).tolist()
+    prefixes = rng.choice([0, 1, 63, 64, 65, 300, 700], 190).tolist()
+    c = Case(counts, prefixes, Hq, Hkv, D, 16, dtype, tree, seed=D)
+    want = c.want()
+    c.check(c.run(), want)
+    c.check(c.run(max_keys=1), want)
