@@ -21,7 +21,7 @@
 
 namespace mllmhip {
 
-enum { SMP_STEPS = 512, SMP_WG = 512, SMP_BIN_BITS = 9, SMP_BINS = 1 << SMP_BIN_BITS, SMP_LAST = 1024, SMP_RANKED = 128, SMP_FEW = 256, SMP_HELD = 2048,
+enum { SMP_STEPS = 512, SMP_WG = 512, SMP_BIN_BITS = 9, SMP_BINS = 1 << SMP_BIN_BITS, SMP_LAST = 1024, SMP_RANKED = 256, SMP_FEW = 256, SMP_HELD = 2048,
        SMP_PIECES = 16, SMP_HOLD = 5, SMP_FOUND = 128 };
 
 struct SampleRow {  // what launch 3 finds out about a row
@@ -386,6 +386,10 @@ struct SampleBounds {
     const bool cut = r.lo < SMP_STEPS;
     const int below = lane < 16 || !cut ? r.lo : lane < 32 ? r.mid + 1 : lane < 48 ? r.hi : r.hi + 1;
     uint32_t no = key_of(-INFINITY), yes = key_of(s.top);  // the keys that have no such step, and that have one (of step 0 and more)
+    // (about where it is, which saves most of the rounds)
+    const float away = (float)below / s.step, about = s.top - away, slack = (fabsf(s.top) + fabsf(away)) * 0x1p-21f;
+    if (s.step_of(about - slack) >= below) no = key_of(about - slack);
+    if (about + slack < s.top && s.step_of(about + slack) < below) yes = key_of(about + slack);
     while (__ballot(yes - no > 1)) {
       const uint64_t width = yes - no;
       const uint32_t probe = no + (uint32_t)(width * (j + 1) >> 4);
@@ -678,6 +682,10 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
     asm volatile("" : "+v"(index));  // (merged with the other load it would be one from a generic address)
     return index;
   };
+  bool all_ranked = false;  // the whole list, by the border by count: the one by mass finds the ranks where they are
+  Ranked own = {0, 0};
+  uint32_t rank = 0;
+  unsigned long long in_front = 0;
   auto border = [&](bool by_mass, unsigned long long want, double target, unsigned long long base) __attribute__((always_inline)) {
     uint32_t low = 0, high = 0xffffffffu, left = r.listed;
     unsigned long long counted = 0, mass = base;
@@ -686,35 +694,40 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
       if (left <= SMP_RANKED) {
         // ranks and masses in front, by comparing all with all; lanes of an element share the others
         __syncthreads();
-        if (tid == 0) s_at = 0;
-        __syncthreads();
-        for (uint32_t i = tid; i < r.listed; i += SMP_LAST) {
-          const uint32_t key = element(i);
-          if (key < low || key > high) continue;
-          s_rank[atomicAdd(&s_at, 1)] = Ranked{(unsigned long long)key << 32 | (0xffffffffu - i), mass_of(i, key)};
-        }
-        if (tid < 2) s_bin[tid] = ~0ull;
-        __syncthreads();
         const int n = (int)left;
         int size = 16;
         while (size < n) size <<= 1;
         const int share_ = SMP_LAST / size, e = tid / share_;  // 2 .. 64 lanes
         const bool live = e < n;
-        const Ranked own = s_rank[live ? e : 0];
-        uint32_t rank = 0;
-        unsigned long long before = 0;
+        if (tid < 2) s_bin[tid] = ~0ull;
+        if (!all_ranked) {
+          if (tid == 0) s_at = 0;
+          __syncthreads();
+          for (uint32_t i = tid; i < r.listed; i += SMP_LAST) {
+            const uint32_t key = element(i);
+            if (key < low || key > high) continue;
+            s_rank[atomicAdd(&s_at, 1)] = Ranked{(unsigned long long)key << 32 | (0xffffffffu - i), mass_of(i, key)};
+          }
+          __syncthreads();
+          own = s_rank[live ? e : 0];
+          rank = 0;
+          in_front = 0;
 #pragma unroll 4
-        for (int i = tid % share_; i < n; i += share_) {
-          const Ranked o = s_rank[i];
-          const bool front = o.order > own.order;
-          rank += front;
-          before += front ? o.mass : 0;
+          for (int i = tid % share_; i < n; i += share_) {
+            const Ranked o = s_rank[i];
+            const bool front = o.order > own.order;
+            rank += front;
+            in_front += front ? o.mass : 0;
+          }
+          for (int d = 1; d < share_; d <<= 1) {
+            rank += __shfl_xor(rank, d);
+            in_front += __shfl_xor(in_front, d);
+          }
+          all_ranked = left == r.listed;
+        } else {
+          __syncthreads();
         }
-        for (int d = 1; d < share_; d <<= 1) {
-          rank += __shfl_xor(rank, d);
-          before += __shfl_xor(before, d);
-        }
-        before += mass;
+        const unsigned long long before = in_front + mass;
         if (live && tid % share_ == 0) {
           // (a mass of nothing or less is reached in front of the first, which is kept all the same)
           const bool it = by_mass ? (double)(before + own.mass) >= target && ((double)before < target || (rank == 0 && counted == 0)) : counted + rank + 1 == want;
