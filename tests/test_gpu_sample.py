@@ -200,3 +200,16 @@ def test_many_kept_of_which_a_share(dtype, k, spread):
     p = np.tile(np.array([1e-6, 0.05, 0.3, 0.6, 0.9, 0.999, 0.999999, 1.0], np.float32), 3)
     t = np.repeat(np.array([0.5, 1.0, 1.7], np.float32), 8)
     _check(x, rng.random(24).astype(np.float32), t, np.full(24, k, np.int32), p, np.zeros(24, np.float32), dtype)
+
+
+@pytest.mark.parametrize("kind", ["few values", "tiny", "denormal", "huge", "one apart", "near zero", "negative", "ramp"])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_logits_of_any_size(kind, dtype):
+    """Logits whose steps have hardly a number in them or nearly all, of either sign, next to zero and next to the largest there is."""
+    announce("sample logits", kind, dtype)
+    rng = np.random.default_rng(len(kind))
+    rows, vocab = 40, 9000
+    n = rng.standard_normal((rows, vocab))
+    x = {"few values": np.round(n), "tiny": n * 1e-20, "denormal": n * 1e-39, "huge": np.clip(n * 2e38, -3.3e38, 3.3e38), "one apart": 1000 + n * 1e-3, "near zero": n * 10.0 ** rng.integers(-30, 1, n.shape),
+         "negative": -500 - np.abs(n) * 4, "ramp": np.linspace(-20, 5, vocab)[None] + 0 * n}[kind].astype(np.float32)
+    _check(x, *_settings(rng, rows), dtype)
