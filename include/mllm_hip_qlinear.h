@@ -664,7 +664,7 @@ int mllm_hip_kv_append(const mllm_hip_heads* q, const mllm_hip_heads* k, const m
  * Position i of sequence b is slot i % page_size of page block_table[b * table_stride + i / page_size] (int32); positions from table_len *
  * page_size on are not there, pages outside the cache read as zeros.  q->x, q->y: F32 or BF16, 16-byte aligned rows (weight is not
  * looked at); rows of q in no sequence stay as they are in y.  y may not be x.  head_dim 64, 128 or 256, heads a multiple of the cache's, scale > 0.
- * max_tokens and max_keys: the host's bounds of a sequence's new tokens (more are left out) and positions (any; it decides into how many
+ * max_tokens and max_keys: the host's bounds of a sequence's new tokens (those behind may be left out) and positions (any; it decides into how many
  * ranges keys are cut).  fp32 results are within fp32 sums of the formula, bf16 ones take the weights p in bf16.
  * workspace: ..._workspace_bytes (0: none), 16-byte aligned; less is MLLM_HIP_E_BADARG.  One launch, two where keys are cut. */
 size_t mllm_hip_attention_paged_workspace_bytes(int dtype, int64_t T, int64_t B, int heads, int kv_heads, int head_dim, int64_t max_tokens,

@@ -14,9 +14,9 @@
 // The row is read three times, from memory once (a row of 151 936 stays in the caches).  Weights and their sums are fp64; the masses that
 // find the border are added by atomics and therefore integers, in units of 2^-44 at 151 936 logits: sums that do not depend on an order.
 //
-// What bounds it, per launch in us: one fp32 row of 151 936, k 50 and p .9: 5, 5, 10, 11 -- reads that wait for one another and barriers, nothing of the
-// chip is busy.  128 bf16 rows, p .9: 13 (39 MB from memory), 31 (two atomics of LDS per logit and a weight of some 20 fp64 instructions), 30 (the
-// read, weights in front of the border), 20 (one workgroup a row: rounds over the listed elements); with k 50 instead 13, 14, 19, 12.
+// What bounds it, per launch in us: one fp32 row of 151 936, k 50 and p .9: 5, 5, 9, 10 -- reads that wait for one another and barriers, nothing of the
+// chip is busy.  128 bf16 rows, p .9: 13 (39 MB from memory), 31 (two atomics of LDS per logit and a weight of some 20 fp64 instructions), 28 (the
+// read, weights in front of the border), 20 (one workgroup a row: rounds over the listed elements); with k 50 instead 13, 14, 18, 11.
 #include "item8.h"
 
 namespace mllmhip {
