@@ -358,3 +358,16 @@ def test_many_ragged_sequences(Hq, Hkv, D, dtype, tree):
     want = c.want()
     c.check(c.run(), want)
     c.check(c.run(max_keys=1), want)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_many_sequences_whatever_the_bound(dtype):
+    """One launch, or ranges of keys over all sequences, by the host's bound of their lengths."""
+    announce("attention many sequences cut and not", dtype)
+    rng = np.random.default_rng(3)
+    counts = rng.choice([0, 1, 1, 1, 3], 160).tolist()
+    prefixes = rng.choice([0, 5, 64, 250, 900], 160).tolist()
+    c = Case(counts, prefixes, 8, 8, 64, 16, dtype, seed=4)
+    want = c.want()
+    for max_keys in (903, 4095, 4096, 100000):
+        c.check(c.run(max_keys=max_keys), want)
