@@ -663,6 +663,7 @@ static AttnPlan attention_plan(bool f32, int64_t B, int heads, int kv, int64_t m
   const bool full = uncut >= 1024 && (row_tiles > 2 || max_keys < 4096 || uncut >= 4096);
   p.ranges = full || max_keys <= (p.min_tiles > 2 ? 2 * p.min_tiles : 4) * kt ? 0 : (int)(wanted < most ? wanted : most);
   if (p.ranges <= 1 && B == 1) p.ranges = 0;
+  if (row_tiles > 2 && p.ranges <= B) p.ranges = 0;  // (no more workgroups than without: 16 prompts of 600 tokens of two key heads of 64 28 us, cut 48)
   return p;
 }
 // partial results of every piece, and of every sequence where its pieces are
