@@ -686,6 +686,7 @@ MLLM_API size_t mllm_hip_attention_paged_workspace_bytes(int dtype, int64_t T, i
                                                          int64_t max_keys) {
   if (!attention_sizes(dtype, T, B, heads, kv_heads, head_dim, max_tokens, max_keys) || !attention_shape(T, B, heads, kv_heads, head_dim, max_tokens, max_keys)) return 0;
   if (T == 0 || B == 0 || max_tokens == 0) return 0;
+  if (max_tokens > T) max_tokens = T;
   const AttnPlan p = attention_plan(dtype == MLLM_HIP_F32, B, heads, kv_heads, max_tokens, max_keys, head_dim);
   return attention_room(p, B, heads, max_tokens, head_dim);
 }
@@ -702,6 +703,7 @@ MLLM_API int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_
       (cache->slot_stride == 0 && cache->page_size > 1))
     return MLLM_HIP_E_SHAPE;
   if (T == 0 || B == 0 || max_tokens == 0) return 0;
+  if (max_tokens > T) max_tokens = T;
   if (!q->x || !q->y || !cache->k || !cache->v || !block_table || !cu_tokens || !prefix || table_len < 1) return MLLM_HIP_E_BADARG;
   const int wide = dtype == MLLM_HIP_F32 ? 4 : 2;
   auto al = [](const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };

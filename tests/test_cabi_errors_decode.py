@@ -126,3 +126,8 @@ def test_attention_over_its_queries_and_of_very_many_tokens():
         C.byref(_part(**dict(dict(y=P + (1 << 30)), **q))), F32, T, C.byref(_cache()), P, 8, 8, P, P, B, tokens, 0, None, 0, 0, 0.1, None, 0, None)
     assert ask(y=P) == BADARG and ask(T=2, tokens=2, y_token_stride=0) == BADARG and ask(y_head_stride=0) == BADARG
     assert ask(T=1 << 22, B=1 << 22) == SHAPE
+
+
+def test_a_bound_of_more_tokens_than_there_are():
+    size = _lib.lib().mllm_hip_attention_paged_workspace_bytes
+    assert size(BF16, 3, 2, 32, 8, 128, 4096, 5000) == size(BF16, 3, 2, 32, 8, 128, 3, 5000) > 0
