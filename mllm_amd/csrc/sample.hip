@@ -323,8 +323,21 @@ __global__ __launch_bounds__(SMP_LAST) void sample_steps_kernel(SampleArgs a) {
   for (int i = threadIdx.x; i < SMP_STEPS; i += SMP_LAST) s_count[i] = 0, s_mass[i] = 0;
   __syncthreads();
   walk([&](int, const float (&v)[SampleSpan<XT>::N]) {
+    constexpr int N = SampleSpan<XT>::N;
+    const float v0 = __uint_as_float(__builtin_amdgcn_readfirstlane(__float_as_uint(v[0])));
+    bool same = true;
 #pragma unroll
-    for (int e = 0; e < SampleSpan<XT>::N; e++) {
+    for (int e = 0; e < N; e++) same &= v[e] == v0;
+    if (!~__ballot(same)) {  // (64 N atomics on one address took 1.2 ms of a call of 128 rows of 151936 equal logits)
+      const int step = s.step_of(v0);
+      if (step < SMP_STEPS && (threadIdx.x & 63) == 0) {
+        atomicAdd(&s_count[step], 64u * N);
+        if (by_mass) atomicAdd(&s_mass[step], s.units(v0, a.unit) * (64 * N));
+      }
+      return;
+    }
+#pragma unroll
+    for (int e = 0; e < N; e++) {
       const int step = s.step_of(fmaxf(v[e], -INFINITY));  // (no number: -inf)
       if (step < SMP_STEPS) {
         atomicAdd(&s_count[step], 1u);
@@ -746,9 +759,16 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
         if (tid == 0) s_ends[0] = 0xffffffffu, s_ends[1] = 0;
         __syncthreads();
         uint32_t least = 0xffffffffu, most = 0;
-        for (uint32_t i = tid; i < r.listed; i += SMP_LAST) {
-          const uint32_t key = element(i);
-          least = min(least, key), most = max(most, key);
+        if (kept_in_lds) {
+          for (uint32_t i = tid; i < r.listed; i += SMP_LAST) least = min(least, s_element[i]), most = max(most, s_element[i]);
+        } else {
+          for (uint32_t i = tid; i < r.listed; i += SMP_LAST * 8) {
+            float v[8];
+#pragma unroll
+            for (int j = 0; j < 8; j++) v[j] = span.at((int)list[min(i + j * SMP_LAST, r.listed - 1)]);
+#pragma unroll
+            for (int j = 0; j < 8; j++) least = min(least, key_of(v[j])), most = max(most, key_of(v[j]));
+          }
         }
 #pragma unroll 1
         for (int d = 32; d; d >>= 1) least = min(least, (uint32_t)__shfl_xor((int)least, d)), most = max(most, (uint32_t)__shfl_xor((int)most, d));
@@ -758,6 +778,24 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
         }
         __syncthreads();
         low = s_ends[0], high = s_ends[1];
+      }
+      if (low == high) {  // very many equal logits: the first so many of them, found by their number in the list, which is in the order of the index
+        const unsigned long long w = units(of_key(high));
+        const double over = w ? ceil((target - (double)mass) / (double)w) : (double)left;
+        const unsigned long long equals = by_mass ? (unsigned long long)fmin(fmax(over, 1.0), (double)left) : want - counted;
+        if (left == r.listed) return SampleBorder{high, index_of((uint32_t)equals - 1), mass + w * equals};
+        __syncthreads();
+        const uint32_t per = (r.listed + SMP_LAST - 1) / SMP_LAST, i0 = min(r.listed, tid * per), i1 = min(r.listed, i0 + per);
+        unsigned long long have = 0;
+        for (uint32_t i = i0; i < i1; i++) have += element(i) == high;
+        const unsigned long long up = running<unsigned long long, SMP_LAST>(have, s_wave);
+        if (up >= equals && up - have < equals) {
+          unsigned long long n = up - have;
+          for (uint32_t i = i0; i < i1; i++)
+            if (element(i) == high && ++n == equals) s_at = index_of(i);
+        }
+        __syncthreads();
+        return SampleBorder{high, s_at, mass + w * equals};
       }
       const uint32_t width = high - low;
       const int bits = width ? 32 - __clz(width) : 0, shift = max(0, bits - SMP_BIN_BITS);
@@ -769,8 +807,17 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
         const uint32_t key = element(i);
         if (key < low || key > high) continue;
         const uint32_t bin = (high - key) >> shift;
+        const unsigned long long w = mass_of(i, key);
+        const uint64_t here = __ballot(true);
+        if (__ballot(key == (uint32_t)__builtin_amdgcn_readfirstlane(key)) == here) {  // (one address)
+          if (lane == __builtin_ctzll(here)) {
+            atomicAdd(&s_count[bin], (uint32_t)__popcll(here));
+            atomicAdd(&s_mass[bin], w * __popcll(here));
+          }
+          continue;
+        }
         atomicAdd(&s_count[bin], 1u);
-        atomicAdd(&s_mass[bin], mass_of(i, key));
+        atomicAdd(&s_mass[bin], w);
       }
       __syncthreads();
       if (wave == 0) {  // a lane's bins, the lanes' sums, the lane that crosses, its bin
@@ -807,23 +854,6 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
       left = (uint32_t)s_bin[2];
       high -= (uint32_t)found << shift;
       low = max(low, high - min(high, (1u << shift) - 1));
-      if (shift == 0 && left > SMP_RANKED) {  // very many equal logits: the first so many of them, found by their number in the list, which is in the order of the index
-        const unsigned long long w = units(of_key(high));
-        const double over = w ? ceil((target - (double)mass) / (double)w) : (double)left;
-        const unsigned long long equals = by_mass ? (unsigned long long)fmin(fmax(over, 1.0), (double)left) : want - counted;
-        __syncthreads();
-        const uint32_t per = (r.listed + SMP_LAST - 1) / SMP_LAST, i0 = min(r.listed, tid * per), i1 = min(r.listed, i0 + per);
-        unsigned long long have = 0;
-        for (uint32_t i = i0; i < i1; i++) have += element(i) == high;
-        const unsigned long long up = running<unsigned long long, SMP_LAST>(have, s_wave);
-        if (up >= equals && up - have < equals) {
-          unsigned long long n = up - have;
-          for (uint32_t i = i0; i < i1; i++)
-            if (element(i) == high && ++n == equals) s_at = index_of(i);
-        }
-        __syncthreads();
-        return SampleBorder{high, s_at, mass + w * equals};
-      }
     }
   };
   uint32_t edge_key = 0;  // what is above it is kept, and what equals it up to index `last`
@@ -889,7 +919,17 @@ __global__ __launch_bounds__(SMP_LAST) void sample_token_kernel(SampleArgs a) {
     __syncthreads();
     for (int i = wave; i < parts; i += W) {
       double sum = 0.0;
-      for (uint32_t j = s_from[i] + lane; j < s_from[i + 1]; j += 64) sum += kept(index_of(j), of_key(element(j)));
+      for (uint32_t j = s_from[i] + lane; j < s_from[i + 1]; j += 64 * 4) {
+        int index[4];
+        float v[4];
+#pragma unroll
+        for (int e = 0; e < 4; e++) index[e] = (int)list[min(j + e * 64, r.listed - 1)];
+#pragma unroll
+        for (int e = 0; e < 4; e++) v[e] = span.at(index[e]);
+#pragma unroll
+        for (int e = 0; e < 4; e++)
+          if (j + e * 64 < s_from[i + 1]) sum += kept(index[e], v[e]);
+      }
 #pragma unroll 1
       for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
       if (lane == 0) s_part[i] += sum;

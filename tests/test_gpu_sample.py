@@ -213,3 +213,18 @@ def test_logits_of_any_size(kind, dtype):
     x = {"few values": np.round(n), "tiny": n * 1e-20, "denormal": n * 1e-39, "huge": np.clip(n * 2e38, -3.3e38, 3.3e38), "one apart": 1000 + n * 1e-3, "near zero": n * 10.0 ** rng.integers(-30, 1, n.shape),
          "negative": -500 - np.abs(n) * 4, "ramp": np.linspace(-20, 5, vocab)[None] + 0 * n}[kind].astype(np.float32)
     _check(x, *_settings(rng, rows), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_rows_of_few_different_logits(dtype):
+    """All equal, two values in turns, long runs of equals, one step's worth of many: lists that are longer than what is kept in LDS."""
+    announce("sample equal logits", dtype)
+    rng = np.random.default_rng(21)
+    vocab = 70001
+    i = np.arange(vocab)
+    kinds = [0 * i, i % 2, i // 4096 % 3, (i // 512 == 7) * 2.0, np.round(rng.standard_normal(vocab)), 1 + (i % 5) / 1024, np.where(i < 60000, 3.0, -np.inf), np.where(i % 3 == 0, np.nan, 0.5)]
+    x = np.repeat(np.stack(kinds).astype(np.float32), 5, 0)
+    rows = len(x)
+    k = np.tile(np.array([0, 50, 255, 5000, 69000], np.int32), len(kinds))
+    for p in (1.0, 0.9, 0.3):
+        _check(x, rng.random(rows).astype(np.float32), rng.choice([0.5, 1.0, 3.0], rows).astype(np.float32), k, np.full(rows, p, np.float32), np.zeros(rows, np.float32), dtype)
