@@ -300,7 +300,7 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
     for (int i = 0; i < NQ; i++)
 #pragma unroll
       for (int ks = 0; ks < KS; ks++) asm volatile("" : "+v"(fq[p][i][ks]));
-  bool odd = false;  // infinities or NaNs among the values of this wave's new tokens
+  bool odd = false;  // infinities or NaNs among the values of this wave's keys in tiles with masks, of the prefix or of new tokens
   // the products of a tile, which is in that half of LDS; `border`: keys that some rows do not see, or behind the last
   const bool busy = row0 + wr * P::ROWS < rows;  // (a wave without rows loads with the others and leaves its SIMD to them)
   auto work = [&](int k0, auto border_, auto half) {
@@ -432,7 +432,7 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
   }
   if (odd) {  // they reach the rows that see them whatever the weight (of 0 or more): no product is needed
 #pragma unroll 1
-    for (int key = max(s.prefix, masked); key < k_end; key++) {
+    for (int key = masked; key < k_end; key++) {
       const uint32_t at_page = __umulhi(2 * (uint32_t)key, a.page_mul) >> a.page_shift;
       const uint32_t id = (uint32_t)table[min((int)at_page, a.table_len - 1)];
       if ((key - k_begin) / 32 % WK != wk || id >= a.pages) continue;
