@@ -660,7 +660,8 @@ int mllm_hip_kv_append(const mllm_hip_heads* q, const mllm_hip_heads* k, const m
  * bits that are not there count as 0.  tree NULL: j <= t.  One token a sequence is a decode step, a tree the verification
  * of drafted tokens, many tokens without a tree a (chunk of a) prompt.
  *   o[t][h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * (q . k_j) - max), of key head h / (heads / kv heads); a token that sees
- *   nothing, or scores of -inf alone: zeros.  What a token does not see has no effect on it, NaN included.
+ *   nothing, or scores of -inf alone: zeros.  What a token does not see has no effect on it, NaN included.  An infinity or a NaN among the values that it
+ *   sees makes that element of its result infinite or NaN, whatever the weight.
  * Position i of sequence b is slot i % page_size of page block_table[b * table_stride + i / page_size] (int32); positions from table_len *
  * page_size on are not there, pages outside the cache read as zeros.  q->x, q->y: F32 or BF16, 16-byte aligned rows (weight is not
  * looked at); rows of q in no sequence stay as they are in y.  y may not be x.  head_dim 64, 128 or 256, heads a multiple of the cache's, scale > 0.

@@ -184,6 +184,55 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t v) {
   return ((v & 0x7f80u) == 0x7f80u ? 0u : v & 0xffffu) | ((v & 0x7f800000u) == 0x7f800000u ? 0u : v & 0xffff0000u);
 }
 
+// Infinities and NaNs among the values make that element of the rows that see them infinite or NaN, whatever the weight: it is their sum.  What the matrix products
+// leave there is NaN where a weight is too small for its type (or a part of one is 0), and without them where they were taken out for rows that do not see
+// them (in tiles with masks; the sum of the weights has its sign set then).  So results of either kind are looked at once more, behind everything else: a lane's elements
+// d .. d + 3 of query head `head`, token `token`, where it says so in `look` (LOOK_WHOLE: among all keys, LOOK_MASKED: those of tiles with masks).  The lanes that are
+// there go through the values of one result after the other together: a call of one token over 4096 keys 19 us, with a NaN among them 80 (a lane for each result: 1043).
+enum { LOOK_MASKED = 1, LOOK_WHOLE = 2 };
+__device__ __forceinline__ uint32_t look_at(at_f32x4 x, float sum, uint32_t sign) {
+  const float most = larger(larger(fabsf(x[0]), fabsf(x[1])), larger(fabsf(x[2]), fabsf(x[3])));
+  return sum != sum ? 0 : !(most < INFINITY) ? LOOK_WHOLE : sign >> 31;  // (scores that are NaN make that of the whole row)
+}
+template <bool F32>
+__device__ __forceinline__ void put_infinities(const AttnArgs& a, const Seq& s, int b, uint32_t look, int head_, int token_, int d_) {
+  const uint64_t active = __ballot(true);
+  const int lanes = __popcll(active), rank = __builtin_amdgcn_mbcnt_hi((uint32_t)(active >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)active, 0));
+  const int32_t* table = a.table + b * a.table_stride;
+#pragma unroll 1
+  for (uint64_t left = __ballot(look); left; left &= left - 1) {
+    const int who = __builtin_ctzll(left), head = __builtin_amdgcn_readlane(head_, who), token = __builtin_amdgcn_readlane(token_, who), d = __builtin_amdgcn_readlane(d_, who);
+    const uint16_t* v = a.v + head / a.group * a.head_stride + d;
+    const int end = a.tree ? s.keys : (int)min((int64_t)s.keys, (int64_t)s.prefix + token + 1);
+    uint32_t nans = 0, above = 0, below = 0;  // which of the elements have a NaN, an infinity, one below 0
+    for (int k0 = __builtin_amdgcn_readlane(look, who) == LOOK_WHOLE ? 0 : min(s.prefix, s.keys - 1) & ~63; k0 < end && nans != 15; k0 += lanes) {
+      const int key = min(k0 + rank, end - 1);
+      const uint32_t page = __umulhi(2 * (uint32_t)key, a.page_mul) >> a.page_shift, id = (uint32_t)table[min((int)page, a.table_len - 1)];
+      const uint64_t at = (uint64_t)id * a.page_bytes + (((uint32_t)key - page * a.page) * a.slot_bytes + (uint64_t)(uintptr_t)v);
+      const u32x2 x = *reinterpret_cast<const __attribute__((address_space(1))) u32x2*>(id < a.pages ? at : (uint64_t)(uintptr_t)g_zero_row);
+      const bool has = (odd_pair(x.x) || odd_pair(x.y)) && (seen_keys(a, s, key, token) & 1);
+      if (!__ballot(has)) continue;
+      const uint32_t w[4] = {x.x << 16, x.x & 0xffff0000u, x.y << 16, x.y & 0xffff0000u};
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        if (__ballot(has && (w[e] & 0x7fffffffu) > 0x7f800000u)) nans |= 1u << e;
+        if (__ballot(has && w[e] == 0x7f800000u)) above |= 1u << e;
+        if (__ballot(has && w[e] == 0xff800000u)) below |= 1u << e;
+      }
+    }
+    nans |= above & below;
+    if ((int)(threadIdx.x & 63) != who) continue;
+    const int64_t to = (s.first + token) * a.o_token + head * a.o_head + d;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      if (!((nans | above | below) >> e & 1)) continue;
+      const uint32_t sum = nans >> e & 1 ? 0x7fc00000u : above >> e & 1 ? 0x7f800000u : 0xff800000u;
+      if (F32) reinterpret_cast<uint32_t*>(a.o)[to + e] = sum;
+      else reinterpret_cast<uint16_t*>(a.o)[to + e] = (uint16_t)(sum >> 16);
+    }
+  }
+}
+
 // The part of sequence b with keys k_begin .. k_end - 1, for key head h and row tile rt; `range` and `count` say where partial results go
 template <int D, int NQ, int WR, bool F32>
 __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s, int b, int h, int rt, int k_begin, int k_end, int range, int count) {
@@ -300,7 +349,7 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
     for (int i = 0; i < NQ; i++)
 #pragma unroll
       for (int ks = 0; ks < KS; ks++) asm volatile("" : "+v"(fq[p][i][ks]));
-  bool odd = false;  // infinities or NaNs among the values of this wave's keys in tiles with masks, of the prefix or of new tokens
+  bool odd = false;  // infinities or NaNs among the values of this wave's keys in tiles with masks
   // the products of a tile, which is in that half of LDS; `border`: keys that some rows do not see, or behind the last
   const bool busy = row0 + wr * P::ROWS < rows;  // (a wave without rows loads with the others and leaves its SIMD to them)
   auto work = [&](int k0, auto border_, auto half) {
@@ -370,7 +419,7 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
         const at_s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(s_v + at));
         const at_s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(s_v + at + 4 * D));
         u32x4 vt = __builtin_bit_cast(u32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7));
-        if (border) {  // a value that a row does not see must not reach it, and 0 * NaN would: such values are taken out here and added below
+        if (border) {  // a value that a row does not see must not reach it, and 0 * NaN would: such values are taken out here and come back below
           if (__ballot(odd_pair(vt.x) || odd_pair(vt.y) || odd_pair(vt.z) || odd_pair(vt.w))) {
             vt = u32x4{finite_pair(vt.x), finite_pair(vt.y), finite_pair(vt.z), finite_pair(vt.w)};
             odd = true;
@@ -425,30 +474,9 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
     turn(std::false_type(), Upper(), Lower());
     half = 0;
   }
-  const int masked = k0;
   while (k0 < k_end) {
     turn(std::true_type(), half, half ^ 1);
     half ^= 1;
-  }
-  if (odd) {  // they reach the rows that see them whatever the weight (of 0 or more): no product is needed
-#pragma unroll 1
-    for (int key = masked; key < k_end; key++) {
-      const uint32_t at_page = __umulhi(2 * (uint32_t)key, a.page_mul) >> a.page_shift;
-      const uint32_t id = (uint32_t)table[min((int)at_page, a.table_len - 1)];
-      if ((key - k_begin) / 32 % WK != wk || id >= a.pages) continue;
-      const uint64_t at = (uint64_t)id * a.page_bytes + (((uint32_t)key - at_page * a.page) * a.slot_bytes + (uint64_t)(uintptr_t)(a.v + h * a.head_stride) + g * 8);
-#pragma unroll
-      for (int i = 0; i < NQ; i++) {
-        const bool seen = seen_keys(a, s, key, token[i]) & 1;
-#pragma unroll
-        for (int d = 0; d < DT; d++) {
-          const u32x2 v = *reinterpret_cast<const __attribute__((address_space(1))) u32x2*>(at + 32 * d);
-          const uint32_t w[4] = {v.x << 16, v.x & 0xffff0000u, v.y << 16, v.y & 0xffff0000u};
-#pragma unroll
-          for (int e = 0; e < 4; e++) acc[i][d][e] += seen && (w[e] & 0x7f800000u) == 0x7f800000u ? __uint_as_float(w[e]) : 0.f;
-        }
-      }
-    }
   }
 #pragma unroll
   for (int i = 0; i < NQ; i++) l[i] = sum32(sum16(l[i]));
@@ -466,20 +494,27 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
     const int64_t at = ((int64_t)(range + b) * a.max_tokens + t) * heads + head;
     return To{t < a.max_tokens ? a.part_o + at * D : nullptr, a.part_ml + 2 * at, true};
   };
-  auto put = [&](const To& to, int d, at_f32x4 x, float mm, float ll) {
+  // `ll`: the sum of the weights, its sign as l's.  How the result has to be looked at once more
+  auto put = [&](const To& to, int d, at_f32x4 x, float mm, float ll) -> uint32_t {
     if (to.part) {
-      if (!to.o) return;
+      if (!to.o) return 0;
       *reinterpret_cast<at_f32x4*>(reinterpret_cast<float*>(to.o) + d) = x;
       if (d == 0) {
         to.ml[0] = mm;
         to.ml[1] = ll;
       }
-    } else {
-      x *= ll > 0.f ? 1.0f / ll : (ll == 0.f ? 0.f : ll);  // (no key seen: zeros; a NaN stays)
-      if (F32) *reinterpret_cast<at_f32x4*>(reinterpret_cast<float*>(to.o) + d) = x;
-      else *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(to.o) + d) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+      return 0;
     }
+    const float sum = fabsf(ll);
+    x *= sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);  // (no key seen: zeros; a NaN stays)
+    if (F32) *reinterpret_cast<at_f32x4*>(reinterpret_cast<float*>(to.o) + d) = x;
+    else *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(to.o) + d) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+    return look_at(x, sum, __float_as_uint(ll));
   };
+#pragma unroll
+  for (int i = 0; i < NQ; i++) l[i] = odd ? -l[i] : l[i];
+  uint32_t look = 0;  // two bits for every result of a lane
+  constexpr int HALF = D / 2, IT = 16 * (HALF / 4) / (WK * 64);  // (half of O at a time: four waves' rows of 256 elements would not fit)
   // The waves along keys meet in LDS, 16 rows at a time: O of a row at [row][HALF], its maximum and sum apart.
   if constexpr (WK == 1) {
 #pragma unroll
@@ -488,13 +523,13 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
       if (row >= rows) continue;
       const To to = where(row);
 #pragma unroll
-      for (int d = 0; d < DT; d++) put(to, 16 * d + 4 * g, acc[i][d], m[i], l[i]);
+      for (int d = 0; d < DT; d++) look |= put(to, 16 * d + 4 * g, acc[i][d], m[i], l[i]) << 2 * (i * DT + d);
     }
   } else {
-    constexpr int HALF = D / 2;  // (half of O at a time: four waves' rows of 256 elements would not fit)
     float* so = reinterpret_cast<float*>(s_k);   // [wave][16][HALF]
     float* sm = reinterpret_cast<float*>(s_v);   // [wave][16][2]
     static_assert(4 * 16 * HALF * 4 <= KT * D * 2 && 4 * 16 * 2 * 4 <= KT * D * 2, "");
+    static_assert(16 * (HALF / 4) == IT * WK * 64 && NQ * 2 * IT <= 16, "");
 #pragma unroll
     for (int i = 0; i < NQ; i++) {
 #pragma unroll
@@ -508,8 +543,9 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
         }
         __syncthreads();
         // the WK waves of row block w: every one of them joins a share of its 16 rows
-        for (int e = wk * 64 + lane; e < 16 * (HALF / 4); e += WK * 64) {
-          const int r = e / (HALF / 4), p = e % (HALF / 4);
+#pragma unroll
+        for (int it = 0; it < IT; it++) {
+          const int e = wk * 64 + lane + it * WK * 64, r = e / (HALF / 4), p = e % (HALF / 4);
           const int row = row0 + wr * P::ROWS + i * 16 + r;
           if (row >= rows) continue;
           float top = -INFINITY;
@@ -518,16 +554,34 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
           const float ref = top == -INFINITY ? 0.f : top;
           at_f32x4 x = {0.f, 0.f, 0.f, 0.f};
           float sum = 0.f;
+          uint32_t sign = 0;
 #pragma unroll
           for (int w = 0; w < WK; w++) {
             const int at = (w * WR + wr) * 16 + r;
             const float f = __builtin_amdgcn_exp2f(sm[at * 2] - ref);
-            sum += sm[at * 2 + 1] * f;
+            sum += fabsf(sm[at * 2 + 1]) * f;
+            sign |= __float_as_uint(sm[at * 2 + 1]);
             x += *reinterpret_cast<const at_f32x4*>(so + at * HALF + (p ^ (r & 7)) * 4) * f;
           }
-          put(where(row), part * HALF + p * 4, x, top, sum);
+          look |= put(where(row), part * HALF + p * 4, x, top, __uint_as_float((__float_as_uint(sum) & 0x7fffffffu) | (sign & 0x80000000u))) << 2 * ((i * 2 + part) * IT + it);
         }
       }
+    }
+  }
+  if (__builtin_expect(__ballot(look) != 0, 0)) {
+#pragma unroll 1
+    for (int n = 0; n < (WK == 1 ? NQ * DT : NQ * 2 * IT); n++) {
+      int row, d;
+      if (WK == 1) {
+        row = n / DT * 16 + col;
+        d = n % DT * 16 + 4 * g;
+      } else {
+        const int e = wk * 64 + lane + n % IT * (WK * 64);
+        row = n / (2 * IT) * 16 + e / (HALF / 4);
+        d = n / IT % 2 * HALF + e % (HALF / 4) * 4;
+      }
+      row += row0 + wr * P::ROWS;
+      put_infinities<F32>(a, s, b, look >> 2 * n & 3, h * a.group + row % a.group, row / a.group, d);
     }
   }
 }
@@ -583,6 +637,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a) {
   const bool live = i < min((int64_t)s.n * heads, all);
   const int d = tid % L * 4;
   float m = -INFINITY, sum = 0.f;
+  uint32_t sign = 0;  // of any piece's sum
   at_f32x4 x = {0.f, 0.f, 0.f, 0.f};
   if (live) {
     const float* ml = a.part_ml + 2 * (first * all + i);
@@ -604,7 +659,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a) {
         const float next = fmaxf(m, mk[j]), ref = next == -INFINITY ? 0.f : next;
         const float f = __builtin_amdgcn_exp2f(m - ref), fk = __builtin_amdgcn_exp2f(mk[j] - ref);
         x = x * f + xk[j] * fk;
-        sum = sum * f + lk[j] * fk;
+        sum = sum * f + fabsf(lk[j]) * fk;
+        sign |= __float_as_uint(lk[j]);
         m = next;
       }
     }
@@ -613,7 +669,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a) {
     s_x[tid] = x;
     if (d == 0) {
       s_ml[tid / L * 2] = m;
-      s_ml[tid / L * 2 + 1] = sum;
+      s_ml[tid / L * 2 + 1] = __uint_as_float((__float_as_uint(sum) & 0x7fffffffu) | (sign & 0x80000000u));
     }
     __syncthreads();
     if (group) return;
@@ -624,9 +680,10 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a) {
     x = at_f32x4{0.f, 0.f, 0.f, 0.f};
     sum = 0.f;
     for (int k = 0; k < G; k++) {
-      const float f = __builtin_amdgcn_exp2f(s_ml[(k * PER + row) * 2] - ref);
+      const float f = __builtin_amdgcn_exp2f(s_ml[(k * PER + row) * 2] - ref), part = s_ml[(k * PER + row) * 2 + 1];
       x += s_x[tid + k * PER * L] * f;
-      sum += s_ml[(k * PER + row) * 2 + 1] * f;
+      sum += fabsf(part) * f;
+      sign |= __float_as_uint(part);
     }
   }
   if (!live) return;
@@ -634,6 +691,8 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a) {
   const int64_t token = i / heads, to = (s.first + token) * a.o_token + (i - token * heads) * a.o_head + d;
   if (F32) *reinterpret_cast<at_f32x4*>(reinterpret_cast<float*>(a.o) + to) = x;
   else *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(a.o) + to) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+  const uint32_t look = look_at(x, sum, sign);
+  if (__builtin_expect(__ballot(look) != 0, 0)) put_infinities<F32>(a, s, b, look, (int)(i - token * heads), (int)token, d);
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------
