@@ -379,17 +379,44 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
       at_bf16x8 fp[P::PPARTS][NQ];
 #pragma unroll
       for (int i = 0; i < NQ; i++) {
-        float y[8] = {sa[i][0], sa[i][1], sa[i][2], sa[i][3], sb[i][0], sb[i][1], sb[i][2], sb[i][3]};
-        if (border) {
-          const uint32_t see = seen_keys(a, s, key0 + 8 * g, token[i]);
+        float y[8], top;
+        auto scores = [&](const at_f32x4& a0, const at_f32x4& b0) {
 #pragma unroll
-          for (int j = 0; j < 8; j++) y[j] = see >> j & 1 ? y[j] : -INFINITY;
-        }
-        // (maximum, which hands a NaN on, is one instruction for three; fmaxf quiets each of its operands first)
-        float top = larger(larger(larger(y[0], y[1]), larger(y[2], y[3])), larger(larger(y[4], y[5]), larger(y[6], y[7])));
-        top = across<16>(top);
-        top = across<32>(top) * a.c;
-        if (__ballot(top > m[i] + 8.f)) {  // (weights of up to 2^8 do as well: most steps leave O alone)
+          for (int j = 0; j < 4; j++) y[j] = a0[j], y[4 + j] = b0[j];
+          if (border) {
+            const uint32_t see = seen_keys(a, s, key0 + 8 * g, token[i]);
+#pragma unroll
+            for (int j = 0; j < 8; j++) y[j] = see >> j & 1 ? y[j] : -INFINITY;
+          }
+          // (maximum, which hands a NaN on, is one instruction for three; fmaxf quiets each of its operands first)
+          top = larger(larger(larger(y[0], y[1]), larger(y[2], y[3])), larger(larger(y[4], y[5]), larger(y[6], y[7])));
+          top = across<16>(top);
+          top = across<32>(top) * a.c;
+        };
+        scores(sa[i], sb[i]);
+        if (__ballot(F32 ? !(top <= m[i] + 8.f) : top > m[i] + 8.f)) {  // (weights of up to 2^8 do as well: most steps leave O alone)
+          if constexpr (F32) {
+            // An infinite element of a key makes a NaN with the second and third part of a query's, which may be 0: it counts with the first alone, which
+            // has the sign.  Such scores, and those that are NaN anyway, are formed once more.
+            if (__builtin_expect(__ballot(top != top) != 0, 0)) {
+              at_f32x4 ta = {0.f, 0.f, 0.f, 0.f}, tb = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int ks = 0; ks < KS; ks++) {
+                const int at = ra * D + ((4 * ks + g) ^ x) * 8;
+                const u32x4 ka = *reinterpret_cast<const u32x4*>(s_k + at), kb = *reinterpret_cast<const u32x4*>(s_k + at + 4 * D);
+                const at_bf16x8 fa = frag(u32x4{finite_pair(ka.x), finite_pair(ka.y), finite_pair(ka.z), finite_pair(ka.w)}),
+                                fb = frag(u32x4{finite_pair(kb.x), finite_pair(kb.y), finite_pair(kb.z), finite_pair(kb.w)});
+#pragma unroll
+                for (int p = P::PARTS - 1; p > 0; p--) {
+                  ta = mma(fa, fq[p][i][ks], ta);
+                  tb = mma(fb, fq[p][i][ks], tb);
+                }
+                ta = mma(frag(ka), fq[0][i][ks], ta);
+                tb = mma(frag(kb), fq[0][i][ks], tb);
+              }
+              scores(ta, tb);
+            }
+          }
           const float next = fmaxf(m[i], top), fix = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - next);
           m[i] = next;
           l[i] *= fix;
