@@ -114,8 +114,13 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
         ss = group_sum<G>(ss);
         // 1 / sqrt by the hardware's (off by an ulp) and a step of Newton's: within an ulp, in a fifth of the instructions of a division and a root
         const float m = fmaf(ss, a.inv_d, a.eps);
-        float rms = __builtin_amdgcn_rsqf(m);
-        rms = m > 0.f && m < INFINITY ? fmaf(rms * 0.5f, fmaf(-m * rms, rms, 1.0f), rms) : rms;
+        auto root = [](float x) {
+          const float r = __builtin_amdgcn_rsqf(x);
+          return fmaf(r * 0.5f, fmaf(-x * r, r, 1.0f), r);
+        };
+        const bool normal = __builtin_amdgcn_classf(m, 1 << 8);
+        float rms = normal ? root(m) : __builtin_amdgcn_rsqf(m);
+        if (__builtin_expect(__ballot(!normal) != 0, 0)) rms = m > 0.f && m < 0x1p-126f ? root(m * 0x1p64f) * 0x1p32f : rms;  // (the hardware's takes what is subnormal for 0)
         if (q.live) {
           const float4 w0 = *reinterpret_cast<const float4*>(q.g.w + e), w1 = *reinterpret_cast<const float4*>(q.g.w + e + 4);
           const float w[8] = {w0.x, w0.y, w0.z, w0.w, w1.x, w1.y, w1.z, w1.w};
