@@ -679,8 +679,11 @@ int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_t T, cons
  *   w_i = exp((x_i - max) / temperature), 0 below 2^-52; in descending order (equal logits: lowest index first) the first top_k are kept (0 or
  *   less: all), of these the shortest beginning whose mass is top_p of theirs or more (at least one; 1 or more: all), of these the ones with
  *   w_i >= min_p (1 at most).  The token is the first kept one, in the order of the index, at which the running sum exceeds u times the sum of what is kept.
+ * The masses that top_p compares are sums of weights that are each rounded to a unit: 2^-(62 - ceil(log2 vocab)) (151 936 logits: 2^-44), 2^-51 where that is smaller.  The
+ * border is where masses that are off by up to vocab / 2 units put it, which in a long run of very light logits may be some of them away from the exact one.
  * temperature of 0 or less: the largest logit's lowest index.  A NaN counts as -inf; infinite maxima share the weight; a row without a logit
- * above -inf gives -1.  Settings are fp32 / int32 [rows] each; NULL: 1, 0, 1, 0.  Sums in fp64, the same result on every call.
+ * above -inf gives -1.  Settings are fp32 / int32 [rows] each; NULL: 1, 0, 1, 0.  Weights (within 2^-46 of themselves) and the sums of what is kept
+ * are fp64, the result is the same on every call.
  * vocab <= 2^24, rows <= 65535.  workspace: ..._workspace_bytes, 16-byte aligned; less is MLLM_HIP_E_BADARG.  Up to four launches. */
 size_t mllm_hip_sample_workspace_bytes(int64_t rows, int64_t vocab);
 int mllm_hip_sample(const void* logits, int dtype, int64_t row_stride, int64_t rows, int64_t vocab, const float* u, const float* temperature,

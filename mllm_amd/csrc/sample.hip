@@ -11,8 +11,10 @@
 //   3  the step (or steps) the border lies in; sums of the weights above it, piece by piece; the elements within it, in order of their index
 //   4  one workgroup per row: the border itself, by counts and masses over ever narrower ranges of the bits of those elements' logits; the piece
 //      in which the running sum crosses u, and the element
-// The row is read three times, from memory once (a row of 151 936 stays in the caches).  Weights and their sums are fp64; the masses that
-// find the border are added by atomics and therefore integers, in units of 2^-44 at 151 936 logits: sums that do not depend on an order.
+// The row is read three times, from memory once (a row of 151 936 stays in the caches).  Weights and the sums of what is kept are fp64; the masses that
+// find the border are added by atomics and therefore integers, in units of 2^-44 at 151 936 logits (2^-38 at 2^24): sums that do not depend on an order.  Each
+// weight is rounded to a unit, so a mass is off by up to half a unit for every logit in it, 2^-28 of a row of 151 936 whose heaviest weighs 1; top_p itself has
+// 24 bits.  Seen in the border: 75 000 equal logits of 2^-30 behind a peak, two of them more or fewer.
 //
 // What bounds it, per launch in us: one fp32 row of 151 936, k 50 and p .9: 5, 5, 9, 10 -- reads that wait for one another and barriers, nothing of the
 // chip is busy.  128 bf16 rows, p .9: 13 (39 MB from memory), 31 (two atomics of LDS per logit and a weight of some 20 fp64 instructions), 28 (the
