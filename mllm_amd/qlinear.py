@@ -685,7 +685,7 @@ def attention_paged(q, k_cache, v_cache, block_table, cu_tokens, prefix, max_tok
     """softmax(scale * q k^T) v of new tokens, which the cache holds already, over their sequences: q [T, Hq, D] fp32 or bf16 (D 64, 128 or 256), rows
     cu_tokens[b] .. cu_tokens[b + 1] - 1 (int32 [B + 1]) of sequence b behind the prefix[b] (int32 [B]) positions it had; position i is place
     i % page_size of page block_table[b, i // page_size] (int32 [B, n]) of k_cache / v_cache as in kv_append.  A token sees the prefix and, of its
-    sequence's new tokens, the ones of its row of `tree` (int64 [T, words] of 64 bits, as tree_mask makes them; None: itself and
+    sequence's new tokens, the ones of its row of `tree` (int64 [T, words] of 64 bits on the device; tree_mask makes such rows on the host; None: itself and
     those before it).  max_tokens, max_keys: bounds of a sequence's new tokens and of its positions with them.  scale: 1 / sqrt(D).  A token that sees nothing
     gets zeros; rows in no sequence are left as they are in `out` (a new tensor has any numbers there)."""
     return _calls().attention_paged(q, k_cache, v_cache, block_table, cu_tokens, prefix, max_tokens, max_keys, tree, scale, out, workspace)
