@@ -731,11 +731,9 @@ struct AttnPlan {
 // than four tiles and than two ranges have, into ranges that give every CU two workgroups, of twice as many keys as rows at least: what a range hands over
 // is rows, what it reads keys.  One token of 32 heads, uncut / cut, us: 128 keys 7.8 / 10.1, 256 9.4 / 10.5, 320 10.4 / 11.1, 500 13.2 / 10.4, 768 16.8 / 10.5:
 // the second launch, which joins the ranges, is what cutting costs (4 of them).  Prompts with no more keys than two ranges: four of 300 tokens 21.5 / 38,
-// eight chunks of 30 over 500 keys 24.8 / 30.0, one of 128 over 500 24.7 / 22.4; up to four ranges: one of 128 over 1000 39 / 25.
-// From 1024 workgroups on, cutting evens out unequal lengths.  Single tokens over up to n keys, a quarter of it at least: 128 of them, n 8000, 524 / 464, 4097 274 / 253,
-// 2000 136 / 132, 1000 74 / 77; 64 trees of 64, n 8192, 582 / 535, 4097 308 / 295, 2000 170 / 176.  Where lengths are equal it costs a little: 128 tokens over 4097 keys 379 / 382,
-// 64 trees 388 / 397.  So it is done from 4096 keys on, up to two row tiles (a prompt's ranges are not alike) and 4096 workgroups, from where it gains as little as it may
-// cost: 512 single tokens over up to 4097 keys 967 / 950, over 4097 each 1445 / 1489.
+// eight chunks of 30 over 500 keys 24.8 / 30.0, one of 128 over 500 24.7 / 22.4; up to four ranges: one of 128 over 1000 39 / 25.  With 1024 workgroups and more, sequences of unequal lengths pay for
+// it and its workspace from 6144 keys on, up to two row tiles (a prompt's ranges are not alike): 128 single tokens over up to 8000 keys 510 / 460, 64 trees of 64
+// 534 / 489; over up to 4097 keys 264 / 249, 2000 129 / 130, 500 39 / 46.
 static AttnPlan attention_plan(bool f32, int64_t B, int heads, int kv, int64_t max_tokens, int64_t max_keys, int D) {
   AttnPlan p;
   const int64_t rows = max_tokens * (heads / kv);
@@ -748,7 +746,7 @@ static AttnPlan attention_plan(bool f32, int64_t B, int heads, int kv, int64_t m
   p.min_tiles = (int)((2 * (rows < per ? rows : per) + kt - 1) / kt);
   const int64_t most = B * ((max_keys + p.min_tiles * kt - 1) / (p.min_tiles * kt)), wanted = (512 + kv * row_tiles - 1) / (kv * row_tiles);
   const int64_t uncut = B * kv * row_tiles;
-  const bool full = uncut >= 1024 && (row_tiles > 2 || max_keys < 4096 || uncut >= 4096);
+  const bool full = uncut >= 1024 && (row_tiles > 2 || max_keys < 6144 || uncut >= 4096);
   p.ranges = full || max_keys <= (p.min_tiles > 2 ? 2 * p.min_tiles : 4) * kt ? 0 : (int)(wanted < most ? wanted : most);
   if (p.ranges <= 1 && B == 1) p.ranges = 0;
   if (row_tiles > 2 && p.ranges <= B) p.ranges = 0;  // (no more workgroups than without: 16 prompts of 600 tokens of two key heads of 64 28 us, cut 48)
