@@ -661,10 +661,12 @@ int mllm_hip_kv_append(const mllm_hip_heads* q, const mllm_hip_heads* k, const m
  * of drafted tokens, many tokens without a tree a (chunk of a) prompt.
  *   o[t][h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * (q . k_j) - max), of key head h / (heads / kv heads); a token that sees
  *   nothing, or scores of -inf alone: zeros.  What a token does not see has no effect on it, NaN included.  An infinity or a NaN among the values that it
- *   sees makes that element of its result infinite or NaN, whatever the weight.
+ *   sees makes that element of its result infinite or NaN, whatever the weight.  Finite scores times scale are below 2^30 (exponents are fp32: the weights of
+ *   larger ones may all be too small or too large for it).
  * Position i of sequence b is slot i % page_size of page block_table[b * table_stride + i / page_size] (int32); positions from table_len *
  * page_size on are not there, pages outside the cache read as zeros.  q->x, q->y: F32 or BF16, 16-byte aligned rows (weight is not
- * looked at); rows of q in no sequence stay as they are in y.  y may not be x.  head_dim 64, 128 or 256, heads a multiple of the cache's, scale > 0.
+ * looked at); rows of q in no sequence stay as they are in y.  y may not be x.  head_dim 64, 128 or 256, heads a multiple of the cache's,
+ * 0 < scale <= 2e38.
  * max_tokens and max_keys: the host's bounds of a sequence's new tokens (those behind may be left out) and positions (any; it decides into how many
  * ranges keys are cut).  fp32 results are within fp32 sums of the formula, bf16 ones take the weights p in bf16.
  * workspace: ..._workspace_bytes (0: none), 16-byte aligned; less is MLLM_HIP_E_BADARG.  One launch, two where keys are cut. */

@@ -781,7 +781,7 @@ MLLM_API int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_
                                       int64_t table_stride, int64_t table_len, const int32_t* cu_tokens, const int32_t* prefix, int64_t B,
                                       int64_t max_tokens, int64_t max_keys, const uint64_t* tree, int64_t tree_stride, int64_t tree_words, float scale,
                                       void* workspace, size_t workspace_bytes, void* stream) {
-  if (!q || !cache || table_len < 0 || tree_words < 0 || !(scale > 0.f) || scale > 3e38f || cache->pages < 1 || cache->page_size < 1) return MLLM_HIP_E_BADARG;
+  if (!q || !cache || table_len < 0 || tree_words < 0 || !(scale > 0.f) || scale > 2e38f || cache->pages < 1 || cache->page_size < 1) return MLLM_HIP_E_BADARG;
   if (!attention_sizes(dtype, T, B, q->heads, cache->heads, cache->head_dim, max_tokens, max_keys)) return MLLM_HIP_E_BADARG;
   if (!attention_shape(T, B, q->heads, cache->heads, cache->head_dim, max_tokens, max_keys) || cache->pages > 0x7fffffff / cache->page_size ||
       table_len > 0x7fff0000 / cache->page_size || tree_words > 0x1ffffff || cache->page_stride < 0 || cache->slot_stride < 0 || cache->page_stride > 0x7fffffff ||
