@@ -616,8 +616,10 @@ __device__ __forceinline__ void attention_piece(const AttnArgs& a, const Seq& s,
 template <int D, int NQ, int WR, bool F32>
 __global__ __launch_bounds__(256, (Attn<D, NQ, WR, F32>::WAVES)) void attention_kernel(AttnArgs a) {
   constexpr int KT = Attn<D, NQ, WR, F32>::KT;
-  // workgroup i runs on XCD i % 8: the row tiles of a range of keys follow one another on one XCD, whose L2 they share
-  const int idx = blockIdx.x >> 3, rt = idx % a.row_tiles, place = (idx / a.row_tiles) * 8 + (blockIdx.x & 7);
+  // Workgroup i runs on XCD i % 8: the row tiles of a range of keys follow one another on one XCD, whose L2 they share.  The last tile comes first: without a tree it
+  // has the most keys, and the shorter ones fill the end.  Prompts of 1000 (fp32), 2048, 4096 and 8192 tokens, first tile first / last tile first: 65.8 / 54.8 us,
+  // 82 / 75, 231 / 187, 738 / 640; up to 1024 bf16 tokens, with a tree, and in chunks of 1024 over 8192 keys no difference.
+  const int idx = blockIdx.x >> 3, rt = a.row_tiles - 1 - idx % a.row_tiles, place = (idx / a.row_tiles) * 8 + (blockIdx.x & 7);
   const int h = place % a.kv, range = place / a.kv;
   Place p = {{0, 0, 0, 0}, range, 0, 0, 0};
   int tile = 0, end;
@@ -731,9 +733,11 @@ struct AttnPlan {
 // than four tiles and than two ranges have, into ranges that give every CU two workgroups, of twice as many keys as rows at least: what a range hands over
 // is rows, what it reads keys.  One token of 32 heads, uncut / cut, us: 128 keys 7.8 / 10.1, 256 9.4 / 10.5, 320 10.4 / 11.1, 500 13.2 / 10.4, 768 16.8 / 10.5:
 // the second launch, which joins the ranges, is what cutting costs (4 of them).  Prompts with no more keys than two ranges: four of 300 tokens 21.5 / 38,
-// eight chunks of 30 over 500 keys 24.8 / 30.0, one of 128 over 500 24.7 / 22.4; up to four ranges: one of 128 over 1000 39 / 25.  With 1024 workgroups and more, sequences of unequal lengths pay for
-// it and its workspace from 6144 keys on, up to two row tiles (a prompt's ranges are not alike): 128 single tokens over up to 8000 keys 510 / 460, 64 trees of 64
-// 534 / 489; over up to 4097 keys 264 / 249, 2000 129 / 130, 500 39 / 46.
+// eight chunks of 30 over 500 keys 24.8 / 30.0, one of 128 over 500 24.7 / 22.4; up to four ranges: one of 128 over 1000 39 / 25.
+// From 1024 workgroups on, cutting evens out unequal lengths.  Single tokens over up to n keys, a quarter of it at least: 128 of them, n 8000, 524 / 464, 6144 406 / 361,
+// 4097 274 / 253, 2000 136 / 132, 1000 74 / 77; 64 trees of 64, n 8192, 582 / 535, 4097 308 / 295, 2000 170 / 176.  Of equal lengths it costs 1 to 2 %: 128 tokens over 4097 keys
+// 379 / 382, 64 trees 388 / 397, and its workspace (64 trees: 102 MB).  So it is done from 6144 keys on, where it gains 8 to 12 %, up to two row tiles (a prompt's ranges
+// are not alike) and 4096 workgroups, from where it gains as little as it may cost: 512 single tokens over up to 8000 keys 1870 / 1820, 4097 967 / 950, 4097 each 1445 / 1489.
 static AttnPlan attention_plan(bool f32, int64_t B, int heads, int kv, int64_t max_tokens, int64_t max_keys, int D) {
   AttnPlan p;
   const int64_t rows = max_tokens * (heads / kv);
