@@ -22,10 +22,10 @@
 // whose O, maximum and sum meet in the workspace; a second launch joins them.
 //
 // What bounds it, 32 query and 8 key heads of 128: with few rows the reading of keys and values (16 fp32 tokens over up to 8000 keys each 75 us, 341 MB: 4.5
-// TB/s; a copy of 2 GB has 4.96), one token over 4097 keys (12.8 us, 16.8 MB) two launches and the loads that wait for one another in each: lengths, table, keys,
-// partial results.  32 trees of 64 tokens over up to 8192 keys (253 us, 137 GFLOP, 711 MB) the matrix and the vector pipe in turns, 30 and 40 % of the
-// time busy: registers leave two waves a SIMD, and LDS is busy 30 %.  Eight trees of 29 over up to 5000 (50 us) keys and values at 4 TB/s and, half
-// of the time, partial results (34 MB written and read) and starts.  A prompt of 8192 bf16 tokens 690 us, 800 TFLOP/s of what it has to compute.
+// TB/s; a copy of 2 GB has 4.96), one token over 4097 keys (13.2 us, 16.8 MB) two launches and the loads that wait for one another in each: lengths, table, keys,
+// partial results.  32 trees of 64 tokens over up to 8192 keys (256 us, 137 GFLOP, 711 MB) the matrix and the vector pipe in turns, 30 and 40 % of the
+// time busy: two waves a SIMD, as 256 registers each and 64 KB of LDS a workgroup both have it; LDS is busy 30 %.  Eight trees of 29 over up to 5000 (50 us) keys and
+// values at 4 TB/s and, half of the time, partial results (34 MB written and read) and starts.  A prompt of 8192 bf16 tokens 637 us, 860 TFLOP/s of what it has to compute.
 #include <type_traits>
 
 #include "item8.h"
@@ -671,7 +671,7 @@ __global__ __launch_bounds__(256) void attention_join_kernel(AttnArgs a) {
   if (live) {
     const float* ml = a.part_ml + 2 * (first * all + i);
     const float* o = a.part_o + (first * all + i) * D + d;
-    constexpr int U = G > 1 ? 8 : 4;  // loads in flight
+    constexpr int U = G > 1 ? 8 : 4;  // pieces a turn; each is read where there is one (all of a turn at once: one token over 4097 keys 13.9 -> 13.0 us, eight trees of 29 over 5000, with few pieces a row, 55 -> 62)
     for (int k = group; k < count; k += U * G) {
       float mk[U], lk[U];
       at_f32x4 xk[U];
@@ -753,7 +753,7 @@ static AttnPlan attention_plan(bool f32, int64_t B, int heads, int kv, int64_t m
   const bool full = uncut >= 1024 && (row_tiles > 2 || max_keys < 6144 || uncut >= 4096);
   p.ranges = full || max_keys <= (p.min_tiles > 2 ? 2 * p.min_tiles : 4) * kt ? 0 : (int)(wanted < most ? wanted : most);
   if (p.ranges <= 1 && B == 1) p.ranges = 0;
-  if (row_tiles > 2 && p.ranges <= B) p.ranges = 0;  // (no more workgroups than without: 16 prompts of 600 tokens of two key heads of 64 28 us, cut 48)
+  if (row_tiles > 2 && p.ranges <= B) p.ranges = 0;  // (no more workgroups than without: 16 prompts of 600 tokens of two key heads of 64 24 us, cut 43)
   return p;
 }
 // partial results of every piece, and of every sequence where its pieces are

@@ -8,8 +8,8 @@
 // A workgroup has one token: its cosines and sines are computed once into LDS (64 pairs of 128 wide heads) while the first heads
 // are on their way from memory, and every head of the token uses them.  Per byte there is nothing else to do: bound by memory
 // with many tokens, by the launch and two dependent loads with few.  32 query and 8 key heads of 128, norm and halves turned:
-// 8191 bf16 tokens 42.6 us (168 MB: 3.9 TB/s, a copy of 2 GB has 4.96), one fp32 token 3.2 in the kernel; 6007 bf16 tokens of 16 query and 4 key heads,
-// pairs turned, keys and values into the cache, 16.5 us (74 MB: 4.5 TB/s).
+// 8191 bf16 tokens 43 us (168 MB: 3.9 TB/s, a copy of 2 GB has 4.96), one fp32 token 3.2 in the kernel; 6007 bf16 tokens of 16 query and 4 key heads,
+// pairs turned, keys and values into the cache, 16.6 us (74 MB: 4.5 TB/s).
 #include "item8.h"
 
 namespace mllmhip {
