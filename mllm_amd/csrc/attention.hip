@@ -187,7 +187,7 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t v) {
 // Infinities and NaNs among the values make that element of the rows that see them infinite or NaN, whatever the weight: it is their sum.  What the matrix products
 // leave there is NaN where a weight is too small for its type (or a part of one is 0), and without them where they were taken out for rows that do not see
 // them (in tiles with masks; the sum of the weights has its sign set then).  So results of either kind are looked at once more, behind everything else: a lane's elements
-// d .. d + 3 of query head `head`, token `token`, where it says so in `look` (LOOK_WHOLE: among all keys, LOOK_MASKED: those of tiles with masks).  The lanes that are
+// d .. d + 3 of query head `head`, token `token`, where it says so in `look` (LOOK_WHOLE: among all keys, LOOK_MASKED: those of tiles with masks, the first of which has the prefix's end or the last key).  The lanes that are
 // there go through the values of one result after the other together: a call of one token over 4096 keys 19 us, with a NaN among them 80 (a lane for each result: 1043).
 enum { LOOK_MASKED = 1, LOOK_WHOLE = 2 };
 __device__ __forceinline__ uint32_t look_at(at_f32x4 x, float sum, uint32_t sign) {
@@ -205,7 +205,7 @@ __device__ __forceinline__ void put_infinities(const AttnArgs& a, const Seq& s, 
     const uint16_t* v = a.v + head / a.group * a.head_stride + d;
     const int end = a.tree ? s.keys : (int)min((int64_t)s.keys, (int64_t)s.prefix + token + 1);
     uint32_t nans = 0, above = 0, below = 0;  // which of the elements have a NaN, an infinity, one below 0
-    for (int k0 = __builtin_amdgcn_readlane(look, who) == LOOK_WHOLE ? 0 : min(s.prefix, s.keys - 1) & ~63; k0 < end && nans != 15; k0 += lanes) {
+    for (int k0 = __builtin_amdgcn_readlane(look, who) == LOOK_WHOLE ? 0 : min(s.prefix, s.keys - 1) / 64 * 64; k0 < end && nans != 15; k0 += lanes) {
       const int key = min(k0 + rank, end - 1);
       const uint32_t page = __umulhi(2 * (uint32_t)key, a.page_mul) >> a.page_shift, id = (uint32_t)table[min((int)page, a.table_len - 1)];
       const uint64_t at = (uint64_t)id * a.page_bytes + (((uint32_t)key - page * a.page) * a.slot_bytes + (uint64_t)(uintptr_t)v);
@@ -221,14 +221,14 @@ __device__ __forceinline__ void put_infinities(const AttnArgs& a, const Seq& s, 
       }
     }
     nans |= above & below;
-    if ((int)(threadIdx.x & 63) != who) continue;
     const int64_t to = (s.first + token) * a.o_token + head * a.o_head + d;
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      if (!((nans | above | below) >> e & 1)) continue;
       const uint32_t sum = nans >> e & 1 ? 0x7fc00000u : above >> e & 1 ? 0x7f800000u : 0xff800000u;
-      if (F32) reinterpret_cast<uint32_t*>(a.o)[to + e] = sum;
-      else reinterpret_cast<uint16_t*>(a.o)[to + e] = (uint16_t)(sum >> 16);
+      if ((int)(threadIdx.x & 63) == who && (nans | above | below) >> e & 1) {  // (by the lane that has stored the result)
+        if (F32) reinterpret_cast<uint32_t*>(a.o)[to + e] = sum;
+        else reinterpret_cast<uint16_t*>(a.o)[to + e] = (uint16_t)(sum >> 16);
+      }
     }
   }
 }

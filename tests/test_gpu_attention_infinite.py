@@ -40,3 +40,45 @@ def test_values_whatever_their_weight(n, prefix, keys, Hq, D, tree, dtype, max_k
             far[..., [5, 33]] = 0
             assert far.max() <= 1, (key, score, far.max())
             c.k[page, slot], c.v[page, slot] = kept
+
+
+@pytest.mark.parametrize("n,prefix,keys,Hq,D,tree", [(1, 700, [5, 650, 699], 4, 128, False), (1, 40, [3], 2, 64, False), (9, 300, [10, 299], 4, 128, True), (70, 130, [0, 129], 2, 256, False)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("max_keys", [1, LONG])
+def test_values_of_scores_of_minus_infinity(n, prefix, keys, Hq, D, tree, dtype, max_keys):
+    """The weight is 0 and the value counts all the same; the row's other elements are as if the key were not there."""
+    announce("attention infinite values of scores of -inf", n, prefix, keys, Hq, D, tree, dtype, max_keys)
+    c = Case([n], [prefix], Hq, 1, D, 16, dtype, _random_tree if tree else None, seed=n + prefix)
+    c.q[..., 7] = 1.0
+    terms = c.want()[2]
+    for key in keys:
+        at = _place(c, key)
+        kept = c.k[at].clone(), c.v[at].clone()
+        c.k[at][:, 7] = -INF
+        want, size, _ = c.want()
+        c.v[at][:, 5], c.v[at][:, 33] = INF, -INF
+        got = c.run(max_keys=max_keys).cpu().double()
+        assert (got[..., 5] == INF).all() and (got[..., 33] == -INF).all(), key
+        far = (got - want).abs() / _bound(want, size, terms, dtype, D, prefix + n)
+        far[..., [5, 33]] = 0
+        assert far.max() <= 1, (key, far.max())
+        c.k[at], c.v[at] = kept
+
+
+@pytest.mark.parametrize("Hq,Hkv,D", [(8, 2, 64), (8, 8, 128), (6, 2, 256)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("tree", [None, _random_tree])
+@pytest.mark.parametrize("max_keys", [1, LONG])
+def test_other_sequences_and_heads_keep_their_bits(Hq, Hkv, D, dtype, tree, max_keys):
+    announce("attention infinite values of one sequence", Hq, Hkv, D, dtype, tree is not None, max_keys)
+    c = Case([3, 1, 40, 2], [70, 900, 200, 63], Hq, Hkv, D, 16, dtype, tree, seed=D, spare=3)
+    out = torch.full(c.q.shape, 7.0, dtype=dtype, device="cuda")
+    clean = c.run(max_keys=max_keys, out=out.clone())
+    for b, key in ((1, 900), (1, 3), (2, 199), (2, 205), (2, 100)):  # new tokens and the prefix, key head 1
+        c.v[_place(c, key, b)][1, 9] = INF if key % 2 else float("nan")
+    got = c.run(max_keys=max_keys, out=out.clone())
+    group = Hq // Hkv
+    hit = torch.zeros(c.q.shape, dtype=torch.bool, device="cuda")
+    hit[int(c.cu[1]):int(c.cu[3]), group:2 * group, 9] = True
+    assert not torch.isfinite(got[hit]).any()
+    assert torch.equal(got[~hit], clean[~hit]) and (got[int(c.cu[-1]):] == 7).all()
