@@ -654,6 +654,17 @@ int mllm_hip_kv_append(const mllm_hip_heads* q, const mllm_hip_heads* k, const m
                        const mllm_hip_kv_cache* cache, const int64_t* slots, float epsilon, int add_unit_offset,
                        const int32_t* positions, const double* inv_freq, int rot_dim, int interleaved, void* stream);
 
+/* The two calls above with positions on several axes (time, height and width of a picture's or a video's patches): pair j turns by the token's position on axis
+ * axes[j], angle positions[axes[j] * axis_stride + t * token_stride] * inv_freq[j].  naxes 1 to 4 axes; axes int32 [rot_dim / 2] on the device, in any order; a
+ * pair whose axis is none of 0 .. naxes - 1 is not turned.  With the same position on every axis: the results of the calls above, bit for bit. */
+int mllm_hip_qk_norm_rope_axes(int nparts, const mllm_hip_heads* parts, int dtype, int64_t T, int head_dim, float epsilon, int add_unit_offset,
+                               const int32_t* positions, int64_t axis_stride, int64_t token_stride, int naxes, const int32_t* axes,
+                               const double* inv_freq, int rot_dim, int interleaved, void* stream);
+int mllm_hip_kv_append_axes(const mllm_hip_heads* q, const mllm_hip_heads* k, const mllm_hip_heads* v, int dtype, int64_t T,
+                            const mllm_hip_kv_cache* cache, const int64_t* slots, float epsilon, int add_unit_offset, const int32_t* positions,
+                            int64_t axis_stride, int64_t token_stride, int naxes, const int32_t* axes, const double* inv_freq, int rot_dim,
+                            int interleaved, void* stream);
+
 /* Attention of new tokens over a paged cache that holds them already: token t of sequence b (rows cu_tokens[b] + t of q, cu_tokens
  * int32 [B + 1]) sees the first prefix[b] positions of its sequence and, of the sequence's new tokens (positions prefix[b] + j), the ones
  * whose bit is set in its row of the tree: bit j % 64 of word j / 64, tree_words words a row, rows of q tree_stride words apart;
@@ -691,6 +702,34 @@ size_t mllm_hip_sample_workspace_bytes(int64_t rows, int64_t vocab);
 int mllm_hip_sample(const void* logits, int dtype, int64_t row_stride, int64_t rows, int64_t vocab, const float* u, const float* temperature,
                     const int32_t* top_k, const float* top_p, const float* min_p, int32_t* tokens, void* workspace, size_t workspace_bytes,
                     void* stream);
+
+/* Penalties for tokens that a row has seen, biases, and the tokens that a grammar allows, on logits [rows][vocab] (F32 or BF16, rows x_stride elements apart; results
+ * in y likewise): in front of mllm_hip_sample.  For element i of a row, in fp32, rounded once:
+ *   i in the row's history:                              x = x > 0 ? x / repetition : x * repetition
+ *   n > 0 times among the tokens from prompts on:        x = x - (frequency * n + presence)
+ *   i among the row's bias tokens (several times: the last one counts):  x = x + bias
+ *   bit i % 32 of word i / 32 of the row's mask is 0:    x = -inf
+ * history int32 [rows][history_len]: a row's first lengths[row] tokens (NULL: all; held to 0 .. history_len), of which the first prompts[row] (NULL: none) were given and the
+ * others chosen.  bias_tokens int32, bias fp32 [rows][biases].  Tokens outside 0 .. vocab - 1 count for nothing.  masks uint32 [masks_count][ceil(vocab / 32)]; row r takes mask
+ * mask_of[r], any number that is none of them: no mask; mask_of NULL: mask r, and there are masks_count >= rows of them.  repetition, presence, frequency fp32
+ * [rows]; NULL: 1, 0, 0.  Strides in elements; those of inputs may be 0 (one for all rows).  A NaN stays one unless it is masked; a row whose mask leaves nothing is all -inf.
+ * y is x with the same stride or shares no element with any input, its rows do not overlap.  vocab <= 2^24, rows <= 65535.  One launch, no workspace. */
+typedef struct mllm_hip_logits {
+  const void* x;
+  void* y;
+  int64_t x_stride, y_stride;
+  const int32_t* history;
+  int64_t history_stride, history_len; /* 0: no history */
+  const int32_t *lengths, *prompts;
+  const float *repetition, *presence, *frequency;
+  const int32_t* bias_tokens;
+  const float* bias;
+  int64_t bias_tokens_stride, bias_stride, biases; /* 0: none */
+  const uint32_t* masks;
+  int64_t masks_stride, masks_count; /* 0: none */
+  const int32_t* mask_of;
+} mllm_hip_logits;
+int mllm_hip_logits_adjust(const mllm_hip_logits* logits, int dtype, int64_t rows, int64_t vocab, void* stream);
 
 #ifdef __cplusplus
 }

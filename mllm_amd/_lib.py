@@ -34,6 +34,14 @@ class KVCache(C.Structure):
                 ("pages", C.c_int64), ("page_size", C.c_int64), ("heads", C.c_int), ("head_dim", C.c_int)]
 
 
+class Logits(C.Structure):
+    """mllm_hip_logits"""
+    _fields_ = [("x", C.c_void_p), ("y", C.c_void_p), ("x_stride", C.c_int64), ("y_stride", C.c_int64), ("history", C.c_void_p), ("history_stride", C.c_int64),
+                ("history_len", C.c_int64), ("lengths", C.c_void_p), ("prompts", C.c_void_p), ("repetition", C.c_void_p), ("presence", C.c_void_p),
+                ("frequency", C.c_void_p), ("bias_tokens", C.c_void_p), ("bias", C.c_void_p), ("bias_tokens_stride", C.c_int64), ("bias_stride", C.c_int64),
+                ("biases", C.c_int64), ("masks", C.c_void_p), ("masks_stride", C.c_int64), ("masks_count", C.c_int64), ("mask_of", C.c_void_p)]
+
+
 class HipQLinearError(RuntimeError):
     pass
 
@@ -197,12 +205,15 @@ def lib():
         cf, rp, kv = C.c_float, C.POINTER(Heads), C.POINTER(KVCache)
         L.mllm_hip_qk_norm_rope.argtypes = [ci, rp, ci, i64, ci, cf, ci, vp, vp, ci, ci, vp]
         L.mllm_hip_kv_append.argtypes = [rp, rp, rp, ci, i64, kv, vp, cf, ci, vp, vp, ci, ci, vp]
+        L.mllm_hip_qk_norm_rope_axes.argtypes = [ci, rp, ci, i64, ci, cf, ci, vp, i64, i64, ci, vp, vp, ci, ci, vp]
+        L.mllm_hip_kv_append_axes.argtypes = [rp, rp, rp, ci, i64, kv, vp, cf, ci, vp, i64, i64, ci, vp, vp, ci, ci, vp]
         L.mllm_hip_attention_paged_workspace_bytes.restype = C.c_size_t
         L.mllm_hip_attention_paged_workspace_bytes.argtypes = [ci, i64, i64, ci, ci, ci, i64, i64]
         L.mllm_hip_attention_paged.argtypes = [rp, ci, i64, kv, vp, i64, i64, vp, vp, i64, i64, i64, vp, i64, i64, cf, vp, C.c_size_t, vp]
         L.mllm_hip_sample_workspace_bytes.restype = C.c_size_t
         L.mllm_hip_sample_workspace_bytes.argtypes = [i64, i64]
         L.mllm_hip_sample.argtypes = [vp, ci, i64, i64, i64, vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp]
+        L.mllm_hip_logits_adjust.argtypes = [C.POINTER(Logits), ci, i64, i64, vp]
         _lib = L
     return _lib
 

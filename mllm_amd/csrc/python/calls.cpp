@@ -335,13 +335,33 @@ struct Rotation {
   const int32_t* positions;
   const double* inv_freq;
   int rot_dim;
+  const int32_t* axes;  // null: positions of one axis
+  int naxes;
+  int64_t axis_stride, token_stride;
 };
-Rotation rotation_of(PyObject* positions, PyObject* inv_freq, int64_t T, int64_t device) {
+Rotation rotation_of(PyObject* positions, PyObject* inv_freq, PyObject* axes, int64_t T, int64_t device) {
   require((positions == Py_None) == (inv_freq == Py_None));
-  if (positions == Py_None) return Rotation{nullptr, nullptr, 0};
+  Rotation r = {};
+  if (positions == Py_None) {
+    require(axes == Py_None);
+    return r;
+  }
   const at::Tensor& f = local(inv_freq, device, at::kDouble);
   require(f.dim() == 1 && f.is_contiguous() && f.size(0) <= 65536);
-  return Rotation{vector_of<int32_t>(positions, device, at::kInt, T), static_cast<const double*>(f.data_ptr()), 2 * (int)f.size(0)};
+  r.inv_freq = static_cast<const double*>(f.data_ptr());
+  r.rot_dim = 2 * (int)f.size(0);
+  if (axes == Py_None) {
+    r.positions = vector_of<int32_t>(positions, device, at::kInt, T);
+    return r;
+  }
+  const at::Tensor& p = local(positions, device, at::kInt);
+  require(p.dim() == 2 && p.size(0) >= 1 && p.size(0) <= 65536 && p.size(1) == T);
+  r.positions = static_cast<const int32_t*>(p.data_ptr());
+  r.axes = vector_of<int32_t>(axes, device, at::kInt, f.size(0));
+  r.naxes = (int)p.size(0);
+  r.axis_stride = stride_of(p, 0);
+  r.token_stride = stride_of(p, 1);
+  return r;
 }
 // keys and values [pages, page_size, heads, D] of one layout
 mllm_hip_kv_cache cache_of(PyObject* ko, PyObject* vo, int64_t device) {
@@ -361,7 +381,7 @@ void* workspace_on(int64_t device, PyObject* o, size_t bytes, at::Tensor& made) 
   return workspace(o, bytes, made);
 }
 
-// (q, k, positions, inv_freq, q_weight, k_weight, eps, add_unit_offset, interleaved, out)
+// (q, k, positions, inv_freq, q_weight, k_weight, eps, add_unit_offset, interleaved, out, axes)
 PyObject* qk_norm_rope(Args a) {
   const int64_t device = current_device();
   const at::Tensor &q = tensor(a[0]), &k = tensor(a[1]);
@@ -380,17 +400,22 @@ PyObject* qk_norm_rope(Args a) {
   require(T == 0 || parts[0].y != parts[1].y);
   parts[0].weight = vector_of<float>(a[4], device, at::kFloat, D);
   parts[1].weight = vector_of<float>(a[5], device, at::kFloat, D);
-  const Rotation r = rotation_of(a[2], a[3], T, device);
+  const Rotation r = rotation_of(a[2], a[3], a[10], T, device);
   const float eps = (float)real(a[6]);
   const int unit = truth(a[7]), next = truth(a[8]);
   require(D <= 65536);
   void* st = stream();
-  run("mllm_hip_qk_norm_rope", [&] { return mllm_hip_qk_norm_rope(2, parts, dtype, T, (int)D, eps, unit, r.positions, r.inv_freq, r.rot_dim, next, st); });
+  if (a[10] != Py_None)
+    run("mllm_hip_qk_norm_rope_axes", [&] {
+      return mllm_hip_qk_norm_rope_axes(2, parts, dtype, T, (int)D, eps, unit, r.positions, r.axis_stride, r.token_stride, r.naxes, r.axes, r.inv_freq, r.rot_dim, next, st);
+    });
+  else
+    run("mllm_hip_qk_norm_rope", [&] { return mllm_hip_qk_norm_rope(2, parts, dtype, T, (int)D, eps, unit, r.positions, r.inv_freq, r.rot_dim, next, st); });
   Owned qo(THPVariable_Wrap(yq)), ko(THPVariable_Wrap(yk));
   return PyTuple_Pack(2, qo.o, ko.o);
 }
 
-// (k, v, k_cache, v_cache, slots, positions, inv_freq, k_weight, q, q_weight, eps, add_unit_offset, interleaved, out)
+// (k, v, k_cache, v_cache, slots, positions, inv_freq, k_weight, q, q_weight, eps, add_unit_offset, interleaved, out, axes)
 PyObject* kv_append(Args a) {
   const int64_t device = current_device();
   const at::Tensor &k = tensor(a[0]), &v = tensor(a[1]);
@@ -411,13 +436,17 @@ PyObject* kv_append(Args a) {
   }
   require(a[4] != Py_None);
   const int64_t* slots = vector_of<int64_t>(a[4], device, at::kLong, T);
-  const Rotation r = rotation_of(a[5], a[6], T, device);
+  const Rotation r = rotation_of(a[5], a[6], a[14], T, device);
   const float eps = (float)real(a[10]);
   const int unit = truth(a[11]), next = truth(a[12]);
   void* st = stream();
-  run("mllm_hip_kv_append", [&] {
-    return mllm_hip_kv_append(a[8] != Py_None ? &qp : nullptr, &kp, &vp, dtype, T, &cache, slots, eps, unit, r.positions, r.inv_freq, r.rot_dim, next, st);
-  });
+  const mllm_hip_heads* qs = a[8] != Py_None ? &qp : nullptr;
+  if (a[14] != Py_None)
+    run("mllm_hip_kv_append_axes", [&] {
+      return mllm_hip_kv_append_axes(qs, &kp, &vp, dtype, T, &cache, slots, eps, unit, r.positions, r.axis_stride, r.token_stride, r.naxes, r.axes, r.inv_freq, r.rot_dim, next, st);
+    });
+  else
+    run("mllm_hip_kv_append", [&] { return mllm_hip_kv_append(qs, &kp, &vp, dtype, T, &cache, slots, eps, unit, r.positions, r.inv_freq, r.rot_dim, next, st); });
   if (a[8] == Py_None) Py_RETURN_NONE;
   return THPVariable_Wrap(y);
 }
@@ -481,6 +510,58 @@ PyObject* sample(Args a) {
   return a[6] == Py_None ? THPVariable_Wrap(made) : given(a[6]);
 }
 
+// (logits, history, lengths, prompts, repetition, presence, frequency, bias_tokens, bias, masks, mask_of, out)
+PyObject* adjust_logits(Args a) {
+  const int64_t device = current_device();
+  const at::Tensor& x = tensor(a[0]);
+  const int dtype = xdtype(x);
+  // rows in one piece, any number of elements apart
+  auto matrix = [&](PyObject* o, at::ScalarType type, int64_t rows) -> const at::Tensor& {
+    const at::Tensor& t = local(o, device, type);
+    require(t.dim() == 2 && (rows < 0 || t.size(0) == rows) && (t.size(1) <= 1 || t.stride(1) == 1));
+    return t;
+  };
+  const int64_t rows = matrix(a[0], x.scalar_type(), -1).size(0), vocab = x.size(1);
+  require(vocab >= 1);
+  mllm_hip_logits l = {};
+  l.x = x.data_ptr();
+  l.x_stride = stride_of(x, 0);
+  if (a[1] != Py_None) {
+    const at::Tensor& t = matrix(a[1], at::kInt, rows);
+    l.history = static_cast<const int32_t*>(t.data_ptr());
+    l.history_stride = stride_of(t, 0), l.history_len = t.size(1);
+  }
+  require(a[1] != Py_None || (a[2] == Py_None && a[3] == Py_None));
+  l.lengths = vector_of<int32_t>(a[2], device, at::kInt, rows);
+  l.prompts = vector_of<int32_t>(a[3], device, at::kInt, rows);
+  l.repetition = vector_of<float>(a[4], device, at::kFloat, rows);
+  l.presence = vector_of<float>(a[5], device, at::kFloat, rows);
+  l.frequency = vector_of<float>(a[6], device, at::kFloat, rows);
+  require((a[7] == Py_None) == (a[8] == Py_None));
+  if (a[7] != Py_None) {
+    const at::Tensor &t = matrix(a[7], at::kInt, rows), &b = matrix(a[8], at::kFloat, rows);
+    require(t.size(1) == b.size(1));
+    l.bias_tokens = static_cast<const int32_t*>(t.data_ptr());
+    l.bias = static_cast<const float*>(b.data_ptr());
+    l.bias_tokens_stride = stride_of(t, 0), l.bias_stride = stride_of(b, 0), l.biases = t.size(1);
+  }
+  require(a[9] != Py_None || a[10] == Py_None);
+  if (a[9] != Py_None) {
+    const at::Tensor& t = matrix(a[9], at::kInt, -1);
+    require(t.size(1) == (vocab + 31) / 32 && (a[10] != Py_None || t.size(0) == rows));
+    l.masks = static_cast<const uint32_t*>(t.data_ptr());
+    l.masks_stride = stride_of(t, 0), l.masks_count = t.size(0);
+  }
+  l.mask_of = vector_of<int32_t>(a[10], device, at::kInt, rows);
+  at::Tensor made = a[11] == Py_None ? at::empty({rows, vocab}, x.options()) : tensor(a[11]);
+  if (a[11] != Py_None) require(matrix(a[11], x.scalar_type(), rows).size(1) == vocab && (rows <= 1 || made.stride(0) >= vocab));
+  l.y = made.data_ptr();
+  l.y_stride = stride_of(made, 0);
+  void* st = stream();
+  run("mllm_hip_logits_adjust", [&] { return mllm_hip_logits_adjust(&l, dtype, rows, vocab, st); });
+  return THPVariable_Wrap(made);
+}
+
 template <PyObject* (*F)(Args), int N>
 PyObject* entry(PyObject*, Args args, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -498,7 +579,8 @@ PyObject* entry(PyObject*, Args args, Py_ssize_t n) {
 #define CALL(name, n) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(entry<name, n>)), METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {CALL(linear_q_gemv, 8), CALL(linear_q_gemv_multi, 6), CALL(softmax, 1), CALL(topk, 4), CALL(matmul, 5),
                            CALL(w8a8_linear_packed, 7), CALL(w4a16_gemm_packed, 6), CALL(linear_q_gemm, 7), CALL(linear_kq_gemm, 6),
-                           CALL(qk_norm_rope, 10), CALL(kv_append, 14), CALL(attention_paged, 12), CALL(sample, 8), {nullptr, nullptr, 0, nullptr}};
+                           CALL(qk_norm_rope, 11), CALL(kv_append, 15), CALL(attention_paged, 12), CALL(sample, 8),
+                           CALL(adjust_logits, 12), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "mllm_calls", nullptr, -1, g_methods};
 
 }  // namespace

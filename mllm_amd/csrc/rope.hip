@@ -2,6 +2,7 @@
 //
 //   n = x * (w * rms),  rms = 1 / sqrt(mean over the head (x^2) + epsilon)      (as mllm_hip_rmsnorm; left out without a weight)
 //   pair (a, b) number j of a head at position p:  a' = a cos - b sin,  b' = b cos + a sin,  angle = p * inv_freq[j]
+//   with positions on several axes (time, height, width): p is the token's position on axis axes[j]
 //
 // Everything is fp32 between the load and the one rounding of the store.  The angle is not: fp32 holds p * f of a far position to
 // a tenth of a radian at best, so it is multiplied in fp64, reduced to a fraction of a turn there, and only that goes to fp32.
@@ -28,6 +29,10 @@ struct RopeArgs {
   float eps, inv_d;
   const int32_t* positions;
   const double* inv_freq;
+  // positions of several axes: which one each pair turns by (null: there is one), elements from a token to the next, from an axis to the next
+  const int32_t* axes;
+  int64_t pos_token, pos_axis;
+  int naxes;
   // the cache's addressing
   const int64_t* slots;
   int64_t page_stride, slot_stride, head_stride, slot_count;
@@ -48,7 +53,7 @@ __device__ __forceinline__ float across(float v) {
 
 // G lanes per head of up to 8 * G elements.  A wave has 64 / G heads of one part at a time -- addresses are numbers of the scalar unit -- and goes through
 // `passes` of them, up to ROPE_AHEAD on their way from memory at once.
-enum { ROPE_AHEAD = 3 };
+enum { ROPE_AHEAD = 3, ROPE_AXES = 4 };
 template <int XT, int G, bool NEXT>
 __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
   __shared__ __align__(16) float s_cos[256];
@@ -91,8 +96,21 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
     }
     if (p0 == 0 && half > 0) {
       if (tid < half) {
+        int place = 0;
+        if (a.axes) {
+          // The token's positions are numbers of the scalar unit, asked for beside the pair's axis: with an address from it they would come one trip to memory later.
+          const int32_t* at = a.positions + t * a.pos_token;
+          const uint32_t axis = (uint32_t)a.axes[tid];
+#pragma unroll
+          for (int i = 0; i < ROPE_AXES; i++) {
+            const int there = i < a.naxes ? at[i * a.pos_axis] : 0;
+            place = axis == (uint32_t)i ? there : place;
+          }
+        } else {
+          place = a.positions[t];
+        }
         // turns in fp64: p * f is off by 2^-53 of itself, which at 2^20 radians is 1e-10
-        double turn = (double)a.positions[t] * a.inv_freq[tid] * 0.15915494309189533577;
+        double turn = (double)place * a.inv_freq[tid] * 0.15915494309189533577;
         turn -= rint(turn);
         float sn, cs;
         sincospif(2.0f * (float)turn, &sn, &cs);
@@ -216,6 +234,23 @@ static int rope_launch(RopeArgs& a, int dtype, int64_t T, int head_dim, int rot_
   return (int)hipGetLastError();
 }
 
+// positions of several axes
+struct RopeAxes {
+  int64_t axis_stride, token_stride;
+  int n;
+  const int32_t* axes;
+};
+static int rope_axes(RopeArgs& a, int64_t T, int rot_dim, const RopeAxes& x) {
+  if (x.n < 1 || (T && rot_dim && !x.axes)) return MLLM_HIP_E_BADARG;
+  if (x.n > ROPE_AXES) return MLLM_HIP_E_SHAPE;
+  if (reinterpret_cast<uintptr_t>(x.axes) % 4) return MLLM_HIP_E_ALIGN;
+  a.axes = x.axes;
+  a.naxes = x.n;
+  a.pos_axis = x.axis_stride;
+  a.pos_token = x.token_stride;
+  return 0;
+}
+
 // what both calls check of the rotation
 static int rope_checks(int dtype, int64_t T, int head_dim, const int32_t* positions, const double* inv_freq, int rot_dim) {
   if ((dtype != MLLM_HIP_F32 && dtype != MLLM_HIP_BF16) || T < 0 || head_dim < 1 || rot_dim < 0) return MLLM_HIP_E_BADARG;
@@ -225,17 +260,13 @@ static int rope_checks(int dtype, int64_t T, int head_dim, const int32_t* positi
   return 0;
 }
 
-}  // namespace mllmhip
-
-using namespace mllmhip;
-
-MLLM_API int mllm_hip_qk_norm_rope(int nparts, const mllm_hip_heads* parts, int dtype, int64_t T, int head_dim, float epsilon,
-                                   int add_unit_offset, const int32_t* positions, const double* inv_freq, int rot_dim,
-                                   int interleaved, void* stream) {
+static int norm_rope(int nparts, const mllm_hip_heads* parts, int dtype, int64_t T, int head_dim, float epsilon, int add_unit_offset, const int32_t* positions,
+                     const RopeAxes* axes, const double* inv_freq, int rot_dim, int interleaved, void* stream) {
   if (nparts < 1 || nparts > 4 || !parts) return MLLM_HIP_E_BADARG;
   RC_RET(rope_checks(dtype, T, head_dim, positions, inv_freq, rot_dim));
-  if (T == 0) return 0;  // (tensors without elements have no addresses)
   RopeArgs a = {};
+  if (axes) RC_RET(rope_axes(a, T, rot_dim, *axes));
+  if (T == 0) return 0;  // (tensors without elements have no addresses)
   for (int i = 0; i < nparts; i++) RC_RET(rope_group(parts[i], dtype, T, true, a.part[i]));
   a.nparts = nparts;
   a.eps = epsilon;
@@ -245,9 +276,8 @@ MLLM_API int mllm_hip_qk_norm_rope(int nparts, const mllm_hip_heads* parts, int 
   return rope_launch(a, dtype, T, head_dim, rot_dim, interleaved, (hipStream_t)stream);
 }
 
-MLLM_API int mllm_hip_kv_append(const mllm_hip_heads* q, const mllm_hip_heads* k, const mllm_hip_heads* v, int dtype, int64_t T,
-                                const mllm_hip_kv_cache* cache, const int64_t* slots, float epsilon, int add_unit_offset,
-                                const int32_t* positions, const double* inv_freq, int rot_dim, int interleaved, void* stream) {
+static int append(const mllm_hip_heads* q, const mllm_hip_heads* k, const mllm_hip_heads* v, int dtype, int64_t T, const mllm_hip_kv_cache* cache, const int64_t* slots,
+                  float epsilon, int add_unit_offset, const int32_t* positions, const RopeAxes* axes, const double* inv_freq, int rot_dim, int interleaved, void* stream) {
   if (!k || !v || !cache || !cache->k || !cache->v || (T && !slots) || cache->heads < 1 || cache->pages < 1 || cache->page_size < 1) return MLLM_HIP_E_BADARG;
   RC_RET(rope_checks(dtype, T, cache->head_dim, positions, inv_freq, rot_dim));
   if (k->heads != cache->heads || v->heads != cache->heads || cache->pages > 0x7fffffff / cache->page_size || cache->page_stride < 0 ||
@@ -257,8 +287,9 @@ MLLM_API int mllm_hip_kv_append(const mllm_hip_heads* q, const mllm_hip_heads* k
   if (!al16(cache->k) || !al16(cache->v) || cache->page_stride % 8 || cache->slot_stride % 8 || cache->head_stride % 8 ||
       reinterpret_cast<uintptr_t>(slots) % 8)
     return MLLM_HIP_E_ALIGN;
-  if (T == 0) return 0;
   RopeArgs a = {};
+  if (axes) RC_RET(rope_axes(a, T, rot_dim, *axes));
+  if (T == 0) return 0;
   RC_RET(rope_group(*k, dtype, T, false, a.part[0]));
   RC_RET(rope_group(*v, dtype, T, false, a.part[1]));
   a.part[0].y = cache->k;
@@ -282,4 +313,35 @@ MLLM_API int mllm_hip_kv_append(const mllm_hip_heads* q, const mllm_hip_heads* k
   a.slot_count = cache->pages * cache->page_size;
   a.page = (uint32_t)cache->page_size;
   return rope_launch(a, dtype, T, cache->head_dim, rot_dim, interleaved, (hipStream_t)stream);
+}
+
+}  // namespace mllmhip
+
+using namespace mllmhip;
+
+MLLM_API int mllm_hip_qk_norm_rope(int nparts, const mllm_hip_heads* parts, int dtype, int64_t T, int head_dim, float epsilon,
+                                   int add_unit_offset, const int32_t* positions, const double* inv_freq, int rot_dim,
+                                   int interleaved, void* stream) {
+  return norm_rope(nparts, parts, dtype, T, head_dim, epsilon, add_unit_offset, positions, nullptr, inv_freq, rot_dim, interleaved, stream);
+}
+
+MLLM_API int mllm_hip_qk_norm_rope_axes(int nparts, const mllm_hip_heads* parts, int dtype, int64_t T, int head_dim, float epsilon, int add_unit_offset,
+                                        const int32_t* positions, int64_t axis_stride, int64_t token_stride, int naxes, const int32_t* axes,
+                                        const double* inv_freq, int rot_dim, int interleaved, void* stream) {
+  const RopeAxes x = {axis_stride, token_stride, naxes, axes};
+  return norm_rope(nparts, parts, dtype, T, head_dim, epsilon, add_unit_offset, positions, &x, inv_freq, rot_dim, interleaved, stream);
+}
+
+MLLM_API int mllm_hip_kv_append(const mllm_hip_heads* q, const mllm_hip_heads* k, const mllm_hip_heads* v, int dtype, int64_t T,
+                                const mllm_hip_kv_cache* cache, const int64_t* slots, float epsilon, int add_unit_offset,
+                                const int32_t* positions, const double* inv_freq, int rot_dim, int interleaved, void* stream) {
+  return append(q, k, v, dtype, T, cache, slots, epsilon, add_unit_offset, positions, nullptr, inv_freq, rot_dim, interleaved, stream);
+}
+
+MLLM_API int mllm_hip_kv_append_axes(const mllm_hip_heads* q, const mllm_hip_heads* k, const mllm_hip_heads* v, int dtype, int64_t T,
+                                     const mllm_hip_kv_cache* cache, const int64_t* slots, float epsilon, int add_unit_offset, const int32_t* positions,
+                                     int64_t axis_stride, int64_t token_stride, int naxes, const int32_t* axes, const double* inv_freq, int rot_dim,
+                                     int interleaved, void* stream) {
+  const RopeAxes x = {axis_stride, token_stride, naxes, axes};
+  return append(q, k, v, dtype, T, cache, slots, epsilon, add_unit_offset, positions, &x, inv_freq, rot_dim, interleaved, stream);
 }

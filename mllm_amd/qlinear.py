@@ -666,19 +666,21 @@ def matmul(a, b, transpose_a=False, transpose_b=False, out=None):
 
 
 # ----------------------------------------------------------------------------- between a layer's projections: heads, the paged cache
-def qk_norm_rope(q, k, positions=None, inv_freq=None, q_weight=None, k_weight=None, eps=1e-6, add_unit_offset=False, interleaved=False, out=None):
+def qk_norm_rope(q, k, positions=None, inv_freq=None, q_weight=None, k_weight=None, eps=1e-6, add_unit_offset=False, interleaved=False, out=None, axes=None):
     """RMSNorm of every head (q_weight / k_weight fp32 [D], None: no norm) and rotation by positions int32 [T] times inv_freq fp64
     [rot_dim / 2] (None: no rotation) of q [T, Hq, D] and k [T, Hkv, D], fp32 or bf16, any strides of whole 16 bytes with heads in one piece.
-    Pairs: elements j and j + rot_dim / 2, interleaved: 2j and 2j + 1.  Returns (q, k) anew, or in out=(q, k), which may be the inputs."""
-    return _calls().qk_norm_rope(q, k, positions, inv_freq, q_weight, k_weight, eps, add_unit_offset, interleaved, out)
+    Pairs: elements j and j + rot_dim / 2, interleaved: 2j and 2j + 1.  Returns (q, k) anew, or in out=(q, k), which may be the inputs.
+    axes int32 [rot_dim / 2]: positions are int32 [A, T] of up to four axes (time, height, width), pair j turns by the one on axis axes[j]."""
+    return _calls().qk_norm_rope(q, k, positions, inv_freq, q_weight, k_weight, eps, add_unit_offset, interleaved, out, axes)
 
 
 def kv_append(k, v, k_cache, v_cache, slots, positions=None, inv_freq=None, k_weight=None, q=None, q_weight=None, eps=1e-6, add_unit_offset=False,
-              interleaved=False, out=None):
+              interleaved=False, out=None, axes=None):
     """k [T, Hkv, D], normed and rotated as by qk_norm_rope, and v into a paged cache: k_cache, v_cache bf16 [pages, page_size, Hkv, D] of
     one layout (any strides of whole 16 bytes); token t goes to slots[t] (int64: page * page_size + place in the page; outside the cache:
-    stored nowhere; two tokens with one slot leave either's elements).  q [T, Hq, D]: the queries in the same launch, returned anew or in `out`."""
-    return _calls().kv_append(k, v, k_cache, v_cache, slots, positions, inv_freq, k_weight, q, q_weight, eps, add_unit_offset, interleaved, out)
+    stored nowhere; two tokens with one slot leave either's elements).  q [T, Hq, D]: the queries in the same launch, returned anew or in `out`.
+    positions and axes as in qk_norm_rope."""
+    return _calls().kv_append(k, v, k_cache, v_cache, slots, positions, inv_freq, k_weight, q, q_weight, eps, add_unit_offset, interleaved, out, axes)
 
 
 def attention_paged(q, k_cache, v_cache, block_table, cu_tokens, prefix, max_tokens, max_keys, tree=None, scale=None, out=None, workspace=None):
@@ -710,6 +712,16 @@ def tree_mask(parents, words=None):
 
 
 # ----------------------------------------------------------------------------- the token that follows
+def adjust_logits(logits, history=None, lengths=None, prompts=None, repetition=None, presence=None, frequency=None, bias_tokens=None, bias=None, masks=None, mask_of=None,
+                  out=None):
+    """Logits [rows, vocab] (fp32 or bf16) with the penalties of tokens in a row's history, biases, and -inf where a grammar's mask forbids a token, for `sample`; anew, or in
+    `out`, which may be `logits`.  history int32 [rows, L]: the first lengths[row] of a row count (None: all), the first prompts[row] of them (None: none) were given, the others
+    chosen.  In the history: x / repetition where x > 0, x * repetition elsewhere; n times among the chosen: x - (frequency n + presence).  bias_tokens int32, bias fp32 [rows, n]:
+    added (of a token's several the last).  masks int32 [m, ceil(vocab / 32)], bit i % 32 of word i // 32 is token i's, mask_of int32 [rows]: which one a row has, outside
+    0 .. m - 1: none (None: row r has mask r).  Tokens outside the vocabulary count for nothing; repetition, presence, frequency fp32 [rows], lengths and prompts int32 [rows]."""
+    return _calls().adjust_logits(logits, history, lengths, prompts, repetition, presence, frequency, bias_tokens, bias, masks, mask_of, out)
+
+
 def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, out=None, workspace=None):
     """A token int32 [rows] from every row of logits [rows, vocab] (fp32 or bf16) and uniform numbers u fp32 [rows]: weights exp((x - max) /
     temperature); the top_k largest (0: all), of these the shortest beginning with top_p of their mass (1: all), of these the ones of min_p of the

@@ -1,0 +1,61 @@
+"""Refusals of the operators over images and long contexts at the C ABI, without a GPU: made-up addresses that a refused call never reads."""
+import ctypes as C
+
+import pytest
+
+from mllm_amd import _lib
+
+P = 0x7F0000100000
+ODD = P + 2
+BADARG, SHAPE, ALIGN = -1, -2, -3
+F32, BF16 = 0, 1
+
+
+def _part(**changed):
+    p = dict(x=P, y=P, weight=P, x_token_stride=512, x_head_stride=128, y_token_stride=512, y_head_stride=128, heads=4)
+    p.update(changed)
+    return _lib.Heads(**p)
+
+
+def _cache(**changed):
+    c = dict(k=P, v=P, page_stride=16 * 512, slot_stride=512, head_stride=128, pages=8, page_size=16, heads=4, head_dim=128)
+    c.update(changed)
+    return _lib.KVCache(**c)
+
+
+def _rope(T=1, pos=P, naxes=3, axes=P, freq=P, rot=128, part=None):
+    return _lib.lib().mllm_hip_qk_norm_rope_axes(1, C.byref(part or _part()), F32, T, 128, 1e-6, 0, pos, 8, 1, naxes, axes, freq, rot, 0, None)
+
+
+def _append(T=1, pos=P, naxes=3, axes=P, freq=P, rot=128, cache=None):
+    p = _part()
+    return _lib.lib().mllm_hip_kv_append_axes(None, C.byref(p), C.byref(p), BF16, T, C.byref(cache or _cache()), P, 1e-6, 0, pos, 8, 1, naxes, axes, freq, rot, 0, None)
+
+
+@pytest.mark.parametrize("call", [_rope, _append])
+@pytest.mark.parametrize("args,want", [
+    (dict(naxes=0), BADARG), (dict(naxes=5), SHAPE), (dict(axes=None), BADARG), (dict(axes=ODD), ALIGN), (dict(pos=None), BADARG), (dict(pos=P + 1), ALIGN), (dict(freq=None), BADARG),
+    (dict(rot=24), SHAPE), (dict(T=-1), BADARG), (dict(T=1 << 24), SHAPE), (dict(T=0), 0), (dict(T=0, naxes=5), SHAPE), (dict(T=0, pos=None, axes=None, freq=None), 0)])
+def test_rotation_by_several_axes(call, args, want):
+    assert call(**args) == want
+
+
+def _adjust(dtype=F32, rows=2, vocab=1000, **changed):
+    l = dict(x=P, y=P, x_stride=1000, y_stride=1000, history=P, history_stride=8, history_len=8, lengths=P, prompts=P, repetition=P, presence=P, frequency=P, bias_tokens=P, bias=P,
+             bias_tokens_stride=4, bias_stride=4, biases=4, masks=P, masks_stride=32, masks_count=2, mask_of=None)
+    l.update(changed)
+    return _lib.lib().mllm_hip_logits_adjust(C.byref(_lib.Logits(**l)), dtype, rows, vocab, None)
+
+
+@pytest.mark.parametrize("args,want", [
+    (dict(dtype=2), BADARG), (dict(rows=-1), BADARG), (dict(vocab=0), BADARG), (dict(vocab=(1 << 24) + 1), SHAPE), (dict(rows=65536), SHAPE), (dict(x=None), BADARG), (dict(y=None), BADARG),
+    (dict(history=None), BADARG), (dict(history_len=-1), BADARG), (dict(history_len=1 << 31), SHAPE), (dict(biases=-1), BADARG), (dict(biases=(1 << 31) - 1), SHAPE), (dict(bias=None), BADARG),
+    (dict(bias_tokens=None), BADARG), (dict(masks=None), BADARG), (dict(masks_count=1), BADARG), (dict(masks_count=-1), BADARG), (dict(y_stride=999), BADARG), (dict(y_stride=0), BADARG),
+    (dict(y_stride=1001), BADARG), (dict(x_stride=0), BADARG), (dict(x=ODD), ALIGN), (dict(y=P + 1, dtype=BF16), ALIGN), (dict(rows=0, x=None), 0)] +
+    [({name: ODD}, ALIGN) for name in ("history", "lengths", "prompts", "repetition", "presence", "frequency", "bias_tokens", "bias", "masks", "mask_of")])
+def test_logits_adjust(args, want):
+    assert _adjust(**args) == want
+
+
+def test_logits_adjust_without_a_struct():
+    assert _lib.lib().mllm_hip_logits_adjust(None, F32, 1, 10, None) == BADARG
