@@ -688,6 +688,27 @@ int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_t T, cons
                              int64_t max_tokens, int64_t max_keys, const uint64_t* tree, int64_t tree_stride, int64_t tree_words, float scale,
                              void* workspace, size_t workspace_bytes, void* stream);
 
+/* Attention over an encoder's states, which have another length than the queries and no order among them: token t of sequence b (row cu_tokens[b] + t of q, cu_tokens int32
+ * [B + 1]) sees keys key_first[b] .. key_first[b] + key_count[b] - 1 (int32 [B], held to 0 .. keys), of key head h / (heads / kv heads).  A decoder's tokens over a picture's
+ * states; with as many keys as tokens an encoder's own attention, whole or in windows (a sequence each); sequences may share keys.
+ *   o[t][h] = sum_j p_j v_j / sum_j p_j,  p_j = exp(scale * (q . k_j) - max); a token without keys, or with scores of -inf alone: zeros.  Keys of others have no effect, NaN
+ * included; an infinity or a NaN among a token's values makes that element of its result infinite or NaN.  Finite scores times scale are below 2^30.
+ * q->x, q->y: F32 or BF16 (weight is not looked at); rows of q in no sequence, and those behind a sequence's first max_tokens, stay as they are in y.  y may not be x.
+ * head_dim % 8 == 0, <= 256 (64, 80, 96, 128 and 256 are what the kernels are made for, others take the next); heads a multiple of kv->heads; 0 < scale <= 2e38; B <= 65535.
+ * max_keys: the host's bound of a sequence's keys (any; it decides into how many pieces keys are cut).  fp32 results are within fp32 sums of the formula, bf16 ones take the weights p in bf16.
+ * workspace: ..._workspace_bytes (0: none), 16-byte aligned; less is MLLM_HIP_E_BADARG.  One launch, two where keys are cut. */
+typedef struct mllm_hip_states { /* keys and values in bf16: key j of head h at element j * k_stride + h * k_head_stride of k, head_dim elements in a row; v likewise */
+  const void* k;
+  const void* v;
+  int64_t k_stride, k_head_stride, v_stride, v_head_stride; /* multiples of 8, pointers 16-byte aligned; 0 <= k_stride, v_stride <= 2^23 */
+  int64_t keys;                                             /* rows that are there, < 2^31 */
+  int heads, head_dim;
+} mllm_hip_states;
+size_t mllm_hip_attention_cross_workspace_bytes(int dtype, int64_t T, int64_t B, int heads, int kv_heads, int head_dim, int64_t max_tokens, int64_t max_keys);
+int mllm_hip_attention_cross(const mllm_hip_heads* q, int dtype, int64_t T, const mllm_hip_states* kv, const int32_t* cu_tokens, const int32_t* key_first,
+                             const int32_t* key_count, int64_t B, int64_t max_tokens, int64_t max_keys, float scale, void* workspace, size_t workspace_bytes,
+                             void* stream);
+
 /* A token from every row of logits [rows][vocab] (F32 or BF16, rows row_stride elements apart) and a uniform number u[row] in [0, 1):
  *   w_i = exp((x_i - max) / temperature), 0 below 2^-52; in descending order (equal logits: lowest index first) the first top_k are kept (0 or
  *   less: all), of these the shortest beginning whose mass is top_p of theirs or more (at least one; 1 or more: all), of these the ones with

@@ -34,6 +34,12 @@ class KVCache(C.Structure):
                 ("pages", C.c_int64), ("page_size", C.c_int64), ("heads", C.c_int), ("head_dim", C.c_int)]
 
 
+class States(C.Structure):
+    """mllm_hip_states"""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_stride", C.c_int64), ("k_head_stride", C.c_int64), ("v_stride", C.c_int64), ("v_head_stride", C.c_int64),
+                ("keys", C.c_int64), ("heads", C.c_int), ("head_dim", C.c_int)]
+
+
 class Logits(C.Structure):
     """mllm_hip_logits"""
     _fields_ = [("x", C.c_void_p), ("y", C.c_void_p), ("x_stride", C.c_int64), ("y_stride", C.c_int64), ("history", C.c_void_p), ("history_stride", C.c_int64),
@@ -213,6 +219,9 @@ def lib():
         L.mllm_hip_sample_workspace_bytes.restype = C.c_size_t
         L.mllm_hip_sample_workspace_bytes.argtypes = [i64, i64]
         L.mllm_hip_sample.argtypes = [vp, ci, i64, i64, i64, vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp]
+        L.mllm_hip_attention_cross_workspace_bytes.restype = C.c_size_t
+        L.mllm_hip_attention_cross_workspace_bytes.argtypes = [ci, i64, i64, ci, ci, ci, i64, i64]
+        L.mllm_hip_attention_cross.argtypes = [rp, ci, i64, C.POINTER(States), vp, vp, vp, i64, i64, i64, cf, vp, C.c_size_t, vp]
         L.mllm_hip_logits_adjust.argtypes = [C.POINTER(Logits), ci, i64, i64, vp]
         _lib = L
     return _lib

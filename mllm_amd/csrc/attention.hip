@@ -28,14 +28,9 @@
 // values at 4 TB/s and, half of the time, partial results (34 MB written and read) and starts.  A prompt of 8192 bf16 tokens 637 us, 860 TFLOP/s of what it has to compute.
 #include <type_traits>
 
-#include "item8.h"
+#include "attention_common.h"
 
 namespace mllmhip {
-
-typedef short at_s16x4 __attribute__((ext_vector_type(4)));
-typedef short at_s16x8 __attribute__((ext_vector_type(8)));
-typedef __bf16 at_bf16x8 __attribute__((ext_vector_type(8)));
-typedef float at_f32x4 __attribute__((ext_vector_type(4)));
 
 struct AttnArgs {
   const void* q;
@@ -125,16 +120,6 @@ __device__ __forceinline__ Place find_place(const AttnArgs& a, int range) {
   return p;
 }
 
-__device__ __forceinline__ float larger(float x, float y) { return __builtin_elementwise_maximum(x, y); }
-template <int N>  // the larger of a lane's and that of the lane N away
-__device__ __forceinline__ float across(float v) {
-  const u32x2 r = N == 16 ? lanes16(__float_as_uint(v)) : lanes32(__float_as_uint(v));
-  return larger(__uint_as_float(r.x), __uint_as_float(r.y));
-}
-// 8 bf16 of a register quad as an operand
-__device__ __forceinline__ at_bf16x8 frag(u32x4 v) { return __builtin_bit_cast(at_bf16x8, v); }
-__device__ __forceinline__ at_f32x4 mma(at_bf16x8 x, at_bf16x8 y, at_f32x4 acc) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(x, y, acc, 0, 0, 0); }
-
 template <int D, int NQ, int WR, bool F32>
 struct Attn {
   static constexpr int WK = 4 / WR;                      // waves along keys
@@ -148,17 +133,6 @@ struct Attn {
   static __device__ __forceinline__ int swz(int row) { return (C == 8) ? (row & 3) | ((row >> 3) & 1) << 2 : (row & 3) | ((row >> 3) & 3) << 2; }
 };
 
-// Two numbers as three bf16 each, cut off after 8 bits of what is left: together they are the numbers.
-__device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t& mid, uint32_t& lo) {
-  const uint32_t xh = __float_as_uint(x), yh = __float_as_uint(y);
-  const float x1 = x - __uint_as_float(xh & 0xffff0000u), y1 = y - __uint_as_float(yh & 0xffff0000u);
-  const uint32_t xm = __float_as_uint(x1), ym = __float_as_uint(y1);
-  const float x2 = x1 - __uint_as_float(xm & 0xffff0000u), y2 = y1 - __uint_as_float(ym & 0xffff0000u);
-  hi = __builtin_amdgcn_perm(yh, xh, 0x07060302u);  // the high halves of both
-  mid = __builtin_amdgcn_perm(ym, xm, 0x07060302u);
-  lo = __builtin_amdgcn_perm(__float_as_uint(y2), __float_as_uint(x2), 0x07060302u);
-}
-__device__ __forceinline__ float finite(float x) { return (__float_as_uint(x) & 0x7f800000u) == 0x7f800000u ? 0.f : x; }
 // which of the keys k0 .. k0 + 7 token `token` of the sequence sees
 __device__ __forceinline__ uint32_t seen_keys(const AttnArgs& a, const Seq& s, int k0, int token) {
   uint32_t see = 0;
@@ -178,12 +152,6 @@ __device__ __forceinline__ uint32_t seen_keys(const AttnArgs& a, const Seq& s, i
   const int left = s.keys - k0;
   return left >= 8 ? see & 0xff : left <= 0 ? 0 : see & ((1u << left) - 1);
 }
-// whether one of two bf16 is infinite or no number
-__device__ __forceinline__ bool odd_pair(uint32_t v) { return ((v & 0x7f80u) == 0x7f80u) | ((v & 0x7f800000u) == 0x7f800000u); }
-__device__ __forceinline__ uint32_t finite_pair(uint32_t v) {
-  return ((v & 0x7f80u) == 0x7f80u ? 0u : v & 0xffffu) | ((v & 0x7f800000u) == 0x7f800000u ? 0u : v & 0xffff0000u);
-}
-
 // Infinities and NaNs among the values make that element of the rows that see them infinite or NaN, whatever the weight: it is their sum.  What the matrix products
 // leave there is NaN where a weight is too small for its type (or a part of one is 0), and without them where they were taken out for rows that do not see
 // them (in tiles with masks; the sum of the weights has its sign set then).  So results of either kind are looked at once more, behind everything else: a lane's elements

@@ -1,0 +1,517 @@
+// Attention over an encoder's states, which have another length than the queries and no order among them, for gfx950.
+//
+//   o[t][h] = sum_j p_j v_j / sum_j p_j,   p_j = exp(scale * (q[t][h] . k_j) - m),  m = max_j,  over all keys j of the sequence that token t is of.
+//
+// The products are turned as over the paged cache: S^T = K Q^T leaves a lane with one row of Q (a pair of a token and a query head of the group that shares a
+// key head) and eight consecutive keys, which is what the second operand of O^T = V^T P^T takes.  Scores, maxima, sums and O are fp32; P is rounded to bf16 for
+// the product with V (off by 2^-8 of each weight at most, of either sign), fp32 queries and their P enter as three bf16 parts each.
+//
+// A workgroup has four waves, WR along rows times 4 / WR along keys, and goes through the keys in tiles of 64: 16-byte loads into registers while the tile
+// before them is worked on, from there into LDS.  Heads of 72 or 80 elements take three steps of 32 in the first product (zeros behind them) and five tiles of 16 in the second.
+// Where rows, heads and sequences leave CUs idle the keys are cut into pieces, whose O, maximum and sum meet in the workspace; a second launch joins them.
+#include <type_traits>
+
+#include "attention_common.h"
+
+namespace mllmhip {
+
+struct CrossArgs {
+  const void* q;
+  void* o;
+  int64_t q_token, q_head, o_token, o_head;
+  const uint16_t *k, *v;
+  int64_t k_head, v_head;
+  uint32_t k_bytes, v_bytes;  // from a key to the next
+  const int32_t *cu, *first, *count;
+  int64_t keys;  // rows of k and v
+  int T, B, kv, group, D, max_tokens, row_tiles, pieces, min_tiles;
+  float c;                  // scale * log2 e
+  float *part_o, *part_ml;  // [piece][T][heads][D], [2]
+};
+__device__ u32x4 g_no_state[32];  // what keys behind the last read as (never written)
+
+struct CrossSeq {
+  int first, n;  // rows of q
+  int64_t key;   // its first key
+  int keys, per, pieces;  // its number of keys, tiles of a piece, pieces
+};
+__device__ __forceinline__ CrossSeq cross_sequence(const CrossArgs& a, int b) {
+  CrossSeq s;
+  const int lo = max(a.cu[b], 0), hi = min(a.cu[b + 1], a.T);
+  s.first = lo;
+  s.n = min(max(hi - lo, 0), a.max_tokens);
+  s.key = min((int64_t)max(a.first[b], 0), a.keys);
+  s.keys = (int)min((int64_t)max(a.count[b], 0), a.keys - s.key);
+  const int tiles = (s.keys + 63) / 64;
+  s.per = max(a.min_tiles, (tiles + a.pieces - 1) / a.pieces);
+  s.pieces = max(1, (tiles + s.per - 1) / s.per);
+  return s;
+}
+
+template <int DP, int DT, int NQ, int WR, bool F32>
+struct Cross {
+  static constexpr int WK = 4 / WR;          // waves along keys
+  static constexpr int KT = 64;              // keys of a tile
+  static constexpr int SUB = KT / (WK * 32); // 32-key steps of a wave per tile
+  static constexpr int C = DP / 8;           // 16-byte pieces of a row
+  static constexpr int NLOAD = KT * C / 256; // pieces of a tile that a lane loads, of keys and of values
+  static constexpr int PARTS = F32 ? 3 : 1;
+  static constexpr int ROWS = NQ * 16;       // rows of a wave
+  static constexpr int WAVES = DP == 256 ? 1 : 2;
+  // Rows of 8 and of 16 or 32 pieces begin in the same banks every second or every row; rows of 12 every fourth.
+  static __device__ __forceinline__ int swz(int row) {
+    return C == 12 ? (row >> 3) & 3 : C == 8 ? (row & 3) | ((row >> 3) & 1) << 2 : (row & 3) | ((row >> 3) & 3) << 2;
+  }
+};
+
+template <int DP, int DT, int NQ, int WR, bool F32>
+__global__ __launch_bounds__(256, (Cross<DP, DT, NQ, WR, F32>::WAVES)) void cross_kernel(CrossArgs a) {
+  typedef Cross<DP, DT, NQ, WR, F32> P;
+  constexpr int KT = P::KT, C = P::C, WK = P::WK, NLOAD = P::NLOAD, KS = DP / 32, PARTS = P::PARTS;
+  __shared__ __align__(16) uint16_t s_k[2 * KT * DP];
+  __shared__ __align__(16) uint16_t s_v[2 * KT * DP];
+  // Workgroup i runs on XCD i % 8: the row tiles of a piece of keys follow one another on one XCD, whose L2 they share.
+  const int idx = blockIdx.x >> 3, rt = idx % a.row_tiles, place = (idx / a.row_tiles) * 8 + (blockIdx.x & 7);
+  const int h = place % a.kv, piece = place / a.kv % a.pieces, b = place / a.kv / a.pieces;
+  if (b >= a.B) return;
+  const CrossSeq s = cross_sequence(a, b);
+  const int rows = s.n * a.group, row0 = rt * P::ROWS * WR;
+  if (row0 >= rows || piece >= s.pieces) return;
+  const int k_begin = piece * s.per * KT, k_end = min(k_begin + s.per * KT, s.keys);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave % WR, wk = wave / WR;
+  const int col = lane & 15, g = lane >> 4;
+
+  // Piece i of a lane's: piece at[i] % C of row at[i] / C of a tile.  Pieces behind a head's end are zeros in LDS from the beginning.
+  const int real = a.D / 8;
+  int row_of[NLOAD], to[NLOAD];
+  uint32_t koff[NLOAD], voff[NLOAD];
+  bool has[NLOAD];
+#pragma unroll
+  for (int i = 0; i < NLOAD; i++) {
+    const int e = i * 256 + tid, r = e / C, p = e % C;
+    row_of[i] = r;
+    has[i] = p < real;
+    to[i] = r * DP + (p ^ P::swz(r)) * 8;
+    koff[i] = r * a.k_bytes + p * 16;
+    voff[i] = r * a.v_bytes + p * 16;
+    if (!has[i]) {
+#pragma unroll
+      for (int half = 0; half < 2; half++) {
+        *reinterpret_cast<u32x4*>(s_k + half * KT * DP + to[i]) = u32x4{0, 0, 0, 0};
+        *reinterpret_cast<u32x4*>(s_v + half * KT * DP + to[i]) = u32x4{0, 0, 0, 0};
+      }
+    }
+  }
+  typedef const __attribute__((address_space(1))) u32x4* global_row;
+  const uint64_t zero = (uint64_t)(uintptr_t)g_no_state;
+  const uint64_t k_at = (uint64_t)(uintptr_t)(a.k + h * a.k_head) + s.key * a.k_bytes, v_at = (uint64_t)(uintptr_t)(a.v + h * a.v_head) + s.key * a.v_bytes;
+  u32x4 rk[NLOAD], rv[NLOAD];
+  auto ask_tile = [&](int k0) {
+#pragma unroll
+    for (int i = 0; i < NLOAD; i++) {
+      const bool good = k0 + row_of[i] < k_end && has[i];
+      rk[i] = *reinterpret_cast<global_row>(good ? k_at + (uint64_t)k0 * a.k_bytes + koff[i] : zero);
+      rv[i] = *reinterpret_cast<global_row>(good ? v_at + (uint64_t)k0 * a.v_bytes + voff[i] : zero);
+    }
+  };
+  auto put_tile = [&](auto half) {
+#pragma unroll
+    for (int i = 0; i < NLOAD; i++) {
+      if (!has[i]) continue;
+      *reinterpret_cast<u32x4*>(s_k + half * (KT * DP) + to[i]) = rk[i];
+      *reinterpret_cast<u32x4*>(s_v + half * (KT * DP) + to[i]) = rv[i];
+    }
+  };
+  if (k_begin < k_end) ask_tile(k_begin);
+
+  // Q: second operand, row `col` of every 16, elements 32 s + 8 g .. + 7
+  at_bf16x8 fq[NQ][KS][PARTS];
+#pragma unroll
+  for (int i = 0; i < NQ; i++) {
+    const int r = row0 + wr * P::ROWS + i * 16 + col;
+    const bool live = r < rows;
+    const int token = live ? r / a.group : 0, head = h * a.group + (live ? r - token * a.group : 0);
+    const int64_t at = (s.first + token) * a.q_token + head * a.q_head + 8 * g;
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) query_parts<F32>(a.q, at + 32 * ks, live && 32 * ks + 8 * g < a.D, fq[i][ks]);
+  }
+#pragma unroll
+  for (int i = 0; i < NQ; i++)
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+      for (int p = 0; p < PARTS; p++) asm volatile("" : "+v"(fq[i][ks][p]));  // (here from now on: a wait for it in the loop would be one for the next tile's loads)
+
+  at_f32x4 acc[NQ][DT];
+  float m[NQ], l[NQ];  // the maximum so far times c; the sum of this lane's keys
+#pragma unroll
+  for (int i = 0; i < NQ; i++) {
+    m[i] = -INFINITY;
+    l[i] = 0.f;
+#pragma unroll
+    for (int d = 0; d < DT; d++) acc[i][d] = at_f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  const bool busy = row0 + wr * P::ROWS < rows;  // (a wave without rows loads with the others and leaves its SIMD to them)
+  auto work = [&](int k0, auto last_, auto half) {
+    constexpr bool last = decltype(last_)::value;  // the tile may have keys behind the last
+#pragma unroll
+    for (int u = 0; u < P::SUB; u++) {
+      const int base = (u * WK + wk) * 32, key0 = k0 + base;
+      if (last && key0 >= k_end) break;
+      at_f32x4 sa[NQ], sb[NQ];
+#pragma unroll
+      for (int i = 0; i < NQ; i++) sa[i] = sb[i] = at_f32x4{0.f, 0.f, 0.f, 0.f};
+      const int ra = half * KT + base + 8 * (col >> 2) + (col & 3), x = P::swz(ra);
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) {
+        const int at = ra * DP + ((4 * ks + g) ^ x) * 8;
+        const at_bf16x8 ka = frag(*reinterpret_cast<const u32x4*>(s_k + at)), kb = frag(*reinterpret_cast<const u32x4*>(s_k + at + 4 * DP));
+#pragma unroll
+        for (int i = 0; i < NQ; i++) {
+#pragma unroll
+          for (int p = PARTS - 1; p >= 0; p--) {  // the smallest part first
+            sa[i] = mma(ka, fq[i][ks][p], sa[i]);
+            sb[i] = mma(kb, fq[i][ks][p], sb[i]);
+          }
+        }
+      }
+      at_bf16x8 fp[PARTS][NQ];
+#pragma unroll
+      for (int i = 0; i < NQ; i++) {
+        float y[8], top;
+        auto scores = [&](const at_f32x4& a0, const at_f32x4& b0) {
+#pragma unroll
+          for (int j = 0; j < 4; j++) y[j] = a0[j], y[4 + j] = b0[j];
+          if (last) {
+            const int left = k_end - key0 - 8 * g;
+#pragma unroll
+            for (int j = 0; j < 8; j++) y[j] = j < left ? y[j] : -INFINITY;
+          }
+          top = larger(larger(larger(y[0], y[1]), larger(y[2], y[3])), larger(larger(y[4], y[5]), larger(y[6], y[7])));
+          top = across<16>(top);
+          top = across<32>(top) * a.c;
+        };
+        scores(sa[i], sb[i]);
+        if (__ballot(F32 ? !(top <= m[i] + 8.f) : top > m[i] + 8.f)) {  // (weights of up to 2^8 do as well: most steps leave O alone)
+          if constexpr (F32) {
+            // An infinite element of a key makes a NaN with the second and third part of a query's, which may be 0: it counts with the first alone, which
+            // has the sign.  Such scores, and those that are NaN anyway, are formed once more.
+            if (__builtin_expect(__ballot(top != top) != 0, 0)) {
+              at_f32x4 ta = {0.f, 0.f, 0.f, 0.f}, tb = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+              for (int ks = 0; ks < KS; ks++) {
+                const int at = ra * DP + ((4 * ks + g) ^ x) * 8;
+                const u32x4 ka = *reinterpret_cast<const u32x4*>(s_k + at), kb = *reinterpret_cast<const u32x4*>(s_k + at + 4 * DP);
+                const at_bf16x8 fa = frag(u32x4{finite_pair(ka.x), finite_pair(ka.y), finite_pair(ka.z), finite_pair(ka.w)}),
+                                fb = frag(u32x4{finite_pair(kb.x), finite_pair(kb.y), finite_pair(kb.z), finite_pair(kb.w)});
+#pragma unroll
+                for (int p = PARTS - 1; p > 0; p--) {
+                  ta = mma(fa, fq[i][ks][p], ta);
+                  tb = mma(fb, fq[i][ks][p], tb);
+                }
+                ta = mma(frag(ka), fq[i][ks][0], ta);
+                tb = mma(frag(kb), fq[i][ks][0], tb);
+              }
+              scores(ta, tb);
+            }
+          }
+          const float next = fmaxf(m[i], top), fix = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - next);
+          m[i] = next;
+          l[i] *= fix;
+#pragma unroll
+          for (int d = 0; d < DT; d++) acc[i][d] *= fix;
+        }
+        const float ref = m[i] == -INFINITY ? 0.f : m[i];  // (nothing seen yet: every p is exp2(-inf))
+#pragma unroll
+        for (int j = 0; j < 8; j++) y[j] = __builtin_amdgcn_exp2f(fmaf(y[j], a.c, -ref));
+        l[i] += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+        if constexpr (!F32) {
+          fp[0][i] = frag(u32x4{pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7])});
+        } else {
+          uint32_t part[3][4];
+#pragma unroll
+          for (int j = 0; j < 4; j++) split2(y[2 * j], y[2 * j + 1], part[0][j], part[1][j], part[2][j]);
+#pragma unroll
+          for (int p = 0; p < 3; p++) fp[p][i] = frag(u32x4{part[p][0], part[p][1], part[p][2], part[p][3]});
+        }
+      }
+      // V^T: lane i of 16 asks for elements 4 (i % 4) .. + 3 of key 8 g + i / 4 and gets element i of keys 8 g .. + 3
+      const int rv0 = half * KT + base + 8 * g + (col >> 2), xv = P::swz(rv0);
+#pragma unroll
+      for (int d = 0; d < DT; d++) {
+        const int at = rv0 * DP + ((2 * d + ((col & 3) >> 1)) ^ xv) * 8 + (col & 1) * 4;
+        typedef __attribute__((address_space(3))) at_s16x4* lds_ptr;
+        const at_s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(s_v + at));
+        const at_s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(s_v + at + 4 * DP));
+        const at_bf16x8 fv = frag(__builtin_bit_cast(u32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7)));
+#pragma unroll
+        for (int i = 0; i < NQ; i++) {
+#pragma unroll
+          for (int p = PARTS - 1; p >= 0; p--) acc[i][d] = mma(fv, fp[p][i], acc[i][d]);
+        }
+      }
+    }
+  };
+  typedef std::integral_constant<int, 0> Lower;
+  typedef std::integral_constant<int, 1> Upper;
+  int k0 = k_begin;  // the tile that is worked on
+  if (k_begin < k_end) {
+    put_tile(Lower());
+    if (k_begin + KT < k_end) ask_tile(k_begin + KT);
+    __syncthreads();
+  }
+  auto turn = [&](auto last_, auto half, auto other) {
+    if (busy) work(k0, last_, half);
+    k0 += KT;
+    if (k0 < k_end) {  // into the other half of LDS: everyone is past the tile that was there
+      put_tile(other);
+      if (k0 + KT < k_end) ask_tile(k0 + KT);
+      __syncthreads();
+    }
+  };
+  // Whole tiles in turns whose halves of LDS are constants; then, in code of its own, the one that may end before its last key.
+  int half = 0;
+  while (k0 + KT <= k_end) {
+    turn(std::false_type(), Lower(), Upper());
+    half = 1;
+    if (k0 + KT > k_end) break;
+    turn(std::false_type(), Upper(), Lower());
+    half = 0;
+  }
+  if (k0 < k_end) turn(std::true_type(), half, half ^ 1);
+#pragma unroll
+  for (int i = 0; i < NQ; i++) l[i] = sum32(sum16(l[i]));
+
+  const int heads = a.kv * a.group;
+  // a row's elements d .. d + 3
+  auto put = [&](int row, int d, at_f32x4 x, float mm, float sum) {
+    if (d >= a.D) return;
+    const int t = s.first + row / a.group, head = h * a.group + row % a.group;
+    if (s.pieces > 1) {
+      const int64_t at = ((int64_t)piece * a.T + t) * heads + head;
+      *reinterpret_cast<at_f32x4*>(a.part_o + at * a.D + d) = x;
+      if (d == 0) {
+        a.part_ml[2 * at] = mm;
+        a.part_ml[2 * at + 1] = sum;
+      }
+      return;
+    }
+    x *= sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);  // (no key: zeros; a NaN stays)
+    const int64_t at = t * a.o_token + head * a.o_head + d;
+    if (F32) *reinterpret_cast<at_f32x4*>(reinterpret_cast<float*>(a.o) + at) = x;
+    else *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(a.o) + at) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+  };
+  if constexpr (WK == 1) {
+#pragma unroll
+    for (int i = 0; i < NQ; i++) {
+      const int row = row0 + wr * P::ROWS + i * 16 + col;
+      if (row >= rows) continue;
+#pragma unroll
+      for (int d = 0; d < DT; d++) put(row, 16 * d + 4 * g, acc[i][d], m[i], l[i]);
+    }
+  } else {
+    // The waves along keys meet in LDS, 16 rows at a time: O of a row where the keys were, its maximum and sum where the values were.
+    constexpr int Q4 = DT * 4, IT = (16 * Q4 + WK * 64 - 1) / (WK * 64);  // quads of a row; quads of a lane
+    float* so = reinterpret_cast<float*>(s_k);            // [wave][16][DT * 16]
+    float* sm = reinterpret_cast<float*>(s_v);            // [wave][16][2]
+    static_assert(4 * 16 * DT * 16 * 4 <= 2 * KT * DP * 2, "");
+#pragma unroll
+    for (int i = 0; i < NQ; i++) {
+      __syncthreads();
+#pragma unroll
+      for (int d = 0; d < DT; d++) *reinterpret_cast<at_f32x4*>(so + ((wave * 16 + col) * Q4 + ((4 * d + g) ^ (col & 3))) * 4) = acc[i][d];
+      if (g == 0) {
+        sm[(wave * 16 + col) * 2] = m[i];
+        sm[(wave * 16 + col) * 2 + 1] = l[i];
+      }
+      __syncthreads();
+#pragma unroll
+      for (int it = 0; it < IT; it++) {
+        const int e = wk * 64 + lane + it * WK * 64, r = e / Q4, p = e % Q4;
+        const int row = row0 + wr * P::ROWS + i * 16 + r;
+        if (r >= 16 || row >= rows) continue;
+        float top = -INFINITY;
+#pragma unroll
+        for (int w = 0; w < WK; w++) top = fmaxf(top, sm[((w * WR + wr) * 16 + r) * 2]);
+        const float ref = top == -INFINITY ? 0.f : top;
+        at_f32x4 x = {0.f, 0.f, 0.f, 0.f};
+        float sum = 0.f;
+#pragma unroll
+        for (int w = 0; w < WK; w++) {
+          const int at = (w * WR + wr) * 16 + r;
+          const float f = __builtin_amdgcn_exp2f(sm[at * 2] - ref);
+          sum += sm[at * 2 + 1] * f;
+          x += *reinterpret_cast<const at_f32x4*>(so + (at * Q4 + (p ^ (r & 3))) * 4) * f;
+        }
+        put(row, p * 4, x, top, sum);
+      }
+    }
+  }
+}
+
+// Joins the pieces of a row: 16 bytes of it per lane, L lanes a row
+template <int L, bool F32>
+__global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
+  const int heads = a.kv * a.group, b = blockIdx.y, tid = threadIdx.x, d = tid % L * 4;
+  const CrossSeq s = cross_sequence(a, b);
+  if (s.pieces < 2) return;
+  const int i = blockIdx.x * (256 / L) + tid / L;
+  if (i >= s.n * heads || d >= a.D) return;
+  const int64_t all = (int64_t)a.T * heads, at = (int64_t)s.first * heads + i;
+  float m = -INFINITY, sum = 0.f;
+  at_f32x4 x = {0.f, 0.f, 0.f, 0.f};
+  constexpr int U = 4;
+  for (int k = 0; k < s.pieces; k += U) {
+    float mk[U], lk[U];
+    at_f32x4 xk[U];
+#pragma unroll
+    for (int j = 0; j < U; j++) {
+      const int64_t from = min(k + j, s.pieces - 1) * all + at;
+      mk[j] = a.part_ml[2 * from];
+      lk[j] = a.part_ml[2 * from + 1];
+      xk[j] = *reinterpret_cast<const at_f32x4*>(a.part_o + from * a.D + d);
+    }
+#pragma unroll
+    for (int j = 0; j < U; j++) {
+      if (k + j >= s.pieces) break;
+      const float next = fmaxf(m, mk[j]), ref = next == -INFINITY ? 0.f : next;
+      const float f = __builtin_amdgcn_exp2f(m - ref), fk = __builtin_amdgcn_exp2f(mk[j] - ref);
+      x = x * f + xk[j] * fk;
+      sum = sum * f + lk[j] * fk;
+      m = next;
+    }
+  }
+  x *= sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
+  const int t = i / heads;
+  const int64_t to = (s.first + t) * a.o_token + (i - t * heads) * a.o_head + d;
+  if (F32) *reinterpret_cast<at_f32x4*>(reinterpret_cast<float*>(a.o) + to) = x;
+  else *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(a.o) + to) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+}
+
+// ---- host side ------------------------------------------------------------------------------------------------------------
+struct CrossPlan {
+  int nq, wr, row_tiles, pieces, min_tiles;
+};
+// Rows of a workgroup by the rows there are; keys are cut while there are under 1024 workgroups without that, into pieces of two tiles and of twice as many keys as rows at least.
+static CrossPlan cross_plan(bool f32, int64_t B, int heads, int kv, int64_t max_tokens, int64_t max_keys, int D) {
+  CrossPlan p;
+  if (max_keys > 0x7fffffff) max_keys = 0x7fffffff;
+  const int64_t rows = max_tokens * (heads / kv);
+  p.nq = rows <= 64 || f32 || D > 128 ? 1 : 2;
+  p.wr = rows <= 32 ? 2 : 4;
+  const int64_t per = (int64_t)p.nq * 16 * p.wr, row_tiles = (rows + per - 1) / per;
+  p.row_tiles = (int)row_tiles;
+  const int64_t least = (2 * (rows < per ? rows : per) + 63) / 64;
+  p.min_tiles = (int)(least > 2 ? least : 2);
+  const int64_t tiles = (max_keys + 63) / 64, most = (tiles + p.min_tiles - 1) / p.min_tiles, uncut = B * kv * row_tiles, wanted = (1023 + uncut) / uncut;
+  p.pieces = (int)(uncut >= 512 || most < 2 ? 1 : wanted < most ? wanted : most);
+  return p;
+}
+static size_t cross_room(const CrossPlan& p, int64_t T, int heads, int D) { return p.pieces > 1 ? (size_t)p.pieces * T * heads * (D + 2) * sizeof(float) : 0; }
+static bool cross_sizes(int dtype, int64_t T, int64_t B, int heads, int kv, int head_dim, int64_t max_tokens, int64_t max_keys) {
+  return (dtype == MLLM_HIP_F32 || dtype == MLLM_HIP_BF16) && T >= 0 && B >= 0 && heads >= 1 && kv >= 1 && head_dim >= 1 && max_tokens >= 0 && max_keys >= 0;
+}
+static bool cross_shape(int64_t T, int64_t B, int heads, int kv, int head_dim, int64_t max_tokens) {
+  return head_dim % 8 == 0 && head_dim <= 256 && heads % kv == 0 && heads <= 65536 && T <= 0x7fffffff / heads && B <= 65535 && max_tokens <= 0x7fffffff / heads;
+}
+
+}  // namespace mllmhip
+
+using namespace mllmhip;
+
+MLLM_API size_t mllm_hip_attention_cross_workspace_bytes(int dtype, int64_t T, int64_t B, int heads, int kv_heads, int head_dim, int64_t max_tokens, int64_t max_keys) {
+  if (!cross_sizes(dtype, T, B, heads, kv_heads, head_dim, max_tokens, max_keys) || !cross_shape(T, B, heads, kv_heads, head_dim, max_tokens)) return 0;
+  if (T == 0 || B == 0 || max_tokens == 0) return 0;
+  if (max_tokens > T) max_tokens = T;
+  return cross_room(cross_plan(dtype == MLLM_HIP_F32, B, heads, kv_heads, max_tokens, max_keys, head_dim), T, heads, head_dim);
+}
+
+MLLM_API int mllm_hip_attention_cross(const mllm_hip_heads* q, int dtype, int64_t T, const mllm_hip_states* kv, const int32_t* cu_tokens, const int32_t* key_first,
+                                      const int32_t* key_count, int64_t B, int64_t max_tokens, int64_t max_keys, float scale, void* workspace, size_t workspace_bytes,
+                                      void* stream) {
+  if (!q || !kv || kv->keys < 0 || !(scale > 0.f) || scale > 2e38f) return MLLM_HIP_E_BADARG;
+  if (!cross_sizes(dtype, T, B, q->heads, kv->heads, kv->head_dim, max_tokens, max_keys)) return MLLM_HIP_E_BADARG;
+  if (!cross_shape(T, B, q->heads, kv->heads, kv->head_dim, max_tokens) || kv->keys > 0x7fffffff || kv->k_stride < 0 || kv->v_stride < 0 || kv->k_stride > (1 << 23) ||
+      kv->v_stride > (1 << 23))
+    return MLLM_HIP_E_SHAPE;
+  if (T == 0 || B == 0 || max_tokens == 0) return 0;
+  if (max_tokens > T) max_tokens = T;
+  if (!q->x || !q->y || (kv->keys && (!kv->k || !kv->v)) || !cu_tokens || !key_first || !key_count) return MLLM_HIP_E_BADARG;
+  const int wide = dtype == MLLM_HIP_F32 ? 4 : 2;
+  auto al = [](const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
+  auto whole = [&](int64_t stride) { return stride * wide % 16 == 0; };
+  if (!al(q->x, 16) || !al(q->y, 16) || !al(kv->k, 16) || !al(kv->v, 16) || !whole(q->x_token_stride) || !whole(q->x_head_stride) || !whole(q->y_token_stride) ||
+      !whole(q->y_head_stride) || kv->k_stride % 8 || kv->v_stride % 8 || kv->k_head_stride % 8 || kv->v_head_stride % 8 || !al(cu_tokens, 4) || !al(key_first, 4) ||
+      !al(key_count, 4) || !al(workspace, 16))
+    return MLLM_HIP_E_ALIGN;
+  if (q->x == q->y || !own_places(*q, T)) return MLLM_HIP_E_BADARG;
+  const bool f32 = dtype == MLLM_HIP_F32;
+  const int heads = q->heads, D = kv->head_dim;
+  const CrossPlan p = cross_plan(f32, B, heads, kv->heads, max_tokens, max_keys, D);
+  const size_t need = cross_room(p, T, heads, D);
+  if (need && (!workspace || workspace_bytes < need)) return MLLM_HIP_E_BADARG;
+  const int64_t groups = (B * kv->heads * p.pieces + 7) / 8 * 8;
+  if (groups > 0xffffff / p.row_tiles) return MLLM_HIP_E_SHAPE;
+  CrossArgs a = {};
+  a.q = q->x;
+  a.o = q->y;
+  a.q_token = q->x_token_stride;
+  a.q_head = q->x_head_stride;
+  a.o_token = q->y_token_stride;
+  a.o_head = q->y_head_stride;
+  a.k = reinterpret_cast<const uint16_t*>(kv->k);
+  a.v = reinterpret_cast<const uint16_t*>(kv->v);
+  a.k_head = kv->k_head_stride;
+  a.v_head = kv->v_head_stride;
+  a.k_bytes = (uint32_t)kv->k_stride * 2;
+  a.v_bytes = (uint32_t)kv->v_stride * 2;
+  a.cu = cu_tokens;
+  a.first = key_first;
+  a.count = key_count;
+  a.keys = kv->keys;
+  a.T = (int)T;
+  a.B = (int)B;
+  a.kv = kv->heads;
+  a.group = heads / kv->heads;
+  a.D = D;
+  a.max_tokens = (int)max_tokens;
+  a.row_tiles = p.row_tiles;
+  a.pieces = p.pieces;
+  a.min_tiles = p.pieces > 1 ? p.min_tiles : 1;
+  a.c = scale * 1.44269504088896341f;
+  a.part_o = reinterpret_cast<float*>(workspace);
+  a.part_ml = p.pieces > 1 ? a.part_o + (size_t)p.pieces * T * heads * D : nullptr;
+  hipStream_t st = (hipStream_t)stream;
+  const dim3 grid((unsigned)(groups * p.row_tiles));
+  const int form = p.nq * 10 + p.wr;
+  auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a); };
+#define CROSS(DP_, DT_)                                                      \
+  if (f32) {                                                                 \
+    if (form == 12) go(cross_kernel<DP_, DT_, 1, 2, true>);                  \
+    else go(cross_kernel<DP_, DT_, 1, 4, true>);                             \
+  } else {                                                                   \
+    if (form == 12) go(cross_kernel<DP_, DT_, 1, 2, false>);                 \
+    else if (form == 14) go(cross_kernel<DP_, DT_, 1, 4, false>);            \
+    else go(cross_kernel<DP_, DT_, DP_ == 256 ? 1 : 2, 4, false>);           \
+  }
+  if (D <= 64) { CROSS(64, 4) }
+  else if (D <= 80) { CROSS(96, 5) }
+  else if (D <= 96) { CROSS(96, 6) }
+  else if (D <= 128) { CROSS(128, 8) }
+  else { CROSS(256, 16) }
+#undef CROSS
+  RC_RET((int)hipGetLastError());
+  if (p.pieces > 1) {
+    const int lanes = D <= 64 ? 16 : D <= 128 ? 32 : 64, per = 256 / lanes;
+    const dim3 jgrid((unsigned)((max_tokens * heads + per - 1) / per), (unsigned)B);
+    auto join = [&](auto kern) { hipLaunchKernelGGL(kern, jgrid, dim3(256), 0, st, a); };
+#define JOIN(L_)                              \
+  if (f32) join(cross_join_kernel<L_, true>); \
+  else join(cross_join_kernel<L_, false>)
+    if (lanes == 16) { JOIN(16); }
+    else if (lanes == 32) { JOIN(32); }
+    else { JOIN(64); }
+#undef JOIN
+  }
+  return (int)hipGetLastError();
+}

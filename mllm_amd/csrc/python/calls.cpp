@@ -489,6 +489,32 @@ PyObject* attention_paged(Args a) {
   return THPVariable_Wrap(y);
 }
 
+// (q, k, v, cu_tokens, key_first, key_count, max_tokens, max_keys, scale, out, workspace)
+PyObject* attention_cross(Args a) {
+  const int64_t device = current_device();
+  const at::Tensor& q = tensor(a[0]);
+  const int dtype = xdtype(q);
+  const at::Tensor &k = local(a[1], device, at::kBFloat16), &v = local(a[2], device, at::kBFloat16);
+  require(q.dim() == 3 && k.dim() == 3 && k.sizes() == v.sizes() && k.size(1) >= 1 && k.size(1) <= 65536 && k.size(2) >= 1 && k.size(2) <= 65536);
+  require(k.size(2) == 1 || ((k.stride(2) == 1 && v.stride(2) == 1) || k.size(0) == 0));
+  const int64_t T = q.size(0), D = k.size(2);
+  mllm_hip_heads qp = heads_of(q, T, D, q.scalar_type(), device);
+  const mllm_hip_states kv = {k.data_ptr(), v.data_ptr(), stride_of(k, 0), stride_of(k, 1), stride_of(v, 0), stride_of(v, 1), k.size(0), (int)k.size(1), (int)D};
+  require(a[3] != Py_None && a[4] != Py_None && a[5] != Py_None);
+  const int64_t B = local(a[4], device, at::kInt).numel(), tokens = integer(a[6]), keys = integer(a[7]);
+  const int32_t *cu = vector_of<int32_t>(a[3], device, at::kInt, B + 1), *first = vector_of<int32_t>(a[4], device, at::kInt, B),
+                *count = vector_of<int32_t>(a[5], device, at::kInt, B);
+  const float scale = a[8] == Py_None ? 1.0f / std::sqrt((float)D) : (float)real(a[8]);
+  at::Tensor y, work;
+  results_to(qp, q, a[9], y, device);
+  require(T == 0 || qp.y != qp.x);
+  const size_t need = mllm_hip_attention_cross_workspace_bytes(dtype, T, B, qp.heads, kv.heads, (int)D, tokens, keys);
+  void* wp = workspace_on(device, a[10], need, work);
+  void* st = stream();
+  run("mllm_hip_attention_cross", [&] { return mllm_hip_attention_cross(&qp, dtype, T, &kv, cu, first, count, B, tokens, keys, scale, wp, need, st); });
+  return THPVariable_Wrap(y);
+}
+
 // (logits, u, temperature, top_k, top_p, min_p, out, workspace)
 PyObject* sample(Args a) {
   const int64_t device = current_device();
@@ -580,7 +606,7 @@ PyObject* entry(PyObject*, Args args, Py_ssize_t n) {
 PyMethodDef g_methods[] = {CALL(linear_q_gemv, 8), CALL(linear_q_gemv_multi, 6), CALL(softmax, 1), CALL(topk, 4), CALL(matmul, 5),
                            CALL(w8a8_linear_packed, 7), CALL(w4a16_gemm_packed, 6), CALL(linear_q_gemm, 7), CALL(linear_kq_gemm, 6),
                            CALL(qk_norm_rope, 11), CALL(kv_append, 15), CALL(attention_paged, 12), CALL(sample, 8),
-                           CALL(adjust_logits, 12), {nullptr, nullptr, 0, nullptr}};
+                           CALL(adjust_logits, 12), CALL(attention_cross, 11), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "mllm_calls", nullptr, -1, g_methods};
 
 }  // namespace

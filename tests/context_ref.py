@@ -44,3 +44,25 @@ def adjust(x, said=(), prompt=0, repetition=1.0, presence=0.0, frequency=0.0, bi
     if allowed is not None:
         x[~np.asarray(allowed, bool)] = -np.inf
     return x, size
+
+
+def cross(q, k, v, cu, first, count, scale):
+    """q [T, Hq, D]; k, v [S, Hkv, D] -> float64 [T, Hq, D] (rows in no sequence NaN) and, for error bounds, the same with |v| for v and the largest sum of a
+    score's absolute terms [T, Hq, 1]"""
+    q, k, v = [x.detach().cpu().double() for x in (q, k, v)]
+    group = q.shape[1] // k.shape[1]
+    out, size, terms = torch.full(q.shape, float("nan"), dtype=torch.float64), torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape[:2] + (1,), dtype=torch.float64)
+    for b in range(len(first)):
+        rows = slice(int(cu[b]), int(cu[b + 1]))
+        lo = min(max(int(first[b]), 0), k.shape[0])
+        n = min(max(int(count[b]), 0), k.shape[0] - lo)
+        for h in range(q.shape[1]):
+            kh, vh, qh = k[lo:lo + n, h // group], v[lo:lo + n, h // group], q[rows, h]
+            if n == 0:
+                out[rows, h] = 0
+                continue
+            p = torch.softmax(qh @ kh.t() * scale, -1)
+            out[rows, h], size[rows, h] = p @ vh, p @ vh.abs()
+            if len(qh):
+                terms[rows, h] = (qh.abs() @ kh.abs().t()).amax(-1, keepdim=True) * scale
+    return out, size, terms

@@ -59,3 +59,35 @@ def test_logits_adjust(args, want):
 
 def test_logits_adjust_without_a_struct():
     assert _lib.lib().mllm_hip_logits_adjust(None, F32, 1, 10, None) == BADARG
+
+
+def _states(**changed):
+    s = dict(k=P, v=P, k_stride=512, k_head_stride=128, v_stride=512, v_head_stride=128, keys=100, heads=4, head_dim=128)
+    s.update(changed)
+    return _lib.States(**s)
+
+
+def _cross(q=None, kv=None, dtype=BF16, T=2, cu=P, first=P, count=P, B=1, tokens=2, keys=40, scale=0.1, work=P, size=1 << 30, no_q=False, no_kv=False):
+    q, kv = q if q is not None else _part(heads=8, y=P + (1 << 30)), kv if kv is not None else _states()
+    return _lib.lib().mllm_hip_attention_cross(None if no_q else C.byref(q), dtype, T, None if no_kv else C.byref(kv), cu, first, count, B, tokens, keys, scale, work, size, None)
+
+
+@pytest.mark.parametrize("args,want", [
+    (dict(no_q=True), BADARG), (dict(no_kv=True), BADARG), (dict(dtype=2), BADARG), (dict(T=-1), BADARG), (dict(B=-1), BADARG), (dict(B=65536), SHAPE), (dict(tokens=-1), BADARG),
+    (dict(keys=-1), BADARG), (dict(keys=1 << 40, size=100), BADARG), (dict(cu=None), BADARG), (dict(first=None), BADARG), (dict(count=None), BADARG), (dict(scale=0.0), BADARG),
+    (dict(scale=float("nan")), BADARG), (dict(scale=float("inf")), BADARG), (dict(scale=3e38), BADARG), (dict(T=1 << 29), SHAPE), (dict(tokens=1 << 29), SHAPE),
+    (dict(kv=_states(head_dim=100)), SHAPE), (dict(kv=_states(head_dim=264)), SHAPE), (dict(kv=_states(head_dim=0)), BADARG), (dict(kv=_states(heads=3)), SHAPE), (dict(kv=_states(heads=0)), BADARG),
+    (dict(kv=_states(k=None)), BADARG), (dict(kv=_states(v=None)), BADARG), (dict(kv=_states(k=ODD)), ALIGN), (dict(kv=_states(v=P + 8)), ALIGN), (dict(kv=_states(k_stride=516)), ALIGN),
+    (dict(kv=_states(v_head_stride=4)), ALIGN), (dict(kv=_states(keys=-1)), BADARG), (dict(kv=_states(keys=1 << 31)), SHAPE), (dict(kv=_states(k_stride=(1 << 23) + 8)), SHAPE),
+    (dict(kv=_states(v_stride=-8)), SHAPE), (dict(q=_part(heads=8, x=None)), BADARG), (dict(q=_part(heads=8)), BADARG), (dict(q=_part(heads=8, x=ODD, y=P)), ALIGN),
+    (dict(q=_part(heads=8, y=P + 8)), ALIGN), (dict(q=_part(heads=8, y=P + 32, y_token_stride=0)), BADARG), (dict(cu=ODD), ALIGN), (dict(first=ODD), ALIGN), (dict(count=ODD), ALIGN),
+    (dict(work=P + 8), ALIGN), (dict(keys=9000, work=None), BADARG), (dict(keys=9000, size=100), BADARG), (dict(T=0), 0), (dict(B=0), 0), (dict(tokens=0), 0)])
+def test_attention_cross(args, want):
+    assert _cross(**args) == want
+
+
+def test_attention_cross_workspace():
+    size = _lib.lib().mllm_hip_attention_cross_workspace_bytes
+    assert size(BF16, 1, 1, 32, 8, 128, 1, 100) == 0 and size(BF16, 1, 1, 32, 8, 128, 1, 5000) > 0
+    assert size(BF16, 3, 2, 32, 8, 128, 4096, 5000) == size(BF16, 3, 2, 32, 8, 128, 3, 5000) > 0
+    assert size(2, 1, 1, 32, 8, 128, 1, 5000) == 0 and size(BF16, 1, 1, 30, 8, 128, 1, 5000) == 0 and size(BF16, 0, 1, 32, 8, 128, 1, 5000) == 0 and size(BF16, 1, 1, 32, 8, 100, 1, 5000) == 0
