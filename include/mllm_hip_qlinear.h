@@ -688,6 +688,30 @@ int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_t T, cons
                              int64_t max_tokens, int64_t max_keys, const uint64_t* tree, int64_t tree_stride, int64_t tree_words, float scale,
                              void* workspace, size_t workspace_bytes, void* stream);
 
+/* What every cached key gets of the new tokens' attention, by which `mllm_hip_kv_evict` judges it: tokens, sequences and positions as in mllm_hip_attention_paged without a tree (a
+ * token sees its sequence's prefix, the new tokens before it and itself; the cache's v is not looked at).  For position j of sequence b and key head h
+ *   mass[b * mass_stride + h * mass_head_stride + j] = (j < prefix[b] ? decay * mass[..] : 0) + sum over the tokens t that see j and the query heads of the group of
+ *       exp(scale * (q . k_j) - max) / (their sum over the keys that t sees)
+ * in fp32, decay 1: added up over calls, 0: mass is not read before.  Tokens that see nothing, or scores of -inf alone, add nothing; a NaN among a token's scores makes NaN of what all its keys get.
+ * Sequences without new tokens and positions from prefix + new tokens on stay as they are.  max_tokens, max_keys: a sequence's new tokens behind the first max_tokens add
+ * nothing; positions from max_keys on are neither seen nor get anything; positions from mass_len on are seen, and what they get is stored nowhere.  q: F32 or BF16 (y and weight are not looked at).
+ * head_dim % 8 == 0, <= 256; heads a multiple of the cache's; 0 < scale <= 2e38; 0 <= decay <= 2e38; table_len * page_size and max_keys up to 2^30, B * kv heads up to 65535.  The sums do not depend on any order of execution: the same
+ * inputs give the same bits.  workspace: ..._workspace_bytes, 16-byte aligned; less is MLLM_HIP_E_BADARG.  Up to three launches. */
+size_t mllm_hip_attention_weights_workspace_bytes(int dtype, int64_t T, int64_t B, int heads, int kv_heads, int head_dim, int64_t max_tokens, int64_t max_keys);
+int mllm_hip_attention_weights(const mllm_hip_heads* q, int dtype, int64_t T, const mllm_hip_kv_cache* cache, float* mass, int64_t mass_stride,
+                               int64_t mass_head_stride, int64_t mass_len, const int32_t* block_table, int64_t table_stride, int64_t table_len,
+                               const int32_t* cu_tokens, const int32_t* prefix, int64_t B, int64_t max_tokens, int64_t max_keys, float decay, float scale,
+                               void* workspace, size_t workspace_bytes, void* stream);
+/* The keys that are worth keeping, copied to the pages of another table: of the first lengths[b] (int32, held to 0 .. what the table and mass_len have) positions of sequence b the first
+ * `first` and the last `recent` stay, of the others the ones with the largest mass (equal ones: lowest position first; a NaN is the smallest), `keep` in all, for every key head its own.
+ * All of them where there are no more than that.  They go, in their order, to places 0, 1, .. of the pages in to_table (int32 [B][to_len], to_stride apart), keys and values;
+ * kept int32 [B][heads][keep] are their positions (-1 behind the last), kept_mass fp32 [B][heads][keep] their mass (0), apart from mass itself.  Nothing else changes: pages that other
+ * sequences share stay whole.  No page of to_table may be one that block_table has, or twice in it.  A page of block_table outside the cache reads as zeros, one of to_table
+ * stores nothing.  first + recent <= keep <= to_len * page_size; head_dim % 8 == 0, <= 512; B * heads <= 65535.  Two launches, no workspace. */
+int mllm_hip_kv_evict(const mllm_hip_kv_cache* cache, const float* mass, int64_t mass_stride, int64_t mass_head_stride, int64_t mass_len, const int32_t* block_table,
+                      int64_t table_stride, int64_t table_len, const int32_t* lengths, int64_t B, const int32_t* to_table, int64_t to_stride, int64_t to_len, int64_t keep,
+                      int64_t first, int64_t recent, int32_t* kept, float* kept_mass, void* stream);
+
 /* Attention over an encoder's states, which have another length than the queries and no order among them: token t of sequence b (row cu_tokens[b] + t of q, cu_tokens int32
  * [B + 1]) sees keys key_first[b] .. key_first[b] + key_count[b] - 1 (int32 [B], held to 0 .. keys), of key head h / (heads / kv heads).  A decoder's tokens over a picture's
  * states; with as many keys as tokens an encoder's own attention, whole or in windows (a sequence each); sequences may share keys.

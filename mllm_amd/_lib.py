@@ -219,6 +219,10 @@ def lib():
         L.mllm_hip_sample_workspace_bytes.restype = C.c_size_t
         L.mllm_hip_sample_workspace_bytes.argtypes = [i64, i64]
         L.mllm_hip_sample.argtypes = [vp, ci, i64, i64, i64, vp, vp, vp, vp, vp, vp, vp, C.c_size_t, vp]
+        L.mllm_hip_attention_weights_workspace_bytes.restype = C.c_size_t
+        L.mllm_hip_attention_weights_workspace_bytes.argtypes = [ci, i64, i64, ci, ci, ci, i64, i64]
+        L.mllm_hip_attention_weights.argtypes = [rp, ci, i64, kv, vp, i64, i64, i64, vp, i64, i64, vp, vp, i64, i64, i64, cf, cf, vp, C.c_size_t, vp]
+        L.mllm_hip_kv_evict.argtypes = [kv, vp, i64, i64, i64, vp, i64, i64, vp, i64, vp, i64, i64, i64, i64, i64, vp, vp, vp]
         L.mllm_hip_attention_cross_workspace_bytes.restype = C.c_size_t
         L.mllm_hip_attention_cross_workspace_bytes.argtypes = [ci, i64, i64, ci, ci, ci, i64, i64]
         L.mllm_hip_attention_cross.argtypes = [rp, ci, i64, C.POINTER(States), vp, vp, vp, i64, i64, i64, cf, vp, C.c_size_t, vp]

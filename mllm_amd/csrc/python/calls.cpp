@@ -489,6 +489,79 @@ PyObject* attention_paged(Args a) {
   return THPVariable_Wrap(y);
 }
 
+// masses [B, heads, n] with a row in one piece
+const at::Tensor& mass_of(PyObject* o, int64_t B, int64_t heads, int64_t device) {
+  const at::Tensor& m = local(o, device, at::kFloat);
+  require(m.dim() == 3 && m.size(0) == B && m.size(1) == heads && (m.size(2) <= 1 || m.stride(2) == 1));
+  return m;
+}
+
+// (q, k_cache, mass, block_table, cu_tokens, prefix, max_tokens, max_keys, decay, scale, workspace)
+PyObject* attention_weights(Args a) {
+  const int64_t device = current_device();
+  const at::Tensor& q = tensor(a[0]);
+  const int dtype = xdtype(q);
+  require(q.dim() == 3);
+  const mllm_hip_kv_cache cache = cache_of(a[1], a[1], device);
+  const int64_t T = q.size(0);
+  mllm_hip_heads qp = heads_of(q, T, cache.head_dim, q.scalar_type(), device);
+  const at::Tensor& table = local(a[3], device, at::kInt);
+  require(table.dim() == 2 && (table.size(1) <= 1 || table.stride(1) == 1));
+  const int64_t B = table.size(0), tokens = integer(a[6]), keys = integer(a[7]);
+  const at::Tensor& mass = mass_of(a[2], B, cache.heads, device);
+  require((B <= 1 || mass.stride(0)) && (cache.heads <= 1 || mass.stride(1)));  // (a place for every head's)
+  require(a[4] != Py_None && a[5] != Py_None);
+  const int32_t *cu = vector_of<int32_t>(a[4], device, at::kInt, B + 1), *prefix = vector_of<int32_t>(a[5], device, at::kInt, B);
+  const float decay = (float)real(a[8]), scale = a[9] == Py_None ? 1.0f / std::sqrt((float)cache.head_dim) : (float)real(a[9]);
+  at::Tensor work;
+  const size_t need = mllm_hip_attention_weights_workspace_bytes(dtype, T, B, qp.heads, cache.heads, cache.head_dim, tokens, keys);
+  void* wp = workspace_on(device, a[10], need, work);
+  void* st = stream();
+  const int64_t table_stride = stride_of(table, 0), table_len = table.size(1), mass_stride = stride_of(mass, 0), mass_head = stride_of(mass, 1), mass_len = mass.size(2);
+  const int32_t* tp = static_cast<const int32_t*>(table.data_ptr());
+  float* mp = static_cast<float*>(mass.data_ptr());
+  run("mllm_hip_attention_weights", [&] {
+    return mllm_hip_attention_weights(&qp, dtype, T, &cache, mp, mass_stride, mass_head, mass_len, tp, table_stride, table_len, cu, prefix, B, tokens, keys, decay, scale, wp, need, st);
+  });
+  return given(a[2]);
+}
+
+// (k_cache, v_cache, mass, block_table, lengths, to_table, keep, first, recent, out)
+PyObject* kv_evict(Args a) {
+  const int64_t device = current_device();
+  const mllm_hip_kv_cache cache = cache_of(a[0], a[1], device);
+  require((cache.page_stride || cache.pages == 1) && (cache.head_stride || cache.heads == 1));  // (what is stored has a place of its own)
+  const at::Tensor &table = local(a[3], device, at::kInt), &to = local(a[5], device, at::kInt);
+  require(table.dim() == 2 && (table.size(1) <= 1 || table.stride(1) == 1) && to.dim() == 2 && (to.size(1) <= 1 || to.stride(1) == 1));
+  const int64_t B = table.size(0), keep = integer(a[6]), first = integer(a[7]), recent = integer(a[8]);
+  require(to.size(0) == B && a[4] != Py_None && keep >= 0 && keep < (1ll << 31));
+  const at::Tensor& mass = mass_of(a[2], B, cache.heads, device);
+  const int32_t* lengths = vector_of<int32_t>(a[4], device, at::kInt, B);
+  at::Tensor kept, kept_mass;
+  if (a[9] == Py_None) {
+    kept = empty({B, cache.heads, keep}, at::kInt);
+    kept_mass = empty({B, cache.heads, keep}, at::kFloat);
+  } else {
+    require(PyTuple_Check(a[9]) && PyTuple_GET_SIZE(a[9]) == 2);
+    kept = local(PyTuple_GET_ITEM(a[9], 0), device, at::kInt);
+    kept_mass = local(PyTuple_GET_ITEM(a[9], 1), device, at::kFloat);
+    for (const at::Tensor* t : {&kept, &kept_mass})
+      require(t->dim() == 3 && t->size(0) == B && t->size(1) == cache.heads && t->size(2) == keep && t->is_contiguous());
+  }
+  void* st = stream();
+  const int64_t mass_stride = stride_of(mass, 0), mass_head = stride_of(mass, 1), mass_len = mass.size(2), table_stride = stride_of(table, 0), table_len = table.size(1),
+                to_stride = stride_of(to, 0), to_len = to.size(1);
+  const float* mp = static_cast<const float*>(mass.data_ptr());
+  const int32_t *tp = static_cast<const int32_t*>(table.data_ptr()), *top = static_cast<const int32_t*>(to.data_ptr());
+  int32_t* kp = static_cast<int32_t*>(kept.data_ptr());
+  float* kmp = static_cast<float*>(kept_mass.data_ptr());
+  run("mllm_hip_kv_evict", [&] {
+    return mllm_hip_kv_evict(&cache, mp, mass_stride, mass_head, mass_len, tp, table_stride, table_len, lengths, B, top, to_stride, to_len, keep, first, recent, kp, kmp, st);
+  });
+  Owned ko(THPVariable_Wrap(kept)), mo(THPVariable_Wrap(kept_mass));
+  return PyTuple_Pack(2, ko.o, mo.o);
+}
+
 // (q, k, v, cu_tokens, key_first, key_count, max_tokens, max_keys, scale, out, workspace)
 PyObject* attention_cross(Args a) {
   const int64_t device = current_device();
@@ -606,7 +679,8 @@ PyObject* entry(PyObject*, Args args, Py_ssize_t n) {
 PyMethodDef g_methods[] = {CALL(linear_q_gemv, 8), CALL(linear_q_gemv_multi, 6), CALL(softmax, 1), CALL(topk, 4), CALL(matmul, 5),
                            CALL(w8a8_linear_packed, 7), CALL(w4a16_gemm_packed, 6), CALL(linear_q_gemm, 7), CALL(linear_kq_gemm, 6),
                            CALL(qk_norm_rope, 11), CALL(kv_append, 15), CALL(attention_paged, 12), CALL(sample, 8),
-                           CALL(adjust_logits, 12), CALL(attention_cross, 11), {nullptr, nullptr, 0, nullptr}};
+                           CALL(adjust_logits, 12), CALL(attention_cross, 11), CALL(attention_weights, 11),
+                           CALL(kv_evict, 10), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "mllm_calls", nullptr, -1, g_methods};
 
 }  // namespace

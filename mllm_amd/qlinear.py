@@ -693,6 +693,21 @@ def attention_paged(q, k_cache, v_cache, block_table, cu_tokens, prefix, max_tok
     return _calls().attention_paged(q, k_cache, v_cache, block_table, cu_tokens, prefix, max_tokens, max_keys, tree, scale, out, workspace)
 
 
+def attention_weights(q, k_cache, mass, block_table, cu_tokens, prefix, max_tokens, max_keys, decay=1.0, scale=None, workspace=None):
+    """Adds to mass fp32 [B, Hkv, n] (rows in one piece) what every cached key gets of the new tokens' attention: the sum over tokens that see it and query heads of its
+    group of softmax(scale * q k^T), tokens, sequences and positions as in attention_paged without a tree.  Prefix positions: decay * mass + that; the new tokens' own: that alone, whatever was
+    there.  Tokens behind max_tokens add nothing, positions from max_keys on are neither seen nor get anything, from n on get it nowhere.  Returns mass."""
+    return _calls().attention_weights(q, k_cache, mass, block_table, cu_tokens, prefix, max_tokens, max_keys, decay, scale, workspace)
+
+
+def kv_evict(k_cache, v_cache, mass, block_table, lengths, to_table, keep, first=0, recent=0, out=None):
+    """Copies the `keep` keys and values of every sequence and key head that are worth it to places 0, 1, .. of the pages in to_table (int32 [B, m]), in their order: of the first
+    lengths[b] (int32 [B]) positions the first `first`, the last `recent`, and those of the largest mass (fp32 [B, Hkv, n]; equal: lowest position first; NaN: the
+    smallest).  Returns (their positions int32 [B, Hkv, keep], -1 behind the last where there are fewer; their mass, 0 there), anew or in out; a sequence has min(lengths[b], keep)
+    positions then.  The pages read stay as they are (other sequences may share them); none of them may be in to_table, and none twice."""
+    return _calls().kv_evict(k_cache, v_cache, mass, block_table, lengths, to_table, keep, first, recent, out)
+
+
 def attention_cross(q, k, v, cu_tokens, key_first, key_count, max_tokens, max_keys, scale=None, out=None, workspace=None):
     """softmax(scale * q k^T) v over an encoder's states: q [T, Hq, D] fp32 or bf16, k and v bf16 [S, Hkv, D] (D of whole eights up to 256; any strides of whole 16 bytes); rows
     cu_tokens[b] .. cu_tokens[b + 1] - 1 (int32 [B + 1]) of q see key_count[b] keys from key_first[b] on (int32 [B]), all of them, whatever their order.  An encoder's

@@ -46,6 +46,11 @@ def adjust(x, said=(), prompt=0, repetition=1.0, presence=0.0, frequency=0.0, bi
     return x, size
 
 
+def finite(x):
+    """sizes of terms that are rounded: a score with an infinite one is infinite or no number, exactly"""
+    return torch.where(torch.isfinite(x), x.abs(), 0.0)
+
+
 def cross(q, k, v, cu, first, count, scale):
     """q [T, Hq, D]; k, v [S, Hkv, D] -> float64 [T, Hq, D] (rows in no sequence NaN) and, for error bounds, the same with |v| for v and the largest sum of a
     score's absolute terms [T, Hq, 1]"""
@@ -64,5 +69,40 @@ def cross(q, k, v, cu, first, count, scale):
             p = torch.softmax(qh @ kh.t() * scale, -1)
             out[rows, h], size[rows, h] = p @ vh, p @ vh.abs()
             if len(qh):
-                terms[rows, h] = (qh.abs() @ kh.abs().t()).amax(-1, keepdim=True) * scale
+                terms[rows, h] = (finite(qh) @ finite(kh).t()).amax(-1, keepdim=True) * scale
     return out, size, terms
+
+
+def weights(q, k_cache, table, cu, prefix, scale, max_tokens=None, max_keys=None):
+    """per sequence: what its positions get, float64 [Hkv, positions], and, for error bounds, the largest sum of a score's absolute terms.  Positions of pages outside the cache count as zeros."""
+    q = q.detach().cpu().double()
+    pages, page, kv, D = k_cache.shape
+    group, out = q.shape[1] // kv, []
+    for b in range(len(cu) - 1):
+        lo, n = int(cu[b]), int(cu[b + 1] - cu[b])
+        length = min(int(prefix[b]) + n, table.shape[1] * page, max_keys if max_keys is not None else 1 << 62)
+        at = torch.arange(length)
+        ids = table[b].cpu().long()[at // page] if length else at
+        good = (ids >= 0) & (ids < pages)
+        k = k_cache.detach()[torch.where(good, ids, 0).to(k_cache.device), (at % page).to(k_cache.device)].cpu().double()
+        k = torch.where(good[:, None, None], k, 0.0)
+        got, most = torch.zeros((kv, length), dtype=torch.float64), 0.0
+        for t in range(min(n, max_tokens if max_tokens is not None else n)):
+            m = min(int(prefix[b]) + t + 1, length)
+            for h in range(q.shape[1]):
+                s = k[:m, h // group] @ q[lo + t, h] * scale
+                if m == 0 or (s == -np.inf).all():
+                    continue
+                got[h // group, :m] += torch.softmax(s, 0)
+                most = max(most, float((finite(k[:m, h // group]) @ finite(q[lo + t, h])).max() * scale))
+        out.append((got, most))
+    return out
+
+
+def evict(mass, length, keep, first, recent):
+    """one head's masses (numpy fp32): the positions that stay, in order"""
+    n = len(mass[:max(0, length)])
+    if n <= keep:
+        return np.arange(n)
+    order = sorted(range(first, n - recent), key=lambda i: (0 if np.isnan(mass[i]) else -1, 0.0 if np.isnan(mass[i]) else -float(mass[i]), i))
+    return np.array(sorted(list(range(first)) + list(range(n - recent, n)) + order[:keep - first - recent]), dtype=np.int64)

@@ -91,3 +91,45 @@ def test_attention_cross_workspace():
     assert size(BF16, 1, 1, 32, 8, 128, 1, 100) == 0 and size(BF16, 1, 1, 32, 8, 128, 1, 5000) > 0
     assert size(BF16, 3, 2, 32, 8, 128, 4096, 5000) == size(BF16, 3, 2, 32, 8, 128, 3, 5000) > 0
     assert size(2, 1, 1, 32, 8, 128, 1, 5000) == 0 and size(BF16, 1, 1, 30, 8, 128, 1, 5000) == 0 and size(BF16, 0, 1, 32, 8, 128, 1, 5000) == 0 and size(BF16, 1, 1, 32, 8, 100, 1, 5000) == 0
+
+
+def _weights(q=None, cache=None, dtype=BF16, T=2, mass=P, stride=2000, head=500, n=500, table=P, table_len=4, cu=P, prefix=P, B=1, tokens=2, keys=40, decay=1.0, scale=0.1, work=P, size=1 << 30,
+             no_q=False, no_cache=False):
+    q, cache = q if q is not None else _part(heads=8, y=None), cache if cache is not None else _cache(v=None)
+    return _lib.lib().mllm_hip_attention_weights(None if no_q else C.byref(q), dtype, T, None if no_cache else C.byref(cache), mass, stride, head, n, table, 4, table_len, cu, prefix, B, tokens, keys,
+                                                 decay, scale, work, size, None)
+
+
+@pytest.mark.parametrize("args,want", [
+    (dict(no_q=True), BADARG), (dict(no_cache=True), BADARG), (dict(dtype=2), BADARG), (dict(T=-1), BADARG), (dict(B=-1), BADARG), (dict(tokens=-1), BADARG), (dict(keys=-1), BADARG),
+    (dict(keys=(1 << 30) + 1), SHAPE), (dict(mass=None), BADARG), (dict(n=-1), BADARG), (dict(table=None), BADARG), (dict(table_len=0), BADARG), (dict(table_len=-1), BADARG),
+    (dict(table_len=1 << 27), SHAPE), (dict(cu=None), BADARG), (dict(prefix=None), BADARG), (dict(scale=0.0), BADARG), (dict(scale=3e38), BADARG), (dict(decay=-1.0), BADARG),
+    (dict(decay=float("inf")), BADARG), (dict(decay=float("nan")), BADARG), (dict(T=1 << 29), SHAPE), (dict(B=1 << 14), SHAPE), (dict(B=2, stride=0), BADARG), (dict(head=0), BADARG),
+    (dict(q=_part(heads=6)), SHAPE), (dict(q=_part(heads=8, x=None)), BADARG), (dict(q=_part(heads=8, x=ODD)), ALIGN), (dict(q=_part(heads=8, x_token_stride=516)), ALIGN),
+    (dict(cache=_cache(head_dim=100)), SHAPE), (dict(cache=_cache(head_dim=264)), SHAPE), (dict(cache=_cache(k=None)), BADARG), (dict(cache=_cache(k=ODD)), ALIGN), (dict(cache=_cache(slot_stride=4)), ALIGN),
+    (dict(cache=_cache(pages=0)), BADARG), (dict(cache=_cache(pages=1 << 27)), SHAPE), (dict(mass=ODD), ALIGN), (dict(table=ODD), ALIGN), (dict(cu=ODD), ALIGN), (dict(prefix=ODD), ALIGN),
+    (dict(work=P + 8), ALIGN), (dict(work=None), BADARG), (dict(size=100), BADARG), (dict(T=0), 0), (dict(B=0), 0), (dict(tokens=0), 0), (dict(keys=0), 0)])
+def test_attention_weights(args, want):
+    assert _weights(**args) == want
+
+
+def _evict(cache=None, mass=P, stride=2000, head=500, n=500, table=P, table_len=8, lengths=P, B=1, to=P, to_len=4, keep=40, first=4, recent=8, kept=P, kept_mass=P + 4096, no_cache=False):
+    cache = cache if cache is not None else _cache()
+    return _lib.lib().mllm_hip_kv_evict(None if no_cache else C.byref(cache), mass, stride, head, n, table, 8, table_len, lengths, B, to, 4, to_len, keep, first, recent, kept, kept_mass, None)
+
+
+@pytest.mark.parametrize("args,want", [
+    (dict(no_cache=True), BADARG), (dict(cache=_cache(k=None)), BADARG), (dict(cache=_cache(v=None)), BADARG), (dict(cache=_cache(v=ODD)), ALIGN), (dict(cache=_cache(head_dim=100)), SHAPE),
+    (dict(cache=_cache(head_dim=520)), SHAPE), (dict(cache=_cache(heads=0)), BADARG), (dict(cache=_cache(page_stride=100)), ALIGN), (dict(cache=_cache(pages=1 << 27)), SHAPE), (dict(mass=None), BADARG),
+    (dict(mass=ODD), ALIGN), (dict(n=-1), BADARG), (dict(table=None), BADARG), (dict(table=ODD), ALIGN), (dict(table_len=-1), BADARG), (dict(lengths=None), BADARG), (dict(lengths=ODD), ALIGN),
+    (dict(B=-1), BADARG), (dict(B=1 << 14), SHAPE), (dict(to=None), BADARG), (dict(to=ODD), ALIGN), (dict(to_len=-1), BADARG), (dict(to_len=2), SHAPE), (dict(keep=65), SHAPE), (dict(keep=-1), BADARG),
+    (dict(keep=11), BADARG), (dict(first=-1), BADARG), (dict(first=41), BADARG), (dict(recent=-1), BADARG), (dict(recent=1 << 62), BADARG), (dict(kept=None), BADARG), (dict(kept=ODD), ALIGN),
+    (dict(kept_mass=None), BADARG), (dict(kept_mass=ODD), ALIGN), (dict(kept_mass=P), BADARG), (dict(B=0), 0), (dict(keep=0, first=0, recent=0), 0)])
+def test_kv_evict(args, want):
+    assert _evict(**args) == want
+
+
+def test_attention_weights_workspace():
+    size = _lib.lib().mllm_hip_attention_weights_workspace_bytes
+    assert size(BF16, 1, 1, 32, 8, 128, 1, 5000) >= 32 * 5000 * 4
+    assert size(F32, 640, 20, 32, 8, 128, 32, 5000) >= 640 * 32 * 8 and size(2, 1, 1, 32, 8, 128, 1, 100) == 0 and size(BF16, 0, 1, 32, 8, 128, 1, 100) == 0 and size(BF16, 1, 1, 30, 8, 128, 1, 100) == 0
