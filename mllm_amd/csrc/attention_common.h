@@ -36,17 +36,14 @@ __device__ __forceinline__ uint32_t finite_pair(uint32_t v) {
   return ((v & 0x7f80u) == 0x7f80u ? 0u : v & 0xffffu) | ((v & 0x7f800000u) == 0x7f800000u ? 0u : v & 0xffff0000u);
 }
 
-// Elements at .. at + 7 of a query as an operand: bf16 as they are, fp32 as three parts of 8 bits each (what is infinite or no number: all in the first).  Zeros where not `live`.
+// Eight elements of a query as an operand: bf16 as they are, fp32 as three parts of 8 bits each (what is infinite or no number: all in the first)
 template <bool F32>
-__device__ __forceinline__ void query_parts(const void* q, int64_t at, bool live, at_bf16x8 (&part)[F32 ? 3 : 1]) {
-  constexpr int XT = F32 ? MLLM_HIP_F32 : MLLM_HIP_BF16;
-  Item8<XT> it = {};
-  if (live) item_load<XT>(q, at, it);
+__device__ __forceinline__ void item_parts(const Item8<F32 ? MLLM_HIP_F32 : MLLM_HIP_BF16>& it, at_bf16x8 (&part)[F32 ? 3 : 1]) {
   if constexpr (!F32) {
     part[0] = frag(it.r[0]);
   } else {
     float v[8];
-    item_to_f32<XT>(it, v);
+    item_to_f32<MLLM_HIP_F32>(it, v);
     uint32_t w[3][4];
 #pragma unroll
     for (int j = 0; j < 4; j++) {
@@ -57,6 +54,13 @@ __device__ __forceinline__ void query_parts(const void* q, int64_t at, bool live
 #pragma unroll
     for (int p = 0; p < 3; p++) part[p] = frag(u32x4{w[p][0], w[p][1], w[p][2], w[p][3]});
   }
+}
+// elements at .. at + 7, zeros where not `live`
+template <bool F32>
+__device__ __forceinline__ void query_parts(const void* q, int64_t at, bool live, at_bf16x8 (&part)[F32 ? 3 : 1]) {
+  Item8<F32 ? MLLM_HIP_F32 : MLLM_HIP_BF16> it = {};
+  if (live) item_load<F32 ? MLLM_HIP_F32 : MLLM_HIP_BF16>(q, at, it);
+  item_parts<F32>(it, part);
 }
 
 }  // namespace mllmhip

@@ -48,6 +48,25 @@ __device__ __forceinline__ CrossSeq cross_sequence(const CrossArgs& a, int b) {
   return s;
 }
 
+// Elements d .. d + 3 of a row's result: O, its maximum and sum go to the workspace where keys are cut
+template <bool F32>
+__device__ __forceinline__ void cross_put(const CrossArgs& a, const CrossSeq& s, int piece, int t, int head, int d, at_f32x4 x, float m, float sum) {
+  if (d >= a.D) return;
+  if (s.pieces > 1) {
+    const int64_t at = ((int64_t)piece * a.T + t) * (a.kv * a.group) + head;
+    *reinterpret_cast<at_f32x4*>(a.part_o + at * a.D + d) = x;
+    if (d == 0) {
+      a.part_ml[2 * at] = m;
+      a.part_ml[2 * at + 1] = sum;
+    }
+    return;
+  }
+  x *= sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);  // (no key: zeros; a NaN stays)
+  const int64_t at = t * a.o_token + head * a.o_head + d;
+  if (F32) *reinterpret_cast<at_f32x4*>(reinterpret_cast<float*>(a.o) + at) = x;
+  else *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(a.o) + at) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+}
+
 template <int DP, int DT, int NQ, int WR, bool F32>
 struct Cross {
   static constexpr int WK = 4 / WR;          // waves along keys
@@ -282,24 +301,8 @@ __global__ __launch_bounds__(256, (Cross<DP, DT, NQ, WR, F32>::WAVES)) void cros
 #pragma unroll
   for (int i = 0; i < NQ; i++) l[i] = sum32(sum16(l[i]));
 
-  const int heads = a.kv * a.group;
-  // a row's elements d .. d + 3
   auto put = [&](int row, int d, at_f32x4 x, float mm, float sum) {
-    if (d >= a.D) return;
-    const int t = s.first + row / a.group, head = h * a.group + row % a.group;
-    if (s.pieces > 1) {
-      const int64_t at = ((int64_t)piece * a.T + t) * heads + head;
-      *reinterpret_cast<at_f32x4*>(a.part_o + at * a.D + d) = x;
-      if (d == 0) {
-        a.part_ml[2 * at] = mm;
-        a.part_ml[2 * at + 1] = sum;
-      }
-      return;
-    }
-    x *= sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);  // (no key: zeros; a NaN stays)
-    const int64_t at = t * a.o_token + head * a.o_head + d;
-    if (F32) *reinterpret_cast<at_f32x4*>(reinterpret_cast<float*>(a.o) + at) = x;
-    else *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(a.o) + at) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+    cross_put<F32>(a, s, piece, s.first + row / a.group, h * a.group + row % a.group, d, x, mm, sum);
   };
   if constexpr (WK == 1) {
 #pragma unroll
@@ -347,6 +350,177 @@ __global__ __launch_bounds__(256, (Cross<DP, DT, NQ, WR, F32>::WAVES)) void cros
       }
     }
   }
+}
+
+// Many rows of bf16 queries: a wave has 32 of them, v_mfma_f32_32x32x16_bf16, DK steps of 16 elements in the first product and DT tiles of 32 in the second.  First operand rows
+// 8 a + 4 b + c = keys 16 (a / 2) + 8 b + 4 (a % 2) + c leave a lane with one row of Q and, of every 16 keys, the eight consecutive ones that the second product takes.
+// Keys and values go from memory to LDS directly, keys a tile ahead: the scores of the next tile are matrix instructions between the exponents of this one.
+template <int DK, int DT>
+struct Wide {
+  static constexpr int C = 2 * DK, DP = 16 * DK, KT = 64;
+  static constexpr int CHUNKS = KT * C / 64;  // 64 pieces each, a wave's load
+  // Eight lanes of a key operand have rows 0 - 3 and 8 - 11 (or 4 - 7 and 12 - 15) and one piece, 16 of a value operand four rows and two pieces: in different banks.
+  static __device__ __forceinline__ int swz(int row) {
+    return C == 16 ? (row & 7) << 1 | ((row >> 3) & 1) : C == 12 ? (row >> 2) & 3 : C == 10 ? (row >> 3) & 1 : ((row >> 1) & 3) << 1 | ((row >> 3) & 1);
+  }
+};
+typedef float at_f32x16 __attribute__((ext_vector_type(16)));
+__device__ __forceinline__ at_f32x16 mma32(at_bf16x8 x, at_bf16x8 y, at_f32x16 acc) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, acc, 0, 0, 0); }
+
+template <int DK, int DT>
+__global__ __launch_bounds__(256, 2) void cross_wide_kernel(CrossArgs a) {
+  typedef Wide<DK, DT> P;
+  constexpr int KT = P::KT, C = P::C, DP = P::DP, CHUNKS = P::CHUNKS;
+  __shared__ __align__(16) uint16_t s_k0[KT * DP], s_k1[KT * DP], s_v0[KT * DP + 16], s_v1[KT * DP + 16];  // (tiles of 32 of the last value end behind it)
+  const int idx = blockIdx.x >> 3, rt = idx % a.row_tiles, place = (idx / a.row_tiles) * 8 + (blockIdx.x & 7);
+  const int h = place % a.kv, piece = place / a.kv % a.pieces, b = place / a.kv / a.pieces;
+  if (b >= a.B) return;
+  const CrossSeq s = cross_sequence(a, b);
+  const int rows = s.n * a.group, row0 = rt * 128;
+  if (row0 >= rows || piece >= s.pieces) return;
+  const int k_begin = piece * s.per * KT, k_end = min(k_begin + s.per * KT, s.keys);
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, g = lane >> 5;
+
+  // Chunk i of a wave's: 64 pieces one behind the other in LDS; a lane's is piece at[i] ^ swz of its row
+  constexpr int NLOAD = (CHUNKS + 3) / 4;
+  const int real = a.D / 8;
+  uint32_t koff[NLOAD], voff[NLOAD];
+  int row_of[NLOAD];  // KT: zeros
+#pragma unroll
+  for (int i = 0; i < NLOAD; i++) {
+    const int e = (i * 4 + wave) * 64 + lane, r = e / C, p = (e % C) ^ P::swz(r);
+    row_of[i] = p < real ? r : 1 << 30;
+    koff[i] = r * a.k_bytes + p * 16;
+    voff[i] = r * a.v_bytes + p * 16;
+  }
+  typedef const __attribute__((address_space(1))) void* global_ptr;
+  typedef __attribute__((address_space(3))) void* lds_ptr;
+  const uint64_t zero = (uint64_t)(uintptr_t)g_no_state;
+  const uint64_t k_at = (uint64_t)(uintptr_t)(a.k + h * a.k_head) + s.key * a.k_bytes, v_at = (uint64_t)(uintptr_t)(a.v + h * a.v_head) + s.key * a.v_bytes;
+  auto ask = [&](uint64_t at, uint32_t bytes, const uint32_t (&off)[NLOAD], int k0, uint16_t* to) {
+    if (k0 >= k_end) return;
+#pragma unroll
+    for (int i = 0; i < NLOAD; i++) {
+      if (CHUNKS % 4 && i * 4 + wave >= CHUNKS) break;
+      const uint64_t from = k0 + row_of[i] < k_end ? at + (uint64_t)k0 * bytes + off[i] : zero;
+      __builtin_amdgcn_global_load_lds(reinterpret_cast<global_ptr>(from), (lds_ptr)(to + (i * 4 + wave) * 512), 16, 0, 0);
+    }
+  };
+  // Q: second operand, row `col`, elements 16 s + 8 g .. + 7
+  at_bf16x8 fq[DK];
+  const int row = row0 + wave * 32 + col;
+  const bool live = row < rows;
+  const int token = live ? row / a.group : 0, head = h * a.group + (live ? row - token * a.group : 0);
+  {
+    at_bf16x8 part[1];
+#pragma unroll
+    for (int ks = 0; ks < DK; ks++) {
+      query_parts<false>(a.q, (s.first + token) * a.q_token + head * a.q_head + 16 * ks + 8 * g, live && 16 * ks + 8 * g < a.D, part);
+      fq[ks] = part[0];
+    }
+  }
+  at_f32x16 acc[DT] = {};
+  float m = -INFINITY, l = 0.f;  // the maximum so far times c; the sum of this lane's keys
+  const int krow = (col & 3) | ((col >> 3) & 1) << 2 | ((col >> 2) & 1) << 3 | (col >> 4) << 4;
+  // scores of 32 keys
+  auto scores = [&](const uint16_t* k, int u) {
+    at_f32x16 y = {};
+    const int r = u * 32 + krow, x = P::swz(r);
+#pragma unroll
+    for (int ks = 0; ks < DK; ks++) y = mma32(frag(*reinterpret_cast<const u32x4*>(k + r * DP + ((2 * ks + g) ^ x) * 8)), fq[ks], y);
+    return y;
+  };
+  auto arrived = [&]() {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+  };
+  at_f32x16 y[2];
+  ask(k_at, a.k_bytes, koff, k_begin, s_k0);
+  arrived();
+  ask(k_at, a.k_bytes, koff, k_begin + KT, s_k1);
+  ask(v_at, a.v_bytes, voff, k_begin, s_v0);
+  if (k_begin < k_end) y[0] = scores(s_k0, 0), y[1] = scores(s_k0, 1);
+  // one tile: its scores are there; keys of the next are in `k`, of the one behind that go where this tile's were
+  auto turn = [&](int k0, auto last_, const uint16_t* k, uint16_t* k_next, const uint16_t* v, uint16_t* v_next) {
+    constexpr bool last = decltype(last_)::value;
+    arrived();
+    if (!last) {
+      ask(k_at, a.k_bytes, koff, k0 + 2 * KT, k_next);
+      ask(v_at, a.v_bytes, voff, k0 + KT, v_next);
+    }
+    if (last) {
+      const int left = k_end - k0 - 8 * g;
+#pragma unroll
+      for (int u = 0; u < 2; u++)
+#pragma unroll
+        for (int j = 0; j < 16; j++) y[u][j] = 32 * u + 16 * (j >> 3) + (j & 7) < left ? y[u][j] : -INFINITY;
+    }
+    float top = larger(y[0][0], y[1][0]);
+#pragma unroll
+    for (int j = 1; j < 16; j++) top = larger(top, larger(y[0][j], y[1][j]));
+    top = across<32>(top) * a.c;
+    if (__ballot(top > m + 8.f)) {  // (weights of up to 2^8 do as well: most tiles leave O alone)
+      const float next = fmaxf(m, top), fix = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - next);
+      m = next;
+      l *= fix;
+#pragma unroll
+      for (int d = 0; d < DT; d++) acc[d] *= fix;
+    }
+    const float ref = m == -INFINITY ? 0.f : m;  // (nothing seen yet: every p is exp2(-inf))
+    at_bf16x8 fp[4];
+    at_f32x16 z[2];
+#pragma unroll
+    for (int u = 0; u < 2; u++) {
+      if (!last) z[u] = scores(k, u);
+      float sum[2];
+#pragma unroll
+      for (int hf = 0; hf < 2; hf++) {
+        float e[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) e[j] = __builtin_amdgcn_exp2f(fmaf(y[u][8 * hf + j], a.c, -ref));
+        sum[hf] = ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
+        fp[2 * u + hf] = frag(u32x4{pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7])});
+      }
+      l += sum[0] + sum[1];
+    }
+    // V^T: lane i of 16 asks for elements 4 (i % 4) .. + 3 of key 8 g + i / 4 and gets element i of keys 8 g .. + 3
+    const int i = lane & 15, half = (lane >> 4) & 1;
+#pragma unroll
+    for (int kk = 0; kk < 4; kk++) {
+      const int r = 16 * kk + 8 * g + (i >> 2), x = P::swz(r), x4 = P::swz(r + 4);
+#pragma unroll
+      for (int d = 0; d < DT; d++) {
+        const int p = 4 * d + 2 * half + ((i & 3) >> 1);
+        typedef __attribute__((address_space(3))) at_s16x4* lds_quad;
+        const at_s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_quad)(v + r * DP + (p ^ x) * 8 + (i & 1) * 4));
+        const at_s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_quad)(v + (r + 4) * DP + (p ^ x4) * 8 + (i & 1) * 4));
+        acc[d] = mma32(frag(__builtin_bit_cast(u32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7))), fp[kk], acc[d]);
+      }
+    }
+    if (!last) y[0] = z[0], y[1] = z[1];
+  };
+  int k0 = k_begin;
+  bool odd = false;
+  while (k0 + KT < k_end) {
+    turn(k0, std::false_type(), s_k1, s_k0, s_v0, s_v1);
+    k0 += KT;
+    odd = true;
+    if (k0 + KT >= k_end) break;
+    turn(k0, std::false_type(), s_k0, s_k1, s_v1, s_v0);
+    k0 += KT;
+    odd = false;
+  }
+  if (k0 < k_end) {
+    if (odd) turn(k0, std::true_type(), s_k0, s_k1, s_v1, s_v0);
+    else turn(k0, std::true_type(), s_k1, s_k0, s_v0, s_v1);
+  }
+  l = sum32(l);
+  if (!live) return;
+#pragma unroll
+  for (int d = 0; d < DT; d++)
+#pragma unroll
+    for (int j = 0; j < 4; j++)
+      cross_put<false>(a, s, piece, s.first + token, head, 32 * d + 8 * j + 4 * g, at_f32x4{acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]}, m, l);
 }
 
 // Joins the pieces of a row: 16 bytes of it per lane, L lanes a row
@@ -485,20 +659,20 @@ MLLM_API int mllm_hip_attention_cross(const mllm_hip_heads* q, int dtype, int64_
   const dim3 grid((unsigned)(groups * p.row_tiles));
   const int form = p.nq * 10 + p.wr;
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a); };
-#define CROSS(DP_, DT_)                                                      \
+#define CROSS(DP_, DT_, DK_)                                                   \
   if (f32) {                                                                 \
     if (form == 12) go(cross_kernel<DP_, DT_, 1, 2, true>);                  \
     else go(cross_kernel<DP_, DT_, 1, 4, true>);                             \
   } else {                                                                   \
     if (form == 12) go(cross_kernel<DP_, DT_, 1, 2, false>);                 \
     else if (form == 14) go(cross_kernel<DP_, DT_, 1, 4, false>);            \
-    else go(cross_kernel<DP_, DT_, DP_ == 256 ? 1 : 2, 4, false>);           \
+    else if constexpr (DP_ < 256) go(cross_wide_kernel<DK_, (DK_ + 1) / 2>); \
   }
-  if (D <= 64) { CROSS(64, 4) }
-  else if (D <= 80) { CROSS(96, 5) }
-  else if (D <= 96) { CROSS(96, 6) }
-  else if (D <= 128) { CROSS(128, 8) }
-  else { CROSS(256, 16) }
+  if (D <= 64) { CROSS(64, 4, 4) }
+  else if (D <= 80) { CROSS(96, 5, 5) }
+  else if (D <= 96) { CROSS(96, 6, 6) }
+  else if (D <= 128) { CROSS(128, 8, 8) }
+  else { CROSS(256, 16, 16) }
 #undef CROSS
   RC_RET((int)hipGetLastError());
   if (p.pieces > 1) {

@@ -12,6 +12,8 @@
 //   More rows: the first finds maxima and sums, a wave's rows in registers and keys going by (a small launch joins them where keys are cut into ranges); the second has a wave's
 //   keys in registers and rows going by, so that what a key gets is a sum in a lane.
 // No atomics: what a key gets is summed by one wave in one order.
+#include <type_traits>
+
 #include "attention_common.h"
 
 namespace mllmhip {
@@ -36,6 +38,8 @@ struct WeightArgs {
   int rows, pitch;
   f32x2* ml;     // few rows: [range][B][kv][rows]; more: [range][T][heads], maximum (times c) and sum
   f32x2* row;    // [T][heads]: maximum (times c) and 1 / sum of all keys
+  float* part;   // [split][B][kv][pitch]: what keys get of a part of the rows
+  int splits;
 };
 __device__ u32x4 g_no_key[32];  // what a page outside the cache reads as (never written)
 
@@ -64,6 +68,18 @@ __device__ __forceinline__ void load_key(const WeightArgs& a, const int32_t* tab
     const int e = 32 * ks + 8 * g;
     r[ks] = *reinterpret_cast<const __attribute__((address_space(1))) u32x4*>(e < a.D ? at + e * 2 : (uint64_t)(uintptr_t)g_no_key);
   }
+}
+
+// Rows of C 16-byte pieces lie in LDS with their pieces exclusive-ored by bits of the row's number, so that 16 rows' pieces of one number are in different banks.
+template <int C>
+__device__ __forceinline__ int swizzle(int row) {
+  return C == 8 ? (row >> 1) & 7 : C == 12 ? (row >> 2) & 3 : row & 15;
+}
+// what a key gets
+__device__ __forceinline__ void put_mass(const WeightArgs& a, const WeightSeq& s, int b, int h, int key, float v) {
+  if (key >= a.mass_len) return;
+  float* mass = a.mass + b * a.mass_seq + h * a.mass_head + key;
+  *mass = key < s.prefix && a.decay != 0.f ? a.decay * *mass + v : v;
 }
 
 // Scores (times 1) of 16 keys and 16 rows.  With fp32 queries an infinite element of a key makes a NaN with the second and third part of a query's, which may be 0: it
@@ -171,62 +187,160 @@ __global__ __launch_bounds__(256) void weights_sum_kernel(WeightArgs a) {
   }
   __syncthreads();
   const int key = blockIdx.x * 256 + threadIdx.x;
-  if (key >= s.keys || key >= a.mass_len) return;
+  if (key >= s.keys) return;
   const float* score = a.score + (int64_t)blockIdx.y * a.rows * a.pitch + key;
   float sum = 0.f;
   for (int r = 0; r < a.rows; r++) {
     const float p = __builtin_amdgcn_exp2f(fmaf(score[(int64_t)r * a.pitch], a.c, -s_row[r].x)) * s_row[r].y;
     sum += key <= s.prefix + r / a.group ? p : 0.f;  // (a row without a number has none for keys that it sees)
   }
-  float* mass = a.mass + b * a.mass_seq + h * a.mass_head + key;
-  *mass = key < s.prefix && a.decay != 0.f ? a.decay * *mass + sum : sum;
+  put_mass(a, s, b, h, key, sum);
 }
 
 // ---- more rows ------------------------------------------------------------------------------------------------------------
-enum { WEIGHT_NQ = 2, WEIGHT_ROWS = 4 * WEIGHT_NQ * 16, WEIGHT_NK = 2, WEIGHT_KEYS = 4 * WEIGHT_NK * 16 };
+// Maxima and sums: four waves, WR along rows times 4 / WR along keys, 64 keys in LDS at a time, the next ones on their way.
+enum { WEIGHT_TILE = 64 };
+// rows of a wave, in sixteens (fp32 queries of 256 elements take 96 registers for sixteen)
+static constexpr int weight_nq(int ks, bool f32) { return ks == 8 && f32 ? 1 : 2; }
 
-template <int KS, bool F32>
-__global__ __launch_bounds__(256) void weights_max_kernel(WeightArgs a) {
-  constexpr int NQ = WEIGHT_NQ;
-  const int h = blockIdx.y % a.kv, b = blockIdx.y / a.kv, range = blockIdx.x % a.ranges, rt = blockIdx.x / a.ranges;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+template <int KS, int WR, bool F32>
+__global__ __launch_bounds__(256, 2) void weights_max_kernel(WeightArgs a) {
+  constexpr int NQ = weight_nq(KS, F32), DP = KS * 32, C = DP / 8, KT = WEIGHT_TILE, NLOAD = KT * C / 256, WK = 4 / WR, NB = KT / 16 / WK, PARTS = F32 ? 3 : 1;
+  __shared__ __align__(16) uint16_t s_k[2 * KT * DP];
+  __shared__ f32x2 s_ml[4][NQ * 16];
+  // Workgroup i runs on XCD i % 8: the row tiles of a range of keys follow one another on one XCD, whose L2 they share.
+  const int idx = blockIdx.x >> 3, rt = idx % a.row_tiles, place = (idx / a.row_tiles) * 8 + (blockIdx.x & 7);
+  const int h = place % a.kv, range = place / a.kv % a.ranges, b = place / a.kv / a.ranges;
+  if (b >= a.B) return;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave % WR, wk = wave / WR, col = lane & 15, g = lane >> 4;
   const WeightSeq s = weight_sequence(a, b);
-  const int rows = s.n * a.group, row0 = rt * WEIGHT_ROWS + wave * NQ * 16;
+  const int rows = s.n * a.group, row0 = rt * (WR * NQ * 16);
   if (row0 >= rows) return;
-  // (keys behind this wave's last token are seen by none of its rows)
-  const int last = (min(rows, row0 + NQ * 16) - 1) / a.group;
-  const int per = ((s.keys + a.ranges - 1) / a.ranges + 15) / 16 * 16, begin = range * per, end = min(min(begin + per, s.keys), s.prefix + last + 1);
+  const int first = row0 / a.group, last = (min(rows, row0 + WR * NQ * 16) - 1) / a.group;
+  const int per = ((s.keys + a.ranges - 1) / a.ranges + KT - 1) / KT * KT, begin = range * per;
+  const int end = min(min(begin + per, s.keys), s.prefix + last + 1);  // (keys behind the last token are seen by none of these rows)
+  const int plain = min(end, s.prefix + first + 1) - KT;               // the last tile that may begin there and needs no masks
   const int32_t* table = a.table + b * a.table_stride;
+  const int real = a.D / 8;
+  int row_of[NLOAD], to[NLOAD], ids[NLOAD];
+  bool has[NLOAD];
   const uint64_t k_at = (uint64_t)(uintptr_t)(a.k + h * a.head_stride);
-  at_bf16x8 q[NQ][KS][F32 ? 3 : 1];
+#pragma unroll
+  for (int i = 0; i < NLOAD; i++) {
+    const int e = i * 256 + tid, r = e / C, p = e % C;
+    row_of[i] = r;
+    has[i] = p < real;
+    to[i] = r * DP + (p ^ swizzle<C>(r)) * 8;
+    if (!has[i]) *reinterpret_cast<u32x4*>(s_k + to[i]) = *reinterpret_cast<u32x4*>(s_k + KT * DP + to[i]) = u32x4{0, 0, 0, 0};
+  }
+  auto page_of = [&](int key) { return __umulhi(2 * (uint32_t)key, a.page_mul) >> a.page_shift; };
+  auto ask_ids = [&](int k0) {
+#pragma unroll
+    for (int i = 0; i < NLOAD; i++) {
+      const int key = k0 + row_of[i];
+      ids[i] = key < end && has[i] ? table[page_of(key)] : -1;
+    }
+  };
+  u32x4 rk[NLOAD];
+  auto ask_tile = [&](int k0) {
+#pragma unroll
+    for (int i = 0; i < NLOAD; i++) {
+      const uint32_t key = (uint32_t)(k0 + row_of[i]), id = (uint32_t)ids[i];
+      const uint64_t at = k_at + (uint64_t)id * a.page_bytes + ((key - page_of((int)key) * a.page) * a.slot_bytes + (i * 256 + tid) % C * 16);
+      rk[i] = *reinterpret_cast<const __attribute__((address_space(1))) u32x4*>(id < a.pages ? at : (uint64_t)(uintptr_t)g_no_key);
+    }
+    ask_ids(k0 + KT);
+  };
+  auto put_tile = [&](int half) {
+#pragma unroll
+    for (int i = 0; i < NLOAD; i++)
+      if (has[i]) *reinterpret_cast<u32x4*>(s_k + half * (KT * DP) + to[i]) = rk[i];
+  };
+  at_bf16x8 q[NQ][KS][PARTS];
   int token[NQ];
   float m[NQ], l[NQ];
+  if (begin < end) {
+    ask_ids(begin);
+    ask_tile(begin);
+  }
 #pragma unroll
   for (int i = 0; i < NQ; i++) {
-    const int r = row0 + i * 16 + col;
+    const int r = row0 + (wr * NQ + i) * 16 + col;
     load_rows<KS, F32>(a, s, h, r, rows, g, q[i]);
     token[i] = r < rows ? r / a.group : -1;
     m[i] = -INFINITY;
     l[i] = 0.f;
   }
-  for (int k0 = begin; k0 < end; k0 += 16) {
-    u32x4 k[KS];
-    load_key<KS>(a, table, k_at, k0 + col, k0 + col < end, g, k);
+  const bool busy = row0 + wr * NQ * 16 < rows;
+  auto work = [&](int k0, auto border_, int half) {
+    constexpr bool border = decltype(border_)::value;
+    at_f32x4 y[NB][NQ];
+#pragma unroll
+    for (int u = 0; u < NB; u++) {
+      const int row = half * KT + (u * WK + wk) * 16 + col, x = swizzle<C>(row);
+      u32x4 k[KS];
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) k[ks] = *reinterpret_cast<const u32x4*>(s_k + row * DP + ((4 * ks + g) ^ x) * 8);
+#pragma unroll
+      for (int i = 0; i < NQ; i++) {
+        y[u][i] = key_scores<KS, F32>(k, q[i]);
+        if (border) {
+          const int seen = min(s.prefix + token[i] + 1, end) - (k0 + (u * WK + wk) * 16 + 4 * g);
+#pragma unroll
+          for (int j = 0; j < 4; j++) y[u][i][j] = j < seen && token[i] >= 0 ? y[u][i][j] : -INFINITY;
+        }
+      }
+    }
 #pragma unroll
     for (int i = 0; i < NQ; i++) {
-      at_f32x4 y = key_scores<KS, F32>(k, q[i]);
-      const int seen = min(s.prefix + token[i] + 1, end) - (k0 + 4 * g);
+      float top = -INFINITY;
 #pragma unroll
-      for (int j = 0; j < 4; j++) y[j] = j < seen && token[i] >= 0 ? y[j] : -INFINITY;
-      take(m[i], l[i], y, a.c);
+      for (int u = 0; u < NB; u++) top = larger(top, larger(larger(y[u][i][0], y[u][i][1]), larger(y[u][i][2], y[u][i][3])));
+      const float next = larger(m[i], top * a.c), ref = next == -INFINITY ? 0.f : next;
+      float sum = 0.f;
+#pragma unroll
+      for (int u = 0; u < NB; u++)
+#pragma unroll
+        for (int j = 0; j < 4; j++) sum += __builtin_amdgcn_exp2f(fmaf(y[u][i][j], a.c, -ref));
+      l[i] = fmaf(l[i], __builtin_amdgcn_exp2f(m[i] - ref), sum);
+      m[i] = next;
+    }
+  };
+  if (begin < end) {
+    put_tile(0);
+    if (begin + KT < end) ask_tile(begin + KT);
+    __syncthreads();
+  }
+  int half = 0;
+  for (int k0 = begin; k0 < end; k0 += KT, half ^= 1) {
+    if (busy) {
+      if (k0 <= plain) work(k0, std::false_type(), half);
+      else work(k0, std::true_type(), half);
+    }
+    if (k0 + KT < end) {
+      put_tile(half ^ 1);
+      if (k0 + 2 * KT < end) ask_tile(k0 + 2 * KT);
+      __syncthreads();
     }
   }
   const int heads = a.kv * a.group;
 #pragma unroll
+  for (int i = 0; i < NQ; i++) join_lanes(m[i], l[i]);
+  if constexpr (WK > 1) {  // the waves along keys
+#pragma unroll
+    for (int i = 0; i < NQ; i++)
+      if (g == 0) s_ml[wave][i * 16 + col] = f32x2{m[i], l[i]};
+    __syncthreads();
+    if (wk) return;
+#pragma unroll
+    for (int i = 0; i < NQ; i++)
+#pragma unroll
+      for (int w = 1; w < WK; w++) join(m[i], l[i], s_ml[w * WR + wr][i * 16 + col].x, s_ml[w * WR + wr][i * 16 + col].y);
+  }
+#pragma unroll
   for (int i = 0; i < NQ; i++) {
-    join_lanes(m[i], l[i]);
     if (g || token[i] < 0) continue;
-    const int64_t at = (int64_t)(s.first + token[i]) * heads + h * a.group + (row0 + i * 16 + col - token[i] * a.group);
+    const int64_t at = (int64_t)(s.first + token[i]) * heads + h * a.group + (row0 + (wr * NQ + i) * 16 + col - token[i] * a.group);
     if (a.ranges == 1) a.row[at] = final_row(m[i], l[i]);
     else a.ml[(int64_t)range * a.T * heads + at] = f32x2{m[i], l[i]};
   }
@@ -236,18 +350,68 @@ __global__ __launch_bounds__(256) void weights_join_kernel(WeightArgs a) {
   const int64_t all = (int64_t)a.T * a.kv * a.group, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= all) return;
   float m = -INFINITY, l = 0.f;
-  for (int r = 0; r < a.ranges; r++) join(m, l, a.ml[r * all + i].x, a.ml[r * all + i].y);  // (rows of no sequence: any numbers, never used)
+  constexpr int U = 8;
+  for (int r = 0; r < a.ranges; r += U) {  // (rows of no sequence: any numbers, never used)
+    f32x2 x[U];
+#pragma unroll
+    for (int u = 0; u < U; u++) x[u] = a.ml[min(r + u, a.ranges - 1) * all + i];
+#pragma unroll
+    for (int u = 0; u < U; u++)
+      if (r + u < a.ranges) join(m, l, x[u].x, x[u].y);
+  }
   a.row[i] = final_row(m, l);
 }
 
+// The weights: a wave has NK * 16 keys in registers, rows go by in LDS, 32 at a time (16 of 256 elements), the next ones on their way.  Where keys leave CUs idle rows are cut into
+// `splits`, whose sums a last launch adds.
 template <int KS, bool F32>
-__global__ __launch_bounds__(256) void weights_mass_kernel(WeightArgs a) {
-  constexpr int NK = WEIGHT_NK;
-  const int h = blockIdx.y % a.kv, b = blockIdx.y / a.kv;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+struct Mass {
+  static constexpr int NK = KS < 8 ? 4 : F32 ? 1 : 2, RT = KS == 8 ? 16 : 32, KEYS = 4 * NK * 16;
+};
+template <int KS, bool F32>
+__global__ __launch_bounds__(256, 2) void weights_mass_kernel(WeightArgs a) {
+  typedef Mass<KS, F32> P;
+  constexpr int NK = P::NK, RT = P::RT, DP = KS * 32, C = DP / 8, PARTS = F32 ? 3 : 1, NL = (RT * C + 255) / 256, XT = F32 ? MLLM_HIP_F32 : MLLM_HIP_BF16;
+  __shared__ __align__(16) uint16_t s_q[2][PARTS][RT * DP];
+  __shared__ f32x2 s_row[2][RT];
+  const int h = blockIdx.y % a.kv, b = blockIdx.y / a.kv, split = blockIdx.z;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 15, g = lane >> 4;
   const WeightSeq s = weight_sequence(a, b);
-  const int rows = s.n * a.group, k0 = blockIdx.x * WEIGHT_KEYS + wave * NK * 16;
-  if (rows == 0 || k0 >= s.keys) return;
+  const int rows = s.n * a.group, kg = blockIdx.x * P::KEYS, k0 = kg + wave * NK * 16;
+  if (rows == 0 || kg >= s.keys) return;
+  const int per = ((rows + a.splits - 1) / a.splits + RT - 1) / RT * RT, begin = max(split * per, max(kg - s.prefix, 0) * a.group / RT * RT), end = min(split * per + per, rows);
+  const int heads = a.kv * a.group;
+  // rows r0 .. r0 + RT - 1 on their way, 8 elements a piece
+  Item8<XT> it[NL];
+  f32x2 factor;
+  auto ask_rows = [&](int r0) {
+#pragma unroll
+    for (int i = 0; i < NL; i++) {
+      const int e = i * 256 + tid, r = r0 + e / C, p = e % C;
+      it[i] = Item8<XT>{};
+      if (e < RT * C && r < end && p * 8 < a.D) {
+        const int token = r / a.group;
+        item_load<XT>(a.q, (s.first + token) * a.q_token + (h * a.group + r - token * a.group) * a.q_head + p * 8, it[i]);
+      }
+    }
+    if (tid < RT) {
+      const int r = r0 + tid, token = r / a.group;
+      factor = r < end ? a.row[(int64_t)(s.first + token) * heads + h * a.group + (r - token * a.group)] : f32x2{0.f, 0.f};
+    }
+  };
+  auto put_rows = [&](int half) {
+#pragma unroll
+    for (int i = 0; i < NL; i++) {
+      const int e = i * 256 + tid, r = e / C, p = e % C;
+      if (RT * C % 256 && e >= RT * C) break;
+      at_bf16x8 part[PARTS];
+      item_parts<F32>(it[i], part);
+#pragma unroll
+      for (int j = 0; j < PARTS; j++) *reinterpret_cast<at_bf16x8*>(&s_q[half][j][r * DP + (p ^ swizzle<C>(r)) * 8]) = part[j];
+    }
+    if (tid < RT) s_row[half][tid] = factor;
+  };
+  if (begin < end) ask_rows(begin);
   const int32_t* table = a.table + b * a.table_stride;
   const uint64_t k_at = (uint64_t)(uintptr_t)(a.k + h * a.head_stride);
   u32x4 k[NK][KS];
@@ -258,23 +422,68 @@ __global__ __launch_bounds__(256) void weights_mass_kernel(WeightArgs a) {
     load_key<KS>(a, table, k_at, key, key < s.keys, g, k[i]);
     sum[i] = at_f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  const int heads = a.kv * a.group;
-  const int from = max(k0 - s.prefix, 0) * a.group / 16 * 16;  // the first token that sees the first of these keys
-  for (int r0 = from; r0 < rows; r0 += 16) {
-    at_bf16x8 q[KS][F32 ? 3 : 1];
-    const int r = r0 + col;
-    load_rows<KS, F32>(a, s, h, r, rows, g, q);
-    const int token = r < rows ? r / a.group : -1;
-    const f32x2 row = token >= 0 ? a.row[(int64_t)(s.first + token) * heads + h * a.group + (r - token * a.group)] : f32x2{0.f, 0.f};
+  if (begin < end) put_rows(0);
+  if (begin + RT < end) ask_rows(begin + RT);
+  __syncthreads();
+  int half = 0;
+  for (int r0 = begin; r0 < end; r0 += RT, half ^= 1) {
+#pragma unroll 1
+    for (int rb = 0; rb < RT / 16; rb++) {
+      const int r = r0 + rb * 16;
+      if (r >= end) break;
+      at_f32x4 y[NK];
 #pragma unroll
-    for (int i = 0; i < NK; i++) {
-      at_f32x4 y = key_scores<KS, F32>(k[i], q);
-      const int seen = min(s.prefix + token + 1, s.keys) - (k0 + i * 16 + 4 * g);
+      for (int i = 0; i < NK; i++) y[i] = at_f32x4{0.f, 0.f, 0.f, 0.f};
+      const int x = swizzle<C>(rb * 16 + col);
+      auto query = [&](int ks, int p) { return *reinterpret_cast<const at_bf16x8*>(&s_q[half][p][(rb * 16 + col) * DP + ((4 * ks + g) ^ x) * 8]); };
 #pragma unroll
-      for (int j = 0; j < 4; j++) {
-        const float p = __builtin_amdgcn_exp2f(fmaf(y[j], a.c, -row.x)) * row.y;
-        sum[i][j] += j < seen && token >= 0 ? p : 0.f;
+      for (int ks = 0; ks < KS; ks++) {
+#pragma unroll
+        for (int p = PARTS - 1; p >= 0; p--) {  // the smallest part first
+          const at_bf16x8 q = query(ks, p);
+#pragma unroll
+          for (int i = 0; i < NK; i++) y[i] = mma(frag(k[i][ks]), q, y[i]);
+        }
       }
+      if constexpr (F32) {  // (as in key_scores)
+#pragma unroll
+        for (int i = 0; i < NK; i++) {
+          const float all = (y[i][0] + y[i][1]) + (y[i][2] + y[i][3]);
+          if (__builtin_expect(__ballot(all != all) != 0, 0)) {
+            y[i] = at_f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int ks = 0; ks < KS; ks++) {
+              const at_bf16x8 f = frag(u32x4{finite_pair(k[i][ks].x), finite_pair(k[i][ks].y), finite_pair(k[i][ks].z), finite_pair(k[i][ks].w)});
+              y[i] = mma(f, query(ks, 2), y[i]);
+              y[i] = mma(f, query(ks, 1), y[i]);
+              y[i] = mma(frag(k[i][ks]), query(ks, 0), y[i]);
+            }
+          }
+        }
+      }
+      const f32x2 row = s_row[half][rb * 16 + col];
+      if (k0 + NK * 16 <= s.prefix + r / a.group + 1) {  // the first of these rows sees all of the wave's keys, so all do
+#pragma unroll
+        for (int i = 0; i < NK; i++)
+#pragma unroll
+          for (int j = 0; j < 4; j++) sum[i][j] = fmaf(__builtin_amdgcn_exp2f(fmaf(y[i][j], a.c, -row.x)), row.y, sum[i][j]);
+      } else {
+        const int token = r + col < end ? (r + col) / a.group : -1;
+#pragma unroll
+        for (int i = 0; i < NK; i++) {
+          const int seen = token < 0 ? 0 : s.prefix + token + 1 - (k0 + i * 16 + 4 * g);
+#pragma unroll
+          for (int j = 0; j < 4; j++) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(y[i][j], a.c, -row.x)) * row.y;
+            sum[i][j] += j < seen ? p : 0.f;  // (a row without a number has none for keys that it sees)
+          }
+        }
+      }
+    }
+    if (r0 + RT < end) {
+      put_rows(half ^ 1);
+      if (r0 + 2 * RT < end) ask_rows(r0 + 2 * RT);
+      __syncthreads();
     }
   }
 #pragma unroll
@@ -283,32 +492,46 @@ __global__ __launch_bounds__(256) void weights_mass_kernel(WeightArgs a) {
     for (int j = 0; j < 4; j++) {
       const float v = group_sum<16>(sum[i][j]);
       const int key = k0 + i * 16 + 4 * g + j;
-      if (col != j || key >= s.keys || key >= a.mass_len) continue;
-      float* mass = a.mass + b * a.mass_seq + h * a.mass_head + key;
-      *mass = key < s.prefix && a.decay != 0.f ? a.decay * *mass + v : v;
+      if (col != j || key >= s.keys) continue;
+      if (a.splits > 1) a.part[((int64_t)split * gridDim.y + blockIdx.y) * a.pitch + key] = v;
+      else put_mass(a, s, b, h, key, v);
     }
   }
+}
+
+__global__ __launch_bounds__(256) void weights_add_kernel(WeightArgs a) {
+  const int h = blockIdx.y % a.kv, b = blockIdx.y / a.kv, key = blockIdx.x * 256 + threadIdx.x;
+  const WeightSeq s = weight_sequence(a, b);
+  if (s.n == 0 || key >= s.keys) return;
+  float sum = 0.f;
+  for (int i = 0; i < a.splits; i++) sum += a.part[((int64_t)i * gridDim.y + blockIdx.y) * a.pitch + key];
+  put_mass(a, s, b, h, key, sum);
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------
 struct WeightPlan {
   bool few;
-  int rows, pitch, ranges, row_tiles;
+  int rows, pitch, ranges, row_tiles, wr, splits, keys;
 };
-static WeightPlan weight_plan(int64_t B, int heads, int kv, int64_t max_tokens, int64_t max_keys) {
+static WeightPlan weight_plan(bool f32, int64_t B, int heads, int kv, int D, int64_t max_tokens, int64_t max_keys) {
   WeightPlan p = {};
   const int64_t rows = max_tokens * (heads / kv);
   p.few = rows <= 16;
   p.rows = p.few ? (int)rows : 0;
   p.pitch = (int)((max_keys + 63) / 64 * 64);
-  p.row_tiles = p.few ? 1 : (int)((rows + WEIGHT_ROWS - 1) / WEIGHT_ROWS);
+  const int64_t wave = weight_nq(D > 128 ? 8 : 4, f32) * 16;
+  p.wr = rows <= wave ? 1 : rows <= 2 * wave ? 2 : 4;
+  p.row_tiles = p.few ? 1 : (int)((rows + p.wr * wave - 1) / (p.wr * wave));
   const int64_t uncut = B * kv * p.row_tiles, most = (max_keys + 255) / 256, wanted = (1023 + uncut) / uncut;
   p.ranges = (int)(uncut >= 1024 || most < 2 ? 1 : wanted < most ? wanted : most);
+  p.keys = D <= 128 ? Mass<4, false>::KEYS : f32 ? Mass<8, true>::KEYS : Mass<8, false>::KEYS;
+  const int64_t groups = B * kv * ((max_keys + p.keys - 1) / p.keys), parts = (rows + 127) / 128, split = (511 + groups) / groups;
+  p.splits = (int)(p.few || groups >= 512 || parts < 2 ? 1 : split < parts ? split : parts);
   return p;
 }
 static size_t weight_room(const WeightPlan& p, int64_t T, int64_t B, int heads, int kv) {
   if (p.few) return ((size_t)B * kv * p.rows * p.pitch + (size_t)p.ranges * B * kv * p.rows * 2) * sizeof(float);
-  return (size_t)(p.ranges > 1 ? p.ranges + 1 : 1) * T * heads * 2 * sizeof(float);
+  return ((size_t)(p.ranges > 1 ? p.ranges + 1 : 1) * T * heads * 2 + (p.splits > 1 ? (size_t)p.splits * B * kv * p.pitch : 0)) * sizeof(float);
 }
 static bool weight_sizes(int dtype, int64_t T, int64_t B, int heads, int kv, int head_dim, int64_t max_tokens, int64_t max_keys) {
   return (dtype == MLLM_HIP_F32 || dtype == MLLM_HIP_BF16) && T >= 0 && B >= 0 && heads >= 1 && kv >= 1 && head_dim >= 1 && max_tokens >= 0 && max_keys >= 0;
@@ -326,7 +549,7 @@ MLLM_API size_t mllm_hip_attention_weights_workspace_bytes(int dtype, int64_t T,
   if (!weight_sizes(dtype, T, B, heads, kv_heads, head_dim, max_tokens, max_keys) || !weight_shape(T, B, heads, kv_heads, head_dim, max_tokens, max_keys)) return 0;
   if (T == 0 || B == 0 || max_tokens == 0 || max_keys == 0) return 0;
   if (max_tokens > T) max_tokens = T;
-  return weight_room(weight_plan(B, heads, kv_heads, max_tokens, max_keys), T, B, heads, kv_heads);
+  return weight_room(weight_plan(dtype == MLLM_HIP_F32, B, heads, kv_heads, head_dim, max_tokens, max_keys), T, B, heads, kv_heads);
 }
 
 MLLM_API int mllm_hip_attention_weights(const mllm_hip_heads* q, int dtype, int64_t T, const mllm_hip_kv_cache* cache, float* mass, int64_t mass_stride,
@@ -351,10 +574,11 @@ MLLM_API int mllm_hip_attention_weights(const mllm_hip_heads* q, int dtype, int6
     return MLLM_HIP_E_ALIGN;
   const int heads = q->heads, D = cache->head_dim;
   const bool f32 = dtype == MLLM_HIP_F32;
-  const WeightPlan p = weight_plan(B, heads, cache->heads, max_tokens, max_keys);
+  const WeightPlan p = weight_plan(f32, B, heads, cache->heads, D, max_tokens, max_keys);
   const size_t need = weight_room(p, T, B, heads, cache->heads);
   if (!workspace || workspace_bytes < need) return MLLM_HIP_E_BADARG;
-  if (p.row_tiles > 0xffffff / p.ranges) return MLLM_HIP_E_SHAPE;
+  const int64_t groups = (B * cache->heads * p.ranges + 7) / 8 * 8;
+  if (groups > 0xffffff / p.row_tiles) return MLLM_HIP_E_SHAPE;
   WeightArgs a = {};
   a.q = q->x;
   a.q_token = q->x_token_stride;
@@ -393,30 +617,44 @@ MLLM_API int mllm_hip_attention_weights(const mllm_hip_heads* q, int dtype, int6
   a.pitch = p.pitch;
   hipStream_t st = (hipStream_t)stream;
   const unsigned heads_of_all = (unsigned)(B * cache->heads);
-#define KSTEPS(KERNEL_, GRID_)                                                                                \
-  {                                                                                                           \
-    auto go = [&](auto kern) { hipLaunchKernelGGL(kern, GRID_, dim3(256), 0, st, a); };                       \
-    if (D <= 64) { if (f32) go(KERNEL_<2, true>); else go(KERNEL_<2, false>); }                               \
-    else if (D <= 96) { if (f32) go(KERNEL_<3, true>); else go(KERNEL_<3, false>); }                          \
-    else if (D <= 128) { if (f32) go(KERNEL_<4, true>); else go(KERNEL_<4, false>); }                         \
-    else { if (f32) go(KERNEL_<8, true>); else go(KERNEL_<8, false>); }                                       \
-    RC_RET((int)hipGetLastError());                                                                           \
+#define KSTEPS(GRID_, ...)                                                              \
+  {                                                                                     \
+    auto go = [&](auto ks, auto f) {                                                    \
+      constexpr int KS = decltype(ks)::value;                                           \
+      constexpr bool F32 = decltype(f)::value;                                          \
+      hipLaunchKernelGGL((__VA_ARGS__), GRID_, dim3(256), 0, st, a);                    \
+    };                                                                                  \
+    auto by_type = [&](auto ks) { if (f32) go(ks, std::true_type()); else go(ks, std::false_type()); }; \
+    if (D <= 64) by_type(std::integral_constant<int, 2>());                             \
+    else if (D <= 96) by_type(std::integral_constant<int, 3>());                        \
+    else if (D <= 128) by_type(std::integral_constant<int, 4>());                       \
+    else by_type(std::integral_constant<int, 8>());                                     \
+    RC_RET((int)hipGetLastError());                                                     \
   }
   if (p.few) {
     a.score = reinterpret_cast<float*>(workspace);
     a.ml = reinterpret_cast<f32x2*>(a.score + (size_t)B * cache->heads * p.rows * p.pitch);
-    KSTEPS(weights_scores_kernel, dim3((unsigned)p.ranges, heads_of_all))
+    KSTEPS(dim3((unsigned)p.ranges, heads_of_all), weights_scores_kernel<KS, F32>)
     hipLaunchKernelGGL(weights_sum_kernel, dim3((unsigned)((max_keys + 255) / 256), heads_of_all), dim3(256), 0, st, a);
     return (int)hipGetLastError();
   }
   a.row = reinterpret_cast<f32x2*>(workspace);
   a.ml = a.row + (size_t)T * heads;
-  KSTEPS(weights_max_kernel, dim3((unsigned)(p.row_tiles * p.ranges), heads_of_all))
+  a.part = reinterpret_cast<float*>(a.row + (size_t)(p.ranges > 1 ? p.ranges + 1 : 1) * T * heads);
+  a.splits = p.splits;
+  const dim3 grid((unsigned)(groups * p.row_tiles));
+  if (p.wr == 1) KSTEPS(grid, weights_max_kernel<KS, 1, F32>)
+  else if (p.wr == 2) KSTEPS(grid, weights_max_kernel<KS, 2, F32>)
+  else KSTEPS(grid, weights_max_kernel<KS, 4, F32>)
   if (p.ranges > 1) {
     hipLaunchKernelGGL(weights_join_kernel, dim3((unsigned)((T * heads + 255) / 256)), dim3(256), 0, st, a);
     RC_RET((int)hipGetLastError());
   }
-  KSTEPS(weights_mass_kernel, dim3((unsigned)((max_keys + WEIGHT_KEYS - 1) / WEIGHT_KEYS), heads_of_all))
+  KSTEPS(dim3((unsigned)((max_keys + p.keys - 1) / p.keys), heads_of_all, (unsigned)p.splits), weights_mass_kernel<KS, F32>)
 #undef KSTEPS
+  if (p.splits > 1) {
+    hipLaunchKernelGGL(weights_add_kernel, dim3((unsigned)((max_keys + 255) / 256), heads_of_all), dim3(256), 0, st, a);
+    RC_RET((int)hipGetLastError());
+  }
   return 0;
 }
