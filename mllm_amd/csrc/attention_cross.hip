@@ -24,16 +24,17 @@ struct CrossArgs {
   uint32_t k_bytes, v_bytes;  // from a key to the next
   const int32_t *cu, *first, *count;
   int64_t keys;  // rows of k and v
-  int T, B, kv, group, D, max_tokens, row_tiles, pieces, min_tiles;
+  int T, B, kv, group, D, max_tokens, row_tiles, rows_of_tile, pieces, min_tiles;
+  int whole, tiles;         // row tiles whose keys are not cut, and all of them
   float c;                  // scale * log2 e
-  float *part_o, *part_ml;  // [piece][T][heads][D], [2]
+  float *part_o, *part_ml;  // of the tiles that are cut, [piece][tile][row][D], [2]
 };
 __device__ u32x4 g_no_state[32];  // what keys behind the last read as (never written)
 
 struct CrossSeq {
   int first, n;  // rows of q
   int64_t key;   // its first key
-  int keys, per, pieces;  // its number of keys, tiles of a piece, pieces
+  int keys;
 };
 __device__ __forceinline__ CrossSeq cross_sequence(const CrossArgs& a, int b) {
   CrossSeq s;
@@ -42,18 +43,73 @@ __device__ __forceinline__ CrossSeq cross_sequence(const CrossArgs& a, int b) {
   s.n = min(max(hi - lo, 0), a.max_tokens);
   s.key = min((int64_t)max(a.first[b], 0), a.keys);
   s.keys = (int)min((int64_t)max(a.count[b], 0), a.keys - s.key);
-  const int tiles = (s.keys + 63) / 64;
-  s.per = max(a.min_tiles, (tiles + a.pieces - 1) / a.pieces);
-  s.pieces = max(1, (tiles + s.per - 1) / s.per);
   return s;
+}
+// What a workgroup has: row tile `tile` of all (those of a sequence's key head one behind the other), and of its keys piece `piece`
+struct CrossPlace {
+  CrossSeq s;
+  int b, h, tile, piece, pieces, row0, rows, k_begin, k_end;
+};
+// of a tile that is cut: tiles of 64 keys in a piece, and pieces
+__device__ __forceinline__ void cut(const CrossArgs& a, int keys, int& per, int& pieces) {
+  const int tiles = (keys + 63) / 64;
+  per = max(a.min_tiles, (tiles + a.pieces - 1) / a.pieces);
+  pieces = max(1, (tiles + per - 1) / per);
+}
+// Row tile `tile` in the order of workgroups.  Of several row tiles a head, key heads, which have equal work, go round the XCDs (workgroup i runs on XCD i % 8), the row tiles of one, which share its keys, stay on theirs;
+// of one each, neighbouring heads, whose states share cache lines, are on one.
+__device__ __forceinline__ void cross_tile(const CrossArgs& a, int tile, int& place, int& rt) {
+  if (a.whole == 0 || a.row_tiles == 1) {
+    const int j = a.whole ? xcd_run(tile, a.tiles) : tile;
+    rt = j % a.row_tiles;
+    place = j / a.row_tiles;
+    return;
+  }
+  const int heads = a.B * a.kv, round = heads / 8 * 8 * a.row_tiles;
+  if (tile < round) {
+    const int q = tile >> 3;
+    rt = q % a.row_tiles;
+    place = q / a.row_tiles * 8 + (tile & 7);
+  } else {
+    const int j = round + xcd_run(tile - round, heads * a.row_tiles - round);
+    rt = j % a.row_tiles;
+    place = j / a.row_tiles;
+  }
+}
+__device__ __forceinline__ bool cross_place(const CrossArgs& a, CrossPlace& p) {
+  const int i = blockIdx.x;
+  p.piece = 0;
+  p.tile = i;
+  if (i >= a.whole) {  // (a multiple of 8, or all)
+    const int j = xcd_run(i - a.whole, (a.tiles - a.whole) * a.pieces);
+    p.tile = a.whole + j / a.pieces;
+    p.piece = j % a.pieces;
+  }
+  int place, rt;
+  cross_tile(a, p.tile, place, rt);
+  p.h = place % a.kv;
+  p.b = place / a.kv;
+  p.s = cross_sequence(a, p.b);
+  p.rows = p.s.n * a.group;
+  p.row0 = rt * a.rows_of_tile;
+  p.pieces = 1;
+  p.k_begin = 0;
+  p.k_end = p.s.keys;
+  if (i >= a.whole && a.pieces > 1) {
+    int per;
+    cut(a, p.s.keys, per, p.pieces);
+    p.k_begin = p.piece * per * 64;
+    p.k_end = min(p.k_begin + per * 64, p.s.keys);
+  }
+  return p.row0 < p.rows && p.piece < p.pieces;
 }
 
 // Elements d .. d + 3 of a row's result: O, its maximum and sum go to the workspace where keys are cut
 template <bool F32>
-__device__ __forceinline__ void cross_put(const CrossArgs& a, const CrossSeq& s, int piece, int t, int head, int d, at_f32x4 x, float m, float sum) {
+__device__ __forceinline__ void cross_put(const CrossArgs& a, const CrossPlace& p, int row, int token, int head, int d, at_f32x4 x, float m, float sum) {
   if (d >= a.D) return;
-  if (s.pieces > 1) {
-    const int64_t at = ((int64_t)piece * a.T + t) * (a.kv * a.group) + head;
+  if (p.pieces > 1) {
+    const int64_t at = ((int64_t)p.piece * (a.tiles - a.whole) + (p.tile - a.whole)) * a.rows_of_tile + (row - p.row0);
     *reinterpret_cast<at_f32x4*>(a.part_o + at * a.D + d) = x;
     if (d == 0) {
       a.part_ml[2 * at] = m;
@@ -62,7 +118,7 @@ __device__ __forceinline__ void cross_put(const CrossArgs& a, const CrossSeq& s,
     return;
   }
   x *= sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);  // (no key: zeros; a NaN stays)
-  const int64_t at = t * a.o_token + head * a.o_head + d;
+  const int64_t at = (p.s.first + token) * a.o_token + head * a.o_head + d;
   if (F32) *reinterpret_cast<at_f32x4*>(reinterpret_cast<float*>(a.o) + at) = x;
   else *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(a.o) + at) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
 }
@@ -89,14 +145,10 @@ __global__ __launch_bounds__(256, (Cross<DP, DT, NQ, WR, F32>::WAVES)) void cros
   constexpr int KT = P::KT, C = P::C, WK = P::WK, NLOAD = P::NLOAD, KS = DP / 32, PARTS = P::PARTS;
   __shared__ __align__(16) uint16_t s_k[2 * KT * DP];
   __shared__ __align__(16) uint16_t s_v[2 * KT * DP];
-  // Workgroup i runs on XCD i % 8: the row tiles of a piece of keys follow one another on one XCD, whose L2 they share.
-  const int idx = blockIdx.x >> 3, rt = idx % a.row_tiles, place = (idx / a.row_tiles) * 8 + (blockIdx.x & 7);
-  const int h = place % a.kv, piece = place / a.kv % a.pieces, b = place / a.kv / a.pieces;
-  if (b >= a.B) return;
-  const CrossSeq s = cross_sequence(a, b);
-  const int rows = s.n * a.group, row0 = rt * P::ROWS * WR;
-  if (row0 >= rows || piece >= s.pieces) return;
-  const int k_begin = piece * s.per * KT, k_end = min(k_begin + s.per * KT, s.keys);
+  CrossPlace place;
+  if (!cross_place(a, place)) return;
+  const CrossSeq& s = place.s;
+  const int h = place.h, rows = place.rows, row0 = place.row0, k_begin = place.k_begin, k_end = place.k_end;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), wr = wave % WR, wk = wave / WR;
   const int col = lane & 15, g = lane >> 4;
 
@@ -302,7 +354,7 @@ __global__ __launch_bounds__(256, (Cross<DP, DT, NQ, WR, F32>::WAVES)) void cros
   for (int i = 0; i < NQ; i++) l[i] = sum32(sum16(l[i]));
 
   auto put = [&](int row, int d, at_f32x4 x, float mm, float sum) {
-    cross_put<F32>(a, s, piece, s.first + row / a.group, h * a.group + row % a.group, d, x, mm, sum);
+    cross_put<F32>(a, place, row, row / a.group, h * a.group + row % a.group, d, x, mm, sum);
   };
   if constexpr (WK == 1) {
 #pragma unroll
@@ -354,7 +406,7 @@ __global__ __launch_bounds__(256, (Cross<DP, DT, NQ, WR, F32>::WAVES)) void cros
 
 // Many rows of bf16 queries: a wave has 32 of them, v_mfma_f32_32x32x16_bf16, DK steps of 16 elements in the first product and DT tiles of 32 in the second.  First operand rows
 // 8 a + 4 b + c = keys 16 (a / 2) + 8 b + 4 (a % 2) + c leave a lane with one row of Q and, of every 16 keys, the eight consecutive ones that the second product takes.
-// Keys and values go from memory to LDS directly, keys a tile ahead: the scores of the next tile are matrix instructions between the exponents of this one.
+// Keys and values go from memory to LDS directly.  FULL: heads of 16 DK elements.
 template <int DK, int DT>
 struct Wide {
   static constexpr int C = 2 * DK, DP = 16 * DK, KT = 64;
@@ -365,45 +417,59 @@ struct Wide {
   }
 };
 typedef float at_f32x16 __attribute__((ext_vector_type(16)));
+// the sum of two bf16 and z
+__device__ __forceinline__ float pair_sum(uint32_t w, float z) {
+  return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf16x2, w), __builtin_bit_cast(bf16x2, 0x3f803f80u), z, false);
+}
 __device__ __forceinline__ at_f32x16 mma32(at_bf16x8 x, at_bf16x8 y, at_f32x16 acc) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, acc, 0, 0, 0); }
 
-template <int DK, int DT>
-__global__ __launch_bounds__(256, 2) void cross_wide_kernel(CrossArgs a) {
+template <int DK, int DT, bool FULL>
+__global__ __launch_bounds__(256, DK <= 6 ? 3 : 2) void cross_wide_kernel(CrossArgs a) {
   typedef Wide<DK, DT> P;
   constexpr int KT = P::KT, C = P::C, DP = P::DP, CHUNKS = P::CHUNKS;
-  __shared__ __align__(16) uint16_t s_k0[KT * DP], s_k1[KT * DP], s_v0[KT * DP + 16], s_v1[KT * DP + 16];  // (tiles of 32 of the last value end behind it)
-  const int idx = blockIdx.x >> 3, rt = idx % a.row_tiles, place = (idx / a.row_tiles) * 8 + (blockIdx.x & 7);
-  const int h = place % a.kv, piece = place / a.kv % a.pieces, b = place / a.kv / a.pieces;
-  if (b >= a.B) return;
-  const CrossSeq s = cross_sequence(a, b);
-  const int rows = s.n * a.group, row0 = rt * 128;
-  if (row0 >= rows || piece >= s.pieces) return;
-  const int k_begin = piece * s.per * KT, k_end = min(k_begin + s.per * KT, s.keys);
+  __shared__ __align__(16) uint16_t s_all[4 * KT * DP];
+  // in LDS: two tiles of values, two of keys (a tile of 32 elements of the last value may end behind it, where keys are)
+  constexpr int TILE = KT * DP;
+  CrossPlace place;
+  if (!cross_place(a, place)) return;
+  const CrossSeq& s = place.s;
+  const int h = place.h, rows = place.rows, row0 = place.row0, k_begin = place.k_begin, k_end = place.k_end;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, g = lane >> 5;
 
-  // Chunk i of a wave's: 64 pieces one behind the other in LDS; a lane's is piece at[i] ^ swz of its row
-  constexpr int NLOAD = (CHUNKS + 3) / 4;
+  // Two waves load keys and two values, half of a tile each: chunks of 64 pieces one behind the other in LDS, of which a lane loads the one that swz puts there.  Pieces behind a head's
+  // end are zeros from the beginning.
+  constexpr int NLOAD = CHUNKS / 2;
+  const bool keys = wave < 2;
   const int real = a.D / 8;
-  uint32_t koff[NLOAD], voff[NLOAD];
-  int row_of[NLOAD];  // KT: zeros
+  const uint32_t bytes = keys ? a.k_bytes : a.v_bytes;
+  const uint64_t base = (uint64_t)(uintptr_t)(keys ? a.k + h * a.k_head : a.v + h * a.v_head) + s.key * bytes;
+  uint16_t* const to = s_all + (keys ? 2 * TILE : 0) + (wave & 1) * (TILE / 2);
+  uint32_t off[NLOAD];
 #pragma unroll
   for (int i = 0; i < NLOAD; i++) {
-    const int e = (i * 4 + wave) * 64 + lane, r = e / C, p = (e % C) ^ P::swz(r);
-    row_of[i] = p < real ? r : 1 << 30;
-    koff[i] = r * a.k_bytes + p * 16;
-    voff[i] = r * a.v_bytes + p * 16;
-  }
-  typedef const __attribute__((address_space(1))) void* global_ptr;
-  typedef __attribute__((address_space(3))) void* lds_ptr;
-  const uint64_t zero = (uint64_t)(uintptr_t)g_no_state;
-  const uint64_t k_at = (uint64_t)(uintptr_t)(a.k + h * a.k_head) + s.key * a.k_bytes, v_at = (uint64_t)(uintptr_t)(a.v + h * a.v_head) + s.key * a.v_bytes;
-  auto ask = [&](uint64_t at, uint32_t bytes, const uint32_t (&off)[NLOAD], int k0, uint16_t* to) {
-    if (k0 >= k_end) return;
+    const int e = ((wave & 1) * NLOAD + i) * 64 + lane, r = e / C, p = (e % C) ^ P::swz(r);
+    off[i] = p < real ? r * bytes + p * 16 : ~0u;
+    if (!FULL && p >= real)
 #pragma unroll
-    for (int i = 0; i < NLOAD; i++) {
-      if (CHUNKS % 4 && i * 4 + wave >= CHUNKS) break;
-      const uint64_t from = k0 + row_of[i] < k_end ? at + (uint64_t)k0 * bytes + off[i] : zero;
-      __builtin_amdgcn_global_load_lds(reinterpret_cast<global_ptr>(from), (lds_ptr)(to + (i * 4 + wave) * 512), 16, 0, 0);
+      for (int t = 0; t < 2; t++) *reinterpret_cast<u32x4*>(to + t * TILE + (i * 64 + lane) * 8) = u32x4{0, 0, 0, 0};
+  }
+  typedef const __attribute__((address_space(1))) char* global_ptr;
+  typedef const __attribute__((address_space(1))) void* global_any;
+  typedef __attribute__((address_space(3))) void* lds_ptr;
+  auto ask = [&](int k0, int half) {
+    if (k0 >= k_end) return;
+    const global_ptr at = reinterpret_cast<global_ptr>(base + (uint64_t)k0 * bytes);
+    if (k0 + KT <= k_end) {
+#pragma unroll
+      for (int i = 0; i < NLOAD; i++)
+        if (FULL || off[i] != ~0u) __builtin_amdgcn_global_load_lds((global_any)(at + off[i]), (lds_ptr)(to + half * TILE + i * 512), 16, 0, 0);
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < NLOAD; i++) {  // (keys behind the last: zeros)
+      const int r = (((wave & 1) * NLOAD + i) * 64 + lane) / C;
+      const global_ptr from = k0 + r < k_end ? at + off[i] : reinterpret_cast<global_ptr>((uint64_t)(uintptr_t)g_no_state);
+      if (FULL || off[i] != ~0u) __builtin_amdgcn_global_load_lds((global_any)from, (lds_ptr)(to + half * TILE + i * 512), 16, 0, 0);
     }
   };
   // Q: second operand, row `col`, elements 16 s + 8 g .. + 7
@@ -420,7 +486,7 @@ __global__ __launch_bounds__(256, 2) void cross_wide_kernel(CrossArgs a) {
     }
   }
   at_f32x16 acc[DT] = {};
-  float m = -INFINITY, l = 0.f;  // the maximum so far times c; the sum of this lane's keys
+  float m = -INFINITY, l2[2] = {0.f, 0.f};  // the maximum so far times c; the sums of this lane's keys
   const int krow = (col & 3) | ((col >> 3) & 1) << 2 | ((col >> 2) & 1) << 3 | (col >> 4) << 4;
   // scores of 32 keys
   auto scores = [&](const uint16_t* k, int u) {
@@ -434,120 +500,104 @@ __global__ __launch_bounds__(256, 2) void cross_wide_kernel(CrossArgs a) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
   };
-  at_f32x16 y[2];
-  ask(k_at, a.k_bytes, koff, k_begin, s_k0);
-  arrived();
-  ask(k_at, a.k_bytes, koff, k_begin + KT, s_k1);
-  ask(v_at, a.v_bytes, voff, k_begin, s_v0);
-  if (k_begin < k_end) y[0] = scores(s_k0, 0), y[1] = scores(s_k0, 1);
-  // one tile: its scores are there; keys of the next are in `k`, of the one behind that go where this tile's were
-  auto turn = [&](int k0, auto last_, const uint16_t* k, uint16_t* k_next, const uint16_t* v, uint16_t* v_next) {
+  auto turn = [&](int k0, auto last_, int half) {
     constexpr bool last = decltype(last_)::value;
+    const uint16_t *v = s_all + half * TILE, *k = v + 2 * TILE;
     arrived();
-    if (!last) {
-      ask(k_at, a.k_bytes, koff, k0 + 2 * KT, k_next);
-      ask(v_at, a.v_bytes, voff, k0 + KT, v_next);
-    }
-    if (last) {
-      const int left = k_end - k0 - 8 * g;
-#pragma unroll
-      for (int u = 0; u < 2; u++)
-#pragma unroll
-        for (int j = 0; j < 16; j++) y[u][j] = 32 * u + 16 * (j >> 3) + (j & 7) < left ? y[u][j] : -INFINITY;
-    }
-    float top = larger(y[0][0], y[1][0]);
-#pragma unroll
-    for (int j = 1; j < 16; j++) top = larger(top, larger(y[0][j], y[1][j]));
-    top = across<32>(top) * a.c;
-    if (__ballot(top > m + 8.f)) {  // (weights of up to 2^8 do as well: most tiles leave O alone)
-      const float next = fmaxf(m, top), fix = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - next);
-      m = next;
-      l *= fix;
-#pragma unroll
-      for (int d = 0; d < DT; d++) acc[d] *= fix;
-    }
-    const float ref = m == -INFINITY ? 0.f : m;  // (nothing seen yet: every p is exp2(-inf))
-    at_bf16x8 fp[4];
-    at_f32x16 z[2];
+    if (!last) ask(k0 + KT, half ^ 1);
 #pragma unroll
     for (int u = 0; u < 2; u++) {
-      if (!last) z[u] = scores(k, u);
-      float sum[2];
+      if (last && k0 + 32 * u >= k_end) break;
+      at_f32x16 y = scores(k, u);
+      if (last) {
+        const int left = k_end - k0 - 32 * u - 8 * g;
+#pragma unroll
+        for (int j = 0; j < 16; j++) y[j] = 16 * (j >> 3) + (j & 7) < left ? y[j] : -INFINITY;
+      }
+      float top = larger(larger(y[0], y[1]), y[2]);
+#pragma unroll
+      for (int j = 3; j < 15; j += 2) top = larger(larger(y[j], y[j + 1]), top);
+      top = larger(top, y[15]);
+      top = across<32>(top) * a.c;
+      if (__ballot(top > m + 8.f)) {  // (weights of up to 2^8 do as well: most tiles leave O alone)
+        const float next = fmaxf(m, top), fix = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - next);
+        m = next;
+        l2[0] *= fix;
+        l2[1] *= fix;
+#pragma unroll
+        for (int d = 0; d < DT; d++) acc[d] *= fix;
+      }
+      const float ref = m == -INFINITY ? 0.f : m;  // (nothing seen yet: every p is exp2(-inf))
+      at_bf16x8 fp[2];
 #pragma unroll
       for (int hf = 0; hf < 2; hf++) {
         float e[8];
 #pragma unroll
-        for (int j = 0; j < 8; j++) e[j] = __builtin_amdgcn_exp2f(fmaf(y[u][8 * hf + j], a.c, -ref));
-        sum[hf] = ((e[0] + e[1]) + (e[2] + e[3])) + ((e[4] + e[5]) + (e[6] + e[7]));
-        fp[2 * u + hf] = frag(u32x4{pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7])});
+        for (int j = 0; j < 8; j++) e[j] = __builtin_amdgcn_exp2f(fmaf(y[8 * hf + j], a.c, -ref));
+        const u32x4 w = {pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7])};
+        fp[hf] = frag(w);
+        // (the sum of the weights as they are multiplied, two an instruction)
+        l2[hf] = pair_sum(w.x, pair_sum(w.y, l2[hf]));
+        l2[hf] = pair_sum(w.z, pair_sum(w.w, l2[hf]));
       }
-      l += sum[0] + sum[1];
-    }
-    // V^T: lane i of 16 asks for elements 4 (i % 4) .. + 3 of key 8 g + i / 4 and gets element i of keys 8 g .. + 3
-    const int i = lane & 15, half = (lane >> 4) & 1;
+      // V^T: lane i of 16 asks for elements 4 (i % 4) .. + 3 of key 8 g + i / 4 and gets element i of keys 8 g .. + 3
+      const int i = lane & 15, upper = (lane >> 4) & 1;
 #pragma unroll
-    for (int kk = 0; kk < 4; kk++) {
-      const int r = 16 * kk + 8 * g + (i >> 2), x = P::swz(r), x4 = P::swz(r + 4);
+      for (int kk = 0; kk < 2; kk++) {
+        const int r = 32 * u + 16 * kk + 8 * g + (i >> 2), x = P::swz(r), x4 = P::swz(r + 4);
 #pragma unroll
-      for (int d = 0; d < DT; d++) {
-        const int p = 4 * d + 2 * half + ((i & 3) >> 1);
-        typedef __attribute__((address_space(3))) at_s16x4* lds_quad;
-        const at_s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_quad)(v + r * DP + (p ^ x) * 8 + (i & 1) * 4));
-        const at_s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_quad)(v + (r + 4) * DP + (p ^ x4) * 8 + (i & 1) * 4));
-        acc[d] = mma32(frag(__builtin_bit_cast(u32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7))), fp[kk], acc[d]);
+        for (int d = 0; d < DT; d++) {
+          const int p = 4 * d + 2 * upper + ((i & 3) >> 1);
+          typedef __attribute__((address_space(3))) at_s16x4* lds_quad;
+          const at_s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_quad)(v + r * DP + (p ^ x) * 8 + (i & 1) * 4));
+          const at_s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_quad)(v + (r + 4) * DP + (p ^ x4) * 8 + (i & 1) * 4));
+          acc[d] = mma32(frag(__builtin_bit_cast(u32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7))), fp[kk], acc[d]);
+        }
       }
     }
-    if (!last) y[0] = z[0], y[1] = z[1];
   };
-  int k0 = k_begin;
-  bool odd = false;
-  while (k0 + KT < k_end) {
-    turn(k0, std::false_type(), s_k1, s_k0, s_v0, s_v1);
-    k0 += KT;
-    odd = true;
-    if (k0 + KT >= k_end) break;
-    turn(k0, std::false_type(), s_k0, s_k1, s_v1, s_v0);
-    k0 += KT;
-    odd = false;
-  }
-  if (k0 < k_end) {
-    if (odd) turn(k0, std::true_type(), s_k0, s_k1, s_v1, s_v0);
-    else turn(k0, std::true_type(), s_k1, s_k0, s_v0, s_v1);
-  }
-  l = sum32(l);
+  ask(k_begin, 0);
+  int k0 = k_begin, half = 0;
+  for (; k0 + KT < k_end; k0 += KT, half ^= 1) turn(k0, std::false_type(), half);
+  if (k0 < k_end) turn(k0, std::true_type(), half);
+  const float l = sum32(l2[0] + l2[1]);
   if (!live) return;
 #pragma unroll
   for (int d = 0; d < DT; d++)
 #pragma unroll
     for (int j = 0; j < 4; j++)
-      cross_put<false>(a, s, piece, s.first + token, head, 32 * d + 8 * j + 4 * g, at_f32x4{acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]}, m, l);
+      cross_put<false>(a, place, row, token, head, 32 * d + 8 * j + 4 * g, at_f32x4{acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]}, m, l);
 }
 
 // Joins the pieces of a row: 16 bytes of it per lane, L lanes a row
 template <int L, bool F32>
 __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
-  const int heads = a.kv * a.group, b = blockIdx.y, tid = threadIdx.x, d = tid % L * 4;
+  const int tid = threadIdx.x, d = tid % L * 4, tile = blockIdx.y;
+  int place, rt;
+  cross_tile(a, a.whole + tile, place, rt);
+  const int b = place / a.kv, h = place % a.kv;
   const CrossSeq s = cross_sequence(a, b);
-  if (s.pieces < 2) return;
-  const int i = blockIdx.x * (256 / L) + tid / L;
-  if (i >= s.n * heads || d >= a.D) return;
-  const int64_t all = (int64_t)a.T * heads, at = (int64_t)s.first * heads + i;
+  int per, pieces;
+  cut(a, s.keys, per, pieces);
+  const int i = blockIdx.x * (256 / L) + tid / L, row = rt * a.rows_of_tile + i;
+  if (pieces < 2 || i >= a.rows_of_tile || row >= s.n * a.group || d >= a.D) return;
+  const int64_t all = (int64_t)(a.tiles - a.whole) * a.rows_of_tile, at = (int64_t)tile * a.rows_of_tile + i;
   float m = -INFINITY, sum = 0.f;
   at_f32x4 x = {0.f, 0.f, 0.f, 0.f};
-  constexpr int U = 4;
-  for (int k = 0; k < s.pieces; k += U) {
+  constexpr int U = 8;
+  for (int k = 0; k < pieces; k += U) {
     float mk[U], lk[U];
     at_f32x4 xk[U];
 #pragma unroll
     for (int j = 0; j < U; j++) {
-      const int64_t from = min(k + j, s.pieces - 1) * all + at;
+      const int64_t from = min(k + j, pieces - 1) * all + at;
       mk[j] = a.part_ml[2 * from];
       lk[j] = a.part_ml[2 * from + 1];
       xk[j] = *reinterpret_cast<const at_f32x4*>(a.part_o + from * a.D + d);
     }
 #pragma unroll
     for (int j = 0; j < U; j++) {
-      if (k + j >= s.pieces) break;
+      if (k + j >= pieces) break;
       const float next = fmaxf(m, mk[j]), ref = next == -INFINITY ? 0.f : next;
       const float f = __builtin_amdgcn_exp2f(m - ref), fk = __builtin_amdgcn_exp2f(mk[j] - ref);
       x = x * f + xk[j] * fk;
@@ -556,37 +606,44 @@ __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
     }
   }
   x *= sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
-  const int t = i / heads;
-  const int64_t to = (s.first + t) * a.o_token + (i - t * heads) * a.o_head + d;
+  const int t = row / a.group;
+  const int64_t to = (s.first + t) * a.o_token + (h * a.group + row - t * a.group) * a.o_head + d;
   if (F32) *reinterpret_cast<at_f32x4*>(reinterpret_cast<float*>(a.o) + to) = x;
   else *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(a.o) + to) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
 }
 
 // ---- host side ------------------------------------------------------------------------------------------------------------
 struct CrossPlan {
-  int nq, wr, row_tiles, pieces, min_tiles;
+  int nq, wr, row_tiles, rows_of_tile, pieces, min_tiles;
+  int64_t whole, tiles;
 };
-// Rows of a workgroup by the rows there are; keys are cut while there are under 1024 workgroups without that, into pieces of two tiles and of twice as many keys as rows at least.
+// Rows of a workgroup by the rows there are.  CUs have two workgroups each: as many row tiles as make whole rounds of 512 go through all of their keys, the keys of
+// those that are left are cut into as many pieces as fill another, of two tiles and of twice as many keys as rows at least.
 static CrossPlan cross_plan(bool f32, int64_t B, int heads, int kv, int64_t max_tokens, int64_t max_keys, int D) {
   CrossPlan p;
   if (max_keys > 0x7fffffff) max_keys = 0x7fffffff;
   const int64_t rows = max_tokens * (heads / kv);
   p.nq = rows <= 64 || f32 || D > 128 ? 1 : 2;
   p.wr = rows <= 32 ? 2 : 4;
-  const int64_t per = (int64_t)p.nq * 16 * p.wr, row_tiles = (rows + per - 1) / per;
+  p.rows_of_tile = p.nq * 16 * p.wr;
+  const int64_t per = p.rows_of_tile, row_tiles = (rows + per - 1) / per;
   p.row_tiles = (int)row_tiles;
   const int64_t least = (2 * (rows < per ? rows : per) + 63) / 64;
   p.min_tiles = (int)(least > 2 ? least : 2);
-  const int64_t tiles = (max_keys + 63) / 64, most = (tiles + p.min_tiles - 1) / p.min_tiles, uncut = B * kv * row_tiles, wanted = (1023 + uncut) / uncut;
-  p.pieces = (int)(uncut >= 512 || most < 2 ? 1 : wanted < most ? wanted : most);
+  const int64_t slots = 512, most = (max_keys + p.min_tiles * 64 - 1) / (p.min_tiles * 64);
+  p.tiles = B * kv * row_tiles;
+  p.whole = p.tiles / slots * slots;
+  const int64_t rest = p.tiles - p.whole, wanted = rest ? slots / rest : 1;
+  p.pieces = (int)(most < 2 || wanted < 2 ? 1 : wanted < most ? wanted : most);
+  if (p.pieces == 1) p.whole = p.tiles;
   return p;
 }
-static size_t cross_room(const CrossPlan& p, int64_t T, int heads, int D) { return p.pieces > 1 ? (size_t)p.pieces * T * heads * (D + 2) * sizeof(float) : 0; }
+static size_t cross_room(const CrossPlan& p, int D) { return (size_t)(p.tiles - p.whole) * p.pieces * p.rows_of_tile * (D + 2) * sizeof(float); }
 static bool cross_sizes(int dtype, int64_t T, int64_t B, int heads, int kv, int head_dim, int64_t max_tokens, int64_t max_keys) {
   return (dtype == MLLM_HIP_F32 || dtype == MLLM_HIP_BF16) && T >= 0 && B >= 0 && heads >= 1 && kv >= 1 && head_dim >= 1 && max_tokens >= 0 && max_keys >= 0;
 }
 static bool cross_shape(int64_t T, int64_t B, int heads, int kv, int head_dim, int64_t max_tokens) {
-  return head_dim % 8 == 0 && head_dim <= 256 && heads % kv == 0 && heads <= 65536 && T <= 0x7fffffff / heads && B <= 65535 && max_tokens <= 0x7fffffff / heads;
+  return head_dim % 8 == 0 && head_dim <= 256 && heads % kv == 0 && heads <= 65536 && T <= 0x7fff0000 / heads && B <= 0x7fffffff / heads && max_tokens <= 0x7fffffff / heads;
 }
 
 }  // namespace mllmhip
@@ -597,7 +654,7 @@ MLLM_API size_t mllm_hip_attention_cross_workspace_bytes(int dtype, int64_t T, i
   if (!cross_sizes(dtype, T, B, heads, kv_heads, head_dim, max_tokens, max_keys) || !cross_shape(T, B, heads, kv_heads, head_dim, max_tokens)) return 0;
   if (T == 0 || B == 0 || max_tokens == 0) return 0;
   if (max_tokens > T) max_tokens = T;
-  return cross_room(cross_plan(dtype == MLLM_HIP_F32, B, heads, kv_heads, max_tokens, max_keys, head_dim), T, heads, head_dim);
+  return cross_room(cross_plan(dtype == MLLM_HIP_F32, B, heads, kv_heads, max_tokens, max_keys, head_dim), head_dim);
 }
 
 MLLM_API int mllm_hip_attention_cross(const mllm_hip_heads* q, int dtype, int64_t T, const mllm_hip_states* kv, const int32_t* cu_tokens, const int32_t* key_first,
@@ -622,10 +679,9 @@ MLLM_API int mllm_hip_attention_cross(const mllm_hip_heads* q, int dtype, int64_
   const bool f32 = dtype == MLLM_HIP_F32;
   const int heads = q->heads, D = kv->head_dim;
   const CrossPlan p = cross_plan(f32, B, heads, kv->heads, max_tokens, max_keys, D);
-  const size_t need = cross_room(p, T, heads, D);
+  const size_t need = cross_room(p, D);
   if (need && (!workspace || workspace_bytes < need)) return MLLM_HIP_E_BADARG;
-  const int64_t groups = (B * kv->heads * p.pieces + 7) / 8 * 8;
-  if (groups > 0xffffff / p.row_tiles) return MLLM_HIP_E_SHAPE;
+  if (p.whole + (p.tiles - p.whole) * p.pieces > 0xffffff) return MLLM_HIP_E_SHAPE;
   CrossArgs a = {};
   a.q = q->x;
   a.o = q->y;
@@ -650,13 +706,17 @@ MLLM_API int mllm_hip_attention_cross(const mllm_hip_heads* q, int dtype, int64_
   a.D = D;
   a.max_tokens = (int)max_tokens;
   a.row_tiles = p.row_tiles;
+  a.rows_of_tile = p.rows_of_tile;
   a.pieces = p.pieces;
-  a.min_tiles = p.pieces > 1 ? p.min_tiles : 1;
+  a.min_tiles = p.min_tiles;
+  a.whole = (int)p.whole;
+  a.tiles = (int)p.tiles;
   a.c = scale * 1.44269504088896341f;
   a.part_o = reinterpret_cast<float*>(workspace);
-  a.part_ml = p.pieces > 1 ? a.part_o + (size_t)p.pieces * T * heads * D : nullptr;
+  const int64_t rest = p.tiles - p.whole;
+  a.part_ml = rest ? a.part_o + (size_t)rest * p.pieces * p.rows_of_tile * D : nullptr;
   hipStream_t st = (hipStream_t)stream;
-  const dim3 grid((unsigned)(groups * p.row_tiles));
+  const dim3 grid((unsigned)(p.whole + rest * p.pieces));
   const int form = p.nq * 10 + p.wr;
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a); };
 #define CROSS(DP_, DT_, DK_)                                                   \
@@ -666,7 +726,10 @@ MLLM_API int mllm_hip_attention_cross(const mllm_hip_heads* q, int dtype, int64_
   } else {                                                                   \
     if (form == 12) go(cross_kernel<DP_, DT_, 1, 2, false>);                 \
     else if (form == 14) go(cross_kernel<DP_, DT_, 1, 4, false>);            \
-    else if constexpr (DP_ < 256) go(cross_wide_kernel<DK_, (DK_ + 1) / 2>); \
+    else if constexpr (DP_ < 256) {                                          \
+      if (D == 16 * DK_) go(cross_wide_kernel<DK_, (DK_ + 1) / 2, true>);    \
+      else go(cross_wide_kernel<DK_, (DK_ + 1) / 2, false>);                 \
+    }                                                                        \
   }
   if (D <= 64) { CROSS(64, 4, 4) }
   else if (D <= 80) { CROSS(96, 5, 5) }
@@ -675,9 +738,10 @@ MLLM_API int mllm_hip_attention_cross(const mllm_hip_heads* q, int dtype, int64_
   else { CROSS(256, 16, 16) }
 #undef CROSS
   RC_RET((int)hipGetLastError());
-  if (p.pieces > 1) {
+  if (rest) {
     const int lanes = D <= 64 ? 16 : D <= 128 ? 32 : 64, per = 256 / lanes;
-    const dim3 jgrid((unsigned)((max_tokens * heads + per - 1) / per), (unsigned)B);
+    const int64_t rows = max_tokens * a.group, most = rows < p.rows_of_tile ? rows : p.rows_of_tile;
+    const dim3 jgrid((unsigned)((most + per - 1) / per), (unsigned)rest);
     auto join = [&](auto kern) { hipLaunchKernelGGL(kern, jgrid, dim3(256), 0, st, a); };
 #define JOIN(L_)                              \
   if (f32) join(cross_join_kernel<L_, true>); \

@@ -73,7 +73,7 @@ def _cross(q=None, kv=None, dtype=BF16, T=2, cu=P, first=P, count=P, B=1, tokens
 
 
 @pytest.mark.parametrize("args,want", [
-    (dict(no_q=True), BADARG), (dict(no_kv=True), BADARG), (dict(dtype=2), BADARG), (dict(T=-1), BADARG), (dict(B=-1), BADARG), (dict(B=65536), SHAPE), (dict(tokens=-1), BADARG),
+    (dict(no_q=True), BADARG), (dict(no_kv=True), BADARG), (dict(dtype=2), BADARG), (dict(T=-1), BADARG), (dict(B=-1), BADARG), (dict(B=1 << 23), SHAPE), (dict(B=1 << 29), SHAPE), (dict(tokens=-1), BADARG),
     (dict(keys=-1), BADARG), (dict(keys=1 << 40, size=100), BADARG), (dict(cu=None), BADARG), (dict(first=None), BADARG), (dict(count=None), BADARG), (dict(scale=0.0), BADARG),
     (dict(scale=float("nan")), BADARG), (dict(scale=float("inf")), BADARG), (dict(scale=3e38), BADARG), (dict(T=1 << 29), SHAPE), (dict(tokens=1 << 29), SHAPE),
     (dict(kv=_states(head_dim=100)), SHAPE), (dict(kv=_states(head_dim=264)), SHAPE), (dict(kv=_states(head_dim=0)), BADARG), (dict(kv=_states(heads=3)), SHAPE), (dict(kv=_states(heads=0)), BADARG),
