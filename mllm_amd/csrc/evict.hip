@@ -25,7 +25,7 @@ struct EvictArgs {
   float* kept_mass;
 };
 
-enum { EVICT_WG = 1024, EVICT_HELD = 16384, EVICT_BINS = 2048 };
+enum { EVICT_WG = 1024, EVICT_HELD = 16, EVICT_BINS = 2048 };
 
 // larger weights, larger numbers; -0 as 0, a NaN below all
 __device__ __forceinline__ uint32_t weight_order(float v) {
@@ -34,41 +34,53 @@ __device__ __forceinline__ uint32_t weight_order(float v) {
   return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-__global__ __launch_bounds__(EVICT_WG) void evict_select_kernel(EvictArgs a) {
-  __shared__ uint32_t s_key[EVICT_HELD];
+// Each wave has a run of the positions, 64 at a time a lane each.  HELD: up to EVICT_HELD of 64, which stay in registers; else they are read again every time.
+template <bool HELD>
+__device__ __forceinline__ void evict_select(const EvictArgs& a, const float* mass, int n, int32_t* kept, float* kept_mass) {
   __shared__ uint32_t s_bin[EVICT_BINS];
   __shared__ uint32_t s_wave[2][EVICT_WG / 64];
   __shared__ uint32_t s_found[2];
   constexpr int WAVES = EVICT_WG / 64;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), b = blockIdx.y, h = blockIdx.x;
-  const int n = min(max(a.length[b], 0), a.most);
-  const float* mass = a.mass + b * a.mass_seq + h * a.mass_head;
-  int32_t* kept = a.kept + ((int64_t)b * a.heads + h) * a.keep;
-  float* kept_mass = a.kept_mass + ((int64_t)b * a.heads + h) * a.keep;
-  if (n <= a.keep) {
-    for (int i = tid; i < a.keep; i += EVICT_WG) {
-      kept[i] = i < n ? i : -1;
-      kept_mass[i] = i < n ? mass[i] : 0.f;
-    }
-    return;
-  }
-  const bool held = n <= EVICT_HELD;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lo = a.first, hi = n - a.recent;  // the ones that go by their weights: more of them than `want`
   uint32_t want = a.keep - a.first - a.recent;
-  if (held)
-    for (int i = tid; i < n; i += EVICT_WG) s_key[i] = weight_order(mass[i]);
-  auto key_at = [&](int i) { return held ? s_key[i] : weight_order(mass[i]); };
-  // the want-th largest key: `prefix` are its digits so far, `want` which one it is among the keys that begin with them
+  const bool none = want == 0;
+  const int share = (n + EVICT_WG - 1) / EVICT_WG, from = wave * share * 64 + lane;  // in 64s
+  float v[HELD ? EVICT_HELD : 1];
+  if constexpr (HELD) {
+#pragma unroll
+    for (int j = 0; j < EVICT_HELD; j++) v[j] = j < share && from + 64 * j < n ? mass[from + 64 * j] : 0.f;
+  }
+  // f(position, weight) of every one of this lane's positions, the wave's 64 together
+  auto each = [&](auto f) {
+    if constexpr (HELD) {
+#pragma unroll
+      for (int j = 0; j < EVICT_HELD; j++)
+        if (j < share) f(from + 64 * j, v[j]);
+    } else {
+      constexpr int U = 8;
+      for (int j0 = 0; j0 < share; j0 += U) {
+        float w[U];
+#pragma unroll
+        for (int j = 0; j < U; j++) w[j] = j0 + j < share && from + 64 * (j0 + j) < n ? mass[from + 64 * (j0 + j)] : 0.f;
+#pragma unroll
+        for (int j = 0; j < U; j++)
+          if (j0 + j < share) f(from + 64 * (j0 + j), w[j]);
+      }
+    }
+  };
+  // the want-th largest: `prefix` are its digits so far, `want` which one it is among the weights that begin with them
   uint32_t prefix = 0;
   const int shifts[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
 #pragma unroll
+  for (int i = tid; i < EVICT_BINS; i += EVICT_WG) s_bin[i] = 0;
+  __syncthreads();
+#pragma unroll
   for (int d = 0; d < 3; d++) {
-    for (int i = tid; i < EVICT_BINS; i += EVICT_WG) s_bin[i] = 0;
-    __syncthreads();
-    for (int i = lo + tid; i < hi; i += EVICT_WG) {
-      const uint32_t k = key_at(i);
-      if (d == 0 || k >> (shifts[d] + bits[d]) == prefix) atomicAdd(&s_bin[k >> shifts[d] & ((1u << bits[d]) - 1)], 1u);
-    }
+    each([&](int i, float w) {
+      const uint32_t k = weight_order(w);
+      if (i >= lo && i < hi && (d == 0 || k >> (shifts[d] + bits[d]) == prefix)) atomicAdd(&s_bin[k >> shifts[d] & ((1u << bits[d]) - 1)], 1u);
+    });
     __syncthreads();
     // bins from the largest down, two a thread: the one that the want-th is in
     const int top = EVICT_BINS - 1 - 2 * tid;
@@ -80,9 +92,11 @@ __global__ __launch_bounds__(EVICT_WG) void evict_select_kernel(EvictArgs a) {
       up += lane >= s ? o : 0;
     }
     if (lane == 63) s_wave[0][wave] = up;
+    s_bin[top] = s_bin[top - 1] = 0;  // (by the thread that has read them: for the next digit)
     __syncthreads();
     uint32_t front = up - c0 - c1;
-    for (int w = 0; w < wave; w++) front += s_wave[0][w];
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) front += w < wave ? s_wave[0][w] : 0;
     if (want && front < want && want <= front + c0 + c1) {
       const bool first = want <= front + c0;
       s_found[0] = first ? top : top - 1;
@@ -93,43 +107,58 @@ __global__ __launch_bounds__(EVICT_WG) void evict_select_kernel(EvictArgs a) {
       prefix = prefix << bits[d] | s_found[0];
       want = s_found[1];
     }
-    __syncthreads();
   }
-  const bool none = a.keep == a.first + a.recent;
-  // Each wave has a share of the positions; of keys that equal the border the first `want` stay.
-  const int share = ((n + WAVES - 1) / WAVES + 63) / 64 * 64, from = min(wave * share, n), to = min(from + share, n);
-  uint32_t above = 0, equal = 0;
-  for (int i0 = from; i0 < to; i0 += 64) {
-    const int i = i0 + lane;
-    const uint32_t k = i < to ? key_at(i) : 0;
-    const bool middle = i >= lo && i < hi, is_above = i < to && (!middle || (!none && k > prefix)), is_equal = i < to && middle && !none && k == prefix;
-    above += __popcll(__ballot(is_above));
-    equal += __popcll(__ballot(is_equal));
-  }
+  // of weights that equal the border the first `want` stay
+  auto above = [&](int i, uint32_t k) { return i < n && (i < lo || i >= hi || (!none && k > prefix)); };
+  auto equal = [&](int i, uint32_t k) { return i >= lo && i < hi && !none && k == prefix; };
+  uint32_t n_above = 0, n_equal = 0;
+  each([&](int i, float w) {
+    const uint32_t k = weight_order(w);
+    n_above += __popcll(__ballot(above(i, k)));
+    n_equal += __popcll(__ballot(equal(i, k)));
+  });
+  __syncthreads();
   if (lane == 0) {
-    s_wave[0][wave] = above;
-    s_wave[1][wave] = equal;
+    s_wave[0][wave] = n_above;
+    s_wave[1][wave] = n_equal;
   }
   __syncthreads();
-  above = equal = 0;
-  for (int w = 0; w < wave; w++) {
-    above += s_wave[0][w];
-    equal += s_wave[1][w];
+  n_above = n_equal = 0;
+#pragma unroll
+  for (int w = 0; w < WAVES; w++) {
+    n_above += w < wave ? s_wave[0][w] : 0;
+    n_equal += w < wave ? s_wave[1][w] : 0;
   }
-  for (int i0 = from; i0 < to; i0 += 64) {
-    const int i = i0 + lane;
-    const uint32_t k = i < to ? key_at(i) : 0;
-    const bool middle = i >= lo && i < hi, is_above = i < to && (!middle || (!none && k > prefix)), is_equal = i < to && middle && !none && k == prefix;
+  const uint64_t below = (1ull << lane) - 1;
+  each([&](int i, float w) {
+    const uint32_t k = weight_order(w);
+    const bool is_above = above(i, k), is_equal = equal(i, k);
     const uint64_t va = __ballot(is_above), ve = __ballot(is_equal);
-    const uint64_t below = (1ull << lane) - 1;
-    const uint32_t e = equal + __popcll(ve & below);  // equal ones in front
+    const uint32_t e = n_equal + __popcll(ve & below);  // equal ones in front
     if (is_above || (is_equal && e < want)) {
-      const uint32_t at = above + __popcll(va & below) + min(e, want);
+      const uint32_t at = n_above + __popcll(va & below) + min(e, want);
       kept[at] = i;
-      kept_mass[at] = mass[i];
+      kept_mass[at] = w;
     }
-    above += __popcll(va);
-    equal += __popcll(ve);
+    n_above += __popcll(va);
+    n_equal += __popcll(ve);
+  });
+}
+
+__global__ __launch_bounds__(EVICT_WG) void evict_select_kernel(EvictArgs a) {
+  const int b = blockIdx.y, h = blockIdx.x, n = min(max(a.length[b], 0), a.most);
+  const float* mass = a.mass + b * a.mass_seq + h * a.mass_head;
+  int32_t* kept = a.kept + ((int64_t)b * a.heads + h) * a.keep;
+  float* kept_mass = a.kept_mass + ((int64_t)b * a.heads + h) * a.keep;
+  if (n <= a.keep) {
+    for (int i = threadIdx.x; i < a.keep; i += EVICT_WG) {
+      kept[i] = i < n ? i : -1;
+      kept_mass[i] = i < n ? mass[i] : 0.f;
+    }
+  } else if (n <= EVICT_HELD * EVICT_WG) {
+    evict_select<true>(a, mass, n, kept, kept_mass);
+  } else {
+    evict_select<false>(a, mass, n, kept, kept_mass);
   }
 }
 
