@@ -97,7 +97,9 @@ __device__ __forceinline__ at_f32x4 key_scores(const u32x4 (&k)[KS], const at_bf
       s = at_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int ks = 0; ks < KS; ks++) {
-        const at_bf16x8 f = frag(u32x4{finite_pair(k[ks].x), finite_pair(k[ks].y), finite_pair(k[ks].z), finite_pair(k[ks].w)});
+        u32x4 x = k[ks];
+        asm volatile("" : "+v"(x));  // (worked out here and not in front of the branch, where it was most of the kernel's instructions)
+        const at_bf16x8 f = frag(u32x4{finite_pair(x.x), finite_pair(x.y), finite_pair(x.z), finite_pair(x.w)});
         s = mma(f, q[ks][2], s);
         s = mma(f, q[ks][1], s);
         s = mma(frag(k[ks]), q[ks][0], s);
@@ -453,7 +455,9 @@ __global__ __launch_bounds__(256, 2) void weights_mass_kernel(WeightArgs a) {
             y[i] = at_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
-              const at_bf16x8 f = frag(u32x4{finite_pair(k[i][ks].x), finite_pair(k[i][ks].y), finite_pair(k[i][ks].z), finite_pair(k[i][ks].w)});
+              u32x4 x = k[i][ks];
+              asm volatile("" : "+v"(x));
+              const at_bf16x8 f = frag(u32x4{finite_pair(x.x), finite_pair(x.y), finite_pair(x.z), finite_pair(x.w)});
               y[i] = mma(f, query(ks, 2), y[i]);
               y[i] = mma(f, query(ks, 1), y[i]);
               y[i] = mma(frag(k[i][ks]), query(ks, 0), y[i]);
