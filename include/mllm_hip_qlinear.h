@@ -696,7 +696,8 @@ int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_t T, cons
  * Sequences without new tokens and positions from prefix + new tokens on stay as they are.  max_tokens, max_keys: a sequence's new tokens behind the first max_tokens add
  * nothing; positions from max_keys on are neither seen nor get anything; positions from mass_len on are seen, and what they get is stored nowhere.  q: F32 or BF16 (y and weight are not looked at).
  * head_dim % 8 == 0, <= 256; heads a multiple of the cache's; 0 < scale <= 2e38; 0 <= decay <= 2e38; table_len * page_size and max_keys up to 2^30, B * kv heads up to 65535.  The sums do not depend on any order of execution: the same
- * inputs give the same bits.  workspace: ..._workspace_bytes, 16-byte aligned; less is MLLM_HIP_E_BADARG.  Up to three launches. */
+ * inputs give the same bits.  workspace: ..._workspace_bytes (0: none), 16-byte aligned; less is MLLM_HIP_E_BADARG.  One launch, two or three over many keys, up to five
+ * with many rows. */
 size_t mllm_hip_attention_weights_workspace_bytes(int dtype, int64_t T, int64_t B, int heads, int kv_heads, int head_dim, int64_t max_tokens, int64_t max_keys);
 int mllm_hip_attention_weights(const mllm_hip_heads* q, int dtype, int64_t T, const mllm_hip_kv_cache* cache, float* mass, int64_t mass_stride,
                                int64_t mass_head_stride, int64_t mass_len, const int32_t* block_table, int64_t table_stride, int64_t table_len,

@@ -40,6 +40,7 @@ struct WeightArgs {
   f32x2* row;    // [T][heads]: maximum (times c) and 1 / sum of all keys
   float* part;   // [split][B][kv][pitch]: what keys get of a part of the rows
   int splits;
+  uint16_t* parts;  // fp32 queries as three bf16 parts, [3][T][heads][D]
 };
 __device__ u32x4 g_no_key[32];  // what a page outside the cache reads as (never written)
 
@@ -57,17 +58,21 @@ __device__ __forceinline__ WeightSeq weight_sequence(const WeightArgs& a, int b)
   return s;
 }
 
-// 16 bytes ks * 32 + 8 g .. of key `key` of a sequence
+__device__ __forceinline__ uint32_t page_of(const WeightArgs& a, int key) { return __umulhi(2 * (uint32_t)key, a.page_mul) >> a.page_shift; }
+// elements 32 ks + 8 g .. + 7 of key `key`, which is in page `id`
 template <int KS>
-__device__ __forceinline__ void load_key(const WeightArgs& a, const int32_t* table, uint64_t k_at, int key, bool there, int g, u32x4 (&r)[KS]) {
-  const uint32_t page = __umulhi(2 * (uint32_t)key, a.page_mul) >> a.page_shift, id = (uint32_t)(there ? table[page] : -1);
-  const bool good = id < a.pages;
-  const uint64_t at = good ? k_at + (uint64_t)id * a.page_bytes + ((uint32_t)key - page * a.page) * a.slot_bytes : (uint64_t)(uintptr_t)g_no_key;
+__device__ __forceinline__ void load_key_of(const WeightArgs& a, uint64_t k_at, int id, int key, int g, u32x4 (&r)[KS]) {
+  const bool good = (uint32_t)id < a.pages;
+  const uint64_t at = good ? k_at + (uint64_t)(uint32_t)id * a.page_bytes + ((uint32_t)key - page_of(a, key) * a.page) * a.slot_bytes : (uint64_t)(uintptr_t)g_no_key;
 #pragma unroll
   for (int ks = 0; ks < KS; ks++) {
     const int e = 32 * ks + 8 * g;
     r[ks] = *reinterpret_cast<const __attribute__((address_space(1))) u32x4*>(e < a.D ? at + e * 2 : (uint64_t)(uintptr_t)g_no_key);
   }
+}
+template <int KS>
+__device__ __forceinline__ void load_key(const WeightArgs& a, const int32_t* table, uint64_t k_at, int key, bool there, int g, u32x4 (&r)[KS]) {
+  load_key_of<KS>(a, k_at, there ? table[page_of(a, key)] : -1, key, g, r);
 }
 
 // Rows of C 16-byte pieces lie in LDS with their pieces exclusive-ored by bits of the row's number, so that 16 rows' pieces of one number are in different banks.
@@ -108,11 +113,20 @@ __device__ __forceinline__ at_f32x4 key_scores(const u32x4 (&k)[KS], const at_bf
   }
   return s;
 }
-// Rows r0 .. r0 + 15 of a sequence as an operand: row `col` of lane col
-template <int KS, bool F32>
+// Rows r0 .. r0 + 15 of a sequence as an operand: row `col` of lane col.  MADE: the parts of fp32 queries are in the workspace.
+template <int KS, bool F32, bool MADE = false>
 __device__ __forceinline__ void load_rows(const WeightArgs& a, const WeightSeq& s, int h, int r, int rows, int g, at_bf16x8 (&q)[KS][F32 ? 3 : 1]) {
   const bool live = r < rows;
   const int token = live ? r / a.group : 0, head = h * a.group + (live ? r - token * a.group : 0);
+  if constexpr (MADE) {
+    const int64_t heads = a.kv * a.group, at = ((s.first + token) * heads + head) * a.D + 8 * g;
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++)
+#pragma unroll
+      for (int p = 0; p < 3; p++)
+        q[ks][p] = frag(live && 32 * ks + 8 * g < a.D ? *reinterpret_cast<const u32x4*>(a.parts + p * a.T * heads * a.D + at + 32 * ks) : u32x4{0, 0, 0, 0});
+    return;
+  }
   const int64_t at = (s.first + token) * a.q_token + head * a.q_head + 8 * g;
 #pragma unroll
   for (int ks = 0; ks < KS; ks++) query_parts<F32>(a.q, at + 32 * ks, live && 32 * ks + 8 * g < a.D, q[ks]);
@@ -139,9 +153,19 @@ __device__ __forceinline__ void join_lanes(float& m, float& l) {  // over the fo
 __device__ __forceinline__ f32x2 final_row(float m, float l) { return f32x2{m == -INFINITY ? 0.f : m, l == 0.f ? 0.f : 1.0f / l}; }
 
 // ---- up to 16 rows --------------------------------------------------------------------------------------------------------
+// a lane's scores of 16 keys from k0 on, -inf where its row does not see them
+template <int KS, bool F32>
+__device__ __forceinline__ at_f32x4 seen_scores(const u32x4 (&k)[KS], const at_bf16x8 (&q)[KS][F32 ? 3 : 1], int seen) {
+  at_f32x4 y = key_scores<KS, F32>(k, q);
+#pragma unroll
+  for (int j = 0; j < 4; j++) y[j] = j < seen ? y[j] : -INFINITY;
+  return y;
+}
+
 template <int KS, bool F32>
 __global__ __launch_bounds__(256) void weights_scores_kernel(WeightArgs a) {
   __shared__ f32x2 s_ml[4][16];
+  constexpr int U = KS == 8 ? 1 : 2, STEP = 64 * U;  // sixteens of keys of a wave at a time; keys of a workgroup
   const int h = blockIdx.y % a.kv, b = blockIdx.y / a.kv, range = blockIdx.x;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
   const WeightSeq s = weight_sequence(a, b);
@@ -150,20 +174,40 @@ __global__ __launch_bounds__(256) void weights_scores_kernel(WeightArgs a) {
   const int per = ((s.keys + a.ranges - 1) / a.ranges + 63) / 64 * 64, begin = range * per, end = min(begin + per, s.keys);
   const int32_t* table = a.table + b * a.table_stride;
   const uint64_t k_at = (uint64_t)(uintptr_t)(a.k + h * a.head_stride);
+  // Keys are on their way while the ones before them are worked on, and the pages of those behind.
+  int ids[U];
+  u32x4 next[U][KS];
+  const int first = begin + wave * 16 * U + col;
+  auto ask_ids = [&](int k0) {
+#pragma unroll
+    for (int u = 0; u < U; u++) ids[u] = k0 + 16 * u < end ? table[page_of(a, k0 + 16 * u)] : -1;
+  };
+  auto ask = [&](int k0) {
+#pragma unroll
+    for (int u = 0; u < U; u++) load_key_of<KS>(a, k_at, ids[u], k0 + 16 * u, g, next[u]);
+    ask_ids(k0 + STEP);
+  };
+  ask_ids(first);
+  ask(first);
   at_bf16x8 q[KS][F32 ? 3 : 1];
   load_rows<KS, F32>(a, s, h, col, rows, g, q);
-  const int token = col < rows ? col / a.group : -1;
+  const int token = col < rows ? col / a.group : -1, sees = token < 0 ? 0 : min(s.prefix + token + 1, end);
   float m = -INFINITY, l = 0.f;
   float* score = a.score + ((int64_t)blockIdx.y * a.rows + col) * a.pitch;
-  for (int k0 = begin + wave * 16; k0 < end; k0 += 64) {
-    u32x4 k[KS];
-    load_key<KS>(a, table, k_at, k0 + col, k0 + col < end, g, k);
-    at_f32x4 y = key_scores<KS, F32>(k, q);
-    const int seen = min(s.prefix + token + 1, end) - (k0 + 4 * g);  // of this lane's keys
+  for (int k0 = begin + wave * 16 * U; k0 < end; k0 += STEP) {
+    u32x4 k[U][KS];
 #pragma unroll
-    for (int j = 0; j < 4; j++) y[j] = j < seen && token >= 0 ? y[j] : -INFINITY;
-    if (col < a.rows) *reinterpret_cast<at_f32x4*>(score + k0 + 4 * g) = y;
-    take(m, l, y, a.c);
+    for (int u = 0; u < U; u++)
+#pragma unroll
+      for (int ks = 0; ks < KS; ks++) k[u][ks] = next[u][ks];
+    if (k0 + STEP < end) ask(k0 + STEP + col);
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      if (k0 + 16 * u >= end) break;
+      const at_f32x4 y = seen_scores<KS, F32>(k[u], q, sees - (k0 + 16 * u + 4 * g));
+      if (col < a.rows) *reinterpret_cast<at_f32x4*>(score + k0 + 16 * u + 4 * g) = y;
+      take(m, l, y, a.c);
+    }
   }
   join_lanes(m, l);
   if (g == 0) s_ml[wave][col] = f32x2{m, l};
@@ -174,32 +218,104 @@ __global__ __launch_bounds__(256) void weights_scores_kernel(WeightArgs a) {
   }
 }
 
+// R: at least the rows.  What a key reads is asked for in front of the joining of the ranges' maxima and sums.
+template <int R>
 __global__ __launch_bounds__(256) void weights_sum_kernel(WeightArgs a) {
-  __shared__ f32x2 s_row[16];
-  const int h = blockIdx.y % a.kv, b = blockIdx.y / a.kv;
-  const WeightSeq s = weight_sequence(a, b);
-  if (s.n == 0) return;
-  if (threadIdx.x < a.rows) {
-    float m = -INFINITY, l = 0.f;
-    for (int r = 0; r < a.ranges; r++) {
-      const f32x2 x = a.ml[((int64_t)r * gridDim.y + blockIdx.y) * a.rows + threadIdx.x];
-      join(m, l, x.x, x.y);
+  __shared__ f32x2 s_part[256 / R][R];
+  __shared__ f32x2 s_row[R];
+  const int h = blockIdx.y % a.kv, b = blockIdx.y / a.kv, tid = threadIdx.x, key = blockIdx.x * 256 + tid;
+  const float* score = a.score + (int64_t)blockIdx.y * a.rows * a.pitch + min(key, a.pitch - 1);
+  float y[R];
+#pragma unroll
+  for (int r = 0; r < R; r++) y[r] = score[(int64_t)min(r, a.rows - 1) * a.pitch];  // (of keys that are not there: any numbers, never used)
+  const int r = tid % R, group = tid / R;
+  float m = -INFINITY, l = 0.f;
+  if (r < a.rows) {
+    constexpr int U = 4;
+    for (int i = group; i < a.ranges; i += U * (256 / R)) {
+      f32x2 x[U];
+#pragma unroll
+      for (int u = 0; u < U; u++) x[u] = a.ml[((int64_t)min(i + u * (256 / R), a.ranges - 1) * gridDim.y + blockIdx.y) * a.rows + r];
+#pragma unroll
+      for (int u = 0; u < U; u++)
+        if (i + u * (256 / R) < a.ranges) join(m, l, x[u].x, x[u].y);
     }
-    s_row[threadIdx.x] = final_row(m, l);
+  }
+  const WeightSeq s = weight_sequence(a, b);
+  if (s.n == 0 || blockIdx.x * 256 >= s.keys) return;
+  s_part[group][r] = f32x2{m, l};
+  __syncthreads();
+  if (tid < R) {
+    for (int i = 1; i < 256 / R && i < a.ranges; i++) join(m, l, s_part[i][tid].x, s_part[i][tid].y);
+    s_row[tid] = final_row(m, l);
   }
   __syncthreads();
-  const int key = blockIdx.x * 256 + threadIdx.x;
   if (key >= s.keys) return;
-  const float* score = a.score + (int64_t)blockIdx.y * a.rows * a.pitch + key;
   float sum = 0.f;
-  for (int r = 0; r < a.rows; r++) {
-    const float p = __builtin_amdgcn_exp2f(fmaf(score[(int64_t)r * a.pitch], a.c, -s_row[r].x)) * s_row[r].y;
-    sum += key <= s.prefix + r / a.group ? p : 0.f;  // (a row without a number has none for keys that it sees)
+#pragma unroll
+  for (int i = 0; i < R; i++) {
+    const float p = __builtin_amdgcn_exp2f(fmaf(y[i], a.c, -s_row[i].x)) * s_row[i].y;
+    sum += i < a.rows && key <= s.prefix + i / a.group ? p : 0.f;  // (a row without a number has none for keys that it sees)
   }
   put_mass(a, s, b, h, key, sum);
 }
 
+// The whole of it in one launch where keys are few: a workgroup has a key head of a sequence, scores stay in LDS.
+enum { WEIGHT_ONE = 960, WEIGHT_PITCH = WEIGHT_ONE + 4 };  // 16 rows in less than 64 KB
+template <int KS, bool F32>
+__global__ __launch_bounds__(512) void weights_one_kernel(WeightArgs a) {
+  extern __shared__ __align__(16) float s_score[];  // [rows][WEIGHT_PITCH]
+  __shared__ f32x2 s_ml[8][16];
+  __shared__ f32x2 s_row[16];
+  const int h = blockIdx.x % a.kv, b = blockIdx.x / a.kv;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), col = lane & 15, g = lane >> 4;
+  const WeightSeq s = weight_sequence(a, b);
+  const int rows = min(s.n * a.group, a.rows);
+  if (rows == 0) return;
+  const int32_t* table = a.table + b * a.table_stride;
+  const uint64_t k_at = (uint64_t)(uintptr_t)(a.k + h * a.head_stride);
+  at_bf16x8 q[KS][F32 ? 3 : 1];
+  load_rows<KS, F32>(a, s, h, col, rows, g, q);
+  const int token = col < rows ? col / a.group : -1, sees = token < 0 ? 0 : min(s.prefix + token + 1, s.keys);
+  float m = -INFINITY, l = 0.f;
+  for (int k0 = wave * 16; k0 < s.keys; k0 += 128) {
+    u32x4 k[KS];
+    load_key<KS>(a, table, k_at, k0 + col, k0 + col < s.keys, g, k);
+    const at_f32x4 y = seen_scores<KS, F32>(k, q, sees - (k0 + 4 * g));
+    if (col < rows) *reinterpret_cast<at_f32x4*>(s_score + col * WEIGHT_PITCH + k0 + 4 * g) = y;
+    take(m, l, y, a.c);
+  }
+  join_lanes(m, l);
+  if (g == 0) s_ml[wave][col] = f32x2{m, l};
+  __syncthreads();
+  if (threadIdx.x < 16) {
+    for (int w = 1; w < 8; w++) join(m, l, s_ml[w][col].x, s_ml[w][col].y);
+    s_row[col] = final_row(m, l);
+  }
+  __syncthreads();
+  for (int key = threadIdx.x; key < s.keys; key += 512) {
+    float sum = 0.f;
+    for (int r = 0; r < rows; r++) {
+      const float p = __builtin_amdgcn_exp2f(fmaf(s_score[r * WEIGHT_PITCH + key], a.c, -s_row[r].x)) * s_row[r].y;
+      sum += key <= s.prefix + r / a.group ? p : 0.f;
+    }
+    put_mass(a, s, b, h, key, sum);
+  }
+}
+
 // ---- more rows ------------------------------------------------------------------------------------------------------------
+// fp32 queries as three bf16 parts, once for all that read them
+__global__ __launch_bounds__(256) void weights_parts_kernel(WeightArgs a) {
+  const int pieces = a.D / 8, heads = a.kv * a.group;
+  const int64_t all = (int64_t)a.T * heads * pieces, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= all) return;
+  const int64_t row = i / pieces, token = row / heads;
+  at_bf16x8 part[3];
+  query_parts<true>(a.q, token * a.q_token + (row - token * heads) * a.q_head + (i - row * pieces) * 8, true, part);
+#pragma unroll
+  for (int p = 0; p < 3; p++) *reinterpret_cast<at_bf16x8*>(a.parts + (p * all + i) * 8) = part[p];
+}
+
 // Maxima and sums: four waves, WR along rows times 4 / WR along keys, 64 keys in LDS at a time, the next ones on their way.
 enum { WEIGHT_TILE = 64 };
 // rows of a wave, in sixteens (fp32 queries of 256 elements take 96 registers for sixteen)
@@ -235,12 +351,11 @@ __global__ __launch_bounds__(256, 2) void weights_max_kernel(WeightArgs a) {
     to[i] = r * DP + (p ^ swizzle<C>(r)) * 8;
     if (!has[i]) *reinterpret_cast<u32x4*>(s_k + to[i]) = *reinterpret_cast<u32x4*>(s_k + KT * DP + to[i]) = u32x4{0, 0, 0, 0};
   }
-  auto page_of = [&](int key) { return __umulhi(2 * (uint32_t)key, a.page_mul) >> a.page_shift; };
   auto ask_ids = [&](int k0) {
 #pragma unroll
     for (int i = 0; i < NLOAD; i++) {
       const int key = k0 + row_of[i];
-      ids[i] = key < end && has[i] ? table[page_of(key)] : -1;
+      ids[i] = key < end && has[i] ? table[page_of(a, key)] : -1;
     }
   };
   u32x4 rk[NLOAD];
@@ -248,7 +363,7 @@ __global__ __launch_bounds__(256, 2) void weights_max_kernel(WeightArgs a) {
 #pragma unroll
     for (int i = 0; i < NLOAD; i++) {
       const uint32_t key = (uint32_t)(k0 + row_of[i]), id = (uint32_t)ids[i];
-      const uint64_t at = k_at + (uint64_t)id * a.page_bytes + ((key - page_of((int)key) * a.page) * a.slot_bytes + (i * 256 + tid) % C * 16);
+      const uint64_t at = k_at + (uint64_t)id * a.page_bytes + ((key - page_of(a, (int)key) * a.page) * a.slot_bytes + (i * 256 + tid) % C * 16);
       rk[i] = *reinterpret_cast<const __attribute__((address_space(1))) u32x4*>(id < a.pages ? at : (uint64_t)(uintptr_t)g_no_key);
     }
     ask_ids(k0 + KT);
@@ -268,7 +383,7 @@ __global__ __launch_bounds__(256, 2) void weights_max_kernel(WeightArgs a) {
 #pragma unroll
   for (int i = 0; i < NQ; i++) {
     const int r = row0 + (wr * NQ + i) * 16 + col;
-    load_rows<KS, F32>(a, s, h, r, rows, g, q[i]);
+    load_rows<KS, F32, F32>(a, s, h, r, rows, g, q[i]);
     token[i] = r < rows ? r / a.group : -1;
     m[i] = -INFINITY;
     l[i] = 0.f;
@@ -373,7 +488,7 @@ struct Mass {
 template <int KS, bool F32>
 __global__ __launch_bounds__(256, 2) void weights_mass_kernel(WeightArgs a) {
   typedef Mass<KS, F32> P;
-  constexpr int NK = P::NK, RT = P::RT, DP = KS * 32, C = DP / 8, PARTS = F32 ? 3 : 1, NL = (RT * C + 255) / 256, XT = F32 ? MLLM_HIP_F32 : MLLM_HIP_BF16;
+  constexpr int NK = P::NK, RT = P::RT, DP = KS * 32, C = DP / 8, PARTS = F32 ? 3 : 1, NL = (RT * C + 255) / 256;
   __shared__ __align__(16) uint16_t s_q[2][PARTS][RT * DP];
   __shared__ f32x2 s_row[2][RT];
   const int h = blockIdx.y % a.kv, b = blockIdx.y / a.kv, split = blockIdx.z;
@@ -384,16 +499,20 @@ __global__ __launch_bounds__(256, 2) void weights_mass_kernel(WeightArgs a) {
   const int per = ((rows + a.splits - 1) / a.splits + RT - 1) / RT * RT, begin = max(split * per, max(kg - s.prefix, 0) * a.group / RT * RT), end = min(split * per + per, rows);
   const int heads = a.kv * a.group;
   // rows r0 .. r0 + RT - 1 on their way, 8 elements a piece
-  Item8<XT> it[NL];
+  u32x4 it[NL][PARTS];
   f32x2 factor;
   auto ask_rows = [&](int r0) {
 #pragma unroll
     for (int i = 0; i < NL; i++) {
       const int e = i * 256 + tid, r = r0 + e / C, p = e % C;
-      it[i] = Item8<XT>{};
-      if (e < RT * C && r < end && p * 8 < a.D) {
-        const int token = r / a.group;
-        item_load<XT>(a.q, (s.first + token) * a.q_token + (h * a.group + r - token * a.group) * a.q_head + p * 8, it[i]);
+      const bool there = e < RT * C && r < end && p * 8 < a.D;
+      const int token = there ? r / a.group : 0, head = h * a.group + (there ? r - token * a.group : 0);
+#pragma unroll
+      for (int j = 0; j < PARTS; j++) {
+        it[i][j] = u32x4{0, 0, 0, 0};
+        if (!there) continue;
+        if (F32) it[i][j] = *reinterpret_cast<const u32x4*>(a.parts + (((int64_t)j * a.T + s.first + token) * heads + head) * a.D + p * 8);
+        else it[i][j] = *reinterpret_cast<const u32x4*>(reinterpret_cast<const uint16_t*>(a.q) + (s.first + token) * a.q_token + head * a.q_head + p * 8);
       }
     }
     if (tid < RT) {
@@ -406,10 +525,8 @@ __global__ __launch_bounds__(256, 2) void weights_mass_kernel(WeightArgs a) {
     for (int i = 0; i < NL; i++) {
       const int e = i * 256 + tid, r = e / C, p = e % C;
       if (RT * C % 256 && e >= RT * C) break;
-      at_bf16x8 part[PARTS];
-      item_parts<F32>(it[i], part);
 #pragma unroll
-      for (int j = 0; j < PARTS; j++) *reinterpret_cast<at_bf16x8*>(&s_q[half][j][r * DP + (p ^ swizzle<C>(r)) * 8]) = part[j];
+      for (int j = 0; j < PARTS; j++) *reinterpret_cast<u32x4*>(&s_q[half][j][r * DP + (p ^ swizzle<C>(r)) * 8]) = it[i][j];
     }
     if (tid < RT) s_row[half][tid] = factor;
   };
@@ -514,28 +631,30 @@ __global__ __launch_bounds__(256) void weights_add_kernel(WeightArgs a) {
 
 // ---- host side ------------------------------------------------------------------------------------------------------------
 struct WeightPlan {
-  bool few;
+  bool few, one;
   int rows, pitch, ranges, row_tiles, wr, splits, keys;
 };
 static WeightPlan weight_plan(bool f32, int64_t B, int heads, int kv, int D, int64_t max_tokens, int64_t max_keys) {
   WeightPlan p = {};
   const int64_t rows = max_tokens * (heads / kv);
   p.few = rows <= 16;
+  p.one = p.few && max_keys <= WEIGHT_ONE;
   p.rows = p.few ? (int)rows : 0;
   p.pitch = (int)((max_keys + 63) / 64 * 64);
   const int64_t wave = weight_nq(D > 128 ? 8 : 4, f32) * 16;
   p.wr = rows <= wave ? 1 : rows <= 2 * wave ? 2 : 4;
   p.row_tiles = p.few ? 1 : (int)((rows + p.wr * wave - 1) / (p.wr * wave));
-  const int64_t uncut = B * kv * p.row_tiles, most = (max_keys + 255) / 256, wanted = (1023 + uncut) / uncut;
+  const int64_t uncut = B * kv * p.row_tiles, most = (max_keys + 255) / 256, wanted = p.few ? (1023 + uncut) / uncut : (511 + uncut) / uncut;
   p.ranges = (int)(uncut >= 1024 || most < 2 ? 1 : wanted < most ? wanted : most);
   p.keys = D <= 128 ? Mass<4, false>::KEYS : f32 ? Mass<8, true>::KEYS : Mass<8, false>::KEYS;
   const int64_t groups = B * kv * ((max_keys + p.keys - 1) / p.keys), parts = (rows + 127) / 128, split = (511 + groups) / groups;
   p.splits = (int)(p.few || groups >= 512 || parts < 2 ? 1 : split < parts ? split : parts);
   return p;
 }
-static size_t weight_room(const WeightPlan& p, int64_t T, int64_t B, int heads, int kv) {
+static size_t weight_room(const WeightPlan& p, bool f32, int64_t T, int64_t B, int heads, int kv, int D) {
+  if (p.one) return 0;
   if (p.few) return ((size_t)B * kv * p.rows * p.pitch + (size_t)p.ranges * B * kv * p.rows * 2) * sizeof(float);
-  return ((size_t)(p.ranges > 1 ? p.ranges + 1 : 1) * T * heads * 2 + (p.splits > 1 ? (size_t)p.splits * B * kv * p.pitch : 0)) * sizeof(float);
+  return ((size_t)(p.ranges > 1 ? p.ranges + 1 : 1) * T * heads * 2 + (p.splits > 1 ? (size_t)p.splits * B * kv * p.pitch : 0)) * sizeof(float) + (f32 ? (size_t)T * heads * D * 6 : 0) + 16;
 }
 static bool weight_sizes(int dtype, int64_t T, int64_t B, int heads, int kv, int head_dim, int64_t max_tokens, int64_t max_keys) {
   return (dtype == MLLM_HIP_F32 || dtype == MLLM_HIP_BF16) && T >= 0 && B >= 0 && heads >= 1 && kv >= 1 && head_dim >= 1 && max_tokens >= 0 && max_keys >= 0;
@@ -553,7 +672,7 @@ MLLM_API size_t mllm_hip_attention_weights_workspace_bytes(int dtype, int64_t T,
   if (!weight_sizes(dtype, T, B, heads, kv_heads, head_dim, max_tokens, max_keys) || !weight_shape(T, B, heads, kv_heads, head_dim, max_tokens, max_keys)) return 0;
   if (T == 0 || B == 0 || max_tokens == 0 || max_keys == 0) return 0;
   if (max_tokens > T) max_tokens = T;
-  return weight_room(weight_plan(dtype == MLLM_HIP_F32, B, heads, kv_heads, head_dim, max_tokens, max_keys), T, B, heads, kv_heads);
+  return weight_room(weight_plan(dtype == MLLM_HIP_F32, B, heads, kv_heads, head_dim, max_tokens, max_keys), dtype == MLLM_HIP_F32, T, B, heads, kv_heads, head_dim);
 }
 
 MLLM_API int mllm_hip_attention_weights(const mllm_hip_heads* q, int dtype, int64_t T, const mllm_hip_kv_cache* cache, float* mass, int64_t mass_stride,
@@ -579,8 +698,8 @@ MLLM_API int mllm_hip_attention_weights(const mllm_hip_heads* q, int dtype, int6
   const int heads = q->heads, D = cache->head_dim;
   const bool f32 = dtype == MLLM_HIP_F32;
   const WeightPlan p = weight_plan(f32, B, heads, cache->heads, D, max_tokens, max_keys);
-  const size_t need = weight_room(p, T, B, heads, cache->heads);
-  if (!workspace || workspace_bytes < need) return MLLM_HIP_E_BADARG;
+  const size_t need = weight_room(p, f32, T, B, heads, cache->heads, D);
+  if (need && (!workspace || workspace_bytes < need)) return MLLM_HIP_E_BADARG;
   const int64_t groups = (B * cache->heads * p.ranges + 7) / 8 * 8;
   if (groups > 0xffffff / p.row_tiles) return MLLM_HIP_E_SHAPE;
   WeightArgs a = {};
@@ -635,17 +754,41 @@ MLLM_API int mllm_hip_attention_weights(const mllm_hip_heads* q, int dtype, int6
     else by_type(std::integral_constant<int, 8>());                                     \
     RC_RET((int)hipGetLastError());                                                     \
   }
+  if (p.one) {
+    // (blocks of 512 threads: the launches below have 256)
+    const size_t lds = (size_t)p.rows * WEIGHT_PITCH * sizeof(float);
+    auto one = [&](auto ks) {
+      constexpr int KS = decltype(ks)::value;
+      if (f32) hipLaunchKernelGGL((weights_one_kernel<KS, true>), dim3(heads_of_all), dim3(512), lds, st, a);
+      else hipLaunchKernelGGL((weights_one_kernel<KS, false>), dim3(heads_of_all), dim3(512), lds, st, a);
+    };
+    if (D <= 64) one(std::integral_constant<int, 2>());
+    else if (D <= 96) one(std::integral_constant<int, 3>());
+    else if (D <= 128) one(std::integral_constant<int, 4>());
+    else one(std::integral_constant<int, 8>());
+    return (int)hipGetLastError();
+  }
   if (p.few) {
     a.score = reinterpret_cast<float*>(workspace);
     a.ml = reinterpret_cast<f32x2*>(a.score + (size_t)B * cache->heads * p.rows * p.pitch);
     KSTEPS(dim3((unsigned)p.ranges, heads_of_all), weights_scores_kernel<KS, F32>)
-    hipLaunchKernelGGL(weights_sum_kernel, dim3((unsigned)((max_keys + 255) / 256), heads_of_all), dim3(256), 0, st, a);
+    const dim3 sums((unsigned)((max_keys + 255) / 256), heads_of_all);
+    if (p.rows <= 2) hipLaunchKernelGGL(weights_sum_kernel<2>, sums, dim3(256), 0, st, a);
+    else if (p.rows <= 4) hipLaunchKernelGGL(weights_sum_kernel<4>, sums, dim3(256), 0, st, a);
+    else if (p.rows <= 8) hipLaunchKernelGGL(weights_sum_kernel<8>, sums, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL(weights_sum_kernel<16>, sums, dim3(256), 0, st, a);
     return (int)hipGetLastError();
   }
   a.row = reinterpret_cast<f32x2*>(workspace);
   a.ml = a.row + (size_t)T * heads;
   a.part = reinterpret_cast<float*>(a.row + (size_t)(p.ranges > 1 ? p.ranges + 1 : 1) * T * heads);
   a.splits = p.splits;
+  if (f32) {
+    const uintptr_t behind = reinterpret_cast<uintptr_t>(a.part) + (p.splits > 1 ? (size_t)p.splits * B * cache->heads * p.pitch * sizeof(float) : 0);
+    a.parts = reinterpret_cast<uint16_t*>((behind + 15) / 16 * 16);
+    hipLaunchKernelGGL(weights_parts_kernel, dim3((unsigned)((T * heads * (D / 8) + 255) / 256)), dim3(256), 0, st, a);
+    RC_RET((int)hipGetLastError());
+  }
   const dim3 grid((unsigned)(groups * p.row_tiles));
   if (p.wr == 1) KSTEPS(grid, weights_max_kernel<KS, 1, F32>)
   else if (p.wr == 2) KSTEPS(grid, weights_max_kernel<KS, 2, F32>)

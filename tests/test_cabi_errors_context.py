@@ -108,7 +108,7 @@ def _weights(q=None, cache=None, dtype=BF16, T=2, mass=P, stride=2000, head=500,
     (dict(q=_part(heads=6)), SHAPE), (dict(q=_part(heads=8, x=None)), BADARG), (dict(q=_part(heads=8, x=ODD)), ALIGN), (dict(q=_part(heads=8, x_token_stride=516)), ALIGN),
     (dict(cache=_cache(head_dim=100)), SHAPE), (dict(cache=_cache(head_dim=264)), SHAPE), (dict(cache=_cache(k=None)), BADARG), (dict(cache=_cache(k=ODD)), ALIGN), (dict(cache=_cache(slot_stride=4)), ALIGN),
     (dict(cache=_cache(pages=0)), BADARG), (dict(cache=_cache(pages=1 << 27)), SHAPE), (dict(mass=ODD), ALIGN), (dict(table=ODD), ALIGN), (dict(cu=ODD), ALIGN), (dict(prefix=ODD), ALIGN),
-    (dict(work=P + 8), ALIGN), (dict(work=None), BADARG), (dict(size=100), BADARG), (dict(T=0), 0), (dict(B=0), 0), (dict(tokens=0), 0), (dict(keys=0), 0)])
+    (dict(work=P + 8), ALIGN), (dict(keys=4000, work=None), BADARG), (dict(keys=4000, size=100), BADARG), (dict(T=0), 0), (dict(B=0), 0), (dict(tokens=0), 0), (dict(keys=0), 0)])
 def test_attention_weights(args, want):
     assert _weights(**args) == want
 

@@ -212,6 +212,6 @@ def test_nothing_and_refusals():
         with pytest.raises((AssertionError, TypeError)):
             ql.attention_weights(**dict(a, **bad))
     for bad in (dict(q=torch.zeros((5, 3, 64), device="cuda")), dict(scale=0.0), dict(scale=float("inf")), dict(decay=-0.5), dict(decay=float("nan")), dict(max_tokens=-1), dict(max_keys=-1),
-                dict(max_keys=1 << 31), dict(workspace=torch.empty(16, dtype=torch.uint8, device="cuda")), dict(block_table=_int(c.table)[:, :0])):
+                dict(max_keys=1 << 31), dict(workspace=torch.empty(16, dtype=torch.uint8, device="cuda"), max_keys=5000), dict(block_table=_int(c.table)[:, :0])):
         with pytest.raises(_lib.HipQLinearError):
             ql.attention_weights(**dict(a, **bad))
