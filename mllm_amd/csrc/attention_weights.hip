@@ -87,29 +87,38 @@ __device__ __forceinline__ void put_mass(const WeightArgs& a, const WeightSeq& s
   *mass = key < s.prefix && a.decay != 0.f ? a.decay * *mass + v : v;
 }
 
-// Scores (times 1) of 16 keys and 16 rows.  With fp32 queries an infinite element of a key makes a NaN with the second and third part of a query's, which may be 0: it
-// counts with the first alone, which has the sign.  Such scores, and those that are NaN anyway, are formed once more.
+// Scores (times 1) of 16 keys and 16 rows
 template <int KS, bool F32>
-__device__ __forceinline__ at_f32x4 key_scores(const u32x4 (&k)[KS], const at_bf16x8 (&q)[KS][F32 ? 3 : 1]) {
+__device__ __forceinline__ at_f32x4 raw_scores(const u32x4 (&k)[KS], const at_bf16x8 (&q)[KS][F32 ? 3 : 1]) {
   at_f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
   for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-    for (int p = (F32 ? 3 : 1) - 1; p >= 0; p--) s = mma(frag(k[ks]), q[ks][p], s);
+    for (int p = (F32 ? 3 : 1) - 1; p >= 0; p--) s = mma(frag(k[ks]), q[ks][p], s);  // the smallest part first
+  return s;
+}
+// With fp32 queries an infinite element of a key makes a NaN with the second and third part of a query's, which may be 0: it counts with the first alone, which has the sign.  Scores that
+// are NaN are formed once more like this.  (The keys go through an asm: what follows from them would else be worked out in front of the branch that leads here, and be most of the instructions.)
+template <int KS>
+__device__ __forceinline__ at_f32x4 scores_again(const u32x4 (&k)[KS], const at_bf16x8 (&q)[KS][3]) {
+  at_f32x4 s = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int ks = 0; ks < KS; ks++) {
+    u32x4 x = k[ks];
+    asm volatile("" : "+v"(x));
+    const at_bf16x8 f = frag(u32x4{finite_pair(x.x), finite_pair(x.y), finite_pair(x.z), finite_pair(x.w)});
+    s = mma(f, q[ks][2], s);
+    s = mma(f, q[ks][1], s);
+    s = mma(frag(x), q[ks][0], s);
+  }
+  return s;
+}
+template <int KS, bool F32>
+__device__ __forceinline__ at_f32x4 key_scores(const u32x4 (&k)[KS], const at_bf16x8 (&q)[KS][F32 ? 3 : 1]) {
+  at_f32x4 s = raw_scores<KS, F32>(k, q);
   if constexpr (F32) {
     const float all = (s[0] + s[1]) + (s[2] + s[3]);
-    if (__builtin_expect(__ballot(all != all) != 0, 0)) {
-      s = at_f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int ks = 0; ks < KS; ks++) {
-        u32x4 x = k[ks];
-        asm volatile("" : "+v"(x));  // (worked out here and not in front of the branch, where it was most of the kernel's instructions)
-        const at_bf16x8 f = frag(u32x4{finite_pair(x.x), finite_pair(x.y), finite_pair(x.z), finite_pair(x.w)});
-        s = mma(f, q[ks][2], s);
-        s = mma(f, q[ks][1], s);
-        s = mma(frag(k[ks]), q[ks][0], s);
-      }
-    }
+    if (__builtin_expect(__ballot(all != all) != 0, 0)) s = scores_again<KS>(k, q);
   }
   return s;
 }
@@ -392,27 +401,48 @@ __global__ __launch_bounds__(256, 2) void weights_max_kernel(WeightArgs a) {
   auto work = [&](int k0, auto border_, int half) {
     constexpr bool border = decltype(border_)::value;
     at_f32x4 y[NB][NQ];
-#pragma unroll
-    for (int u = 0; u < NB; u++) {
+    auto load = [&](int u, u32x4 (&k)[KS]) {
       const int row = half * KT + (u * WK + wk) * 16 + col, x = swizzle<C>(row);
-      u32x4 k[KS];
 #pragma unroll
       for (int ks = 0; ks < KS; ks++) k[ks] = *reinterpret_cast<const u32x4*>(s_k + row * DP + ((4 * ks + g) ^ x) * 8);
+    };
+    auto mask = [&](int u, int i) {
+      if (!border) return;
+      const int seen = token[i] < 0 ? 0 : min(s.prefix + token[i] + 1, end) - (k0 + (u * WK + wk) * 16 + 4 * g);
+#pragma unroll
+      for (int j = 0; j < 4; j++) y[u][i][j] = j < seen ? y[u][i][j] : -INFINITY;
+    };
+    auto highest = [&](int i) {
+      float top = -INFINITY;
+#pragma unroll
+      for (int u = 0; u < NB; u++) top = larger(larger(y[u][i][0], y[u][i][1]), larger(larger(y[u][i][2], y[u][i][3]), top));
+      return top;
+    };
+#pragma unroll
+    for (int u = 0; u < NB; u++) {
+      u32x4 k[KS];
+      load(u, k);
 #pragma unroll
       for (int i = 0; i < NQ; i++) {
-        y[u][i] = key_scores<KS, F32>(k, q[i]);
-        if (border) {
-          const int seen = min(s.prefix + token[i] + 1, end) - (k0 + (u * WK + wk) * 16 + 4 * g);
-#pragma unroll
-          for (int j = 0; j < 4; j++) y[u][i][j] = j < seen && token[i] >= 0 ? y[u][i][j] : -INFINITY;
-        }
+        y[u][i] = raw_scores<KS, F32>(k, q[i]);
+        mask(u, i);
       }
     }
 #pragma unroll
     for (int i = 0; i < NQ; i++) {
-      float top = -INFINITY;
+      float top = highest(i);  // (a NaN is handed on)
+      if constexpr (F32) {
+        if (__builtin_expect(__ballot(top != top) != 0, 0)) {
 #pragma unroll
-      for (int u = 0; u < NB; u++) top = larger(top, larger(larger(y[u][i][0], y[u][i][1]), larger(y[u][i][2], y[u][i][3])));
+          for (int u = 0; u < NB; u++) {
+            u32x4 k[KS];
+            load(u, k);
+            y[u][i] = scores_again<KS>(k, q[i]);
+            mask(u, i);
+          }
+          top = highest(i);
+        }
+      }
       const float next = larger(m[i], top * a.c), ref = next == -INFINITY ? 0.f : next;
       float sum = 0.f;
 #pragma unroll
@@ -564,20 +594,22 @@ __global__ __launch_bounds__(256, 2) void weights_mass_kernel(WeightArgs a) {
           for (int i = 0; i < NK; i++) y[i] = mma(frag(k[i][ks]), q, y[i]);
         }
       }
-      if constexpr (F32) {  // (as in key_scores)
+      if constexpr (F32) {  // (as in scores_again)
+        float all = 0.f;
 #pragma unroll
-        for (int i = 0; i < NK; i++) {
-          const float all = (y[i][0] + y[i][1]) + (y[i][2] + y[i][3]);
-          if (__builtin_expect(__ballot(all != all) != 0, 0)) {
+        for (int i = 0; i < NK; i++) all += (y[i][0] + y[i][1]) + (y[i][2] + y[i][3]);
+        if (__builtin_expect(__ballot(all != all) != 0, 0)) {  // (infinities of both signs make one too: formed once more to no harm)
+#pragma unroll
+          for (int i = 0; i < NK; i++) {
             y[i] = at_f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int ks = 0; ks < KS; ks++) {
-              u32x4 x = k[i][ks];
-              asm volatile("" : "+v"(x));
-              const at_bf16x8 f = frag(u32x4{finite_pair(x.x), finite_pair(x.y), finite_pair(x.z), finite_pair(x.w)});
+              u32x4 f4 = k[i][ks];
+              asm volatile("" : "+v"(f4));
+              const at_bf16x8 f = frag(u32x4{finite_pair(f4.x), finite_pair(f4.y), finite_pair(f4.z), finite_pair(f4.w)});
               y[i] = mma(f, query(ks, 2), y[i]);
               y[i] = mma(f, query(ks, 1), y[i]);
-              y[i] = mma(frag(k[i][ks]), query(ks, 0), y[i]);
+              y[i] = mma(frag(f4), query(ks, 0), y[i]);
             }
           }
         }
