@@ -569,9 +569,12 @@ __global__ __launch_bounds__(256, DK <= 6 ? 3 : 2) void cross_wide_kernel(CrossA
       cross_put<false>(a, place, row, token, head, 32 * d + 8 * j + 4 * g, at_f32x4{acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]}, m, l);
 }
 
-// Joins the pieces of a row: 16 bytes of it per lane, L lanes a row
-template <int L, bool F32>
+// Joins the pieces of a row: 16 bytes of it per lane, L lanes a row, G groups of lanes along the pieces
+template <int L, bool F32, int G>
 __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
+  constexpr int PER = 256 / L / G;
+  __shared__ at_f32x4 s_x[G > 1 ? 256 : 1];
+  __shared__ float s_ml[G > 1 ? 256 / L * 2 : 1];
   const int tid = threadIdx.x, d = tid % L * 4, tile = blockIdx.y;
   int place, rt;
   cross_tile(a, a.whole + tile, place, rt);
@@ -579,32 +582,55 @@ __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
   const CrossSeq s = cross_sequence(a, b);
   int per, pieces;
   cut(a, s.keys, per, pieces);
-  const int i = blockIdx.x * (256 / L) + tid / L, row = rt * a.rows_of_tile + i;
-  if (pieces < 2 || i >= a.rows_of_tile || row >= s.n * a.group || d >= a.D) return;
+  const int i = blockIdx.x * PER + tid / L % PER, group = tid / L / PER, row = rt * a.rows_of_tile + i;
+  if (pieces < 2) return;
+  const bool live = i < a.rows_of_tile && row < s.n * a.group && d < a.D;
   const int64_t all = (int64_t)(a.tiles - a.whole) * a.rows_of_tile, at = (int64_t)tile * a.rows_of_tile + i;
   float m = -INFINITY, sum = 0.f;
   at_f32x4 x = {0.f, 0.f, 0.f, 0.f};
-  constexpr int U = 8;
-  for (int k = 0; k < pieces; k += U) {
-    float mk[U], lk[U];
-    at_f32x4 xk[U];
+  if (live) {
+    constexpr int U = 4;
+    for (int k = group; k < pieces; k += U * G) {
+      float mk[U], lk[U];
+      at_f32x4 xk[U];
 #pragma unroll
-    for (int j = 0; j < U; j++) {
-      const int64_t from = min(k + j, pieces - 1) * all + at;
-      mk[j] = a.part_ml[2 * from];
-      lk[j] = a.part_ml[2 * from + 1];
-      xk[j] = *reinterpret_cast<const at_f32x4*>(a.part_o + from * a.D + d);
-    }
+      for (int j = 0; j < U; j++) {
+        const int64_t from = min(k + j * G, pieces - 1) * all + at;
+        mk[j] = a.part_ml[2 * from];
+        lk[j] = a.part_ml[2 * from + 1];
+        xk[j] = *reinterpret_cast<const at_f32x4*>(a.part_o + from * a.D + d);
+      }
 #pragma unroll
-    for (int j = 0; j < U; j++) {
-      if (k + j >= pieces) break;
-      const float next = fmaxf(m, mk[j]), ref = next == -INFINITY ? 0.f : next;
-      const float f = __builtin_amdgcn_exp2f(m - ref), fk = __builtin_amdgcn_exp2f(mk[j] - ref);
-      x = x * f + xk[j] * fk;
-      sum = sum * f + lk[j] * fk;
-      m = next;
+      for (int j = 0; j < U; j++) {
+        if (k + j * G >= pieces) break;
+        const float next = fmaxf(m, mk[j]), ref = next == -INFINITY ? 0.f : next;
+        const float f = __builtin_amdgcn_exp2f(m - ref), fk = __builtin_amdgcn_exp2f(mk[j] - ref);
+        x = x * f + xk[j] * fk;
+        sum = sum * f + lk[j] * fk;
+        m = next;
+      }
     }
   }
+  if constexpr (G > 1) {
+    s_x[tid] = x;
+    if (d == 0) {
+      s_ml[tid / L * 2] = m;
+      s_ml[tid / L * 2 + 1] = sum;
+    }
+    __syncthreads();
+    if (group) return;
+    float top = -INFINITY;
+    for (int k = 0; k < G; k++) top = fmaxf(top, s_ml[(k * PER + tid / L) * 2]);
+    const float ref = top == -INFINITY ? 0.f : top;
+    x = at_f32x4{0.f, 0.f, 0.f, 0.f};
+    sum = 0.f;
+    for (int k = 0; k < G; k++) {
+      const float f = __builtin_amdgcn_exp2f(s_ml[(k * PER + tid / L) * 2] - ref);
+      x += s_x[tid + k * PER * L] * f;
+      sum += s_ml[(k * PER + tid / L) * 2 + 1] * f;
+    }
+  }
+  if (!live) return;
   x *= sum > 0.f ? 1.0f / sum : (sum == 0.f ? 0.f : sum);
   const int t = row / a.group;
   const int64_t to = (s.first + t) * a.o_token + (h * a.group + row - t * a.group) * a.o_head + d;
@@ -739,16 +765,22 @@ MLLM_API int mllm_hip_attention_cross(const mllm_hip_heads* q, int dtype, int64_
 #undef CROSS
   RC_RET((int)hipGetLastError());
   if (rest) {
-    const int lanes = D <= 64 ? 16 : D <= 128 ? 32 : 64, per = 256 / lanes;
+    const bool many = p.pieces >= 8;  // lanes along the pieces
+    const int lanes = D <= 64 ? 16 : D <= 128 ? 32 : 64, per = many ? 1 : 256 / lanes;
     const int64_t rows = max_tokens * a.group, most = rows < p.rows_of_tile ? rows : p.rows_of_tile;
     const dim3 jgrid((unsigned)((most + per - 1) / per), (unsigned)rest);
     auto join = [&](auto kern) { hipLaunchKernelGGL(kern, jgrid, dim3(256), 0, st, a); };
-#define JOIN(L_)                              \
-  if (f32) join(cross_join_kernel<L_, true>); \
-  else join(cross_join_kernel<L_, false>)
-    if (lanes == 16) { JOIN(16); }
-    else if (lanes == 32) { JOIN(32); }
-    else { JOIN(64); }
+#define JOIN(L_)                                                              \
+  if (many) {                                                                 \
+    if (f32) join(cross_join_kernel<L_, true, 256 / L_>);                     \
+    else join(cross_join_kernel<L_, false, 256 / L_>);                        \
+  } else {                                                                    \
+    if (f32) join(cross_join_kernel<L_, true, 1>);                            \
+    else join(cross_join_kernel<L_, false, 1>);                               \
+  }
+    if (lanes == 16) { JOIN(16) }
+    else if (lanes == 32) { JOIN(32) }
+    else { JOIN(64) }
 #undef JOIN
   }
   return (int)hipGetLastError();
