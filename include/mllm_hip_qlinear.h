@@ -708,7 +708,7 @@ int mllm_hip_attention_weights(const mllm_hip_heads* q, int dtype, int64_t T, co
  * All of them where there are no more than that.  They go, in their order, to places 0, 1, .. of the pages in to_table (int32 [B][to_len], to_stride apart), keys and values;
  * kept int32 [B][heads][keep] are their positions (-1 behind the last), kept_mass fp32 [B][heads][keep] their mass (0), apart from mass itself.  Nothing else changes: pages that other
  * sequences share stay whole.  No page of to_table may be one that block_table has, or twice in it.  A page of block_table outside the cache reads as zeros, one of to_table
- * stores nothing.  first + recent <= keep <= to_len * page_size; head_dim % 8 == 0, <= 512; B * heads <= 65535.  Two launches, no workspace. */
+ * stores nothing.  first + recent <= keep <= to_len * page_size; both tables up to 2^30 positions; head_dim % 8 == 0, <= 512; B * heads <= 65535.  Two launches, no workspace. */
 int mllm_hip_kv_evict(const mllm_hip_kv_cache* cache, const float* mass, int64_t mass_stride, int64_t mass_head_stride, int64_t mass_len, const int32_t* block_table,
                       int64_t table_stride, int64_t table_len, const int32_t* lengths, int64_t B, const int32_t* to_table, int64_t to_stride, int64_t to_len, int64_t keep,
                       int64_t first, int64_t recent, int32_t* kept, float* kept_mass, void* stream);

@@ -207,7 +207,7 @@ MLLM_API int mllm_hip_kv_evict(const mllm_hip_kv_cache* cache, const float* mass
     return MLLM_HIP_E_BADARG;
   if (cache->head_dim % 8 || cache->head_dim > 512 || cache->heads > 65536 || cache->pages > 0x7fffffff / cache->page_size || cache->page_stride < 0 || cache->slot_stride < 0 ||
       cache->page_stride > 0x7fffffff || cache->slot_stride > 0x3fffffff / cache->page_size || (cache->slot_stride == 0 && cache->page_size > 1) ||
-      table_len > 0x7fff0000 / cache->page_size || to_len > 0x7fff0000 / cache->page_size || B > 65535 / cache->heads || keep > to_len * cache->page_size)
+      table_len > 0x40000000 / cache->page_size || to_len > 0x40000000 / cache->page_size || B > 65535 / cache->heads || keep > to_len * cache->page_size)
     return MLLM_HIP_E_SHAPE;
   if (B == 0 || keep == 0) return 0;
   if ((mass_len && !mass) || (table_len && !block_table) || !lengths || !to_table || !kept || !kept_mass || kept_mass == mass) return MLLM_HIP_E_BADARG;

@@ -122,7 +122,7 @@ def _evict(cache=None, mass=P, stride=2000, head=500, n=500, table=P, table_len=
     (dict(no_cache=True), BADARG), (dict(cache=_cache(k=None)), BADARG), (dict(cache=_cache(v=None)), BADARG), (dict(cache=_cache(v=ODD)), ALIGN), (dict(cache=_cache(head_dim=100)), SHAPE),
     (dict(cache=_cache(head_dim=520)), SHAPE), (dict(cache=_cache(heads=0)), BADARG), (dict(cache=_cache(page_stride=100)), ALIGN), (dict(cache=_cache(pages=1 << 27)), SHAPE), (dict(mass=None), BADARG),
     (dict(mass=ODD), ALIGN), (dict(n=-1), BADARG), (dict(table=None), BADARG), (dict(table=ODD), ALIGN), (dict(table_len=-1), BADARG), (dict(lengths=None), BADARG), (dict(lengths=ODD), ALIGN),
-    (dict(B=-1), BADARG), (dict(B=1 << 14), SHAPE), (dict(to=None), BADARG), (dict(to=ODD), ALIGN), (dict(to_len=-1), BADARG), (dict(to_len=2), SHAPE), (dict(keep=65), SHAPE), (dict(keep=-1), BADARG),
+    (dict(B=-1), BADARG), (dict(B=1 << 14), SHAPE), (dict(to=None), BADARG), (dict(to=ODD), ALIGN), (dict(to_len=-1), BADARG), (dict(to_len=2), SHAPE), (dict(table_len=1 << 27), SHAPE), (dict(to_len=1 << 27), SHAPE), (dict(keep=65), SHAPE), (dict(keep=-1), BADARG),
     (dict(keep=11), BADARG), (dict(first=-1), BADARG), (dict(first=41), BADARG), (dict(recent=-1), BADARG), (dict(recent=1 << 62), BADARG), (dict(kept=None), BADARG), (dict(kept=ODD), ALIGN),
     (dict(kept_mass=None), BADARG), (dict(kept_mass=ODD), ALIGN), (dict(kept_mass=P), BADARG), (dict(B=0), 0), (dict(keep=0, first=0, recent=0), 0)])
 def test_kv_evict(args, want):
