@@ -27,14 +27,13 @@ struct EvictArgs {
 
 enum { EVICT_WG = 1024, EVICT_HELD = 16, EVICT_BINS = 2048 };
 
-// larger weights, larger numbers; -0 as 0, a NaN below all
+// larger weights, larger numbers; -0 as 0, a NaN below all numbers.  0 and ~0 are no weight's: a position that is not there, and one that stays whatever its weight.
 __device__ __forceinline__ uint32_t weight_order(float v) {
-  if (v != v) return 0;
   const uint32_t b = __float_as_uint(v + 0.0f);
-  return b & 0x80000000u ? ~b : b | 0x80000000u;
+  return v != v ? 1 : b & 0x80000000u ? ~b : b | 0x80000000u;
 }
 
-// Each wave has a run of the positions, 64 at a time a lane each.  HELD: up to EVICT_HELD of 64, which stay in registers; else they are read again every time.
+// Each wave has a run of the positions, 64 at a time a lane each.  HELD: up to EVICT_HELD of 64, whose order stays in registers; else it is worked out again every time.
 template <bool HELD>
 __device__ __forceinline__ void evict_select(const EvictArgs& a, const float* mass, int n, int32_t* kept, float* kept_mass) {
   __shared__ uint32_t s_bin[EVICT_BINS];
@@ -44,19 +43,25 @@ __device__ __forceinline__ void evict_select(const EvictArgs& a, const float* ma
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int lo = a.first, hi = n - a.recent;  // the ones that go by their weights: more of them than `want`
   uint32_t want = a.keep - a.first - a.recent;
-  const bool none = want == 0;
   const int share = (n + EVICT_WG - 1) / EVICT_WG, from = wave * share * 64 + lane;  // in 64s
-  float v[HELD ? EVICT_HELD : 1];
+  auto order_of = [&](int i, float w) { return i >= n ? 0u : i < lo || i >= hi ? ~0u : weight_order(w); };
+  uint32_t k[HELD ? EVICT_HELD : 1];
   if constexpr (HELD) {
+    float w[EVICT_HELD];
 #pragma unroll
-    for (int j = 0; j < EVICT_HELD; j++) v[j] = j < share && from + 64 * j < n ? mass[from + 64 * j] : 0.f;
+    for (int j = 0; j < EVICT_HELD; j++) w[j] = j < share && from + 64 * j < n ? mass[from + 64 * j] : 0.f;
+    for (int i = tid; i < EVICT_BINS; i += EVICT_WG) s_bin[i] = 0;
+#pragma unroll
+    for (int j = 0; j < EVICT_HELD; j++) k[j] = j < share ? order_of(from + 64 * j, w[j]) : 0;
+  } else {
+    for (int i = tid; i < EVICT_BINS; i += EVICT_WG) s_bin[i] = 0;
   }
-  // f(position, weight) of every one of this lane's positions, the wave's 64 together
+  // f(position, order) of every one of this lane's positions, the wave's 64 together
   auto each = [&](auto f) {
     if constexpr (HELD) {
 #pragma unroll
       for (int j = 0; j < EVICT_HELD; j++)
-        if (j < share) f(from + 64 * j, v[j]);
+        if (j < share) f(from + 64 * j, k[j]);
     } else {
       constexpr int U = 8;
       for (int j0 = 0; j0 < share; j0 += U) {
@@ -65,83 +70,78 @@ __device__ __forceinline__ void evict_select(const EvictArgs& a, const float* ma
         for (int j = 0; j < U; j++) w[j] = j0 + j < share && from + 64 * (j0 + j) < n ? mass[from + 64 * (j0 + j)] : 0.f;
 #pragma unroll
         for (int j = 0; j < U; j++)
-          if (j0 + j < share) f(from + 64 * (j0 + j), w[j]);
+          if (j0 + j < share) f(from + 64 * (j0 + j), order_of(from + 64 * (j0 + j), w[j]));
       }
     }
   };
-  // the want-th largest: `prefix` are its digits so far, `want` which one it is among the weights that begin with them
+  // The want-th largest: `prefix` are its digits so far, `want` which one it is among those that begin with them.  (No weight begins with the eleven ones of ~0; positions that
+  // are not there are below all.)
   uint32_t prefix = 0;
   const int shifts[3] = {21, 10, 0}, bits[3] = {11, 11, 10};
-#pragma unroll
-  for (int i = tid; i < EVICT_BINS; i += EVICT_WG) s_bin[i] = 0;
   __syncthreads();
+  if (want == 0) {
+    prefix = ~1u;  // between the ones that stay and all weights
+  } else {
 #pragma unroll
-  for (int d = 0; d < 3; d++) {
-    each([&](int i, float w) {
-      const uint32_t k = weight_order(w);
-      if (i >= lo && i < hi && (d == 0 || k >> (shifts[d] + bits[d]) == prefix)) atomicAdd(&s_bin[k >> shifts[d] & ((1u << bits[d]) - 1)], 1u);
-    });
-    __syncthreads();
-    // bins from the largest down, two a thread: the one that the want-th is in
-    const int top = EVICT_BINS - 1 - 2 * tid;
-    const uint32_t c0 = s_bin[top], c1 = s_bin[top - 1];
-    uint32_t up = c0 + c1;
+    for (int d = 0; d < 3; d++) {
+      each([&](int, uint32_t x) {
+        if (d == 0 ? x != 0 && x != ~0u : x >> (shifts[d] + bits[d]) == prefix) atomicAdd(&s_bin[x >> shifts[d] & ((1u << bits[d]) - 1)], 1u);
+      });
+      __syncthreads();
+      // bins from the largest down, two a thread: the one that the want-th is in
+      const int top = EVICT_BINS - 1 - 2 * tid;
+      const uint32_t c0 = s_bin[top], c1 = s_bin[top - 1];
+      uint32_t up = c0 + c1;
 #pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-      const uint32_t o = __shfl_up(up, s);
-      up += lane >= s ? o : 0;
-    }
-    if (lane == 63) s_wave[0][wave] = up;
-    s_bin[top] = s_bin[top - 1] = 0;  // (by the thread that has read them: for the next digit)
-    __syncthreads();
-    uint32_t front = up - c0 - c1;
+      for (int s = 1; s < 64; s <<= 1) {
+        const uint32_t o = __shfl_up(up, s);
+        up += lane >= s ? o : 0;
+      }
+      if (lane == 63) s_wave[0][wave] = up;
+      s_bin[top] = s_bin[top - 1] = 0;  // (by the thread that has read them: for the next digit)
+      __syncthreads();
+      uint32_t front = up - c0 - c1;
 #pragma unroll
-    for (int w = 0; w < WAVES; w++) front += w < wave ? s_wave[0][w] : 0;
-    if (want && front < want && want <= front + c0 + c1) {
-      const bool first = want <= front + c0;
-      s_found[0] = first ? top : top - 1;
-      s_found[1] = want - front - (first ? 0 : c0);
-    }
-    __syncthreads();
-    if (want) {
+      for (int w = 0; w < WAVES; w++) front += w < wave ? s_wave[0][w] : 0;
+      if (front < want && want <= front + c0 + c1) {
+        const bool first = want <= front + c0;
+        s_found[0] = first ? top : top - 1;
+        s_found[1] = want - front - (first ? 0 : c0);
+      }
+      __syncthreads();
       prefix = prefix << bits[d] | s_found[0];
       want = s_found[1];
     }
   }
   // of weights that equal the border the first `want` stay
-  auto above = [&](int i, uint32_t k) { return i < n && (i < lo || i >= hi || (!none && k > prefix)); };
-  auto equal = [&](int i, uint32_t k) { return i >= lo && i < hi && !none && k == prefix; };
-  uint32_t n_above = 0, n_equal = 0;
-  each([&](int i, float w) {
-    const uint32_t k = weight_order(w);
-    n_above += __popcll(__ballot(above(i, k)));
-    n_equal += __popcll(__ballot(equal(i, k)));
+  uint32_t above = 0, equal = 0;
+  each([&](int, uint32_t x) {
+    above += __popcll(__ballot(x > prefix));
+    equal += __popcll(__ballot(x == prefix));
   });
   __syncthreads();
   if (lane == 0) {
-    s_wave[0][wave] = n_above;
-    s_wave[1][wave] = n_equal;
+    s_wave[0][wave] = above;
+    s_wave[1][wave] = equal;
   }
   __syncthreads();
-  n_above = n_equal = 0;
+  above = equal = 0;
 #pragma unroll
   for (int w = 0; w < WAVES; w++) {
-    n_above += w < wave ? s_wave[0][w] : 0;
-    n_equal += w < wave ? s_wave[1][w] : 0;
+    above += w < wave ? s_wave[0][w] : 0;
+    equal += w < wave ? s_wave[1][w] : 0;
   }
   const uint64_t below = (1ull << lane) - 1;
-  each([&](int i, float w) {
-    const uint32_t k = weight_order(w);
-    const bool is_above = above(i, k), is_equal = equal(i, k);
-    const uint64_t va = __ballot(is_above), ve = __ballot(is_equal);
-    const uint32_t e = n_equal + __popcll(ve & below);  // equal ones in front
-    if (is_above || (is_equal && e < want)) {
-      const uint32_t at = n_above + __popcll(va & below) + min(e, want);
+  each([&](int i, uint32_t x) {
+    const uint64_t va = __ballot(x > prefix), ve = __ballot(x == prefix);
+    const uint32_t e = equal + __popcll(ve & below);  // equal ones in front
+    if (x > prefix || (x == prefix && e < want)) {
+      const uint32_t at = above + __popcll(va & below) + min(e, want);
       kept[at] = i;
-      kept_mass[at] = w;
+      kept_mass[at] = mass[i];
     }
-    n_above += __popcll(va);
-    n_equal += __popcll(ve);
+    above += __popcll(va);
+    equal += __popcll(ve);
   });
 }
 
