@@ -409,11 +409,13 @@ __global__ __launch_bounds__(256, (Cross<DP, DT, NQ, WR, F32>::WAVES)) void cros
 // Keys and values go from memory to LDS directly.  FULL: heads of 16 DK elements.
 template <int DK, int DT>
 struct Wide {
-  static constexpr int C = 2 * DK, DP = 16 * DK, KT = 64;
-  static constexpr int CHUNKS = KT * C / 64;  // 64 pieces each, a wave's load
-  // Eight lanes of a key operand have rows 0 - 3 and 8 - 11 (or 4 - 7 and 12 - 15) and one piece, 16 of a value operand four rows and two pieces: in different banks.
+  static constexpr int C = DK == 5 ? 12 : 2 * DK, DP = 8 * C, KT = 64;  // (pieces of a row in LDS: ten of them would lie in the same banks every third row)
+  static constexpr int CHUNKS = KT * C / 64;                            // 64 pieces each, a wave's load
+  static constexpr bool ONES = DK == 5;                                 // the tiles of 32 of the second product reach behind the values: what lies there is 1, and O has the sum of the weights
+  // Eight lanes of a key operand have rows 0 - 3 and 8 - 11 (or 4 - 7 and 12 - 15) and one piece, 32 of a value operand four rows and the four pieces of a tile of 32: each in banks of their own.
+  // A KB of values, pitch 10 / 12 / 16 / 16 pieces with rows exclusive-ored by 0 / row / 4 / row / 0 / 4 (row % 4): 3.4 / 2.0 / 6.8 / 1.9 ns.
   static __device__ __forceinline__ int swz(int row) {
-    return C == 16 ? (row & 7) << 1 | ((row >> 3) & 1) : C == 12 ? (row >> 2) & 3 : C == 10 ? (row >> 3) & 1 : ((row >> 1) & 3) << 1 | ((row >> 3) & 1);
+    return C == 16 ? (row & 3) << 2 | ((row >> 2) & 1) << 1 | ((row >> 3) & 1) : C == 12 ? (row >> 2) & 3 : ((row >> 1) & 1) << 2 | ((row >> 2) & 1) << 1 | ((row >> 3) & 1);
   }
 };
 typedef float at_f32x16 __attribute__((ext_vector_type(16)));
@@ -437,7 +439,7 @@ __global__ __launch_bounds__(256, DK <= 6 ? 3 : 2) void cross_wide_kernel(CrossA
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), col = lane & 31, g = lane >> 5;
 
   // Two waves load keys and two values, half of a tile each: chunks of 64 pieces one behind the other in LDS, of which a lane loads the one that swz puts there.  Pieces behind a head's
-  // end are zeros from the beginning.
+  // end are zeros (ones, where O has the sum) from the beginning.
   constexpr int NLOAD = CHUNKS / 2;
   const bool keys = wave < 2;
   const int real = a.D / 8;
@@ -449,9 +451,11 @@ __global__ __launch_bounds__(256, DK <= 6 ? 3 : 2) void cross_wide_kernel(CrossA
   for (int i = 0; i < NLOAD; i++) {
     const int e = ((wave & 1) * NLOAD + i) * 64 + lane, r = e / C, p = (e % C) ^ P::swz(r);
     off[i] = p < real ? r * bytes + p * 16 : ~0u;
-    if (!FULL && p >= real)
+    if (!FULL && p >= real) {
+      const uint32_t fill = P::ONES && !keys && p >= 2 * DK ? 0x3f803f80u : 0;
 #pragma unroll
-      for (int t = 0; t < 2; t++) *reinterpret_cast<u32x4*>(to + t * TILE + (i * 64 + lane) * 8) = u32x4{0, 0, 0, 0};
+      for (int t = 0; t < 2; t++) *reinterpret_cast<u32x4*>(to + t * TILE + (i * 64 + lane) * 8) = u32x4{fill, fill, fill, fill};
+    }
   }
   typedef const __attribute__((address_space(1))) char* global_ptr;
   typedef const __attribute__((address_space(1))) void* global_any;
@@ -536,9 +540,10 @@ __global__ __launch_bounds__(256, DK <= 6 ? 3 : 2) void cross_wide_kernel(CrossA
         for (int j = 0; j < 8; j++) e[j] = __builtin_amdgcn_exp2f(fmaf(y[8 * hf + j], a.c, -ref));
         const u32x4 w = {pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7])};
         fp[hf] = frag(w);
-        // (the sum of the weights as they are multiplied, two an instruction)
-        l2[hf] = pair_sum(w.x, pair_sum(w.y, l2[hf]));
-        l2[hf] = pair_sum(w.z, pair_sum(w.w, l2[hf]));
+        if (!P::ONES) {  // (the sum of the weights as they are multiplied, two an instruction)
+          l2[hf] = pair_sum(w.x, pair_sum(w.y, l2[hf]));
+          l2[hf] = pair_sum(w.z, pair_sum(w.w, l2[hf]));
+        }
       }
       // V^T: lane i of 16 asks for elements 4 (i % 4) .. + 3 of key 8 g + i / 4 and gets element i of keys 8 g .. + 3
       const int i = lane & 15, upper = (lane >> 4) & 1;
@@ -560,7 +565,7 @@ __global__ __launch_bounds__(256, DK <= 6 ? 3 : 2) void cross_wide_kernel(CrossA
   int k0 = k_begin, half = 0;
   for (; k0 + KT < k_end; k0 += KT, half ^= 1) turn(k0, std::false_type(), half);
   if (k0 < k_end) turn(k0, std::true_type(), half);
-  const float l = sum32(l2[0] + l2[1]);
+  const float l = P::ONES ? acc[DT - 1][8] : sum32(l2[0] + l2[1]);  // (element 16 DK of O, and four behind it in the other half of the lanes)
   if (!live) return;
 #pragma unroll
   for (int d = 0; d < DT; d++)
@@ -753,7 +758,7 @@ MLLM_API int mllm_hip_attention_cross(const mllm_hip_heads* q, int dtype, int64_
     if (form == 12) go(cross_kernel<DP_, DT_, 1, 2, false>);                 \
     else if (form == 14) go(cross_kernel<DP_, DT_, 1, 4, false>);            \
     else if constexpr (DP_ < 256) {                                          \
-      if (D == 16 * DK_) go(cross_wide_kernel<DK_, (DK_ + 1) / 2, true>);    \
+      if (D == 16 * DK_ && DK_ != 5) go(cross_wide_kernel<DK_, (DK_ + 1) / 2, true>); \
       else go(cross_wide_kernel<DK_, (DK_ + 1) / 2, false>);                 \
     }                                                                        \
   }
