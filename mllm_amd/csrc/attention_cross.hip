@@ -425,8 +425,8 @@ __device__ __forceinline__ float pair_sum(uint32_t w, float z) {
 }
 __device__ __forceinline__ at_f32x16 mma32(at_bf16x8 x, at_bf16x8 y, at_f32x16 acc) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, y, acc, 0, 0, 0); }
 
-template <int DK, int DT, bool FULL>
-__global__ __launch_bounds__(256, DK <= 6 ? 3 : 2) void cross_wide_kernel(CrossArgs a) {
+template <int DK, int DT, int NR, bool FULL>
+__global__ __launch_bounds__(256, DK <= 6 && NR == 1 ? 3 : 2) void cross_wide_kernel(CrossArgs a) {
   typedef Wide<DK, DT> P;
   constexpr int KT = P::KT, C = P::C, DP = P::DP, CHUNKS = P::CHUNKS;
   __shared__ __align__(16) uint16_t s_all[4 * KT * DP];
@@ -477,29 +477,27 @@ __global__ __launch_bounds__(256, DK <= 6 ? 3 : 2) void cross_wide_kernel(CrossA
     }
   };
   // Q: second operand, row `col`, elements 16 s + 8 g .. + 7
-  at_bf16x8 fq[DK];
-  const int row = row0 + wave * 32 + col;
-  const bool live = row < rows;
-  const int token = live ? row / a.group : 0, head = h * a.group + (live ? row - token * a.group : 0);
-  {
+  at_bf16x8 fq[NR][DK];
+  int row[NR], token[NR], head[NR];
+  bool live[NR];
+#pragma unroll
+  for (int r = 0; r < NR; r++) {
+    row[r] = row0 + (wave * NR + r) * 32 + col;
+    live[r] = row[r] < rows;
+    token[r] = live[r] ? row[r] / a.group : 0;
+    head[r] = h * a.group + (live[r] ? row[r] - token[r] * a.group : 0);
     at_bf16x8 part[1];
 #pragma unroll
     for (int ks = 0; ks < DK; ks++) {
-      query_parts<false>(a.q, (s.first + token) * a.q_token + head * a.q_head + 16 * ks + 8 * g, live && 16 * ks + 8 * g < a.D, part);
-      fq[ks] = part[0];
+      query_parts<false>(a.q, (s.first + token[r]) * a.q_token + head[r] * a.q_head + 16 * ks + 8 * g, live[r] && 16 * ks + 8 * g < a.D, part);
+      fq[r][ks] = part[0];
     }
   }
-  at_f32x16 acc[DT] = {};
-  float m = -INFINITY, l2[2] = {0.f, 0.f};  // the maximum so far times c; the sums of this lane's keys
-  const int krow = (col & 3) | ((col >> 3) & 1) << 2 | ((col >> 2) & 1) << 3 | (col >> 4) << 4;
-  // scores of 32 keys
-  auto scores = [&](const uint16_t* k, int u) {
-    at_f32x16 y = {};
-    const int r = u * 32 + krow, x = P::swz(r);
+  at_f32x16 acc[NR][DT] = {};
+  float m[NR], l2[NR][2] = {};  // the maximum so far times c; the sums of this lane's keys
 #pragma unroll
-    for (int ks = 0; ks < DK; ks++) y = mma32(frag(*reinterpret_cast<const u32x4*>(k + r * DP + ((2 * ks + g) ^ x) * 8)), fq[ks], y);
-    return y;
-  };
+  for (int r = 0; r < NR; r++) m[r] = -INFINITY;
+  const int krow = (col & 3) | ((col >> 3) & 1) << 2 | ((col >> 2) & 1) << 3 | (col >> 4) << 4;
   auto arrived = [&]() {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __syncthreads();
@@ -512,37 +510,50 @@ __global__ __launch_bounds__(256, DK <= 6 ? 3 : 2) void cross_wide_kernel(CrossA
 #pragma unroll
     for (int u = 0; u < 2; u++) {
       if (last && k0 + 32 * u >= k_end) break;
-      at_f32x16 y = scores(k, u);
-      if (last) {
-        const int left = k_end - k0 - 32 * u - 8 * g;
+      at_f32x16 ys[NR] = {};
+      {
+        const int r = u * 32 + krow, x = P::swz(r);
 #pragma unroll
-        for (int j = 0; j < 16; j++) y[j] = 16 * (j >> 3) + (j & 7) < left ? y[j] : -INFINITY;
+        for (int ks = 0; ks < DK; ks++) {
+          const at_bf16x8 fk = frag(*reinterpret_cast<const u32x4*>(k + r * DP + ((2 * ks + g) ^ x) * 8));
+#pragma unroll
+          for (int n = 0; n < NR; n++) ys[n] = mma32(fk, fq[n][ks], ys[n]);
+        }
       }
-      float top = larger(larger(y[0], y[1]), y[2]);
+      at_bf16x8 fp[NR][2];
 #pragma unroll
-      for (int j = 3; j < 15; j += 2) top = larger(larger(y[j], y[j + 1]), top);
-      top = larger(top, y[15]);
-      top = across<32>(top) * a.c;
-      if (__ballot(top > m + 8.f)) {  // (weights of up to 2^8 do as well: most tiles leave O alone)
-        const float next = fmaxf(m, top), fix = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - next);
-        m = next;
-        l2[0] *= fix;
-        l2[1] *= fix;
+      for (int n = 0; n < NR; n++) {
+        at_f32x16& y = ys[n];
+        if (last) {
+          const int left = k_end - k0 - 32 * u - 8 * g;
 #pragma unroll
-        for (int d = 0; d < DT; d++) acc[d] *= fix;
-      }
-      const float ref = m == -INFINITY ? 0.f : m;  // (nothing seen yet: every p is exp2(-inf))
-      at_bf16x8 fp[2];
+          for (int j = 0; j < 16; j++) y[j] = 16 * (j >> 3) + (j & 7) < left ? y[j] : -INFINITY;
+        }
+        float top = larger(larger(y[0], y[1]), y[2]);
 #pragma unroll
-      for (int hf = 0; hf < 2; hf++) {
-        float e[8];
+        for (int j = 3; j < 15; j += 2) top = larger(larger(y[j], y[j + 1]), top);
+        top = larger(top, y[15]);
+        top = across<32>(top) * a.c;
+        if (__ballot(top > m[n] + 8.f)) {  // (weights of up to 2^8 do as well: most tiles leave O alone)
+          const float next = fmaxf(m[n], top), fix = m[n] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[n] - next);
+          m[n] = next;
+          l2[n][0] *= fix;
+          l2[n][1] *= fix;
 #pragma unroll
-        for (int j = 0; j < 8; j++) e[j] = __builtin_amdgcn_exp2f(fmaf(y[8 * hf + j], a.c, -ref));
-        const u32x4 w = {pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7])};
-        fp[hf] = frag(w);
-        if (!P::ONES) {  // (the sum of the weights as they are multiplied, two an instruction)
-          l2[hf] = pair_sum(w.x, pair_sum(w.y, l2[hf]));
-          l2[hf] = pair_sum(w.z, pair_sum(w.w, l2[hf]));
+          for (int d = 0; d < DT; d++) acc[n][d] *= fix;
+        }
+        const float ref = m[n] == -INFINITY ? 0.f : m[n];  // (nothing seen yet: every p is exp2(-inf))
+#pragma unroll
+        for (int hf = 0; hf < 2; hf++) {
+          float e[8];
+#pragma unroll
+          for (int j = 0; j < 8; j++) e[j] = __builtin_amdgcn_exp2f(fmaf(y[8 * hf + j], a.c, -ref));
+          const u32x4 w = {pack_bf16(e[0], e[1]), pack_bf16(e[2], e[3]), pack_bf16(e[4], e[5]), pack_bf16(e[6], e[7])};
+          fp[n][hf] = frag(w);
+          if (!P::ONES) {  // (the sum of the weights as they are multiplied, two an instruction)
+            l2[n][hf] = pair_sum(w.x, pair_sum(w.y, l2[n][hf]));
+            l2[n][hf] = pair_sum(w.z, pair_sum(w.w, l2[n][hf]));
+          }
         }
       }
       // V^T: lane i of 16 asks for elements 4 (i % 4) .. + 3 of key 8 g + i / 4 and gets element i of keys 8 g .. + 3
@@ -556,7 +567,9 @@ __global__ __launch_bounds__(256, DK <= 6 ? 3 : 2) void cross_wide_kernel(CrossA
           typedef __attribute__((address_space(3))) at_s16x4* lds_quad;
           const at_s16x4 v0 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_quad)(v + r * DP + (p ^ x) * 8 + (i & 1) * 4));
           const at_s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_quad)(v + (r + 4) * DP + (p ^ x4) * 8 + (i & 1) * 4));
-          acc[d] = mma32(frag(__builtin_bit_cast(u32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7))), fp[kk], acc[d]);
+          const at_bf16x8 fv = frag(__builtin_bit_cast(u32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7)));
+#pragma unroll
+          for (int n = 0; n < NR; n++) acc[n][d] = mma32(fv, fp[n][kk], acc[n][d]);
         }
       }
     }
@@ -565,13 +578,17 @@ __global__ __launch_bounds__(256, DK <= 6 ? 3 : 2) void cross_wide_kernel(CrossA
   int k0 = k_begin, half = 0;
   for (; k0 + KT < k_end; k0 += KT, half ^= 1) turn(k0, std::false_type(), half);
   if (k0 < k_end) turn(k0, std::true_type(), half);
-  const float l = P::ONES ? acc[DT - 1][8] : sum32(l2[0] + l2[1]);  // (element 16 DK of O, and four behind it in the other half of the lanes)
-  if (!live) return;
 #pragma unroll
-  for (int d = 0; d < DT; d++)
+  for (int n = 0; n < NR; n++) {
+    const float l = P::ONES ? acc[n][DT - 1][8] : sum32(l2[n][0] + l2[n][1]);  // (element 16 DK of O, and four behind it in the other half of the lanes)
+    if (!live[n]) continue;
 #pragma unroll
-    for (int j = 0; j < 4; j++)
-      cross_put<false>(a, place, row, token, head, 32 * d + 8 * j + 4 * g, at_f32x4{acc[d][4 * j], acc[d][4 * j + 1], acc[d][4 * j + 2], acc[d][4 * j + 3]}, m, l);
+    for (int d = 0; d < DT; d++)
+#pragma unroll
+      for (int j = 0; j < 4; j++)
+        cross_put<false>(a, place, row[n], token[n], head[n], 32 * d + 8 * j + 4 * g,
+                         at_f32x4{acc[n][d][4 * j], acc[n][d][4 * j + 1], acc[n][d][4 * j + 2], acc[n][d][4 * j + 3]}, m[n], l);
+  }
 }
 
 // Joins the pieces of a row: 16 bytes of it per lane, L lanes a row, G groups of lanes along the pieces
@@ -648,20 +665,23 @@ struct CrossPlan {
   int nq, wr, row_tiles, rows_of_tile, pieces, min_tiles;
   int64_t whole, tiles;
 };
-// Rows of a workgroup by the rows there are.  CUs have two workgroups each: as many row tiles as make whole rounds of 512 go through all of their keys, the keys of
-// those that are left are cut into as many pieces as fill another, of two tiles and of twice as many keys as rows at least.
+// Rows of a wave by the rows there are: 16, 32, and 64 where heads are of 96 elements at most, there is work for all CUs and the last tile's idle rows weigh little (each row of LDS read is
+// used twice, a SIMD has two waves instead of three or four.  Heads of 80, 64 / 32 rows: 16 heads, 7000 tokens 302 / 348 us, 64 sequences of 200 tokens 32.1 / 39.1; but 8 of 1100
+// 71.8 / 67.4, and with few tiles 2 of 600 over 6000 keys 93 / 67).  CUs have two workgroups each (one, of 64 rows a wave: 4900 tokens over 4900 keys 176 us, with two 209): as many
+// row tiles as make whole rounds go through all of their keys, the keys of those that are left are cut into as many pieces as fill another, of two tiles and of twice as many keys as rows at least.
 static CrossPlan cross_plan(bool f32, int64_t B, int heads, int kv, int64_t max_tokens, int64_t max_keys, int D) {
   CrossPlan p;
   if (max_keys > 0x7fffffff) max_keys = 0x7fffffff;
   const int64_t rows = max_tokens * (heads / kv);
-  p.nq = rows <= 64 || f32 || D > 128 ? 1 : 2;
+  const int64_t narrow = (rows + 127) / 128, twice = (narrow + 1) / 2;
+  p.nq = rows <= 64 || f32 || D > 128 ? 1 : D > 96 || twice * B * kv < 384 || (narrow % 2 && narrow < 20) ? 2 : 4;
   p.wr = rows <= 32 ? 2 : 4;
   p.rows_of_tile = p.nq * 16 * p.wr;
   const int64_t per = p.rows_of_tile, row_tiles = (rows + per - 1) / per;
   p.row_tiles = (int)row_tiles;
   const int64_t least = (2 * (rows < per ? rows : per) + 63) / 64;
   p.min_tiles = (int)(least > 2 ? least : 2);
-  const int64_t slots = 512, most = (max_keys + p.min_tiles * 64 - 1) / (p.min_tiles * 64);
+  const int64_t slots = p.nq == 4 ? 256 : 512, most = (max_keys + p.min_tiles * 64 - 1) / (p.min_tiles * 64);
   p.tiles = B * kv * row_tiles;
   p.whole = p.tiles / slots * slots;
   const int64_t rest = p.tiles - p.whole, wanted = rest ? slots / rest : 1;
@@ -670,6 +690,27 @@ static CrossPlan cross_plan(bool f32, int64_t B, int heads, int kv, int64_t max_
   return p;
 }
 static size_t cross_room(const CrossPlan& p, int D) { return (size_t)(p.tiles - p.whole) * p.pieces * p.rows_of_tile * (D + 2) * sizeof(float); }
+// Elements of a head that are held, tiles of 16 and steps of 16 they take (the latter of the forms with products of 32 x 32)
+template <int DP, int DT, int DK>
+static void cross_launch(const CrossPlan& p, bool f32, dim3 grid, hipStream_t st, const CrossArgs& a) {
+  auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a); };
+  if (f32) return p.wr == 2 ? go(cross_kernel<DP, DT, 1, 2, true>) : go(cross_kernel<DP, DT, 1, 4, true>);
+  if (p.nq == 1) return p.wr == 2 ? go(cross_kernel<DP, DT, 1, 2, false>) : go(cross_kernel<DP, DT, 1, 4, false>);
+  if constexpr (DK > 0) {
+    constexpr int D2 = (DK + 1) / 2;
+    const bool full = a.D == 16 * DK;
+    if constexpr (DK <= 6) {
+      if constexpr (DK != 5) {
+        if (p.nq == 4 && full) return go(cross_wide_kernel<DK, D2, 2, true>);
+      }
+      if (p.nq == 4) return go(cross_wide_kernel<DK, D2, 2, false>);
+    }
+    if constexpr (DK != 5) {
+      if (full) return go(cross_wide_kernel<DK, D2, 1, true>);
+    }
+    go(cross_wide_kernel<DK, D2, 1, false>);
+  }
+}
 static bool cross_sizes(int dtype, int64_t T, int64_t B, int heads, int kv, int head_dim, int64_t max_tokens, int64_t max_keys) {
   return (dtype == MLLM_HIP_F32 || dtype == MLLM_HIP_BF16) && T >= 0 && B >= 0 && heads >= 1 && kv >= 1 && head_dim >= 1 && max_tokens >= 0 && max_keys >= 0;
 }
@@ -748,26 +789,11 @@ MLLM_API int mllm_hip_attention_cross(const mllm_hip_heads* q, int dtype, int64_
   a.part_ml = rest ? a.part_o + (size_t)rest * p.pieces * p.rows_of_tile * D : nullptr;
   hipStream_t st = (hipStream_t)stream;
   const dim3 grid((unsigned)(p.whole + rest * p.pieces));
-  const int form = p.nq * 10 + p.wr;
-  auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a); };
-#define CROSS(DP_, DT_, DK_)                                                   \
-  if (f32) {                                                                 \
-    if (form == 12) go(cross_kernel<DP_, DT_, 1, 2, true>);                  \
-    else go(cross_kernel<DP_, DT_, 1, 4, true>);                             \
-  } else {                                                                   \
-    if (form == 12) go(cross_kernel<DP_, DT_, 1, 2, false>);                 \
-    else if (form == 14) go(cross_kernel<DP_, DT_, 1, 4, false>);            \
-    else if constexpr (DP_ < 256) {                                          \
-      if (D == 16 * DK_ && DK_ != 5) go(cross_wide_kernel<DK_, (DK_ + 1) / 2, true>); \
-      else go(cross_wide_kernel<DK_, (DK_ + 1) / 2, false>);                 \
-    }                                                                        \
-  }
-  if (D <= 64) { CROSS(64, 4, 4) }
-  else if (D <= 80) { CROSS(96, 5, 5) }
-  else if (D <= 96) { CROSS(96, 6, 6) }
-  else if (D <= 128) { CROSS(128, 8, 8) }
-  else { CROSS(256, 16, 16) }
-#undef CROSS
+  if (D <= 64) cross_launch<64, 4, 4>(p, f32, grid, st, a);
+  else if (D <= 80) cross_launch<96, 5, 5>(p, f32, grid, st, a);
+  else if (D <= 96) cross_launch<96, 6, 6>(p, f32, grid, st, a);
+  else if (D <= 128) cross_launch<128, 8, 8>(p, f32, grid, st, a);
+  else cross_launch<256, 16, 0>(p, f32, grid, st, a);
   RC_RET((int)hipGetLastError());
   if (rest) {
     const bool many = p.pieces >= 8;  // lanes along the pieces

@@ -82,6 +82,33 @@ def test_against_the_formula(counts, held, Hq, Hkv, D, dtype):
     c.check(c.run())
 
 
+@pytest.mark.parametrize("D", [40, 64, 72, 80, 88, 96])
+@pytest.mark.parametrize("tokens,group,keys", [(150, 1, 800), (256, 1, 65), (66, 3, 1100), (1300, 2, 130)])
+def test_many_rows_of_many_heads(D, tokens, group, keys):
+    """tiles of 256 rows: partly filled, of sequences without tokens or keys, those behind the last whole round in pieces"""
+    announce("attention_cross many rows", D, tokens, group, keys)
+    counts, held = [tokens, 1, 0, tokens - 2, tokens // 2, 63], [keys, keys // 2, 5, 0, keys - 1, keys // 3]
+    if tokens > 1000:
+        counts, held = [tokens, 100], [keys, keys - 40]
+    kv = 64 // (2 if tokens > 1000 else 1)
+    c = Case(counts, held, kv * group, kv, D, torch.bfloat16, seed=D + tokens)
+    c.check(c.run())
+
+
+@pytest.mark.parametrize("D", [64, 80])
+def test_many_rows_with_a_nan_and_an_infinity(D):
+    """a query's NaN stays in its row, an infinite value in its sequence, head and element"""
+    announce("attention_cross many rows, nan", D)
+    c = Case([200, 130], [300, 190], 192, 192, D, torch.bfloat16, seed=D)
+    clean = c.run()
+    c.q[17, 5, 2] = float("nan")
+    c.v[int(c.first[1]) + 189, 11, D - 1] = float("inf")
+    got = c.run()
+    assert torch.isnan(got[17, 5]).all() and not torch.isfinite(got[200:330, 11, D - 1]).any()
+    got[17, 5], got[200:330, 11, D - 1] = clean[17, 5], clean[200:330, 11, D - 1]
+    assert torch.equal(got, clean)
+
+
 @pytest.mark.parametrize("layout", ["rows", "heads", "both"])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("counts,held,D", [([5, 9], [333, 90], 80), ([1], [3000], 128), ([100], [100], 72)])
