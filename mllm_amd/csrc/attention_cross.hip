@@ -123,7 +123,7 @@ __device__ __forceinline__ void cross_put(const CrossArgs& a, const CrossPlace& 
   else *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(a.o) + at) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
 }
 
-template <int DP, int DT, int NQ, int WR, bool F32>
+template <int DP, int DT, int WR, bool F32>
 struct Cross {
   static constexpr int WK = 4 / WR;          // waves along keys
   static constexpr int KT = 64;              // keys of a tile
@@ -131,7 +131,6 @@ struct Cross {
   static constexpr int C = DP / 8;           // 16-byte pieces of a row
   static constexpr int NLOAD = KT * C / 256; // pieces of a tile that a lane loads, of keys and of values
   static constexpr int PARTS = F32 ? 3 : 1;
-  static constexpr int ROWS = NQ * 16;       // rows of a wave
   static constexpr int WAVES = DP == 256 ? 1 : 2;
   // Rows of 8 and of 16 or 32 pieces begin in the same banks every second or every row; rows of 12 every fourth.
   static __device__ __forceinline__ int swz(int row) {
@@ -139,9 +138,9 @@ struct Cross {
   }
 };
 
-template <int DP, int DT, int NQ, int WR, bool F32>
-__global__ __launch_bounds__(256, (Cross<DP, DT, NQ, WR, F32>::WAVES)) void cross_kernel(CrossArgs a) {
-  typedef Cross<DP, DT, NQ, WR, F32> P;
+template <int DP, int DT, int WR, bool F32>
+__global__ __launch_bounds__(256, (Cross<DP, DT, WR, F32>::WAVES)) void cross_kernel(CrossArgs a) {
+  typedef Cross<DP, DT, WR, F32> P;
   constexpr int KT = P::KT, C = P::C, WK = P::WK, NLOAD = P::NLOAD, KS = DP / 32, PARTS = P::PARTS;
   __shared__ __align__(16) uint16_t s_k[2 * KT * DP];
   __shared__ __align__(16) uint16_t s_v[2 * KT * DP];
@@ -195,116 +194,96 @@ __global__ __launch_bounds__(256, (Cross<DP, DT, NQ, WR, F32>::WAVES)) void cros
   };
   if (k_begin < k_end) ask_tile(k_begin);
 
-  // Q: second operand, row `col` of every 16, elements 32 s + 8 g .. + 7
-  at_bf16x8 fq[NQ][KS][PARTS];
+  // Q: second operand, row `col`, elements 32 s + 8 g .. + 7
+  at_bf16x8 fq[KS][PARTS];
+  const int own = row0 + wr * 16 + col;
+  const bool live = own < rows;
+  const int token = live ? own / a.group : 0, head = h * a.group + (live ? own - token * a.group : 0);
+  const int64_t q_at = (s.first + token) * a.q_token + head * a.q_head + 8 * g;
 #pragma unroll
-  for (int i = 0; i < NQ; i++) {
-    const int r = row0 + wr * P::ROWS + i * 16 + col;
-    const bool live = r < rows;
-    const int token = live ? r / a.group : 0, head = h * a.group + (live ? r - token * a.group : 0);
-    const int64_t at = (s.first + token) * a.q_token + head * a.q_head + 8 * g;
+  for (int ks = 0; ks < KS; ks++) query_parts<F32>(a.q, q_at + 32 * ks, live && 32 * ks + 8 * g < a.D, fq[ks]);
 #pragma unroll
-    for (int ks = 0; ks < KS; ks++) query_parts<F32>(a.q, at + 32 * ks, live && 32 * ks + 8 * g < a.D, fq[i][ks]);
-  }
+  for (int ks = 0; ks < KS; ks++)
 #pragma unroll
-  for (int i = 0; i < NQ; i++)
-#pragma unroll
-    for (int ks = 0; ks < KS; ks++)
-#pragma unroll
-      for (int p = 0; p < PARTS; p++) asm volatile("" : "+v"(fq[i][ks][p]));  // (here from now on: a wait for it in the loop would be one for the next tile's loads)
+    for (int p = 0; p < PARTS; p++) asm volatile("" : "+v"(fq[ks][p]));  // (here from now on: a wait for it in the loop would be one for the next tile's loads)
 
-  at_f32x4 acc[NQ][DT];
-  float m[NQ], l[NQ];  // the maximum so far times c; the sum of this lane's keys
-#pragma unroll
-  for (int i = 0; i < NQ; i++) {
-    m[i] = -INFINITY;
-    l[i] = 0.f;
-#pragma unroll
-    for (int d = 0; d < DT; d++) acc[i][d] = at_f32x4{0.f, 0.f, 0.f, 0.f};
-  }
-  const bool busy = row0 + wr * P::ROWS < rows;  // (a wave without rows loads with the others and leaves its SIMD to them)
+  at_f32x4 acc[DT] = {};
+  float m = -INFINITY, l = 0.f;  // the maximum so far times c; the sum of this lane's keys
+  const bool busy = row0 + wr * 16 < rows;  // (a wave without rows loads with the others and leaves its SIMD to them)
   auto work = [&](int k0, auto last_, auto half) {
     constexpr bool last = decltype(last_)::value;  // the tile may have keys behind the last
 #pragma unroll
     for (int u = 0; u < P::SUB; u++) {
       const int base = (u * WK + wk) * 32, key0 = k0 + base;
       if (last && key0 >= k_end) break;
-      at_f32x4 sa[NQ], sb[NQ];
-#pragma unroll
-      for (int i = 0; i < NQ; i++) sa[i] = sb[i] = at_f32x4{0.f, 0.f, 0.f, 0.f};
+      at_f32x4 sa = {0.f, 0.f, 0.f, 0.f}, sb = {0.f, 0.f, 0.f, 0.f};
       const int ra = half * KT + base + 8 * (col >> 2) + (col & 3), x = P::swz(ra);
 #pragma unroll
       for (int ks = 0; ks < KS; ks++) {
         const int at = ra * DP + ((4 * ks + g) ^ x) * 8;
         const at_bf16x8 ka = frag(*reinterpret_cast<const u32x4*>(s_k + at)), kb = frag(*reinterpret_cast<const u32x4*>(s_k + at + 4 * DP));
 #pragma unroll
-        for (int i = 0; i < NQ; i++) {
-#pragma unroll
-          for (int p = PARTS - 1; p >= 0; p--) {  // the smallest part first
-            sa[i] = mma(ka, fq[i][ks][p], sa[i]);
-            sb[i] = mma(kb, fq[i][ks][p], sb[i]);
-          }
+        for (int p = PARTS - 1; p >= 0; p--) {  // the smallest part first
+          sa = mma(ka, fq[ks][p], sa);
+          sb = mma(kb, fq[ks][p], sb);
         }
       }
-      at_bf16x8 fp[PARTS][NQ];
+      at_bf16x8 fp[PARTS];
+      float y[8], top;
+      auto scores = [&](const at_f32x4& a0, const at_f32x4& b0) {
 #pragma unroll
-      for (int i = 0; i < NQ; i++) {
-        float y[8], top;
-        auto scores = [&](const at_f32x4& a0, const at_f32x4& b0) {
+        for (int j = 0; j < 4; j++) y[j] = a0[j], y[4 + j] = b0[j];
+        if (last) {
+          const int left = k_end - key0 - 8 * g;
 #pragma unroll
-          for (int j = 0; j < 4; j++) y[j] = a0[j], y[4 + j] = b0[j];
-          if (last) {
-            const int left = k_end - key0 - 8 * g;
+          for (int j = 0; j < 8; j++) y[j] = j < left ? y[j] : -INFINITY;
+        }
+        top = larger(larger(larger(y[0], y[1]), larger(y[2], y[3])), larger(larger(y[4], y[5]), larger(y[6], y[7])));
+        top = across<16>(top);
+        top = across<32>(top) * a.c;
+      };
+      scores(sa, sb);
+      if (__ballot(F32 ? !(top <= m + 8.f) : top > m + 8.f)) {  // (weights of up to 2^8 do as well: most steps leave O alone)
+        if constexpr (F32) {
+          // An infinite element of a key makes a NaN with the second and third part of a query's, which may be 0: it counts with the first alone, which
+          // has the sign.  Such scores, and those that are NaN anyway, are formed once more.
+          if (__builtin_expect(__ballot(top != top) != 0, 0)) {
+            at_f32x4 ta = {0.f, 0.f, 0.f, 0.f}, tb = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-            for (int j = 0; j < 8; j++) y[j] = j < left ? y[j] : -INFINITY;
-          }
-          top = larger(larger(larger(y[0], y[1]), larger(y[2], y[3])), larger(larger(y[4], y[5]), larger(y[6], y[7])));
-          top = across<16>(top);
-          top = across<32>(top) * a.c;
-        };
-        scores(sa[i], sb[i]);
-        if (__ballot(F32 ? !(top <= m[i] + 8.f) : top > m[i] + 8.f)) {  // (weights of up to 2^8 do as well: most steps leave O alone)
-          if constexpr (F32) {
-            // An infinite element of a key makes a NaN with the second and third part of a query's, which may be 0: it counts with the first alone, which
-            // has the sign.  Such scores, and those that are NaN anyway, are formed once more.
-            if (__builtin_expect(__ballot(top != top) != 0, 0)) {
-              at_f32x4 ta = {0.f, 0.f, 0.f, 0.f}, tb = {0.f, 0.f, 0.f, 0.f};
+            for (int ks = 0; ks < KS; ks++) {
+              const int at = ra * DP + ((4 * ks + g) ^ x) * 8;
+              const u32x4 ka = *reinterpret_cast<const u32x4*>(s_k + at), kb = *reinterpret_cast<const u32x4*>(s_k + at + 4 * DP);
+              const at_bf16x8 fa = frag(u32x4{finite_pair(ka.x), finite_pair(ka.y), finite_pair(ka.z), finite_pair(ka.w)}),
+                              fb = frag(u32x4{finite_pair(kb.x), finite_pair(kb.y), finite_pair(kb.z), finite_pair(kb.w)});
 #pragma unroll
-              for (int ks = 0; ks < KS; ks++) {
-                const int at = ra * DP + ((4 * ks + g) ^ x) * 8;
-                const u32x4 ka = *reinterpret_cast<const u32x4*>(s_k + at), kb = *reinterpret_cast<const u32x4*>(s_k + at + 4 * DP);
-                const at_bf16x8 fa = frag(u32x4{finite_pair(ka.x), finite_pair(ka.y), finite_pair(ka.z), finite_pair(ka.w)}),
-                                fb = frag(u32x4{finite_pair(kb.x), finite_pair(kb.y), finite_pair(kb.z), finite_pair(kb.w)});
-#pragma unroll
-                for (int p = PARTS - 1; p > 0; p--) {
-                  ta = mma(fa, fq[i][ks][p], ta);
-                  tb = mma(fb, fq[i][ks][p], tb);
-                }
-                ta = mma(frag(ka), fq[i][ks][0], ta);
-                tb = mma(frag(kb), fq[i][ks][0], tb);
+              for (int p = PARTS - 1; p > 0; p--) {
+                ta = mma(fa, fq[ks][p], ta);
+                tb = mma(fb, fq[ks][p], tb);
               }
-              scores(ta, tb);
+              ta = mma(frag(ka), fq[ks][0], ta);
+              tb = mma(frag(kb), fq[ks][0], tb);
             }
+            scores(ta, tb);
           }
-          const float next = fmaxf(m[i], top), fix = m[i] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[i] - next);
-          m[i] = next;
-          l[i] *= fix;
-#pragma unroll
-          for (int d = 0; d < DT; d++) acc[i][d] *= fix;
         }
-        const float ref = m[i] == -INFINITY ? 0.f : m[i];  // (nothing seen yet: every p is exp2(-inf))
+        const float next = fmaxf(m, top), fix = m == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m - next);
+        m = next;
+        l *= fix;
 #pragma unroll
-        for (int j = 0; j < 8; j++) y[j] = __builtin_amdgcn_exp2f(fmaf(y[j], a.c, -ref));
-        l[i] += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
-        if constexpr (!F32) {
-          fp[0][i] = frag(u32x4{pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7])});
-        } else {
-          uint32_t part[3][4];
+        for (int d = 0; d < DT; d++) acc[d] *= fix;
+      }
+      const float ref = m == -INFINITY ? 0.f : m;  // (nothing seen yet: every p is exp2(-inf))
 #pragma unroll
-          for (int j = 0; j < 4; j++) split2(y[2 * j], y[2 * j + 1], part[0][j], part[1][j], part[2][j]);
+      for (int j = 0; j < 8; j++) y[j] = __builtin_amdgcn_exp2f(fmaf(y[j], a.c, -ref));
+      l += ((y[0] + y[1]) + (y[2] + y[3])) + ((y[4] + y[5]) + (y[6] + y[7]));
+      if constexpr (!F32) {
+        fp[0] = frag(u32x4{pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]), pack_bf16(y[4], y[5]), pack_bf16(y[6], y[7])});
+      } else {
+        uint32_t part[3][4];
 #pragma unroll
-          for (int p = 0; p < 3; p++) fp[p][i] = frag(u32x4{part[p][0], part[p][1], part[p][2], part[p][3]});
-        }
+        for (int j = 0; j < 4; j++) split2(y[2 * j], y[2 * j + 1], part[0][j], part[1][j], part[2][j]);
+#pragma unroll
+        for (int p = 0; p < 3; p++) fp[p] = frag(u32x4{part[p][0], part[p][1], part[p][2], part[p][3]});
       }
       // V^T: lane i of 16 asks for elements 4 (i % 4) .. + 3 of key 8 g + i / 4 and gets element i of keys 8 g .. + 3
       const int rv0 = half * KT + base + 8 * g + (col >> 2), xv = P::swz(rv0);
@@ -316,10 +295,7 @@ __global__ __launch_bounds__(256, (Cross<DP, DT, NQ, WR, F32>::WAVES)) void cros
         const at_s16x4 v1 = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_ptr)(s_v + at + 4 * DP));
         const at_bf16x8 fv = frag(__builtin_bit_cast(u32x4, __builtin_shufflevector(v0, v1, 0, 1, 2, 3, 4, 5, 6, 7)));
 #pragma unroll
-        for (int i = 0; i < NQ; i++) {
-#pragma unroll
-          for (int p = PARTS - 1; p >= 0; p--) acc[i][d] = mma(fv, fp[p][i], acc[i][d]);
-        }
+        for (int p = PARTS - 1; p >= 0; p--) acc[d] = mma(fv, fp[p], acc[d]);
       }
     }
   };
@@ -350,56 +326,48 @@ __global__ __launch_bounds__(256, (Cross<DP, DT, NQ, WR, F32>::WAVES)) void cros
     half = 0;
   }
   if (k0 < k_end) turn(std::true_type(), half, half ^ 1);
-#pragma unroll
-  for (int i = 0; i < NQ; i++) l[i] = sum32(sum16(l[i]));
+  l = sum32(sum16(l));
 
   auto put = [&](int row, int d, at_f32x4 x, float mm, float sum) {
     cross_put<F32>(a, place, row, row / a.group, h * a.group + row % a.group, d, x, mm, sum);
   };
   if constexpr (WK == 1) {
+    if (!live) return;
 #pragma unroll
-    for (int i = 0; i < NQ; i++) {
-      const int row = row0 + wr * P::ROWS + i * 16 + col;
-      if (row >= rows) continue;
-#pragma unroll
-      for (int d = 0; d < DT; d++) put(row, 16 * d + 4 * g, acc[i][d], m[i], l[i]);
-    }
+    for (int d = 0; d < DT; d++) put(own, 16 * d + 4 * g, acc[d], m, l);
   } else {
-    // The waves along keys meet in LDS, 16 rows at a time: O of a row where the keys were, its maximum and sum where the values were.
+    // The waves along keys meet in LDS: O of a row where the keys were, its maximum and sum where the values were.
     constexpr int Q4 = DT * 4, IT = (16 * Q4 + WK * 64 - 1) / (WK * 64);  // quads of a row; quads of a lane
     float* so = reinterpret_cast<float*>(s_k);            // [wave][16][DT * 16]
     float* sm = reinterpret_cast<float*>(s_v);            // [wave][16][2]
     static_assert(4 * 16 * DT * 16 * 4 <= 2 * KT * DP * 2, "");
+    __syncthreads();
 #pragma unroll
-    for (int i = 0; i < NQ; i++) {
-      __syncthreads();
+    for (int d = 0; d < DT; d++) *reinterpret_cast<at_f32x4*>(so + ((wave * 16 + col) * Q4 + ((4 * d + g) ^ (col & 3))) * 4) = acc[d];
+    if (g == 0) {
+      sm[(wave * 16 + col) * 2] = m;
+      sm[(wave * 16 + col) * 2 + 1] = l;
+    }
+    __syncthreads();
 #pragma unroll
-      for (int d = 0; d < DT; d++) *reinterpret_cast<at_f32x4*>(so + ((wave * 16 + col) * Q4 + ((4 * d + g) ^ (col & 3))) * 4) = acc[i][d];
-      if (g == 0) {
-        sm[(wave * 16 + col) * 2] = m[i];
-        sm[(wave * 16 + col) * 2 + 1] = l[i];
+    for (int it = 0; it < IT; it++) {
+      const int e = wk * 64 + lane + it * WK * 64, r = e / Q4, p = e % Q4;
+      const int row = row0 + wr * 16 + r;
+      if (r >= 16 || row >= rows) continue;
+      float top = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < WK; w++) top = fmaxf(top, sm[((w * WR + wr) * 16 + r) * 2]);
+      const float ref = top == -INFINITY ? 0.f : top;
+      at_f32x4 x = {0.f, 0.f, 0.f, 0.f};
+      float sum = 0.f;
+#pragma unroll
+      for (int w = 0; w < WK; w++) {
+        const int at = (w * WR + wr) * 16 + r;
+        const float f = __builtin_amdgcn_exp2f(sm[at * 2] - ref);
+        sum += sm[at * 2 + 1] * f;
+        x += *reinterpret_cast<const at_f32x4*>(so + (at * Q4 + (p ^ (r & 3))) * 4) * f;
       }
-      __syncthreads();
-#pragma unroll
-      for (int it = 0; it < IT; it++) {
-        const int e = wk * 64 + lane + it * WK * 64, r = e / Q4, p = e % Q4;
-        const int row = row0 + wr * P::ROWS + i * 16 + r;
-        if (r >= 16 || row >= rows) continue;
-        float top = -INFINITY;
-#pragma unroll
-        for (int w = 0; w < WK; w++) top = fmaxf(top, sm[((w * WR + wr) * 16 + r) * 2]);
-        const float ref = top == -INFINITY ? 0.f : top;
-        at_f32x4 x = {0.f, 0.f, 0.f, 0.f};
-        float sum = 0.f;
-#pragma unroll
-        for (int w = 0; w < WK; w++) {
-          const int at = (w * WR + wr) * 16 + r;
-          const float f = __builtin_amdgcn_exp2f(sm[at * 2] - ref);
-          sum += sm[at * 2 + 1] * f;
-          x += *reinterpret_cast<const at_f32x4*>(so + (at * Q4 + (p ^ (r & 3))) * 4) * f;
-        }
-        put(row, p * 4, x, top, sum);
-      }
+      put(row, p * 4, x, top, sum);
     }
   }
 }
@@ -700,8 +668,8 @@ static size_t cross_room(const CrossPlan& p, int D) { return (size_t)(p.tiles - 
 template <int DP, int DT, int DK>
 static void cross_launch(const CrossPlan& p, bool f32, dim3 grid, hipStream_t st, const CrossArgs& a) {
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a); };
-  if (f32) return p.wr == 2 ? go(cross_kernel<DP, DT, 1, 2, true>) : go(cross_kernel<DP, DT, 1, 4, true>);
-  if (p.nq == 1) return p.wr == 2 ? go(cross_kernel<DP, DT, 1, 2, false>) : go(cross_kernel<DP, DT, 1, 4, false>);
+  if (f32) return p.wr == 2 ? go(cross_kernel<DP, DT, 2, true>) : go(cross_kernel<DP, DT, 4, true>);
+  if (p.nq == 1) return p.wr == 2 ? go(cross_kernel<DP, DT, 2, false>) : go(cross_kernel<DP, DT, 4, false>);
   if constexpr (DK > 0) {
     constexpr int D2 = (DK + 1) / 2;
     const bool full = a.D == 16 * DK;
