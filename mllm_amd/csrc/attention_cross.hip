@@ -643,6 +643,8 @@ struct CrossPlan {
 // used twice, a SIMD has two waves instead of three or four.  Heads of 80, 64 / 32 rows: 16 heads, 7000 tokens 302 / 348 us, 64 sequences of 200 tokens 32.1 / 39.1; but 8 of 1100
 // 71.8 / 67.4, and with few tiles 2 of 600 over 6000 keys 93 / 67).  CUs have two workgroups each (one, of 64 rows a wave: 4900 tokens over 4900 keys 176 us, with two 209): as many
 // row tiles as make whole rounds go through all of their keys, the keys of those that are left are cut into as many pieces as fill another, of two tiles and of twice as many keys as rows at least.
+// Few keys are not cut, for the second launch takes longer than they do: two tokens of 32 heads of 128 over 179 keys 9.8 us cut, 7.1 uncut, over 300 10.1 both, over 500 10.6 and 12.3; heads of 64 over 300 9.6 and 7.8, over
+// 500 9.7 and 12.0.
 static CrossPlan cross_plan(bool f32, int64_t B, int heads, int kv, int64_t max_tokens, int64_t max_keys, int D) {
   CrossPlan p;
   if (max_keys > 0x7fffffff) max_keys = 0x7fffffff;
@@ -659,7 +661,7 @@ static CrossPlan cross_plan(bool f32, int64_t B, int heads, int kv, int64_t max_
   p.tiles = B * kv * row_tiles;
   p.whole = p.tiles / slots * slots;
   const int64_t rest = p.tiles - p.whole, wanted = rest ? slots / rest : 1;
-  p.pieces = (int)(most < 2 || wanted < 2 ? 1 : wanted < most ? wanted : most);
+  p.pieces = (int)(max_keys <= (D <= 64 ? 384 : 256) || most < 2 || wanted < 2 ? 1 : wanted < most ? wanted : most);
   if (p.pieces == 1) p.whole = p.tiles;
   return p;
 }
