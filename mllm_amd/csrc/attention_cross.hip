@@ -6,9 +6,16 @@
 // key head) and eight consecutive keys, which is what the second operand of O^T = V^T P^T takes.  Scores, maxima, sums and O are fp32; P is rounded to bf16 for
 // the product with V (off by 2^-8 of each weight at most, of either sign), fp32 queries and their P enter as three bf16 parts each.
 //
-// A workgroup has four waves, WR along rows times 4 / WR along keys, and goes through the keys in tiles of 64: 16-byte loads into registers while the tile
-// before them is worked on, from there into LDS.  Heads of 72 or 80 elements take three steps of 32 in the first product (zeros behind them) and five tiles of 16 in the second.
+// Two forms.  Up to 64 rows of a sequence and key head, fp32 queries and heads of more than 128 elements: cross_kernel, on products of 16 x 16 x 32.  A workgroup has four waves, WR along rows times
+// 4 / WR along keys, and goes through the keys in tiles of 64: 16-byte loads into registers while the tile before them is worked on, from there into LDS.  Heads of 72 or 80 elements take three
+// steps of 32 in the first product (zeros behind them) and five tiles of 16 in the second.  More bf16 rows: cross_wide_kernel, on products of 32 x 32 x 16, keys and values from memory to LDS directly.
 // Where rows, heads and sequences leave CUs idle the keys are cut into pieces, whose O, maximum and sum meet in the workspace; a second launch joins them.
+//
+// What bounds it.  Few rows: memory, behind the chain of two launches (64 sequences of one token over 1601 keys, 32 query and 8 key heads of 128, 74 us: 4.4 TB/s where a copy of 2 GB has 5.18; four
+// fp32 tokens over 1601 keys 15.4, of which the join takes 3.9).  64 x 64 windows of 160 images, 16 heads of 80: 23 us, 3.4 TB/s.  Many rows: matrix and vector instructions, which share a SIMD's issue and overlap only
+// in part, at the clock that both leave (1.8 GHz): 4900 tokens over 4900 keys, 16 heads of 80, 157 us (780 TFLOP/s; a product of 8192^3 has 1229), 3 x 700 tokens over up to 6404 keys, 32 heads of 128, 155 to 180
+// (730 to 850), 10 000 over 10 000, four query heads a key head, 550 (930).  Matrix pipes are busy 45 % of the time, no LDS read meets a taken bank.
+// Next tile's scores between this one's exponents (a third more registers) and four waves a SIMD (spills) were no faster; equal shares of the keys of all tiles per CU, whose parts are joined, cost 24 us to join.
 #include <type_traits>
 
 #include "attention_common.h"
@@ -372,7 +379,7 @@ __global__ __launch_bounds__(256, (Cross<DP, DT, WR, F32>::WAVES)) void cross_ke
   }
 }
 
-// Many rows of bf16 queries: a wave has 32 of them, v_mfma_f32_32x32x16_bf16, DK steps of 16 elements in the first product and DT tiles of 32 in the second.  First operand rows
+// Many rows of bf16 queries: a wave has 32 NR of them, v_mfma_f32_32x32x16_bf16, DK steps of 16 elements in the first product and DT tiles of 32 in the second.  First operand rows
 // 8 a + 4 b + c = keys 16 (a / 2) + 8 b + 4 (a % 2) + c leave a lane with one row of Q and, of every 16 keys, the eight consecutive ones that the second product takes.
 // Keys and values go from memory to LDS directly.  FULL: heads of 16 DK elements.
 template <int DK, int DT>

@@ -11,7 +11,12 @@
 //   these and adds up the weights from the scores.  Keys are read once.
 //   More rows: the first finds maxima and sums, a wave's rows in registers and keys going by (a small launch joins them where keys are cut into ranges); the second has a wave's
 //   keys in registers and rows going by, so that what a key gets is a sum in a lane.
+//   Few keys and up to 16 rows: one launch, a workgroup a key head, scores in LDS.
 // No atomics: what a key gets is summed by one wave in one order.
+//
+// What bounds it.  Tokens: memory (a token of 16 sequences over up to 8000 keys, 32 query and 8 key heads of 128, 57 us: scores 47, of which keys arrive at 3.7 TB/s, sums 9.5; neither more ranges, nor ranges of equal
+// length over all sequences, nor heads of a range on one XCD changed that).  More rows: matrix instructions, three parts of fp32 queries in both passes (32 tokens of six sequences over up to 7000 keys 77 us:
+// parts 5.6, maxima 35, join 4.7, weights 40; the bytes alone would take 12, the products at a library's rate 25).  Storing the scores of many rows instead of forming them twice would write and read more bytes than that.
 #include <type_traits>
 
 #include "attention_common.h"
@@ -283,13 +288,25 @@ __global__ __launch_bounds__(512) void weights_one_kernel(WeightArgs a) {
   if (rows == 0) return;
   const int32_t* table = a.table + b * a.table_stride;
   const uint64_t k_at = (uint64_t)(uintptr_t)(a.k + h * a.head_stride);
+  // Keys are on their way while the ones before them are worked on, and the page of those behind.
+  auto page_at = [&](int key) { return key < s.keys ? table[page_of(a, key)] : -1; };
+  const int first = wave * 16 + col;
+  int id = page_at(first);
+  u32x4 next[KS];
+  load_key_of<KS>(a, k_at, id, first, g, next);
+  id = page_at(first + 128);
   at_bf16x8 q[KS][F32 ? 3 : 1];
   load_rows<KS, F32>(a, s, h, col, rows, g, q);
   const int token = col < rows ? col / a.group : -1, sees = token < 0 ? 0 : min(s.prefix + token + 1, s.keys);
   float m = -INFINITY, l = 0.f;
   for (int k0 = wave * 16; k0 < s.keys; k0 += 128) {
     u32x4 k[KS];
-    load_key<KS>(a, table, k_at, k0 + col, k0 + col < s.keys, g, k);
+#pragma unroll
+    for (int ks = 0; ks < KS; ks++) k[ks] = next[ks];
+    if (k0 + 128 < s.keys) {
+      load_key_of<KS>(a, k_at, id, k0 + 128 + col, g, next);
+      id = page_at(k0 + 256 + col);
+    }
     const at_f32x4 y = seen_scores<KS, F32>(k, q, sees - (k0 + 4 * g));
     if (col < rows) *reinterpret_cast<at_f32x4*>(s_score + col * WEIGHT_PITCH + k0 + 4 * g) = y;
     take(m, l, y, a.c);
