@@ -275,10 +275,10 @@ __global__ __launch_bounds__(256) void weights_sum_kernel(WeightArgs a) {
 }
 
 // The whole of it in one launch where keys are few: a workgroup has a key head of a sequence, scores stay in LDS.
-enum { WEIGHT_ONE = 960, WEIGHT_PITCH = WEIGHT_ONE + 4 };  // 16 rows in less than 64 KB
+enum { WEIGHT_LDS = 16 * 964 };  // floats: with what else there is less than 64 KB
 template <int KS, bool F32>
 __global__ __launch_bounds__(512) void weights_one_kernel(WeightArgs a) {
-  extern __shared__ __align__(16) float s_score[];  // [rows][WEIGHT_PITCH]
+  extern __shared__ __align__(16) float s_score[];  // [rows][pitch]
   __shared__ f32x2 s_ml[8][16];
   __shared__ f32x2 s_row[16];
   const int h = blockIdx.x % a.kv, b = blockIdx.x / a.kv;
@@ -308,7 +308,7 @@ __global__ __launch_bounds__(512) void weights_one_kernel(WeightArgs a) {
       id = page_at(k0 + 256 + col);
     }
     const at_f32x4 y = seen_scores<KS, F32>(k, q, sees - (k0 + 4 * g));
-    if (col < rows) *reinterpret_cast<at_f32x4*>(s_score + col * WEIGHT_PITCH + k0 + 4 * g) = y;
+    if (col < rows) *reinterpret_cast<at_f32x4*>(s_score + col * a.pitch + k0 + 4 * g) = y;
     take(m, l, y, a.c);
   }
   join_lanes(m, l);
@@ -322,7 +322,7 @@ __global__ __launch_bounds__(512) void weights_one_kernel(WeightArgs a) {
   for (int key = threadIdx.x; key < s.keys; key += 512) {
     float sum = 0.f;
     for (int r = 0; r < rows; r++) {
-      const float p = __builtin_amdgcn_exp2f(fmaf(s_score[r * WEIGHT_PITCH + key], a.c, -s_row[r].x)) * s_row[r].y;
+      const float p = __builtin_amdgcn_exp2f(fmaf(s_score[r * a.pitch + key], a.c, -s_row[r].x)) * s_row[r].y;
       sum += key <= s.prefix + r / a.group ? p : 0.f;
     }
     put_mass(a, s, b, h, key, sum);
@@ -687,9 +687,10 @@ static WeightPlan weight_plan(bool f32, int64_t B, int heads, int kv, int D, int
   WeightPlan p = {};
   const int64_t rows = max_tokens * (heads / kv);
   p.few = rows <= 16;
-  p.one = p.few && max_keys <= WEIGHT_ONE;
   p.rows = p.few ? (int)rows : 0;
   p.pitch = (int)((max_keys + 63) / 64 * 64);
+  p.one = p.few && (p.pitch + 4) * rows <= WEIGHT_LDS && (max_keys <= 960 || B * kv >= 256);
+  if (p.one) p.pitch += 4;  // (rows begin in banks of their own)
   const int64_t wave = weight_nq(D > 128 ? 8 : 4, f32) * 16;
   p.wr = rows <= wave ? 1 : rows <= 2 * wave ? 2 : 4;
   p.row_tiles = p.few ? 1 : (int)((rows + p.wr * wave - 1) / (p.wr * wave));
@@ -805,7 +806,7 @@ MLLM_API int mllm_hip_attention_weights(const mllm_hip_heads* q, int dtype, int6
   }
   if (p.one) {
     // (blocks of 512 threads: the launches below have 256)
-    const size_t lds = (size_t)p.rows * WEIGHT_PITCH * sizeof(float);
+    const size_t lds = (size_t)p.rows * p.pitch * sizeof(float);
     auto one = [&](auto ks) {
       constexpr int KS = decltype(ks)::value;
       if (f32) hipLaunchKernelGGL((weights_one_kernel<KS, true>), dim3(heads_of_all), dim3(512), lds, st, a);
