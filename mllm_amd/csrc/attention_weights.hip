@@ -11,11 +11,11 @@
 //   these and adds up the weights from the scores.  Keys are read once.
 //   More rows: the first finds maxima and sums, a wave's rows in registers and keys going by (a small launch joins them where keys are cut into ranges); the second has a wave's
 //   keys in registers and rows going by, so that what a key gets is a sum in a lane.
-//   Few keys and up to 16 rows: one launch, a workgroup a key head, scores in LDS.
+//   Up to 16 rows whose scores fit into 64 KB, of few keys or many sequences: the two in one launch, a workgroup a key head, scores in LDS.
 // No atomics: what a key gets is summed by one wave in one order.
 //
 // What bounds it.  Tokens: memory (a token of 16 sequences over up to 8000 keys, 32 query and 8 key heads of 128, 57 us: scores 47, of which keys arrive at 3.7 TB/s, sums 9.5; neither more ranges, nor ranges of equal
-// length over all sequences, nor heads of a range on one XCD changed that).  More rows: matrix instructions, three parts of fp32 queries in both passes (32 tokens of six sequences over up to 7000 keys 77 us:
+// length over all sequences, nor heads of a range on one XCD changed that; 64 sequences over up to 3800 keys 88, 3.7 TB/s too, whether 64 or 128 KB a CU are on their way).  More rows: matrix instructions, three parts of fp32 queries in both passes (32 tokens of six sequences over up to 7000 keys 77 us:
 // parts 5.6, maxima 35, join 4.7, weights 40; the bytes alone would take 12, the products at a library's rate 25).  Storing the scores of many rows instead of forming them twice would write and read more bytes than that.
 #include <type_traits>
 
@@ -274,7 +274,7 @@ __global__ __launch_bounds__(256) void weights_sum_kernel(WeightArgs a) {
   put_mass(a, s, b, h, key, sum);
 }
 
-// The whole of it in one launch where keys are few: a workgroup has a key head of a sequence, scores stay in LDS.
+// The whole of it in one launch: a workgroup has a key head of a sequence, scores stay in LDS.
 enum { WEIGHT_LDS = 16 * 964 };  // floats: with what else there is less than 64 KB
 template <int KS, bool F32>
 __global__ __launch_bounds__(512) void weights_one_kernel(WeightArgs a) {
@@ -683,6 +683,11 @@ struct WeightPlan {
   bool few, one;
   int rows, pitch, ranges, row_tiles, wr, splits, keys;
 };
+// Up to 16 rows (an operand's): 16 sequences of four tokens with groups of four over 4000 keys 35 us, as more rows 56.
+// One launch of those, a workgroup a key head, where scores fit and either keys are few or every CU has a head.  One token, groups of four, one launch / two: one sequence over 200 keys 5.9 / 8.8 us, eight over 600 9.3 / 9.5, over 960
+// 11.8 / 11.5; 32 over 1200 15.8 / 19.8, over 3800 45 / 50; 64 over 3800 89 / 103; but 24 over 3800 38.9 / 36.2, 16 over 3800 35.5 / 25.5.
+// Ranges of keys of two launches: workgroups for 1024 of tokens, 512 of more rows (16 x 1 over up to 8000 keys with 512 / 1024 / 2048 58.6 / 56.7 / 54.8, a sequence of 4 over 4000 12.9 / 13.5 / 12.6; 6 x 32 fp32
+// over up to 7000 with 256 / 512 / 1024 91 / 83 / 87, 2 x 100 over 3000 66 / 59 / 67).  Where keys alone give fewer than 512 workgroups rows are split as well: 500 tokens over 4000 keys 73 us, unsplit 116.
 static WeightPlan weight_plan(bool f32, int64_t B, int heads, int kv, int D, int64_t max_tokens, int64_t max_keys) {
   WeightPlan p = {};
   const int64_t rows = max_tokens * (heads / kv);
