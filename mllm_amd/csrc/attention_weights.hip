@@ -42,7 +42,7 @@ struct WeightArgs {
   float* score;  // [B][kv][rows][pitch]
   int rows, pitch;
   f32x2* ml;     // few rows: [range][B][kv][rows]; more: [range][T][heads], maximum (times c) and sum
-  f32x2* row;    // [T][heads]: maximum (times c) and 1 / sum of all keys
+  f32x2* row;    // [T][heads]: maximum (times c) and 1 / sum of all keys; null where what needs them joins the ranges'
   float* part;   // [split][B][kv][pitch]: what keys get of a part of the rows
   int splits;
   uint16_t* parts;  // fp32 queries as three bf16 parts, [3][T][heads][D]
@@ -528,13 +528,17 @@ __global__ __launch_bounds__(256) void weights_join_kernel(WeightArgs a) {
 
 // The weights: a wave has NK * 16 keys in registers, rows go by in LDS, 32 at a time (16 of 256 elements), the next ones on their way.  Where keys leave CUs idle rows are cut into
 // `splits`, whose sums a last launch adds.
-template <int KS, bool F32>
+// FEW: 64 keys a workgroup where those of the other form leave CUs idle and rows are too few to be split (one sequence of 16 tokens over 1000 keys, groups of four: 21.4 -> 17.8 us, four of 30 fp32 tokens over 800
+// 38 -> 33, but 500 tokens over 4000 75 -> 91).  It joins the maxima and sums of up to eight ranges of keys itself (16 over 1000 16.1 -> 14.1; the registers that takes would cost the other form a wave: 6 x 32 fp32
+// tokens over up to 7000 83 -> 89).
+enum { WEIGHT_JOIN = 8 };
+template <int KS, bool F32, bool FEW>
 struct Mass {
-  static constexpr int NK = KS < 8 ? 4 : F32 ? 1 : 2, RT = KS == 8 ? 16 : 32, KEYS = 4 * NK * 16;
+  static constexpr int MOST = KS < 8 ? 4 : F32 ? 1 : 2, NK = FEW ? 1 : MOST, RT = KS == 8 ? 16 : 32, KEYS = 4 * NK * 16;
 };
-template <int KS, bool F32>
+template <int KS, bool F32, bool FEW>
 __global__ __launch_bounds__(256, 2) void weights_mass_kernel(WeightArgs a) {
-  typedef Mass<KS, F32> P;
+  typedef Mass<KS, F32, FEW> P;
   constexpr int NK = P::NK, RT = P::RT, DP = KS * 32, C = DP / 8, PARTS = F32 ? 3 : 1, NL = (RT * C + 255) / 256;
   __shared__ __align__(16) uint16_t s_q[2][PARTS][RT * DP];
   __shared__ f32x2 s_row[2][RT];
@@ -547,7 +551,7 @@ __global__ __launch_bounds__(256, 2) void weights_mass_kernel(WeightArgs a) {
   const int heads = a.kv * a.group;
   // rows r0 .. r0 + RT - 1 on their way, 8 elements a piece
   u32x4 it[NL][PARTS];
-  f32x2 factor;
+  f32x2 factor[FEW ? WEIGHT_JOIN : 1];
   auto ask_rows = [&](int r0) {
 #pragma unroll
     for (int i = 0; i < NL; i++) {
@@ -564,7 +568,12 @@ __global__ __launch_bounds__(256, 2) void weights_mass_kernel(WeightArgs a) {
     }
     if (tid < RT) {
       const int r = r0 + tid, token = r / a.group;
-      factor = r < end ? a.row[(int64_t)(s.first + token) * heads + h * a.group + (r - token * a.group)] : f32x2{0.f, 0.f};
+      const int64_t at = (int64_t)(s.first + token) * heads + h * a.group + (r - token * a.group);
+      factor[0] = r < end ? (!FEW || a.row ? a.row[at] : a.ml[at]) : f32x2{0.f, 0.f};
+      if (FEW && !a.row) {
+#pragma unroll
+        for (int i = 1; i < (FEW ? WEIGHT_JOIN : 1); i++) factor[i] = r < end && i < a.ranges ? a.ml[(int64_t)i * a.T * heads + at] : f32x2{-INFINITY, 0.f};
+      }
     }
   };
   auto put_rows = [&](int half) {
@@ -575,7 +584,15 @@ __global__ __launch_bounds__(256, 2) void weights_mass_kernel(WeightArgs a) {
 #pragma unroll
       for (int j = 0; j < PARTS; j++) *reinterpret_cast<u32x4*>(&s_q[half][j][r * DP + (p ^ swizzle<C>(r)) * 8]) = it[i][j];
     }
-    if (tid < RT) s_row[half][tid] = factor;
+    if (tid < RT) {
+      if (FEW && !a.row) {
+        float m = factor[0].x, l = factor[0].y;
+#pragma unroll
+        for (int i = 1; i < (FEW ? WEIGHT_JOIN : 1); i++) join(m, l, factor[i].x, factor[i].y);
+        factor[0] = final_row(m, l);
+      }
+      s_row[half][tid] = factor[0];
+    }
   };
   if (begin < end) ask_rows(begin);
   const int32_t* table = a.table + b * a.table_stride;
@@ -680,14 +697,15 @@ __global__ __launch_bounds__(256) void weights_add_kernel(WeightArgs a) {
 
 // ---- host side ------------------------------------------------------------------------------------------------------------
 struct WeightPlan {
-  bool few, one;
+  bool few, one, few_keys;
   int rows, pitch, ranges, row_tiles, wr, splits, keys;
 };
 // Up to 16 rows (an operand's): 16 sequences of four tokens with groups of four over 4000 keys 35 us, as more rows 56.
 // One launch of those, a workgroup a key head, where scores fit and either keys are few or every CU has a head.  One token, groups of four, one launch / two: one sequence over 200 keys 5.9 / 8.8 us, eight over 600 9.3 / 9.5, over 960
 // 11.8 / 11.5; 32 over 1200 15.8 / 19.8, over 3800 45 / 50; 64 over 3800 89 / 103; but 24 over 3800 38.9 / 36.2, 16 over 3800 35.5 / 25.5.
 // Ranges of keys of two launches: workgroups for 1024 of tokens, 512 of more rows (16 x 1 over up to 8000 keys with 512 / 1024 / 2048 58.6 / 56.7 / 54.8, a sequence of 4 over 4000 12.9 / 13.5 / 12.6; 6 x 32 fp32
-// over up to 7000 with 256 / 512 / 1024 91 / 83 / 87, 2 x 100 over 3000 66 / 59 / 67).  Where keys alone give fewer than 512 workgroups rows are split as well: 500 tokens over 4000 keys 73 us, unsplit 116.
+// over up to 7000 with 256 / 512 / 1024 91 / 83 / 87, 2 x 100 over 3000 66 / 59 / 67), of 256 keys or, of more rows and 257 to 1024 keys, 128 (16 over 1000 17.8 -> 15.5, 2 x 60 over 500 23.1 -> 21.5, but 8 x 8 over 700
+// 17.5 -> 17.8, and over 8000 29.7 -> 33).  Where keys alone give fewer than 512 workgroups rows are split as well: 500 tokens over 4000 keys 73 us, unsplit 116.
 static WeightPlan weight_plan(bool f32, int64_t B, int heads, int kv, int D, int64_t max_tokens, int64_t max_keys) {
   WeightPlan p = {};
   const int64_t rows = max_tokens * (heads / kv);
@@ -699,9 +717,11 @@ static WeightPlan weight_plan(bool f32, int64_t B, int heads, int kv, int D, int
   const int64_t wave = weight_nq(D > 128 ? 8 : 4, f32) * 16;
   p.wr = rows <= wave ? 1 : rows <= 2 * wave ? 2 : 4;
   p.row_tiles = p.few ? 1 : (int)((rows + p.wr * wave - 1) / (p.wr * wave));
-  const int64_t uncut = B * kv * p.row_tiles, most = (max_keys + 255) / 256, wanted = p.few ? (1023 + uncut) / uncut : (511 + uncut) / uncut;
+  const int64_t uncut = B * kv * p.row_tiles, least = p.few || max_keys <= 256 || max_keys > 1024 ? 256 : 128, most = (max_keys + least - 1) / least, wanted = p.few ? (1023 + uncut) / uncut : (511 + uncut) / uncut;
   p.ranges = (int)(uncut >= 1024 || most < 2 ? 1 : wanted < most ? wanted : most);
-  p.keys = D <= 128 ? Mass<4, false>::KEYS : f32 ? Mass<8, true>::KEYS : Mass<8, false>::KEYS;
+  const int most_keys = D <= 128 ? Mass<4, false, false>::KEYS : f32 ? Mass<8, true, false>::KEYS : Mass<8, false, false>::KEYS, few_keys = Mass<4, false, true>::KEYS;
+  p.few_keys = !p.few && most_keys > few_keys && B * kv * ((max_keys + most_keys - 1) / most_keys) < 256 && rows <= 256;
+  p.keys = p.few_keys ? few_keys : most_keys;
   const int64_t groups = B * kv * ((max_keys + p.keys - 1) / p.keys), parts = (rows + 127) / 128, split = (511 + groups) / groups;
   p.splits = (int)(p.few || groups >= 512 || parts < 2 ? 1 : split < parts ? split : parts);
   return p;
@@ -834,9 +854,11 @@ MLLM_API int mllm_hip_attention_weights(const mllm_hip_heads* q, int dtype, int6
     else hipLaunchKernelGGL(weights_sum_kernel<16>, sums, dim3(256), 0, st, a);
     return (int)hipGetLastError();
   }
-  a.row = reinterpret_cast<f32x2*>(workspace);
-  a.ml = a.row + (size_t)T * heads;
-  a.part = reinterpret_cast<float*>(a.row + (size_t)(p.ranges > 1 ? p.ranges + 1 : 1) * T * heads);
+  const bool joined = p.few_keys && p.ranges > 1 && p.ranges <= WEIGHT_JOIN;
+  f32x2* const room = reinterpret_cast<f32x2*>(workspace);
+  a.row = joined ? nullptr : room;
+  a.ml = room + (size_t)T * heads;
+  a.part = reinterpret_cast<float*>(room + (size_t)(p.ranges > 1 ? p.ranges + 1 : 1) * T * heads);
   a.splits = p.splits;
   if (f32) {
     const uintptr_t behind = reinterpret_cast<uintptr_t>(a.part) + (p.splits > 1 ? (size_t)p.splits * B * cache->heads * p.pitch * sizeof(float) : 0);
@@ -848,11 +870,13 @@ MLLM_API int mllm_hip_attention_weights(const mllm_hip_heads* q, int dtype, int6
   if (p.wr == 1) KSTEPS(grid, weights_max_kernel<KS, 1, F32>)
   else if (p.wr == 2) KSTEPS(grid, weights_max_kernel<KS, 2, F32>)
   else KSTEPS(grid, weights_max_kernel<KS, 4, F32>)
-  if (p.ranges > 1) {
+  if (p.ranges > 1 && !joined) {
     hipLaunchKernelGGL(weights_join_kernel, dim3((unsigned)((T * heads + 255) / 256)), dim3(256), 0, st, a);
     RC_RET((int)hipGetLastError());
   }
-  KSTEPS(dim3((unsigned)((max_keys + p.keys - 1) / p.keys), heads_of_all, (unsigned)p.splits), weights_mass_kernel<KS, F32>)
+  const dim3 mass_grid((unsigned)((max_keys + p.keys - 1) / p.keys), heads_of_all, (unsigned)p.splits);
+  if (p.few_keys) KSTEPS(mass_grid, weights_mass_kernel<KS, F32, KS < 8 || !F32>)
+  else KSTEPS(mass_grid, weights_mass_kernel<KS, F32, false>)
 #undef KSTEPS
   if (p.splits > 1) {
     hipLaunchKernelGGL(weights_add_kernel, dim3((unsigned)((max_keys + 255) / 256), heads_of_all), dim3(256), 0, st, a);

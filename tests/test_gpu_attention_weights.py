@@ -79,6 +79,19 @@ def test_against_the_formula(counts, prefixes, Hq, Hkv, D, page, dtype, decay):
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("D", [64, 80, 128, 256])
+@pytest.mark.parametrize("tokens,longest,Hq", [(1, 1900, 16), (2, 959, 64), (2, 961, 64), (3, 70, 8), (20, 330, 8), (70, 45, 16)])
+def test_many_sequences(tokens, longest, Hq, D, dtype):
+    """as many key heads as CUs and more; among the sequences some without tokens or prefix"""
+    announce("attention_weights many", tokens, longest, Hq, D, dtype)
+    n = 33
+    counts = [tokens if b % 5 else b % 2 for b in range(n)]
+    prefixes = [longest if b == 7 else (b * 97) % (longest // 2) if b % 4 else 0 for b in range(n)]
+    c = Case(counts, prefixes, Hq, 8, D, 16, dtype, seed=tokens + D)
+    c.check(c.run(decay=0.75), 0.75)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 @pytest.mark.parametrize("counts,prefixes", [([3, 2], [70, 300]), ([30, 12], [70, 300])])
 def test_bounds_of_tokens_keys_and_masses(counts, prefixes, dtype):
     announce("attention_weights bounds", counts, prefixes, dtype)
