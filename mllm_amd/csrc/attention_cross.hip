@@ -6,13 +6,13 @@
 // key head) and eight consecutive keys, which is what the second operand of O^T = V^T P^T takes.  Scores, maxima, sums and O are fp32; P is rounded to bf16 for
 // the product with V (off by 2^-8 of each weight at most, of either sign), fp32 queries and their P enter as three bf16 parts each.
 //
-// Two forms.  Up to 64 rows of a sequence and key head, fp32 queries and heads of more than 128 elements: cross_kernel, on products of 16 x 16 x 32.  A workgroup has four waves, WR along rows times
+// Two forms.  Up to 64 rows of a sequence and key head or keys of a sequence, fp32 queries and heads of more than 128 elements: cross_kernel, on products of 16 x 16 x 32.  A workgroup has four waves, WR along rows times
 // 4 / WR along keys, and goes through the keys in tiles of 64: 16-byte loads into registers while the tile before them is worked on, from there into LDS.  Heads of 72 or 80 elements take three
 // steps of 32 in the first product (zeros behind them) and five tiles of 16 in the second.  More bf16 rows: cross_wide_kernel, on products of 32 x 32 x 16, keys and values from memory to LDS directly.
 // Where rows, heads and sequences leave CUs idle the keys are cut into pieces, whose O, maximum and sum meet in the workspace; a second launch joins them.
 //
 // What bounds it.  Few rows: memory, behind the chain of two launches (64 sequences of one token over 1601 keys, 32 query and 8 key heads of 128, 74 us: 4.4 TB/s where a copy of 2 GB has 5.18; four
-// fp32 tokens over 1601 keys 15.4, of which the join takes 3.9).  64 x 64 windows of 160 images, 16 heads of 80: 23 us, 3.4 TB/s.  Many rows: matrix and vector instructions, which share a SIMD's issue and overlap only
+// fp32 tokens over 1601 keys 15.4, of which the join takes 3.9).  64 x 64 windows of 160 images, 16 heads of 80: 20 us, 3.9 TB/s.  Many rows: matrix and vector instructions, which share a SIMD's issue and overlap only
 // in part, at the clock that both leave (1.8 GHz): 4900 tokens over 4900 keys, 16 heads of 80, 157 us (780 TFLOP/s; a product of 8192^3 has 1229), 3 x 700 tokens over up to 6404 keys, 32 heads of 128, 155 to 180
 // (730 to 850), 10 000 over 10 000, four query heads a key head, 550 (930).  Matrix pipes are busy 45 % of the time, no LDS read meets a taken bank.
 // Next tile's scores between this one's exponents (a third more registers) and four waves a SIMD (spills) were no faster; equal shares of the keys of all tiles per CU, whose parts are joined, cost 24 us to join.
@@ -130,7 +130,10 @@ __device__ __forceinline__ void cross_put(const CrossArgs& a, const CrossPlace& 
   else *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(a.o) + at) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
 }
 
-template <int DP, int DT, int WR, bool F32>
+// ONE: sequences of one tile of keys, as the host says.  Half the LDS and registers for no second tile leave room for six workgroups a CU instead of three, whose loads and stores overlap:
+// 160 windows of 64, 16 heads of 80, 23.8 -> 20.8 us, 300 of 49 and 72 33.6 -> 25.6, 100 fp32 ones of 80 30.2 -> 22.9.  More rows than 64 as well, which the other form has by 128: 4000 tokens over 64 keys, heads of 128,
+// 14.6 -> 13.5, 20 x 300 19.1 -> 17.4 (4 x 400 over 40 8.3 both).
+template <int DP, int DT, int WR, bool F32, bool ONE>
 struct Cross {
   static constexpr int WK = 4 / WR;          // waves along keys
   static constexpr int KT = 64;              // keys of a tile
@@ -138,19 +141,20 @@ struct Cross {
   static constexpr int C = DP / 8;           // 16-byte pieces of a row
   static constexpr int NLOAD = KT * C / 256; // pieces of a tile that a lane loads, of keys and of values
   static constexpr int PARTS = F32 ? 3 : 1;
-  static constexpr int WAVES = DP == 256 ? 1 : 2;
+  static constexpr int WAVES = DP == 256 ? 1 : ONE ? 3 : 2;
   // Rows of 8 and of 16 or 32 pieces begin in the same banks every second or every row; rows of 12 every fourth.
   static __device__ __forceinline__ int swz(int row) {
     return C == 12 ? (row >> 3) & 3 : C == 8 ? (row & 3) | ((row >> 3) & 1) << 2 : (row & 3) | ((row >> 3) & 3) << 2;
   }
 };
 
-template <int DP, int DT, int WR, bool F32>
-__global__ __launch_bounds__(256, (Cross<DP, DT, WR, F32>::WAVES)) void cross_kernel(CrossArgs a) {
-  typedef Cross<DP, DT, WR, F32> P;
+template <int DP, int DT, int WR, bool F32, bool ONE>
+__global__ __launch_bounds__(256, (Cross<DP, DT, WR, F32, ONE>::WAVES)) void cross_kernel(CrossArgs a) {
+  typedef Cross<DP, DT, WR, F32, ONE> P;
   constexpr int KT = P::KT, C = P::C, WK = P::WK, NLOAD = P::NLOAD, KS = DP / 32, PARTS = P::PARTS;
-  __shared__ __align__(16) uint16_t s_k[2 * KT * DP];
-  __shared__ __align__(16) uint16_t s_v[2 * KT * DP];
+  constexpr int HALVES = ONE ? 1 : 2;  // of LDS: tiles in turn
+  __shared__ __align__(16) uint16_t s_k[HALVES * KT * DP];
+  __shared__ __align__(16) uint16_t s_v[HALVES * KT * DP];
   CrossPlace place;
   if (!cross_place(a, place)) return;
   const CrossSeq& s = place.s;
@@ -173,7 +177,7 @@ __global__ __launch_bounds__(256, (Cross<DP, DT, WR, F32>::WAVES)) void cross_ke
     voff[i] = r * a.v_bytes + p * 16;
     if (!has[i]) {
 #pragma unroll
-      for (int half = 0; half < 2; half++) {
+      for (int half = 0; half < HALVES; half++) {
         *reinterpret_cast<u32x4*>(s_k + half * KT * DP + to[i]) = u32x4{0, 0, 0, 0};
         *reinterpret_cast<u32x4*>(s_v + half * KT * DP + to[i]) = u32x4{0, 0, 0, 0};
       }
@@ -207,8 +211,11 @@ __global__ __launch_bounds__(256, (Cross<DP, DT, WR, F32>::WAVES)) void cross_ke
   const bool live = own < rows;
   const int token = live ? own / a.group : 0, head = h * a.group + (live ? own - token * a.group : 0);
   const int64_t q_at = (s.first + token) * a.q_token + head * a.q_head + 8 * g;
+  auto load_q = [&](int64_t at, bool there) {
 #pragma unroll
-  for (int ks = 0; ks < KS; ks++) query_parts<F32>(a.q, q_at + 32 * ks, live && 32 * ks + 8 * g < a.D, fq[ks]);
+    for (int ks = 0; ks < KS; ks++) query_parts<F32>(a.q, at + 32 * ks, there && 32 * ks + 8 * g < a.D, fq[ks]);
+  };
+  load_q(q_at, live);
 #pragma unroll
   for (int ks = 0; ks < KS; ks++)
 #pragma unroll
@@ -311,28 +318,52 @@ __global__ __launch_bounds__(256, (Cross<DP, DT, WR, F32>::WAVES)) void cross_ke
   int k0 = k_begin;  // the tile that is worked on
   if (k_begin < k_end) {
     put_tile(Lower());
-    if (k_begin + KT < k_end) ask_tile(k_begin + KT);
+    if (!ONE && k_begin + KT < k_end) ask_tile(k_begin + KT);
     __syncthreads();
   }
-  auto turn = [&](auto last_, auto half, auto other) {
-    if (busy) work(k0, last_, half);
-    k0 += KT;
-    if (k0 < k_end) {  // into the other half of LDS: everyone is past the tile that was there
-      put_tile(other);
-      if (k0 + KT < k_end) ask_tile(k0 + KT);
+  if constexpr (ONE) {
+    if (busy && k0 < k_end) work(k0, std::true_type(), Lower());
+    // More keys than the host said: a tile at a time.  Where it lies and the rows of Q are found once more: they would else stay in registers, which costs most of what this form gains.
+    for (k0 += KT; k0 < k_end; k0 += KT) {
+      int t = tid;
+      asm volatile("" : "+v"(t));
       __syncthreads();
+#pragma unroll 1
+      for (int e = t; e < KT * C; e += 256) {
+        const int r = e / C, p = e % C, there = r * DP + (p ^ P::swz(r)) * 8;
+        if (p >= real) continue;
+        const bool good = k0 + r < k_end;
+        *reinterpret_cast<u32x4*>(s_k + there) = *reinterpret_cast<global_row>(good ? k_at + (uint64_t)(k0 + r) * a.k_bytes + p * 16 : zero);
+        *reinterpret_cast<u32x4*>(s_v + there) = *reinterpret_cast<global_row>(good ? v_at + (uint64_t)(k0 + r) * a.v_bytes + p * 16 : zero);
+      }
+      __syncthreads();
+      const int row = row0 + wr * 16 + (t & 15);
+      const bool has_row = row < rows;
+      const int of = has_row ? row / a.group : 0;
+      load_q((s.first + of) * a.q_token + (h * a.group + (has_row ? row - of * a.group : 0)) * a.q_head + 8 * (t >> 4 & 3), has_row);
+      if (busy) work(k0, std::true_type(), Lower());
     }
-  };
-  // Whole tiles in turns whose halves of LDS are constants; then, in code of its own, the one that may end before its last key.
-  int half = 0;
-  while (k0 + KT <= k_end) {
-    turn(std::false_type(), Lower(), Upper());
-    half = 1;
-    if (k0 + KT > k_end) break;
-    turn(std::false_type(), Upper(), Lower());
-    half = 0;
+  } else {
+    auto turn = [&](auto last_, auto half, auto other) {
+      if (busy) work(k0, last_, half);
+      k0 += KT;
+      if (k0 < k_end) {  // into the other half of LDS: everyone is past the tile that was there
+        put_tile(other);
+        if (k0 + KT < k_end) ask_tile(k0 + KT);
+        __syncthreads();
+      }
+    };
+    // Whole tiles in turns whose halves of LDS are constants; then, in code of its own, the one that may end before its last key.
+    int half = 0;
+    while (k0 + KT <= k_end) {
+      turn(std::false_type(), Lower(), Upper());
+      half = 1;
+      if (k0 + KT > k_end) break;
+      turn(std::false_type(), Upper(), Lower());
+      half = 0;
+    }
+    if (k0 < k_end) turn(std::true_type(), half, half ^ 1);
   }
-  if (k0 < k_end) turn(std::true_type(), half, half ^ 1);
   l = sum32(sum16(l));
 
   auto put = [&](int row, int d, at_f32x4 x, float mm, float sum) {
@@ -645,6 +676,7 @@ __global__ __launch_bounds__(256) void cross_join_kernel(CrossArgs a) {
 struct CrossPlan {
   int nq, wr, row_tiles, rows_of_tile, pieces, min_tiles;
   int64_t whole, tiles;
+  bool one;  // tile of keys a sequence
 };
 // Rows of a wave by the rows there are: 16, 32, and 64 where heads are of 96 elements at most, there is work for all CUs and the last tile's idle rows weigh little (each row of LDS read is
 // used twice, a SIMD has two waves instead of three or four.  Heads of 80, 64 / 32 rows: 16 heads, 7000 tokens 302 / 348 us, 64 sequences of 200 tokens 32.1 / 39.1; but 8 of 1100
@@ -657,8 +689,9 @@ static CrossPlan cross_plan(bool f32, int64_t B, int heads, int kv, int64_t max_
   if (max_keys > 0x7fffffff) max_keys = 0x7fffffff;
   const int64_t rows = max_tokens * (heads / kv);
   const int64_t narrow = (rows + 127) / 128, twice = (narrow + 1) / 2;
-  p.nq = rows <= 64 || f32 || D > 128 ? 1 : D > 96 || twice * B * kv < 384 || (narrow % 2 && narrow < 20) ? 2 : 4;
+  p.nq = rows <= 64 || f32 || D > 128 || max_keys <= 64 ? 1 : D > 96 || twice * B * kv < 384 || (narrow % 2 && narrow < 20) ? 2 : 4;
   p.wr = rows <= 32 ? 2 : 4;
+  p.one = max_keys <= 64;
   p.rows_of_tile = p.nq * 16 * p.wr;
   const int64_t per = p.rows_of_tile, row_tiles = (rows + per - 1) / per;
   p.row_tiles = (int)row_tiles;
@@ -677,8 +710,11 @@ static size_t cross_room(const CrossPlan& p, int D) { return (size_t)(p.tiles - 
 template <int DP, int DT, int DK>
 static void cross_launch(const CrossPlan& p, bool f32, dim3 grid, hipStream_t st, const CrossArgs& a) {
   auto go = [&](auto kern) { hipLaunchKernelGGL(kern, grid, dim3(256), 0, st, a); };
-  if (f32) return p.wr == 2 ? go(cross_kernel<DP, DT, 2, true>) : go(cross_kernel<DP, DT, 4, true>);
-  if (p.nq == 1) return p.wr == 2 ? go(cross_kernel<DP, DT, 2, false>) : go(cross_kernel<DP, DT, 4, false>);
+  if constexpr (DK > 0) {
+    if (p.nq == 1 && p.wr == 4 && p.one) return f32 ? go(cross_kernel<DP, DT, 4, true, true>) : go(cross_kernel<DP, DT, 4, false, true>);
+  }
+  if (f32) return p.wr == 2 ? go(cross_kernel<DP, DT, 2, true, false>) : go(cross_kernel<DP, DT, 4, true, false>);
+  if (p.nq == 1) return p.wr == 2 ? go(cross_kernel<DP, DT, 2, false, false>) : go(cross_kernel<DP, DT, 4, false, false>);
   if constexpr (DK > 0) {
     constexpr int D2 = (DK + 1) / 2;
     const bool full = a.D == 16 * DK;

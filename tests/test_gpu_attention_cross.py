@@ -135,6 +135,19 @@ def test_any_bound_of_keys(bound, dtype):
     c.check(c.run(max_keys=bound))
 
 
+@pytest.mark.parametrize("D", [64, 72, 96, 128, 256])
+@pytest.mark.parametrize("counts,held,group", [([64, 64, 64, 50], [64, 64, 64, 50], 1), ([49, 0, 49], [49, 3, 0], 2), ([400, 65, 1, 33], [64, 1, 33, 0], 1), ([30, 17], [63, 64], 3)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_one_tile_of_keys(counts, held, group, D, dtype):
+    """and sequences that have more than the host's bound"""
+    announce("attention_cross one tile", counts, held, group, D, dtype)
+    c = Case(counts, held, 2 * group, 2, D, dtype, seed=D + len(counts))
+    c.check(c.run())
+    c = Case(counts, [n * 3 + 1 for n in held], 2 * group, 2, D, dtype, seed=D)
+    for bound in (1, 64):
+        c.check(c.run(max_keys=bound))
+
+
 def test_sequences_that_share_keys_and_keys_that_are_not_there():
     announce("attention_cross shared")
     for dtype in (torch.float32, torch.bfloat16):
