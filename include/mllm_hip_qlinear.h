@@ -720,7 +720,8 @@ int mllm_hip_kv_evict(const mllm_hip_kv_cache* cache, const float* mass, int64_t
  * included; an infinity or a NaN among a token's values makes that element of its result infinite or NaN.  Finite scores times scale are below 2^30.
  * q->x, q->y: F32 or BF16 (weight is not looked at); rows of q in no sequence, and those behind a sequence's first max_tokens, stay as they are in y.  y may not be x.
  * head_dim % 8 == 0, <= 256 (64, 80, 96, 128 and 256 are what the kernels are made for, others take the next); heads a multiple of kv->heads; 0 < scale <= 2e38.
- * max_keys: the host's bound of a sequence's keys (any; it decides into how many pieces keys are cut).  fp32 results are within fp32 sums of the formula, bf16 ones take the weights p in bf16.
+ * max_keys: the host's bound of a sequence's keys (any; it decides into how many pieces keys are cut, and up to 64 takes a form made for that many: more keys than it says count all the same, at
+ * less than full speed).  fp32 results are within fp32 sums of the formula, bf16 ones take the weights p in bf16.
  * workspace: ..._workspace_bytes (0: none), 16-byte aligned; less is MLLM_HIP_E_BADARG.  One launch, two where keys are cut. */
 typedef struct mllm_hip_states { /* keys and values in bf16: key j of head h at element j * k_stride + h * k_head_stride of k, head_dim elements in a row; v likewise */
   const void* k;

@@ -712,7 +712,7 @@ def attention_cross(q, k, v, cu_tokens, key_first, key_count, max_tokens, max_ke
     """softmax(scale * q k^T) v over an encoder's states: q [T, Hq, D] fp32 or bf16, k and v bf16 [S, Hkv, D] (D of whole eights up to 256; any strides of whole 16 bytes); rows
     cu_tokens[b] .. cu_tokens[b + 1] - 1 (int32 [B + 1]) of q see key_count[b] keys from key_first[b] on (int32 [B]), all of them, whatever their order.  An encoder's
     own attention, whole or in windows, has cu_tokens[:-1] and their lengths there; sequences may share keys.  max_tokens, max_keys: bounds of a sequence's tokens (those
-    behind it are left out) and keys (decides how keys are cut).  scale: 1 / sqrt(D).  A token without keys gets zeros; rows in no sequence are left as they are in `out`."""
+    behind it are left out) and keys (decides the form and how keys are cut; more count all the same).  scale: 1 / sqrt(D).  A token without keys gets zeros; rows in no sequence are left as they are in `out`."""
     return _calls().attention_cross(q, k, v, cu_tokens, key_first, key_count, max_tokens, max_keys, scale, out, workspace)
 
 
