@@ -548,6 +548,10 @@ __global__ __launch_bounds__(256, 2) void weights_mass_kernel(WeightArgs a) {
   const int rows = s.n * a.group, kg = blockIdx.x * P::KEYS, k0 = kg + wave * NK * 16;
   if (rows == 0 || kg >= s.keys) return;
   const int per = ((rows + a.splits - 1) / a.splits + RT - 1) / RT * RT, begin = max(split * per, max(kg - s.prefix, 0) * a.group / RT * RT), end = min(split * per + per, rows);
+  // Sixteens of rows from row `plain` on, plain_rows of them, need no masks: each sees all of the wave's keys, and all sixteen are there.  (One that is not would add what its zeros make of an infinite
+  // element of a key, which is no number.)
+  const int plain = max(k0 + NK * 16 - 1 - s.prefix, 0) * a.group;
+  const uint32_t plain_rows = max(end - 15 - plain, 0);
   const int heads = a.kv * a.group;
   // rows r0 .. r0 + RT - 1 on their way, 8 elements a piece
   u32x4 it[NL][PARTS];
@@ -649,7 +653,7 @@ __global__ __launch_bounds__(256, 2) void weights_mass_kernel(WeightArgs a) {
         }
       }
       const f32x2 row = s_row[half][rb * 16 + col];
-      if (k0 + NK * 16 <= s.prefix + r / a.group + 1) {  // the first of these rows sees all of the wave's keys, so all do
+      if ((uint32_t)(r - plain) < plain_rows) {
 #pragma unroll
         for (int i = 0; i < NK; i++)
 #pragma unroll

@@ -146,6 +146,29 @@ def test_infinities_and_nans(counts, dtype):
     assert torch.isnan(got[0, 0, 0]) and torch.isfinite(got[0, 0, 1:n]).all() and torch.isfinite(got[1]).all()
 
 
+# (sequences, tokens of the first, heads of a group, key heads, positions before them): row numbers that are no multiple of 16, with 64 keys a workgroup or more, rows in one piece or several
+@pytest.mark.parametrize("seqs,tokens,group,kv,prefix", [(1, 41, 2, 1, 300), (2, 17, 1, 2, 300), (1, 7, 5, 2, 900), (1, 131, 2, 1, 300), (40, 17, 2, 8, 300), (40, 3, 7, 8, 300)])
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_an_infinite_key_and_rows_that_fill_no_sixteen(seqs, tokens, group, kv, prefix, D, dtype):
+    """a key whose scores are -inf for all that see it gets nothing, whatever is behind the last row"""
+    announce("attention_weights infinite, ragged rows", seqs, tokens, group, kv, prefix, D, dtype)
+    c = Case([tokens - b % 2 for b in range(seqs)], [prefix] * seqs, group * kv, kv, D, 16, dtype, seed=tokens + D)
+    c.q[:, :, 3] = c.q[:, :, 3].abs() + 0.5
+    c.k[(c.k == c.k).all(-1)[..., None] & (torch.arange(D, device="cuda") == 3)] = 0.5  # (places of no sequence stay NaN)
+    at = [(b, j) for b in range(seqs) for j in (0, 7, 100, prefix - 1)]
+    for b, j in at:
+        c.k[int(c.table[b, j // 16]), j % 16, :, 3] = -float("inf")
+    got = c.run(decay=0.0)
+    c.check(got, 0.0)
+    for b, j in at:
+        assert (got[b, :, j] == 0).all(), (b, j)
+    # the old masses go on as they were
+    got = c.run(decay=0.75)
+    for b, j in at:
+        assert torch.equal(got[b, :, j], c.old[b, :, j] * 0.75), (b, j)
+
+
 def test_pages_outside_the_cache_and_shared_pages():
     announce("attention_weights pages")
     for counts in ([2, 2], [30, 30]):
