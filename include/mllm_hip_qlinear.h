@@ -760,7 +760,7 @@ int mllm_hip_sample(const void* logits, int dtype, int64_t row_stride, int64_t r
  * others chosen.  bias_tokens int32, bias fp32 [rows][biases].  Tokens outside 0 .. vocab - 1 count for nothing.  masks uint32 [masks_count][ceil(vocab / 32)]; row r takes mask
  * mask_of[r], any number that is none of them: no mask; mask_of NULL: mask r, and there are masks_count >= rows of them.  repetition, presence, frequency fp32
  * [rows]; NULL: 1, 0, 0.  Strides in elements; those of inputs may be 0 (one for all rows).  A NaN stays one unless it is masked; a row whose mask leaves nothing is all -inf.
- * y is x with the same stride or shares no element with any input, its rows do not overlap.  vocab <= 2^24, rows <= 65535.  One launch, no workspace. */
+ * y is x with the same stride or shares no element with any input, its rows do not overlap.  vocab <= 2^24, rows <= 65535, history_len and biases <= 2^30.  One launch, no workspace. */
 typedef struct mllm_hip_logits {
   const void* x;
   void* y;

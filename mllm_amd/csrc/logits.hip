@@ -181,7 +181,7 @@ using namespace mllmhip;
 MLLM_API int mllm_hip_logits_adjust(const mllm_hip_logits* l, int dtype, int64_t rows, int64_t vocab, void* stream) {
   if (!l || (dtype != MLLM_HIP_F32 && dtype != MLLM_HIP_BF16) || rows < 0 || vocab < 1) return MLLM_HIP_E_BADARG;
   if (l->history_len < 0 || l->biases < 0 || l->masks_count < 0) return MLLM_HIP_E_BADARG;
-  if (vocab > (1 << 24) || rows > 65535 || l->history_len > 0x7fffffff || l->biases > 0x7ffffffe) return MLLM_HIP_E_SHAPE;
+  if (vocab > (1 << 24) || rows > 65535 || l->history_len > 0x40000000 || l->biases > 0x40000000) return MLLM_HIP_E_SHAPE;  // (the kernel's places go past the last by some thousands)
   if (rows == 0) return 0;
   if (!l->x || !l->y || (l->history_len && !l->history) || (l->biases && (!l->bias_tokens || !l->bias)) || (l->masks_count && !l->masks)) return MLLM_HIP_E_BADARG;
   if (l->masks_count && !l->mask_of && l->masks_count < rows) return MLLM_HIP_E_BADARG;

@@ -57,6 +57,12 @@ def test_logits_adjust(args, want):
     assert _adjust(**args) == want
 
 
+@pytest.mark.parametrize("args", [dict(history_len=(1 << 30) + 1), dict(history_len=(1 << 31) - 1), dict(history_len=(1 << 31) - 4096, lengths=None), dict(biases=(1 << 30) + 1), dict(biases=(1 << 31) - 2)])
+def test_logits_adjust_of_more_than_the_kernel_counts_to(args):
+    """places are 32-bit numbers there, which go some thousands past the last: histories and biases of up to 2^30"""
+    assert _adjust(**args) == SHAPE
+
+
 def test_logits_adjust_without_a_struct():
     assert _lib.lib().mllm_hip_logits_adjust(None, F32, 1, 10, None) == BADARG
 
