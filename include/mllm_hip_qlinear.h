@@ -727,7 +727,7 @@ typedef struct mllm_hip_states { /* keys and values in bf16: key j of head h at 
   const void* k;
   const void* v;
   int64_t k_stride, k_head_stride, v_stride, v_head_stride; /* multiples of 8, pointers 16-byte aligned; 0 <= k_stride, v_stride <= 2^23 */
-  int64_t keys;                                             /* rows that are there, < 2^31 */
+  int64_t keys;                                             /* rows that are there, <= 2^30 */
   int heads, head_dim;
 } mllm_hip_states;
 size_t mllm_hip_attention_cross_workspace_bytes(int dtype, int64_t T, int64_t B, int heads, int kv_heads, int head_dim, int64_t max_tokens, int64_t max_keys);

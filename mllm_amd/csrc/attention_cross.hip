@@ -753,8 +753,8 @@ MLLM_API int mllm_hip_attention_cross(const mllm_hip_heads* q, int dtype, int64_
                                       void* stream) {
   if (!q || !kv || kv->keys < 0 || !(scale > 0.f) || scale > 2e38f) return MLLM_HIP_E_BADARG;
   if (!cross_sizes(dtype, T, B, q->heads, kv->heads, kv->head_dim, max_tokens, max_keys)) return MLLM_HIP_E_BADARG;
-  if (!cross_shape(T, B, q->heads, kv->heads, kv->head_dim, max_tokens) || kv->keys > 0x7fffffff || kv->k_stride < 0 || kv->v_stride < 0 || kv->k_stride > (1 << 23) ||
-      kv->v_stride > (1 << 23))
+  if (!cross_shape(T, B, q->heads, kv->heads, kv->head_dim, max_tokens) || kv->keys > 0x40000000 || kv->k_stride < 0 || kv->v_stride < 0 || kv->k_stride > (1 << 23) ||
+      kv->v_stride > (1 << 23))  // (the kernels' places of keys go tiles past the last)
     return MLLM_HIP_E_SHAPE;
   if (T == 0 || B == 0 || max_tokens == 0) return 0;
   if (max_tokens > T) max_tokens = T;

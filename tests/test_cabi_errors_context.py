@@ -92,6 +92,13 @@ def test_attention_cross(args, want):
     assert _cross(**args) == want
 
 
+@pytest.mark.parametrize("keys", [(1 << 30) + 1, (1 << 31) - 64, (1 << 31) - 1])
+@pytest.mark.parametrize("stride", [512, 0])
+def test_attention_cross_of_more_keys_than_the_kernels_count_to(keys, stride):
+    """places of keys are 32-bit numbers there, which go tiles past the last: states of up to 2^30 rows"""
+    assert _cross(kv=_states(keys=keys, k_stride=stride, v_stride=stride)) == SHAPE
+
+
 def test_attention_cross_workspace():
     size = _lib.lib().mllm_hip_attention_cross_workspace_bytes
     assert size(BF16, 1, 1, 32, 8, 128, 1, 100) == 0 and size(BF16, 1, 1, 32, 8, 128, 1, 5000) > 0
