@@ -656,7 +656,7 @@ int mllm_hip_kv_append(const mllm_hip_heads* q, const mllm_hip_heads* k, const m
 
 /* The two calls above with positions on several axes (time, height and width of a picture's or a video's patches): pair j turns by the token's position on axis
  * axes[j], angle positions[axes[j] * axis_stride + t * token_stride] * inv_freq[j].  naxes 1 to 4 axes; axes int32 [rot_dim / 2] on the device, in any order; a
- * pair whose axis is none of 0 .. naxes - 1 is not turned.  With the same position on every axis: the results of the calls above, bit for bit. */
+ * pair whose axis is none of 0 .. naxes - 1 is not turned, whatever its frequency and its other element are.  With the same position on every axis: the results of the calls above, bit for bit. */
 int mllm_hip_qk_norm_rope_axes(int nparts, const mllm_hip_heads* parts, int dtype, int64_t T, int head_dim, float epsilon, int add_unit_offset,
                                const int32_t* positions, int64_t axis_stride, int64_t token_stride, int naxes, const int32_t* axes,
                                const double* inv_freq, int rot_dim, int interleaved, void* stream);

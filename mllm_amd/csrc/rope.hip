@@ -60,6 +60,7 @@ template <int XT, int G, bool NEXT, bool AXES>
 __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
   __shared__ __align__(16) float s_cos[256];
   __shared__ __align__(16) float s_sin[256];
+  __shared__ __align__(16) uint32_t s_other[AXES ? 256 : 4];  // 0 for a pair on no axis, whose elements do not look at one another (0 times infinity is no number), else ~0
   constexpr int H = 64 / G;
   const int tid = threadIdx.x, lane = tid & 63, lg = lane % G, e = lg * 8;
   const int64_t t = blockIdx.x;
@@ -99,6 +100,7 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
     if (p0 == 0 && half > 0) {
       if (tid < half) {
         int place = 0;
+        bool on = true;
         if (AXES) {
           // The token's positions are numbers of the scalar unit, asked for beside the pair's axis: with an address from it they would come one trip to memory later.
           const int32_t* at = a.positions + t * a.pos_token;
@@ -108,12 +110,15 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
             const int there = i < a.naxes ? at[i * a.pos_axis] : 0;
             place = axis == (uint32_t)i ? there : place;
           }
+          on = axis < (uint32_t)a.naxes;
+          s_other[tid] = on ? ~0u : 0;
         } else {
           place = a.positions[t];
         }
         // turns in fp64: p * f is off by 2^-53 of itself, which at 2^20 radians is 1e-10
         double turn = (double)place * a.inv_freq[tid] * 0.15915494309189533577;
         turn -= rint(turn);
+        if (!on) turn = 0;  // (whatever its frequency is)
         float sn, cs;
         sincospif(2.0f * (float)turn, &sn, &cs);
         s_cos[tid] = cs;
@@ -155,21 +160,31 @@ __global__ __launch_bounds__(256) void rope_kernel(RopeArgs a) {
 #pragma unroll
             for (int j = 0; j < 4; j++) {
               const float cs = s_cos[e / 2 + j], sn = s_sin[e / 2 + j], x = v[2 * j], y = v[2 * j + 1];
-              v[2 * j] = x * cs - y * sn;
-              v[2 * j + 1] = y * cs + x * sn;
+              const uint32_t other = AXES ? s_other[e / 2 + j] : ~0u;
+              v[2 * j] = x * cs - __uint_as_float(__float_as_uint(y) & other) * sn;
+              v[2 * j + 1] = y * cs + __uint_as_float(__float_as_uint(x) & other) * sn;
             }
           }
         } else {  // the other element of every pair is half / 8 lanes away
           const bool first = e < half;
           const int j0 = first ? e : e - half;
-          float o[8];
+          float o[8], w[8];  // (masked in front of the exchange: behind it the kernel takes 2 % longer, with a choice between results 10 %)
+#pragma unroll
+          for (int j = 0; j < 8; j++) w[j] = v[j];
+          if (AXES) {
+            const uint32_t* at = s_other + min(j0, 248);  // (of lanes behind the pairs: any, looked at by none)
+            const u32x4 m0 = *reinterpret_cast<const u32x4*>(at), m1 = *reinterpret_cast<const u32x4*>(at + 4);
+            const uint32_t m[8] = {m0.x, m0.y, m0.z, m0.w, m1.x, m1.y, m1.z, m1.w};
+#pragma unroll
+            for (int j = 0; j < 8; j++) w[j] = __uint_as_float(__float_as_uint(v[j]) & m[j]);
+          }
           if (half == 8 * (G / 2)) {  // (the whole of a head of 8 G elements: the usual one)
 #pragma unroll
-            for (int j = 0; j < 8; j++) o[j] = across<G / 2>(v[j]);
+            for (int j = 0; j < 8; j++) o[j] = across<G / 2>(w[j]);
           } else {
             const int from = first ? lane + half / 8 : lane - half / 8;
 #pragma unroll
-            for (int j = 0; j < 8; j++) o[j] = __shfl(v[j], from);
+            for (int j = 0; j < 8; j++) o[j] = __shfl(w[j], from);
           }
           if (turns) {
             const float4 c0 = *reinterpret_cast<const float4*>(s_cos + j0), c1 = *reinterpret_cast<const float4*>(s_cos + j0 + 4);

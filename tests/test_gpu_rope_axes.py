@@ -89,6 +89,34 @@ def test_one_position_on_every_axis_and_axes_that_are_not_there():
         assert torch.equal(yq[..., j], q[..., j]) and torch.equal(yk[..., j], k[..., j])
 
 
+@pytest.mark.parametrize("D,rot,interleaved", [(64, 64, False), (80, 64, False), (128, 128, False), (128, 128, True), (128, 32, False), (256, 256, True), (512, 512, False)])
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T", [3, 700])
+def test_pairs_on_no_axis_stay_as_they_are(T, D, rot, interleaved, dtype):
+    """bit for bit, whatever the other element of the pair and its frequency are; alone and on the way into a cache"""
+    announce("qk_norm_rope axes: pairs on none", T, D, rot, interleaved, dtype)
+    gen = torch.Generator(device="cuda").manual_seed(T + D)
+    inf, half = float("inf"), rot // 2
+    x = torch.randn((T, 8, D), device="cuda", generator=gen).to(dtype)
+    pos, f, axes = torch.randint(1, 50000, (3, T), device="cuda", generator=gen).int(), _freq(rot), _axes(half, 3, "turns")
+    still = [1, 2, half - 1]
+    axes[still] = torch.tensor([3, -1, 2 ** 31 - 1], dtype=torch.int32, device="cuda")
+    f[1], f[half - 1] = inf, float("nan")
+    first, second = [[2 * j + i if interleaved else j + i * half for j in still] for i in range(2)]
+    x[0, :, first[0]], x[1, :, second[1]], x[-1, 2, first[2]], x[1, 3, second[0]], x[2, 1, first[1]] = inf, -inf, inf, float("nan"), -0.0
+    q, k = x[:, :6], x[:, 6:]
+    same = lambda a, b: torch.equal(a.contiguous().view(torch.int16), b.contiguous().view(torch.int16))  # noqa: E731
+    kc, vc = [torch.zeros((T, 1, 2, D), dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    yq, yk = ql.qk_norm_rope(q, k, pos, f, interleaved=interleaved, axes=axes)
+    zq = ql.kv_append(k, k, kc, vc, torch.arange(T, device="cuda"), pos, f, None, q, None, interleaved=interleaved, axes=axes)
+    for d in first + second:
+        assert same(yq[..., d], q[..., d]) and same(yk[..., d], k[..., d]) and same(zq[..., d], q[..., d]) and torch.equal(kc[:, 0, :, d].nan_to_num(9.0), k[..., d].bfloat16().nan_to_num(9.0)), d
+    rest = [d for d in range(D) if d not in first + second]
+    for y, x0 in ((yq, q), (yk, k), (zq, q)):
+        want, size = norm_rope_axes(x0.nan_to_num(0.0, 0.0, 0.0), None, 1e-6, pos, axes, f, interleaved)
+        _check(y[..., rest], want[..., rest], size[..., rest], dtype)
+
+
 def test_a_captured_call_takes_new_positions():
     announce("qk_norm_rope axes in a graph")
     gen = torch.Generator(device="cuda").manual_seed(6)
