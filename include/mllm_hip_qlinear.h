@@ -693,6 +693,7 @@ int mllm_hip_attention_paged(const mllm_hip_heads* q, int dtype, int64_t T, cons
  *   mass[b * mass_stride + h * mass_head_stride + j] = (j < prefix[b] ? decay * mass[..] : 0) + sum over the tokens t that see j and the query heads of the group of
  *       exp(scale * (q . k_j) - max) / (their sum over the keys that t sees)
  * in fp32, decay 1: added up over calls, 0: mass is not read before.  Tokens that see nothing, or scores of -inf alone, add nothing; a NaN among a token's scores makes NaN of what all its keys get.
+ * Finite scores times scale are below 2^30.
  * Sequences without new tokens and positions from prefix + new tokens on stay as they are.  max_tokens, max_keys: a sequence's new tokens behind the first max_tokens add
  * nothing; positions from max_keys on are neither seen nor get anything; positions from mass_len on are seen, and what they get is stored nowhere.  q: F32 or BF16 (y and weight are not looked at).
  * head_dim % 8 == 0, <= 256; heads a multiple of the cache's; 0 < scale <= 2e38; 0 <= decay <= 2e38; table_len * page_size and max_keys up to 2^30, B * kv heads up to 65535.  The sums do not depend on any order of execution: the same

@@ -11,10 +11,10 @@
 // steps of 32 in the first product (zeros behind them) and five tiles of 16 in the second.  More bf16 rows: cross_wide_kernel, on products of 32 x 32 x 16, keys and values from memory to LDS directly.
 // Where rows, heads and sequences leave CUs idle the keys are cut into pieces, whose O, maximum and sum meet in the workspace; a second launch joins them.
 //
-// What bounds it.  Few rows: memory, behind the chain of two launches (64 sequences of one token over 1601 keys, 32 query and 8 key heads of 128, 74 us: 4.4 TB/s where a copy of 2 GB has 5.18; four
+// What bounds it.  Few rows: memory, behind the chain of two launches (64 sequences of one token over 1601 keys, 32 query and 8 key heads of 128, 74 to 79 us: 4.1 to 4.4 TB/s where a copy of 2 GB has 5.18; four
 // fp32 tokens over 1601 keys 15.4, of which the join takes 3.9).  64 x 64 windows of 160 images, 16 heads of 80: 20 us, 3.9 TB/s.  Many rows: matrix and vector instructions, which share a SIMD's issue and overlap only
 // in part, at the clock that both leave (1.8 GHz): 4900 tokens over 4900 keys, 16 heads of 80, 157 us (780 TFLOP/s; a product of 8192^3 has 1229), 3 x 700 tokens over up to 6404 keys, 32 heads of 128, 155 to 180
-// (730 to 850), 10 000 over 10 000, four query heads a key head, 550 (930).  Matrix pipes are busy 45 % of the time, no LDS read meets a taken bank.
+// (730 to 850), 10 000 over 10 000, four query heads a key head, 550 (930).  The wide form's matrix pipes are busy 43 to 48 % of the time, and none of its LDS reads meets a taken bank.
 // Next tile's scores between this one's exponents (a third more registers) and four waves a SIMD (spills) were no faster; equal shares of the keys of all tiles per CU, whose parts are joined, cost 24 us to join.
 #include <type_traits>
 
@@ -130,7 +130,7 @@ __device__ __forceinline__ void cross_put(const CrossArgs& a, const CrossPlace& 
   else *reinterpret_cast<u32x2*>(reinterpret_cast<uint16_t*>(a.o) + at) = u32x2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
 }
 
-// ONE: sequences of one tile of keys, as the host says.  Half the LDS and registers for no second tile leave room for six workgroups a CU instead of three, whose loads and stores overlap:
+// ONE: sequences of one tile of keys, as the host says.  Half the LDS and registers for no second tile leave room for more workgroups a CU (heads of 80: five of bf16, four of fp32; two to three of the other form), whose loads and stores overlap:
 // 160 windows of 64, 16 heads of 80, 23.8 -> 20.8 us, 300 of 49 and 72 33.6 -> 25.6, 100 fp32 ones of 80 30.2 -> 22.9.  More rows than 64 as well, which the other form has by 128: 4000 tokens over 64 keys, heads of 128,
 // 14.6 -> 13.5, 20 x 300 19.1 -> 17.4 (4 x 400 over 40 8.3 both).
 template <int DP, int DT, int WR, bool F32, bool ONE>
@@ -436,7 +436,7 @@ __global__ __launch_bounds__(256, DK <= 6 && NR == 1 ? 3 : 2) void cross_wide_ke
   typedef Wide<DK, DT> P;
   constexpr int KT = P::KT, C = P::C, DP = P::DP, CHUNKS = P::CHUNKS;
   __shared__ __align__(16) uint16_t s_all[4 * KT * DP];
-  // in LDS: two tiles of values, two of keys (a tile of 32 elements of the last value may end behind it, where keys are)
+  // in LDS: two tiles of values, two of keys
   constexpr int TILE = KT * DP;
   // Of three or four waves of a SIMD the ones that multiply go first, and the others' exponents fill what they leave: heads of 64, 3000 tokens 65.6 -> 59.2 us, 200 over 2000 keys 36.6 -> 34.1, heads of
   // 80 76.8 -> 72.5.  (Of two waves, heads of 128, 3 x 700 tokens over up to 6404 keys 179 -> 190: the compiler moves nothing over the switches.)

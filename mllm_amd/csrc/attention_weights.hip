@@ -14,9 +14,9 @@
 //   Up to 16 rows whose scores fit into 64 KB, of few keys or many sequences: the two in one launch, a workgroup a key head, scores in LDS.
 // No atomics: what a key gets is summed by one wave in one order.
 //
-// What bounds it.  Tokens: memory (a token of 16 sequences over up to 8000 keys, 32 query and 8 key heads of 128, 57 us: scores 47, of which keys arrive at 3.7 TB/s, sums 9.5; neither more ranges, nor ranges of equal
-// length over all sequences, nor heads of a range on one XCD changed that; 64 sequences over up to 3800 keys 88, 3.7 TB/s too, whether 64 or 128 KB a CU are on their way).  More rows: matrix instructions, three parts of fp32 queries in both passes (32 tokens of six sequences over up to 7000 keys 77 us:
-// parts 5.6, maxima 35, join 4.7, weights 40; the bytes alone would take 12, the products at a library's rate 25).  Storing the scores of many rows instead of forming them twice would write and read more bytes than that.
+// What bounds it.  Tokens: memory (a token of 16 sequences over up to 8000 keys, 32 query and 8 key heads of 128, 57 us: scores 47, of which keys arrive at 3.7 TB/s (a load of a wave is 64 bytes of each of 16 keys; attention over an encoder's states, whose loads are whole rows, has 4.1 to 4.4), sums 9.5; neither more ranges, nor ranges of equal
+// length over all sequences, nor heads of a range on one XCD changed that; 64 sequences over up to 3800 keys 88, 3.7 TB/s too, whether 64 or 128 KB a CU are on their way).  More rows: matrix instructions, three parts of fp32 queries in both passes (32 tokens of six sequences over up to 7000 keys 76 to 81 us:
+// parts 5.6, maxima 35, join 4.7, weights 40; the bytes alone would take 12, the products at a library's rate 25; bf16 queries 54 where the products take 11, 500 of them over 4000 keys 68 to 70 where they take 27).  Storing the scores of many rows instead of forming them twice would write and read more bytes than that.
 #include <type_traits>
 
 #include "attention_common.h"

@@ -8,7 +8,7 @@
 // in 32) by counting in LDS, and the positions are written in order by a count in front of each wave's share.  The second copies the rows.
 //
 // What bounds it: 2048 of 24 x 6000 positions, 8 heads of 128, 99 us: the copy 88 (403 MB: 4.6 TB/s), the first launch 12.  4096 of 16 384 positions of one sequence 22.5: the first launch 14.2, eight workgroups in a chain of
-// three counts with four barriers each (16 masses a lane in registers: the call takes 33 with masses read again for every digit), the copy 8.4.
+// three counts with three barriers each (16 masses a lane in registers: the call takes 33 with masses read again for every digit, as behind 16 384 positions), the copy 8.4.  16 384 of 65 536 104 us, 8192 of 32 768 55.
 #include "item8.h"
 
 namespace mllmhip {

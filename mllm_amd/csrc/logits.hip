@@ -9,7 +9,7 @@
 // integers and of several biases for a token the last one counts (the largest index, by a maximum), so nothing depends on the order of the atomics.
 //
 // What bounds it: one row, a launch (kernel 4.4 us) and the call.  96 bf16 rows of 151 936 with histories of up to 6000 tokens 23.6 us (61 MB: 2.6 TB/s; a copy of 2 GB has 5.18): the
-// histories, which each of the 38 slices of a row goes through; without them 62 rows of 233 096 14.0 us (4.1 TB/s).
+// histories, which each of the 38 slices of a row goes through, on all eight XCDs; without them 62 rows of 233 096 14.0 us (4.1 TB/s).
 #include "item8.h"
 
 namespace mllmhip {

@@ -11,7 +11,8 @@
 // with many tokens, by the launch and two dependent loads with few.  32 query and 8 key heads of 128, norm and halves turned:
 // 8191 bf16 tokens 43 us (168 MB: 3.9 TB/s, a copy of 2 GB has 4.96), one fp32 token 3.2 in the kernel; 6007 bf16 tokens of 16 query and 4 key heads,
 // pairs turned, keys and values into the cache, 16.6 us (74 MB: 4.5 TB/s).  Several axes cost a lookup of the pair's axis and up to four positions per workgroup, loaded together: 5185 bf16 tokens of
-// 32 query and 8 key heads of 128 on three axes 29.3 us (106 MB: 3.6 TB/s), four fp32 tokens into the cache 3.9 in the kernel.
+// 32 query and 8 key heads of 128 on three axes 29.6 us (106 MB: 3.6 TB/s), four fp32 tokens into the cache 3.9 in the kernel.  Vector instructions are not hidden behind memory there: eight choices more an item
+// take 10 %.
 #include "item8.h"
 
 namespace mllmhip {
